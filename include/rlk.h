@@ -478,6 +478,45 @@ int rlk_logits_logp_backward(const void* logits, int dtype, int64_t row_stride, 
                              int64_t vocab_start, int64_t real_vocab, void* stream);
 
 /*
+ * Scores of given tokens from materialised logits [T, V] (rlk_dtype, rows row_stride elements apart, any alignment):
+ *   y = z / temperature over the columns [0, real_vocab); lse = log sum exp(y); logp = y_target - lse;
+ *   entropy = -sum p log p with p = exp(y - lse); top_ids / top_logp [T, top_k]: the columns with the largest logits, equal
+ *   ones from the lowest column on (a NaN ranks with -inf), and their log-probabilities.
+ * temperature [T] may be NULL. A target outside [0, real_vocab) gives logp = NaN; a temperature that is not positive, a NaN or
+ * +inf logit and a row without a logit above -inf give NaN throughout (lse is -inf for the latter). The bits of logp and lse are
+ * those of rlk_logp_from_logits with 64 tiles where 64 divides V. row_lse: log-sum-exps of the rows that exist already (those of
+ * rlk_linear_logp_fwd_logits); target, logp and lse may then be NULL, and top_logp is taken against it, at most 0.
+ * top_k: 0 (top_logp and top_ids may be NULL) to RLK_SCORES_MAX_TOP_K. A row's results never depend on the other rows.
+ */
+#define RLK_SCORES_MAX_TOP_K 64
+#define RLK_SCORES_MAX_VOCAB (1 << 28)
+size_t rlk_logits_scores_workspace_bytes(int T, int top_k);
+int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
+                      const float* row_lse, int T, int64_t V, int64_t real_vocab, int top_k, float* logp, float* lse,
+                      float* entropy, float* top_logp, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * d(logits) of sum(g_logp logp + g_lse lse + g_entropy entropy) + sum(g_top top_logp), each gradient [T] (g_top [T, top_k]) or
+ * NULL; lse, entropy and top_ids are the forward's. Written once in grad_dtype: that of the logits, or bf16 for fp32 logits; zero on
+ * the columns [real_vocab, grad_cols), grad_cols >= V. p is taken as 0 on a row whose lse is not finite.
+ */
+int rlk_logits_scores_backward(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
+                               const float* lse, const float* entropy, const float* g_logp, const float* g_lse,
+                               const float* g_entropy, const int64_t* top_ids, const float* g_top, int top_k, void* grad,
+                               int grad_dtype, int64_t grad_row_stride, int64_t grad_cols, int T, int64_t V, int64_t real_vocab,
+                               void* stream);
+
+/*
+ * The products at the end of a linear layer's backward over the vocabulary: grad_hidden[T, D] = dlogits weight and
+ * grad_weight[V, D] = dlogits^T hidden, bf16, either NULL. dlogits: bf16 [T, rlk_linear_dlogits_row_stride(V)], 256-byte aligned,
+ * zero behind column V. The same products as rlk_linear_logp_bwd; grad_hidden serves as scratch before it is written.
+ */
+int64_t rlk_linear_dlogits_row_stride(int V);
+int rlk_linear_dlogits_bwd(const void* dlogits, const void* hidden, int64_t h_row_stride, const void* weight, int64_t w_row_stride,
+                           void* grad_hidden, int64_t gh_row_stride, void* grad_weight, int64_t gw_row_stride, int T, int D, int V,
+                           void* stream);
+
+/*
  * Value checks without a copy back: flags[0] is set to 1 when one of the n ids lies outside [lo, hi), flags[1] when a
  * temperature (may be NULL) is <= 0. `flags` points to two words the device can write, normally pinned host memory that
  * the caller has zeroed and reads after an event behind this call.

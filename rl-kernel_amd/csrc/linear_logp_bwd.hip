@@ -403,6 +403,58 @@ LinearBackwardPlan linear_logp_bwd_plan(int T, int D, int V) {
                               BackwardOf::kLogp);
 }
 
+bool logp_operands_vectorise(const MatView& H, const MatView& W, int D) {
+  return W.k_stride == 1 && H.k_stride == 1 && (W.row_stride % kChunkElems) == 0 && (H.row_stride % kChunkElems) == 0 &&
+         (reinterpret_cast<uintptr_t>(W.ptr) & 15) == 0 && (reinterpret_cast<uintptr_t>(H.ptr) & 15) == 0 &&
+         (D % kChunkElems) == 0 && pitch_fits_lane_offsets(W.row_stride) && pitch_fits_lane_offsets(H.row_stride);
+}
+
+// grad_hidden = dz W and grad_weight = dz^T H (either may be null) from a d(logits) of row stride linear_logp_dz_row_stride(V)
+// whose rows are zero behind V.
+hipError_t linear_logp_gradients_launch(const MatView& H, const MatView& W, const bf16_bits* dz, void* grad_hidden, int64_t gh_row_stride,
+                                        void* grad_weight, int64_t gw_row_stride, int T, int D, int V, bool force_staged,
+                                        hipStream_t stream) {
+  const bool vec = logp_operands_vectorise(H, W, D);
+  hipError_t err = hipSuccess;
+  const int gemm_config = force_staged ? (RLK_GEMM_CFG_AUTO | RLK_GEMM_CFG_FORCE_STAGED) : RLK_GEMM_CFG_AUTO;
+  const GemmProblem to_hidden = hidden_gradient(W, dz, grad_hidden, gh_row_stride, T, D, V);
+  const GemmProblem to_weight = weight_gradient(H, dz, grad_weight, gw_row_stride, T, D, V);
+  const LinearBackwardPlan plan = grad_hidden && grad_weight && !force_staged
+                                      ? linear_backward_plan(to_hidden, to_weight, BackwardOf::kLogp)
+                                      : LinearBackwardPlan{RLK_LINEAR_BWD_CFG_SEPARATE, 0};
+  if (plan.config != RLK_LINEAR_BWD_CFG_SEPARATE || plan.solo_tokens != 0) {
+    err = linear_backward_launch(to_hidden, to_weight, plan, stream);
+    if (err != hipSuccess) return err;
+    grad_hidden = grad_weight = nullptr;  // done
+  }
+  if (grad_weight) {
+    // Both operands are K-major as they lie. From 512 tokens on the hidden states are transposed first (into the
+    // grad_hidden buffer, which has exactly their size and is written only afterwards), so that the feature operand
+    // runs the plain ping-pong loads: lm_head at 8192 tokens 8.32 -> 7.79 ms plus 0.04 ms for the transposition.
+    // Up to 256 tokens the streaming kernel takes the K-major operand as it is.
+    const bool via_transposed_hidden =
+        grad_hidden != nullptr && gh_row_stride == D && !force_staged && T >= 512 && T % kChunkElems == 0 && vec &&
+        (reinterpret_cast<uintptr_t>(grad_hidden) & 15) == 0;
+    if (via_transposed_hidden) {
+      bf16_bits* hidden_t = reinterpret_cast<bf16_bits*>(grad_hidden);
+      hipLaunchKernelGGL(transpose_bf16_kernel, dim3((D + kTransposeTile - 1) / kTransposeTile, (T + kTransposeTile - 1) / kTransposeTile),
+                         dim3(256), 0, stream, H.ptr, H.row_stride, hidden_t, T, D);
+      err = hipGetLastError();
+      if (err != hipSuccess) return err;
+      const MatView h_rows{hidden_t, T, 1, D};  // rows = d, reduction index = t contiguous
+      err = det_gemm_launch(h_rows, to_weight.X, grad_weight, gw_row_stride, V, D, T, false, gemm_config, stream);
+    } else {
+      err = det_gemm_launch(to_weight.W, to_weight.X, grad_weight, gw_row_stride, V, D, T, false, gemm_config, stream);
+    }
+    if (err != hipSuccess) return err;
+  }
+  if (grad_hidden) {
+    err = det_gemm_launch(to_hidden.W, to_hidden.X, grad_hidden, gh_row_stride, T, D, V, false, gemm_config, stream);
+    if (err != hipSuccess) return err;
+  }
+  return err;
+}
+
 hipError_t linear_logp_bwd_launch(const MatView& H, const MatView& W, const int64_t* target, const float* bias,
                                   const float* temperature, const float* lse, const float* logits,
                                   int64_t logits_ld, const float* grad_logp, const float* grad_lse, void* grad_hidden, int64_t gh_row_stride, void* grad_weight,
@@ -428,10 +480,7 @@ hipError_t linear_logp_bwd_launch(const MatView& H, const MatView& W, const int6
   a.group_m = 1;
   a.bias_part = grad_bias ? reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + dz_bytes(T, V)) : nullptr;
 
-  const bool vec = W.k_stride == 1 && H.k_stride == 1 && (W.row_stride % kChunkElems) == 0 &&
-                   (H.row_stride % kChunkElems) == 0 && (reinterpret_cast<uintptr_t>(W.ptr) & 15) == 0 &&
-                   (reinterpret_cast<uintptr_t>(H.ptr) & 15) == 0 && (D % kChunkElems) == 0 &&
-                   pitch_fits_lane_offsets(W.row_stride) && pitch_fits_lane_offsets(H.row_stride);
+  const bool vec = logp_operands_vectorise(H, W, D);
   const bool force_staged = (config & RLK_LOGP_CFG_FORCE_STAGED) != 0;
   config &= ~RLK_LOGP_CFG_FORCE_STAGED;
   // 257 ... 384 tokens are three 128-token tiles or two 256-token ones, a third of them padding
@@ -477,42 +526,8 @@ hipError_t linear_logp_bwd_launch(const MatView& H, const MatView& W, const int6
   }
   if (err != hipSuccess) return err;
 
-  const int gemm_config = force_staged ? (RLK_GEMM_CFG_AUTO | RLK_GEMM_CFG_FORCE_STAGED) : RLK_GEMM_CFG_AUTO;
-  const GemmProblem to_hidden = hidden_gradient(W, a.dz, grad_hidden, gh_row_stride, T, D, V);
-  const GemmProblem to_weight = weight_gradient(H, a.dz, grad_weight, gw_row_stride, T, D, V);
-  const LinearBackwardPlan plan = grad_hidden && grad_weight && !force_staged
-                                      ? linear_backward_plan(to_hidden, to_weight, BackwardOf::kLogp)
-                                      : LinearBackwardPlan{RLK_LINEAR_BWD_CFG_SEPARATE, 0};
-  if (plan.config != RLK_LINEAR_BWD_CFG_SEPARATE || plan.solo_tokens != 0) {
-    err = linear_backward_launch(to_hidden, to_weight, plan, stream);
-    if (err != hipSuccess) return err;
-    grad_hidden = grad_weight = nullptr;  // done
-  }
-  if (grad_weight) {
-    // Both operands are K-major as they lie. From 512 tokens on the hidden states are transposed first (into the
-    // grad_hidden buffer, which has exactly their size and is written only afterwards), so that the feature operand
-    // runs the plain ping-pong loads: lm_head at 8192 tokens 8.32 -> 7.79 ms plus 0.04 ms for the transposition.
-    // Up to 256 tokens the streaming kernel takes the K-major operand as it is.
-    const bool via_transposed_hidden =
-        grad_hidden != nullptr && gh_row_stride == D && !force_staged && T >= 512 && T % kChunkElems == 0 && vec &&
-        (reinterpret_cast<uintptr_t>(grad_hidden) & 15) == 0;
-    if (via_transposed_hidden) {
-      bf16_bits* hidden_t = reinterpret_cast<bf16_bits*>(grad_hidden);
-      hipLaunchKernelGGL(transpose_bf16_kernel, dim3((D + kTransposeTile - 1) / kTransposeTile, (T + kTransposeTile - 1) / kTransposeTile),
-                         dim3(256), 0, stream, H.ptr, H.row_stride, hidden_t, T, D);
-      err = hipGetLastError();
-      if (err != hipSuccess) return err;
-      const MatView h_rows{hidden_t, T, 1, D};  // rows = d, reduction index = t contiguous
-      err = det_gemm_launch(h_rows, to_weight.X, grad_weight, gw_row_stride, V, D, T, false, gemm_config, stream);
-    } else {
-      err = det_gemm_launch(to_weight.W, to_weight.X, grad_weight, gw_row_stride, V, D, T, false, gemm_config, stream);
-    }
-    if (err != hipSuccess) return err;
-  }
-  if (grad_hidden) {
-    err = det_gemm_launch(to_hidden.W, to_hidden.X, grad_hidden, gh_row_stride, T, D, V, false, gemm_config, stream);
-    if (err != hipSuccess) return err;
-  }
+  err = linear_logp_gradients_launch(H, W, a.dz, grad_hidden, gh_row_stride, grad_weight, gw_row_stride, T, D, V, force_staged, stream);
+  if (err != hipSuccess) return err;
   if (grad_bias) {
     const int tiles = (T + tile_tokens - 1) / tile_tokens;
     hipLaunchKernelGGL(logp_bias_merge_kernel, dim3((V + 255) / 256), dim3(256), 0, stream, a.bias_part, grad_bias,

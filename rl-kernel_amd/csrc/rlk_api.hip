@@ -598,6 +598,89 @@ int rlk_check_rows(const int64_t* ids, const float* temperature, int n, int64_t 
   return err == hipSuccess ? RLK_OK : device_error("rlk_check_rows", err);
 }
 
+static int check_score_args(const char* what, const void* logits, int dtype, int64_t row_stride, int T, int64_t V, int64_t real_vocab,
+                            int top_k) {
+  int rc = check_logits_args(what, logits, dtype, row_stride, T, V, 0, real_vocab);
+  if (rc != RLK_OK) return rc;
+  if (V > RLK_SCORES_MAX_VOCAB || real_vocab > V) {
+    set_last_error("%s: real_vocab %lld must be in [1, V = %lld], V at most %d", what, (long long)real_vocab, (long long)V,
+                   RLK_SCORES_MAX_VOCAB);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (top_k < 0 || top_k > RLK_SCORES_MAX_TOP_K || top_k > real_vocab) {
+    set_last_error("%s: top_k %d must be in [0, min(%d, real_vocab)]", what, top_k, RLK_SCORES_MAX_TOP_K);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  return RLK_OK;
+}
+
+size_t rlk_logits_scores_workspace_bytes(int T, int top_k) { return T > 0 ? token_scores_workspace_bytes(T, top_k) : 0; }
+
+int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
+                      const float* row_lse, int T, int64_t V, int64_t real_vocab, int top_k, float* logp, float* lse,
+                      float* entropy, float* top_logp, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_score_args("rlk_logits_scores", logits, dtype, row_stride, T, V, real_vocab, top_k);
+  if (rc != RLK_OK) return rc;
+  if (T == 0) return RLK_OK;
+  if (entropy == nullptr || (row_lse == nullptr && (target == nullptr || logp == nullptr || lse == nullptr)) ||
+      (top_k > 0 && (top_logp == nullptr || top_ids == nullptr))) {
+    set_last_error("rlk_logits_scores: null target or output");
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  const size_t need = token_scores_workspace_bytes(T, top_k);
+  if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
+    set_last_error("rlk_logits_scores: 16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  hipError_t err = token_scores_launch(logits, dtype, row_stride, target, temperature, row_lse, T, (int)V, (int)real_vocab, top_k,
+                                       logp, lse, entropy, top_logp, top_ids, workspace, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error("rlk_logits_scores", err);
+}
+
+int rlk_logits_scores_backward(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
+                               const float* lse, const float* entropy, const float* g_logp, const float* g_lse,
+                               const float* g_entropy, const int64_t* top_ids, const float* g_top, int top_k, void* grad,
+                               int grad_dtype, int64_t grad_row_stride, int64_t grad_cols, int T, int64_t V, int64_t real_vocab,
+                               void* stream) {
+  int rc = check_score_args("rlk_logits_scores_backward", logits, dtype, row_stride, T, V, real_vocab, g_top ? top_k : 0);
+  if (rc != RLK_OK) return rc;
+  if (grad_dtype != dtype && !(dtype == RLK_DTYPE_FP32 && grad_dtype == RLK_DTYPE_BF16)) {
+    set_last_error("rlk_logits_scores_backward: the gradient has the type of the logits, or bf16 for fp32 logits");
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (T == 0) return RLK_OK;
+  if (lse == nullptr || grad == nullptr || (g_logp && !target) || (g_entropy && !entropy) || (g_top && !top_ids) || grad_cols < V ||
+      grad_cols > RLK_SCORES_MAX_VOCAB + 64 || grad_row_stride < grad_cols) {
+    set_last_error("rlk_logits_scores_backward: null argument, or V <= grad_cols <= grad_row_stride does not hold");
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  hipError_t err = token_scores_backward_launch(logits, dtype, row_stride, target, temperature, lse, entropy, g_logp, g_lse, g_entropy,
+                                                top_ids, g_top, top_k, grad, grad_dtype, grad_row_stride, (int)grad_cols, T, (int)V,
+                                                (int)real_vocab, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error("rlk_logits_scores_backward", err);
+}
+
+int64_t rlk_linear_dlogits_row_stride(int V) { return V > 0 ? linear_logp_dz_row_stride(V) : 0; }
+
+int rlk_linear_dlogits_bwd(const void* dlogits, const void* hidden, int64_t h_row_stride, const void* weight, int64_t w_row_stride,
+                           void* grad_hidden, int64_t gh_row_stride, void* grad_weight, int64_t gw_row_stride, int T, int D, int V,
+                           void* stream) {
+  if (T <= 0 || D <= 0 || V <= 0) {
+    set_last_error("rlk_linear_dlogits_bwd: T=%d D=%d V=%d must be positive", T, D, V);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (dlogits == nullptr || (reinterpret_cast<uintptr_t>(dlogits) & 255) != 0 || hidden == nullptr || weight == nullptr ||
+      h_row_stride < D || w_row_stride < D || (grad_hidden && gh_row_stride < D) || (grad_weight && gw_row_stride < D)) {
+    set_last_error("rlk_linear_dlogits_bwd: null or unaligned operand, or a row stride below D");
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  const MatView H{reinterpret_cast<const bf16_bits*>(hidden), h_row_stride, 1, T};
+  const MatView W{reinterpret_cast<const bf16_bits*>(weight), w_row_stride, 1, V};
+  hipError_t err = linear_logp_gradients_launch(H, W, reinterpret_cast<const bf16_bits*>(dlogits), grad_hidden, gh_row_stride, grad_weight,
+                                                gw_row_stride, T, D, V, false, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error("rlk_linear_dlogits_bwd", err);
+}
+
 static bool activation_dtype_ok(int dtype) {
   return dtype == RLK_DTYPE_BF16 || dtype == RLK_DTYPE_FP16 || dtype == RLK_DTYPE_FP32;
 }

@@ -206,6 +206,23 @@ hipError_t linear_logp_bwd_launch(const MatView& H, const MatView& W, const int6
                                   float* grad_bias, void* workspace, int T, int D, int V, int64_t vocab_start,
                                   int vocab_limit, int config, hipStream_t stream);
 
+// The two products at its end: dz W and dz^T H of a d(logits) with row stride linear_logp_dz_row_stride(V), zero behind V.
+hipError_t linear_logp_gradients_launch(const MatView& H, const MatView& W, const bf16_bits* dz, void* grad_hidden, int64_t gh_row_stride,
+                                        void* grad_weight, int64_t gw_row_stride, int T, int D, int V, bool force_staged,
+                                        hipStream_t stream);
+
+// Scores of given tokens from materialised logits (token_scores.hip); row_lse: log-sum-exps that exist, or null.
+size_t token_scores_workspace_bytes(int T, int top_k);
+hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
+                               const float* row_lse, int T, int V, int real, int top_k, float* logp, float* lse, float* entropy,
+                               float* top_logp, int64_t* top_ids, void* workspace, hipStream_t stream);
+// Their gradient, in the type of the logits or (fp32 logits) in bf16; columns [V, grad_cols) are written as zeros.
+hipError_t token_scores_backward_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target,
+                                        const float* temperature, const float* lse, const float* entropy, const float* g_logp,
+                                        const float* g_lse, const float* g_entropy, const int64_t* top_ids, const float* g_top,
+                                        int top_k, void* grad, int grad_dtype, int64_t grad_row_stride, int grad_cols, int T, int V,
+                                        int real, hipStream_t stream);
+
 // SwiGLU on rows of `dtype` (rlk_dtype; strides in elements): forward writes y = out; backward
 // writes d_gate = out, d_up = out2.
 hipError_t swiglu_launch(const void* gate, int64_t ld_g, const void* up, int64_t ld_u, const void* dy, int64_t ld_dy,

@@ -871,6 +871,115 @@ def hip_deterministic_logp_backward(
     return grad
 
 
+def logits_scores(
+    logits: torch.Tensor,
+    target: Optional[torch.Tensor],
+    real_vocab: int,
+    top_k: int = 0,
+    *,
+    temperature: Optional[torch.Tensor] = None,
+    row_lse: Optional[torch.Tensor] = None,
+) -> List[Optional[torch.Tensor]]:
+    """``[logp, lse, entropy, top_logp, top_ids]`` of materialised logits ``[rows, V]`` (bf16 / fp16 / fp32, any row stride).
+
+    fp32 ``[rows]``, ``[rows, top_k]`` for the alternatives (``None`` without them), int64 ids. ``row_lse``: log-sum-exps that
+    exist already; ``logp`` and ``lse`` are then ``None`` and ``target`` is not looked at. ``temperature``: fp32, one per row."""
+    code = _logits_dtype_code(logits)
+    src = _row_contiguous(logits)
+    rows, vocab = src.shape
+    device = src.device
+    for name, t, dtype in (("target", target, torch.int64), ("temperature", temperature, torch.float32), ("row_lse", row_lse, torch.float32)):
+        if t is not None and (t.device != device or t.dtype != dtype or t.numel() != rows or not t.is_contiguous()):
+            raise RuntimeError(f"logits_scores: {name} must be a contiguous {dtype} tensor beside the logits, one value per row")
+    if target is None and row_lse is None:
+        raise RuntimeError("logits_scores: target is required without row_lse")
+    logp = lse = top_logp = top_ids = None
+    if row_lse is None:
+        logp = torch.empty((rows,), dtype=torch.float32, device=device)
+        lse = torch.empty((rows,), dtype=torch.float32, device=device)
+    entropy = torch.empty((rows,), dtype=torch.float32, device=device)
+    if top_k:
+        top_logp = torch.empty((rows, top_k), dtype=torch.float32, device=device)
+        top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=device)
+    lib = _lib.load()
+    ws_bytes = int(lib.rlk_logits_scores_workspace_bytes(rows, top_k))
+    workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=device)
+    with _on(device):
+        status = lib.rlk_logits_scores(
+            src.data_ptr(), code, src.stride(0), _ptr(target), _ptr(temperature), _ptr(row_lse), rows, vocab, real_vocab, top_k,
+            _ptr(logp), _ptr(lse), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids), workspace.data_ptr(), ws_bytes,
+            _stream_handle(device),
+        )  # fmt: skip
+    _lib.check(status, "rlk_logits_scores failed")
+    return [logp, lse, entropy, top_logp, top_ids]
+
+
+def logits_scores_backward(
+    logits: torch.Tensor,
+    target: torch.Tensor,
+    real_vocab: int,
+    lse: torch.Tensor,
+    entropy: torch.Tensor,
+    top_ids: Optional[torch.Tensor],
+    grads: tuple,
+    *,
+    temperature: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """d(logits) for ``grads = (g_logp, g_lse, g_entropy, g_top)`` (fp32 like the outputs of :func:`logits_scores`, or ``None``),
+    in the dtype of ``logits``; ``out``: a ``[rows, >= V]`` buffer in its place (bf16 for fp32 logits), zeros behind column V."""
+    code = _logits_dtype_code(logits)
+    src = _row_contiguous(logits)
+    rows, vocab = src.shape
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=src.dtype, device=src.device)
+    elif out.dim() != 2 or out.size(0) != rows or out.size(1) < vocab or out.stride(1) != 1 or out.device != src.device:
+        raise RuntimeError("logits_scores_backward: out must have a contiguous row of at least V columns for every row of logits")
+    if rows == 0:
+        return out
+    top_k = top_ids.size(-1) if top_ids is not None else 0
+    grads = tuple(g if g is None else g.reshape(rows, -1).to(dtype=torch.float32).contiguous() for g in grads)
+    for g, width in zip(grads, (1, 1, 1, top_k)):
+        if g is not None and (g.size(1) != width or g.device != src.device):
+            raise RuntimeError("logits_scores_backward: a gradient must have the shape of its output, beside the logits")
+    with _on(src.device):
+        status = _lib.load().rlk_logits_scores_backward(
+            src.data_ptr(), code, src.stride(0), target.data_ptr(), _ptr(temperature), lse.data_ptr(), entropy.data_ptr(),
+            _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), _ptr(top_ids), _ptr(grads[3]), top_k, out.data_ptr(),
+            _act_dtype_code(out), out.stride(0), out.size(1), rows, vocab, real_vocab, _stream_handle(src.device),
+        )  # fmt: skip
+    _lib.check(status, "rlk_logits_scores_backward failed")
+    return out
+
+
+def linear_dlogits_row_stride(vocab: int) -> int:
+    """Columns of the bf16 d(logits) that :func:`linear_dlogits_bwd` takes: the vocabulary and zeros behind it."""
+    return int(_lib.load().rlk_linear_dlogits_row_stride(int(vocab)))
+
+
+def linear_dlogits_bwd(
+    dlogits: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor, need_grad_hidden: bool = True, need_grad_weight: bool = True,
+) -> List[Optional[torch.Tensor]]:  # fmt: skip
+    """``[dlogits @ weight, dlogits.T @ hidden]`` in bf16 for contiguous bf16 ``hidden [T, D]``, ``weight [V, D]`` and
+    ``dlogits [T, linear_dlogits_row_stride(V)]``; ``None`` for the one that is not wanted."""
+    n, d = hidden.shape
+    v = weight.size(0)
+    for name, t, shape in (("dlogits", dlogits, (n, linear_dlogits_row_stride(v))), ("hidden", hidden, (n, d)), ("weight", weight, (v, d))):
+        if t.dtype != _BF16 or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda or t.device != hidden.device:
+            raise RuntimeError(f"linear_dlogits_bwd: {name} must be a contiguous bf16 {list(shape)} CUDA tensor beside hidden")
+    grad_hidden = torch.empty((n, d), dtype=_BF16, device=hidden.device) if need_grad_hidden else None
+    grad_weight = torch.empty((v, d), dtype=_BF16, device=hidden.device) if need_grad_weight else None
+    if n == 0:
+        return [grad_hidden, grad_weight.zero_() if grad_weight is not None else None]
+    with _on(hidden.device):
+        status = _lib.load().rlk_linear_dlogits_bwd(
+            dlogits.data_ptr(), hidden.data_ptr(), d, weight.data_ptr(), d, _ptr(grad_hidden), d, _ptr(grad_weight), d, n, d, v,
+            _stream_handle(hidden.device),
+        )  # fmt: skip
+    _lib.check(status, "rlk_linear_dlogits_bwd failed")
+    return [grad_hidden, grad_weight]
+
+
 class RowChecks:
     """Value checks of ids and temperatures that run on the device in front of the work that uses them.
 

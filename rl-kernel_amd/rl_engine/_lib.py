@@ -62,6 +62,8 @@ TREE_LEAF_SPACE = 0x100  # RLK_TREE_CFG_LEAF_SPACE: OR-ed into rlk_tree_config 0
 NOALLOC_SCRATCH_BYTES = 32 << 20  # RLK_NOALLOC_SCRATCH_BYTES
 # rlk_dtype (element types of materialised logits)
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
+SCORES_MAX_TOP_K = 64  # RLK_SCORES_MAX_TOP_K
+SCORES_MAX_VOCAB = 1 << 28  # RLK_SCORES_MAX_VOCAB
 # rlk_logp_config
 LOGP_CONFIGS = {
     "auto": 0, "256": 1, "128": 2, "64": 3, "16": 4, "64_streams": 5, "128_streams": 6, "256_streams": 7, "192_streams": 8,
@@ -97,6 +99,11 @@ EXPORTED_SYMBOLS = (
     "rlk_logp_from_logits_workspace_bytes",
     "rlk_logp_from_logits",
     "rlk_logits_logp_backward",
+    "rlk_logits_scores_workspace_bytes",
+    "rlk_logits_scores",
+    "rlk_logits_scores_backward",
+    "rlk_linear_dlogits_row_stride",
+    "rlk_linear_dlogits_bwd",
     "rlk_check_rows",
     "rlk_swiglu_fwd",
     "rlk_swiglu_bwd",
@@ -204,6 +211,19 @@ def load() -> ctypes.CDLL:
     lib.rlk_logp_from_logits.argtypes = [vp, i32, i64, vp, vp, i32, i64, i64, i64, i32, vp, vp, vp, sz, vp]
     lib.rlk_logits_logp_backward.restype = i32
     lib.rlk_logits_logp_backward.argtypes = [vp, i32, i64, vp, vp, vp, vp, vp, vp, i64, i32, i64, i64, i64, vp]
+
+    lib.rlk_logits_scores_workspace_bytes.restype = sz
+    lib.rlk_logits_scores_workspace_bytes.argtypes = [i32, i32]
+    lib.rlk_logits_scores.restype = i32
+    lib.rlk_logits_scores.argtypes = [vp, i32, i64, vp, vp, vp, i32, i64, i64, i32, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.rlk_logits_scores_backward.restype = i32
+    lib.rlk_logits_scores_backward.argtypes = [
+        vp, i32, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, i32, i64, i64, i32, i64, i64, vp,
+    ]  # fmt: skip
+    lib.rlk_linear_dlogits_row_stride.restype = i64
+    lib.rlk_linear_dlogits_row_stride.argtypes = [i32]
+    lib.rlk_linear_dlogits_bwd.restype = i32
+    lib.rlk_linear_dlogits_bwd.argtypes = [vp, vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, vp]
 
     lib.rlk_check_rows.restype = i32
     lib.rlk_check_rows.argtypes = [vp, vp, i32, i64, i64, vp, vp]

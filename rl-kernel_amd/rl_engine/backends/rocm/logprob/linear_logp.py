@@ -110,8 +110,9 @@ def recompute_logits() -> Iterator[None]:
         _recompute.reset(token)
 
 
-def _logits_to_save(hidden_2d: torch.Tensor, vocab: int) -> Optional[torch.Tensor]:
+def _logits_to_save(hidden_2d: torch.Tensor, vocab: int, written_anyway: bool = False) -> Optional[torch.Tensor]:
     """A buffer for the forward's logits, or None where the backward computes them again (the same bits).
+    ``written_anyway``: the forward writes them whether they are kept or not, so only memory counts.
 
     Only memory that the device can spare is taken: at most 8 GiB for all graphs alive together, and for each buffer, with
     the bf16 d(logits) that its backward needs beside it, at most a quarter of what the driver has free (what the
@@ -121,11 +122,11 @@ def _logits_to_save(hidden_2d: torch.Tensor, vocab: int) -> Optional[torch.Tenso
     n, d = hidden_2d.shape
     shape = (n, _C.linear_logp_logits_row_stride(vocab))
     size = 4 * shape[0] * shape[1]
-    if n == 0 or d < _SAVED_LOGITS_MIN_HIDDEN or size > _SAVED_LOGITS_MAX_BYTES or _recompute.get():
+    if n == 0 or size > _SAVED_LOGITS_MAX_BYTES or _recompute.get() or (d < _SAVED_LOGITS_MIN_HIDDEN and not written_anyway):
         return None
     if torch._C._autograd._top_saved_tensors_default_hooks(True) is not None or torch.cuda.is_current_stream_capturing():
         return None
-    if n < _SAVED_LOGITS_MIN_TOKENS and d < _SAVED_LOGITS_ANY_TOKENS_HIDDEN and 2 * vocab * d <= _MEMORY_SIDE_CACHE_BYTES:
+    if not written_anyway and n < _SAVED_LOGITS_MIN_TOKENS and d < _SAVED_LOGITS_ANY_TOKENS_HIDDEN and 2 * vocab * d <= _MEMORY_SIDE_CACHE_BYTES:
         return None
     device = hidden_2d.device
     with _saved_logits_lock:
