@@ -517,6 +517,57 @@ int rlk_linear_dlogits_bwd(const void* dlogits, const void* hidden, int64_t h_ro
                            void* stream);
 
 /*
+ * What lies between two blocks of a transformer, for rows of `width` elements:
+ *   u = block * r1 * post_weight, r1 = 1 / sqrt(mean(block^2) + eps)          (u = block where post_weight is NULL)
+ *   total = residual + residual_scale * gate * u                              (total = residual where block is NULL)
+ *   normed = total * r2 * pre_weight, r2 = 1 / sqrt(mean(total^2) + eps)      (none where pre_weight is NULL; of the unrounded total)
+ * block and normed have `dtype`, residual and total residual_dtype (dtype or fp32), gate and the weights theirs (dtype or fp32).
+ * gate: RLK_GATE_CHANNEL [width], RLK_GATE_TOKEN [tokens] (gate_row_stride apart), RLK_GATE_FULL [tokens, width], or none. Outputs
+ * and gradients are contiguous. Arithmetic and sums in fp32, each result rounded once.
+ */
+typedef enum rlk_gate { RLK_GATE_NONE = 0, RLK_GATE_CHANNEL = 1, RLK_GATE_TOKEN = 2, RLK_GATE_FULL = 3 } rlk_gate;
+#define RLK_NORM_MAX_WIDTH 16384
+typedef struct rlk_block_norm {
+  const void* block;       /* [tokens, width], row stride block_row_stride, or NULL */
+  const void* residual;    /* [tokens, width], row stride residual_row_stride */
+  const void* gate;
+  const void* post_weight; /* [width] or NULL */
+  const void* pre_weight;  /* [width] or NULL */
+  float* rstd;             /* [2][tokens]: r1 and r2, written by the forward (or NULL) and read by the backward */
+  int64_t block_row_stride, residual_row_stride, gate_row_stride;
+  int64_t tokens;
+  int width, dtype, residual_dtype, gate_kind, gate_dtype, post_dtype, pre_dtype;
+  float eps, residual_scale;
+} rlk_block_norm;
+
+/* total or normed may be NULL where it is not wanted; normed is required with pre_weight. */
+int rlk_block_norm_forward(const rlk_block_norm* host_norm, void* total, void* normed, void* stream);
+
+/* Gradients in the types of their tensors, each output NULL where it is not wanted: g_total and g_normed (NULL: zero) are those of
+ * the outputs; d_gate has the gate's shape. The workspace holds the parts of the weights' and a channel gate's sums over tokens. */
+size_t rlk_block_norm_workspace_bytes(int64_t tokens, int width);
+int rlk_block_norm_backward(const rlk_block_norm* host_norm, const void* g_total, const void* g_normed, void* d_block, void* d_residual,
+                            void* d_gate, void* d_post_weight, void* d_pre_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Eight-bit copies of activations that wait for their backward: int8 codes [rows, cols] and one scale byte for each run of 32
+ * columns of a row ([rows, ceil(cols / 32)], the last run may be shorter), both contiguous. A run's scale is the power of two, at
+ * least 2^-126, that takes its largest magnitude into [64, 128), stored as its exponent + 127; a code is the nearest whole number of
+ * scales (halves to even), at most 127 of them. A run with a value that is not finite has the scale byte 255 and is NaN throughout.
+ * x = code * scale is exact in fp32 and bf16.
+ */
+int rlk_mx8_encode(const void* x, int64_t row_stride, int dtype, int8_t* codes, uint8_t* scales, int64_t rows, int cols, void* stream);
+int rlk_mx8_decode(const int8_t* codes, const uint8_t* scales, void* x, int64_t row_stride, int dtype, int64_t rows, int cols, void* stream);
+
+/* rlk_swiglu_fwd that also writes the eight-bit copies of gate and up, and rlk_swiglu_bwd on such copies; y (or NULL): the
+ * activation of the copies, for a product behind it. y, d_gate and d_up are contiguous. */
+int rlk_mx8_swiglu_forward(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype, void* y, int8_t* gate_codes,
+                           uint8_t* gate_scales, int8_t* up_codes, uint8_t* up_scales, int64_t rows, int cols, void* stream);
+int rlk_mx8_swiglu_backward(const void* dy, int64_t ld_dy, int dtype, const int8_t* gate_codes, const uint8_t* gate_scales,
+                            const int8_t* up_codes, const uint8_t* up_scales, void* d_gate, void* d_up, void* y, int64_t rows, int cols,
+                            void* stream);
+
+/*
  * Value checks without a copy back: flags[0] is set to 1 when one of the n ids lies outside [lo, hi), flags[1] when a
  * temperature (may be NULL) is <= 0. `flags` points to two words the device can write, normally pinned host memory that
  * the caller has zeroed and reads after an event behind this call.

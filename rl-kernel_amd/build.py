@@ -19,7 +19,7 @@ HOST_SOURCE = CSRC / "torch_host.cpp"
 HOST_MODULE = PKG_DIR / "rl_engine" / "_torch_host.so"
 OBJ_DIR = PKG_DIR / "build"  # object files (git-ignored)
 SOURCES = ["det_gemm.hip", "det_gemm_pair.hip", "det_gemm_stream.hip", "det_gemm_shortk.hip", "det_gemm_tree.hip", "det_gemm_seq.hip", "linear_logp.hip",
-    "linear_logp_bwd.hip", "logits_logp.hip", "token_scores.hip", "swiglu.hip", "grpo.hip", "rlk_api.hip"]
+    "linear_logp_bwd.hip", "logits_logp.hip", "token_scores.hip", "block_norm.hip", "mx8.hip", "swiglu.hip", "grpo.hip", "rlk_api.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -151,6 +151,93 @@ struct RawVector<RLK_DTYPE_FP32, ALIGNED> {
   }
 };
 
+typedef u32x4_t u32x4_at2_t __attribute__((aligned(2)));
+typedef u32x4_t u32x4_at4_t __attribute__((aligned(4)));
+template <int BYTES>
+struct UnalignedPart {
+  using type = u32x4_at2_t;
+};
+template <>
+struct UnalignedPart<4> {
+  using type = u32x4_at4_t;
+};
+
+// Eight logits of a row. Rows may start at any element: the loads ask for the element's alignment only.
+template <int ELEM>
+struct RowVector {
+  using E = typename LogitElem<ELEM>::type;
+  static constexpr int kParts = (int)sizeof(E) / 2;
+  using Part = typename UnalignedPart<(int)sizeof(E)>::type;
+  u32x4_t w[kParts];
+
+  template <bool NT>
+  __device__ __forceinline__ void load(const E* p) {
+    const Part* src = reinterpret_cast<const Part*>(p);
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      if constexpr (NT) {
+        w[i] = __builtin_nontemporal_load(src + i);
+      } else {
+        w[i] = src[i];
+      }
+    }
+  }
+  // vector g of a row of `cols` columns, those behind it 0
+  template <bool NT>
+  __device__ __forceinline__ void load_edge(const E* row, int g, int cols) {
+    if ((int64_t)g * 8 + 8 <= cols) {
+      load<NT>(row + (int64_t)g * 8);
+    } else {
+      E vals[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vals[i] = (int64_t)g * 8 + i < cols ? row[(int64_t)g * 8 + i] : E(0);
+      __builtin_memcpy(w, vals, sizeof(w));
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&y)[8]) const {
+    E vals[8];
+    __builtin_memcpy(vals, w, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = LogitElem<ELEM>::to_float(vals[i]);
+  }
+  // (fp16: the fp32 value is fixed first. Left alone the compiler rounds some last products straight to fp16, some not.)
+  __device__ __forceinline__ void pack(const float (&y)[8]) {
+    E vals[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = y[i];
+      if constexpr (ELEM == RLK_DTYPE_FP16) asm volatile("" : "+v"(v));
+      vals[i] = LogitElem<ELEM>::from_float(v);
+    }
+    __builtin_memcpy(w, vals, sizeof(w));
+  }
+  template <bool NT>
+  __device__ __forceinline__ void store(E* p) const {
+    Part* dst = reinterpret_cast<Part*>(p);
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      if constexpr (NT) {
+        __builtin_nontemporal_store(w[i], dst + i);
+      } else {
+        dst[i] = w[i];
+      }
+    }
+  }
+  // to columns [col, col + 8) of a row, those from `cols` on left as they are
+  template <bool NT>
+  __device__ __forceinline__ void store_edge(E* row, int64_t col, int64_t cols) const {
+    if (col + 8 <= cols) {
+      store<NT>(row + col);
+    } else {
+      E vals[8];
+      __builtin_memcpy(vals, w, sizeof(w));
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < cols) row[col + i] = vals[i];
+    }
+  }
+};
+
 // max(a, b, c) in one instruction. (fmaxf on values that come out of integer shifts costs an extra
 // canonicalising instruction per operand; v_max3_f32 needs none. For the non-NaN values of this contract it
 // returns what nested fmaxf returns.)

@@ -785,6 +785,128 @@ int rlk_det_gemm_swiglu_training_bf16(const void* a, int64_t a_row_stride, const
   return err == hipSuccess ? RLK_OK : device_error("rlk_det_gemm_swiglu_training_bf16", err);
 }
 
+static int check_block_norm(const char* who, const rlk_block_norm* n) {
+  if (n == nullptr || n->tokens < 0 || n->tokens > 0x7fffffff || n->width < 1 || n->width > RLK_NORM_MAX_WIDTH) {
+    set_last_error("%s: null description, or tokens / width outside [0, 2^31) / [1, %d]", who, RLK_NORM_MAX_WIDTH);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  const bool types = activation_dtype_ok(n->dtype) && (n->residual_dtype == n->dtype || n->residual_dtype == RLK_DTYPE_FP32) &&
+                     (n->gate_dtype == n->dtype || n->gate_dtype == RLK_DTYPE_FP32 || n->gate_kind == RLK_GATE_NONE) &&
+                     (n->post_weight == nullptr || n->post_dtype == n->dtype || n->post_dtype == RLK_DTYPE_FP32) &&
+                     (n->pre_weight == nullptr || n->pre_dtype == n->dtype || n->pre_dtype == RLK_DTYPE_FP32);
+  if (!types) {
+    set_last_error("%s: residual, gate and weights have the type of the block or fp32", who);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (n->gate_kind < RLK_GATE_NONE || n->gate_kind > RLK_GATE_FULL) {
+    set_last_error("%s: unknown gate kind %d", who, n->gate_kind);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (n->tokens == 0) return RLK_OK;  // (the addresses of empty tensors say nothing)
+  if (n->block == nullptr && (n->gate_kind != RLK_GATE_NONE || n->post_weight)) {
+    set_last_error("%s: a gate or a post norm without a block", who);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (n->residual == nullptr || n->residual_row_stride < n->width || (n->block && n->block_row_stride < n->width) ||
+      (n->gate_kind != RLK_GATE_NONE && n->gate == nullptr) || (n->gate_kind == RLK_GATE_FULL && n->gate_row_stride < n->width) ||
+      (n->gate_kind == RLK_GATE_TOKEN && n->gate_row_stride < 0)) {
+    set_last_error("%s: null residual or gate, or a row stride below the width", who);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  return RLK_OK;
+}
+
+int rlk_block_norm_forward(const rlk_block_norm* n, void* total, void* normed, void* stream) {
+  int rc = check_block_norm("rlk_block_norm_forward", n);
+  if (rc != RLK_OK || n->tokens == 0) return rc;
+  if ((n->pre_weight != nullptr) != (normed != nullptr)) {
+    set_last_error("rlk_block_norm_forward: normed goes with pre_weight");
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  hipError_t err = block_norm_forward_launch(n, total, normed, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error("rlk_block_norm_forward", err);
+}
+
+size_t rlk_block_norm_workspace_bytes(int64_t tokens, int width) { return width > 0 ? block_norm_workspace_bytes(tokens, width) : 0; }
+
+int rlk_block_norm_backward(const rlk_block_norm* n, const void* g_total, const void* g_normed, void* d_block, void* d_residual,
+                            void* d_gate, void* d_post_weight, void* d_pre_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_block_norm("rlk_block_norm_backward", n);
+  if (rc != RLK_OK) return rc;
+  if ((d_pre_weight && !n->pre_weight) || (d_post_weight && !n->post_weight) || (d_gate && n->gate_kind == RLK_GATE_NONE) ||
+      (d_block && !n->block)) {
+    set_last_error("rlk_block_norm_backward: a gradient of something that is not there");
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (n->tokens == 0) {  // sums over no tokens
+    auto bytes = [](int dtype) { return dtype == RLK_DTYPE_FP32 ? 4 : 2; };
+    hipError_t err = hipSuccess;
+    if (d_pre_weight) err = fill_zero_launch(d_pre_weight, 1, n->width, n->width, bytes(n->pre_dtype), s);
+    if (err == hipSuccess && d_post_weight) err = fill_zero_launch(d_post_weight, 1, n->width, n->width, bytes(n->post_dtype), s);
+    if (err == hipSuccess && d_gate && n->gate_kind == RLK_GATE_CHANNEL) err = fill_zero_launch(d_gate, 1, n->width, n->width, bytes(n->gate_dtype), s);
+    return err == hipSuccess ? RLK_OK : device_error("rlk_block_norm_backward", err);
+  }
+  const size_t need = block_norm_workspace_bytes(n->tokens, n->width);
+  if (n->rstd == nullptr || workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3) != 0) {
+    set_last_error("rlk_block_norm_backward: the forward's rstd and a workspace of %zu bytes are needed, %zu given", need, workspace_bytes);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  hipError_t err = block_norm_backward_launch(n, g_total, g_normed, d_block, d_residual, d_gate, d_post_weight, d_pre_weight, workspace, s);
+  return err == hipSuccess ? RLK_OK : device_error("rlk_block_norm_backward", err);
+}
+
+static int check_mx8(const char* who, int64_t rows, int cols, int dtype, bool complete, bool strides) {
+  if (rows < 0 || cols < 0 || cols > (1 << 28)) {
+    set_last_error("%s: bad sizes rows=%lld cols=%d", who, (long long)rows, cols);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (!activation_dtype_ok(dtype)) {
+    set_last_error("%s: unknown dtype %d", who, dtype);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (rows > 0 && cols > 0 && !(complete && strides)) {
+    set_last_error("%s: null operand or row stride < cols", who);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  return RLK_OK;
+}
+
+int rlk_mx8_encode(const void* x, int64_t row_stride, int dtype, int8_t* codes, uint8_t* scales, int64_t rows, int cols, void* stream) {
+  int rc = check_mx8("rlk_mx8_encode", rows, cols, dtype, x && codes && scales, row_stride >= cols);
+  if (rc != RLK_OK || rows == 0 || cols == 0) return rc;
+  hipError_t err = mx8_encode_launch(x, row_stride, dtype, codes, scales, rows, cols, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error("rlk_mx8_encode", err);
+}
+
+int rlk_mx8_decode(const int8_t* codes, const uint8_t* scales, void* x, int64_t row_stride, int dtype, int64_t rows, int cols, void* stream) {
+  int rc = check_mx8("rlk_mx8_decode", rows, cols, dtype, x && codes && scales, row_stride >= cols);
+  if (rc != RLK_OK || rows == 0 || cols == 0) return rc;
+  hipError_t err = mx8_decode_launch(codes, scales, x, row_stride, dtype, rows, cols, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error("rlk_mx8_decode", err);
+}
+
+int rlk_mx8_swiglu_forward(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype, void* y, int8_t* gate_codes,
+                           uint8_t* gate_scales, int8_t* up_codes, uint8_t* up_scales, int64_t rows, int cols, void* stream) {
+  int rc = check_mx8("rlk_mx8_swiglu_forward", rows, cols, dtype, gate && up && y && gate_codes && gate_scales && up_codes && up_scales,
+                     ld_gate >= cols && ld_up >= cols);
+  if (rc != RLK_OK || rows == 0 || cols == 0) return rc;
+  hipError_t err = mx8_swiglu_forward_launch(gate, ld_gate, up, ld_up, dtype, y, gate_codes, gate_scales, up_codes, up_scales, rows, cols,
+                                             reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error("rlk_mx8_swiglu_forward", err);
+}
+
+int rlk_mx8_swiglu_backward(const void* dy, int64_t ld_dy, int dtype, const int8_t* gate_codes, const uint8_t* gate_scales,
+                            const int8_t* up_codes, const uint8_t* up_scales, void* d_gate, void* d_up, void* y, int64_t rows, int cols,
+                            void* stream) {
+  int rc = check_mx8("rlk_mx8_swiglu_backward", rows, cols, dtype, dy && gate_codes && gate_scales && up_codes && up_scales && d_gate && d_up,
+                     ld_dy >= cols);
+  if (rc != RLK_OK || rows == 0 || cols == 0) return rc;
+  hipError_t err = mx8_swiglu_backward_launch(dy, ld_dy, dtype, gate_codes, gate_scales, up_codes, up_scales, d_gate, d_up, y, rows, cols,
+                                              reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error("rlk_mx8_swiglu_backward", err);
+}
+
 size_t rlk_grpo_workspace_bytes(int rollouts) { return rollouts > 0 ? (size_t)3 * rollouts * sizeof(float) : 0; }
 
 int rlk_grpo_ratio_kl_loss(const float* logp, const float* old_logp, const float* ref_logp,

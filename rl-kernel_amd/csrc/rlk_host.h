@@ -223,6 +223,22 @@ hipError_t token_scores_backward_launch(const void* logits, int dtype, int64_t r
                                         int top_k, void* grad, int grad_dtype, int64_t grad_row_stride, int grad_cols, int T, int V,
                                         int real, hipStream_t stream);
 
+// What lies between two blocks (block_norm.hip).
+size_t block_norm_workspace_bytes(int64_t T, int H);
+hipError_t block_norm_forward_launch(const rlk_block_norm* n, void* total, void* normed, hipStream_t stream);
+hipError_t block_norm_backward_launch(const rlk_block_norm* n, const void* g_total, const void* g_normed, void* d_block, void* d_residual,
+                                      void* d_gate, void* d_post_weight, void* d_pre_weight, void* workspace, hipStream_t stream);
+
+// Eight-bit copies (mx8.hip): codes[rows, cols] and a scale byte per run of 32 columns, both contiguous.
+hipError_t mx8_encode_launch(const void* x, int64_t ld, int dtype, int8_t* codes, uint8_t* scales, int64_t rows, int cols, hipStream_t stream);
+hipError_t mx8_decode_launch(const int8_t* codes, const uint8_t* scales, void* x, int64_t ld, int dtype, int64_t rows, int cols,
+                             hipStream_t stream);
+hipError_t mx8_swiglu_forward_launch(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype, void* y, int8_t* gate_codes,
+                                     uint8_t* gate_scales, int8_t* up_codes, uint8_t* up_scales, int64_t rows, int cols, hipStream_t stream);
+hipError_t mx8_swiglu_backward_launch(const void* dy, int64_t ld_dy, int dtype, const int8_t* gate_codes, const uint8_t* gate_scales,
+                                      const int8_t* up_codes, const uint8_t* up_scales, void* d_gate, void* d_up, void* y, int64_t rows,
+                                      int cols, hipStream_t stream);
+
 // SwiGLU on rows of `dtype` (rlk_dtype; strides in elements): forward writes y = out; backward
 // writes d_gate = out, d_up = out2.
 hipError_t swiglu_launch(const void* gate, int64_t ld_g, const void* up, int64_t ld_u, const void* dy, int64_t ld_dy,

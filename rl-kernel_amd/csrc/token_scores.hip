@@ -26,57 +26,6 @@ constexpr int kScoreSlices = kScoreTiles * kTileLanes;
 constexpr int kScorePlanes = 4;  // max, sum, target, weighted sum: stats[row][plane][tile]
 constexpr float kFarBelow = -256.f;  // e(x) is zero from here down
 
-typedef u32x4_t u32x4_at2_t __attribute__((aligned(2)));
-typedef u32x4_t u32x4_at4_t __attribute__((aligned(4)));
-template <int BYTES>
-struct UnalignedPart {
-  using type = u32x4_at2_t;
-};
-template <>
-struct UnalignedPart<4> {
-  using type = u32x4_at4_t;
-};
-
-// Eight logits of a row. Rows may start at any element: the loads ask for the element's alignment only.
-template <int ELEM>
-struct ScoreVector {
-  using E = typename LogitElem<ELEM>::type;
-  static constexpr int kParts = (int)sizeof(E) / 2;
-  using Part = typename UnalignedPart<(int)sizeof(E)>::type;
-  u32x4_t w[kParts];
-
-  template <bool NT>
-  __device__ __forceinline__ void load(const E* p) {
-    const Part* src = reinterpret_cast<const Part*>(p);
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      if constexpr (NT) {
-        w[i] = __builtin_nontemporal_load(src + i);
-      } else {
-        w[i] = src[i];
-      }
-    }
-  }
-  // vector g of a row of `cols` columns, those behind it 0
-  template <bool NT>
-  __device__ __forceinline__ void load_edge(const E* row, int g, int cols) {
-    if ((int64_t)g * 8 + 8 <= cols) {
-      load<NT>(row + (int64_t)g * 8);
-    } else {
-      E vals[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vals[i] = (int64_t)g * 8 + i < cols ? row[(int64_t)g * 8 + i] : E(0);
-      __builtin_memcpy(w, vals, sizeof(w));
-    }
-  }
-  __device__ __forceinline__ void unpack(float (&y)[8]) const {
-    E vals[8];
-    __builtin_memcpy(vals, w, sizeof(w));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = LogitElem<ELEM>::to_float(vals[i]);
-  }
-};
-
 struct ScoreArgs {
   const void* logits;
   int64_t row_stride;  // elements
@@ -196,7 +145,7 @@ __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
     int g = g0 + l16;  // this lane's next vector
     // The loads rotate through four raw vectors: a vector's registers are free once it is unpacked, and the same vector
     // of the next batch is fetched into them before the fold, so a lane always has three or four loads in flight.
-    ScoreVector<ELEM> raw[kBatch];
+    RowVector<ELEM> raw[kBatch];
     if (clean > 0) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) raw[u].template load<NT>(row_ptr + (int64_t)(g + u * kTileLanes) * 8);
@@ -431,7 +380,7 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   const E* row_ptr = reinterpret_cast<const E*>(a.logits) + (int64_t)row * a.row_stride;
   const int rounds = ((a.tile_size + 14) / 8 + kTileLanes - 1) / kTileLanes;  // vectors of a slice, at most
   const uint32_t jobs = (uint32_t)(slices * rounds);  // (rounds <= 2^28 / 64 / 128 + 1)
-  ScoreVector<ELEM> next;
+  RowVector<ELEM> next;
   int next_lo = 0, next_hi = 0, next_g = 0;  // columns [lo, hi) of vector g
   auto fetch = [&](uint32_t job) __attribute__((always_inline)) {
     next_lo = next_hi = next_g = 0;
@@ -572,7 +521,7 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
   const E* row_in = reinterpret_cast<const E*>(a.logits) + (int64_t)row * a.row_stride;
   O* row_out = reinterpret_cast<O*>(a.grad) + (int64_t)row * a.grad_row_stride;
 
-  ScoreVector<ELEM> raw[kScoreBackVectors];
+  RowVector<ELEM> raw[kScoreBackVectors];
 #pragma unroll
   for (int u = 0; u < kScoreBackVectors; ++u) {
     const int64_t col = first + (int64_t)(u * kScoreBackThreads + threadIdx.x) * 8;
@@ -636,26 +585,11 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = at == i ? out[i] + hit_grad[h] : out[i];
     }
-    O vals[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) vals[i] = LogitElem<OUT>::from_float(out[i] * inv_t);
-    if (col + 8 <= a.grad_cols) {
-      typename ScoreVector<OUT>::Part* dst = reinterpret_cast<typename ScoreVector<OUT>::Part*>(row_out + col);
-      u32x4_t w[ScoreVector<OUT>::kParts];
-      __builtin_memcpy(w, vals, sizeof(w));
-#pragma unroll
-      for (int i = 0; i < ScoreVector<OUT>::kParts; ++i) {
-        if constexpr (STREAM) {
-          __builtin_nontemporal_store(w[i], dst + i);
-        } else {
-          dst[i] = w[i];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < a.grad_cols) row_out[col + i] = vals[i];
-    }
+    for (int i = 0; i < 8; ++i) out[i] = out[i] * inv_t;
+    RowVector<OUT> packed;
+    packed.pack(out);
+    packed.template store_edge<STREAM>(row_out, col, a.grad_cols);
   }
 }
 

@@ -726,6 +726,11 @@ def _logits_dtype_code(logits: torch.Tensor) -> int:
     return codes[logits.dtype]
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between the rows of a 2-D tensor; of a single row, whose stride may be anything, its length."""
+    return t.stride(0) if t.size(0) > 1 else t.size(1)
+
+
 def _row_contiguous(logits: torch.Tensor) -> torch.Tensor:
     return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.size(1) else logits.contiguous()
 
@@ -906,7 +911,7 @@ def logits_scores(
     workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=device)
     with _on(device):
         status = lib.rlk_logits_scores(
-            src.data_ptr(), code, src.stride(0), _ptr(target), _ptr(temperature), _ptr(row_lse), rows, vocab, real_vocab, top_k,
+            src.data_ptr(), code, _row_stride(src), _ptr(target), _ptr(temperature), _ptr(row_lse), rows, vocab, real_vocab, top_k,
             _ptr(logp), _ptr(lse), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids), workspace.data_ptr(), ws_bytes,
             _stream_handle(device),
         )  # fmt: skip
@@ -944,9 +949,9 @@ def logits_scores_backward(
             raise RuntimeError("logits_scores_backward: a gradient must have the shape of its output, beside the logits")
     with _on(src.device):
         status = _lib.load().rlk_logits_scores_backward(
-            src.data_ptr(), code, src.stride(0), target.data_ptr(), _ptr(temperature), lse.data_ptr(), entropy.data_ptr(),
+            src.data_ptr(), code, _row_stride(src), target.data_ptr(), _ptr(temperature), lse.data_ptr(), entropy.data_ptr(),
             _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), _ptr(top_ids), _ptr(grads[3]), top_k, out.data_ptr(),
-            _act_dtype_code(out), out.stride(0), out.size(1), rows, vocab, real_vocab, _stream_handle(src.device),
+            _act_dtype_code(out), _row_stride(out), out.size(1), rows, vocab, real_vocab, _stream_handle(src.device),
         )  # fmt: skip
     _lib.check(status, "rlk_logits_scores_backward failed")
     return out
@@ -1121,6 +1126,105 @@ def swiglu_packed_backward(dy: torch.Tensor, gate_up: torch.Tensor) -> List[torc
             )  # fmt: skip
         _lib.check(status, "rlk_swiglu_bwd failed")
     return [d_gate, d_up]
+
+
+def _mx8_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise RuntimeError(f"{name} must be fp16, bf16, or fp32, got {t.dtype}")
+    if t.dim() != 2:
+        raise RuntimeError(f"{name} must be [rows, columns]")
+    return t if t.stride(1) == 1 and t.stride(0) >= t.size(1) else t.contiguous()
+
+
+def _mx8_buffers(rows: int, cols: int, device: torch.device) -> tuple:
+    return (
+        torch.empty((rows, cols), dtype=torch.int8, device=device),
+        torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=device),
+    )
+
+
+def _check_mx8(codes: torch.Tensor, scales: torch.Tensor, name: str) -> None:
+    if not codes.is_cuda or scales.device != codes.device:
+        raise RuntimeError(f"{name}: codes and scales must be CUDA tensors on one device")
+    if codes.dtype != torch.int8 or scales.dtype != torch.uint8 or not codes.is_contiguous() or not scales.is_contiguous():
+        raise RuntimeError(f"{name}: codes must be contiguous int8, scales contiguous uint8")
+    if codes.dim() != 2 or tuple(scales.shape) != (codes.size(0), (codes.size(1) + 31) // 32):
+        raise RuntimeError(f"{name}: expect codes [rows, columns] and scales [rows, ceil(columns / 32)]")
+
+
+def mx8_encode(x: torch.Tensor) -> tuple:
+    """``(codes, scales)`` of ``x [rows, columns]``: int8 and one exponent byte per run of 32 columns (rlk_mx8_encode)."""
+    src = _mx8_rows(x, "x")
+    rows, cols = src.shape
+    codes, scales = _mx8_buffers(rows, cols, src.device)
+    with _on(src.device):
+        status = _lib.load().rlk_mx8_encode(
+            src.data_ptr(), _row_stride(src), _act_dtype_code(src), codes.data_ptr(), scales.data_ptr(), rows, cols, _stream_handle(src.device)
+        )
+    _lib.check(status, "rlk_mx8_encode failed")
+    return codes, scales
+
+
+def mx8_decode(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """What :func:`mx8_encode` kept, in ``dtype`` (exact in bf16 and fp32)."""
+    _check_mx8(codes, scales, "mx8_decode")
+    if dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise RuntimeError(f"mx8_decode: dtype must be fp16, bf16, or fp32, got {dtype}")
+    rows, cols = codes.shape
+    x = torch.empty((rows, cols), dtype=dtype, device=codes.device)
+    with _on(codes.device):
+        status = _lib.load().rlk_mx8_decode(
+            codes.data_ptr(), scales.data_ptr(), x.data_ptr(), cols, _act_dtype_code(x), rows, cols, _stream_handle(codes.device)
+        )
+    _lib.check(status, "rlk_mx8_decode failed")
+    return x
+
+
+def swiglu_mx8_forward(gate: torch.Tensor, up: torch.Tensor) -> tuple:
+    """``(swiglu_forward(gate, up), gate codes, gate scales, up codes, up scales)`` of ``[rows, columns]`` tensors."""
+    gate, up = _mx8_rows(gate, "gate"), _mx8_rows(up, "up")
+    if gate.device != up.device:
+        raise RuntimeError(f"gate and up must be on the same CUDA device, got {gate.device} and {up.device}")
+    if gate.shape != up.shape:
+        raise RuntimeError("gate and up must share shape")
+    _same_act_dtype(gate, "gate", up, "up")
+    rows, cols = gate.shape
+    y = torch.empty((rows, cols), dtype=gate.dtype, device=gate.device)
+    kept = (*_mx8_buffers(rows, cols, gate.device), *_mx8_buffers(rows, cols, gate.device))
+    with _on(gate.device):
+        status = _lib.load().rlk_mx8_swiglu_forward(
+            gate.data_ptr(), _row_stride(gate), up.data_ptr(), _row_stride(up), _act_dtype_code(gate), y.data_ptr(),
+            *(t.data_ptr() for t in kept), rows, cols, _stream_handle(gate.device),
+        )  # fmt: skip
+    _lib.check(status, "rlk_mx8_swiglu_forward failed")
+    return (y, *kept)
+
+
+def swiglu_mx8_backward(
+    dy: torch.Tensor, gate_codes: torch.Tensor, gate_scales: torch.Tensor, up_codes: torch.Tensor, up_scales: torch.Tensor,
+    with_activation: bool = False,
+) -> List[Optional[torch.Tensor]]:  # fmt: skip
+    """``[d_gate, d_up, y]``: :func:`swiglu_backward` on the copies, and (on request) their activation."""
+    dy = _mx8_rows(dy, "dy")
+    _check_mx8(gate_codes, gate_scales, "swiglu_mx8_backward")
+    _check_mx8(up_codes, up_scales, "swiglu_mx8_backward")
+    if gate_codes.shape != up_codes.shape or dy.shape != gate_codes.shape:
+        raise RuntimeError("dy and the copies of gate and up must share shape")
+    if dy.device != gate_codes.device or dy.device != up_codes.device:
+        raise RuntimeError("dy and the copies of gate and up must be on the same CUDA device")
+    rows, cols = dy.shape
+    d_gate = torch.empty((rows, cols), dtype=dy.dtype, device=dy.device)
+    d_up = torch.empty((rows, cols), dtype=dy.dtype, device=dy.device)
+    y = torch.empty((rows, cols), dtype=dy.dtype, device=dy.device) if with_activation else None
+    with _on(dy.device):
+        status = _lib.load().rlk_mx8_swiglu_backward(
+            dy.data_ptr(), _row_stride(dy), _act_dtype_code(dy), gate_codes.data_ptr(), gate_scales.data_ptr(), up_codes.data_ptr(),
+            up_scales.data_ptr(), d_gate.data_ptr(), d_up.data_ptr(), _ptr(y), rows, cols, _stream_handle(dy.device),
+        )  # fmt: skip
+    _lib.check(status, "rlk_mx8_swiglu_backward failed")
+    return [d_gate, d_up, y]
 
 
 def det_gemm_swiglu(a: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -64,6 +64,9 @@ NOALLOC_SCRATCH_BYTES = 32 << 20  # RLK_NOALLOC_SCRATCH_BYTES
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 SCORES_MAX_TOP_K = 64  # RLK_SCORES_MAX_TOP_K
 SCORES_MAX_VOCAB = 1 << 28  # RLK_SCORES_MAX_VOCAB
+# rlk_gate
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
+NORM_MAX_WIDTH = 16384  # RLK_NORM_MAX_WIDTH
 # rlk_logp_config
 LOGP_CONFIGS = {
     "auto": 0, "256": 1, "128": 2, "64": 3, "16": 4, "64_streams": 5, "128_streams": 6, "256_streams": 7, "192_streams": 8,
@@ -104,6 +107,13 @@ EXPORTED_SYMBOLS = (
     "rlk_logits_scores_backward",
     "rlk_linear_dlogits_row_stride",
     "rlk_linear_dlogits_bwd",
+    "rlk_block_norm_forward",
+    "rlk_block_norm_workspace_bytes",
+    "rlk_block_norm_backward",
+    "rlk_mx8_encode",
+    "rlk_mx8_decode",
+    "rlk_mx8_swiglu_forward",
+    "rlk_mx8_swiglu_backward",
     "rlk_check_rows",
     "rlk_swiglu_fwd",
     "rlk_swiglu_bwd",
@@ -114,6 +124,18 @@ EXPORTED_SYMBOLS = (
     "rlk_grpo_ratio_kl_loss",
     "rlk_grpo_ratio_kl_loss_bwd",
 )
+
+
+class BlockNorm(ctypes.Structure):
+    """rlk_block_norm."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("block", "residual", "gate", "post_weight", "pre_weight", "rstd")),
+        *((name, ctypes.c_int64) for name in ("block_row_stride", "residual_row_stride", "gate_row_stride", "tokens")),
+        *((name, ctypes.c_int) for name in ("width", "dtype", "residual_dtype", "gate_kind", "gate_dtype", "post_dtype", "pre_dtype")),
+        ("eps", ctypes.c_float),
+        ("residual_scale", ctypes.c_float),
+    ]
 
 
 class RlkLibraryMissing(RuntimeError):
@@ -224,6 +246,22 @@ def load() -> ctypes.CDLL:
     lib.rlk_linear_dlogits_row_stride.argtypes = [i32]
     lib.rlk_linear_dlogits_bwd.restype = i32
     lib.rlk_linear_dlogits_bwd.argtypes = [vp, vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, vp]
+
+    norm = c.POINTER(BlockNorm)
+    lib.rlk_block_norm_forward.restype = i32
+    lib.rlk_block_norm_forward.argtypes = [norm, vp, vp, vp]
+    lib.rlk_block_norm_workspace_bytes.restype = sz
+    lib.rlk_block_norm_workspace_bytes.argtypes = [i64, i32]
+    lib.rlk_block_norm_backward.restype = i32
+    lib.rlk_block_norm_backward.argtypes = [norm, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.rlk_mx8_encode.restype = i32
+    lib.rlk_mx8_encode.argtypes = [vp, i64, i32, vp, vp, i64, i32, vp]
+    lib.rlk_mx8_decode.restype = i32
+    lib.rlk_mx8_decode.argtypes = [vp, vp, vp, i64, i32, i64, i32, vp]
+    lib.rlk_mx8_swiglu_forward.restype = i32
+    lib.rlk_mx8_swiglu_forward.argtypes = [vp, i64, vp, i64, i32, vp, vp, vp, vp, vp, i64, i32, vp]
+    lib.rlk_mx8_swiglu_backward.restype = i32
+    lib.rlk_mx8_swiglu_backward.argtypes = [vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp]
 
     lib.rlk_check_rows.restype = i32
     lib.rlk_check_rows.argtypes = [vp, vp, i32, i64, i64, vp, vp]

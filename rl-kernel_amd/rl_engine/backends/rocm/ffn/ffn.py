@@ -9,7 +9,9 @@ Forward:  gate_up = x @ W_gu^T -> SwiGLU -> @ W_down^T, every GEMM under the det
 contract, so a token's output never depends on the batch it arrives in. Inference fuses the
 activation into the gate/up GEMM; training keeps ``gate_up`` for the backward
 (``swiglu_packed_backward``, two input-gradient and three weight-gradient GEMMs, the gate
-and up input gradients added in bf16 as the reference does, ffn.py:960-975).
+and up input gradients added in bf16 as the reference does, ffn.py:960-975). With ``checkpoint_bits=8``
+it keeps its input, gate and up in eight bits each instead (csrc/mx8.hip), and its activation not at all:
+H + 2 I bytes and a thirty-second of that a token in place of 2 H + 6 I.
 """
 
 from __future__ import annotations
@@ -18,6 +20,7 @@ from typing import Any
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from rl_engine import _C, _host, _lib
 from rl_engine._checks import enforce
@@ -29,6 +32,7 @@ from rl_engine.backends.rocm.gemm.det_gemm import (
     det_gemm_linear_weight_gradient,
     mfma_linear_gradients,
 )
+from rl_engine.backends.rocm.norm.block_norm import gated_residual_norm
 
 QWEN3_8B_HIDDEN_SIZE = 4096
 QWEN3_8B_INTERMEDIATE_SIZE = 12288
@@ -200,17 +204,92 @@ class _DeterministicFFNFunction(torch.autograd.Function):
         return grad_x.reshape(ctx.input_shape) if grad_x is not None else None, *grads, None
 
 
+class _CheckpointedFFNFunction(torch.autograd.Function):
+    """The same forward, to the bit; the backward is that of the eight-bit copies of its input, gate and up."""
+
+    @staticmethod
+    def forward(ctx, rmsnorm_output, gate_weight, up_weight, down_weight, fused_gate_up_weight):
+        shape = rmsnorm_output.shape
+        x = rmsnorm_output.reshape(-1, shape[-1]).contiguous()
+        if fused_gate_up_weight is not None:
+            gate, up = det_gemm_linear(x, fused_gate_up_weight).chunk(2, dim=1)
+        else:
+            gate, up = det_gemm_linear(x, gate_weight), det_gemm_linear(x, up_weight)
+        activated, *kept = _C.swiglu_mx8_forward(gate, up)
+        ctx.save_for_backward(*_C.mx8_encode(x), *kept, gate_weight, up_weight, down_weight)
+        ctx.input_shape = shape
+        output = det_gemm_linear(activated, down_weight)
+        return output.reshape(*shape[:-1], output.size(-1))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        codes, scales, *kept, gate_weight, up_weight, down_weight = ctx.saved_tensors
+        need_x, need_gate, need_up, need_down = ctx.needs_input_grad[:4]
+        grad_output = grad_output.reshape(-1, grad_output.size(-1)).to(torch.bfloat16).contiguous()
+        grad_activated = det_gemm_linear_input_gradient(grad_output, down_weight)
+        grad_gate, grad_up, activated = _C.swiglu_mx8_backward(grad_activated, *kept, with_activation=need_down)
+        del grad_activated
+        grad_down_weight = det_gemm_linear_weight_gradient(activated, grad_output) if need_down else None
+        del activated
+        x = _C.mx8_decode(codes, scales) if need_gate or need_up else None
+        grad_x, grad_gate_weight = _linear_gradients(x, gate_weight, grad_gate, need_x, need_gate)
+        from_up, grad_up_weight = _linear_gradients(x, up_weight, grad_up, need_x, need_up)
+        if need_x:
+            grad_x = grad_x.add_(from_up).reshape(ctx.input_shape)
+        return grad_x, grad_gate_weight, grad_up_weight, grad_down_weight, None
+
+
+class _CheckpointedSwiglu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up):
+        y, *kept = _C.swiglu_mx8_forward(gate, up)
+        ctx.save_for_backward(*kept)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        d_gate, d_up, _ = _C.swiglu_mx8_backward(dy, *ctx.saved_tensors)
+        need_gate, need_up = ctx.needs_input_grad
+        return d_gate if need_gate else None, d_up if need_up else None
+
+
+def checkpointed_swiglu(gate: Tensor, up: Tensor) -> Tensor:
+    """``silu(gate) * up`` (bf16, fp16 or fp32, ``[..., columns]``) that keeps its operands for the backward in eight bits: an int8
+    code each and an exponent per run of 32 columns, so that a value is off by at most 2^-7 of the largest in its run. The
+    result is that of ``_C.swiglu_forward``, the gradients are those of ``_C.swiglu_backward`` on what was kept: to the bit in bf16
+    and fp32, rounded from the fp32 results in fp16. A run with a value that is not finite comes back as NaN."""
+    enforce([
+        (isinstance(gate, Tensor) and isinstance(up, Tensor), TypeError, "gate and up must be torch.Tensors."),
+        (lambda: gate.dim() >= 1 and gate.shape == up.shape, ValueError, lambda: f"gate and up must share shape, got {tuple(gate.shape)} and {tuple(up.shape)}."),
+    ])  # fmt: skip
+    shape = gate.shape
+    if len(shape) != 2:
+        rows = gate.numel() // shape[-1] if shape[-1] else 0
+        gate, up = gate.reshape(rows, shape[-1]), up.reshape(rows, shape[-1])
+    if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
+        y = _CheckpointedSwiglu.apply(gate, up)
+    else:
+        y = _C.swiglu_forward(gate.contiguous(), up.contiguous())
+    return y.reshape(shape)
+
+
 def qwen3_ffn(
     rmsnorm_output: Tensor, gate_weight: Tensor, up_weight: Tensor, down_weight: Tensor, *,
     fused_gate_up_weight: Tensor | None = None, tp_group: Any = None, cp_group: Any = None,
     sequence_parallel: bool = False, deterministic: bool | None = None, disable_split_k: bool | None = None,
+    checkpoint_bits: int | None = None,
 ) -> Tensor:
     """SiLU-gated FFN ``down(swiglu(gate(x), up(x)))`` with deterministic forward and backward.
 
     Signature of ``qwen3_ffn`` (ffn.py:976-1050 of the reference). ``fused_gate_up_weight``
     (``[2 I, H]`` = ``cat(gate_weight, up_weight)``) lets the forward run one GEMM while the
-    gradients are still returned for the separate gate / up weights.
+    gradients are still returned for the separate gate / up weights. ``checkpoint_bits=8``: what waits for the backward waits in
+    eight bits (:func:`checkpointed_swiglu`); the output's bits are the same, the gradients those of the copies.
     """
+    if checkpoint_bits not in (None, 8) or isinstance(checkpoint_bits, bool):
+        raise ValueError(f"checkpoint_bits must be None or 8, got {checkpoint_bits!r}.")
     if not isinstance(sequence_parallel, bool):
         raise TypeError("sequence_parallel must be a bool.")
     for name, value in (("deterministic", deterministic), ("disable_split_k", disable_split_k)):
@@ -222,13 +301,36 @@ def qwen3_ffn(
         raise ValueError("sequence_parallel requires a tensor-parallel group.")
     _single_rank(tp_group, "tensor")
     _single_rank(cp_group, "context")
-    if fused_gate_up_weight is None and not torch.compiler.is_compiling() and det_gemm_backend() == "hip_mfma":
+    checkpointed = checkpoint_bits == 8 and torch.is_grad_enabled() and any(
+        isinstance(t, Tensor) and t.requires_grad for t in (rmsnorm_output, gate_weight, up_weight, down_weight)
+    )
+    if not checkpointed and fused_gate_up_weight is None and not torch.compiler.is_compiling() and det_gemm_backend() == "hip_mfma":
         y = _host.native().ffn(rmsnorm_output, gate_weight, up_weight, down_weight)  # everyday operands, natively
         if y is not None:
             return y
     _validate_ffn_inputs(rmsnorm_output, gate_weight, up_weight, down_weight, fused_gate_up_weight)
     _lib.load()
-    return _DeterministicFFNFunction.apply(rmsnorm_output, gate_weight, up_weight, down_weight, fused_gate_up_weight)
+    function = _CheckpointedFFNFunction if checkpointed else _DeterministicFFNFunction
+    return function.apply(rmsnorm_output, gate_weight, up_weight, down_weight, fused_gate_up_weight)
+
+
+def qwen3_ffn_block(
+    residual: Tensor, normed: Tensor, gate_weight: Tensor, up_weight: Tensor, down_weight: Tensor, next_norm_weight: Tensor | None = None, *,
+    post_norm_weight: Tensor | None = None, gate: Tensor | None = None, residual_scale: float = 1.0, eps: float = 1e-6,
+    fused_gate_up_weight: Tensor | None = None, checkpoint_bits: int | None = None,
+) -> tuple[Tensor, Tensor | None]:
+    """One FFN block of a transformer: ``normed``, the norm of the ``residual`` stream (``ops.norm.rms_norm`` for the first block),
+    through :func:`qwen3_ffn`, and what stands behind it (``ops.norm.gated_residual_norm``). Returns the new residual stream and
+    its norm with ``next_norm_weight``, which the next block takes."""
+    if fused_gate_up_weight is not None and not torch.is_grad_enabled():
+        y = qwen3_ffn_packed_inference(normed, fused_gate_up_weight, down_weight)
+    else:
+        y = qwen3_ffn(
+            normed, gate_weight, up_weight, down_weight, fused_gate_up_weight=fused_gate_up_weight, checkpoint_bits=checkpoint_bits
+        )
+    return gated_residual_norm(
+        y, residual, next_norm_weight, post_weight=post_norm_weight, gate=gate, residual_scale=residual_scale, eps=eps
+    )
 
 
 class Qwen3FFNOp:
@@ -250,4 +352,4 @@ class Qwen3FFNOp:
     __call__ = apply
 
 
-__all__ = ["BACKEND_ID", "Qwen3FFNOp", "qwen3_ffn", "qwen3_ffn_packed_inference"]
+__all__ = ["BACKEND_ID", "Qwen3FFNOp", "checkpointed_swiglu", "qwen3_ffn", "qwen3_ffn_block", "qwen3_ffn_packed_inference"]
