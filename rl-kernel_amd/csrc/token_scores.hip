@@ -328,7 +328,7 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   low = max(__builtin_amdgcn_readfirstlane(low), 1u);  // 0: a slice without columns
 
   // Slices from a limit on that at least k of them reach and not many more (any such limit is as good as the k-th best).
-  const int enough = k + k / 2 + 8;
+  const int enough = k + k / 8 + 2;
   int reach = count_from(low);
   uint32_t beyond = high + 1;  // (high is the key of a number, under 2^32 - 1)
   while (reach > enough && beyond - low > 1) {
@@ -376,14 +376,18 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   }
   wave_lds_sync();
 
-  // The picked slices' vectors, a lane each; the next ones are on their way while these are looked at.
+  // The picked slices' vectors, a lane each, some of a lane's on their way while as many are looked at. An element costs a comparison with
+  // the floor's logit, whose result is a mask over the lanes already; only masks that are not empty go on to the keys.
   const E* row_ptr = reinterpret_cast<const E*>(a.logits) + (int64_t)row * a.row_stride;
   const int rounds = ((a.tile_size + 14) / 8 + kTileLanes - 1) / kTileLanes;  // vectors of a slice, at most
   const uint32_t jobs = (uint32_t)(slices * rounds);  // (rounds <= 2^28 / 64 / 128 + 1)
-  RowVector<ELEM> next;
-  int next_lo = 0, next_hi = 0, next_g = 0;  // columns [lo, hi) of vector g
-  auto fetch = [&](uint32_t job) __attribute__((always_inline)) {
-    next_lo = next_hi = next_g = 0;
+  constexpr int kAhead = ELEM == RLK_DTYPE_FP32 ? 2 : 4;
+  struct Piece {
+    RowVector<ELEM> v;
+    int g, lo, hi;  // columns [lo, hi) of vector g
+  } now[kAhead], next[kAhead];
+  auto fetch = [&](uint32_t job, Piece& p) __attribute__((always_inline)) {
+    p.g = p.lo = p.hi = 0;
     if (job < jobs) {
       const int slice = picked[job / (uint32_t)rounds];
       const int tile = slice / kTileLanes;
@@ -392,31 +396,51 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
       const int hi_col = hi64 < a.real ? (int)hi64 : a.real;
       const int g = lo_col / 8 + slice % kTileLanes + (int)(job % (uint32_t)rounds) * kTileLanes;
       if ((int64_t)g * 8 < hi_col) {
-        next_g = g;
-        next_lo = max(lo_col - g * 8, 0);
-        next_hi = min(hi_col - g * 8, 8);
-        next.template load_edge<false>(row_ptr, g, a.V);
+        p.g = g;
+        p.lo = max(lo_col - g * 8, 0);
+        p.hi = min(hi_col - g * 8, 8);
+        p.v.template load_edge<false>(row_ptr, g, a.V);
       }
     }
   };
   int n = 0;
-  fetch(lane);
-  for (uint32_t first = 0; first < jobs; first += kWave) {
-    float y[8];
-    next.unpack(y);
-    const int lo = next_lo, hi = next_hi, g = next_g;
-    fetch(first + kWave + lane);
-    if (n > kFinishKeys - 8 * kWave) {
-      floor = keep_largest(keys, n, k, lane);
-      n = k;
+  float least = low > ordered_bits(kNegInf) ? from_ordered_bits(low) : kNegInf;  // the floor's logit
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) fetch(u * kWave + lane, next[u]);
+  for (uint32_t first = 0; first < jobs; first += kAhead * kWave) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) now[u] = next[u];
+    if (first + kAhead * kWave < jobs) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) fetch(first + (kAhead + u) * kWave + lane, next[u]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint64_t key = (uint64_t)ordered_bits(y[i]) << 32 | (0xffffffffu - (uint32_t)(g * 8 + i));
-      const bool take = i >= lo && i < hi && key >= floor;
-      const uint64_t mask = __ballot(take);
-      if (take) keys[n + lanes_below(mask)] = key;
-      n += __popcll(mask);
+    for (int u = 0; u < kAhead; ++u) {
+      if (first + u * kWave >= jobs) break;
+      float y[8];
+      uint64_t hit[8], any = 0;
+      now[u].v.unpack(y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = fmaxf(y[i], kNegInf);  // (a NaN counts as -inf)
+        hit[i] = __ballot(i >= now[u].lo && i < now[u].hi && y[i] >= least);
+        any |= hit[i];
+      }
+      if (any == 0) continue;
+      if (n > kFinishKeys - 8 * kWave) {
+        floor = keep_largest(keys, n, k, lane);
+        least = from_ordered_bits((uint32_t)(floor >> 32));
+        n = k;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (hit[i] == 0) continue;
+        const uint64_t key = (uint64_t)ordered_bits(y[i]) << 32 | (0xffffffffu - (uint32_t)(now[u].g * 8 + i));
+        const bool take = ((hit[i] >> lane) & 1) != 0 && key >= floor;
+        const uint64_t mask = __ballot(take);
+        if (take) keys[n + lanes_below(mask)] = key;
+        n += __popcll(mask);
+      }
     }
     wave_lds_sync();
   }
@@ -429,11 +453,16 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   int rank[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < 2; ++i) mine[i] = i * kWave + lane < n ? keys[i * kWave + lane] : 0;
-  for (int j = 0; j < n; ++j) {
-    const uint64_t other = keys[j];
+  auto rank_against = [&](uint64_t of, int count) __attribute__((always_inline)) {
+    for (int j = 0; j < count; ++j) {
+      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(of >> 32), j) << 32 |
+                             (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)of, j);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) rank[i] += other > mine[i] ? 1 : 0;
-  }
+      for (int i = 0; i < 2; ++i) rank[i] += other > mine[i] ? 1 : 0;
+    }
+  };
+  rank_against(mine[0], min(n, kWave));
+  rank_against(mine[1], max(n - kWave, 0));
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     if (i * kWave + lane >= n || rank[i] >= k) continue;
@@ -458,7 +487,7 @@ __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(Scor
   const float big = wave_max_f32(m);
   const float shrink = pinned_exp(m - big);
   const float term = m > kNegInf ? s * shrink : 0.f;
-  float sum = 0.f;
+  float sum = 0.f;  // (ascending)
 #pragma unroll
   for (int t = 0; t < kScoreTiles; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
   const float weighted = wave_sum_f32(m > kNegInf ? shrink * __builtin_fmaf(s, m - big, w) : 0.f);

@@ -48,9 +48,21 @@ decltype(&rlk_swiglu_bwd) swiglu_bwd_entry = nullptr;
 decltype(&rlk_grpo_workspace_bytes) grpo_workspace_entry = nullptr;
 decltype(&rlk_grpo_ratio_kl_loss) grpo_entry = nullptr;
 decltype(&rlk_grpo_ratio_kl_loss_bwd) grpo_bwd_entry = nullptr;
+decltype(&rlk_logits_scores_workspace_bytes) scores_workspace_entry = nullptr;
+decltype(&rlk_logits_scores) scores_entry = nullptr;
+decltype(&rlk_logits_scores_backward) scores_bwd_entry = nullptr;
+decltype(&rlk_block_norm_forward) norm_entry = nullptr;
+decltype(&rlk_block_norm_workspace_bytes) norm_workspace_entry = nullptr;
+decltype(&rlk_block_norm_backward) norm_bwd_entry = nullptr;
+decltype(&rlk_mx8_encode) mx8_encode_entry = nullptr;
+decltype(&rlk_mx8_swiglu_forward) mx8_swiglu_entry = nullptr;
+decltype(&rlk_mx8_swiglu_backward) mx8_swiglu_bwd_entry = nullptr;
 decltype(&rlk_last_error) last_error_entry = nullptr;
 PyObject* general_linear_gradients = nullptr;  // (a, weight, grad, need_a, need_weight) -> (da, dw)
 PyObject* general_ffn_gradients = nullptr;     // (x, gate, up, activated, three weights, grad, need of x and the weights) -> four
+PyObject* general_scores_gradient = nullptr;   // (logits, target, temperature, lse, entropy, top ids, real, four gradients) -> grad
+PyObject* general_norm_gradients = nullptr;    // (block, residual, gate, two weights, rstd, kind, eps, scale, two gradients, five needs) -> five
+PyObject* general_swiglu_gradients = nullptr;  // (dy, codes and scales of gate and up) -> (d_gate, d_up)
 PyObject* general_grpo_gradient = nullptr;     // (cur, old, ref, adv, mask, g_loss, g_policy, g_kl, clip_eps, beta) -> grad
 
 // What _lib.check() raises.
@@ -345,6 +357,308 @@ struct GrpoFn : torch::autograd::Function<GrpoFn> {
 };
 
 // ---------------------------------------------------------------------------
+// Token scores, norms between blocks, eight-bit copies: the everyday calls of backends/rocm/logprob/token_scores.py,
+// backends/rocm/norm/block_norm.py and of checkpointed_swiglu in backends/rocm/ffn/ffn.py
+// ---------------------------------------------------------------------------
+
+// rlk_dtype of an element type, or -1.
+int dtype_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return RLK_DTYPE_BF16;
+    case at::kHalf: return RLK_DTYPE_FP16;
+    case at::kFloat: return RLK_DTYPE_FP32;
+    default: return -1;
+  }
+}
+bool everyday_floats(const Tensor& t) { return t.defined() && dtype_code(t) >= 0 && everyday(t, t.scalar_type()); }
+bool everyday_floats(const Tensor& t, const Tensor& beside) { return everyday_floats(t) && t.get_device() == beside.get_device(); }
+void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+float* writable(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
+PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }  // (None for an undefined tensor)
+
+// Tensors of which some may be missing, saved for a backward, and back at their places.
+void save_some(AutogradContext* ctx, const variable_list& tensors) {
+  variable_list saved;
+  int64_t which = 0;
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    if (!tensors[i].defined()) continue;
+    which |= (int64_t)1 << i;
+    saved.push_back(tensors[i]);
+  }
+  ctx->save_for_backward(std::move(saved));
+  ctx->saved_data["which"] = which;
+}
+variable_list saved_some(AutogradContext* ctx, size_t count) {
+  const variable_list saved = ctx->get_saved_variables();
+  const int64_t which = ctx->saved_data["which"].toInt();
+  variable_list tensors(count);
+  size_t next = 0;
+  for (size_t i = 0; i < count; ++i)
+    if (which >> i & 1) tensors[i] = saved[next++];
+  return tensors;
+}
+// The tensors of a tuple of `count`, None as undefined ones.
+variable_list tensors_of(const PyRef& tuple, int count) {
+  variable_list out;
+  for (int i = 0; i < count; ++i) out.push_back(tensor_or_none(PyTuple_GetItem(tuple.get(), i)));
+  return out;
+}
+
+struct ScoreInputs {
+  Tensor logits, target, temp;
+  int64_t real;
+  int top_k;
+
+  bool usual() const {
+    return everyday_floats(logits) && everyday_matrix(logits) && logits.size(0) <= INT_MAX && logits.size(1) <= RLK_SCORES_MAX_VOCAB &&
+           everyday(target, at::kLong, logits) && target.dim() == 1 && target.size(0) == logits.size(0) && target.is_contiguous() &&
+           (!temp.defined() || (everyday(temp, at::kFloat, logits) && temp.dim() == 1 && temp.size(0) == logits.size(0) && temp.is_contiguous())) &&
+           real > 0 && real <= logits.size(1) && top_k >= 0 && top_k <= RLK_SCORES_MAX_TOP_K && top_k <= real;
+  }
+};
+
+// logp, lse, entropy and, for alternatives, their log-probabilities and ids.
+variable_list scores(const ScoreInputs& in) {
+  const int64_t rows = in.logits.size(0), vocab = in.logits.size(1);
+  variable_list out = {empty({rows}, at::kFloat, in.logits), empty({rows}, at::kFloat, in.logits), empty({rows}, at::kFloat, in.logits)};
+  if (in.top_k > 0) {
+    out.push_back(empty({rows, in.top_k}, at::kFloat, in.logits));
+    out.push_back(empty({rows, in.top_k}, at::kLong, in.logits));
+  }
+  const size_t bytes = scores_workspace_entry((int)rows, in.top_k);
+  const Tensor workspace = empty({(int64_t)bytes}, at::kByte, in.logits);
+  check_status(scores_entry(in.logits.data_ptr(), dtype_code(in.logits), vocab, static_cast<const int64_t*>(in.target.data_ptr()),
+                            floats(in.temp), nullptr, (int)rows, vocab, in.real, in.top_k, writable(out[0]), writable(out[1]),
+                            writable(out[2]), in.top_k > 0 ? writable(out[3]) : nullptr,
+                            in.top_k > 0 ? static_cast<int64_t*>(out[4].data_ptr()) : nullptr, workspace.data_ptr(), bytes,
+                            stream_of(in.logits)),
+               "rlk_logits_scores failed");
+  return out;
+}
+
+struct ScoresFn : torch::autograd::Function<ScoresFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const ScoreInputs* in) {
+    variable_list out = scores(*in);
+    save_some(ctx, {logits, in->target, in->temp, out[1], out[2], out.size() > 4 ? out[4] : Tensor()});
+    ctx->saved_data["real"] = in->real;
+    ctx->set_materialize_grads(false);
+    if (out.size() > 4) ctx->mark_non_differentiable({out[4]});
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    grads.resize(4);  // of logp, lse, entropy and the alternatives' log-probabilities
+    if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined() && !grads[3].defined()) return {Tensor(), Tensor()};
+    const variable_list s = saved_some(ctx, 6);
+    const Tensor &lse = s[3], &entropy = s[4], &ids = s[5];
+    const int64_t real = ctx->saved_data["real"].toInt();
+    const int top_k = ids.defined() ? (int)ids.size(1) : 0;
+    const ScoreInputs in{s[0], s[1], s[2], real, top_k};
+    bool values = !at::GradMode::is_enabled() && everyday_thread() && in.usual() && everyday(lse, at::kFloat, in.logits) &&
+                  everyday(entropy, at::kFloat, in.logits) && (!ids.defined() || everyday(ids, at::kLong, in.logits));
+    const int64_t rows = values ? in.logits.size(0) : 0;
+    for (int i = 0; values && i < 4; ++i)
+      values = !grads[i].defined() || (everyday(grads[i], at::kFloat, in.logits) && grads[i].is_contiguous() &&
+                                       grads[i].numel() == rows * (i == 3 ? top_k : 1));
+    if (values) {
+      const c10::OptionalDeviceGuard guard(in.logits.device());
+      const int64_t vocab = in.logits.size(1);
+      const Tensor grad = empty({rows, vocab}, in.logits.scalar_type(), in.logits);
+      check_status(scores_bwd_entry(in.logits.data_ptr(), dtype_code(in.logits), vocab, static_cast<const int64_t*>(in.target.data_ptr()),
+                                    floats(in.temp), floats(lse), floats(entropy), floats(grads[0]), floats(grads[1]), floats(grads[2]),
+                                    static_cast<const int64_t*>(address(ids)), floats(grads[3]), top_k, grad.data_ptr(),
+                                    dtype_code(in.logits), vocab, vocab, (int)rows, vocab, real, stream_of(in.logits)),
+                   "rlk_logits_scores_backward failed");
+      return {grad, Tensor()};
+    }
+    const pybind11::gil_scoped_acquire gil;
+    const PyRef args(PyTuple_New(11));
+    for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(args.get(), i, wrap(s[i]));
+    PyTuple_SET_ITEM(args.get(), 6, PyLong_FromLongLong(real));
+    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(args.get(), 7 + i, wrap(grads[i]));
+    const PyRef grad(PyObject_CallObject(general_scores_gradient, args.get()));
+    return {tensor_or_none(grad.get()), Tensor()};
+  }
+};
+
+struct NormInputs {
+  Tensor block, residual, gate, post, pre;  // rows [tokens, width]; all but the residual may be missing
+  int kind;                                 // rlk_gate
+  double eps, scale;
+
+  // The type of block and normed: without a block that of the weight (an fp32 weight: of the residual).
+  at::ScalarType type() const { return block.defined() ? block.scalar_type() : residual.scalar_type(); }
+  bool of_type(const Tensor& t) const {
+    return everyday_floats(t, residual) && t.is_contiguous() && (t.scalar_type() == type() || t.scalar_type() == at::kFloat);
+  }
+  bool usual() const {
+    if (!everyday_floats(residual) || !everyday_matrix(residual) || residual.size(1) > RLK_NORM_MAX_WIDTH || residual.size(0) > INT_MAX) return false;
+    const int64_t width = residual.size(1);
+    if (block.defined() && !(everyday_floats(block, residual) && block.sizes() == residual.sizes() && block.is_contiguous())) return false;
+    if (!of_type(residual)) return false;
+    for (const Tensor* w : {&post, &pre})
+      if (w->defined() && !(of_type(*w) && w->dim() == 1 && w->size(0) == width)) return false;
+    if (kind == RLK_GATE_NONE) return !gate.defined();
+    const int64_t cells = kind == RLK_GATE_CHANNEL ? width : kind == RLK_GATE_TOKEN ? residual.size(0) : residual.numel();
+    return of_type(gate) && gate.numel() == cells;
+  }
+  rlk_block_norm describe(const Tensor& rstd) const {
+    const int64_t width = residual.size(1);
+    rlk_block_norm n{};
+    n.block = address(block);
+    n.residual = residual.data_ptr();
+    n.gate = address(gate);
+    n.post_weight = address(post);
+    n.pre_weight = address(pre);
+    n.rstd = writable(rstd);
+    n.block_row_stride = n.residual_row_stride = width;
+    n.gate_row_stride = kind == RLK_GATE_TOKEN ? 1 : width;
+    n.tokens = residual.size(0);
+    n.width = (int)width;
+    n.dtype = block.defined() ? dtype_code(block) : dtype_code(residual);
+    n.residual_dtype = dtype_code(residual);
+    n.gate_kind = kind;
+    n.gate_dtype = gate.defined() ? dtype_code(gate) : n.dtype;
+    n.post_dtype = post.defined() ? dtype_code(post) : n.dtype;
+    n.pre_dtype = pre.defined() ? dtype_code(pre) : n.dtype;
+    n.eps = (float)eps;
+    n.residual_scale = (float)scale;
+    return n;
+  }
+};
+
+// total (with a block) and normed (with a weight for it), in the residual's shape `shape`
+variable_list norm_forward(const NormInputs& in, const Tensor& rstd, at::IntArrayRef shape) {
+  const rlk_block_norm n = in.describe(rstd);
+  const Tensor total = in.block.defined() ? empty(shape, in.residual.scalar_type(), in.residual) : Tensor();
+  const Tensor normed = in.pre.defined() ? empty(shape, in.type(), in.residual) : Tensor();
+  check_status(norm_entry(&n, address(total), address(normed), stream_of(in.residual)), "rlk_block_norm_forward failed");
+  return {total, normed};
+}
+
+struct NormFn : torch::autograd::Function<NormFn> {
+  using Maybe = std::optional<Tensor>;
+
+  // (the inputs once more as arguments of their own: those are what autograd sees)
+  static variable_list forward(AutogradContext* ctx, const Maybe& block, const Tensor& residual, const Maybe& gate, const Maybe& post,
+                               const Maybe& pre, const NormInputs* in, at::IntArrayRef shape) {
+    const Tensor rstd = empty({2, in->residual.size(0)}, at::kFloat, in->residual);
+    const variable_list out = norm_forward(*in, rstd, shape);
+    auto known = [](const Maybe& t) { return t.has_value() ? *t : Tensor(); };
+    save_some(ctx, {known(block), residual, known(gate), known(post), known(pre), rstd});
+    ctx->saved_data["kind"] = (int64_t)in->kind;
+    ctx->saved_data["eps"] = in->eps;
+    ctx->saved_data["scale"] = in->scale;
+    ctx->saved_data["total"] = out[0].defined();
+    ctx->set_materialize_grads(false);
+    variable_list made;
+    for (const Tensor& t : out)
+      if (t.defined()) made.push_back(t);
+    return made;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list result(7);
+    const bool with_total = ctx->saved_data["total"].toBool();
+    const Tensor g_total = with_total ? grads[0] : Tensor();
+    const Tensor g_normed = with_total ? (grads.size() > 1 ? grads[1] : Tensor()) : grads[0];
+    if (!g_total.defined() && !g_normed.defined()) return result;
+    const variable_list s = saved_some(ctx, 6);
+    auto rows = [](const Tensor& t) { return t.defined() && t.dim() != 2 && t.numel() > 0 ? t.reshape({-1, t.size(-1)}) : t; };
+    NormInputs in{rows(s[0]), rows(s[1]), s[2], s[3], s[4], (int)ctx->saved_data["kind"].toInt(), ctx->saved_data["eps"].toDouble(),
+                  ctx->saved_data["scale"].toDouble()};
+    const Tensor& rstd = s[5];
+    bool values = !at::GradMode::is_enabled() && everyday_thread() && in.usual() && everyday(rstd, at::kFloat, in.residual);
+    if (values && g_total.defined())
+      values = everyday(g_total, in.residual.scalar_type(), in.residual) && g_total.is_contiguous() && g_total.numel() == in.residual.numel();
+    if (values && g_normed.defined())
+      values = everyday(g_normed, in.type(), in.residual) && g_normed.is_contiguous() && g_normed.numel() == in.residual.numel();
+    if (values) {
+      const c10::OptionalDeviceGuard guard(in.residual.device());
+      // needs_input_grad() counts the tensors that were defined
+      int place = 0;
+      for (int i = 0; i < 5; ++i) {
+        if (!s[i].defined()) continue;
+        if (ctx->needs_input_grad(place++)) result[i] = empty(s[i].sizes(), s[i].scalar_type(), in.residual);
+      }
+      const rlk_block_norm n = in.describe(rstd);
+      const size_t bytes = norm_workspace_entry(n.tokens, n.width);
+      const Tensor workspace = empty({(int64_t)bytes}, at::kByte, in.residual);
+      check_status(norm_bwd_entry(&n, address(g_total), address(g_normed), address(result[0]), address(result[1]), address(result[2]),
+                                  address(result[3]), address(result[4]), workspace.data_ptr(), bytes, stream_of(in.residual)),
+                   "rlk_block_norm_backward failed");
+      return result;
+    }
+    const pybind11::gil_scoped_acquire gil;
+    const PyRef args(PyTuple_New(16));
+    for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(args.get(), i, wrap(s[i]));
+    PyTuple_SET_ITEM(args.get(), 6, PyLong_FromLong(in.kind));
+    PyTuple_SET_ITEM(args.get(), 7, PyFloat_FromDouble(in.eps));
+    PyTuple_SET_ITEM(args.get(), 8, PyFloat_FromDouble(in.scale));
+    PyTuple_SET_ITEM(args.get(), 9, wrap(g_total));
+    PyTuple_SET_ITEM(args.get(), 10, wrap(g_normed));
+    int place = 0;
+    for (int i = 0; i < 5; ++i) {
+      const bool need = s[i].defined() && ctx->needs_input_grad(place);
+      if (s[i].defined()) ++place;
+      PyTuple_SET_ITEM(args.get(), 11 + i, PyBool_FromLong(need));
+    }
+    const PyRef five(PyObject_CallObject(general_norm_gradients, args.get()));
+    const variable_list out = tensors_of(five, 5);
+    for (int i = 0; i < 5; ++i) result[i] = out[i];
+    return result;
+  }
+};
+
+bool takes_swiglu(const Tensor& gate, const Tensor& up) {
+  return everyday_floats(gate) && gate.dim() >= 1 && gate.is_contiguous() && gate.numel() > 0 && gate.size(-1) <= (1 << 28) &&
+         everyday(up, gate.scalar_type(), gate) && up.is_contiguous() && up.sizes() == gate.sizes();
+}
+
+struct Mx8SwigluFn : torch::autograd::Function<Mx8SwigluFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up) {
+    const int64_t cols = gate.size(-1), rows = gate.numel() / cols, runs = (cols + 31) / 32;
+    const Tensor y = empty(gate.sizes(), gate.scalar_type(), gate);
+    Tensor codes[2], scales[2];
+    for (int i = 0; i < 2; ++i) {
+      codes[i] = empty({rows, cols}, at::kChar, gate);
+      scales[i] = empty({rows, runs}, at::kByte, gate);
+    }
+    check_status(mx8_swiglu_entry(gate.data_ptr(), cols, up.data_ptr(), cols, dtype_code(gate), y.data_ptr(),
+                                  static_cast<int8_t*>(codes[0].data_ptr()), static_cast<uint8_t*>(scales[0].data_ptr()),
+                                  static_cast<int8_t*>(codes[1].data_ptr()), static_cast<uint8_t*>(scales[1].data_ptr()), rows, (int)cols,
+                                  stream_of(gate)),
+                 "rlk_mx8_swiglu_forward failed");
+    ctx->save_for_backward({codes[0], scales[0], codes[1], scales[1]});
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor& dy = grads[0];
+    const int64_t cols = s[0].size(1), rows = s[0].size(0);
+    bool values = !at::GradMode::is_enabled() && everyday_thread() && everyday_floats(dy) && dy.is_contiguous() && dy.numel() == rows * cols;
+    for (int i = 0; values && i < 4; ++i) values = everyday(s[i], i % 2 ? at::kByte : at::kChar, dy) && s[i].is_contiguous();
+    if (values) {
+      const c10::OptionalDeviceGuard guard(dy.device());
+      const Tensor d_gate = empty(dy.sizes(), dy.scalar_type(), dy), d_up = empty(dy.sizes(), dy.scalar_type(), dy);
+      check_status(mx8_swiglu_bwd_entry(dy.data_ptr(), cols, dtype_code(dy), static_cast<const int8_t*>(s[0].data_ptr()),
+                                        static_cast<const uint8_t*>(s[1].data_ptr()), static_cast<const int8_t*>(s[2].data_ptr()),
+                                        static_cast<const uint8_t*>(s[3].data_ptr()), d_gate.data_ptr(), d_up.data_ptr(), nullptr, rows,
+                                        (int)cols, stream_of(dy)),
+                   "rlk_mx8_swiglu_backward failed");
+      return {ctx->needs_input_grad(0) ? d_gate : Tensor(), ctx->needs_input_grad(1) ? d_up : Tensor()};
+    }
+    const pybind11::gil_scoped_acquire gil;
+    const PyRef args(PyTuple_New(5));
+    PyTuple_SET_ITEM(args.get(), 0, wrap(dy));
+    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(args.get(), 1 + i, wrap(s[i]));
+    const PyRef two(PyObject_CallObject(general_swiglu_gradients, args.get()));
+    return tensors_of(two, 2);
+  }
+};
+
+// ---------------------------------------------------------------------------
 // The Python module
 // ---------------------------------------------------------------------------
 
@@ -439,11 +753,137 @@ PyObject* py_grpo(PyObject*, PyObject* const* args, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of the entry points by name, the general gradients of the linear layer, the FFN and the GRPO loss)
+// A Python argument that is a Tensor, a Parameter or None; false for anything else.
+bool tensor_or_nothing(PyObject* o, Tensor* t) {
+  if (o == Py_None) return true;
+  const Tensor* const exact = exact_tensor(o);
+  if (exact == nullptr) return false;
+  *t = *exact;
+  return true;
+}
+
+// scores(logits, target, temperature or None, real vocabulary, top_k) -> (logp, lse, entropy, top_logp or None, top_ids or None), or None
+PyObject* py_scores(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 5 || scores_entry == nullptr) return none();
+  ScoreInputs in;
+  if (!tensor_or_nothing(args[0], &in.logits) || !tensor_or_nothing(args[1], &in.target) || !tensor_or_nothing(args[2], &in.temp) ||
+      !PyLong_CheckExact(args[3]) || !PyLong_CheckExact(args[4]))
+    return none();
+  int overflow[2];
+  in.real = PyLong_AsLongLongAndOverflow(args[3], &overflow[0]);
+  const long top_k = PyLong_AsLongAndOverflow(args[4], &overflow[1]);
+  if (overflow[0] != 0 || overflow[1] != 0 || top_k < 0 || top_k > RLK_SCORES_MAX_TOP_K) return none();
+  in.top_k = (int)top_k;
+  if (!everyday_caller() || !in.usual()) return none();
+  variable_list out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const c10::OptionalDeviceGuard guard(in.logits.device());
+    out = at::GradMode::is_enabled() && in.logits.requires_grad() ? ScoresFn::apply(in.logits, &in) : scores(in);
+  }
+  out.resize(5);
+  const PyRef logp(wrap(out[0])), lse(wrap(out[1])), entropy(wrap(out[2])), top_logp(wrap(out[3])), top_ids(wrap(out[4]));
+  return PyTuple_Pack(5, logp.get(), lse.get(), entropy.get(), top_logp.get(), top_ids.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// norm(block or None, residual, gate or None, post weight or None, weight or None, eps, scale) -> (total or None, normed or None), or None
+PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 7 || norm_entry == nullptr) return none();
+  Tensor t[5];  // block, residual, gate, post, pre
+  for (int i = 0; i < 5; ++i)
+    if (!tensor_or_nothing(args[i], &t[i])) return none();
+  for (int i = 5; i < 7; ++i)
+    if (!PyFloat_CheckExact(args[i]) && !PyLong_CheckExact(args[i])) return none();
+  const double eps = PyFloat_AsDouble(args[5]), scale = PyFloat_AsDouble(args[6]);
+  if (PyErr_Occurred()) throw python_error();
+  if (!everyday_caller() || !everyday_floats(t[1]) || t[1].dim() < 1 || !t[1].is_contiguous() || t[1].numel() == 0) return none();
+  if (t[0].defined() && !(everyday_floats(t[0], t[1]) && t[0].is_contiguous() && t[0].sizes() == t[1].sizes())) return none();
+  if (!t[0].defined() && (!t[4].defined() || t[2].defined() || t[3].defined())) return none();
+  const at::IntArrayRef shape = t[1].sizes();
+  int kind = RLK_GATE_NONE;
+  if (t[2].defined()) {
+    if (!everyday_floats(t[2], t[1])) return none();
+    if (t[2].dim() == 1 && t[2].size(0) == shape.back()) kind = RLK_GATE_CHANNEL;
+    else if (t[2].sizes() == shape) kind = RLK_GATE_FULL;
+    else if (t[2].dim() == t[1].dim() && t[2].size(-1) == 1 && t[2].sizes().slice(0, shape.size() - 1) == shape.slice(0, shape.size() - 1)) kind = RLK_GATE_TOKEN;
+    else return none();
+  }
+  // (views of rows are made where autograd does not look)
+  NormInputs in;
+  bool differentiable = false;
+  {
+    const at::NoGradGuard no_grad;
+    auto rows = [](const Tensor& x) { return !x.defined() || x.dim() == 2 ? x : x.view({-1, x.size(-1)}); };
+    in = NormInputs{rows(t[0]), rows(t[1]), t[2], t[3], t[4], kind, eps, scale};
+  }
+  if (!in.usual()) return none();
+  for (const Tensor& x : t) differentiable |= x.defined() && x.requires_grad();
+  variable_list out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const c10::OptionalDeviceGuard guard(t[1].device());
+    if (differentiable && at::GradMode::is_enabled()) {
+      auto maybe = [](const Tensor& x) { return x.defined() ? NormFn::Maybe(x) : NormFn::Maybe(); };
+      out = NormFn::apply(maybe(t[0]), t[1], maybe(t[2]), maybe(t[3]), maybe(t[4]), &in, shape);
+      if (!t[0].defined()) out.insert(out.begin(), Tensor());
+      out.resize(2);
+    } else {
+      out = norm_forward(in, Tensor(), shape);
+    }
+  }
+  const PyRef total(wrap(out[0])), normed(wrap(out[1]));
+  return PyTuple_Pack(2, total.get(), normed.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// mx8_swiglu(gate, up) -> silu(gate) * up, differentiable through eight-bit copies, or None
+PyObject* py_mx8_swiglu(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 2 || mx8_swiglu_entry == nullptr) return none();
+  const Tensor *gate = exact_tensor(args[0]), *up = exact_tensor(args[1]);
+  if (gate == nullptr || up == nullptr || !everyday_caller() || !takes_swiglu(*gate, *up)) return none();
+  if (!at::GradMode::is_enabled() || !(gate->requires_grad() || up->requires_grad())) return none();
+  Tensor y;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const c10::OptionalDeviceGuard guard(gate->device());
+    y = Mx8SwigluFn::apply(*gate, *up);
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// mx8_encode(x [rows, columns]) -> (codes, scales), or None
+PyObject* py_mx8_encode(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 1 || mx8_encode_entry == nullptr) return none();
+  const Tensor* const x = exact_tensor(args[0]);
+  if (x == nullptr || !everyday_caller() || !everyday_floats(*x) || !everyday_matrix(*x) || x->size(1) > (1 << 28)) return none();
+  const int64_t rows = x->size(0), cols = x->size(1);
+  Tensor codes, scales;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const c10::OptionalDeviceGuard guard(x->device());
+    codes = empty({rows, cols}, at::kChar, *x);
+    scales = empty({rows, (cols + 31) / 32}, at::kByte, *x);
+    check_status(mx8_encode_entry(x->data_ptr(), cols, dtype_code(*x), static_cast<int8_t*>(codes.data_ptr()),
+                                  static_cast<uint8_t*>(scales.data_ptr()), rows, (int)cols, stream_of(*x)),
+                 "rlk_mx8_encode failed");
+  }
+  const PyRef py_codes(wrap(codes)), py_scales(wrap(scales));
+  return PyTuple_Pack(2, py_codes.get(), py_scales.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(addresses of the entry points by name, the general gradients of the linear layer, the FFN, the GRPO loss, the token scores, the
+// norm between blocks and the SwiGLU of eight-bit copies)
 PyObject* py_bind(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
-  PyObject *addresses, *linear, *ffn, *loss;
-  if (!PyArg_ParseTuple(args, "O!OOO", &PyDict_Type, &addresses, &linear, &ffn, &loss)) return nullptr;
+  PyObject *addresses, *linear, *ffn, *loss, *of_scores = Py_None, *of_norm = Py_None, *of_swiglu = Py_None;
+  if (!PyArg_ParseTuple(args, "O!OOO|OOO", &PyDict_Type, &addresses, &linear, &ffn, &loss, &of_scores, &of_norm, &of_swiglu)) return nullptr;
   auto entry = [&](const char* name, auto& to) {
     PyObject* const at = PyDict_GetItemString(addresses, name);
     void* const address = at != nullptr ? PyLong_AsVoidPtr(at) : nullptr;
@@ -460,6 +900,21 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   entry("rlk_grpo_workspace_bytes", grpo_workspace_entry);
   entry("rlk_grpo_ratio_kl_loss", grpo_entry);
   entry("rlk_grpo_ratio_kl_loss_bwd", grpo_bwd_entry);
+  entry("rlk_logits_scores_workspace_bytes", scores_workspace_entry);
+  entry("rlk_logits_scores_backward", scores_bwd_entry);
+  entry("rlk_block_norm_workspace_bytes", norm_workspace_entry);
+  entry("rlk_block_norm_backward", norm_bwd_entry);
+  entry("rlk_mx8_swiglu_backward", mx8_swiglu_bwd_entry);
+  entry("rlk_mx8_encode", mx8_encode_entry);
+  for (const auto& [from, to] : {std::pair<PyObject*, PyObject**>{of_scores, &general_scores_gradient},
+                                 {of_norm, &general_norm_gradients},
+                                 {of_swiglu, &general_swiglu_gradients}}) {
+    Py_INCREF(from);
+    Py_XSETREF(*to, from);
+  }
+  entry("rlk_logits_scores", scores_entry);
+  entry("rlk_block_norm_forward", norm_entry);
+  entry("rlk_mx8_swiglu_forward", mx8_swiglu_entry);
   Py_INCREF(linear);
   Py_XSETREF(general_linear_gradients, linear);
   Py_INCREF(ffn);
@@ -476,6 +931,10 @@ PyMethodDef methods[] = {
     {"packed_ffn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_packed_ffn)), METH_FASTCALL, nullptr},
     {"ffn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_ffn)), METH_FASTCALL, nullptr},
     {"grpo", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_grpo)), METH_FASTCALL, nullptr},
+    {"scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_scores)), METH_FASTCALL, nullptr},
+    {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm)), METH_FASTCALL, nullptr},
+    {"mx8_swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx8_swiglu)), METH_FASTCALL, nullptr},
+    {"mx8_encode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx8_encode)), METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

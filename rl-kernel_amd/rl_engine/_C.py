@@ -1156,6 +1156,11 @@ def _check_mx8(codes: torch.Tensor, scales: torch.Tensor, name: str) -> None:
 
 def mx8_encode(x: torch.Tensor) -> tuple:
     """``(codes, scales)`` of ``x [rows, columns]``: int8 and one exponent byte per run of 32 columns (rlk_mx8_encode)."""
+    from rl_engine import _host  # (which binds functions of modules that import this one)
+
+    both = _host.native().mx8_encode(x)
+    if both is not None:
+        return both
     src = _mx8_rows(x, "x")
     rows, cols = src.shape
     codes, scales = _mx8_buffers(rows, cols, src.device)

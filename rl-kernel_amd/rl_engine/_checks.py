@@ -40,6 +40,27 @@ def assert_async_or_raise(condition: torch.Tensor, exception: type, message: str
         raise exception(host_message or message)
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("this gradient is not differentiable: it was computed by a kernel without a backward of its own")
+
+
+def without_second_derivative(grads: list) -> list:
+    """``grads`` (tensors or ``None``) that raise when somebody differentiates them, which is possible where a graph of the backward
+    is made (``create_graph``); as they are elsewhere."""
+    if not torch.is_grad_enabled() or all(g is None for g in grads):
+        return grads
+    given = [g for g in grads if g is not None]
+    anchor = torch.empty((0,), device=given[0].device, requires_grad=True)  # (what they were computed from may be gone)
+    given = iter(_NoSecondDerivative.apply(len(given), *given, anchor))
+    return [None if g is None else next(given) for g in grads]
+
+
 def output_buffer_rules(out: torch.Tensor, shape: tuple[int, int], device: torch.device, what: str) -> list[Rule]:
     """Rules for a caller-owned bf16 ``[M, N]`` output with contiguous rows (``what`` prefixes the messages)."""
     return [

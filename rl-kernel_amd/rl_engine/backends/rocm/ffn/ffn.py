@@ -20,10 +20,9 @@ from typing import Any
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from rl_engine import _C, _host, _lib
-from rl_engine._checks import enforce
+from rl_engine._checks import enforce, without_second_derivative
 from rl_engine.backends.rocm.gemm import swiglu_gemm
 from rl_engine.backends.rocm.gemm.det_gemm import (
     det_gemm_backend,
@@ -222,8 +221,13 @@ class _CheckpointedFFNFunction(torch.autograd.Function):
         return output.reshape(*shape[:-1], output.size(-1))
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_output):
+        with torch.no_grad():
+            grads = _CheckpointedFFNFunction.gradients(ctx, grad_output)
+        return *without_second_derivative(grads), None
+
+    @staticmethod
+    def gradients(ctx, grad_output) -> list:
         codes, scales, *kept, gate_weight, up_weight, down_weight = ctx.saved_tensors
         need_x, need_gate, need_up, need_down = ctx.needs_input_grad[:4]
         grad_output = grad_output.reshape(-1, grad_output.size(-1)).to(torch.bfloat16).contiguous()
@@ -237,7 +241,15 @@ class _CheckpointedFFNFunction(torch.autograd.Function):
         from_up, grad_up_weight = _linear_gradients(x, up_weight, grad_up, need_x, need_up)
         if need_x:
             grad_x = grad_x.add_(from_up).reshape(ctx.input_shape)
-        return grad_x, grad_gate_weight, grad_up_weight, grad_down_weight, None
+        return [grad_x, grad_gate_weight, grad_up_weight, grad_down_weight]
+
+
+def kept_swiglu_gradients(dy, gate_codes, gate_scales, up_codes, up_scales) -> tuple:
+    """``(d_gate, d_up)`` in the shape of ``dy``, from the copies of gate and up."""
+    with torch.no_grad():
+        d_gate, d_up, _ = _C.swiglu_mx8_backward(dy.reshape(gate_codes.shape), gate_codes, gate_scales, up_codes, up_scales)
+        grads = [d_gate.reshape(dy.shape), d_up.reshape(dy.shape)]
+    return tuple(without_second_derivative(grads))
 
 
 class _CheckpointedSwiglu(torch.autograd.Function):
@@ -248,9 +260,8 @@ class _CheckpointedSwiglu(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        d_gate, d_up, _ = _C.swiglu_mx8_backward(dy, *ctx.saved_tensors)
+        d_gate, d_up = kept_swiglu_gradients(dy, *ctx.saved_tensors)
         need_gate, need_up = ctx.needs_input_grad
         return d_gate if need_gate else None, d_up if need_up else None
 

@@ -14,10 +14,9 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from rl_engine import _C, _lib
-from rl_engine._checks import enforce
+from rl_engine import _C, _host, _lib
+from rl_engine._checks import enforce, without_second_derivative
 from rl_engine.backends.rocm.logprob.linear_logp import _logits_to_save, _prepare, _requires_grad
 
 # Logits that nobody keeps go through a buffer of at most this size, whole rows of tiles of 256 tokens at a time: 3328 tokens of
@@ -82,6 +81,14 @@ def _shaped(scores, shape: torch.Size) -> TokenScores:
 # ---------------------------------------------------------------------------
 
 
+def scores_gradient(logits, target_1d, temp, lse, entropy, top_ids, real, g_logp, g_lse, g_entropy, g_top) -> torch.Tensor:
+    """d(logits) of the scores of ``logits [rows, V]``, from the forward's answers and the gradients of its outputs (or ``None``)."""
+    grads = (g_logp, g_lse, g_entropy, g_top)
+    with torch.no_grad():
+        grad = _C.logits_scores_backward(logits, target_1d, real, lse, entropy, top_ids, grads, temperature=temp)
+    return without_second_derivative([grad])[0]
+
+
 class _ScoresFromLogits(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target_1d, temp, real, top_k):
@@ -94,14 +101,11 @@ class _ScoresFromLogits(torch.autograd.Function):
         return logp, lse, entropy, top_logp, top_ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_logp, g_lse, g_entropy, g_top, _g_ids):
         grads = (g_logp, g_lse, g_entropy, g_top)
         if all(g is None for g in grads):
             return (None,) * 5
-        logits, target_1d, temp, lse, entropy, top_ids = ctx.saved_tensors
-        grad = _C.logits_scores_backward(logits, target_1d, ctx.real, lse, entropy, top_ids, grads, temperature=temp)
-        return grad, None, None, None, None
+        return scores_gradient(*ctx.saved_tensors, ctx.real, *grads), None, None, None, None
 
 
 def hip_deterministic_scores_from_logits(
@@ -122,6 +126,11 @@ def hip_deterministic_scores_from_logits(
     Without ``validate`` no value is read back: an id outside of the real vocabulary gives ``logp = NaN``, a temperature that is
     not positive NaN throughout. With it such a call raises ``ValueError`` (and cannot be captured into a graph).
     """
+    if not validate and isinstance(logits, torch.Tensor) and logits.dim() == 2 and not torch.compiler.is_compiling():
+        real = logits.size(1) if real_vocab_size is None else real_vocab_size
+        scores = _host.native().scores(logits, target_ids, temperature, real, top_k)  # everyday arguments, natively
+        if scores is not None:
+            return TokenScores(*scores)
     enforce([
         (isinstance(logits, torch.Tensor) and logits.dim() >= 2, ValueError, "logits must be a tensor [..., vocabulary] of at least two dimensions"),
         (lambda: logits.dtype in (torch.bfloat16, torch.float16, torch.float32), TypeError, lambda: f"logits must be bf16, fp16 or fp32, got {logits.dtype}"),
@@ -198,11 +207,16 @@ class _LinearScores(torch.autograd.Function):
         return logp, lse, entropy, top_logp, top_ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_logp, g_lse, g_entropy, g_top, _g_ids):
         grads = (g_logp, g_lse, g_entropy, g_top)
         if all(g is None for g in grads):
             return (None,) * 7
+        with torch.no_grad():
+            two = _LinearScores.gradients(ctx, grads)
+        return *without_second_derivative(two), None, None, None, None, None
+
+    @staticmethod
+    def gradients(ctx, grads) -> list:
         hidden, weight, bias, target, temp, lse, entropy, top_ids, kept = ctx.saved_tensors
         tokens, vocab = hidden.size(0), weight.size(0)
         dz = torch.empty((tokens, _C.linear_dlogits_row_stride(vocab)), dtype=torch.bfloat16, device=hidden.device)
@@ -218,8 +232,7 @@ class _LinearScores(torch.autograd.Function):
                 tuple(_rows(g, first, end) for g in grads), temperature=rows_temp, out=dz[first:end],
             )  # fmt: skip
         del logits
-        grad_hidden, grad_weight = _C.linear_dlogits_bwd(dz, hidden, weight, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return grad_hidden, grad_weight, None, None, None, None, None
+        return _C.linear_dlogits_bwd(dz, hidden, weight, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
 
 
 def hip_deterministic_linear_scores(

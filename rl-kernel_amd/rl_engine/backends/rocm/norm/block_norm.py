@@ -13,11 +13,10 @@ from typing import Optional
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
-from rl_engine import _lib
+from rl_engine import _host, _lib
 from rl_engine._C import _on, _row_stride, _stream_handle
-from rl_engine._checks import enforce
+from rl_engine._checks import enforce, without_second_derivative
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
 
@@ -59,43 +58,50 @@ def _forward(block, residual, gate, gate_kind, post, pre, dtype, eps, scale, wit
     return total, normed, rstd
 
 
+def norm_gradients(
+    block, residual, gate, post, pre, rstd, gate_kind, eps, scale, g_total, g_normed, need_block, need_residual, need_gate, need_post, need_pre,
+    *, dtype: Optional[torch.dtype] = None,
+) -> tuple:  # fmt: skip
+    """The gradients of ``block``, ``residual``, ``gate`` and the weights that are wanted, ``None`` for the others. ``block`` and
+    ``residual`` are rows or batches of rows; ``dtype``: the type of the normed result (that of ``block``, or of ``residual``)."""
+    dtype = dtype or (residual if block is None else block).dtype
+    device, width = residual.device, residual.size(-1)
+    with torch.no_grad():
+        rows = [None if t is None else _rows(t, width) for t in (block, residual)]
+        tokens = rows[1].size(0)
+        g_rows = [None if g is None else g.reshape(tokens, width).to(t).contiguous() for g, t in ((g_total, residual.dtype), (g_normed, dtype))]
+        new = lambda t, want: torch.empty(t.shape, dtype=t.dtype, device=device) if want else None  # noqa: E731
+        made = [new(block, need_block), new(residual, need_residual), new(gate, need_gate), new(post, need_post), new(pre, need_pre)]
+        lib = _lib.load()
+        size = int(lib.rlk_block_norm_workspace_bytes(tokens, width))
+        workspace = torch.empty((size,), dtype=torch.uint8, device=device)
+        flat_gate = gate if gate is None or gate_kind == _lib.GATE_CHANNEL else _rows(gate, gate.size(-1))
+        norm = _describe(*rows, flat_gate, gate_kind, post, pre, rstd, dtype, eps, scale)
+        with _on(device):
+            status = lib.rlk_block_norm_backward(
+                ctypes.byref(norm), *(_address(g) for g in g_rows), *(_address(d) for d in made), workspace.data_ptr(), size,
+                _stream_handle(device),
+            )  # fmt: skip
+        _lib.check(status, "rlk_block_norm_backward failed")
+    return tuple(without_second_derivative(made))
+
+
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, block, residual, gate, post, pre, gate_kind, dtype, eps, scale, with_total):
         total, normed, rstd = _forward(block, residual, gate, gate_kind, post, pre, dtype, eps, scale, with_total, True)
         ctx.save_for_backward(block, residual, gate, post, pre, rstd)
-        ctx.how = (gate_kind, dtype, eps, scale)
+        ctx.how = (gate_kind, eps, scale)
+        ctx.dtype = dtype
         ctx.set_materialize_grads(False)
         return total, normed
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_total, g_normed):
         if g_total is None and g_normed is None:
             return (None,) * 10
-        block, residual, gate, post, pre, rstd = ctx.saved_tensors
-        gate_kind, dtype, eps, scale = ctx.how
-        device = residual.device
-        tokens, width = residual.shape
-        need = ctx.needs_input_grad
-        g_total = None if g_total is None else g_total.contiguous()
-        g_normed = None if g_normed is None else g_normed.contiguous()
-        d_block = torch.empty((tokens, width), dtype=dtype, device=device) if need[0] else None
-        d_residual = torch.empty((tokens, width), dtype=residual.dtype, device=device) if need[1] else None
-        d_gate = torch.empty(gate.shape, dtype=gate.dtype, device=device) if need[2] else None
-        d_post = torch.empty((width,), dtype=post.dtype, device=device) if need[3] else None
-        d_pre = torch.empty((width,), dtype=pre.dtype, device=device) if need[4] else None
-        lib = _lib.load()
-        size = int(lib.rlk_block_norm_workspace_bytes(tokens, width))
-        workspace = torch.empty((size,), dtype=torch.uint8, device=device)
-        norm = _describe(block, residual, gate, gate_kind, post, pre, rstd, dtype, eps, scale)
-        with _on(device):
-            status = lib.rlk_block_norm_backward(
-                ctypes.byref(norm), _address(g_total), _address(g_normed), _address(d_block), _address(d_residual), _address(d_gate),
-                _address(d_post), _address(d_pre), workspace.data_ptr(), size, _stream_handle(device),
-            )  # fmt: skip
-        _lib.check(status, "rlk_block_norm_backward failed")
-        return d_block, d_residual, d_gate, d_post, d_pre, None, None, None, None, None
+        grads = norm_gradients(*ctx.saved_tensors, *ctx.how, g_total, g_normed, *ctx.needs_input_grad[:5], dtype=ctx.dtype)
+        return *grads, None, None, None, None, None
 
 
 def _check_rows(t: Tensor, name: str) -> None:
@@ -162,6 +168,10 @@ def gated_residual_norm(
     ``block [..., width]`` is bf16, fp16 or fp32 and the normed result has its type; ``residual`` (and the sum), ``gate`` and the
     weights have that type or fp32. Arithmetic is in fp32 with one rounding per result. Rows have up to 16384 elements.
     """
+    if isinstance(block, Tensor) and not torch.compiler.is_compiling():
+        both = _host.native().norm(block, residual, gate, post_weight, weight, eps, residual_scale)  # everyday arguments, natively
+        if both is not None:
+            return both
     _check_rows(block, "block")
     _check_beside(residual, "residual", block, block.dtype)
     if residual.shape != block.shape:
@@ -184,6 +194,10 @@ def gated_residual_norm(
 def rms_norm(x: Tensor, weight: Tensor, *, eps: float = 1e-6, dtype: Optional[torch.dtype] = None) -> Tensor:
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension, in ``dtype`` (that of ``x``; an fp32 ``x`` may be normed
     to any); differentiable in ``x`` and ``weight``, which has the result's type or fp32. Rows have up to 16384 elements."""
+    if dtype is None and not torch.compiler.is_compiling():
+        both = _host.native().norm(None, x, None, None, weight, eps, 1.0)
+        if both is not None:
+            return both[1]
     _check_rows(x, "x")
     dtype = x.dtype if dtype is None else dtype
     if dtype not in _DTYPES or x.dtype not in (dtype, torch.float32):
