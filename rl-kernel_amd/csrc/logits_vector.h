@@ -162,6 +162,12 @@ struct UnalignedPart<4> {
   using type = u32x4_at4_t;
 };
 
+// The first of the eight columns that a load at `col` of a row of `cols` columns brings (RowVector::load_window).
+__device__ __forceinline__ int window_of(int col, int cols) {
+  const int last = cols > 8 ? cols - 8 : 0;
+  return col < last ? col : last;
+}
+
 // Eight logits of a row. Rows may start at any element: the loads ask for the element's alignment only.
 template <int ELEM>
 struct RowVector {
@@ -194,11 +200,35 @@ struct RowVector {
       __builtin_memcpy(w, vals, sizeof(w));
     }
   }
-  __device__ __forceinline__ void unpack(float (&y)[8]) const {
-    E vals[8];
-    __builtin_memcpy(vals, w, sizeof(w));
+  // Columns [col, col + 8): a uniform row and a lane's offset of 32 bits (rows have up to 2^28 columns).
+  template <bool NT>
+  __device__ __forceinline__ void load_at(const E* row, uint32_t col) {
+    load<NT>(reinterpret_cast<const E*>(reinterpret_cast<const char*>(row) + col * (uint32_t)sizeof(E)));
+  }
+  // Columns [window_of(col, cols), + 8): a vector that would run past the row is read from further left, so that it is one wide
+  // load as well. (Element by element it was the better half of a kernel's code, all of it fetched once by a call of one row.)
+  template <bool NT>
+  __device__ __forceinline__ void load_window(const E* row, int col, int cols) {
+    if (cols >= 8) {
+      load_at<NT>(row, (uint32_t)(col < cols - 8 ? col : cols - 8));
+    } else if constexpr (sizeof(E) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = LogitElem<ELEM>::to_float(vals[i]);
+      for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = reinterpret_cast<const uint32_t*>(row)[i < cols ? i : cols - 1];
+    } else {
+      const uint16_t* bits = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[0][i] = bits[2 * i < cols ? 2 * i : cols - 1] | (uint32_t)bits[2 * i + 1 < cols ? 2 * i + 1 : cols - 1] << 16;
+    }
+  }
+  // (word by word: held as an array of halves the eight would take a register each while they wait)
+  __device__ __forceinline__ void unpack(float (&y)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (ELEM == RLK_DTYPE_FP32) y[i] = __uint_as_float(w[i / 4][i % 4]);
+      else if constexpr (ELEM == RLK_DTYPE_BF16) y[i] = __uint_as_float(i % 2 ? w[0][i / 2] & 0xffff0000u : w[0][i / 2] << 16);
+      else y[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[0][i / 2] >> (16 * (i % 2))));
+    }
   }
   // (fp16: the fp32 value is fixed first. Left alone the compiler rounds some last products straight to fp16, some not.)
   __device__ __forceinline__ void pack(const float (&y)[8]) {

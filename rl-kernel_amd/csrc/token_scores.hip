@@ -9,12 +9,13 @@
 // (tile = ceil(V / 64) columns), so that logp and lse are that entry's bits wherever 64 divides V; W is carried beside
 // S: a state (m, s, w) seen from a larger maximum n is (s e(m - n), e(m - n) (w + s (m - n))).
 //
-// The alternatives cost the pass one comparison for each vector of eight logits. A lane of a tile sees a fixed slice of
-// the row (every sixteenth vector of its tile), 1024 slices in all, and notes the largest logit of each and the vector
-// that held it first. Under the order (value descending, column ascending) the k best columns of a row lie in the k
-// slices whose best columns come first: a column outside of them has k better ones. So a second, small kernel picks
-// those slices, reads them again (k / 1024 of the row) and ranks what is not under the k-th slice's best. Nothing of it
-// depends on how a row's values are spread: equal logits, rows of one value and masked rows take the same steps.
+// The alternatives cost the pass two instructions for each vector of eight logits. A lane of a tile sees a fixed slice of
+// the row (every sixteenth vector of its tile), 1024 slices in all, and notes the largest logit of each, the vector
+// that held it first, and the largest logit outside of that vector. Under the order (value descending, column ascending) the k
+// best columns of a row lie in the k slices whose best columns come first: a column outside of them has k better ones. So a
+// second, small kernel picks those slices, reads of each that one vector again (the whole slice only where another of its
+// vectors reaches the k-th slice's best as well) and ranks what does. It is right however a row's values are spread: equal
+// logits, rows of one value and masked rows take the same steps, some of them more often.
 //
 // HBM-bound: a logit is read once.
 #include "logits_vector.h"
@@ -32,8 +33,8 @@ struct ScoreArgs {
   const int64_t* target;     // [T] columns
   const float* temperature;  // [T] or null
   float* stats;              // [T][kScorePlanes][kScoreTiles]
-  uint32_t* best;            // [T][kScoreSlices] largest logit of the slice (ordered bits), 0 for a slice without columns
-  uint32_t* best_at;         // [T][kScoreSlices] first vector that holds it
+  uint32_t* best;   // [T][kScoreSlices] largest logit of the slice (ordered bits), 0 for a slice without columns
+  uint32_t* where;  // [T][kScoreSlices] the upper half of the largest logit in its other vectors | number of the first vector that holds the best
   int T, V, real, tile_size, tiles_per_group;
   int64_t streamed;  // workgroups, in the order of their ids, that read past the caches
 };
@@ -51,7 +52,8 @@ __device__ __forceinline__ float from_ordered_bits(uint32_t o) {
 struct ScoreState {
   float m, s, w;  // scaled maximum, sum, weighted sum
   float raw;      // largest logit before the temperature
-  int at;         // first vector that held it
+  float other;    // largest logit outside of the first vector that held it
+  int at;         // that vector
 };
 
 // The eight logits of vector g folded into a lane's state. The maximum is taken before the temperature (times a positive
@@ -59,7 +61,11 @@ struct ScoreState {
 template <bool HAS_TEMP, bool TOP>
 __device__ __forceinline__ void fold_score_vector(float (&y)[8], float inv_t, int g, ScoreState& st) {
   const float most = max3_f32(max3_f32(max3_f32(y[0], y[1], y[2]), y[3], y[4]), y[5], y[6]);
-  if constexpr (TOP) st.at = fmaxf(most, y[7]) > st.raw ? g : st.at;
+  if constexpr (TOP) {
+    const float here = max3_f32(most, y[7], y[7]);
+    st.at = here > st.raw ? g : st.at;
+    st.other = __builtin_amdgcn_fmed3f(here, st.raw, st.other);  // (other <= raw: the second of the three)
+  }
   st.raw = max3_f32(most, y[7], st.raw);
   float n = st.raw;
   if constexpr (HAS_TEMP) {
@@ -103,10 +109,11 @@ __device__ __forceinline__ void merge_score_lanes(int lane, ScoreState& st) {
   st.m = n;
 }
 
-template <int ELEM, bool HAS_TEMP, bool TOP, bool NT>
+// kBatch: vectors that a lane has on their way. OVERLAP: the exponentials of one vector may run under the folds of another, for
+// which they take registers: for waves that have their SIMD to themselves.
+template <int ELEM, bool HAS_TEMP, bool TOP, int kBatch, bool OVERLAP, bool NT>
 __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
   using E = typename LogitElem<ELEM>::type;
-  constexpr int kBatch = 4;
   constexpr int kStep = kTileLanes * kBatch;  // vectors of a tile per batch
   const int row = blockIdx.x;
   const int lane = threadIdx.x & 63;
@@ -129,8 +136,8 @@ __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
     const int g0 = lo_col / 8;
     const int g1 = hi_col > lo_col ? (hi_col + 7) / 8 : g0;
     const int g_last = g1 > g0 ? g1 - 1 : 0;  // a valid vector to clamp loads to
-    // Batches in which all four vectors of every lane are whole vectors of the lane's tile (only the very first one of a
-    // tile may start before it) run without clamps and with one mask.
+    // Batches in which all four vectors of every lane are whole vectors of the lane's tile need no masks, but for the first vector
+    // of a tile, which may start before it.
     const int g_whole = (hi_col % 8) ? g1 - 1 : g1;
     const int my_clean = g_whole > g0 ? (g_whole - g0) / kStep : 0;
     const int my_slots = (g1 - g0 + kTileLanes - 1) / kTileLanes;
@@ -141,57 +148,58 @@ __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
       slots = max(slots, __builtin_amdgcn_readlane(my_slots, other));
     }
 
-    ScoreState st{kNegInf, 0.f, 0.f, kNegInf, g0 + l16};
+    ScoreState st{kNegInf, 0.f, 0.f, kNegInf, kNegInf, g0 + l16};
     int g = g0 + l16;  // this lane's next vector
-    // The loads rotate through four raw vectors: a vector's registers are free once it is unpacked, and the same vector
-    // of the next batch is fetched into them before the fold, so a lane always has three or four loads in flight.
+    // The loads rotate through the raw vectors: a vector's registers are free once it is unpacked, and the same vector of the next
+    // batch is fetched into them before the fold, so a lane always has that many loads, or one less, in flight. (Behind the
+    // tile its last vector is fetched again.)
     RowVector<ELEM> raw[kBatch];
-    if (clean > 0) {
+    auto fetch = [&](int u, int at) __attribute__((always_inline)) {
+      raw[u].template load_window<NT>(row_ptr, (at < g1 ? at : g_last) * 8, a.V);
+    };
+    auto fetch_of_many = [&](int u, int at) __attribute__((always_inline)) {  // of a row that has a window to spare
+      raw[u].template load_at<NT>(row_ptr, (uint32_t)min((at < g1 ? at : g_last) * 8, a.V - 8));
+    };
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) raw[u].template load<NT>(row_ptr + (int64_t)(g + u * kTileLanes) * 8);
-    }
-    auto clean_batch = [&](auto more, bool first) __attribute__((always_inline)) {
+    for (int u = 0; u < kBatch; ++u) fetch(u, g + u * kTileLanes);
+    int b = 0;
+    for (; b < clean; ++b, g += kStep) {  // without a branch between the folds
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
+        const int gu = g + u * kTileLanes;
         float y[8];
         raw[u].unpack(y);
-        if constexpr (decltype(more)::value) raw[u].template load<NT>(row_ptr + (int64_t)(g + kStep + u * kTileLanes) * 8);
-        if (u == 0 && first) {
-          const int lo = lo_col - g * 8;
+        if constexpr (!OVERLAP) __builtin_amdgcn_sched_barrier(0);
+        fetch_of_many(u, gu + kStep);
+        if (u == 0) {
+          const int lo = lo_col - gu * 8;
 #pragma unroll
           for (int i = 0; i < 8; ++i) y[i] = i >= lo ? y[i] : kNegInf;
         }
-        fold_score_vector<HAS_TEMP, TOP>(y, inv_t, g + u * kTileLanes, st);
+        fold_score_vector<HAS_TEMP, TOP>(y, inv_t, gu, st);
+        if constexpr (!OVERLAP) __builtin_amdgcn_sched_barrier(0);
       }
-    };
-    for (int b = 0; b + 1 < clean; ++b, g += kStep) clean_batch(BoolConstant<true>{}, b == 0);
-    if (clean > 0) {
-      clean_batch(BoolConstant<false>{}, clean == 1);
-      g += kStep;
     }
-    for (int b = clean; b * kBatch < slots; ++b, g += kStep) {  // the rest: clamped loads, both edges masked
+    for (; b * kBatch < slots; ++b, g += kStep) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const int gu = g + u * kTileLanes;
-        raw[u].template load_edge<NT>(row_ptr, gu < g1 ? gu : g_last, a.V);
-      }
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (b * kBatch + u >= slots) break;  // uniform
+        if (b * kBatch + u >= slots) break;
         const int gu = g + u * kTileLanes;
         float y[8];
         raw[u].unpack(y);
-        const int lo = lo_col - gu * 8;
-        const int hi = gu < g1 ? hi_col - gu * 8 : lo;  // columns [lo, hi) of the vector count
+        fetch(u, gu + kStep);
+        const int first = window_of(gu * 8, a.V);
+        const int lo = max(lo_col, gu * 8) - first;  // columns [lo, hi) of the window count: none of a vector behind the tile
+        const int hi = gu < g1 ? min(hi_col, gu * 8 + 8) - first : lo;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (i >= lo && i < hi) ? y[i] : kNegInf;
+        for (int i = 0; i < 8; ++i) y[i] = (uint32_t)(i - lo) < (uint32_t)(hi - lo) ? y[i] : kNegInf;
         fold_score_vector<HAS_TEMP, TOP>(y, inv_t, gu, st);  // a vector of -inf changes nothing
       }
     }
     if constexpr (TOP) {
       const int64_t slice = (int64_t)row * kScoreSlices + tile * kTileLanes + l16;
       a.best[slice] = g0 + l16 < g1 ? ordered_bits(st.raw) : 0u;
-      a.best_at[slice] = (uint32_t)st.at;
+      a.where[slice] = (ordered_bits(st.other) & 0xffff0000u) | (uint32_t)((st.at - g0 - l16) / kTileLanes);
     }
     merge_score_lanes<8>(lane, st);
     merge_score_lanes<4>(lane, st);
@@ -216,10 +224,15 @@ __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
 template <int ELEM, bool HAS_TEMP, bool TOP>
 __global__ __launch_bounds__(256) void score_tiles_kernel(ScoreArgs a) {
   if ((int64_t)blockIdx.y * gridDim.x + blockIdx.x < a.streamed) {
-    score_tiles<ELEM, HAS_TEMP, TOP, true>(a);
+    score_tiles<ELEM, HAS_TEMP, TOP, 4, false, true>(a);
   } else {
-    score_tiles<ELEM, HAS_TEMP, TOP, false>(a);
+    score_tiles<ELEM, HAS_TEMP, TOP, 4, false, false>(a);
   }
+}
+
+template <int ELEM, bool HAS_TEMP, bool TOP>
+__global__ __launch_bounds__(64) void score_few_rows_kernel(ScoreArgs a) {
+  score_tiles<ELEM, HAS_TEMP, TOP, 8, true, false>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -234,7 +247,7 @@ struct ScoreFinishArgs {
   const float* row_lse;  // [T] or null: log-sum-exps that exist; logp and lse are then not written, no alternative is above 0
   const float* stats;
   const uint32_t* best;
-  const uint32_t* best_at;
+  const uint32_t* where;
   float* logp;
   float* lse;
   float* entropy;
@@ -244,20 +257,32 @@ struct ScoreFinishArgs {
 };
 
 constexpr int kFinishWaves = 4;
-constexpr int kFinishKeys = 1024;    // candidates that are held at a time
+constexpr int kFinishKeys = 512;     // candidates that are held at a time
 constexpr int kFinishPicked = 128;   // slices
 constexpr int kScoreMostTop = 64;
 
+// A reduction over the wave in six steps of the data-parallel primitives: rows of 16 first, then across them; the result, which
+// ends in the last lane, in all of them. (Shuffles go through the LDS unit: 2.4 us for the merge of a row, now 1.3.)
+template <class Op>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t v, uint32_t neutral, Op op) {
+#define RLK_REDUCE_STEP(CONTROL, ROWS) v = op(v, (uint32_t)__builtin_amdgcn_update_dpp((int)neutral, (int)v, CONTROL, ROWS, 0xf, false))
+  RLK_REDUCE_STEP(0x111, 0xf);  // row_shr 1, 2, 4, 8
+  RLK_REDUCE_STEP(0x112, 0xf);
+  RLK_REDUCE_STEP(0x114, 0xf);
+  RLK_REDUCE_STEP(0x118, 0xf);
+  RLK_REDUCE_STEP(0x142, 0xa);  // row_bcast 15: into rows 1 and 3
+  RLK_REDUCE_STEP(0x143, 0xc);  // row_bcast 31: into rows 2 and 3
+#undef RLK_REDUCE_STEP
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 __device__ __forceinline__ float wave_sum_f32(float v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v = v + __shfl_xor(v, offset);
-  return v;
+  return __uint_as_float(wave_reduce(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 __device__ __forceinline__ float wave_max_f32(float v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v = fmaxf(v, __shfl_xor(v, offset));
-  return v;
+  return __uint_as_float(wave_reduce(__float_as_uint(v), __float_as_uint(kNegInf), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
 }
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) { return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) { return wave_reduce(v, ~0u, [](uint32_t a, uint32_t b) { return a < b ? a : b; }); }
 
 // What one lane of a wave wrote to LDS is seen by the others behind it.
 __device__ __forceinline__ void wave_lds_sync() {
@@ -268,26 +293,76 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// The k largest of n different keys (k <= n <= kFinishKeys) move to the front of `keys`; returns the smallest of them.
-__device__ __forceinline__ uint64_t keep_largest(uint64_t* keys, int n, int k, int lane) {
-  constexpr int kEach = kFinishKeys / kWave;
-  uint64_t mine[kEach];
+// Bits at the end of an ordered logit that its type leaves the same in all logits of a sign: thresholds need not tell them apart.
+template <int ELEM>
+constexpr int kIdleBits = ELEM == RLK_DTYPE_BF16 ? 16 : ELEM == RLK_DTYPE_FP16 ? 13 : 0;
+
+// The largest threshold in [low, high] that at least k values reach, where `reach(low)` >= k: halvings, each a count over the wave.
+// Ends early at a threshold that at most `enough` reach.
+template <class Count>
+__device__ __forceinline__ uint32_t threshold_of(uint32_t low, uint32_t high, int k, int enough, int& reached, Count reach) {
+  while (reached > enough && low < high) {
+    const uint32_t mid = low + (high - low + 1) / 2;
+    const int count = reach(mid);
+    if (count >= k) {
+      low = mid;
+      reached = count;
+    } else {
+      high = mid - 1;
+    }
+  }
+  return low;
+}
+
+// The k largest of n different keys (k <= n <= kFinishKeys; their upper words in [low, high], their columns under V) move to the front
+// of `keys`; returns the smallest of them. First the k-th logit, then, among the keys that have it, the last column.
+template <int ELEM>
+__device__ __noinline__ uint64_t keep_largest(uint64_t* keys, int n, int k, int lane, uint32_t low, uint32_t high, int V) {
+  constexpr int EACH = kFinishKeys / kWave;
+  uint64_t mine[EACH];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) mine[i] = i * kWave + lane < n ? keys[i * kWave + lane] : 0;
-  uint64_t floor = 0;  // the largest number that k keys are not under
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t trial = floor | (uint64_t)1 << bit;
+  for (int i = 0; i < EACH; ++i) mine[i] = i * kWave + lane < n ? keys[i * kWave + lane] : 0;
+  constexpr int kIdle = kIdleBits<ELEM>;
+  int reached = n;
+  const uint32_t at = threshold_of(low >> kIdle, high >> kIdle, k, k, reached, [&](uint32_t t) __attribute__((always_inline)) {
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) count += __popcll(__ballot(mine[i] >= trial));
-    if (count >= k) floor = trial;
+    for (int i = 0; i < EACH; ++i) count += __popcll(__ballot((uint32_t)(mine[i] >> 32) >> kIdle >= t));
+    return count;
+  });
+  uint64_t floor = (uint64_t)at << kIdle << 32;
+  if (reached > k) {  // (the columns of the keys above `at` count in full)
+    const uint32_t last = threshold_of(0u, (uint32_t)V - 1, k, k, reached, [&](uint32_t t) __attribute__((always_inline)) {
+      int count = 0;
+      const uint32_t tail = ~((uint32_t)V - 1 - t);  // columns up to V - 1 - t
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const uint32_t upper = (uint32_t)(mine[i] >> 32) >> kIdle;
+        count += __popcll(__ballot(upper > at || (upper == at && (uint32_t)mine[i] >= tail)));
+      }
+      return count;
+    });
+    uint64_t smallest = ~(uint64_t)0;  // of the keys that are left: their upper words agree in what the type leaves idle
+    const uint32_t tail = ~((uint32_t)V - 1 - last);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const uint32_t upper = (uint32_t)(mine[i] >> 32) >> kIdle;
+      if (upper == at && (uint32_t)mine[i] >= tail && mine[i] < smallest) smallest = mine[i];
+    }
+#pragma unroll
+    for (int offset = 32; offset > 0; offset >>= 1) {
+      const uint64_t other = (uint64_t)__shfl_xor((long long)smallest, offset);
+      smallest = other < smallest ? other : smallest;
+    }
+    floor = smallest;
   }
   wave_lds_sync();
   int kept = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const uint64_t mask = __ballot(mine[i] >= floor);
-    if (mine[i] >= floor) keys[kept + lanes_below(mask)] = mine[i];
+  for (int i = 0; i < EACH; ++i) {
+    const bool keep = mine[i] != 0 && mine[i] >= floor;
+    const uint64_t mask = __ballot(keep);
+    if (keep) keys[kept + lanes_below(mask)] = mine[i];
     kept += __popcll(mask);
   }
   wave_lds_sync();
@@ -296,7 +371,7 @@ __device__ __forceinline__ uint64_t keep_largest(uint64_t* keys, int n, int k, i
 
 template <int ELEM>
 __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, int row, int lane, float lse, float inv_t,
-                                                    uint64_t* keys, uint16_t* picked) {
+                                                    uint64_t* keys, uint32_t* picked) {
   using E = typename LogitElem<ELEM>::type;
   const int k = a.top_k;
   constexpr int kEach = kScoreSlices / kWave;  // a lane has the sixteen slices of one tile
@@ -318,134 +393,140 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   uint32_t tile_most = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) tile_most = max(tile_most, most[i]);
-  uint32_t high = tile_most, low = tile_most;
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) {
-    high = max(high, (uint32_t)__shfl_xor((int)high, offset));
-    low = min(low, (uint32_t)__shfl_xor((int)low, offset));
-  }
-  high = __builtin_amdgcn_readfirstlane(high);
-  low = max(__builtin_amdgcn_readfirstlane(low), 1u);  // 0: a slice without columns
+  const uint32_t high = wave_max_u32(tile_most);
 
-  // Slices from a limit on that at least k of them reach and not many more (any such limit is as good as the k-th best).
-  const int enough = k + k / 8 + 2;
-  int reach = count_from(low);
-  uint32_t beyond = high + 1;  // (high is the key of a number, under 2^32 - 1)
-  while (reach > enough && beyond - low > 1) {
-    const uint32_t mid = low + (beyond - low) / 2;
-    const int count = count_from(mid);
-    if (count >= k) {
-      low = mid;
-      reach = count;
-    } else {
-      beyond = mid;
-    }
-  }
+  // Slices from a limit on that at least k of them reach and not many more (any such limit is as good as the k-th best): first the
+  // limit that k of the 64 tiles reach, where a step of the search is one comparison; of its slices there are few more unless k is
+  // near 64.
+  constexpr int kIdle = kIdleBits<ELEM>;
+  uint32_t low = max(wave_min_u32(tile_most), 1u);  // 0: a slice without columns
+  int reach = kScoreTiles;
+  low = max(threshold_of(low >> kIdle, high >> kIdle, k, k, reach, [&](uint32_t t) __attribute__((always_inline)) {
+              return (int)__popcll(__ballot(tile_most >> kIdle >= t));
+            }) << kIdle, 1u);
+  reach = count_from(low);
+  low = max(threshold_of(low >> kIdle, high >> kIdle, k, k + kWave / 2, reach, [&](uint32_t t) __attribute__((always_inline)) {
+              return count_from(t << kIdle);
+            }) << kIdle, 1u);
   uint64_t floor = (uint64_t)low << 32;  // candidates are not under it; key = (ordered logit, columns behind it)
-  uint32_t last_at = 0xffffffffu;
+
   uint32_t at[kEach];
+  const u32x4_t* where = reinterpret_cast<const u32x4_t*>(a.where + (int64_t)row * kScoreSlices + lane * kEach);
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) at[i] = 0;
-  if (reach > enough) {  // many slices with the same best logit: the first of them, by the vector that holds it
-    const u32x4_t* where = reinterpret_cast<const u32x4_t*>(a.best_at + (int64_t)row * kScoreSlices + lane * kEach);
+  for (int i = 0; i < kEach / 4; ++i) {
+    const u32x4_t v = where[i];
 #pragma unroll
-    for (int i = 0; i < kEach / 4; ++i) {
-      const u32x4_t v = where[i];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) at[4 * i + e] = v[e];
-    }
-    const int above = count_from(low + 1);
+    for (int e = 0; e < 4; ++e) at[4 * i + e] = v[e];
+  }
+  const int64_t tile_lo = (int64_t)lane * a.tile_size;  // a lane has the slices of one tile
+  const int my_g0 = (int)((tile_lo < a.real ? tile_lo : a.real) / 8);
+  uint32_t last_at = 0xffffffffu;
+  if (reach > kFinishPicked) {  // many slices with the same best logit: the first of them, by the vector that holds it
+    const uint32_t same = low >> kIdle;
+    const int above = count_from((same + 1) << kIdle);  // (the largest ordered logit, that of +inf, ends in 23 zeros)
     uint32_t first = 0, end = (uint32_t)(a.V / 8);  // the smallest vector number up to which there are enough
     while (first < end) {
       const uint32_t mid = first + (end - first) / 2;
       int count = above;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) count += __popcll(__ballot(most[i] == low && at[i] <= mid));
+      for (int i = 0; i < kEach; ++i)
+        count += __popcll(__ballot(most[i] >> kIdle == same && (uint32_t)my_g0 + i + (at[i] & 0xffffu) * kTileLanes <= mid));
       if (count >= k) end = mid; else first = mid + 1;
     }
     last_at = first;
     floor |= 0xffffffffu - min((uint64_t)0xffffffffu, (uint64_t)last_at * 8 + 7);
   }
-  int slices = 0;
+  // Of a picked slice its best vector is read, from the front of the list on, or all of it, from the back.
+  int singles = 0, wholes = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const bool take = most[i] > low || (most[i] == low && at[i] <= last_at);
+    const uint32_t g = (uint32_t)my_g0 + i + (at[i] & 0xffffu) * kTileLanes;
+    const bool take = most[i] >= low && (most[i] >> kIdle != low >> kIdle || g <= last_at);
     const uint64_t mask = __ballot(take);
-    if (take) picked[slices + lanes_below(mask)] = (uint16_t)(lane * kEach + i);
-    slices += __popcll(mask);
+    if (mask == 0) continue;
+    const bool whole = at[i] >> 16 >= low >> 16;  // another of its vectors may reach the limit
+    const uint64_t whole_mask = __ballot(take && whole);
+    if (take && !whole) picked[singles + lanes_below(mask & ~whole_mask)] = (uint32_t)(lane << 26) | g;
+    if (take && whole) picked[kFinishPicked - 1 - (wholes + lanes_below(whole_mask))] = (uint32_t)(lane * kEach + i);
+    singles += __popcll(mask & ~whole_mask);
+    wholes += __popcll(whole_mask);
   }
   wave_lds_sync();
 
-  // The picked slices' vectors, a lane each, some of a lane's on their way while as many are looked at. An element costs a comparison with
-  // the floor's logit, whose result is a mask over the lanes already; only masks that are not empty go on to the keys.
+  // The vectors, a lane each, some of a lane's on their way while as many are looked at. An element costs a comparison with the
+  // floor's logit; a lane's candidates of a vector are the bits of a mask, and the wave takes one of each lane at a time.
   const E* row_ptr = reinterpret_cast<const E*>(a.logits) + (int64_t)row * a.row_stride;
   const int rounds = ((a.tile_size + 14) / 8 + kTileLanes - 1) / kTileLanes;  // vectors of a slice, at most
-  const uint32_t jobs = (uint32_t)(slices * rounds);  // (rounds <= 2^28 / 64 / 128 + 1)
-  constexpr int kAhead = ELEM == RLK_DTYPE_FP32 ? 2 : 4;
-  struct Piece {
-    RowVector<ELEM> v;
-    int g, lo, hi;  // columns [lo, hi) of vector g
-  } now[kAhead], next[kAhead];
-  auto fetch = [&](uint32_t job, Piece& p) __attribute__((always_inline)) {
-    p.g = p.lo = p.hi = 0;
-    if (job < jobs) {
-      const int slice = picked[job / (uint32_t)rounds];
-      const int tile = slice / kTileLanes;
-      const int64_t lo64 = (int64_t)tile * a.tile_size, hi64 = lo64 + a.tile_size;
-      const int lo_col = lo64 < a.real ? (int)lo64 : a.real;
-      const int hi_col = hi64 < a.real ? (int)hi64 : a.real;
-      const int g = lo_col / 8 + slice % kTileLanes + (int)(job % (uint32_t)rounds) * kTileLanes;
-      if ((int64_t)g * 8 < hi_col) {
-        p.g = g;
-        p.lo = max(lo_col - g * 8, 0);
-        p.hi = min(hi_col - g * 8, 8);
-        p.v.template load_edge<false>(row_ptr, g, a.V);
-      }
-    }
-  };
+  const uint32_t jobs = (uint32_t)(singles + wholes * rounds);  // (rounds <= 2^28 / 64 / 128 + 1)
+  constexpr int kAhead = 4;
+  RowVector<ELEM> next[kAhead];
+  int next_first[kAhead];  // the window's first column, and which of its eight are the slice's, as bits
+  uint32_t next_of[kAhead];
   int n = 0;
   float least = low > ordered_bits(kNegInf) ? from_ordered_bits(low) : kNegInf;  // the floor's logit
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u) fetch(u * kWave + lane, next[u]);
-  for (uint32_t first = 0; first < jobs; first += kAhead * kWave) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) now[u] = next[u];
-    if (first + kAhead * kWave < jobs) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) fetch(first + (kAhead + u) * kWave + lane, next[u]);
-    }
+  for (uint32_t first = 0; first < jobs + kAhead * kWave; first += kAhead * kWave) {  // (the first turn only loads, the last only looks)
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (first + u * kWave >= jobs) break;
       float y[8];
-      uint64_t hit[8], any = 0;
-      now[u].v.unpack(y);
+      uint32_t mine = 0;
+      const int from = next_first[u];
+      if (first > 0) {
+        next[u].unpack(y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[i] = fmaxf(y[i], kNegInf);  // (a NaN counts as -inf)
-        hit[i] = __ballot(i >= now[u].lo && i < now[u].hi && y[i] >= least);
-        any |= hit[i];
+        for (int i = 0; i < 8; ++i) {
+          y[i] = fmaxf(y[i], kNegInf);  // (a NaN counts as -inf)
+          mine |= y[i] >= least ? 1u << i : 0u;
+        }
+        mine &= next_of[u];
       }
-      if (any == 0) continue;
-      if (n > kFinishKeys - 8 * kWave) {
-        floor = keep_largest(keys, n, k, lane);
-        least = from_ordered_bits((uint32_t)(floor >> 32));
-        n = k;
+      const uint32_t job = first + u * kWave + lane;
+      next_of[u] = 0;
+      next_first[u] = 0;
+      if (job < jobs) {
+        int tile, g;
+        if (job < (uint32_t)singles) {
+          tile = picked[job] >> 26;
+          g = picked[job] & 0x3ffffffu;
+        } else {
+          const uint32_t rest = job - singles, slice = picked[kFinishPicked - 1 - rest / (uint32_t)rounds];
+          tile = slice / kTileLanes;
+          const int64_t lo64 = (int64_t)tile * a.tile_size;
+          g = (int)((lo64 < a.real ? lo64 : a.real) / 8) + slice % kTileLanes + (rest % (uint32_t)rounds) * kTileLanes;
+        }
+        const int64_t lo64 = (int64_t)tile * a.tile_size, hi64 = lo64 + a.tile_size;
+        const int lo_col = lo64 < a.real ? (int)lo64 : a.real;
+        const int hi_col = hi64 < a.real ? (int)hi64 : a.real;
+        if ((int64_t)g * 8 < hi_col) {
+          const int at = window_of(g * 8, a.V);
+          const int lo = max(lo_col, g * 8) - at, hi = min(hi_col, g * 8 + 8) - at;
+          next_of[u] = (1u << hi) - (1u << lo);
+          next_first[u] = at;
+          next[u].template load_window<false>(row_ptr, at, a.V);
+        }
       }
+      while (__ballot(mine != 0) != 0) {
+        const int i = __builtin_ctz(mine | 256u);
+        float v = y[0];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (hit[i] == 0) continue;
-        const uint64_t key = (uint64_t)ordered_bits(y[i]) << 32 | (0xffffffffu - (uint32_t)(now[u].g * 8 + i));
-        const bool take = ((hit[i] >> lane) & 1) != 0 && key >= floor;
+        for (int e = 1; e < 8; ++e) v = i == e ? y[e] : v;
+        const uint64_t key = (uint64_t)ordered_bits(v) << 32 | (0xffffffffu - (uint32_t)(from + i));
+        const bool take = mine != 0 && key >= floor;
         const uint64_t mask = __ballot(take);
         if (take) keys[n + lanes_below(mask)] = key;
         n += __popcll(mask);
+        mine &= mine - 1;
+        if (n > kFinishKeys - kWave) {
+          wave_lds_sync();
+          floor = keep_largest<ELEM>(keys, n, k, lane, low, high, a.V);
+          least = from_ordered_bits((uint32_t)(floor >> 32));
+          n = k;
+        }
       }
     }
-    wave_lds_sync();
   }
+  wave_lds_sync();
   if (n > 2 * kWave) {
-    keep_largest(keys, n, k, lane);
+    keep_largest<ELEM>(keys, n, k, lane, low, high, a.V);
     n = k;
   }
 
@@ -477,7 +558,7 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
 template <int ELEM>
 __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(ScoreFinishArgs a) {
   __shared__ uint64_t keys[kFinishWaves][kFinishKeys];
-  __shared__ uint16_t picked[kFinishWaves][kFinishPicked];
+  __shared__ uint32_t picked[kFinishWaves][kFinishPicked];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x * kFinishWaves + wave;
@@ -488,7 +569,7 @@ __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(Scor
   const float shrink = pinned_exp(m - big);
   const float term = m > kNegInf ? s * shrink : 0.f;
   float sum = 0.f;  // (ascending)
-#pragma unroll
+#pragma unroll 8
   for (int t = 0; t < kScoreTiles; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
   const float weighted = wave_sum_f32(m > kNegInf ? shrink * __builtin_fmaf(s, m - big, w) : 0.f);
   const float log_sum = logf(sum);
@@ -630,16 +711,20 @@ size_t token_scores_workspace_bytes(int T, int top_k) {
   return (size_t)T * (kScorePlanes * kScoreTiles * sizeof(float) + (top_k > 0 ? 2 * kScoreSlices * sizeof(uint32_t) : 0));
 }
 
+template <int ELEM, bool HAS_TEMP, bool TOP>
+static void launch_score_tiles(const ScoreArgs& a, bool few, hipStream_t stream) {
+  const dim3 grid((unsigned)a.T, (unsigned)(kScoreTiles / a.tiles_per_group));
+  if (few) hipLaunchKernelGGL((score_few_rows_kernel<ELEM, HAS_TEMP, TOP>), grid, dim3(64), 0, stream, a);
+  else hipLaunchKernelGGL((score_tiles_kernel<ELEM, HAS_TEMP, TOP>), grid, dim3(256), 0, stream, a);
+}
+
 template <int ELEM>
-static hipError_t token_scores_typed(ScoreArgs a, const ScoreFinishArgs& f, dim3 grid, int threads, hipStream_t stream) {
-  const bool temp = a.temperature != nullptr;
-  if (f.top_k > 0) {
-    if (temp) hipLaunchKernelGGL((score_tiles_kernel<ELEM, true, true>), grid, dim3(threads), 0, stream, a);
-    else hipLaunchKernelGGL((score_tiles_kernel<ELEM, false, true>), grid, dim3(threads), 0, stream, a);
-  } else {
-    if (temp) hipLaunchKernelGGL((score_tiles_kernel<ELEM, true, false>), grid, dim3(threads), 0, stream, a);
-    else hipLaunchKernelGGL((score_tiles_kernel<ELEM, false, false>), grid, dim3(threads), 0, stream, a);
-  }
+static hipError_t token_scores_typed(const ScoreArgs& a, bool few, const ScoreFinishArgs& f, hipStream_t stream) {
+  const bool temp = a.temperature != nullptr, top = f.top_k > 0;
+  if (temp && top) launch_score_tiles<ELEM, true, true>(a, few, stream);
+  else if (top) launch_score_tiles<ELEM, false, true>(a, few, stream);
+  else if (temp) launch_score_tiles<ELEM, true, false>(a, few, stream);
+  else launch_score_tiles<ELEM, false, false>(a, few, stream);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   hipLaunchKernelGGL((score_finish_kernel<ELEM>), dim3((a.T + kFinishWaves - 1) / kFinishWaves), dim3(kFinishWaves * kWave), 0, stream, f);
@@ -656,23 +741,24 @@ hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride
   a.temperature = temperature;
   a.stats = reinterpret_cast<float*>(workspace);
   a.best = reinterpret_cast<uint32_t*>(a.stats + (size_t)T * kScorePlanes * kScoreTiles);
-  a.best_at = a.best + (size_t)T * kScoreSlices;
+  a.where = a.best + (size_t)T * kScoreSlices;
   a.T = T;
   a.V = V;
   a.real = real;
   a.tile_size = (int)(((int64_t)V + kScoreTiles - 1) / kScoreTiles);
-  a.tiles_per_group = kScoreTiles;
-  while ((int64_t)T * (kScoreTiles / a.tiles_per_group) < 16384 && a.tiles_per_group > 16) a.tiles_per_group /= 2;
+  // Few rows: a wave to a workgroup, four tiles each, so that a row has sixteen compute units.
+  const bool few = T <= 128;
+  a.tiles_per_group = few ? kTilesPerWave : kScoreTiles;
+  while (!few && (int64_t)T * (kScoreTiles / a.tiles_per_group) < 16384 && a.tiles_per_group > 16) a.tiles_per_group /= 2;
   const int groups = kScoreTiles / a.tiles_per_group;
   const int64_t bytes = (int64_t)T * V * (dtype == RLK_DTYPE_FP32 ? 4 : 2);
   a.streamed = bytes > kCachedLogitsBytes ? (int64_t)((double)T * groups * (1.0 - (double)kCachedLogitsBytes / bytes)) : 0;
-  const ScoreFinishArgs f{logits, row_stride, target, temperature, row_lse, a.stats, a.best, a.best_at, logp, lse, entropy,
+  const ScoreFinishArgs f{logits, row_stride, target, temperature, row_lse, a.stats, a.best, a.where, logp, lse, entropy,
                           top_logp, top_ids, T, V, real, a.tile_size, top_k};
-  const dim3 grid((unsigned)T, (unsigned)groups);
   switch (dtype) {
-    case RLK_DTYPE_BF16: return token_scores_typed<RLK_DTYPE_BF16>(a, f, grid, 256, stream);
-    case RLK_DTYPE_FP16: return token_scores_typed<RLK_DTYPE_FP16>(a, f, grid, 256, stream);
-    case RLK_DTYPE_FP32: return token_scores_typed<RLK_DTYPE_FP32>(a, f, grid, 256, stream);
+    case RLK_DTYPE_BF16: return token_scores_typed<RLK_DTYPE_BF16>(a, few, f, stream);
+    case RLK_DTYPE_FP16: return token_scores_typed<RLK_DTYPE_FP16>(a, few, f, stream);
+    case RLK_DTYPE_FP32: return token_scores_typed<RLK_DTYPE_FP32>(a, few, f, stream);
     default: return hipErrorInvalidValue;
   }
 }
