@@ -484,16 +484,15 @@ int rlk_logits_logp_backward(const void* logits, int dtype, int64_t row_stride, 
  *   ones from the lowest column on (a NaN ranks with -inf), and their log-probabilities.
  * temperature [T] may be NULL. A target outside [0, real_vocab) gives logp = NaN; a temperature that is not positive, a NaN or
  * +inf logit and a row without a logit above -inf give NaN throughout (lse is -inf for the latter). The bits of logp and lse are
- * those of rlk_logp_from_logits with 64 tiles where 64 divides V. row_lse: log-sum-exps of the rows that exist already (those of
- * rlk_linear_logp_fwd_logits); target, logp and lse may then be NULL, and top_logp is taken against it, at most 0.
+ * those of rlk_logp_from_logits with 64 tiles where 64 divides V.
  * top_k: 0 (top_logp and top_ids may be NULL) to RLK_SCORES_MAX_TOP_K. A row's results never depend on the other rows.
  */
 #define RLK_SCORES_MAX_TOP_K 64
 #define RLK_SCORES_MAX_VOCAB (1 << 28)
 size_t rlk_logits_scores_workspace_bytes(int T, int top_k);
-int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
-                      const float* row_lse, int T, int64_t V, int64_t real_vocab, int top_k, float* logp, float* lse,
-                      float* entropy, float* top_logp, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
+int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature, int T,
+                      int64_t V, int64_t real_vocab, int top_k, float* logp, float* lse, float* entropy, float* top_logp,
+                      int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * d(logits) of sum(g_logp logp + g_lse lse + g_entropy entropy) + sum(g_top top_logp), each gradient [T] (g_top [T, top_k]) or
@@ -505,6 +504,20 @@ int rlk_logits_scores_backward(const void* logits, int dtype, int64_t row_stride
                                const float* g_entropy, const int64_t* top_ids, const float* g_top, int top_k, void* grad,
                                int grad_dtype, int64_t grad_row_stride, int64_t grad_cols, int T, int64_t V, int64_t real_vocab,
                                void* stream);
+
+/*
+ * The same scores from hidden states [T, D] and the lm_head weight [V, D] (bf16): logp and lse are those of rlk_linear_logp_fwd, entropy and
+ * alternatives those of its fp32 logits. The logits go through `logits` (fp32 [T, logits_row_stride], as rlk_linear_logp_fwd_logits
+ * stores them; 16-byte aligned rows of whole 64 columns), which holds them afterwards; where rlk_linear_scores_needs_logits() is 0
+ * it may be NULL, and no logits are written. A token's results never depend on its batch, on top_k or on whether it has logits.
+ */
+size_t rlk_linear_scores_workspace_bytes(int T, int V, int top_k);
+int rlk_linear_scores_needs_logits(const void* hidden, int64_t h_row_stride, const void* weight, int64_t w_row_stride, int has_bias, int T,
+                                   int D, int V, int top_k);
+int rlk_linear_scores_fwd(const void* hidden, int64_t h_row_stride, const void* weight, int64_t w_row_stride, const int64_t* target,
+                          const float* bias, const float* temperature, float* logp, float* lse, float* entropy, float* top_logp,
+                          int64_t* top_ids, float* logits, int64_t logits_row_stride, void* workspace, size_t workspace_bytes, int T,
+                          int D, int V, int real_vocab_end, int top_k, void* stream);
 
 /*
  * The products at the end of a linear layer's backward over the vocabulary: grad_hidden[T, D] = dlogits weight and

@@ -45,6 +45,7 @@ struct LogpArgs {
   int vocab_limit;  // local column bound of the real vocabulary (<= V)
   int64_t vocab_start;
   int tiles_m, n_split, group_m;
+  bool entropy;  // the weighted sums in a fourth plane of `part`
 };
 
 // One (token tile, split). LOOP: 0 generic element loader, 1 register-staged 16-byte loads, 2 direct-to-LDS ping-pong.
@@ -177,10 +178,12 @@ __global__ __launch_bounds__(S::kThreads) void linear_logp_partial_kernel(LogpAr
 // that goes through many units, as in the GEMM, measures the same up to 10 rounds of them; behind 18 the workgroups that share
 // panels have drifted apart: 1 % slower. The two runs of a token folded side by side: 4 % slower.)
 // ST: the tile of a last row of token tiles that has at most ST::BM tokens left, a four-wave loop over 256 columns x ST::BM tokens.
-template <bool LOGITS, class S>
+// ENTROPY: the weighted sums too, a third state of each stream. It waits in scratch memory between the vocabulary tiles: 64 bytes a
+// lane and tile of 256 x 256 x D.
+template <bool LOGITS, bool ENTROPY, class S>
 __device__ __forceinline__ void logp_fold_tile(const LogpArgs& a, const f32x4_t (&acc)[S::TN][S::TM], int jm, int h, int span0, int col0,
                                                bool span_stores, int grp, int split, int m, int tgt, float inv_t, float& run_m,
-                                               float& run_s) {
+                                               float& run_s, float& run_w) {
   __builtin_amdgcn_sched_barrier(0);  // one run of 16 at a time: the accumulators and the next fragments leave few registers
   float y[16];
 #pragma unroll
@@ -199,7 +202,8 @@ __device__ __forceinline__ void logp_fold_tile(const LogpArgs& a, const f32x4_t 
   for (int c = 0; c < 16; ++c) y[c] = y[c] * inv_t;
   const int at = tgt - col0;
   float zt = 0.f;
-  logp_fold_run(y, at, run_m, run_s, zt);
+  if constexpr (ENTROPY) logp_fold_run_weighted(y, at, run_m, run_s, run_w, zt);
+  else logp_fold_run(y, at, run_m, run_s, zt);
   if (at >= 0 && at < 16) a.part[(2 * (int64_t)a.n_split + split) * a.T + m] = zt;  // (logp_store_units() writes the others' zeros)
   __builtin_amdgcn_sched_barrier(0);
 }
@@ -215,9 +219,9 @@ __device__ __forceinline__ float logp_inverse_temperature(const LogpArgs& a, int
 
 // The stream merge of `tokens` tokens whose states lie in LDS, streams `tokens` floats apart; token i of them is row m_of(i). A target
 // among the columns [v_first, v_end) of the unit has had its logit stored by the fold.
-template <class RowOf>
+template <bool ENTROPY, class RowOf>
 __device__ __forceinline__ void logp_store_units(const LogpArgs& a, int split, int v_first, int v_end, const float* xm, const float* xs,
-                                                 int tokens, RowOf m_of) {
+                                                 const float* xw, int tokens, RowOf m_of) {
   const int64_t plane = (int64_t)a.n_split * a.T;
   for (int i = threadIdx.x; i < tokens; i += SoloShape::kThreads) {
     const int m = m_of(i);
@@ -229,10 +233,20 @@ __device__ __forceinline__ void logp_store_units(const LogpArgs& a, int split, i
     a.part[plane + at] = sum;
     const int tgt = logp_target(a, m);
     if (tgt < v_first || tgt >= v_end) a.part[2 * plane + at] = 0.f;
+    if constexpr (ENTROPY) {  // the streams in pairs, in the order of an exchange between lanes
+      float w[kLogpStreams];
+#pragma unroll
+      for (int j = 0; j < kLogpStreams; ++j) w[j] = logp_weighted_term(xm[i + j * tokens], xs[i + j * tokens], xw[i + j * tokens], big);
+#pragma unroll
+      for (int step = 1; step < kLogpStreams; step *= 2)
+#pragma unroll
+        for (int j = 0; j < kLogpStreams; j += 2 * step) w[j] = w[j] + w[j + step];
+      a.part[3 * plane + at] = w[0];
+    }
   }
 }
 
-template <bool LOGITS, class S, int NS>
+template <bool LOGITS, bool ENTROPY, class S, int NS>
 __device__ __forceinline__ void logp_small_unit(const LogpArgs& a, int m0, int split, char* lds) {
   static_assert(S::WN == 2 && S::WM == 2 && S::TN == 8, "a lane holds two streams");
   const int lane = threadIdx.x & 63;
@@ -240,11 +254,12 @@ __device__ __forceinline__ void logp_small_unit(const LogpArgs& a, int m0, int s
   const int grp = lane >> 4;
   const int wave_n = wave % S::WN;
   const int tok_local = wave / S::WN * 16 * S::TM + (lane & 15);
-  float run_m[2][S::TM], run_s[2][S::TM];
+  float run_m[2][S::TM], run_s[2][S::TM], run_w[2][S::TM];
 #pragma unroll
   for (int jm = 0; jm < S::TM; ++jm) {
     run_m[0][jm] = run_m[1][jm] = kNegInf;
     run_s[0][jm] = run_s[1][jm] = 0.f;
+    run_w[0][jm] = run_w[1][jm] = 0.f;
   }
   for (int t = 0; t < kLogpSplitTiles; ++t) {
     const int v0 = split * kLogpSplitCols + t * kLogpTileCols;
@@ -257,12 +272,13 @@ __device__ __forceinline__ void logp_small_unit(const LogpArgs& a, int m0, int s
       const int m = m0 + tok_local + jm * 16;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        logp_fold_tile<LOGITS, S>(a, acc, jm, h, v0 + wave_n * 128 + 64, col + 16 * h, false, grp, split, m, logp_target(a, m),
-                                  logp_inverse_temperature(a, m), run_m[h][jm], run_s[h][jm]);
+        logp_fold_tile<LOGITS, ENTROPY, S>(a, acc, jm, h, v0 + wave_n * 128 + 64, col + 16 * h, false, grp, split, m, logp_target(a, m),
+                                  logp_inverse_temperature(a, m), run_m[h][jm], run_s[h][jm], run_w[h][jm]);
     }
   }
   float* const xm = reinterpret_cast<float*>(lds);  // the loop ended on a barrier
   float* const xs = xm + kLogpStreams * S::BM;
+  float* const xw = xs + kLogpStreams * S::BM;
 #pragma unroll
   for (int jm = 0; jm < S::TM; ++jm) {
     const int tok = tok_local + jm * 16;
@@ -270,11 +286,12 @@ __device__ __forceinline__ void logp_small_unit(const LogpArgs& a, int m0, int s
     for (int h = 0; h < 2; ++h) {
       xm[(wave_n * 8 + grp * 2 + h) * S::BM + tok] = run_m[h][jm];
       xs[(wave_n * 8 + grp * 2 + h) * S::BM + tok] = run_s[h][jm];
+      if constexpr (ENTROPY) xw[(wave_n * 8 + grp * 2 + h) * S::BM + tok] = run_w[h][jm];
     }
   }
   __syncthreads();
   const int v_first = split * kLogpSplitCols;
-  logp_store_units(a, split, v_first, v_first + kLogpSplitCols, xm, xs, S::BM, [&](int i) { return m0 + i; });
+  logp_store_units<ENTROPY>(a, split, v_first, v_first + kLogpSplitCols, xm, xs, xw, S::BM, [&](int i) { return m0 + i; });
   __syncthreads();
 }
 
@@ -282,7 +299,7 @@ struct LogpNoRest {
   static constexpr int BM = 0;
 };
 
-template <bool LOGITS, class ST>
+template <bool LOGITS, bool ENTROPY, class ST>
 __global__ __launch_bounds__(SoloShape::kThreads) void linear_logp_solo_kernel(LogpArgs a) {
   using S = SoloShape;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -291,7 +308,7 @@ __global__ __launch_bounds__(SoloShape::kThreads) void linear_logp_solo_kernel(L
   const int units = a.tiles_m * a.n_split;
   if constexpr (ST::BM > 0) {
     if ((int)blockIdx.x >= units) {
-      logp_small_unit<LOGITS, ST, kSoloLdsBytes / ST::kStageBytes>(a, a.tiles_m * S::BM, blockIdx.x - units, lds);
+      logp_small_unit<LOGITS, ENTROPY, ST, kSoloLdsBytes / ST::kStageBytes>(a, a.tiles_m * S::BM, blockIdx.x - units, lds);
       return;
     }
   }
@@ -305,18 +322,19 @@ __global__ __launch_bounds__(SoloShape::kThreads) void linear_logp_solo_kernel(L
   const int split = within / width;
   if constexpr (ST::BM > 0) {
     if (m0 + ST::BM >= a.T) {
-      logp_small_unit<LOGITS, ST, kSoloLdsBytes / ST::kStageBytes>(a, m0, split, lds);
+      logp_small_unit<LOGITS, ENTROPY, ST, kSoloLdsBytes / ST::kStageBytes>(a, m0, split, lds);
       return;
     }
   }
   const int v_first = split * kLogpSplitCols;
   const int tiles = min(kLogpSplitTiles, (a.V - v_first + kLogpTileCols - 1) / kLogpTileCols);
 
-  float run_m[2][S::TM], run_s[2][S::TM];
+  float run_m[2][S::TM], run_s[2][S::TM], run_w[2][S::TM];
 #pragma unroll
   for (int jm = 0; jm < S::TM; ++jm) {
     run_m[0][jm] = run_m[1][jm] = kNegInf;
     run_s[0][jm] = run_s[1][jm] = 0.f;
+    run_w[0][jm] = run_w[1][jm] = 0.f;
   }
   auto tile_at = [&](int t, int& v0, int& m) __attribute__((always_inline)) {
     v0 = v_first + t * kLogpTileCols;
@@ -338,14 +356,16 @@ __global__ __launch_bounds__(SoloShape::kThreads) void linear_logp_solo_kernel(L
     for (int jm = 0; jm < S::TM; ++jm)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        logp_fold_tile<LOGITS, S>(a, acc, jm, h, span + h * 64, span + h * 64 + grp * 16, span + h * 64 + 64 <= a.V, grp,
-                                  split, m0 + tok_local + jm * 16, tgt[jm], inv_t[jm], run_m[h][jm], run_s[h][jm]);
+        logp_fold_tile<LOGITS, ENTROPY, S>(a, acc, jm, h, span + h * 64, span + h * 64 + grp * 16, span + h * 64 + 64 <= a.V, grp,
+                                  split, m0 + tok_local + jm * 16, tgt[jm], inv_t[jm], run_m[h][jm], run_s[h][jm], run_w[h][jm]);
     if (t + 1 < tiles) return LOGITS && span + 128 <= a.V && m0 + S::BM <= a.T;
 
     // the 16 streams of the unit, 128 tokens at a time
     constexpr int kTokens = 128, kRows = S::TM / 2;
     float* const xm = reinterpret_cast<float*>(scratch);
     float* const xs = xm + kLogpStreams * kTokens;
+    float* const xw = xs + kLogpStreams * kTokens;
+    static_assert(3 * kLogpStreams * kTokens * 4 <= kSoloPartBytes, "the states of 128 tokens");
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
@@ -355,11 +375,12 @@ __global__ __launch_bounds__(SoloShape::kThreads) void linear_logp_solo_kernel(L
         for (int h = 0; h < 2; ++h) {
           xm[(wave_n * 8 + h * 4 + grp) * kTokens + tok] = run_m[h][jm];
           xs[(wave_n * 8 + h * 4 + grp) * kTokens + tok] = run_s[h][jm];
+          if constexpr (ENTROPY) xw[(wave_n * 8 + h * 4 + grp) * kTokens + tok] = run_w[h][jm];
         }
       }
       __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
       wg_barrier();
-      logp_store_units(a, split, v_first, v_first + kLogpSplitCols, xm, xs, kTokens, [&](int i) { return m0 + (i >> 6) * 128 + pass * 64 + (i & 63); });
+      logp_store_units<ENTROPY>(a, split, v_first, v_first + kLogpSplitCols, xm, xs, xw, kTokens, [&](int i) { return m0 + (i >> 6) * 128 + pass * 64 + (i & 63); });
       __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
       wg_barrier();
     }
@@ -741,9 +762,9 @@ static bool logp_rest_behind(int whole_tiles, int n_split, int cus) {
   return whole_tiles >= 8 || whole_tiles * n_split % cus * 4 >= 3 * cus;
 }
 
-template <class ST>
+template <class ST, bool ENTROPY = false>
 static hipError_t launch_logp_solo(LogpArgs a, hipStream_t stream) {
-  auto kernel = a.logits != nullptr ? linear_logp_solo_kernel<true, ST> : linear_logp_solo_kernel<false, ST>;
+  auto kernel = a.logits != nullptr ? linear_logp_solo_kernel<true, ENTROPY, ST> : linear_logp_solo_kernel<false, ENTROPY, ST>;
   static PerDeviceOnce once[2];
   hipError_t err = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kSoloLdsBytes, once[a.logits != nullptr]);
   if (err != hipSuccess) return err;
@@ -786,6 +807,11 @@ static bool logp_solo_pays(const LogpArgs& a) {
 // tokens 597 -> 529, 2100: 1046 -> 988; V = 18992, D = 4096 at 1100 tokens 302 -> 271.
 static hipError_t launch_logp_256(const LogpArgs& a, hipStream_t stream) {
   const int rest = a.T % LogpShape256::BM;
+  if (a.entropy) {  // (linear_logp_gives_entropy)
+    if (rest >= 1 && rest <= 64) return launch_logp_solo<TileShape<256, 64, 2, 2>, true>(a, stream);
+    if (rest >= 1 && rest <= 128) return launch_logp_solo<TileShape<256, 128, 2, 2>, true>(a, stream);
+    return launch_logp_solo<LogpNoRest, true>(a, stream);
+  }
   if (logp_solo_pays(a)) {
     if (rest >= 1 && rest <= 64) return launch_logp_solo<TileShape<256, 64, 2, 2>>(a, stream);
     if (rest >= 1 && rest <= 128) return launch_logp_solo<TileShape<256, 128, 2, 2>>(a, stream);
@@ -948,10 +974,14 @@ int pick_linear_logp_config(int T, int V) {
   return best_streams(T, linear_logp_split_count(V)).config;
 }
 
-hipError_t linear_logp_launch(const MatView& H, const MatView& W, const int64_t* target, const float* bias,
-                              const float* temperature, float* logp, float* lse, float* target_logit,
-                              float* logits, int64_t logits_ld, float* workspace, int T, int D, int V,
-                              int64_t vocab_start, int vocab_limit, int config, hipStream_t stream) {
+static bool logp_operands_vectorised(const LogpArgs& a) {
+  return a.W.k_stride == 1 && a.H.k_stride == 1 && (a.W.row_stride % kChunkElems) == 0 && (a.H.row_stride % kChunkElems) == 0 &&
+         (reinterpret_cast<uintptr_t>(a.W.ptr) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.H.ptr) & 15) == 0 &&
+         (a.D % kChunkElems) == 0 && pitch_fits_lane_offsets(a.W.row_stride) && pitch_fits_lane_offsets(a.H.row_stride);
+}
+
+static LogpArgs logp_args(const MatView& H, const MatView& W, const int64_t* target, const float* bias, const float* temperature,
+                          float* logits, int64_t logits_ld, float* workspace, int T, int D, int V, int64_t vocab_start, int vocab_limit) {
   LogpArgs a;
   a.logits = logits;
   a.logits_ld = logits_ld;
@@ -969,10 +999,27 @@ hipError_t linear_logp_launch(const MatView& H, const MatView& W, const int64_t*
   a.n_split = linear_logp_split_count(V);
   a.tiles_m = 0;
   a.group_m = 1;
-  const bool vec = W.k_stride == 1 && H.k_stride == 1 && (W.row_stride % kChunkElems) == 0 &&
-                   (H.row_stride % kChunkElems) == 0 && (reinterpret_cast<uintptr_t>(W.ptr) & 15) == 0 &&
-                   (reinterpret_cast<uintptr_t>(H.ptr) & 15) == 0 && (D % kChunkElems) == 0 &&
-                   pitch_fits_lane_offsets(W.row_stride) && pitch_fits_lane_offsets(H.row_stride);
+  a.entropy = false;
+  return a;
+}
+
+// Above the token counts of the stream groups one wave per SIMD has the weighted sums of the entropy in its fold (where it is not the
+// faster loop too: it saves the pass over the logits, 8 bytes each with their stores, that the entropy costs otherwise).
+bool linear_logp_gives_entropy(const MatView& H, const MatView& W, const float* bias, const float* logits, int64_t logits_ld, int T, int D,
+                               int V) {
+  const LogpArgs a = logp_args(H, W, nullptr, bias, nullptr, const_cast<float*>(logits), logits_ld, nullptr, T, D, V, 0, V);
+  const bool spans = logits == nullptr || ((logits_ld & 3) == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0);
+  return T > kStreamGroupMaxTokens && bias == nullptr && spans && D % kTileK == 0 && logp_operands_vectorised(a) && solo_offsets_fit(W) &&
+         solo_offsets_fit(H);
+}
+
+hipError_t linear_logp_launch(const MatView& H, const MatView& W, const int64_t* target, const float* bias,
+                              const float* temperature, float* logp, float* lse, float* target_logit,
+                              float* logits, int64_t logits_ld, float* workspace, int T, int D, int V,
+                              int64_t vocab_start, int vocab_limit, int config, hipStream_t stream, bool entropy) {
+  LogpArgs a = logp_args(H, W, target, bias, temperature, logits, logits_ld, workspace, T, D, V, vocab_start, vocab_limit);
+  a.entropy = entropy;
+  const bool vec = logp_operands_vectorised(a);
   const bool force_staged = (config & RLK_LOGP_CFG_FORCE_STAGED) != 0;
   config &= ~RLK_LOGP_CFG_FORCE_STAGED;
   const int requested = config;
@@ -985,6 +1032,7 @@ hipError_t linear_logp_launch(const MatView& H, const MatView& W, const int64_t*
     if (config == RLK_LOGP_CFG_192_STREAMS || config == RLK_LOGP_CFG_256_STREAMS) config = RLK_LOGP_CFG_256;
   }
   if (!vec && config == RLK_LOGP_CFG_256) config = RLK_LOGP_CFG_128;  // which has the element-wise loader
+  if (entropy && !(config == RLK_LOGP_CFG_256 && loop == 2)) return hipErrorInvalidValue;
   hipError_t err;
   const bool streams = config == RLK_LOGP_CFG_128_STREAMS || config == RLK_LOGP_CFG_192_STREAMS || config == RLK_LOGP_CFG_256_STREAMS;
   const int solo_tokens = requested == RLK_LOGP_CFG_AUTO && streams && streams_solo_fits(a) ? pick_streams_solo(a) : 0;

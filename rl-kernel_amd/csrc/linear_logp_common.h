@@ -120,6 +120,49 @@ __device__ __forceinline__ void logp_fold_run(const float (&y)[16], int tl, floa
   run_m = new_m;
 }
 
+// The same step with the weighted sum w = sum e(y - m) (y - m) beside (m, s), for the entropy of the distribution: seen from a larger
+// maximum n it is e(m - n) (w + s (m - n)). (m, s) have the bits of logp_fold_run(). A masked logit is -inf below the maximum:
+// kFarBelow, from where e() is zero, stands for it, as zero times infinity is no number.
+constexpr float kFarBelow = -256.f;
+__device__ __forceinline__ void logp_fold_run_weighted(const float (&y)[16], int tl, float& run_m, float& run_s, float& run_w,
+                                                       float& run_zt) {
+  float tmax = kNegInf;
+#pragma unroll
+  for (int c = 0; c < 16; ++c) tmax = fmaxf(tmax, y[c]);
+  if (tl >= 0 && tl < 16) {
+    float sel = y[0];
+#pragma unroll
+    for (int c = 1; c < 16; ++c) sel = (tl == c) ? y[c] : sel;
+    run_zt = sel;
+  }
+  const float old_m = run_m;
+  const float new_m = fmaxf(old_m, tmax);
+  float d = y[0] - new_m;
+  float e = pinned_exp(d);
+  float sum = e, weighted = e * fmaxf(d, kFarBelow);
+#pragma unroll
+  for (int c = 1; c < 16; ++c) {
+    d = y[c] - new_m;
+    e = pinned_exp(d);
+    sum = sum + e;
+    weighted = __builtin_fmaf(e, fmaxf(d, kFarBelow), weighted);
+  }
+  const float back = old_m - new_m;
+  const float shrink = pinned_exp(back);
+  const float scaled = run_s * shrink;
+  const float moved = __builtin_fmaf(shrink, __builtin_fmaf(run_s, fmaxf(back, kFarBelow), run_w), weighted);
+  const bool any = new_m > kNegInf;
+  run_s = any ? (scaled + sum) : run_s;
+  run_w = any ? moved : run_w;
+  run_m = new_m;
+}
+// A stream's share of its split's weighted sum, seen from the split's maximum.
+__device__ __forceinline__ float logp_weighted_term(float m, float s, float w, float big) {
+  const float back = m - big;
+  const float term = pinned_exp(back) * __builtin_fmaf(s, back, w);
+  return m > kNegInf ? term : 0.f;
+}
+
 // The 16 stream states of a (split, token), merged in ascending stream order. pm / ps / pz
 // point at stream 0; consecutive streams are `stride` floats apart.
 __device__ __forceinline__ void logp_merge_streams(const float* pm, const float* ps, const float* pz, int64_t stride,

@@ -315,7 +315,7 @@ static int linear_logp_fwd_checked(const char* who, const void* hidden, int64_t 
                                    const float* temperature, float* logp, float* lse, float* target_logit,
                                    void* workspace, size_t workspace_bytes, int T, int D, int V, int64_t vocab_start,
                                    int real_vocab_end, int config, void* stream, float* logits = nullptr,
-                                   int64_t logits_row_stride = 0) {
+                                   int64_t logits_row_stride = 0, bool entropy = false) {
   if (T < 0 || D <= 0 || V <= 0) {
     set_last_error("%s: bad sizes T=%d D=%d V=%d", who, T, D, V);
     return RLK_ERR_INVALID_ARGUMENT;
@@ -350,7 +350,7 @@ static int linear_logp_fwd_checked(const char* who, const void* hidden, int64_t 
   MatView W{reinterpret_cast<const bf16_bits*>(weight), w_row_stride, 1, V};
   hipError_t err = linear_logp_launch(H, W, target, bias, temperature, logp, lse, target_logit, logits,
                                       logits_row_stride, reinterpret_cast<float*>(workspace), T, D, V, vocab_start,
-                                      real_vocab_end, config, reinterpret_cast<hipStream_t>(stream));
+                                      real_vocab_end, config, reinterpret_cast<hipStream_t>(stream), entropy);
   return err == hipSuccess ? RLK_OK : device_error(who, err);
 }
 
@@ -616,13 +616,13 @@ static int check_score_args(const char* what, const void* logits, int dtype, int
 
 size_t rlk_logits_scores_workspace_bytes(int T, int top_k) { return T > 0 ? token_scores_workspace_bytes(T, top_k) : 0; }
 
-int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
-                      const float* row_lse, int T, int64_t V, int64_t real_vocab, int top_k, float* logp, float* lse,
-                      float* entropy, float* top_logp, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
+int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature, int T,
+                      int64_t V, int64_t real_vocab, int top_k, float* logp, float* lse, float* entropy, float* top_logp,
+                      int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_score_args("rlk_logits_scores", logits, dtype, row_stride, T, V, real_vocab, top_k);
   if (rc != RLK_OK) return rc;
   if (T == 0) return RLK_OK;
-  if (entropy == nullptr || (row_lse == nullptr && (target == nullptr || logp == nullptr || lse == nullptr)) ||
+  if (target == nullptr || logp == nullptr || lse == nullptr || entropy == nullptr ||
       (top_k > 0 && (top_logp == nullptr || top_ids == nullptr))) {
     set_last_error("rlk_logits_scores: null target or output");
     return RLK_ERR_INVALID_ARGUMENT;
@@ -632,8 +632,8 @@ int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const i
     set_last_error("rlk_logits_scores: 16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     return RLK_ERR_INVALID_ARGUMENT;
   }
-  hipError_t err = token_scores_launch(logits, dtype, row_stride, target, temperature, row_lse, T, (int)V, (int)real_vocab, top_k,
-                                       logp, lse, entropy, top_logp, top_ids, workspace, reinterpret_cast<hipStream_t>(stream));
+  hipError_t err = token_scores_launch(logits, dtype, row_stride, target, temperature, T, (int)V, (int)real_vocab, top_k, logp, lse,
+                                       entropy, top_logp, top_ids, workspace, reinterpret_cast<hipStream_t>(stream));
   return err == hipSuccess ? RLK_OK : device_error("rlk_logits_scores", err);
 }
 
@@ -658,6 +658,62 @@ int rlk_logits_scores_backward(const void* logits, int dtype, int64_t row_stride
                                                 top_ids, g_top, top_k, grad, grad_dtype, grad_row_stride, (int)grad_cols, T, (int)V,
                                                 (int)real_vocab, reinterpret_cast<hipStream_t>(stream));
   return err == hipSuccess ? RLK_OK : device_error("rlk_logits_scores_backward", err);
+}
+
+size_t rlk_linear_scores_workspace_bytes(int T, int V, int top_k) {
+  return T > 0 && V > 0 ? linear_logp_workspace_bytes(T, V) + linear_scores_extra_bytes(T, V, top_k) : 0;
+}
+
+int rlk_linear_scores_needs_logits(const void* hidden, int64_t h_row_stride, const void* weight, int64_t w_row_stride, int has_bias, int T,
+                                   int D, int V, int top_k) {
+  if (T <= 0 || D <= 0 || V <= 0 || top_k > 0 || has_bias) return 1;
+  const MatView H{reinterpret_cast<const bf16_bits*>(hidden), h_row_stride, 1, T};
+  const MatView W{reinterpret_cast<const bf16_bits*>(weight), w_row_stride, 1, V};
+  return linear_logp_gives_entropy(H, W, nullptr, nullptr, 0, T, D, V) ? 0 : 1;
+}
+
+int rlk_linear_scores_fwd(const void* hidden, int64_t h_row_stride, const void* weight, int64_t w_row_stride, const int64_t* target,
+                          const float* bias, const float* temperature, float* logp, float* lse, float* entropy, float* top_logp,
+                          int64_t* top_ids, float* logits, int64_t logits_row_stride, void* workspace, size_t workspace_bytes, int T,
+                          int D, int V, int real_vocab_end, int top_k, void* stream) {
+  const char* who = "rlk_linear_scores_fwd";
+  if (V > RLK_SCORES_MAX_VOCAB || top_k < 0 || top_k > RLK_SCORES_MAX_TOP_K || (T > 0 && top_k > real_vocab_end)) {
+    set_last_error("%s: V at most %d, top_k %d in [0, min(%d, real_vocab_end)]", who, RLK_SCORES_MAX_VOCAB, top_k, RLK_SCORES_MAX_TOP_K);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  bool entropy_in_fold = false;
+  const size_t base = T > 0 && V > 0 ? linear_logp_workspace_bytes(T, V) : 0;
+  if (T > 0 && D > 0 && V > 0) {
+    if (logp == nullptr || lse == nullptr || entropy == nullptr || (top_k > 0 && (top_logp == nullptr || top_ids == nullptr))) {
+      set_last_error("%s: null output", who);
+      return RLK_ERR_INVALID_ARGUMENT;
+    }
+    const MatView H{reinterpret_cast<const bf16_bits*>(hidden), h_row_stride, 1, T};
+    const MatView W{reinterpret_cast<const bf16_bits*>(weight), w_row_stride, 1, V};
+    entropy_in_fold = top_k == 0 && linear_logp_gives_entropy(H, W, bias, logits, logits_row_stride, T, D, V);
+    if (logits == nullptr && !entropy_in_fold) {
+      set_last_error("%s: this call needs logits (rlk_linear_scores_needs_logits)", who);
+      return RLK_ERR_INVALID_ARGUMENT;
+    }
+    if (logits != nullptr && ((reinterpret_cast<uintptr_t>(logits) & 15) != 0 || logits_row_stride % 4 != 0 || logits_row_stride < ((int64_t)V + 63) / 64 * 64)) {
+      set_last_error("%s: logits must be 16-byte aligned rows of at least %lld elements, a multiple of 4 apart", who, ((long long)V + 63) / 64 * 64);
+      return RLK_ERR_INVALID_ARGUMENT;
+    }
+    const size_t need = base + linear_scores_extra_bytes(T, V, top_k);
+    if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
+      set_last_error("%s: 16-byte aligned workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+      return RLK_ERR_INVALID_ARGUMENT;
+    }
+  }
+  // (the weighted sums lie right behind the three planes that the merge reads; above the stream groups' token counts nothing else does)
+  int rc = linear_logp_fwd_checked(who, hidden, h_row_stride, weight, w_row_stride, target, bias, temperature, logp, lse, nullptr, workspace,
+                                   workspace_bytes, T, D, V, 0, real_vocab_end, RLK_LOGP_CFG_AUTO, stream, logits, logits_row_stride,
+                                   entropy_in_fold);
+  if (rc != RLK_OK || T == 0) return rc;
+  hipError_t err = linear_scores_launch(logits, logits_row_stride, temperature, lse, reinterpret_cast<const float*>(workspace), entropy_in_fold,
+                                        T, V, real_vocab_end, linear_logp_split_count(V), top_k, entropy, top_logp, top_ids,
+                                        reinterpret_cast<char*>(workspace) + base, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error(who, err);
 }
 
 int64_t rlk_linear_dlogits_row_stride(int V) { return V > 0 ? linear_logp_dz_row_stride(V) : 0; }

@@ -164,7 +164,11 @@ size_t linear_logp_workspace_bytes(int T, int V);
 hipError_t linear_logp_launch(const MatView& H, const MatView& W, const int64_t* target, const float* bias,
                               const float* temperature, float* logp, float* lse, float* target_logit,
                               float* logits, int64_t logits_ld, float* workspace, int T, int D, int V,
-                              int64_t vocab_start, int vocab_limit, int config, hipStream_t stream);
+                              int64_t vocab_start, int vocab_limit, int config, hipStream_t stream, bool entropy = false);
+// Whether that launch, told to (`entropy`, configuration auto), leaves the weighted sums of the entropy in a fourth plane of partials
+// behind its three of [n_split][T].
+bool linear_logp_gives_entropy(const MatView& H, const MatView& W, const float* bias, const float* logits, int64_t logits_ld, int T, int D,
+                               int V);
 
 // Ascending merge of (max, sum, target logit) partials laid out [3][n_split][T] into
 // lse = M + log(S), logp = target - lse (clamped at 0 when `clamp`) and the merged target
@@ -211,11 +215,17 @@ hipError_t linear_logp_gradients_launch(const MatView& H, const MatView& W, cons
                                         void* grad_weight, int64_t gw_row_stride, int T, int D, int V, bool force_staged,
                                         hipStream_t stream);
 
-// Scores of given tokens from materialised logits (token_scores.hip); row_lse: log-sum-exps that exist, or null.
+// Scores of given tokens from materialised logits (token_scores.hip).
 size_t token_scores_workspace_bytes(int T, int top_k);
-hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
-                               const float* row_lse, int T, int V, int real, int top_k, float* logp, float* lse, float* entropy,
-                               float* top_logp, int64_t* top_ids, void* workspace, hipStream_t stream);
+hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature, int T,
+                               int V, int real, int top_k, float* logp, float* lse, float* entropy, float* top_logp, int64_t* top_ids,
+                               void* workspace, hipStream_t stream);
+// The scores of the fused linear-LogP from its partials [n_split][T] of maxima, sums and weighted sums; the latter from the fp32 logits
+// that it stored unless the launch left them (`have_weighted`, at the start of `extra`), as do the alternatives.
+size_t linear_scores_extra_bytes(int T, int V, int top_k);  // right behind the three planes of the linear-LogP
+hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const float* temperature, const float* lse, const float* part,
+                                bool have_weighted, int T, int V, int real, int n_split, int top_k, float* entropy, float* top_logp,
+                                int64_t* top_ids, void* extra, hipStream_t stream);
 // Their gradient, in the type of the logits or (fp32 logits) in bf16; columns [V, grad_cols) are written as zeros.
 hipError_t token_scores_backward_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target,
                                         const float* temperature, const float* lse, const float* entropy, const float* g_logp,

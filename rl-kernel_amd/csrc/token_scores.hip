@@ -25,7 +25,7 @@ namespace rlk {
 constexpr int kScoreTiles = 64;
 constexpr int kScoreSlices = kScoreTiles * kTileLanes;
 constexpr int kScorePlanes = 4;  // max, sum, target, weighted sum: stats[row][plane][tile]
-constexpr float kFarBelow = -256.f;  // e(x) is zero from here down
+
 
 struct ScoreArgs {
   const void* logits;
@@ -123,7 +123,7 @@ __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
   const int grp = lane / kTileLanes;
   const E* row_ptr = reinterpret_cast<const E*>(a.logits) + (int64_t)row * a.row_stride;
   const float inv_t = HAS_TEMP ? 1.0f / a.temperature[row] : 1.0f;
-  const int64_t wanted = a.target ? a.target[row] : -1;
+  const int64_t wanted = a.target[row];
   const int target = wanted >= 0 && wanted < a.real ? (int)wanted : -1;
 
   const int tile_first = blockIdx.y * a.tiles_per_group;
@@ -239,12 +239,13 @@ __global__ __launch_bounds__(64) void score_few_rows_kernel(ScoreArgs a) {
 // A wave per row: the tiles of the row merged, and its alternatives.
 // ---------------------------------------------------------------------------
 
+// LINEAR: from the partials and stored logits of the fused linear-LogP, see below.
 struct ScoreFinishArgs {
   const void* logits;
   int64_t row_stride;
   const int64_t* target;
   const float* temperature;
-  const float* row_lse;  // [T] or null: log-sum-exps that exist; logp and lse are then not written, no alternative is above 0
+  const float* row_lse;  // LINEAR: [T], the log-sum-exps
   const float* stats;
   const uint32_t* best;
   const uint32_t* where;
@@ -254,6 +255,9 @@ struct ScoreFinishArgs {
   float* top_logp;   // [T][top_k]
   int64_t* top_ids;  // [T][top_k]
   int T, V, real, tile_size, top_k;
+  const float* part;      // LINEAR: [n_split][T] maxima, then sums
+  const float* weighted;  // LINEAR: [n_split][T]
+  int n_split;
 };
 
 constexpr int kFinishWaves = 4;
@@ -369,7 +373,29 @@ __device__ __noinline__ uint64_t keep_largest(uint64_t* keys, int n, int k, int 
   return floor;
 }
 
-template <int ELEM>
+// The vector that is number `step` of a slice, and the columns of its tile. A slice of materialised logits is every sixteenth vector of
+// a tile; one of the fused linear-LogP is a stream of every 64th split: 16 columns of each of its four tiles.
+template <bool LINEAR>
+__device__ __forceinline__ int slice_vector(const ScoreFinishArgs& a, int tile, int l16, int step) {
+  if constexpr (LINEAR) {
+    return (tile + kScoreTiles * (step >> 3)) * (kLogpSplitCols / 8) + (step >> 1 & 3) * (kLogpTileCols / 8) + 2 * l16 + (step & 1);
+  } else {
+    const int64_t lo64 = (int64_t)tile * a.tile_size;
+    return (int)((lo64 < a.real ? lo64 : a.real) / 8) + l16 + step * kTileLanes;
+  }
+}
+template <bool LINEAR>
+__device__ __forceinline__ void tile_columns(const ScoreFinishArgs& a, int tile, int& lo_col, int& hi_col) {
+  lo_col = 0;
+  hi_col = a.real;
+  if constexpr (!LINEAR) {
+    const int64_t lo64 = (int64_t)tile * a.tile_size, hi64 = lo64 + a.tile_size;
+    lo_col = lo64 < a.real ? (int)lo64 : a.real;
+    hi_col = hi64 < a.real ? (int)hi64 : a.real;
+  }
+}
+
+template <int ELEM, bool LINEAR>
 __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, int row, int lane, float lse, float inv_t,
                                                     uint64_t* keys, uint32_t* picked) {
   using E = typename LogitElem<ELEM>::type;
@@ -418,8 +444,6 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
 #pragma unroll
     for (int e = 0; e < 4; ++e) at[4 * i + e] = v[e];
   }
-  const int64_t tile_lo = (int64_t)lane * a.tile_size;  // a lane has the slices of one tile
-  const int my_g0 = (int)((tile_lo < a.real ? tile_lo : a.real) / 8);
   uint32_t last_at = 0xffffffffu;
   if (reach > kFinishPicked) {  // many slices with the same best logit: the first of them, by the vector that holds it
     const uint32_t same = low >> kIdle;
@@ -430,7 +454,7 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
       int count = above;
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
-        count += __popcll(__ballot(most[i] >> kIdle == same && (uint32_t)my_g0 + i + (at[i] & 0xffffu) * kTileLanes <= mid));
+        count += __popcll(__ballot(most[i] >> kIdle == same && (uint32_t)slice_vector<LINEAR>(a, lane, i, at[i] & 0xffffu) <= mid));
       if (count >= k) end = mid; else first = mid + 1;
     }
     last_at = first;
@@ -440,7 +464,7 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   int singles = 0, wholes = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const uint32_t g = (uint32_t)my_g0 + i + (at[i] & 0xffffu) * kTileLanes;
+    const uint32_t g = (uint32_t)slice_vector<LINEAR>(a, lane, i, at[i] & 0xffffu);
     const bool take = most[i] >= low && (most[i] >> kIdle != low >> kIdle || g <= last_at);
     const uint64_t mask = __ballot(take);
     if (mask == 0) continue;
@@ -456,8 +480,9 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   // The vectors, a lane each, some of a lane's on their way while as many are looked at. An element costs a comparison with the
   // floor's logit; a lane's candidates of a vector are the bits of a mask, and the wave takes one of each lane at a time.
   const E* row_ptr = reinterpret_cast<const E*>(a.logits) + (int64_t)row * a.row_stride;
-  const int rounds = ((a.tile_size + 14) / 8 + kTileLanes - 1) / kTileLanes;  // vectors of a slice, at most
-  const uint32_t jobs = (uint32_t)(singles + wholes * rounds);  // (rounds <= 2^28 / 64 / 128 + 1)
+  // vectors of a slice, at most (2^28 / 64 / 128 + 1)
+  const int rounds = LINEAR ? (a.n_split + kScoreTiles - 1) / kScoreTiles * 8 : ((a.tile_size + 14) / 8 + kTileLanes - 1) / kTileLanes;
+  const uint32_t jobs = (uint32_t)(singles + wholes * rounds);
   constexpr int kAhead = 4;
   RowVector<ELEM> next[kAhead];
   int next_first[kAhead];  // the window's first column, and which of its eight are the slice's, as bits
@@ -490,12 +515,10 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
         } else {
           const uint32_t rest = job - singles, slice = picked[kFinishPicked - 1 - rest / (uint32_t)rounds];
           tile = slice / kTileLanes;
-          const int64_t lo64 = (int64_t)tile * a.tile_size;
-          g = (int)((lo64 < a.real ? lo64 : a.real) / 8) + slice % kTileLanes + (rest % (uint32_t)rounds) * kTileLanes;
+          g = slice_vector<LINEAR>(a, tile, slice % kTileLanes, rest % (uint32_t)rounds);
         }
-        const int64_t lo64 = (int64_t)tile * a.tile_size, hi64 = lo64 + a.tile_size;
-        const int lo_col = lo64 < a.real ? (int)lo64 : a.real;
-        const int hi_col = hi64 < a.real ? (int)hi64 : a.real;
+        int lo_col, hi_col;
+        tile_columns<LINEAR>(a, tile, lo_col, hi_col);
         if ((int64_t)g * 8 < hi_col) {
           const int at = window_of(g * 8, a.V);
           const int lo = max(lo_col, g * 8) - at, hi = min(hi_col, g * 8 + 8) - at;
@@ -548,14 +571,14 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   for (int i = 0; i < 2; ++i) {
     if (i * kWave + lane >= n || rank[i] >= k) continue;
     float v = from_ordered_bits((uint32_t)(mine[i] >> 32)) * inv_t - lse;
-    if (a.row_lse != nullptr && v > 0.f) v = 0.f;  // the fused linear-LogP clamps its log-probabilities
+    if (LINEAR && v > 0.f) v = 0.f;  // the fused linear-LogP clamps its log-probabilities
     const int64_t out = (int64_t)row * k + rank[i];
     a.top_ids[out] = (int64_t)(0xffffffffu - (uint32_t)mine[i]);
     a.top_logp[out] = v;
   }
 }
 
-template <int ELEM>
+template <int ELEM, bool LINEAR>
 __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(ScoreFinishArgs a) {
   __shared__ uint64_t keys[kFinishWaves][kFinishKeys];
   __shared__ uint32_t picked[kFinishWaves][kFinishPicked];
@@ -563,31 +586,138 @@ __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(Scor
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x * kFinishWaves + wave;
   if (row >= a.T) return;  // (waves share nothing)
-  const float* stats = a.stats + (int64_t)row * kScorePlanes * kScoreTiles + lane;
-  const float m = stats[0], s = stats[kScoreTiles], w = stats[3 * kScoreTiles];
-  const float big = wave_max_f32(m);
-  const float shrink = pinned_exp(m - big);
-  const float term = m > kNegInf ? s * shrink : 0.f;
-  float sum = 0.f;  // (ascending)
-#pragma unroll 8
-  for (int t = 0; t < kScoreTiles; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
-  const float weighted = wave_sum_f32(m > kNegInf ? shrink * __builtin_fmaf(s, m - big, w) : 0.f);
-  const float log_sum = logf(sum);
   const float temperature = a.temperature ? a.temperature[row] : 1.0f;
   const bool bad_temperature = !(temperature > 0.f);
   const float nan = __builtin_nanf("");
-  float lse = a.row_lse ? a.row_lse[row] : big + log_sum;
-  if (bad_temperature) lse = nan;
-  const float zt = wave_sum_f32(stats[2 * kScoreTiles]);
-  if (lane == 0) {
-    a.entropy[row] = bad_temperature ? nan : log_sum - weighted / sum;
-    if (a.row_lse == nullptr) {
+  float lse;
+  if constexpr (LINEAR) {  // a lane takes every 64th split, ascending
+    const int64_t plane = (int64_t)a.n_split * a.T;
+    float m = kNegInf, s = 0.f, w = 0.f;
+    for (int p = lane; p < a.n_split; p += kWave) m = fmaxf(m, a.part[(int64_t)p * a.T + row]);
+    const float big = wave_max_f32(m);
+    for (int p = lane; p < a.n_split; p += kWave) {
+      const int64_t at = (int64_t)p * a.T + row;
+      const float pm = a.part[at], ps = a.part[plane + at];
+      if (pm > kNegInf) {
+        s = __builtin_fmaf(ps, pinned_exp(pm - big), s);
+        w = w + logp_weighted_term(pm, ps, a.weighted[at], big);
+      }
+    }
+    const float sum = wave_sum_f32(s), weighted = wave_sum_f32(w);
+    lse = a.row_lse[row];
+    if (lane == 0) a.entropy[row] = bad_temperature ? nan : logf(sum) - weighted / sum;
+  } else {
+    const float* stats = a.stats + (int64_t)row * kScorePlanes * kScoreTiles + lane;
+    const float m = stats[0], s = stats[kScoreTiles], w = stats[3 * kScoreTiles];
+    const float big = wave_max_f32(m);
+    const float shrink = pinned_exp(m - big);
+    const float term = m > kNegInf ? s * shrink : 0.f;
+    float sum = 0.f;  // (ascending)
+#pragma unroll 8
+    for (int t = 0; t < kScoreTiles; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
+    const float weighted = wave_sum_f32(m > kNegInf ? shrink * __builtin_fmaf(s, m - big, w) : 0.f);
+    const float log_sum = logf(sum);
+    lse = bad_temperature ? nan : big + log_sum;
+    const float zt = wave_sum_f32(stats[2 * kScoreTiles]);
+    if (lane == 0) {
       const bool bad_target = a.target[row] < 0 || a.target[row] >= a.real;
+      a.entropy[row] = bad_temperature ? nan : log_sum - weighted / sum;
       a.lse[row] = lse;
       a.logp[row] = bad_target ? nan : zt - lse;
     }
   }
-  if (a.top_k > 0) finish_alternatives<ELEM>(a, row, lane, lse, a.temperature ? 1.0f / temperature : 1.0f, keys[wave], picked[wave]);
+  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, lse, a.temperature ? 1.0f / temperature : 1.0f, keys[wave], picked[wave]);
+}
+
+// ---------------------------------------------------------------------------
+// The scores of the fused linear-LogP. Its partials have the maxima and sums of the splits; the weighted sums follow its reduction
+// contract: a chain per stream of a split, tile by tile (logp_fold_run_weighted), the streams of a split in pairs, from their
+// maximum. The four-wave kernel above 1024 tokens has them in its fold. Where it does not run, or alternatives are asked for, they
+// come from the logits that the launch stored, by the kernel below: the same steps on the same values, so the same bits for a token
+// whatever batch it arrives in. A lane has one stream, sixteen of them a split, and goes through every 64th split: these are the
+// slices of the alternatives.
+// ---------------------------------------------------------------------------
+
+struct LinearRowArgs {
+  const float* logits;  // [T, logits_ld], rows of whole 64-column spans, 16-byte aligned
+  int64_t logits_ld;
+  const float* temperature;  // or null
+  float* weighted;           // [n_split][T]
+  uint32_t* best;            // as in ScoreArgs
+  uint32_t* where;
+  int T, V, real, n_split, classes_per_group;
+};
+
+template <bool HAS_TEMP, bool TOP>
+__global__ __launch_bounds__(256) void linear_score_rows_kernel(LinearRowArgs a) {
+  const int row = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = blockDim.x >> 6;
+  const int l16 = lane & (kTileLanes - 1);
+  const float* row_ptr = a.logits + (int64_t)row * a.logits_ld;
+  const float inv_t = HAS_TEMP ? 1.0f / a.temperature[row] : 1.0f;
+  const int first_class = blockIdx.y * a.classes_per_group;
+  for (int c0 = first_class + wave * kTilesPerWave; c0 < first_class + a.classes_per_group; c0 += waves * kTilesPerWave) {
+    const int mine = c0 + lane / kTileLanes;  // this lane's class of splits
+    float best = kNegInf, other = kNegInf;
+    int at = 0;
+    for (int base = 0; base + c0 < a.n_split; base += kScoreTiles) {  // uniform
+      const int split = base + mine;
+      const int col0 = split * kLogpSplitCols + l16 * 16;
+      f32x4_t raw[kLogpSplitTiles][4];
+#pragma unroll
+      for (int t = 0; t < kLogpSplitTiles; ++t) {
+        const int col = col0 + t * kLogpTileCols;
+        if (split < a.n_split && col < a.V) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) raw[t][q] = *reinterpret_cast<const f32x4_t*>(row_ptr + col + 4 * q);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) raw[t][q] = f32x4_t{kNegInf, kNegInf, kNegInf, kNegInf};
+        }
+      }
+      float m = kNegInf, s = 0.f, w = 0.f, unused = 0.f;
+#pragma unroll
+      for (int t = 0; t < kLogpSplitTiles; ++t) {
+        const int col = col0 + t * kLogpTileCols;
+        float y[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) y[c] = col + c < a.real ? raw[t][c / 4][c % 4] : kNegInf;
+        if constexpr (TOP) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* v = y + 8 * h;
+            const float here = max3_f32(max3_f32(max3_f32(max3_f32(v[0], v[1], v[2]), v[3], v[4]), v[5], v[6]), v[7], v[7]);
+            at = here > best ? base / kScoreTiles * 8 + 2 * t + h : at;
+            other = __builtin_amdgcn_fmed3f(here, best, other);
+            best = fmaxf(best, here);
+          }
+        }
+        if constexpr (HAS_TEMP) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) y[c] = y[c] * inv_t;
+        }
+        logp_fold_run_weighted(y, -1, m, s, w, unused);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      float big = fmaxf(m, xor_lane<1>(m));
+      big = fmaxf(big, xor_lane<2>(big));
+      big = fmaxf(big, xor_lane<4>(big));
+      big = fmaxf(big, xor_lane<8>(big));
+      float sum = logp_weighted_term(m, s, w, big);
+      sum = sum + xor_lane<1>(sum);
+      sum = sum + xor_lane<2>(sum);
+      sum = sum + xor_lane<4>(sum);
+      sum = sum + xor_lane<8>(sum);
+      if (l16 == 0 && split < a.n_split) a.weighted[(int64_t)split * a.T + row] = sum;
+    }
+    if constexpr (TOP) {
+      const int64_t slice = (int64_t)row * kScoreSlices + mine * kTileLanes + l16;
+      a.best[slice] = mine * kLogpSplitCols + l16 * 16 < a.real ? ordered_bits(best) : 0u;
+      a.where[slice] = (ordered_bits(other) & 0xffff0000u) | (uint32_t)at;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -727,12 +857,11 @@ static hipError_t token_scores_typed(const ScoreArgs& a, bool few, const ScoreFi
   else launch_score_tiles<ELEM, false, false>(a, few, stream);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL((score_finish_kernel<ELEM>), dim3((a.T + kFinishWaves - 1) / kFinishWaves), dim3(kFinishWaves * kWave), 0, stream, f);
+  hipLaunchKernelGGL((score_finish_kernel<ELEM, false>), dim3((a.T + kFinishWaves - 1) / kFinishWaves), dim3(kFinishWaves * kWave), 0, stream, f);
   return hipGetLastError();
 }
 
-hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
-                               const float* row_lse, int T, int V, int real, int top_k, float* logp, float* lse, float* entropy,
+hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature, int T, int V, int real, int top_k, float* logp, float* lse, float* entropy,
                                float* top_logp, int64_t* top_ids, void* workspace, hipStream_t stream) {
   ScoreArgs a;
   a.logits = logits;
@@ -753,14 +882,44 @@ hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride
   const int groups = kScoreTiles / a.tiles_per_group;
   const int64_t bytes = (int64_t)T * V * (dtype == RLK_DTYPE_FP32 ? 4 : 2);
   a.streamed = bytes > kCachedLogitsBytes ? (int64_t)((double)T * groups * (1.0 - (double)kCachedLogitsBytes / bytes)) : 0;
-  const ScoreFinishArgs f{logits, row_stride, target, temperature, row_lse, a.stats, a.best, a.where, logp, lse, entropy,
-                          top_logp, top_ids, T, V, real, a.tile_size, top_k};
+  const ScoreFinishArgs f{logits, row_stride, target, temperature, nullptr, a.stats, a.best, a.where, logp, lse, entropy,
+                          top_logp, top_ids, T, V, real, a.tile_size, top_k, nullptr, nullptr, 0};
   switch (dtype) {
     case RLK_DTYPE_BF16: return token_scores_typed<RLK_DTYPE_BF16>(a, few, f, stream);
     case RLK_DTYPE_FP16: return token_scores_typed<RLK_DTYPE_FP16>(a, few, f, stream);
     case RLK_DTYPE_FP32: return token_scores_typed<RLK_DTYPE_FP32>(a, few, f, stream);
     default: return hipErrorInvalidValue;
   }
+}
+
+size_t linear_scores_extra_bytes(int T, int V, int top_k) {
+  const size_t weighted = (size_t)linear_logp_split_count(V) * T * sizeof(float);
+  return weighted + 16 + (top_k > 0 ? (size_t)T * 2 * kScoreSlices * sizeof(uint32_t) : 0);
+}
+
+hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const float* temperature, const float* lse, const float* part,
+                                bool have_weighted, int T, int V, int real, int n_split, int top_k, float* entropy, float* top_logp,
+                                int64_t* top_ids, void* extra, hipStream_t stream) {
+  float* weighted = reinterpret_cast<float*>(extra);
+  uint32_t* best = reinterpret_cast<uint32_t*>((reinterpret_cast<uintptr_t>(weighted + (size_t)n_split * T) + 15) / 16 * 16);
+  uint32_t* where = best + (size_t)T * kScoreSlices;
+  if (!have_weighted || top_k > 0) {
+    const bool few = T <= 128;
+    LinearRowArgs a{logits, logits_ld, temperature, weighted, best, where, T, V, real, n_split, few ? kTilesPerWave : kScoreTiles};
+    while (!few && (int64_t)T * (kScoreTiles / a.classes_per_group) < 16384 && a.classes_per_group > 16) a.classes_per_group /= 2;
+    const dim3 grid((unsigned)T, (unsigned)(kScoreTiles / a.classes_per_group)), block(few ? 64 : 256);
+    if (temperature && top_k > 0) hipLaunchKernelGGL((linear_score_rows_kernel<true, true>), grid, block, 0, stream, a);
+    else if (temperature) hipLaunchKernelGGL((linear_score_rows_kernel<true, false>), grid, block, 0, stream, a);
+    else if (top_k > 0) hipLaunchKernelGGL((linear_score_rows_kernel<false, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((linear_score_rows_kernel<false, false>), grid, block, 0, stream, a);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  const ScoreFinishArgs f{logits, logits_ld, nullptr, temperature, lse, nullptr, best, where, nullptr, nullptr, entropy,
+                          top_logp, top_ids, T, V, real, 0, top_k, part, weighted, n_split};
+  hipLaunchKernelGGL((score_finish_kernel<RLK_DTYPE_FP32, true>), dim3((T + kFinishWaves - 1) / kFinishWaves), dim3(kFinishWaves * kWave), 0,
+                     stream, f);
+  return hipGetLastError();
 }
 
 template <int ELEM, int OUT>

@@ -428,7 +428,7 @@ variable_list scores(const ScoreInputs& in) {
   const size_t bytes = scores_workspace_entry((int)rows, in.top_k);
   const Tensor workspace = empty({(int64_t)bytes}, at::kByte, in.logits);
   check_status(scores_entry(in.logits.data_ptr(), dtype_code(in.logits), vocab, static_cast<const int64_t*>(in.target.data_ptr()),
-                            floats(in.temp), nullptr, (int)rows, vocab, in.real, in.top_k, writable(out[0]), writable(out[1]),
+                            floats(in.temp), (int)rows, vocab, in.real, in.top_k, writable(out[0]), writable(out[1]),
                             writable(out[2]), in.top_k > 0 ? writable(out[3]) : nullptr,
                             in.top_k > 0 ? static_cast<int64_t*>(out[4].data_ptr()) : nullptr, workspace.data_ptr(), bytes,
                             stream_of(in.logits)),

@@ -877,46 +877,83 @@ def hip_deterministic_logp_backward(
 
 
 def logits_scores(
-    logits: torch.Tensor,
-    target: Optional[torch.Tensor],
-    real_vocab: int,
-    top_k: int = 0,
-    *,
-    temperature: Optional[torch.Tensor] = None,
-    row_lse: Optional[torch.Tensor] = None,
-) -> List[Optional[torch.Tensor]]:
+    logits: torch.Tensor, target: torch.Tensor, real_vocab: int, top_k: int = 0, *, temperature: Optional[torch.Tensor] = None,
+) -> List[Optional[torch.Tensor]]:  # fmt: skip
     """``[logp, lse, entropy, top_logp, top_ids]`` of materialised logits ``[rows, V]`` (bf16 / fp16 / fp32, any row stride).
 
-    fp32 ``[rows]``, ``[rows, top_k]`` for the alternatives (``None`` without them), int64 ids. ``row_lse``: log-sum-exps that
-    exist already; ``logp`` and ``lse`` are then ``None`` and ``target`` is not looked at. ``temperature``: fp32, one per row."""
+    fp32 ``[rows]``, ``[rows, top_k]`` for the alternatives (``None`` without them), int64 ids. ``target``: int64, ``temperature``:
+    fp32, one per row."""
     code = _logits_dtype_code(logits)
     src = _row_contiguous(logits)
     rows, vocab = src.shape
-    device = src.device
-    for name, t, dtype in (("target", target, torch.int64), ("temperature", temperature, torch.float32), ("row_lse", row_lse, torch.float32)):
-        if t is not None and (t.device != device or t.dtype != dtype or t.numel() != rows or not t.is_contiguous()):
-            raise RuntimeError(f"logits_scores: {name} must be a contiguous {dtype} tensor beside the logits, one value per row")
-    if target is None and row_lse is None:
-        raise RuntimeError("logits_scores: target is required without row_lse")
-    logp = lse = top_logp = top_ids = None
-    if row_lse is None:
-        logp = torch.empty((rows,), dtype=torch.float32, device=device)
-        lse = torch.empty((rows,), dtype=torch.float32, device=device)
-    entropy = torch.empty((rows,), dtype=torch.float32, device=device)
-    if top_k:
-        top_logp = torch.empty((rows, top_k), dtype=torch.float32, device=device)
-        top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=device)
+    _check_per_row("logits_scores", src, target, temperature)
+    logp, lse, entropy, top_logp, top_ids = _score_outputs(rows, top_k, src.device)
     lib = _lib.load()
     ws_bytes = int(lib.rlk_logits_scores_workspace_bytes(rows, top_k))
-    workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=device)
-    with _on(device):
+    workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=src.device)
+    with _on(src.device):
         status = lib.rlk_logits_scores(
-            src.data_ptr(), code, _row_stride(src), _ptr(target), _ptr(temperature), _ptr(row_lse), rows, vocab, real_vocab, top_k,
-            _ptr(logp), _ptr(lse), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids), workspace.data_ptr(), ws_bytes,
-            _stream_handle(device),
+            src.data_ptr(), code, _row_stride(src), target.data_ptr(), _ptr(temperature), rows, vocab, real_vocab, top_k,
+            logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids), workspace.data_ptr(), ws_bytes,
+            _stream_handle(src.device),
         )  # fmt: skip
     _lib.check(status, "rlk_logits_scores failed")
     return [logp, lse, entropy, top_logp, top_ids]
+
+
+def _check_per_row(who: str, rows: torch.Tensor, target: torch.Tensor, temperature: Optional[torch.Tensor]) -> None:
+    for name, t, dtype in (("target", target, torch.int64), ("temperature", temperature, torch.float32)):
+        if name == "temperature" and t is None:
+            continue
+        if t.device != rows.device or t.dtype != dtype or t.numel() != rows.size(0) or not t.is_contiguous():
+            raise RuntimeError(f"{who}: {name} must be a contiguous {dtype} tensor beside the rows, one value per row")
+
+
+def _score_outputs(rows: int, top_k: int, device: torch.device) -> list:
+    three = [torch.empty((rows,), dtype=torch.float32, device=device) for _ in range(3)]
+    if not top_k:
+        return [*three, None, None]
+    return [*three, torch.empty((rows, top_k), dtype=torch.float32, device=device), torch.empty((rows, top_k), dtype=torch.int64, device=device)]
+
+
+def linear_scores_needs_logits(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], top_k: int) -> bool:
+    """Whether :func:`linear_scores` needs a buffer for the logits (contiguous ``hidden [T, D]`` and ``weight [V, D]``)."""
+    (n, d), v = hidden.shape, weight.size(0)
+    return bool(_lib.load().rlk_linear_scores_needs_logits(hidden.data_ptr(), d, weight.data_ptr(), d, bias is not None, n, d, v, top_k))
+
+
+def linear_scores(
+    hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor], temperature: Optional[torch.Tensor],
+    real_vocab: int, top_k: int, logits: Optional[torch.Tensor],
+) -> List[Optional[torch.Tensor]]:  # fmt: skip
+    """``[logp, lse, entropy, top_logp, top_ids]`` of contiguous bf16 ``hidden [T, D]`` through ``weight [V, D]``. ``logits``: fp32
+    ``[T, linear_logp_logits_row_stride(V)]``, where the logits go and stay; ``None`` where :func:`linear_scores_needs_logits` is false."""
+    n, d = hidden.shape
+    v = weight.size(0)
+    for name, t, shape in (("hidden", hidden, (n, d)), ("weight", weight, (v, d))):
+        if t.dtype != _BF16 or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda or t.device != hidden.device:
+            raise RuntimeError(f"linear_scores: {name} must be a contiguous bf16 {list(shape)} CUDA tensor beside hidden")
+    _check_per_row("linear_scores", hidden, target, temperature)
+    if bias is not None:
+        if bias.numel() != v:
+            raise RuntimeError("linear_scores: bias must have V elements")
+        bias = bias.to(device=hidden.device, dtype=torch.float32).contiguous()
+    if logits is not None:
+        _check_kept_logits("linear_scores", logits, hidden, v)
+    outputs = _score_outputs(n, top_k, hidden.device)
+    lib = _lib.load()
+    ws_bytes = int(lib.rlk_linear_scores_workspace_bytes(n, v, top_k))
+    workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=hidden.device)
+    if n == 0:
+        return outputs
+    with _on(hidden.device):
+        status = lib.rlk_linear_scores_fwd(
+            hidden.data_ptr(), d, weight.data_ptr(), d, target.data_ptr(), _ptr(bias), _ptr(temperature), *(_ptr(t) for t in outputs),
+            _ptr(logits), 0 if logits is None else logits.size(1), workspace.data_ptr(), ws_bytes, n, d, v, real_vocab, top_k,
+            _stream_handle(hidden.device),
+        )  # fmt: skip
+    _lib.check(status, "rlk_linear_scores_fwd failed")
+    return outputs
 
 
 def logits_scores_backward(

@@ -105,6 +105,9 @@ EXPORTED_SYMBOLS = (
     "rlk_logits_scores_workspace_bytes",
     "rlk_logits_scores",
     "rlk_logits_scores_backward",
+    "rlk_linear_scores_workspace_bytes",
+    "rlk_linear_scores_needs_logits",
+    "rlk_linear_scores_fwd",
     "rlk_linear_dlogits_row_stride",
     "rlk_linear_dlogits_bwd",
     "rlk_block_norm_forward",
@@ -237,10 +240,18 @@ def load() -> ctypes.CDLL:
     lib.rlk_logits_scores_workspace_bytes.restype = sz
     lib.rlk_logits_scores_workspace_bytes.argtypes = [i32, i32]
     lib.rlk_logits_scores.restype = i32
-    lib.rlk_logits_scores.argtypes = [vp, i32, i64, vp, vp, vp, i32, i64, i64, i32, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.rlk_logits_scores.argtypes = [vp, i32, i64, vp, vp, i32, i64, i64, i32, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.rlk_logits_scores_backward.restype = i32
     lib.rlk_logits_scores_backward.argtypes = [
         vp, i32, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, i32, i64, i64, i32, i64, i64, vp,
+    ]  # fmt: skip
+    lib.rlk_linear_scores_workspace_bytes.restype = sz
+    lib.rlk_linear_scores_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.rlk_linear_scores_needs_logits.restype = i32
+    lib.rlk_linear_scores_needs_logits.argtypes = [vp, i64, vp, i64, i32, i32, i32, i32, i32]
+    lib.rlk_linear_scores_fwd.restype = i32
+    lib.rlk_linear_scores_fwd.argtypes = [
+        vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp, sz, i32, i32, i32, i32, i32, vp,
     ]  # fmt: skip
     lib.rlk_linear_dlogits_row_stride.restype = i64
     lib.rlk_linear_dlogits_row_stride.argtypes = [i32]

@@ -178,26 +178,26 @@ def _rows(t: Optional[torch.Tensor], first: int, end: int) -> Optional[torch.Ten
 
 
 def _linear_scores(hidden, weight, bias, target, temp, real, top_k, kept):
-    """The answers, through ``kept`` (all logits, left in it) or through a buffer of some rows' logits."""
+    """The answers, through ``kept`` (all logits, left in it), through a buffer of some rows' logits, or through none."""
     tokens, vocab = hidden.size(0), weight.size(0)
-    parts = []
-    chunks = [(0, tokens)] if kept is not None or tokens == 0 else _token_chunks(tokens, vocab)
-    logits = kept if kept is not None else _buffer(chunks[0][1], vocab, hidden.device)
-    for first, end in chunks:
-        some = logits[: end - first]
-        rows_temp = _rows(temp, first, end)
-        logp, lse = _C.fused_linear_logp_into(hidden[first:end], weight, target[first:end], bias, rows_temp, real, some)
-        _, _, entropy, top_logp, top_ids = _C.logits_scores(some[:, :vocab], None, real, top_k, temperature=rows_temp, row_lse=lse)
-        parts.append((logp, lse, entropy, top_logp, top_ids))
+    if kept is not None or tokens == 0 or not _C.linear_scores_needs_logits(hidden, weight, bias, top_k):
+        return _C.linear_scores(hidden, weight, target, bias, temp, real, top_k, kept)
+    chunks = _token_chunks(tokens, vocab)
+    logits = _buffer(chunks[0][1], vocab, hidden.device)
+    parts = [
+        _C.linear_scores(hidden[first:end], weight, target[first:end], bias, _rows(temp, first, end), real, top_k, logits[: end - first])
+        for first, end in chunks
+    ]
     if len(parts) == 1:
         return parts[0]
-    return tuple(None if column[0] is None else torch.cat(column) for column in zip(*parts))
+    return [None if column[0] is None else torch.cat(column) for column in zip(*parts)]
 
 
 class _LinearScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, target_1d, temp, real, top_k):
-        kept = _logits_to_save(hidden, weight.size(0), written_anyway=True)
+        written_anyway = hidden.size(0) > 0 and _C.linear_scores_needs_logits(hidden, weight, bias, top_k)
+        kept = _logits_to_save(hidden, weight.size(0), written_anyway)
         logp, lse, entropy, top_logp, top_ids = _linear_scores(hidden, weight, bias, target_1d, temp, real, top_k, kept)
         ctx.save_for_backward(hidden, weight, bias, target_1d, temp, lse, entropy, top_ids, kept)
         ctx.real = real
@@ -251,7 +251,8 @@ def hip_deterministic_linear_scores(
     :func:`~.linear_logp.hip_deterministic_linear_logp`, whose ``logp`` and ``lse`` these are, to the bit.
 
     A differentiable call keeps its fp32 logits for the backward where memory allows, as that function does (at most 8 GiB in
-    all, not under ``recompute_logits``, saved-tensor hooks or graph capture); otherwise they go through a buffer of at most 2 GiB, a part of the tokens at a time. d(logits) is
+    all, not under ``recompute_logits``, saved-tensor hooks or graph capture). Otherwise no logits are written for more than 1024
+    tokens without ``top_k``, and else they go through a buffer of at most 2 GiB, a part of the tokens at a time. d(logits) is
     rounded to bf16 once, as there. A ``bias`` is added but not differentiated.
     """
     if bias is not None and torch.is_grad_enabled() and bias.requires_grad:

@@ -403,6 +403,40 @@ def test_a_buffer_of_some_tokens_gives_the_same_bits(ops, monkeypatch):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("tokens,vocab,hidden,real,tempered", [(1056, 4096, 128, 4096, False), (1100, 1030, 64, 1001, True), (1280, 18992, 64, 18992, True), (1400, 300, 256, 300, False)])
+def test_a_token_has_the_same_bits_with_and_without_logits(ops, tokens, vocab, hidden, real, tempered):
+    """Above 1024 tokens the entropy comes out of the product's fold; with alternatives, in smaller batches and where the logits are
+    kept for a backward it comes from logits that were stored."""
+    from rl_engine import _C
+
+    h, w, target = _head(tokens, vocab, hidden, tokens)
+    target.clamp_(max=real - 1)
+    temp = 0.5 + torch.rand(tokens, generator=_gen(6), device=DEV) if tempered else None
+    assert not _C.linear_scores_needs_logits(h, w, None, 0) and _C.linear_scores_needs_logits(h, w, None, 1)
+    assert _C.linear_scores_needs_logits(h[:1024], w, None, 0)
+    call = ops.deterministic_linear_scores
+    whole = call(h, w, target, temperature=temp, real_vocab_size=real)
+    want = _reference((h.double() @ w.double().t())[:, :real], target, 0, temp)
+    bound = _bound((h.double() @ w.double().t())[:, :real], 16 * vocab, temp)
+    _close(whole.entropy, want["entropy"], 2 * (math.log(vocab) + 1) * bound)
+    top = call(h, w, target, top_k=3, temperature=temp, real_vocab_size=real)
+    grad_h = h.clone().requires_grad_(True)
+    trained = call(grad_h, w, target, temperature=temp, real_vocab_size=real)
+    stored = torch.empty((tokens, _C.linear_logp_logits_row_stride(vocab)), dtype=torch.float32, device=DEV)
+    kept = _C.linear_scores(h, w, target, None, temp, real, 0, stored)
+    for other in (top, trained, kept):
+        for a, b in zip(whole[:3], other[:3]):
+            assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+    for rows in (slice(0, 1), slice(300, 420), slice(tokens - 70, tokens), slice(0, 1024)):
+        part = call(h[rows], w, target[rows], temperature=None if temp is None else temp[rows], real_vocab_size=real)
+        for a, b in zip(part[:3], whole[:3]):
+            assert torch.equal(a.view(torch.int32), b[rows].view(torch.int32))
+    grads = [torch.autograd.grad(trained.entropy.sum(), [grad_h])[0]]
+    with ops.recompute_logits():
+        grads.append(torch.autograd.grad(call(grad_h, w, target, temperature=temp, real_vocab_size=real).entropy.sum(), [grad_h])[0])
+    assert torch.equal(*grads)
+
+
 # ---------------------------------------------------------------------------
 # Streams, graphs, sizes
 # ---------------------------------------------------------------------------
