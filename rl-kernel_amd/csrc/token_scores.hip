@@ -402,13 +402,17 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   const int k = a.top_k;
   constexpr int kEach = kScoreSlices / kWave;  // a lane has the sixteen slices of one tile
   static_assert(kEach == kTileLanes, "a lane per tile");
-  uint32_t most[kEach];
-  const u32x4_t* src = reinterpret_cast<const u32x4_t*>(a.best + (int64_t)row * kScoreSlices + lane * kEach);
+  uint32_t most[kEach], at[kEach];
+  const u32x4_t* best = reinterpret_cast<const u32x4_t*>(a.best + (int64_t)row * kScoreSlices + lane * kEach);
+  const u32x4_t* where = reinterpret_cast<const u32x4_t*>(a.where + (int64_t)row * kScoreSlices + lane * kEach);
 #pragma unroll
   for (int i = 0; i < kEach / 4; ++i) {
-    const u32x4_t v = src[i];
+    const u32x4_t v = best[i], w = where[i];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) most[4 * i + e] = v[e];
+    for (int e = 0; e < 4; ++e) {
+      most[4 * i + e] = v[e];
+      at[4 * i + e] = w[e];
+    }
   }
   auto count_from = [&](uint32_t limit) __attribute__((always_inline)) {
     int count = 0;
@@ -436,14 +440,6 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
             }) << kIdle, 1u);
   uint64_t floor = (uint64_t)low << 32;  // candidates are not under it; key = (ordered logit, columns behind it)
 
-  uint32_t at[kEach];
-  const u32x4_t* where = reinterpret_cast<const u32x4_t*>(a.where + (int64_t)row * kScoreSlices + lane * kEach);
-#pragma unroll
-  for (int i = 0; i < kEach / 4; ++i) {
-    const u32x4_t v = where[i];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) at[4 * i + e] = v[e];
-  }
   uint32_t last_at = 0xffffffffu;
   if (reach > kFinishPicked) {  // many slices with the same best logit: the first of them, by the vector that holds it
     const uint32_t same = low >> kIdle;
