@@ -51,6 +51,10 @@ decltype(&rlk_grpo_ratio_kl_loss_bwd) grpo_bwd_entry = nullptr;
 decltype(&rlk_logits_scores_workspace_bytes) scores_workspace_entry = nullptr;
 decltype(&rlk_logits_scores) scores_entry = nullptr;
 decltype(&rlk_logits_scores_backward) scores_bwd_entry = nullptr;
+decltype(&rlk_linear_scores_workspace_bytes) linear_scores_workspace_entry = nullptr;
+decltype(&rlk_linear_scores_fwd) linear_scores_entry = nullptr;
+decltype(&rlk_linear_dlogits_row_stride) dlogits_stride_entry = nullptr;
+decltype(&rlk_linear_dlogits_bwd) dlogits_bwd_entry = nullptr;
 decltype(&rlk_block_norm_forward) norm_entry = nullptr;
 decltype(&rlk_block_norm_workspace_bytes) norm_workspace_entry = nullptr;
 decltype(&rlk_block_norm_backward) norm_bwd_entry = nullptr;
@@ -61,6 +65,7 @@ decltype(&rlk_last_error) last_error_entry = nullptr;
 PyObject* general_linear_gradients = nullptr;  // (a, weight, grad, need_a, need_weight) -> (da, dw)
 PyObject* general_ffn_gradients = nullptr;     // (x, gate, up, activated, three weights, grad, need of x and the weights) -> four
 PyObject* general_scores_gradient = nullptr;   // (logits, target, temperature, lse, entropy, top ids, real, four gradients) -> grad
+PyObject* general_linear_scores = nullptr;     // (hidden, weight, target, temperature, lse, entropy, top ids, logits, real, four gradients, two needs) -> two
 PyObject* general_norm_gradients = nullptr;    // (block, residual, gate, two weights, rstd, kind, eps, scale, two gradients, five needs) -> five
 PyObject* general_swiglu_gradients = nullptr;  // (dy, codes and scales of gate and up) -> (d_gate, d_up)
 PyObject* general_grpo_gradient = nullptr;     // (cur, old, ref, adv, mask, g_loss, g_policy, g_kl, clip_eps, beta) -> grad
@@ -481,6 +486,94 @@ struct ScoresFn : torch::autograd::Function<ScoresFn> {
   }
 };
 
+struct LinearScoreInputs {
+  Tensor hidden, weight, target, temp, logits;  // logits: where they go and stay
+  int64_t real;
+  int top_k;
+
+  bool usual() const {
+    return projects(hidden, weight) && weight.size(0) <= RLK_SCORES_MAX_VOCAB && everyday(target, at::kLong, hidden) && target.dim() == 1 &&
+           target.size(0) == hidden.size(0) && target.is_contiguous() &&
+           (!temp.defined() || (everyday(temp, at::kFloat, hidden) && temp.dim() == 1 && temp.size(0) == hidden.size(0) && temp.is_contiguous())) &&
+           everyday(logits, at::kFloat, hidden) && logits.dim() == 2 && logits.is_contiguous() && logits.size(0) == hidden.size(0) &&
+           logits.size(1) == (weight.size(0) + 63) / 64 * 64 && real > 0 && real <= weight.size(0) && top_k >= 0 &&
+           top_k <= RLK_SCORES_MAX_TOP_K && top_k <= real;
+  }
+};
+
+variable_list linear_scores(const LinearScoreInputs& in) {
+  const int64_t tokens = in.hidden.size(0), d = in.hidden.size(1), vocab = in.weight.size(0);
+  variable_list out = {empty({tokens}, at::kFloat, in.hidden), empty({tokens}, at::kFloat, in.hidden), empty({tokens}, at::kFloat, in.hidden)};
+  if (in.top_k > 0) {
+    out.push_back(empty({tokens, in.top_k}, at::kFloat, in.hidden));
+    out.push_back(empty({tokens, in.top_k}, at::kLong, in.hidden));
+  }
+  const size_t bytes = linear_scores_workspace_entry((int)tokens, (int)vocab, in.top_k);
+  const Tensor workspace = empty({(int64_t)bytes}, at::kByte, in.hidden);
+  check_status(linear_scores_entry(in.hidden.data_ptr(), d, in.weight.data_ptr(), d, static_cast<const int64_t*>(in.target.data_ptr()), nullptr,
+                                   floats(in.temp), writable(out[0]), writable(out[1]), writable(out[2]),
+                                   in.top_k > 0 ? writable(out[3]) : nullptr,
+                                   in.top_k > 0 ? static_cast<int64_t*>(out[4].data_ptr()) : nullptr, writable(in.logits), in.logits.size(1),
+                                   workspace.data_ptr(), bytes, (int)tokens, (int)d, (int)vocab, (int)in.real, in.top_k, stream_of(in.hidden)),
+               "rlk_linear_scores_fwd failed");
+  return out;
+}
+
+// The scores of a fused linear-LogP whose logits are kept (_LinearScores in backends/rocm/logprob/token_scores.py).
+struct LinearScoresFn : torch::autograd::Function<LinearScoresFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const LinearScoreInputs* in) {
+    variable_list out = linear_scores(*in);
+    save_some(ctx, {hidden, weight, in->target, in->temp, out[1], out[2], out.size() > 4 ? out[4] : Tensor(), in->logits});
+    ctx->saved_data["real"] = in->real;
+    ctx->set_materialize_grads(false);
+    if (out.size() > 4) ctx->mark_non_differentiable({out[4]});
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    grads.resize(4);
+    if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined() && !grads[3].defined()) return {Tensor(), Tensor(), Tensor()};
+    const variable_list s = saved_some(ctx, 8);
+    const Tensor &lse = s[4], &entropy = s[5], &ids = s[6];
+    const int64_t real = ctx->saved_data["real"].toInt();
+    const int top_k = ids.defined() ? (int)ids.size(1) : 0;
+    const LinearScoreInputs in{s[0], s[1], s[2], s[3], s[7], real, top_k};
+    const bool need_hidden = ctx->needs_input_grad(0), need_weight = ctx->needs_input_grad(1);
+    bool values = !at::GradMode::is_enabled() && everyday_thread() && in.usual() && everyday(lse, at::kFloat, in.hidden) &&
+                  everyday(entropy, at::kFloat, in.hidden) && (!ids.defined() || everyday(ids, at::kLong, in.hidden));
+    const int64_t tokens = values ? in.hidden.size(0) : 0;
+    for (int i = 0; values && i < 4; ++i)
+      values = !grads[i].defined() || (everyday(grads[i], at::kFloat, in.hidden) && grads[i].is_contiguous() &&
+                                       grads[i].numel() == tokens * (i == 3 ? top_k : 1));
+    if (values) {
+      const c10::OptionalDeviceGuard guard(in.hidden.device());
+      const int64_t d = in.hidden.size(1), vocab = in.weight.size(0), stride = dlogits_stride_entry((int)vocab);
+      const Tensor dz = empty({tokens, stride}, kBf16, in.hidden);
+      check_status(scores_bwd_entry(in.logits.data_ptr(), RLK_DTYPE_FP32, in.logits.size(1), static_cast<const int64_t*>(in.target.data_ptr()),
+                                    floats(in.temp), floats(lse), floats(entropy), floats(grads[0]), floats(grads[1]), floats(grads[2]),
+                                    static_cast<const int64_t*>(address(ids)), floats(grads[3]), top_k, dz.data_ptr(), RLK_DTYPE_BF16, stride,
+                                    stride, (int)tokens, vocab, real, stream_of(in.hidden)),
+                   "rlk_logits_scores_backward failed");
+      const Tensor d_hidden = need_hidden ? empty({tokens, d}, kBf16, in.hidden) : Tensor();
+      const Tensor d_weight = need_weight ? empty({vocab, d}, kBf16, in.hidden) : Tensor();
+      check_status(dlogits_bwd_entry(dz.data_ptr(), in.hidden.data_ptr(), d, in.weight.data_ptr(), d, address(d_hidden), d, address(d_weight),
+                                     d, (int)tokens, (int)d, (int)vocab, stream_of(in.hidden)),
+                   "rlk_linear_dlogits_bwd failed");
+      return {d_hidden, d_weight, Tensor()};
+    }
+    const pybind11::gil_scoped_acquire gil;
+    const PyRef args(PyTuple_New(15));
+    for (int i = 0; i < 8; ++i) PyTuple_SET_ITEM(args.get(), i, wrap(s[i]));
+    PyTuple_SET_ITEM(args.get(), 8, PyLong_FromLongLong(real));
+    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(args.get(), 9 + i, wrap(grads[i]));
+    PyTuple_SET_ITEM(args.get(), 13, PyBool_FromLong(need_hidden));
+    PyTuple_SET_ITEM(args.get(), 14, PyBool_FromLong(need_weight));
+    const PyRef two(PyObject_CallObject(general_linear_scores, args.get()));
+    const variable_list out = tensors_of(two, 2);
+    return {out[0], out[1], Tensor()};
+  }
+};
+
 struct NormInputs {
   Tensor block, residual, gate, post, pre;  // rows [tokens, width]; all but the residual may be missing
   int kind;                                 // rlk_gate
@@ -788,6 +881,34 @@ PyObject* py_scores(PyObject*, PyObject* const* args, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
+// linear_scores(hidden, weight, target, temperature or None, real vocabulary, top_k, logits to be kept) -> as scores(), or None
+PyObject* py_linear_scores(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 7 || linear_scores_entry == nullptr) return none();
+  LinearScoreInputs in;
+  if (!tensor_or_nothing(args[0], &in.hidden) || !tensor_or_nothing(args[1], &in.weight) || !tensor_or_nothing(args[2], &in.target) ||
+      !tensor_or_nothing(args[3], &in.temp) || !tensor_or_nothing(args[6], &in.logits) || !PyLong_CheckExact(args[4]) ||
+      !PyLong_CheckExact(args[5]))
+    return none();
+  int overflow[2];
+  in.real = PyLong_AsLongLongAndOverflow(args[4], &overflow[0]);
+  const long top_k = PyLong_AsLongAndOverflow(args[5], &overflow[1]);
+  if (overflow[0] != 0 || overflow[1] != 0 || top_k < 0 || top_k > RLK_SCORES_MAX_TOP_K) return none();
+  in.top_k = (int)top_k;
+  if (!everyday_caller() || !in.usual()) return none();
+  variable_list out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const c10::OptionalDeviceGuard guard(in.hidden.device());
+    const bool differentiable = at::GradMode::is_enabled() && (in.hidden.requires_grad() || in.weight.requires_grad());
+    out = differentiable ? LinearScoresFn::apply(in.hidden, in.weight, &in) : linear_scores(in);
+  }
+  out.resize(5);
+  const PyRef logp(wrap(out[0])), lse(wrap(out[1])), entropy(wrap(out[2])), top_logp(wrap(out[3])), top_ids(wrap(out[4]));
+  return PyTuple_Pack(5, logp.get(), lse.get(), entropy.get(), top_logp.get(), top_ids.get());
+  END_HANDLE_TH_ERRORS
+}
+
 // norm(block or None, residual, gate or None, post weight or None, weight or None, eps, scale) -> (total or None, normed or None), or None
 PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
@@ -879,11 +1000,11 @@ PyObject* py_mx8_encode(PyObject*, PyObject* const* args, Py_ssize_t count) {
 }
 
 // bind(addresses of the entry points by name, the general gradients of the linear layer, the FFN, the GRPO loss, the token scores, the
-// norm between blocks and the SwiGLU of eight-bit copies)
+// norm between blocks, the SwiGLU of eight-bit copies and the token scores of hidden states)
 PyObject* py_bind(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
-  PyObject *addresses, *linear, *ffn, *loss, *of_scores = Py_None, *of_norm = Py_None, *of_swiglu = Py_None;
-  if (!PyArg_ParseTuple(args, "O!OOO|OOO", &PyDict_Type, &addresses, &linear, &ffn, &loss, &of_scores, &of_norm, &of_swiglu)) return nullptr;
+  PyObject *addresses, *linear, *ffn, *loss, *of_scores = Py_None, *of_norm = Py_None, *of_swiglu = Py_None, *of_linear_scores = Py_None;
+  if (!PyArg_ParseTuple(args, "O!OOO|OOOO", &PyDict_Type, &addresses, &linear, &ffn, &loss, &of_scores, &of_norm, &of_swiglu, &of_linear_scores)) return nullptr;
   auto entry = [&](const char* name, auto& to) {
     PyObject* const at = PyDict_GetItemString(addresses, name);
     void* const address = at != nullptr ? PyLong_AsVoidPtr(at) : nullptr;
@@ -908,11 +1029,16 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   entry("rlk_mx8_encode", mx8_encode_entry);
   for (const auto& [from, to] : {std::pair<PyObject*, PyObject**>{of_scores, &general_scores_gradient},
                                  {of_norm, &general_norm_gradients},
-                                 {of_swiglu, &general_swiglu_gradients}}) {
+                                 {of_swiglu, &general_swiglu_gradients},
+                                 {of_linear_scores, &general_linear_scores}}) {
     Py_INCREF(from);
     Py_XSETREF(*to, from);
   }
+  entry("rlk_linear_scores_workspace_bytes", linear_scores_workspace_entry);
+  entry("rlk_linear_dlogits_row_stride", dlogits_stride_entry);
+  entry("rlk_linear_dlogits_bwd", dlogits_bwd_entry);
   entry("rlk_logits_scores", scores_entry);
+  entry("rlk_linear_scores_fwd", linear_scores_entry);
   entry("rlk_block_norm_forward", norm_entry);
   entry("rlk_mx8_swiglu_forward", mx8_swiglu_entry);
   Py_INCREF(linear);
@@ -932,6 +1058,7 @@ PyMethodDef methods[] = {
     {"ffn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_ffn)), METH_FASTCALL, nullptr},
     {"grpo", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_grpo)), METH_FASTCALL, nullptr},
     {"scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_scores)), METH_FASTCALL, nullptr},
+    {"linear_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_scores)), METH_FASTCALL, nullptr},
     {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm)), METH_FASTCALL, nullptr},
     {"mx8_swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx8_swiglu)), METH_FASTCALL, nullptr},
     {"mx8_encode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx8_encode)), METH_FASTCALL, nullptr},

@@ -10,7 +10,8 @@ _ENTRIES = (
     "rlk_last_error", "rlk_det_gemm_bf16", "rlk_linear_bwd_bf16", "rlk_det_gemm_swiglu_workspace_bytes", "rlk_det_gemm_swiglu_bf16",
     "rlk_det_gemm_swiglu_training_bf16", "rlk_swiglu_bwd", "rlk_grpo_workspace_bytes", "rlk_grpo_ratio_kl_loss", "rlk_grpo_ratio_kl_loss_bwd",
     "rlk_logits_scores_workspace_bytes", "rlk_logits_scores", "rlk_logits_scores_backward", "rlk_block_norm_forward",
-    "rlk_block_norm_workspace_bytes", "rlk_block_norm_backward", "rlk_mx8_encode", "rlk_mx8_swiglu_forward", "rlk_mx8_swiglu_backward",
+    "rlk_block_norm_workspace_bytes", "rlk_block_norm_backward", "rlk_linear_scores_workspace_bytes", "rlk_linear_scores_fwd",
+    "rlk_linear_dlogits_row_stride", "rlk_linear_dlogits_bwd", "rlk_mx8_encode", "rlk_mx8_swiglu_forward", "rlk_mx8_swiglu_backward",
 )  # fmt: skip
 _native = None
 
@@ -28,11 +29,14 @@ def native():
             ) from missing
         from rl_engine.backends.rocm.ffn.ffn import ffn_gradients, kept_swiglu_gradients
         from rl_engine.backends.rocm.gemm.det_gemm import linear_gradients
-        from rl_engine.backends.rocm.logprob.token_scores import scores_gradient
+        from rl_engine.backends.rocm.logprob.token_scores import linear_scores_gradients, scores_gradient
         from rl_engine.backends.rocm.loss.grpo import _elementwise_gradient
         from rl_engine.backends.rocm.norm.block_norm import norm_gradients
 
         addresses = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ENTRIES}
-        _torch_host.bind(addresses, linear_gradients, ffn_gradients, _elementwise_gradient, scores_gradient, norm_gradients, kept_swiglu_gradients)
+        _torch_host.bind(
+            addresses, linear_gradients, ffn_gradients, _elementwise_gradient, scores_gradient, norm_gradients, kept_swiglu_gradients,
+            linear_scores_gradients,
+        )  # fmt: skip
         _native = _torch_host
     return _native

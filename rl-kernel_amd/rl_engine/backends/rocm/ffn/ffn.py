@@ -271,6 +271,10 @@ def checkpointed_swiglu(gate: Tensor, up: Tensor) -> Tensor:
     code each and an exponent per run of 32 columns, so that a value is off by at most 2^-7 of the largest in its run. The
     result is that of ``_C.swiglu_forward``, the gradients are those of ``_C.swiglu_backward`` on what was kept: to the bit in bf16
     and fp32, rounded from the fp32 results in fp16. A run with a value that is not finite comes back as NaN."""
+    if not torch.compiler.is_compiling():
+        y = _host.native().mx8_swiglu(gate, up)  # everyday operands, natively
+        if y is not None:
+            return y
     enforce([
         (isinstance(gate, Tensor) and isinstance(up, Tensor), TypeError, "gate and up must be torch.Tensors."),
         (lambda: gate.dim() >= 1 and gate.shape == up.shape, ValueError, lambda: f"gate and up must share shape, got {tuple(gate.shape)} and {tuple(up.shape)}."),

@@ -193,13 +193,36 @@ def _linear_scores(hidden, weight, bias, target, temp, real, top_k, kept):
     return [None if column[0] is None else torch.cat(column) for column in zip(*parts)]
 
 
+def linear_scores_gradients(
+    hidden, weight, target, temp, lse, entropy, top_ids, kept, real, g_logp, g_lse, g_entropy, g_top, need_hidden, need_weight, *, bias=None,
+) -> tuple:  # fmt: skip
+    """The gradients of ``hidden`` and ``weight`` that are wanted, ``None`` for the other; ``kept``: the forward's logits, or ``None``
+    where they are computed again, a part of the tokens at a time."""
+    grads = (g_logp, g_lse, g_entropy, g_top)
+    with torch.no_grad():
+        tokens, vocab = hidden.size(0), weight.size(0)
+        dz = torch.empty((tokens, _C.linear_dlogits_row_stride(vocab)), dtype=torch.bfloat16, device=hidden.device)
+        chunks = [(0, tokens)] if kept is not None or tokens == 0 else _token_chunks(tokens, vocab)
+        logits = kept if kept is not None else _buffer(chunks[0][1], vocab, hidden.device)
+        for first, end in chunks:
+            some = logits[: end - first]
+            rows_temp = _rows(temp, first, end)
+            if kept is None:  # the bits of the forward's logits
+                _C.fused_linear_logp_into(hidden[first:end], weight, target[first:end], bias, rows_temp, real, some)
+            _C.logits_scores_backward(
+                some[:, :vocab], target[first:end], real, lse[first:end], entropy[first:end], _rows(top_ids, first, end),
+                tuple(_rows(g, first, end) for g in grads), temperature=rows_temp, out=dz[first:end],
+            )  # fmt: skip
+        del logits
+        made = _C.linear_dlogits_bwd(dz, hidden, weight, need_hidden, need_weight)
+    return tuple(without_second_derivative(made))
+
+
 class _LinearScores(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, bias, target_1d, temp, real, top_k):
-        written_anyway = hidden.size(0) > 0 and _C.linear_scores_needs_logits(hidden, weight, bias, top_k)
-        kept = _logits_to_save(hidden, weight.size(0), written_anyway)
+    def forward(ctx, hidden, weight, bias, target_1d, temp, real, top_k, kept):
         logp, lse, entropy, top_logp, top_ids = _linear_scores(hidden, weight, bias, target_1d, temp, real, top_k, kept)
-        ctx.save_for_backward(hidden, weight, bias, target_1d, temp, lse, entropy, top_ids, kept)
+        ctx.save_for_backward(hidden, weight, target_1d, temp, lse, entropy, top_ids, kept, bias)
         ctx.real = real
         ctx.set_materialize_grads(False)
         if top_ids is not None:
@@ -210,29 +233,10 @@ class _LinearScores(torch.autograd.Function):
     def backward(ctx, g_logp, g_lse, g_entropy, g_top, _g_ids):
         grads = (g_logp, g_lse, g_entropy, g_top)
         if all(g is None for g in grads):
-            return (None,) * 7
-        with torch.no_grad():
-            two = _LinearScores.gradients(ctx, grads)
-        return *without_second_derivative(two), None, None, None, None, None
-
-    @staticmethod
-    def gradients(ctx, grads) -> list:
-        hidden, weight, bias, target, temp, lse, entropy, top_ids, kept = ctx.saved_tensors
-        tokens, vocab = hidden.size(0), weight.size(0)
-        dz = torch.empty((tokens, _C.linear_dlogits_row_stride(vocab)), dtype=torch.bfloat16, device=hidden.device)
-        chunks = [(0, tokens)] if kept is not None or tokens == 0 else _token_chunks(tokens, vocab)
-        logits = kept if kept is not None else _buffer(chunks[0][1], vocab, hidden.device)
-        for first, end in chunks:
-            some = logits[: end - first]
-            rows_temp = _rows(temp, first, end)
-            if kept is None:  # the same launch as the forward's, so the same bits
-                _C.fused_linear_logp_into(hidden[first:end], weight, target[first:end], bias, rows_temp, ctx.real, some)
-            _C.logits_scores_backward(
-                some[:, :vocab], target[first:end], ctx.real, lse[first:end], entropy[first:end], _rows(top_ids, first, end),
-                tuple(_rows(g, first, end) for g in grads), temperature=rows_temp, out=dz[first:end],
-            )  # fmt: skip
-        del logits
-        return _C.linear_dlogits_bwd(dz, hidden, weight, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+            return (None,) * 8
+        *saved, bias = ctx.saved_tensors
+        two = linear_scores_gradients(*saved, ctx.real, *grads, *ctx.needs_input_grad[:2], bias=bias)
+        return *two, None, None, None, None, None, None
 
 
 def hip_deterministic_linear_scores(
@@ -272,7 +276,13 @@ def hip_deterministic_linear_scores(
     if validate and target_1d.numel():
         _validate_values(target_1d, temp, real)
     if _requires_grad(hidden_2d, weight):
-        scores = _LinearScores.apply(hidden_2d, weight, bias, target_1d, temp, real, top_k)
+        written_anyway = hidden_2d.size(0) > 0 and _C.linear_scores_needs_logits(hidden_2d, weight, bias, top_k)
+        kept = _logits_to_save(hidden_2d, vocab, written_anyway)
+        scores = None
+        if kept is not None and bias is None and not torch.compiler.is_compiling():
+            scores = _host.native().linear_scores(hidden_2d, weight, target_1d, temp, real, top_k, kept)  # everyday operands, natively
+        if scores is None:
+            scores = _LinearScores.apply(hidden_2d, weight, bias, target_1d, temp, real, top_k, kept)
     else:
         scores = _linear_scores(hidden_2d, weight, bias, target_1d, temp, real, top_k, None)
     return _shaped(scores, target_ids.shape)

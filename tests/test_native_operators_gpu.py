@@ -68,6 +68,26 @@ def test_scores(general, top_k, tempered):
         _same(list(deterministic_scores_from_logits(z, target, top_k=top_k)), general(lambda: list(deterministic_scores_from_logits(z, target, top_k=top_k))))
 
 
+@pytest.mark.parametrize("top_k", [0, 5])
+@pytest.mark.parametrize("tokens", [7, 1100])
+def test_linear_scores(general, top_k, tokens):
+    from rl_engine.ops.logprob import deterministic_linear_scores
+
+    h, w = _normal(tokens, 1536, seed=1).requires_grad_(True), _normal(500, 1536, seed=2, scale=0.05).requires_grad_(True)
+    target = torch.arange(tokens, device=DEV) % 500
+    temp = 0.5 + torch.rand(tokens, device=DEV)
+
+    def call():
+        s = deterministic_linear_scores(h, w, target, top_k=top_k, temperature=temp, real_vocab_size=497)
+        outputs = [s.logp, s.lse, s.entropy] + ([s.top_logp] if top_k else [])
+        grads = [_normal(*o.shape, seed=10 + i, dtype=FP32) for i, o in enumerate(outputs)]
+        one = torch.autograd.grad(s.entropy, [w], grads[2], retain_graph=True)
+        late = torch.autograd.grad(s.logp, [h], torch.ones((), device=DEV).expand(tokens), retain_graph=True)
+        return [*s, *torch.autograd.grad(outputs, [h, w], grads), *one, *late]
+
+    _same(call(), general(call))
+
+
 @pytest.mark.parametrize("shape", [(6, 200), (2, 3, 200), (200,)])
 @pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
 @pytest.mark.parametrize("post", [False, True])
@@ -132,6 +152,12 @@ def test_checkpointed_swiglu(general, shape):
     _same(call(), general(call))
     flat = gate.detach().reshape(-1, shape[-1])
     _same(mx8_encode(flat), general(lambda: mx8_encode(flat)))
+
+
+def test_the_entry_points_take_the_native_way():
+    for name, call in _calls().items():
+        out = call(_normal(4, 64, seed=1).requires_grad_(True))
+        assert type(out.grad_fn).__name__ == "CppFunction", name
 
 
 def _calls():
