@@ -489,6 +489,7 @@ int rlk_logits_logp_backward(const void* logits, int dtype, int64_t row_stride, 
  */
 #define RLK_SCORES_MAX_TOP_K 64
 #define RLK_SCORES_MAX_VOCAB (1 << 28)
+#define RLK_SCORES_MAX_ROWS ((1 << 24) - 1)
 size_t rlk_logits_scores_workspace_bytes(int T, int top_k);
 int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature, int T,
                       int64_t V, int64_t real_vocab, int top_k, float* logp, float* lse, float* entropy, float* top_logp,

@@ -39,6 +39,7 @@ struct NormArgs {
   void* d_gate;      // kTokenGate [T], kFullGate [T, H]; or null
   float* part;       // [2][G][H]: sums over rows of d w_pre, and of d w_post without a channel gate's factor
   int64_t T;
+  int64_t first_row;  // of a launch of the forward
   int H, gate_kind;
   bool gate_wide, post_wide, pre_wide;  // fp32 where the block's type is narrower
   bool sum_pre, sum_post;               // which sums over rows are wanted
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a) {
   using EA = typename LogitElem<A>::type;
   using ER = typename LogitElem<R>::type;
   __shared__ float slots[2][1][RowSum<THREADS>::kWaves];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first_row + blockIdx.x;
   const float inv_width = 1.0f / (float)a.H;
   RowVector<A> raw_block[C];
   RowVector<R> raw_residual[C];
@@ -405,11 +406,15 @@ static int norm_groups(int64_t T, int H) {
 size_t block_norm_workspace_bytes(int64_t T, int H) { return T > 0 ? (size_t)2 * norm_groups(T, H) * H * sizeof(float) : 0; }
 
 template <int A, int R, int THREADS, int C>
-static void launch_norm_shape(const NormArgs& a, bool backward, hipStream_t stream) {
+static void launch_norm_shape(NormArgs a, bool backward, hipStream_t stream) {
   if (backward) {
     hipLaunchKernelGGL((norm_backward_kernel<A, R, THREADS, C>), dim3((unsigned)norm_groups(a.T, a.H)), dim3(THREADS), 0, stream, a);
   } else {
-    hipLaunchKernelGGL((norm_forward_kernel<A, R, THREADS, C>), dim3((unsigned)a.T), dim3(THREADS), 0, stream, a);
+    constexpr int64_t kMost = 0x7fffffff / THREADS;  // (a launch has fewer than 2^32 threads)
+    for (; a.first_row < a.T; a.first_row += kMost) {
+      const int64_t some = a.T - a.first_row < kMost ? a.T - a.first_row : kMost;
+      hipLaunchKernelGGL((norm_forward_kernel<A, R, THREADS, C>), dim3((unsigned)some), dim3(THREADS), 0, stream, a);
+    }
   }
 }
 

@@ -602,6 +602,10 @@ static int check_score_args(const char* what, const void* logits, int dtype, int
                             int top_k) {
   int rc = check_logits_args(what, logits, dtype, row_stride, T, V, 0, real_vocab);
   if (rc != RLK_OK) return rc;
+  if (T > RLK_SCORES_MAX_ROWS) {
+    set_last_error("%s: %d rows, at most %d", what, T, RLK_SCORES_MAX_ROWS);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
   if (V > RLK_SCORES_MAX_VOCAB || real_vocab > V) {
     set_last_error("%s: real_vocab %lld must be in [1, V = %lld], V at most %d", what, (long long)real_vocab, (long long)V,
                    RLK_SCORES_MAX_VOCAB);
@@ -677,8 +681,9 @@ int rlk_linear_scores_fwd(const void* hidden, int64_t h_row_stride, const void* 
                           int64_t* top_ids, float* logits, int64_t logits_row_stride, void* workspace, size_t workspace_bytes, int T,
                           int D, int V, int real_vocab_end, int top_k, void* stream) {
   const char* who = "rlk_linear_scores_fwd";
-  if (V > RLK_SCORES_MAX_VOCAB || top_k < 0 || top_k > RLK_SCORES_MAX_TOP_K || (T > 0 && top_k > real_vocab_end)) {
-    set_last_error("%s: V at most %d, top_k %d in [0, min(%d, real_vocab_end)]", who, RLK_SCORES_MAX_VOCAB, top_k, RLK_SCORES_MAX_TOP_K);
+  if (T > RLK_SCORES_MAX_ROWS || V > RLK_SCORES_MAX_VOCAB || top_k < 0 || top_k > RLK_SCORES_MAX_TOP_K || (T > 0 && top_k > real_vocab_end)) {
+    set_last_error("%s: at most %d rows and %d columns, top_k %d in [0, min(%d, real_vocab_end)]", who, RLK_SCORES_MAX_ROWS,
+                   RLK_SCORES_MAX_VOCAB, top_k, RLK_SCORES_MAX_TOP_K);
     return RLK_ERR_INVALID_ARGUMENT;
   }
   bool entropy_in_fold = false;
@@ -852,6 +857,10 @@ static int check_block_norm(const char* who, const rlk_block_norm* n) {
                      (n->pre_weight == nullptr || n->pre_dtype == n->dtype || n->pre_dtype == RLK_DTYPE_FP32);
   if (!types) {
     set_last_error("%s: residual, gate and weights have the type of the block or fp32", who);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  if (!(n->eps >= 0.f)) {
+    set_last_error("%s: eps %g is below 0", who, (double)n->eps);
     return RLK_ERR_INVALID_ARGUMENT;
   }
   if (n->gate_kind < RLK_GATE_NONE || n->gate_kind > RLK_GATE_FULL) {

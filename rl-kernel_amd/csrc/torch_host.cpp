@@ -21,12 +21,16 @@
 #include <ATen/record_function.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <climits>
+#include <unordered_set>
 
 #include "../../include/rlk.h"
 
@@ -409,6 +413,33 @@ variable_list tensors_of(const PyRef& tuple, int count) {
   return out;
 }
 
+// Whether a gradient of the backward that runs, from this node on, reaches a node that was made on another stream. Outside of graph
+// capture the engine lets that stream wait; in one it cannot, so such a backward goes to the general functions, which refuse it.
+bool crosses_streams() {
+  const std::shared_ptr<torch::autograd::Node> start = torch::autograd::get_current_node();
+  if (start == nullptr) return false;
+  const auto* const wanted = torch::autograd::get_current_graph_task_exec_info();  // null or empty: all nodes
+  std::vector<torch::autograd::Node*> open = {start.get()};
+  std::unordered_set<torch::autograd::Node*> seen = {start.get()};
+  while (!open.empty()) {
+    torch::autograd::Node* const node = open.back();
+    open.pop_back();
+    for (const torch::autograd::Edge& edge : node->next_edges()) {
+      torch::autograd::Node* const next = edge.function.get();
+      if (next == nullptr || !seen.insert(next).second) continue;
+      if (wanted != nullptr && !wanted->empty()) {
+        const auto at = wanted->find(next);
+        if (at == wanted->end() || !at->second.should_execute()) continue;
+      }
+      const std::optional<c10::Stream> stream = next->stream();
+      if (stream.has_value() && *stream != c10::impl::VirtualGuardImpl(stream->device_type()).getStream(stream->device())) return true;
+      open.push_back(next);
+    }
+  }
+  return false;
+}
+bool leaves_capture() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None && crosses_streams(); }
+
 struct ScoreInputs {
   Tensor logits, target, temp;
   int64_t real;
@@ -459,7 +490,7 @@ struct ScoresFn : torch::autograd::Function<ScoresFn> {
     const int64_t real = ctx->saved_data["real"].toInt();
     const int top_k = ids.defined() ? (int)ids.size(1) : 0;
     const ScoreInputs in{s[0], s[1], s[2], real, top_k};
-    bool values = !at::GradMode::is_enabled() && everyday_thread() && in.usual() && everyday(lse, at::kFloat, in.logits) &&
+    bool values = !at::GradMode::is_enabled() && everyday_thread() && !leaves_capture() && in.usual() && everyday(lse, at::kFloat, in.logits) &&
                   everyday(entropy, at::kFloat, in.logits) && (!ids.defined() || everyday(ids, at::kLong, in.logits));
     const int64_t rows = values ? in.logits.size(0) : 0;
     for (int i = 0; values && i < 4; ++i)
@@ -539,7 +570,7 @@ struct LinearScoresFn : torch::autograd::Function<LinearScoresFn> {
     const int top_k = ids.defined() ? (int)ids.size(1) : 0;
     const LinearScoreInputs in{s[0], s[1], s[2], s[3], s[7], real, top_k};
     const bool need_hidden = ctx->needs_input_grad(0), need_weight = ctx->needs_input_grad(1);
-    bool values = !at::GradMode::is_enabled() && everyday_thread() && in.usual() && everyday(lse, at::kFloat, in.hidden) &&
+    bool values = !at::GradMode::is_enabled() && everyday_thread() && !leaves_capture() && in.usual() && everyday(lse, at::kFloat, in.hidden) &&
                   everyday(entropy, at::kFloat, in.hidden) && (!ids.defined() || everyday(ids, at::kLong, in.hidden));
     const int64_t tokens = values ? in.hidden.size(0) : 0;
     for (int i = 0; values && i < 4; ++i)
@@ -585,7 +616,7 @@ struct NormInputs {
     return everyday_floats(t, residual) && t.is_contiguous() && (t.scalar_type() == type() || t.scalar_type() == at::kFloat);
   }
   bool usual() const {
-    if (!everyday_floats(residual) || !everyday_matrix(residual) || residual.size(1) > RLK_NORM_MAX_WIDTH || residual.size(0) > INT_MAX) return false;
+    if (!(eps >= 0.0) || !everyday_floats(residual) || !everyday_matrix(residual) || residual.size(1) > RLK_NORM_MAX_WIDTH || residual.size(0) > INT_MAX) return false;
     const int64_t width = residual.size(1);
     if (block.defined() && !(everyday_floats(block, residual) && block.sizes() == residual.sizes() && block.is_contiguous())) return false;
     if (!of_type(residual)) return false;
@@ -661,7 +692,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     NormInputs in{rows(s[0]), rows(s[1]), s[2], s[3], s[4], (int)ctx->saved_data["kind"].toInt(), ctx->saved_data["eps"].toDouble(),
                   ctx->saved_data["scale"].toDouble()};
     const Tensor& rstd = s[5];
-    bool values = !at::GradMode::is_enabled() && everyday_thread() && in.usual() && everyday(rstd, at::kFloat, in.residual);
+    bool values = !at::GradMode::is_enabled() && everyday_thread() && !leaves_capture() && in.usual() && everyday(rstd, at::kFloat, in.residual);
     if (values && g_total.defined())
       values = everyday(g_total, in.residual.scalar_type(), in.residual) && g_total.is_contiguous() && g_total.numel() == in.residual.numel();
     if (values && g_normed.defined())
@@ -730,7 +761,7 @@ struct Mx8SwigluFn : torch::autograd::Function<Mx8SwigluFn> {
     const variable_list s = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
     const int64_t cols = s[0].size(1), rows = s[0].size(0);
-    bool values = !at::GradMode::is_enabled() && everyday_thread() && everyday_floats(dy) && dy.is_contiguous() && dy.numel() == rows * cols;
+    bool values = !at::GradMode::is_enabled() && everyday_thread() && !leaves_capture() && everyday_floats(dy) && dy.is_contiguous() && dy.numel() == rows * cols;
     for (int i = 0; values && i < 4; ++i) values = everyday(s[i], i % 2 ? at::kByte : at::kChar, dy) && s[i].is_contiguous();
     if (values) {
       const c10::OptionalDeviceGuard guard(dy.device());
@@ -878,6 +909,13 @@ PyObject* py_scores(PyObject*, PyObject* const* args, Py_ssize_t count) {
   out.resize(5);
   const PyRef logp(wrap(out[0])), lse(wrap(out[1])), entropy(wrap(out[2])), top_logp(wrap(out[3])), top_ids(wrap(out[4]));
   return PyTuple_Pack(5, logp.get(), lse.get(), entropy.get(), top_logp.get(), top_ids.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// crosses_streams() -> whether a gradient of the backward that runs reaches a node that was made on another stream
+PyObject* py_crosses_streams(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  return PyBool_FromLong(crosses_streams());
   END_HANDLE_TH_ERRORS
 }
 
@@ -1058,6 +1096,7 @@ PyMethodDef methods[] = {
     {"ffn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_ffn)), METH_FASTCALL, nullptr},
     {"grpo", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_grpo)), METH_FASTCALL, nullptr},
     {"scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_scores)), METH_FASTCALL, nullptr},
+    {"crosses_streams", py_crosses_streams, METH_NOARGS, nullptr},
     {"linear_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_scores)), METH_FASTCALL, nullptr},
     {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm)), METH_FASTCALL, nullptr},
     {"mx8_swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx8_swiglu)), METH_FASTCALL, nullptr},

@@ -4,6 +4,8 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 from rl_engine import _lib
 
 _ENTRIES = (
@@ -40,3 +42,16 @@ def native():
         )  # fmt: skip
         _native = _torch_host
     return _native
+
+
+def refuse_capture_into_another_graph() -> None:
+    """For a backward in front of its first launch. A leaf keeps the node that gathers its gradient as long as any graph holds the leaf,
+    and the engine orders that node's stream behind the gradient. Under graph capture that stream is not part of the capture: the
+    engine's thread would end the process over it."""
+    from rl_engine import _torch_host
+
+    if torch.cuda.is_current_stream_capturing() and _torch_host.crosses_streams():
+        raise RuntimeError(
+            "a backward cannot be captured into a graph while an autograd graph that was made outside of the capture holds its inputs: "
+            "drop the outputs of the earlier calls first"
+        )

@@ -222,6 +222,7 @@ class _CheckpointedFFNFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
+        _host.refuse_capture_into_another_graph()
         with torch.no_grad():
             grads = _CheckpointedFFNFunction.gradients(ctx, grad_output)
         return *without_second_derivative(grads), None
@@ -246,6 +247,7 @@ class _CheckpointedFFNFunction(torch.autograd.Function):
 
 def kept_swiglu_gradients(dy, gate_codes, gate_scales, up_codes, up_scales) -> tuple:
     """``(d_gate, d_up)`` in the shape of ``dy``, from the copies of gate and up."""
+    _host.refuse_capture_into_another_graph()
     with torch.no_grad():
         d_gate, d_up, _ = _C.swiglu_mx8_backward(dy.reshape(gate_codes.shape), gate_codes, gate_scales, up_codes, up_scales)
         grads = [d_gate.reshape(dy.shape), d_up.reshape(dy.shape)]
@@ -285,6 +287,8 @@ def checkpointed_swiglu(gate: Tensor, up: Tensor) -> Tensor:
         gate, up = gate.reshape(rows, shape[-1]), up.reshape(rows, shape[-1])
     if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
         y = _CheckpointedSwiglu.apply(gate, up)
+    elif gate.dtype == torch.float16:  # (the bits of a differentiated call)
+        y = _C.swiglu_mx8_forward(gate, up)[0]
     else:
         y = _C.swiglu_forward(gate.contiguous(), up.contiguous())
     return y.reshape(shape)

@@ -84,6 +84,7 @@ def _shaped(scores, shape: torch.Size) -> TokenScores:
 def scores_gradient(logits, target_1d, temp, lse, entropy, top_ids, real, g_logp, g_lse, g_entropy, g_top) -> torch.Tensor:
     """d(logits) of the scores of ``logits [rows, V]``, from the forward's answers and the gradients of its outputs (or ``None``)."""
     grads = (g_logp, g_lse, g_entropy, g_top)
+    _host.refuse_capture_into_another_graph()
     with torch.no_grad():
         grad = _C.logits_scores_backward(logits, target_1d, real, lse, entropy, top_ids, grads, temperature=temp)
     return without_second_derivative([grad])[0]
@@ -119,7 +120,7 @@ def hip_deterministic_scores_from_logits(
 ) -> TokenScores:
     """:class:`TokenScores` of ``logits [..., V]`` (bf16 / fp16 / fp32) for ``target_ids [...]``; differentiable in ``logits``.
 
-    ``temperature`` (a number, or one per row) divides the logits; ``real_vocab_size`` leaves out the columns behind it, whatever
+    ``temperature`` (a number, or one per row; not differentiated) divides the logits; ``real_vocab_size`` leaves out the columns behind it, whatever
     they hold. Logits of ``-inf`` are tokens that cannot be drawn: they add nothing to ``lse`` and ``entropy`` and have no
     gradient of their own. A row without any other has no distribution: its ``lse`` is ``-inf``, its other answers are NaN.
 
@@ -199,6 +200,7 @@ def linear_scores_gradients(
     """The gradients of ``hidden`` and ``weight`` that are wanted, ``None`` for the other; ``kept``: the forward's logits, or ``None``
     where they are computed again, a part of the tokens at a time."""
     grads = (g_logp, g_lse, g_entropy, g_top)
+    _host.refuse_capture_into_another_graph()
     with torch.no_grad():
         tokens, vocab = hidden.size(0), weight.size(0)
         dz = torch.empty((tokens, _C.linear_dlogits_row_stride(vocab)), dtype=torch.bfloat16, device=hidden.device)

@@ -64,6 +64,7 @@ def norm_gradients(
 ) -> tuple:  # fmt: skip
     """The gradients of ``block``, ``residual``, ``gate`` and the weights that are wanted, ``None`` for the others. ``block`` and
     ``residual`` are rows or batches of rows; ``dtype``: the type of the normed result (that of ``block``, or of ``residual``)."""
+    _host.refuse_capture_into_another_graph()
     dtype = dtype or (residual if block is None else block).dtype
     device, width = residual.device, residual.size(-1)
     with torch.no_grad():
@@ -111,6 +112,13 @@ def _check_rows(t: Tensor, name: str) -> None:
         (lambda: t.dtype in _DTYPES, TypeError, lambda: f"{name} must be bf16, fp16 or fp32, got {t.dtype}."),
         (lambda: t.is_cuda, RuntimeError, lambda: f"{name} must be on a CUDA/ROCm GPU device, got '{t.device}'."),
     ])  # fmt: skip
+
+
+def _check_eps(eps: float) -> float:
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must be at least 0, got {eps}.")
+    return eps
 
 
 def _check_beside(t: Tensor, name: str, home: Tensor, dtype: torch.dtype) -> None:
@@ -181,7 +189,7 @@ def gated_residual_norm(
     pre = _vector(weight, "weight", block, block.dtype)
     gate_rows, kind = _gate_rows(gate, block)
     args = (_rows(block, width), _rows(residual, width), gate_rows, post, pre)
-    how = (block.dtype, float(eps), float(residual_scale), True)
+    how = (block.dtype, _check_eps(eps), float(residual_scale), True)
     if _differentiable(*args):
         total, normed = _BlockNorm.apply(*args, kind, *how)
     else:
@@ -206,7 +214,7 @@ def rms_norm(x: Tensor, weight: Tensor, *, eps: float = 1e-6, dtype: Optional[to
         raise TypeError("weight must be a torch.Tensor, got None.")
     pre = _vector(weight, "weight", x, dtype)
     rows = _rows(x, x.size(-1))
-    how = (dtype, float(eps), 1.0, False)
+    how = (dtype, _check_eps(eps), 1.0, False)
     if _differentiable(rows, pre):
         normed = _BlockNorm.apply(None, rows, None, None, pre, _lib.GATE_NONE, *how)[1]
     else:

@@ -267,6 +267,18 @@ def test_no_tokens(norm):
     assert got["total"].shape == (0, 64) and not any(bool(got[k].any()) for k in ("d_pre", "d_post", "d_gate"))
 
 
+def test_more_rows_than_one_launch_has():
+    """A launch of the forward has fewer than 2^32 threads, 64 to a row of up to 512 columns."""
+    from rl_engine.ops.norm import rms_norm
+
+    rows = 2**31 // 64 + 5
+    x = torch.ones((rows, 8), dtype=BF16, device=DEV)
+    x[-7:] = _normal(7, 8, seed=1)
+    w = _normal(8, seed=2)
+    got = rms_norm(x, w)
+    assert torch.equal(got[-7:], rms_norm(x[-7:].clone(), w)) and bool((got[:-7] == got[0]).all())
+
+
 def test_infinities_stay_in_their_rows(norm):
     t, *_ = _case(4, 128, BF16, BF16, "none", True, True)
     clean = norm.gated_residual_norm(t["block"], t["residual"], t["pre"], post_weight=t["post"])
@@ -289,6 +301,11 @@ def test_refused_calls(norm):
     ):  # fmt: skip
         with pytest.raises(error):
             call(*args, **kwargs)
+    for eps in (-1e-6, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            call(x, x, w, eps=eps)
+        with pytest.raises(ValueError, match="eps"):
+            norm.rms_norm(x, w, eps=eps)
     for args, kwargs in (((x, None), {}), ((x, w), {"dtype": FP32}), ((x.half(), w), {})):
         with pytest.raises(TypeError):
             norm.rms_norm(*args, **kwargs)

@@ -106,6 +106,17 @@ def test_swiglu_is_that_of_the_copies(native, rows, cols, dtype):
         assert torch.equal(_bits(g), _bits(w))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_result_is_the_same_without_a_gradient(dtype):
+    from rl_engine.ops.ffn import checkpointed_swiglu
+
+    gate, up = _normal(40, 1000, seed=1, dtype=dtype, scale=2.0), _normal(40, 1000, seed=2, dtype=dtype)
+    want = checkpointed_swiglu(gate.clone().requires_grad_(True), up).detach()
+    assert torch.equal(_bits(checkpointed_swiglu(gate, up)), _bits(want))
+    both = torch.cat([gate, up], dim=1).chunk(2, dim=1)
+    assert torch.equal(_bits(checkpointed_swiglu(*both)), _bits(want))
+
+
 def test_gradient_of_what_was_kept_against_differences(native):
     """Central differences of SwiGLU in 64 bits at the kept values; fp32 gradients, off by 2^-20 of their factors."""
     gate, up, dy = _normal(4, 64, seed=5, dtype=torch.float32), _normal(4, 64, seed=6, dtype=torch.float32), _normal(4, 64, seed=7, dtype=torch.float32)

@@ -3,6 +3,8 @@ where the arguments are more than values in memory."""
 
 from __future__ import annotations
 
+import gc
+
 import pytest
 import torch
 
@@ -238,4 +240,107 @@ def test_backward_on_the_stream_of_the_forward():
         out = gated_residual_norm(x, x, w)[1]
     torch.cuda.current_stream().wait_stream(side)
     got = torch.autograd.grad(out.float().square().mean(), [x])[0]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", ["scores", "linear", "norm", "swiglu", "ffn", "behind a cast"])
+def test_a_backward_is_not_captured_into_another_graph(general, name):
+    """The leaf's gatherer belongs to the stream that an earlier graph was made on, which no capture may wait for: refused in front of
+    any launch. The capture goes on, and so does the earlier graph; without it the same capture is taken."""
+    from rl_engine.ops.ffn import qwen3_ffn
+
+    w = _normal(64, 64, seed=3)
+    calls = _calls()
+    swiglu = calls["swiglu"]
+    call = {"ffn": lambda x: qwen3_ffn(x, w, w, w, checkpoint_bits=8), "behind a cast": lambda x: swiglu(x.float()), **calls}[name]
+
+    def refused():
+        x = _normal(4, 64, seed=1).requires_grad_(True)
+        g = torch.ones_like(call(x).detach())
+        step = lambda: torch.autograd.grad(call(x), [x], g)[0]  # noqa: E731
+        want = step()
+        held = call(x)
+        a = torch.ones(64, device=DEV)
+        a + 1
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            inside = call(x)
+            with pytest.raises(RuntimeError, match="cannot be captured"):
+                torch.autograd.grad(inside, [x], g)
+            b = a + 1
+        for start in (3.0, 5.0):
+            a.fill_(start)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert bool((b == start + 1).all())
+        assert torch.equal(torch.autograd.grad(held, [x], g)[0], want)
+        del held, inside
+        gc.collect()  # (what the refusal's traceback holds)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+    refused()
+    general(refused)
+
+
+def test_what_wants_no_gradient_is_no_obstacle(general):
+    """An earlier graph may hold a leaf whose gradient the captured backward does not compute."""
+    from rl_engine.ops.norm import gated_residual_norm
+
+    def captured():
+        x, w = _normal(4, 64, seed=1).requires_grad_(True), _normal(64, seed=2).requires_grad_(True)
+        g = _normal(4, 64, seed=3)
+        step = lambda: torch.autograd.grad(gated_residual_norm(x, x, w)[1], [x], g)[0]  # noqa: E731
+        want = step()
+        held = w * 2  # noqa: F841
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+    captured()
+    general(captured)
+
+
+def test_a_leaf_of_another_stream_is_seen(general):
+    """Outside of a capture such a backward runs, on the stream of its forward."""
+    from rl_engine import _host
+
+    x = _normal(4, 64, seed=1).requires_grad_(True)
+    seen = []
+
+    class Look(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            seen.append(_host.native().crosses_streams())
+            return g * 2
+
+    held = Look.apply(x)  # noqa: F841
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            torch.autograd.grad(Look.apply(x).sum(), [x])
+    assert seen == [False, True] and not _host.native().crosses_streams()
+    call = _calls()["norm"]
+    held = call(x)  # noqa: F841
+    want = torch.autograd.grad(call(x).sum(), [x])[0]
+    with torch.cuda.stream(side):
+        got = torch.autograd.grad(call(x).sum(), [x])[0]
+    torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want)
