@@ -11,7 +11,7 @@
 //   d_u = scale gate d_total;               d_gate = scale u d_total (summed over what the gate is shared by)
 //   h1 = block r1;  b = d_u w_post;         d_block = r1 (b - h1 mean(b h1));              d w_post = sum over rows of d_u h1
 //
-// HBM-bound: every tensor is read or written once. A row belongs to one workgroup and stays in its registers; sums over a row
+// HBM-bound: every tensor is read or written once (forward, bf16 with an fp32 residual, 4096 x 4096: 33 us = 5.0 TB/s). A row belongs to one workgroup and stays in its registers; sums over a row
 // are taken in an order that depends on its width alone, so that a row's results never depend on its batch. Sums over rows:
 // a workgroup of the backward takes every G-th row (G a function of the row count), keeps its sums in registers, and a second
 // launch adds the G of them in a fixed order.
@@ -46,16 +46,58 @@ struct NormArgs {
   float eps, scale;
 };
 
+// Eight columns of a row, at its end moved to the left (RowVector::load_window). SMALL: the row has fewer; kernels of their own take such
+// rows, as the code for single elements, never run, made the forward of 8192 columns a third slower.
+template <bool SMALL, int E>
+__device__ __forceinline__ void load8(RowVector<E>& v, const typename LogitElem<E>::type* row, int col, int cols) {
+  if constexpr (SMALL) v.template load_window<false>(row, col, cols);
+  else v.template load_at<false>(row, (uint32_t)min(col, cols - 8));
+}
+template <bool SMALL, int E>
+__device__ __forceinline__ void store8(const RowVector<E>& v, typename LogitElem<E>::type* row, int col, int cols) {
+  using T = typename LogitElem<E>::type;
+  if constexpr (SMALL) v.template store_edge<false>(row, 0, cols);
+  else v.template store<false>(reinterpret_cast<T*>(reinterpret_cast<char*>(row) + (uint32_t)min(col, cols - 8) * (uint32_t)sizeof(T)));
+}
+
 // Eight values of a vector whose type is that of the block, or fp32.
-template <int A>
+template <int A, bool SMALL>
+struct EitherVector {
+  u32x4_t w[2];
+  __device__ __forceinline__ void load(const void* p, int64_t base, bool wide, int col, int cols) {
+    if (wide || A == RLK_DTYPE_FP32) {
+      RowVector<RLK_DTYPE_FP32> v;
+      load8<SMALL>(v, reinterpret_cast<const float*>(p) + base, col, cols);
+      w[0] = v.w[0];
+      w[1] = v.w[1];
+    } else {
+      RowVector<A> v;
+      load8<SMALL>(v, reinterpret_cast<const typename LogitElem<A>::type*>(p) + base, col, cols);
+      w[0] = v.w[0];
+    }
+  }
+  __device__ __forceinline__ void unpack(bool wide, float (&out)[8]) const {
+    if (wide || A == RLK_DTYPE_FP32) {
+      RowVector<RLK_DTYPE_FP32> v;
+      v.w[0] = w[0];
+      v.w[1] = w[1];
+      v.unpack(out);
+    } else {
+      RowVector<A> v;
+      v.w[0] = w[0];
+      v.unpack(out);
+    }
+  }
+};
+template <int A, bool SMALL>
 __device__ __forceinline__ void load_either(const void* p, int64_t base, bool wide, int col, int cols, float (&out)[8]) {
-  if (wide) {
+  if (wide || A == RLK_DTYPE_FP32) {
     RowVector<RLK_DTYPE_FP32> v;
-    v.load_edge<false>(reinterpret_cast<const float*>(p) + base, col / 8, cols);
+    load8<SMALL>(v, reinterpret_cast<const float*>(p) + base, col, cols);
     v.unpack(out);
   } else {
     RowVector<A> v;
-    v.template load_edge<false>(reinterpret_cast<const typename LogitElem<A>::type*>(p) + base, col / 8, cols);
+    load8<SMALL>(v, reinterpret_cast<const typename LogitElem<A>::type*>(p) + base, col, cols);
     v.unpack(out);
   }
 }
@@ -64,17 +106,32 @@ __device__ __forceinline__ float load_one(const void* p, int64_t at, bool wide) 
   return wide ? reinterpret_cast<const float*>(p)[at] : LogitElem<A>::to_float(reinterpret_cast<const typename LogitElem<A>::type*>(p)[at]);
 }
 
-template <int THREADS>
-struct RowSum {
-  static constexpr int kWaves = THREADS / kWave;
-  // The sum over the workgroup's threads, in all of them: butterflies over the lanes, then the waves ascending. One barrier: a slot
-  // is written again only behind another one.
+// A row is the work of LANES threads: part of a wave up to 256 columns, so that no lane is idle (262144 rows of 128 columns, a wave
+// each / sixteen lanes each: forward 140 / 50 us, backward 253 / 82), else whole waves.
+template <int LANES>
+struct NormShape {
+  static constexpr int kThreads = LANES <= kWave ? 256 : LANES;
+  static constexpr int kRows = kThreads / LANES;  // of a workgroup at a time
+  static constexpr int kWaves = LANES <= kWave ? 1 : LANES / kWave;  // of a row
+
+  // The sum over the threads of a row, in all of them: within sixteen lanes, across them, then the waves ascending. One barrier:
+  // a slot is written again only behind another one.
   template <int N>
-  static __device__ __forceinline__ void over(float (&v)[N], float (*slot)[kWaves]) {
+  static __device__ __forceinline__ void sum(float (&v)[N], float (*slot)[kWaves]) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-#pragma unroll
-      for (int offset = 32; offset > 0; offset >>= 1) v[n] = v[n] + __shfl_xor(v[n], offset);
+      v[n] = v[n] + xor_lane<1>(v[n]);
+      v[n] = v[n] + xor_lane<2>(v[n]);
+      v[n] = v[n] + dpp<0x141>(v[n]);  // row_half_mirror, row_mirror: the other four, the other eight
+      v[n] = v[n] + dpp<0x140>(v[n]);
+      if constexpr (LANES >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[n]), __float_as_uint(v[n]), false, false);
+        v[n] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+      }
+      if constexpr (LANES >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[n]), __float_as_uint(v[n]), false, false);
+        v[n] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+      }
     }
     if constexpr (kWaves > 1) {
       const int wave = threadIdx.x >> 6;
@@ -91,173 +148,309 @@ struct RowSum {
       }
     }
   }
+  template <int CONTROL>
+  static __device__ __forceinline__ float dpp(float v) {
+    const int bits = __float_as_int(v);
+    return __int_as_float(__builtin_amdgcn_update_dpp(bits, bits, CONTROL, 0xf, 0xf, false));
+  }
+};
+
+// A thread's c-th vector: eight columns from `col` on. One that would run past the row is moved to its end (RowVector::load_window)
+// and shares columns with its neighbour: both compute and store the same values, sums over the row take a column once.
+struct NormColumns {
+  int col, cols;
+  bool have, ragged;
+  __device__ __forceinline__ NormColumns(int lane, int lanes, int c, int width)
+      : col((c * lanes + lane) * 8), cols(width), have(col < width), ragged(col + 8 > width) {}
+  __device__ __forceinline__ void once(const float (&x)[8], float (&out)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = x[i];
+    if (ragged) {
+      const int at = window_of(col, cols);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = at + i >= col && at + i < cols ? x[i] : 0.f;
+    }
+  }
 };
 
 // A: type of block, normed and (where they are not fp32) weights and gate. R: type of the residual. C: vectors of eight columns
 // per thread.
-template <int A, int R, int THREADS, int C>
-__global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a) {
+template <int A, int R, int LANES, int C, bool SMALL>
+__global__ __launch_bounds__(NormShape<LANES>::kThreads) void norm_forward_kernel(NormArgs a) {
+  using Shape = NormShape<LANES>;
   using EA = typename LogitElem<A>::type;
   using ER = typename LogitElem<R>::type;
-  __shared__ float slots[2][1][RowSum<THREADS>::kWaves];
-  const int64_t row = a.first_row + blockIdx.x;
+  __shared__ float slots[2][1][Shape::kWaves];
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = Shape::kRows == 1 ? a.first_row + blockIdx.x : a.first_row + (int64_t)blockIdx.x * Shape::kRows + threadIdx.x / LANES;
+  if (Shape::kRows > 1 && row >= a.T) return;
   const float inv_width = 1.0f / (float)a.H;
   RowVector<A> raw_block[C];
   RowVector<R> raw_residual[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int col = (c * THREADS + (int)threadIdx.x) * 8;
-    if (col >= a.H) continue;
-    if (a.block) raw_block[c].template load_edge<false>(reinterpret_cast<const EA*>(a.block) + row * a.ld_block, col / 8, a.H);
-    raw_residual[c].template load_edge<false>(reinterpret_cast<const ER*>(a.residual) + row * a.ld_residual, col / 8, a.H);
+    const NormColumns at(lane, LANES, c, a.H);
+    if (!at.have) continue;
+    if (a.block) load8<SMALL>(raw_block[c], reinterpret_cast<const EA*>(a.block) + row * a.ld_block, at.col, a.H);
+    load8<SMALL>(raw_residual[c], reinterpret_cast<const ER*>(a.residual) + row * a.ld_residual, at.col, a.H);
   }
   float x[C][8], t[C][8];
   float sum[1] = {0.f};
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int col = (c * THREADS + (int)threadIdx.x) * 8;
+    const NormColumns at(lane, LANES, c, a.H);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[c][i] = t[c][i] = 0.f;
-    if (col >= a.H) continue;
+    if (!at.have) continue;
     if (a.block) raw_block[c].unpack(x[c]);
     raw_residual[c].unpack(t[c]);
+    float v[8];
+    at.once(x[c], v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[0] = __builtin_fmaf(x[c][i], x[c][i], sum[0]);
+    for (int i = 0; i < 8; ++i) sum[0] = __builtin_fmaf(v[i], v[i], sum[0]);
   }
   float r1 = 1.f;
   if (a.w_post) {
-    RowSum<THREADS>::over(sum, slots[0]);
+    Shape::sum(sum, slots[0]);
     r1 = 1.0f / sqrtf(__builtin_fmaf(sum[0], inv_width, a.eps));
   }
   const float token_gate = a.gate_kind == kTokenGate ? load_one<A>(a.gate, row * a.ld_gate, a.gate_wide) : 1.f;
   sum[0] = 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int col = (c * THREADS + (int)threadIdx.x) * 8;
-    if (col >= a.H) continue;
+    const NormColumns at(lane, LANES, c, a.H);
+    if (!at.have) continue;
     if (a.block) {
       if (a.w_post) {
         float w[8];
-        load_either<A>(a.w_post, 0, a.post_wide, col, a.H, w);
+        load_either<A, SMALL>(a.w_post, 0, a.post_wide, at.col, a.H, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[c][i] = x[c][i] * r1 * w[i];
       }
       float g[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) g[i] = token_gate;
-      if (a.gate_kind == kChannelGate) load_either<A>(a.gate, 0, a.gate_wide, col, a.H, g);
-      if (a.gate_kind == kFullGate) load_either<A>(a.gate, row * a.ld_gate, a.gate_wide, col, a.H, g);
+      if (a.gate_kind == kChannelGate) load_either<A, SMALL>(a.gate, 0, a.gate_wide, at.col, a.H, g);
+      if (a.gate_kind == kFullGate) load_either<A, SMALL>(a.gate, row * a.ld_gate, a.gate_wide, at.col, a.H, g);
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[c][i] = __builtin_fmaf(a.scale * g[i], x[c][i], t[c][i]);
     }
     if (a.total) {
       RowVector<R> out;
       out.pack(t[c]);
-      out.template store_edge<false>(reinterpret_cast<ER*>(a.total) + row * a.H, col, a.H);
+      store8<SMALL>(out, reinterpret_cast<ER*>(a.total) + row * a.H, at.col, a.H);
     }
+    float v[8];
+    at.once(t[c], v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[0] = __builtin_fmaf(t[c][i], t[c][i], sum[0]);
+    for (int i = 0; i < 8; ++i) sum[0] = __builtin_fmaf(v[i], v[i], sum[0]);
   }
   float r2 = 0.f;
   if (a.w_pre) {
-    RowSum<THREADS>::over(sum, slots[1]);
+    Shape::sum(sum, slots[1]);
     r2 = 1.0f / sqrtf(__builtin_fmaf(sum[0], inv_width, a.eps));
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int col = (c * THREADS + (int)threadIdx.x) * 8;
-      if (col >= a.H) continue;
+      const NormColumns at(lane, LANES, c, a.H);
+      if (!at.have) continue;
       float w[8];
-      load_either<A>(a.w_pre, 0, a.pre_wide, col, a.H, w);
+      load_either<A, SMALL>(a.w_pre, 0, a.pre_wide, at.col, a.H, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = t[c][i] * r2 * w[i];
       RowVector<A> out;
       out.pack(w);
-      out.template store_edge<false>(reinterpret_cast<EA*>(a.normed) + row * a.H, col, a.H);
+      store8<SMALL>(out, reinterpret_cast<EA*>(a.normed) + row * a.H, at.col, a.H);
     }
   }
-  if (a.rstd && threadIdx.x == 0) {
+  if (a.rstd && lane == 0) {
     a.rstd[row] = r1;
     a.rstd[a.T + row] = r2;
   }
 }
 
-template <int A, int R, int THREADS, int C>
-__global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormArgs a) {
+// What a row's backward needs first, eight columns of a thread.
+template <int A, int R, bool FULL, bool SMALL>
+struct NormRow {
+  RowVector<A> block, normed;
+  RowVector<R> residual;
+  EitherVector<A, SMALL> gate;  // FULL
+
+  __device__ __forceinline__ void fetch(const NormArgs& a, int64_t row, int col) {
+    using EA = typename LogitElem<A>::type;
+    using ER = typename LogitElem<R>::type;
+    if (a.block) load8<SMALL>(block, reinterpret_cast<const EA*>(a.block) + row * a.ld_block, col, a.H);
+    load8<SMALL>(residual, reinterpret_cast<const ER*>(a.residual) + row * a.ld_residual, col, a.H);
+    if (a.g_normed) load8<SMALL>(normed, reinterpret_cast<const EA*>(a.g_normed) + row * a.H, col, a.H);
+    if constexpr (FULL) gate.load(a.gate, row * a.ld_gate, a.gate_wide, col, a.H);
+  }
+};
+
+// A workgroup goes through its rows one after the other. Up to 8192 columns (a vector to a thread) the next row is on its way while
+// one is worked on, the sums over rows are in registers, and weights and a channel gate wait in LDS, each thread's own columns, to
+// be read without a barrier (each row loaded as its turn comes, weights from the caches / so, bf16: 4096 x 8192 110 / 90 us, with an
+// fp32 residual 163 / 128, 8192 x 4096 with a full gate 119 / 101 = 5.3 TB/s). Above (two vectors) it is the sums that are in LDS
+// (2048 x 16384, sums in registers, most of which spilled / in LDS: 245 / 154 us). A full gate has kernels of its own: its registers
+// would have the others spill. Four waves to a SIMD: with fewer the loads of a workgroup have nobody to hide behind.
+template <int A, int R, int LANES, int C, bool FULL, bool SMALL>
+__global__ __launch_bounds__(NormShape<LANES>::kThreads) __attribute__((amdgpu_waves_per_eu(4))) void norm_backward_kernel(NormArgs a) {
+  using Shape = NormShape<LANES>;
   using EA = typename LogitElem<A>::type;
   using ER = typename LogitElem<R>::type;
-  __shared__ float slots[2][3][RowSum<THREADS>::kWaves];  // rows take turns: a row may pass one barrier only
+  constexpr bool kAhead = C == 1;
+  constexpr int kPre = 0, kPost = 1, kGate = 2;
+  __shared__ float slots[2][3][Shape::kWaves];  // rows take turns: a row may pass one barrier only
+  __shared__ f32x4_t own[kAhead ? 6 : 4 * C][Shape::kThreads];
   int turn = 0;
+  const int lane = threadIdx.x % LANES;
   const float inv_width = 1.0f / (float)a.H;
   const bool token_sum = a.gate_kind == kTokenGate && a.d_gate;
-  float sum_pre[C][8], sum_post[C][8];
+  auto put = [&](int at, const float (&v)[8]) __attribute__((always_inline)) {
+    own[at][threadIdx.x] = f32x4_t{v[0], v[1], v[2], v[3]};
+    own[at + 1][threadIdx.x] = f32x4_t{v[4], v[5], v[6], v[7]};
+  };
+  auto get = [&](int at, float (&v)[8]) __attribute__((always_inline)) {
+    const f32x4_t lo = own[at][threadIdx.x], hi = own[at + 1][threadIdx.x];
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum_pre[c][i] = sum_post[c][i] = 0.f;
-
-  for (int64_t row = blockIdx.x; row < a.T; row += gridDim.x, turn ^= 1) {
-    RowVector<A> raw_block[C], raw_normed[C];
-    RowVector<R> raw_residual[C], raw_total[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int col = (c * THREADS + (int)threadIdx.x) * 8;
-      if (col >= a.H) continue;
-      if (a.block) raw_block[c].template load_edge<false>(reinterpret_cast<const EA*>(a.block) + row * a.ld_block, col / 8, a.H);
-      raw_residual[c].template load_edge<false>(reinterpret_cast<const ER*>(a.residual) + row * a.ld_residual, col / 8, a.H);
-      if (a.g_normed) raw_normed[c].template load_edge<false>(reinterpret_cast<const EA*>(a.g_normed) + row * a.H, col / 8, a.H);
-      if (a.g_total) raw_total[c].template load_edge<false>(reinterpret_cast<const ER*>(a.g_total) + row * a.H, col / 8, a.H);
+    for (int i = 0; i < 4; ++i) {
+      v[i] = lo[i];
+      v[4 + i] = hi[i];
     }
+  };
+  auto weight = [&](int which, int col, float (&w)[8]) __attribute__((always_inline)) {
+    if constexpr (kAhead) get(2 * which, w);
+    else if (which == kPre) load_either<A, SMALL>(a.w_pre, 0, a.pre_wide, col, a.H, w);
+    else if (which == kPost) load_either<A, SMALL>(a.w_post, 0, a.post_wide, col, a.H, w);
+    else load_either<A, SMALL>(a.gate, 0, a.gate_wide, col, a.H, w);
+  };
+  float sum_pre[8], sum_post[8];  // kAhead: else in `own`
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum_pre[i] = sum_post[i] = 0.f;
+  if constexpr (kAhead) {
+    const NormColumns at(lane, LANES, 0, a.H);
+    float w[8];
+    if (at.have && a.w_pre) {
+      load_either<A, SMALL>(a.w_pre, 0, a.pre_wide, at.col, a.H, w);
+      put(2 * kPre, w);
+    }
+    if (at.have && a.w_post) {
+      load_either<A, SMALL>(a.w_post, 0, a.post_wide, at.col, a.H, w);
+      put(2 * kPost, w);
+    }
+    if (at.have && a.gate_kind == kChannelGate) {
+      load_either<A, SMALL>(a.gate, 0, a.gate_wide, at.col, a.H, w);
+      put(2 * kGate, w);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 2 * C; ++c) put(2 * c, sum_pre);
+  }
+
+  NormRow<A, R, FULL, SMALL> raw[C];
+  const int64_t step = (int64_t)gridDim.x * Shape::kRows;
+  int64_t row = Shape::kRows == 1 ? blockIdx.x : (int64_t)blockIdx.x * Shape::kRows + threadIdx.x / LANES;
+  if constexpr (kAhead) {
+    const NormColumns at(lane, LANES, 0, a.H);
+    if (at.have && row < a.T) raw[0].fetch(a, row, at.col);
+  }
+  for (; row < a.T; row += step, turn ^= 1) {
     const float r1 = a.rstd[row], r2 = a.rstd[a.T + row];
     const float token_gate = a.gate_kind == kTokenGate ? load_one<A>(a.gate, row * a.ld_gate, a.gate_wide) : 1.f;
-    // h2: total, then total * r2; d: g_normed * w_pre, then d_total, then d_u * w_post
-    float h1[C][8], h2[C][8], d[C][8], g[C][8];
+    if constexpr (!kAhead) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const NormColumns at(lane, LANES, c, a.H);
+        if (at.have) raw[c].fetch(a, row, at.col);
+      }
+    }
+    // h1: block * r1 (two vectors: made again from the block where it is used, for want of registers); h2: total, then total * r2;
+    // d: g_normed * w_pre, then d_total, then d_u * w_post
+    float h1[C][8], h2[C][8], d[C][8];
+    auto h1_of = [&](int c, float (&h)[8]) __attribute__((always_inline)) {
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = h1[c][i];
+      } else {
+        raw[c].block.unpack(h);
+        if (a.w_post) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] = h[i] * r1;
+        }
+      }
+    };
+    RowVector<R> raw_total[C];
+    EitherVector<A, SMALL> raw_gate[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const NormColumns at(lane, LANES, c, a.H);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h1[c][i] = h2[c][i] = d[c][i] = 0.f;
+      if (!at.have) continue;
+      raw[c].residual.unpack(h2[c]);
+      if (kAhead && a.block) raw[c].block.unpack(h1[c]);
+      if (a.g_normed) raw[c].normed.unpack(d[c]);
+      if (a.g_total) load8<SMALL>(raw_total[c], reinterpret_cast<const ER*>(a.g_total) + row * a.H, at.col, a.H);
+      if constexpr (FULL) raw_gate[c] = raw[c].gate;
+      if constexpr (kAhead) {
+        __builtin_amdgcn_sched_barrier(0);
+        raw[c].fetch(a, row + step < a.T ? row + step : row, at.col);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    auto gate_of = [&](int c, int col, float (&g)[8]) __attribute__((always_inline)) {
+      if constexpr (FULL) {
+        raw_gate[c].unpack(a.gate_wide, g);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = token_gate;
+        if (a.gate_kind == kChannelGate) weight(kGate, col, g);
+      }
+    };
     float dot[1] = {0.f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int col = (c * THREADS + (int)threadIdx.x) * 8;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        h1[c][i] = h2[c][i] = d[c][i] = 0.f;
-        g[c][i] = token_gate;
-      }
-      if (col >= a.H) continue;
-      raw_residual[c].unpack(h2[c]);
+      const NormColumns at(lane, LANES, c, a.H);
+      if (!at.have) continue;
       if (a.block) {
-        raw_block[c].unpack(h1[c]);
-        if (a.gate_kind == kChannelGate) load_either<A>(a.gate, 0, a.gate_wide, col, a.H, g[c]);
-        if (a.gate_kind == kFullGate) load_either<A>(a.gate, row * a.ld_gate, a.gate_wide, col, a.H, g[c]);
-        float w[8];
+        float g[8], w[8];
+        gate_of(c, at.col, g);
         if (a.w_post) {
-          load_either<A>(a.w_post, 0, a.post_wide, col, a.H, w);
+          weight(kPost, at.col, w);
+          if constexpr (kAhead) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h1[c][i] = h1[c][i] * r1;
+            for (int i = 0; i < 8; ++i) h1[c][i] = h1[c][i] * r1;
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) w[i] = 1.f;
         }
+        float h[8];
+        h1_of(c, h);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h2[c][i] = __builtin_fmaf(a.scale * g[c][i], h1[c][i] * w[i], h2[c][i]);
+        for (int i = 0; i < 8; ++i) h2[c][i] = __builtin_fmaf(a.scale * g[i], h[i] * w[i], h2[c][i]);
       }
       if (a.g_normed) {
-        float w[8];
-        raw_normed[c].unpack(d[c]);
-        load_either<A>(a.w_pre, 0, a.pre_wide, col, a.H, w);
+        float w[8], v[8];
+        weight(kPre, at.col, w);
+        if constexpr (!kAhead) get(4 * c, sum_pre);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           h2[c][i] = h2[c][i] * r2;
-          sum_pre[c][i] = __builtin_fmaf(d[c][i], h2[c][i], sum_pre[c][i]);
+          sum_pre[i] = __builtin_fmaf(d[c][i], h2[c][i], sum_pre[i]);
           d[c][i] = d[c][i] * w[i];
-          dot[0] = __builtin_fmaf(d[c][i], h2[c][i], dot[0]);
         }
+        if constexpr (!kAhead) put(4 * c, sum_pre);
+        at.once(d[c], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot[0] = __builtin_fmaf(v[i], h2[c][i], dot[0]);
       }
     }
-    if (a.g_normed) RowSum<THREADS>::over(dot, slots[turn]);
+    if (a.g_normed) Shape::sum(dot, slots[turn]);
     const float mean = dot[0] * inv_width;
     float sums[2] = {0.f, 0.f};  // of b h1, and of the token gate's gradient
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int col = (c * THREADS + (int)threadIdx.x) * 8;
-      if (col >= a.H) continue;
+      const NormColumns at(lane, LANES, c, a.H);
+      if (!at.have) continue;
       float up[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) up[i] = 0.f;
@@ -267,39 +460,50 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormArgs a) {
       if (a.d_residual) {
         RowVector<R> out;
         out.pack(d[c]);
-        out.template store_edge<false>(reinterpret_cast<ER*>(a.d_residual) + row * a.H, col, a.H);
+        store8<SMALL>(out, reinterpret_cast<ER*>(a.d_residual) + row * a.H, at.col, a.H);
       }
       if (!a.block) continue;
-      float w[8];
+      float w[8], g[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = 1.f;
-      if (a.w_post) load_either<A>(a.w_post, 0, a.post_wide, col, a.H, w);
-      float dg[8];
+      if (a.w_post) weight(kPost, at.col, w);
+      gate_of(c, at.col, g);
+      if constexpr (!kAhead) get(4 * c + 2, sum_post);
+      float dg[8], h[8];
+      h1_of(c, h);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float scaled = a.scale * d[c][i];
-        const float shared = scaled * h1[c][i];
+        const float shared = scaled * h[i];
         dg[i] = shared * w[i];
-        sums[1] = sums[1] + dg[i];
         // a channel gate is the same in every row: it is multiplied to the sum
-        sum_post[c][i] = a.gate_kind == kChannelGate ? sum_post[c][i] + shared : __builtin_fmaf(shared, g[c][i], sum_post[c][i]);
-        d[c][i] = scaled * g[c][i] * w[i];
-        sums[0] = __builtin_fmaf(d[c][i], h1[c][i], sums[0]);
+        sum_post[i] = !FULL && a.gate_kind == kChannelGate ? sum_post[i] + shared : __builtin_fmaf(shared, g[i], sum_post[i]);
+        d[c][i] = scaled * g[i] * w[i];
       }
-      if (a.gate_kind == kFullGate && a.d_gate) {
+      if constexpr (!kAhead) put(4 * c + 2, sum_post);
+      if (FULL && a.d_gate) {
         if (a.gate_wide) {
           RowVector<RLK_DTYPE_FP32> out;
           out.pack(dg);
-          out.store_edge<false>(reinterpret_cast<float*>(a.d_gate) + row * a.H, col, a.H);
+          store8<SMALL>(out, reinterpret_cast<float*>(a.d_gate) + row * a.H, at.col, a.H);
         } else {
           RowVector<A> out;
           out.pack(dg);
-          out.template store_edge<false>(reinterpret_cast<EA*>(a.d_gate) + row * a.H, col, a.H);
+          store8<SMALL>(out, reinterpret_cast<EA*>(a.d_gate) + row * a.H, at.col, a.H);
         }
       }
+      float v[8];
+      at.once(d[c], v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sums[0] = __builtin_fmaf(v[i], h[i], sums[0]);
+      if (token_sum) {
+        at.once(dg, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[1] = sums[1] + v[i];
+      }
     }
-    if (a.w_post || token_sum) RowSum<THREADS>::over(sums, slots[turn] + 1);
-    if (token_sum && threadIdx.x == 0) {
+    if (a.w_post || token_sum) Shape::sum(sums, slots[turn] + 1);
+    if (token_sum && lane == 0) {
       if (a.gate_wide) reinterpret_cast<float*>(a.d_gate)[row] = sums[1];
       else reinterpret_cast<EA*>(a.d_gate)[row] = LogitElem<A>::from_float(sums[1]);
     }
@@ -307,31 +511,55 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormArgs a) {
       const float mean1 = sums[0] * inv_width;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int col = (c * THREADS + (int)threadIdx.x) * 8;
-        if (col >= a.H) continue;
+        const NormColumns at(lane, LANES, c, a.H);
+        if (!at.have) continue;
         if (a.w_post) {
+          float h[8];
+          h1_of(c, h);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[c][i] = r1 * __builtin_fmaf(-h1[c][i], mean1, d[c][i]);
+          for (int i = 0; i < 8; ++i) d[c][i] = r1 * __builtin_fmaf(-h[i], mean1, d[c][i]);
         }
         RowVector<A> out;
         out.pack(d[c]);
-        out.template store_edge<false>(reinterpret_cast<EA*>(a.d_block) + row * a.H, col, a.H);
+        store8<SMALL>(out, reinterpret_cast<EA*>(a.d_block) + row * a.H, at.col, a.H);
       }
     }
   }
+
+  // the workgroup's sums over its rows: those of its rows at a time are added in their order, through `own`
   float* mine = a.part + (int64_t)blockIdx.x * a.H;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int col = (c * THREADS + (int)threadIdx.x) * 8;
-    if (col >= a.H) continue;
-    RowVector<RLK_DTYPE_FP32> out;
-    if (a.sum_pre) {
-      out.pack(sum_pre[c]);
-      out.store_edge<false>(mine, col, a.H);
-    }
-    if (a.sum_post) {
-      out.pack(sum_post[c]);
-      out.store_edge<false>(mine + (int64_t)gridDim.x * a.H, col, a.H);
+  for (int which = 0; which < 2; ++which) {
+    if (which == 0 ? !a.sum_pre : !a.sum_post) continue;
+    float* const to = which == 0 ? mine : mine + (int64_t)gridDim.x * a.H;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const NormColumns at(lane, LANES, c, a.H);
+      float total[8];
+      if constexpr (!kAhead) {
+        get(4 * c + 2 * which, total);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) total[i] = which == 0 ? sum_pre[i] : sum_post[i];
+      }
+      if constexpr (Shape::kRows > 1) {
+        __syncthreads();  // (`own` may still be read)
+        put(0, total);
+        __syncthreads();
+        for (int other = 1; other < Shape::kRows; ++other) {
+          const f32x4_t lo = own[0][other * LANES + lane], hi = own[1][other * LANES + lane];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            total[i] = total[i] + lo[i];
+            total[4 + i] = total[4 + i] + hi[i];
+          }
+        }
+        if (threadIdx.x >= LANES) continue;
+      }
+      if (!at.have) continue;
+      RowVector<RLK_DTYPE_FP32> out;
+      out.pack(total);
+      store8<SMALL>(out, to, at.col, a.H);
     }
   }
 }
@@ -390,37 +618,46 @@ __global__ __launch_bounds__(kSumWaves * kWave) void norm_column_sums_kernel(Nor
 // Host side
 // ---------------------------------------------------------------------------
 
-// Threads of a workgroup: eight columns each up to 8192, in whole waves of a power of two.
-static int norm_threads(int H) {
-  int threads = 64;
-  while (threads < 1024 && threads * 8 < H) threads *= 2;
-  return threads;
+// Threads of a row: eight columns each up to 8192.
+static int norm_lanes(int H) {
+  int lanes = 16;
+  while (lanes < 1024 && lanes * 8 < H) lanes *= 2;
+  return lanes;
 }
 
 // Workgroups of the backward: as many as the chip holds at 16 waves to a compute unit.
 static int norm_groups(int64_t T, int H) {
-  const int64_t most = (int64_t)device_cu_count() * (1024 / norm_threads(H));
-  return (int)(T < most ? T : most);
+  const int lanes = norm_lanes(H), threads = lanes <= kWave ? 256 : lanes;
+  const int64_t most = (int64_t)device_cu_count() * (1024 / threads), all = (T + threads / lanes - 1) / (threads / lanes);
+  return (int)(all < most ? all : most);
 }
 
 size_t block_norm_workspace_bytes(int64_t T, int H) { return T > 0 ? (size_t)2 * norm_groups(T, H) * H * sizeof(float) : 0; }
 
-template <int A, int R, int THREADS, int C>
+template <int A, int R, int LANES, int C, bool SMALL = false>
 static void launch_norm_shape(NormArgs a, bool backward, hipStream_t stream) {
+  using Shape = NormShape<LANES>;
   if (backward) {
-    hipLaunchKernelGGL((norm_backward_kernel<A, R, THREADS, C>), dim3((unsigned)norm_groups(a.T, a.H)), dim3(THREADS), 0, stream, a);
+    const dim3 grid((unsigned)norm_groups(a.T, a.H)), block(Shape::kThreads);
+    if (a.gate_kind == kFullGate) hipLaunchKernelGGL((norm_backward_kernel<A, R, LANES, C, true, SMALL>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((norm_backward_kernel<A, R, LANES, C, false, SMALL>), grid, block, 0, stream, a);
   } else {
-    constexpr int64_t kMost = 0x7fffffff / THREADS;  // (a launch has fewer than 2^32 threads)
-    for (; a.first_row < a.T; a.first_row += kMost) {
-      const int64_t some = a.T - a.first_row < kMost ? a.T - a.first_row : kMost;
-      hipLaunchKernelGGL((norm_forward_kernel<A, R, THREADS, C>), dim3((unsigned)some), dim3(THREADS), 0, stream, a);
+    constexpr int64_t kMost = 0x7fffffff / Shape::kThreads;  // (a launch has fewer than 2^32 threads)
+    for (; a.first_row < a.T; a.first_row += kMost * Shape::kRows) {
+      const int64_t all = (a.T - a.first_row + Shape::kRows - 1) / Shape::kRows;
+      hipLaunchKernelGGL((norm_forward_kernel<A, R, LANES, C, SMALL>), dim3((unsigned)(all < kMost ? all : kMost)), dim3(Shape::kThreads), 0, stream, a);
     }
   }
 }
 
 template <int A, int R>
 static hipError_t launch_norm(const NormArgs& a, bool backward, hipStream_t stream) {
-  switch (norm_threads(a.H)) {
+  switch (norm_lanes(a.H)) {
+    case 16:
+      if (a.H < 8) launch_norm_shape<A, R, 16, 1, true>(a, backward, stream);
+      else launch_norm_shape<A, R, 16, 1>(a, backward, stream);
+      break;
+    case 32: launch_norm_shape<A, R, 32, 1>(a, backward, stream); break;
     case 64: launch_norm_shape<A, R, 64, 1>(a, backward, stream); break;
     case 128: launch_norm_shape<A, R, 128, 1>(a, backward, stream); break;
     case 256: launch_norm_shape<A, R, 256, 1>(a, backward, stream); break;
