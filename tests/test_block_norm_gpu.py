@@ -131,6 +131,16 @@ def test_results_and_gradients(norm, tokens, width, dtype, wide):
     _compare(_run(norm, t, g_total, g_normed), want, t, tokens)
 
 
+@pytest.mark.parametrize("gate", ["channel", "token", "full"])
+@pytest.mark.parametrize("wide", [BF16, FP32])
+@pytest.mark.parametrize("tokens,width", [(40001, 6), (36005, 64), (17003, 128), (9001, 129), (8300, 256), (4200, 301), (2100, 1024), (1100, 2050), (700, 4096), (260, 8190), (259, 16384)])
+def test_rows_that_take_turns(norm, tokens, width, wide, gate):
+    """More rows than the workgroups of a backward take at a time, at both ends of every number of threads to a row."""
+    t, g_total, g_normed = _case(tokens, width, BF16, wide, gate, True, True, seed=width)
+    want = _definition(*(t[k] for k in ("block", "residual", "gate", "post", "pre")), g_total, g_normed)
+    _compare(_run(norm, t, g_total, g_normed), want, t, tokens)
+
+
 @pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("pre", [False, True])
@@ -223,8 +233,9 @@ def test_layouts(norm):
     assert torch.equal(one[0], norm.rms_norm(t["block"], t["pre"])[0])
 
 
-def test_a_row_does_not_depend_on_its_batch(norm):
-    t, g_total, g_normed = _case(3000, 384, BF16, BF16, "token", True, True)
+@pytest.mark.parametrize("width", [20, 130, 384, 1000])
+def test_a_row_does_not_depend_on_its_batch(norm, width):
+    t, g_total, g_normed = _case(3000, width, BF16, BF16, "token", True, True)
     whole = _run(norm, t, g_total, g_normed)
     for rows in (slice(0, 1), slice(2999, 3000), slice(1000, 1077)):
         some = {k: (v if v is None or v.dim() == 1 else v.detach()[rows]) for k, v in t.items()}
