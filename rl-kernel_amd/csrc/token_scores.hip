@@ -24,8 +24,8 @@ namespace rlk {
 
 constexpr int kScoreTiles = 64;
 constexpr int kScoreSlices = kScoreTiles * kTileLanes;
+constexpr int kGroupTiles = 4 * kTilesPerWave;  // of a workgroup: a row has four
 constexpr int kScorePlanes = 4;  // max, sum, target, weighted sum: stats[row][plane][tile]
-
 
 struct ScoreArgs {
   const void* logits;
@@ -35,7 +35,7 @@ struct ScoreArgs {
   float* stats;              // [T][kScorePlanes][kScoreTiles]
   uint32_t* best;   // [T][kScoreSlices] largest logit of the slice (ordered bits), 0 for a slice without columns
   uint32_t* where;  // [T][kScoreSlices] the upper half of the largest logit in its other vectors | number of the first vector that holds the best
-  int T, V, real, tile_size, tiles_per_group;
+  int T, V, real, tile_size;
   int64_t streamed;  // workgroups, in the order of their ids, that read past the caches
 };
 
@@ -109,130 +109,120 @@ __device__ __forceinline__ void merge_score_lanes(int lane, ScoreState& st) {
   st.m = n;
 }
 
-// kBatch: vectors that a lane has on their way. OVERLAP: the exponentials of one vector may run under the folds of another, for
-// which they take registers: for waves that have their SIMD to themselves.
-template <int ELEM, bool HAS_TEMP, bool TOP, int kBatch, bool OVERLAP, bool NT>
+// HBM-bound: 2048 x 131072 bf16 93 us = 5.8 TB/s, with alternatives 105; one row of 151936 7 us, launch and latency. (A form for few rows,
+// one wave to a workgroup and eight vectors of a lane on their way, took 0.3 us less up to 64 rows of 151936 bf16 logits, 0.3 to 2
+// more at the other sizes.)
+template <int ELEM, bool HAS_TEMP, bool TOP, bool NT>
 __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
   using E = typename LogitElem<ELEM>::type;
+  constexpr int kBatch = 4;                   // vectors that a lane has on their way
   constexpr int kStep = kTileLanes * kBatch;  // vectors of a tile per batch
   const int row = blockIdx.x;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int waves = blockDim.x >> 6;
   const int l16 = lane & (kTileLanes - 1);
   const int grp = lane / kTileLanes;
   const E* row_ptr = reinterpret_cast<const E*>(a.logits) + (int64_t)row * a.row_stride;
   const float inv_t = HAS_TEMP ? 1.0f / a.temperature[row] : 1.0f;
-  const int64_t wanted = a.target[row];
-  const int target = wanted >= 0 && wanted < a.real ? (int)wanted : -1;
+  const int tile = blockIdx.y * kGroupTiles + wave * kTilesPerWave + grp;
+  const int64_t lo64 = (int64_t)tile * a.tile_size, hi64 = lo64 + a.tile_size;
+  const int lo_col = lo64 < a.real ? (int)lo64 : a.real;
+  const int hi_col = hi64 < a.real ? (int)hi64 : a.real;
+  const int g0 = lo_col / 8;
+  const int g1 = hi_col > lo_col ? (hi_col + 7) / 8 : g0;
+  const int g_last = g1 > g0 ? g1 - 1 : 0;  // a valid vector to clamp loads to
+  // Batches in which all four vectors of every lane are whole vectors of the lane's tile need no masks, but for the first vector
+  // of a tile, which may start before it.
+  const int g_whole = (hi_col % 8) ? g1 - 1 : g1;
+  const int my_clean = g_whole > g0 ? (g_whole - g0) / kStep : 0;
+  const int my_slots = (g1 - g0 + kTileLanes - 1) / kTileLanes;
+  int clean = __builtin_amdgcn_readlane(my_clean, 0), slots = __builtin_amdgcn_readlane(my_slots, 0);
+#pragma unroll
+  for (int other = kTileLanes; other < kWave; other += kTileLanes) {  // uniform over the wave's four tiles
+    clean = min(clean, __builtin_amdgcn_readlane(my_clean, other));
+    slots = max(slots, __builtin_amdgcn_readlane(my_slots, other));
+  }
 
-  const int tile_first = blockIdx.y * a.tiles_per_group;
-  const int tile_last = min(tile_first + a.tiles_per_group, kScoreTiles);
-  for (int t0 = tile_first + wave * kTilesPerWave; t0 < tile_last; t0 += waves * kTilesPerWave) {
-    const int tile = t0 + grp;  // (a group has a multiple of four tiles)
-    const int64_t lo64 = (int64_t)tile * a.tile_size, hi64 = lo64 + a.tile_size;
-    const int lo_col = lo64 < a.real ? (int)lo64 : a.real;
-    const int hi_col = hi64 < a.real ? (int)hi64 : a.real;
-    const int g0 = lo_col / 8;
-    const int g1 = hi_col > lo_col ? (hi_col + 7) / 8 : g0;
-    const int g_last = g1 > g0 ? g1 - 1 : 0;  // a valid vector to clamp loads to
-    // Batches in which all four vectors of every lane are whole vectors of the lane's tile need no masks, but for the first vector
-    // of a tile, which may start before it.
-    const int g_whole = (hi_col % 8) ? g1 - 1 : g1;
-    const int my_clean = g_whole > g0 ? (g_whole - g0) / kStep : 0;
-    const int my_slots = (g1 - g0 + kTileLanes - 1) / kTileLanes;
-    int clean = __builtin_amdgcn_readlane(my_clean, 0), slots = __builtin_amdgcn_readlane(my_slots, 0);
+  ScoreState st{kNegInf, 0.f, 0.f, kNegInf, kNegInf, g0 + l16};
+  int g = g0 + l16;  // this lane's next vector
+  // The loads rotate through the raw vectors: a vector's registers are free once it is unpacked, and the same vector of the next
+  // batch is fetched into them before the fold, so a lane always has that many loads, or one less, in flight. (Behind the
+  // tile its last vector is fetched again.)
+  RowVector<ELEM> raw[kBatch];
+  auto fetch = [&](int u, int at) __attribute__((always_inline)) {
+    raw[u].template load_window<NT>(row_ptr, (at < g1 ? at : g_last) * 8, a.V);
+  };
+  auto fetch_of_many = [&](int u, int at) __attribute__((always_inline)) {  // of a row that has a window to spare
+    raw[u].template load_at<NT>(row_ptr, (uint32_t)min((at < g1 ? at : g_last) * 8, a.V - 8));
+  };
 #pragma unroll
-    for (int other = kTileLanes; other < kWave; other += kTileLanes) {  // uniform over the wave's four tiles
-      clean = min(clean, __builtin_amdgcn_readlane(my_clean, other));
-      slots = max(slots, __builtin_amdgcn_readlane(my_slots, other));
-    }
-
-    ScoreState st{kNegInf, 0.f, 0.f, kNegInf, kNegInf, g0 + l16};
-    int g = g0 + l16;  // this lane's next vector
-    // The loads rotate through the raw vectors: a vector's registers are free once it is unpacked, and the same vector of the next
-    // batch is fetched into them before the fold, so a lane always has that many loads, or one less, in flight. (Behind the
-    // tile its last vector is fetched again.)
-    RowVector<ELEM> raw[kBatch];
-    auto fetch = [&](int u, int at) __attribute__((always_inline)) {
-      raw[u].template load_window<NT>(row_ptr, (at < g1 ? at : g_last) * 8, a.V);
-    };
-    auto fetch_of_many = [&](int u, int at) __attribute__((always_inline)) {  // of a row that has a window to spare
-      raw[u].template load_at<NT>(row_ptr, (uint32_t)min((at < g1 ? at : g_last) * 8, a.V - 8));
-    };
+  for (int u = 0; u < kBatch; ++u) fetch(u, g + u * kTileLanes);
+  const int64_t target = a.target[row];
+  const bool holds_target = l16 == 0 && target >= lo_col && target < hi_col;
+  E target_logit{};
+  if (holds_target) target_logit = row_ptr[target];
+  int b = 0;
+  for (; b < clean; ++b, g += kStep) {  // without a branch between the folds
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) fetch(u, g + u * kTileLanes);
-    int b = 0;
-    for (; b < clean; ++b, g += kStep) {  // without a branch between the folds
+    for (int u = 0; u < kBatch; ++u) {
+      const int gu = g + u * kTileLanes;
+      float y[8];
+      raw[u].unpack(y);
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_of_many(u, gu + kStep);
+      if (u == 0) {
+        const int lo = lo_col - gu * 8;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int gu = g + u * kTileLanes;
-        float y[8];
-        raw[u].unpack(y);
-        if constexpr (!OVERLAP) __builtin_amdgcn_sched_barrier(0);
-        fetch_of_many(u, gu + kStep);
-        if (u == 0) {
-          const int lo = lo_col - gu * 8;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = i >= lo ? y[i] : kNegInf;
-        }
-        fold_score_vector<HAS_TEMP, TOP>(y, inv_t, gu, st);
-        if constexpr (!OVERLAP) __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < 8; ++i) y[i] = i >= lo ? y[i] : kNegInf;
       }
+      fold_score_vector<HAS_TEMP, TOP>(y, inv_t, gu, st);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    for (; b * kBatch < slots; ++b, g += kStep) {
+  }
+  for (; b * kBatch < slots; ++b, g += kStep) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (b * kBatch + u >= slots) break;
-        const int gu = g + u * kTileLanes;
-        float y[8];
-        raw[u].unpack(y);
-        fetch(u, gu + kStep);
-        const int first = window_of(gu * 8, a.V);
-        const int lo = max(lo_col, gu * 8) - first;  // columns [lo, hi) of the window count: none of a vector behind the tile
-        const int hi = gu < g1 ? min(hi_col, gu * 8 + 8) - first : lo;
+    for (int u = 0; u < kBatch; ++u) {
+      if (b * kBatch + u >= slots) break;
+      const int gu = g + u * kTileLanes;
+      float y[8];
+      raw[u].unpack(y);
+      fetch(u, gu + kStep);
+      const int first = window_of(gu * 8, a.V);
+      const int lo = max(lo_col, gu * 8) - first;  // columns [lo, hi) of the window count: none of a vector behind the tile
+      const int hi = gu < g1 ? min(hi_col, gu * 8 + 8) - first : lo;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (uint32_t)(i - lo) < (uint32_t)(hi - lo) ? y[i] : kNegInf;
-        fold_score_vector<HAS_TEMP, TOP>(y, inv_t, gu, st);  // a vector of -inf changes nothing
-      }
+      for (int i = 0; i < 8; ++i) y[i] = (uint32_t)(i - lo) < (uint32_t)(hi - lo) ? y[i] : kNegInf;
+      fold_score_vector<HAS_TEMP, TOP>(y, inv_t, gu, st);  // a vector of -inf changes nothing
     }
-    if constexpr (TOP) {
-      const int64_t slice = (int64_t)row * kScoreSlices + tile * kTileLanes + l16;
-      a.best[slice] = g0 + l16 < g1 ? ordered_bits(st.raw) : 0u;
-      a.where[slice] = (ordered_bits(st.other) & 0xffff0000u) | (uint32_t)((st.at - g0 - l16) / kTileLanes);
-    }
-    merge_score_lanes<8>(lane, st);
-    merge_score_lanes<4>(lane, st);
-    merge_score_lanes<2>(lane, st);
-    merge_score_lanes<1>(lane, st);
-    if (l16 == 0) {
-      const bool finite = st.m > kNegInf && st.m < -kNegInf;
-      float zt = 0.f;
-      if (target >= lo_col && target < hi_col) {
-        zt = LogitElem<ELEM>::to_float(row_ptr[target]);
-        if (HAS_TEMP) zt = zt * inv_t;
-      }
-      float* out = a.stats + (int64_t)row * kScorePlanes * kScoreTiles + tile;
-      out[0] = st.m;
-      out[kScoreTiles] = finite ? st.s : 0.f;
-      out[2 * kScoreTiles] = zt;
-      out[3 * kScoreTiles] = finite ? st.w : 0.f;
-    }
+  }
+  if constexpr (TOP) {
+    const int64_t slice = (int64_t)row * kScoreSlices + tile * kTileLanes + l16;
+    a.best[slice] = g0 + l16 < g1 ? ordered_bits(st.raw) : 0u;
+    a.where[slice] = (ordered_bits(st.other) & 0xffff0000u) | (uint32_t)((st.at - g0 - l16) / kTileLanes);
+  }
+  merge_score_lanes<8>(lane, st);
+  merge_score_lanes<4>(lane, st);
+  merge_score_lanes<2>(lane, st);
+  merge_score_lanes<1>(lane, st);
+  if (l16 == 0) {
+    const bool finite = st.m > kNegInf && st.m < -kNegInf;
+    float zt = holds_target ? LogitElem<ELEM>::to_float(target_logit) : 0.f;
+    if (HAS_TEMP) zt = holds_target ? zt * inv_t : zt;
+    float* out = a.stats + (int64_t)row * kScorePlanes * kScoreTiles + tile;
+    out[0] = st.m;
+    out[kScoreTiles] = finite ? st.s : 0.f;
+    out[2 * kScoreTiles] = zt;
+    out[3 * kScoreTiles] = finite ? st.w : 0.f;
   }
 }
 
 template <int ELEM, bool HAS_TEMP, bool TOP>
 __global__ __launch_bounds__(256) void score_tiles_kernel(ScoreArgs a) {
   if ((int64_t)blockIdx.y * gridDim.x + blockIdx.x < a.streamed) {
-    score_tiles<ELEM, HAS_TEMP, TOP, 4, false, true>(a);
+    score_tiles<ELEM, HAS_TEMP, TOP, true>(a);
   } else {
-    score_tiles<ELEM, HAS_TEMP, TOP, 4, false, false>(a);
+    score_tiles<ELEM, HAS_TEMP, TOP, false>(a);
   }
-}
-
-template <int ELEM, bool HAS_TEMP, bool TOP>
-__global__ __launch_bounds__(64) void score_few_rows_kernel(ScoreArgs a) {
-  score_tiles<ELEM, HAS_TEMP, TOP, 8, true, false>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -641,7 +631,7 @@ struct LinearRowArgs {
   float* weighted;           // [n_split][T]
   uint32_t* best;            // as in ScoreArgs
   uint32_t* where;
-  int T, V, real, n_split, classes_per_group;
+  int T, V, real, n_split;
 };
 
 template <bool HAS_TEMP, bool TOP>
@@ -649,70 +639,67 @@ __global__ __launch_bounds__(256) void linear_score_rows_kernel(LinearRowArgs a)
   const int row = blockIdx.x;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int waves = blockDim.x >> 6;
   const int l16 = lane & (kTileLanes - 1);
   const float* row_ptr = a.logits + (int64_t)row * a.logits_ld;
   const float inv_t = HAS_TEMP ? 1.0f / a.temperature[row] : 1.0f;
-  const int first_class = blockIdx.y * a.classes_per_group;
-  for (int c0 = first_class + wave * kTilesPerWave; c0 < first_class + a.classes_per_group; c0 += waves * kTilesPerWave) {
-    const int mine = c0 + lane / kTileLanes;  // this lane's class of splits
-    float best = kNegInf, other = kNegInf;
-    int at = 0;
-    for (int base = 0; base + c0 < a.n_split; base += kScoreTiles) {  // uniform
-      const int split = base + mine;
-      const int col0 = split * kLogpSplitCols + l16 * 16;
-      f32x4_t raw[kLogpSplitTiles][4];
+  const int c0 = blockIdx.y * kGroupTiles + wave * kTilesPerWave;
+  const int mine = c0 + lane / kTileLanes;  // this lane's class of splits
+  float best = kNegInf, other = kNegInf;
+  int at = 0;
+  for (int base = 0; base + c0 < a.n_split; base += kScoreTiles) {  // uniform
+    const int split = base + mine;
+    const int col0 = split * kLogpSplitCols + l16 * 16;
+    f32x4_t raw[kLogpSplitTiles][4];
 #pragma unroll
-      for (int t = 0; t < kLogpSplitTiles; ++t) {
-        const int col = col0 + t * kLogpTileCols;
-        if (split < a.n_split && col < a.V) {
+    for (int t = 0; t < kLogpSplitTiles; ++t) {
+      const int col = col0 + t * kLogpTileCols;
+      if (split < a.n_split && col < a.V) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) raw[t][q] = *reinterpret_cast<const f32x4_t*>(row_ptr + col + 4 * q);
-        } else {
+        for (int q = 0; q < 4; ++q) raw[t][q] = *reinterpret_cast<const f32x4_t*>(row_ptr + col + 4 * q);
+      } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) raw[t][q] = f32x4_t{kNegInf, kNegInf, kNegInf, kNegInf};
+        for (int q = 0; q < 4; ++q) raw[t][q] = f32x4_t{kNegInf, kNegInf, kNegInf, kNegInf};
+      }
+    }
+    float m = kNegInf, s = 0.f, w = 0.f, unused = 0.f;
+#pragma unroll
+    for (int t = 0; t < kLogpSplitTiles; ++t) {
+      const int col = col0 + t * kLogpTileCols;
+      float y[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) y[c] = col + c < a.real ? raw[t][c / 4][c % 4] : kNegInf;
+      if constexpr (TOP) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float* v = y + 8 * h;
+          const float here = max3_f32(max3_f32(max3_f32(max3_f32(v[0], v[1], v[2]), v[3], v[4]), v[5], v[6]), v[7], v[7]);
+          at = here > best ? base / kScoreTiles * 8 + 2 * t + h : at;
+          other = __builtin_amdgcn_fmed3f(here, best, other);
+          best = fmaxf(best, here);
         }
       }
-      float m = kNegInf, s = 0.f, w = 0.f, unused = 0.f;
+      if constexpr (HAS_TEMP) {
 #pragma unroll
-      for (int t = 0; t < kLogpSplitTiles; ++t) {
-        const int col = col0 + t * kLogpTileCols;
-        float y[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) y[c] = col + c < a.real ? raw[t][c / 4][c % 4] : kNegInf;
-        if constexpr (TOP) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float* v = y + 8 * h;
-            const float here = max3_f32(max3_f32(max3_f32(max3_f32(v[0], v[1], v[2]), v[3], v[4]), v[5], v[6]), v[7], v[7]);
-            at = here > best ? base / kScoreTiles * 8 + 2 * t + h : at;
-            other = __builtin_amdgcn_fmed3f(here, best, other);
-            best = fmaxf(best, here);
-          }
-        }
-        if constexpr (HAS_TEMP) {
-#pragma unroll
-          for (int c = 0; c < 16; ++c) y[c] = y[c] * inv_t;
-        }
-        logp_fold_run_weighted(y, -1, m, s, w, unused);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int c = 0; c < 16; ++c) y[c] = y[c] * inv_t;
       }
-      float big = fmaxf(m, xor_lane<1>(m));
-      big = fmaxf(big, xor_lane<2>(big));
-      big = fmaxf(big, xor_lane<4>(big));
-      big = fmaxf(big, xor_lane<8>(big));
-      float sum = logp_weighted_term(m, s, w, big);
-      sum = sum + xor_lane<1>(sum);
-      sum = sum + xor_lane<2>(sum);
-      sum = sum + xor_lane<4>(sum);
-      sum = sum + xor_lane<8>(sum);
-      if (l16 == 0 && split < a.n_split) a.weighted[(int64_t)split * a.T + row] = sum;
+      logp_fold_run_weighted(y, -1, m, s, w, unused);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (TOP) {
-      const int64_t slice = (int64_t)row * kScoreSlices + mine * kTileLanes + l16;
-      a.best[slice] = mine * kLogpSplitCols + l16 * 16 < a.real ? ordered_bits(best) : 0u;
-      a.where[slice] = (ordered_bits(other) & 0xffff0000u) | (uint32_t)at;
-    }
+    float big = fmaxf(m, xor_lane<1>(m));
+    big = fmaxf(big, xor_lane<2>(big));
+    big = fmaxf(big, xor_lane<4>(big));
+    big = fmaxf(big, xor_lane<8>(big));
+    float sum = logp_weighted_term(m, s, w, big);
+    sum = sum + xor_lane<1>(sum);
+    sum = sum + xor_lane<2>(sum);
+    sum = sum + xor_lane<4>(sum);
+    sum = sum + xor_lane<8>(sum);
+    if (l16 == 0 && split < a.n_split) a.weighted[(int64_t)split * a.T + row] = sum;
+  }
+  if constexpr (TOP) {
+    const int64_t slice = (int64_t)row * kScoreSlices + mine * kTileLanes + l16;
+    a.best[slice] = mine * kLogpSplitCols + l16 * 16 < a.real ? ordered_bits(best) : 0u;
+    a.where[slice] = (ordered_bits(other) & 0xffff0000u) | (uint32_t)at;
   }
 }
 
@@ -838,19 +825,18 @@ size_t token_scores_workspace_bytes(int T, int top_k) {
 }
 
 template <int ELEM, bool HAS_TEMP, bool TOP>
-static void launch_score_tiles(const ScoreArgs& a, bool few, hipStream_t stream) {
-  const dim3 grid((unsigned)a.T, (unsigned)(kScoreTiles / a.tiles_per_group));
-  if (few) hipLaunchKernelGGL((score_few_rows_kernel<ELEM, HAS_TEMP, TOP>), grid, dim3(64), 0, stream, a);
-  else hipLaunchKernelGGL((score_tiles_kernel<ELEM, HAS_TEMP, TOP>), grid, dim3(256), 0, stream, a);
+static void launch_score_tiles(const ScoreArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)a.T, kScoreTiles / kGroupTiles);
+  hipLaunchKernelGGL((score_tiles_kernel<ELEM, HAS_TEMP, TOP>), grid, dim3(256), 0, stream, a);
 }
 
 template <int ELEM>
-static hipError_t token_scores_typed(const ScoreArgs& a, bool few, const ScoreFinishArgs& f, hipStream_t stream) {
+static hipError_t token_scores_typed(const ScoreArgs& a, const ScoreFinishArgs& f, hipStream_t stream) {
   const bool temp = a.temperature != nullptr, top = f.top_k > 0;
-  if (temp && top) launch_score_tiles<ELEM, true, true>(a, few, stream);
-  else if (top) launch_score_tiles<ELEM, false, true>(a, few, stream);
-  else if (temp) launch_score_tiles<ELEM, true, false>(a, few, stream);
-  else launch_score_tiles<ELEM, false, false>(a, few, stream);
+  if (temp && top) launch_score_tiles<ELEM, true, true>(a, stream);
+  else if (top) launch_score_tiles<ELEM, false, true>(a, stream);
+  else if (temp) launch_score_tiles<ELEM, true, false>(a, stream);
+  else launch_score_tiles<ELEM, false, false>(a, stream);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   hipLaunchKernelGGL((score_finish_kernel<ELEM, false>), dim3((a.T + kFinishWaves - 1) / kFinishWaves), dim3(kFinishWaves * kWave), 0, stream, f);
@@ -871,19 +857,14 @@ hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride
   a.V = V;
   a.real = real;
   a.tile_size = (int)(((int64_t)V + kScoreTiles - 1) / kScoreTiles);
-  // Few rows: a wave to a workgroup, four tiles each, so that a row has sixteen compute units.
-  const bool few = T <= 128;
-  a.tiles_per_group = few ? kTilesPerWave : kScoreTiles;
-  while (!few && (int64_t)T * (kScoreTiles / a.tiles_per_group) < 16384 && a.tiles_per_group > 16) a.tiles_per_group /= 2;
-  const int groups = kScoreTiles / a.tiles_per_group;
   const int64_t bytes = (int64_t)T * V * (dtype == RLK_DTYPE_FP32 ? 4 : 2);
-  a.streamed = bytes > kCachedLogitsBytes ? (int64_t)((double)T * groups * (1.0 - (double)kCachedLogitsBytes / bytes)) : 0;
+  a.streamed = bytes > kCachedLogitsBytes ? (int64_t)((double)T * (kScoreTiles / kGroupTiles) * (1.0 - (double)kCachedLogitsBytes / bytes)) : 0;
   const ScoreFinishArgs f{logits, row_stride, target, temperature, nullptr, a.stats, a.best, a.where, logp, lse, entropy,
                           top_logp, top_ids, T, V, real, a.tile_size, top_k, nullptr, nullptr, 0};
   switch (dtype) {
-    case RLK_DTYPE_BF16: return token_scores_typed<RLK_DTYPE_BF16>(a, few, f, stream);
-    case RLK_DTYPE_FP16: return token_scores_typed<RLK_DTYPE_FP16>(a, few, f, stream);
-    case RLK_DTYPE_FP32: return token_scores_typed<RLK_DTYPE_FP32>(a, few, f, stream);
+    case RLK_DTYPE_BF16: return token_scores_typed<RLK_DTYPE_BF16>(a, f, stream);
+    case RLK_DTYPE_FP16: return token_scores_typed<RLK_DTYPE_FP16>(a, f, stream);
+    case RLK_DTYPE_FP32: return token_scores_typed<RLK_DTYPE_FP32>(a, f, stream);
     default: return hipErrorInvalidValue;
   }
 }
@@ -900,10 +881,8 @@ hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const fl
   uint32_t* best = reinterpret_cast<uint32_t*>((reinterpret_cast<uintptr_t>(weighted + (size_t)n_split * T) + 15) / 16 * 16);
   uint32_t* where = best + (size_t)T * kScoreSlices;
   if (!have_weighted || top_k > 0) {
-    const bool few = T <= 128;
-    LinearRowArgs a{logits, logits_ld, temperature, weighted, best, where, T, V, real, n_split, few ? kTilesPerWave : kScoreTiles};
-    while (!few && (int64_t)T * (kScoreTiles / a.classes_per_group) < 16384 && a.classes_per_group > 16) a.classes_per_group /= 2;
-    const dim3 grid((unsigned)T, (unsigned)(kScoreTiles / a.classes_per_group)), block(few ? 64 : 256);
+    LinearRowArgs a{logits, logits_ld, temperature, weighted, best, where, T, V, real, n_split};
+    const dim3 grid((unsigned)T, kScoreTiles / kGroupTiles), block(256);
     if (temperature && top_k > 0) hipLaunchKernelGGL((linear_score_rows_kernel<true, true>), grid, block, 0, stream, a);
     else if (temperature) hipLaunchKernelGGL((linear_score_rows_kernel<true, false>), grid, block, 0, stream, a);
     else if (top_k > 0) hipLaunchKernelGGL((linear_score_rows_kernel<false, true>), grid, block, 0, stream, a);
