@@ -564,7 +564,8 @@ __global__ __launch_bounds__(NormShape<LANES>::kThreads) __attribute__((amdgpu_w
   }
 }
 
-// The sums over rows: column by column, 16 waves of a workgroup take every 16th of the G parts, then ascending over the waves.
+// The sums over rows: column by column, 16 waves of a workgroup take every 16th of the G parts, then ascending over the waves
+// (512 parts of 4096 columns, both sums: 5 us).
 // Sum 1 is that of scale d_total h1 under a channel gate, which times the gate is d w_post and times w_post d_gate; else d w_post.
 struct NormSumArgs {
   const float* part;  // [2][G][H]
@@ -645,7 +646,8 @@ static void launch_norm_shape(NormArgs a, bool backward, hipStream_t stream) {
     constexpr int64_t kMost = 0x7fffffff / Shape::kThreads;  // (a launch has fewer than 2^32 threads)
     for (; a.first_row < a.T; a.first_row += kMost * Shape::kRows) {
       const int64_t all = (a.T - a.first_row + Shape::kRows - 1) / Shape::kRows;
-      hipLaunchKernelGGL((norm_forward_kernel<A, R, LANES, C, SMALL>), dim3((unsigned)(all < kMost ? all : kMost)), dim3(Shape::kThreads), 0, stream, a);
+      const dim3 grid((unsigned)(all < kMost ? all : kMost)), block(Shape::kThreads);
+      hipLaunchKernelGGL((norm_forward_kernel<A, R, LANES, C, SMALL>), grid, block, 0, stream, a);
     }
   }
 }

