@@ -386,24 +386,15 @@ __device__ __forceinline__ void tile_columns(const ScoreFinishArgs& a, int tile,
 }
 
 template <int ELEM, bool LINEAR>
-__device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, int row, int lane, float lse, float inv_t,
-                                                    uint64_t* keys, uint32_t* picked) {
+__device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, int row, int lane, const uint32_t (&most)[kTileLanes],
+                                                    const uint32_t (&at)[kTileLanes], float lse, float inv_t, uint64_t* keys,
+                                                    uint32_t* picked, uint32_t* where) {
   using E = typename LogitElem<ELEM>::type;
   const int k = a.top_k;
   constexpr int kEach = kScoreSlices / kWave;  // a lane has the sixteen slices of one tile
   static_assert(kEach == kTileLanes, "a lane per tile");
-  uint32_t most[kEach], at[kEach];
-  const u32x4_t* best = reinterpret_cast<const u32x4_t*>(a.best + (int64_t)row * kScoreSlices + lane * kEach);
-  const u32x4_t* where = reinterpret_cast<const u32x4_t*>(a.where + (int64_t)row * kScoreSlices + lane * kEach);
 #pragma unroll
-  for (int i = 0; i < kEach / 4; ++i) {
-    const u32x4_t v = best[i], w = where[i];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      most[4 * i + e] = v[e];
-      at[4 * i + e] = w[e];
-    }
-  }
+  for (int i = 0; i < kEach; ++i) where[i * kWave + lane] = at[i];
   auto count_from = [&](uint32_t limit) __attribute__((always_inline)) {
     int count = 0;
 #pragma unroll
@@ -446,20 +437,31 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
     last_at = first;
     floor |= 0xffffffffu - min((uint64_t)0xffffffffu, (uint64_t)last_at * 8 + 7);
   }
-  // Of a picked slice its best vector is read, from the front of the list on, or all of it, from the back.
-  int singles = 0, wholes = 0;
+  // Of a picked slice its best vector is read, from the front of the list on, or all of it, from the back. The wave takes one slice of
+  // each lane at a time, which leaves two or three turns of a short loop: straight code for all sixteen took 1.7 us a row, most of it to
+  // be fetched.
+  uint32_t takes = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const uint32_t g = (uint32_t)slice_vector<LINEAR>(a, lane, i, at[i] & 0xffffu);
-    const bool take = most[i] >= low && (most[i] >> kIdle != low >> kIdle || g <= last_at);
-    const uint64_t mask = __ballot(take);
-    if (mask == 0) continue;
-    const bool whole = at[i] >> 16 >= low >> 16;  // another of its vectors may reach the limit
-    const uint64_t whole_mask = __ballot(take && whole);
-    if (take && !whole) picked[singles + lanes_below(mask & ~whole_mask)] = (uint32_t)(lane << 26) | g;
-    if (take && whole) picked[kFinishPicked - 1 - (wholes + lanes_below(whole_mask))] = (uint32_t)(lane * kEach + i);
-    singles += __popcll(mask & ~whole_mask);
+  for (int i = 0; i < kEach; ++i) takes |= most[i] >= low ? 1u << i : 0u;
+  if (last_at != 0xffffffffu) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (most[i] >> kIdle == low >> kIdle && (uint32_t)slice_vector<LINEAR>(a, lane, i, at[i] & 0xffffu) > last_at) takes &= ~(1u << i);
+  }
+  int singles = 0, wholes = 0;
+#pragma unroll 1
+  while (__ballot(takes != 0) != 0) {
+    const int i = __builtin_ctz(takes | 1u << (kEach - 1));
+    const uint32_t v = where[i * kWave + lane];
+    const bool whole = v >> 16 >= low >> 16;  // another of its vectors may reach the limit
+    const uint64_t single_mask = __ballot(takes != 0 && !whole), whole_mask = __ballot(takes != 0 && whole);
+    if (takes != 0) {
+      if (whole) picked[kFinishPicked - 1 - (wholes + lanes_below(whole_mask))] = (uint32_t)(lane * kEach + i);
+      else picked[singles + lanes_below(single_mask)] = (uint32_t)lane << 26 | (uint32_t)slice_vector<LINEAR>(a, lane, i, v & 0xffffu);
+    }
+    singles += __popcll(single_mask);
     wholes += __popcll(whole_mask);
+    takes &= takes - 1;
   }
   wave_lds_sync();
 
@@ -539,20 +541,25 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
     n = k;
   }
 
+  // A key's rank is the number of larger ones: all of them read from LDS, four at a time, the same for every lane.
+  if (lane < 4) keys[n + lane] = 0;
+  wave_lds_sync();
   uint64_t mine[2];
   int rank[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < 2; ++i) mine[i] = i * kWave + lane < n ? keys[i * kWave + lane] : 0;
-  auto rank_against = [&](uint64_t of, int count) __attribute__((always_inline)) {
-    for (int j = 0; j < count; ++j) {
-      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(of >> 32), j) << 32 |
-                             (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)of, j);
+  auto rank_all = [&](auto both) __attribute__((always_inline)) {
+    for (int j = 0; j < n; j += 4) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) rank[i] += other > mine[i] ? 1 : 0;
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t other = keys[j + e];
+        rank[0] += other > mine[0] ? 1 : 0;
+        if constexpr (decltype(both)::value) rank[1] += other > mine[1] ? 1 : 0;
+      }
     }
   };
-  rank_against(mine[0], min(n, kWave));
-  rank_against(mine[1], max(n - kWave, 0));
+  if (n <= kWave) rank_all(BoolConstant<false>{});
+  else rank_all(BoolConstant<true>{});
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     if (i * kWave + lane >= n || rank[i] >= k) continue;
@@ -570,10 +577,25 @@ template <int ELEM, bool LINEAR>
 __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(ScoreFinishArgs a) {
   __shared__ uint64_t keys[kFinishWaves][kFinishKeys];
   __shared__ uint32_t picked[kFinishWaves][kFinishPicked];
+  __shared__ uint32_t slices[kFinishWaves][kScoreSlices];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x * kFinishWaves + wave;
   if (row >= a.T) return;  // (waves share nothing)
+  uint32_t most[kTileLanes], at[kTileLanes];  // on their way while the tiles are merged
+  if (a.top_k > 0) {
+    const u32x4_t* best = reinterpret_cast<const u32x4_t*>(a.best + (int64_t)row * kScoreSlices + lane * kTileLanes);
+    const u32x4_t* where = reinterpret_cast<const u32x4_t*>(a.where + (int64_t)row * kScoreSlices + lane * kTileLanes);
+#pragma unroll
+    for (int i = 0; i < kTileLanes / 4; ++i) {
+      const u32x4_t v = best[i], w = where[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        most[4 * i + e] = v[e];
+        at[4 * i + e] = w[e];
+      }
+    }
+  }
   const float temperature = a.temperature ? a.temperature[row] : 1.0f;
   const bool bad_temperature = !(temperature > 0.f);
   const float nan = __builtin_nanf("");
@@ -614,7 +636,7 @@ __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(Scor
       a.logp[row] = bad_target ? nan : zt - lse;
     }
   }
-  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, lse, a.temperature ? 1.0f / temperature : 1.0f, keys[wave], picked[wave]);
+  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, most, at, lse, a.temperature ? 1.0f / temperature : 1.0f, keys[wave], picked[wave], slices[wave]);
 }
 
 // ---------------------------------------------------------------------------
