@@ -179,21 +179,20 @@ __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  for (; b * kBatch < slots; ++b, g += kStep) {
+  // The rest, mostly what is on its way, a vector at a time: the loads move up through the registers.
+#pragma unroll 1
+  for (int slot = b * kBatch; slot < slots; ++slot, g += kTileLanes) {
+    float y[8];
+    raw[0].unpack(y);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      if (b * kBatch + u >= slots) break;
-      const int gu = g + u * kTileLanes;
-      float y[8];
-      raw[u].unpack(y);
-      fetch(u, gu + kStep);
-      const int first = window_of(gu * 8, a.V);
-      const int lo = max(lo_col, gu * 8) - first;  // columns [lo, hi) of the window count: none of a vector behind the tile
-      const int hi = gu < g1 ? min(hi_col, gu * 8 + 8) - first : lo;
+    for (int u = 0; u + 1 < kBatch; ++u) raw[u] = raw[u + 1];
+    if (slot + kBatch < slots) fetch(kBatch - 1, g + kStep);
+    const int first = window_of(g * 8, a.V);
+    const int lo = max(lo_col, g * 8) - first;  // columns [lo, hi) of the window count: none of a vector behind the tile
+    const int hi = g < g1 ? min(hi_col, g * 8 + 8) - first : lo;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = (uint32_t)(i - lo) < (uint32_t)(hi - lo) ? y[i] : kNegInf;
-      fold_score_vector<HAS_TEMP, TOP>(y, inv_t, gu, st);  // a vector of -inf changes nothing
-    }
+    for (int i = 0; i < 8; ++i) y[i] = (uint32_t)(i - lo) < (uint32_t)(hi - lo) ? y[i] : kNegInf;
+    fold_score_vector<HAS_TEMP, TOP>(y, inv_t, g, st);  // a vector of -inf changes nothing
   }
   if constexpr (TOP) {
     const int64_t slice = (int64_t)row * kScoreSlices + tile * kTileLanes + l16;
