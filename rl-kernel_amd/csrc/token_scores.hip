@@ -464,73 +464,69 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   }
   wave_lds_sync();
 
-  // The vectors, a lane each, some of a lane's on their way while as many are looked at. An element costs a comparison with the
-  // floor's logit; a lane's candidates of a vector are the bits of a mask, and the wave takes one of each lane at a time.
+  // The vectors, a lane each, one on its way while one is looked at. (Four on their way took four times the code: 0.8 us more for one
+  // row, nothing less for 2048.) An element costs a comparison with the floor's logit; a lane's candidates of a vector are the bits of a
+  // mask, and the wave takes one of each lane at a time.
   const E* row_ptr = reinterpret_cast<const E*>(a.logits) + (int64_t)row * a.row_stride;
   // vectors of a slice, at most (2^28 / 64 / 128 + 1)
   const int rounds = LINEAR ? (a.n_split + kScoreTiles - 1) / kScoreTiles * 8 : ((a.tile_size + 14) / 8 + kTileLanes - 1) / kTileLanes;
   const uint32_t jobs = (uint32_t)(singles + wholes * rounds);
-  constexpr int kAhead = 4;
-  RowVector<ELEM> next[kAhead];
-  int next_first[kAhead];  // the window's first column, and which of its eight are the slice's, as bits
-  uint32_t next_of[kAhead];
+  RowVector<ELEM> next;
+  int next_first = 0;    // the window's first column,
+  uint32_t next_of = 0;  // and which of its eight are the slice's, as bits
   int n = 0;
   float least = low > ordered_bits(kNegInf) ? from_ordered_bits(low) : kNegInf;  // the floor's logit
-  for (uint32_t first = 0; first < jobs + kAhead * kWave; first += kAhead * kWave) {  // (the first turn only loads, the last only looks)
+  for (uint32_t first = 0; first < jobs + kWave; first += kWave) {  // (the first turn only loads, the last only looks)
+    float y[8];
+    uint32_t mine = 0;
+    const int from = next_first;
+    if (first > 0) {
+      next.unpack(y);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      float y[8];
-      uint32_t mine = 0;
-      const int from = next_first[u];
-      if (first > 0) {
-        next[u].unpack(y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          y[i] = fmaxf(y[i], kNegInf);  // (a NaN counts as -inf)
-          mine |= y[i] >= least ? 1u << i : 0u;
-        }
-        mine &= next_of[u];
+      for (int i = 0; i < 8; ++i) {
+        y[i] = fmaxf(y[i], kNegInf);  // (a NaN counts as -inf)
+        mine |= y[i] >= least ? 1u << i : 0u;
       }
-      const uint32_t job = first + u * kWave + lane;
-      next_of[u] = 0;
-      next_first[u] = 0;
-      if (job < jobs) {
-        int tile, g;
-        if (job < (uint32_t)singles) {
-          tile = picked[job] >> 26;
-          g = picked[job] & 0x3ffffffu;
-        } else {
-          const uint32_t rest = job - singles, slice = picked[kFinishPicked - 1 - rest / (uint32_t)rounds];
-          tile = slice / kTileLanes;
-          g = slice_vector<LINEAR>(a, tile, slice % kTileLanes, rest % (uint32_t)rounds);
-        }
-        int lo_col, hi_col;
-        tile_columns<LINEAR>(a, tile, lo_col, hi_col);
-        if ((int64_t)g * 8 < hi_col) {
-          const int at = window_of(g * 8, a.V);
-          const int lo = max(lo_col, g * 8) - at, hi = min(hi_col, g * 8 + 8) - at;
-          next_of[u] = (1u << hi) - (1u << lo);
-          next_first[u] = at;
-          next[u].template load_window<false>(row_ptr, at, a.V);
-        }
+      mine &= next_of;
+    }
+    const uint32_t job = first + lane;
+    next_of = 0;
+    if (job < jobs) {
+      int tile, g;
+      if (job < (uint32_t)singles) {
+        tile = picked[job] >> 26;
+        g = picked[job] & 0x3ffffffu;
+      } else {
+        const uint32_t rest = job - singles, slice = picked[kFinishPicked - 1 - rest / (uint32_t)rounds];
+        tile = slice / kTileLanes;
+        g = slice_vector<LINEAR>(a, tile, slice % kTileLanes, rest % (uint32_t)rounds);
       }
-      while (__ballot(mine != 0) != 0) {
-        const int i = __builtin_ctz(mine | 256u);
-        float v = y[0];
+      int lo_col, hi_col;
+      tile_columns<LINEAR>(a, tile, lo_col, hi_col);
+      if ((int64_t)g * 8 < hi_col) {
+        const int at = window_of(g * 8, a.V);
+        const int lo = max(lo_col, g * 8) - at, hi = min(hi_col, g * 8 + 8) - at;
+        next_of = (1u << hi) - (1u << lo);
+        next_first = at;
+        next.template load_window<false>(row_ptr, at, a.V);
+      }
+    }
+    while (__ballot(mine != 0) != 0) {
+      const int i = __builtin_ctz(mine | 256u);
+      float v = y[0];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) v = i == e ? y[e] : v;
-        const uint64_t key = (uint64_t)ordered_bits(v) << 32 | (0xffffffffu - (uint32_t)(from + i));
-        const bool take = mine != 0 && key >= floor;
-        const uint64_t mask = __ballot(take);
-        if (take) keys[n + lanes_below(mask)] = key;
-        n += __popcll(mask);
-        mine &= mine - 1;
-        if (n > kFinishKeys - kWave) {
-          wave_lds_sync();
-          floor = keep_largest<ELEM>(keys, n, k, lane, low, high, a.V);
-          least = from_ordered_bits((uint32_t)(floor >> 32));
-          n = k;
-        }
+      for (int e = 1; e < 8; ++e) v = i == e ? y[e] : v;
+      const uint64_t key = (uint64_t)ordered_bits(v) << 32 | (0xffffffffu - (uint32_t)(from + i));
+      const bool take = mine != 0 && key >= floor;
+      const uint64_t mask = __ballot(take);
+      if (take) keys[n + lanes_below(mask)] = key;
+      n += __popcll(mask);
+      mine &= mine - 1;
+      if (n > kFinishKeys - kWave) {
+        wave_lds_sync();
+        floor = keep_largest<ELEM>(keys, n, k, lane, low, high, a.V);
+        least = from_ordered_bits((uint32_t)(floor >> 32));
+        n = k;
       }
     }
   }
@@ -570,8 +566,8 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   }
 }
 
-// 2048 rows: 3 us, 20 with 64 alternatives (17 MB of slices, then two lines of logits for each of some 80 vectors of a row); one row: 2 us,
-// 8 with 20 alternatives, a chain of dependent reads and searches.
+// 2048 rows: 3 us, 17 with 64 alternatives (17 MB of slices, then two lines of logits for each of some 80 vectors of a row); one row: 2 us,
+// 5 with 20 alternatives, a chain of dependent reads and searches whose code is fetched as it is run: short loops throughout.
 template <int ELEM, bool LINEAR>
 __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(ScoreFinishArgs a) {
   __shared__ uint64_t keys[kFinishWaves][kFinishKeys];
