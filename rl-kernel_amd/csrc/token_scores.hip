@@ -225,7 +225,8 @@ __global__ __launch_bounds__(256) void score_tiles_kernel(ScoreArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// A wave per row: the tiles of the row merged, and its alternatives.
+// A wave per row, a workgroup of its own (four to a workgroup: 1 us more at 16 to 64 rows, the same at 2048): the tiles of the row merged, and
+// its alternatives.
 // ---------------------------------------------------------------------------
 
 // LINEAR: from the partials and stored logits of the fused linear-LogP, see below.
@@ -249,7 +250,6 @@ struct ScoreFinishArgs {
   int n_split;
 };
 
-constexpr int kFinishWaves = 4;
 constexpr int kFinishKeys = 512;     // candidates that are held at a time
 constexpr int kFinishPicked = 128;   // slices
 constexpr int kScoreMostTop = 64;
@@ -569,14 +569,12 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
 // 2048 rows: 3 us, 17 with 64 alternatives (17 MB of slices, then two lines of logits for each of some 80 vectors of a row); one row: 2 us,
 // 5 with 20 alternatives, a chain of dependent reads and searches whose code is fetched as it is run: short loops throughout.
 template <int ELEM, bool LINEAR>
-__global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(ScoreFinishArgs a) {
-  __shared__ uint64_t keys[kFinishWaves][kFinishKeys];
-  __shared__ uint32_t picked[kFinishWaves][kFinishPicked];
-  __shared__ uint32_t slices[kFinishWaves][kScoreSlices];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = blockIdx.x * kFinishWaves + wave;
-  if (row >= a.T) return;  // (waves share nothing)
+__global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) {
+  __shared__ uint64_t keys[kFinishKeys];
+  __shared__ uint32_t picked[kFinishPicked];
+  __shared__ uint32_t slices[kScoreSlices];
+  const int lane = threadIdx.x;
+  const int row = blockIdx.x;
   uint32_t most[kTileLanes], at[kTileLanes];  // on their way while the tiles are merged
   if (a.top_k > 0) {
     const u32x4_t* best = reinterpret_cast<const u32x4_t*>(a.best + (int64_t)row * kScoreSlices + lane * kTileLanes);
@@ -631,7 +629,7 @@ __global__ __launch_bounds__(kFinishWaves * kWave) void score_finish_kernel(Scor
       a.logp[row] = bad_target ? nan : zt - lse;
     }
   }
-  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, most, at, lse, a.temperature ? 1.0f / temperature : 1.0f, keys[wave], picked[wave], slices[wave]);
+  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, most, at, lse, a.temperature ? 1.0f / temperature : 1.0f, keys, picked, slices);
 }
 
 // ---------------------------------------------------------------------------
@@ -859,7 +857,7 @@ static hipError_t token_scores_typed(const ScoreArgs& a, const ScoreFinishArgs& 
   else launch_score_tiles<ELEM, false, false>(a, stream);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL((score_finish_kernel<ELEM, false>), dim3((a.T + kFinishWaves - 1) / kFinishWaves), dim3(kFinishWaves * kWave), 0, stream, f);
+  hipLaunchKernelGGL((score_finish_kernel<ELEM, false>), dim3((unsigned)a.T), dim3(kWave), 0, stream, f);
   return hipGetLastError();
 }
 
@@ -913,7 +911,7 @@ hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const fl
   }
   const ScoreFinishArgs f{logits, logits_ld, nullptr, temperature, lse, nullptr, best, where, nullptr, nullptr, entropy,
                           top_logp, top_ids, T, V, real, 0, top_k, part, weighted, n_split};
-  hipLaunchKernelGGL((score_finish_kernel<RLK_DTYPE_FP32, true>), dim3((T + kFinishWaves - 1) / kFinishWaves), dim3(kFinishWaves * kWave), 0,
+  hipLaunchKernelGGL((score_finish_kernel<RLK_DTYPE_FP32, true>), dim3((unsigned)T), dim3(kWave), 0,
                      stream, f);
   return hipGetLastError();
 }
