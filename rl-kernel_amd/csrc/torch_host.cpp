@@ -413,9 +413,10 @@ variable_list tensors_of(const PyRef& tuple, int count) {
   return out;
 }
 
-// Whether a gradient of the backward that runs, from this node on, reaches a node that was made on another stream. Outside of graph
-// capture the engine lets that stream wait; in one it cannot, so such a backward goes to the general functions, which refuse it.
-bool crosses_streams() {
+// Whether a gradient of the backward that runs, on a stream of its own, reaches from this node on one that was made on the default
+// stream. The engine lets that stream wait for the gradient. Under graph capture another stream thereby joins the capture, which the
+// default stream cannot, so such a backward goes to the general functions, which refuse it there.
+bool reaches_default_stream() {
   const std::shared_ptr<torch::autograd::Node> start = torch::autograd::get_current_node();
   if (start == nullptr) return false;
   const auto* const wanted = torch::autograd::get_current_graph_task_exec_info();  // null or empty: all nodes
@@ -432,13 +433,16 @@ bool crosses_streams() {
         if (at == wanted->end() || !at->second.should_execute()) continue;
       }
       const std::optional<c10::Stream> stream = next->stream();
-      if (stream.has_value() && *stream != c10::impl::VirtualGuardImpl(stream->device_type()).getStream(stream->device())) return true;
+      if (stream.has_value()) {
+        const c10::impl::VirtualGuardImpl impl(stream->device_type());
+        if (*stream == impl.getDefaultStream(stream->device()) && *stream != impl.getStream(stream->device())) return true;
+      }
       open.push_back(next);
     }
   }
   return false;
 }
-bool leaves_capture() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None && crosses_streams(); }
+bool leaves_capture() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None && reaches_default_stream(); }
 
 struct ScoreInputs {
   Tensor logits, target, temp;
@@ -912,10 +916,10 @@ PyObject* py_scores(PyObject*, PyObject* const* args, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
-// crosses_streams() -> whether a gradient of the backward that runs reaches a node that was made on another stream
-PyObject* py_crosses_streams(PyObject*, PyObject*) {
+// reaches_default_stream() -> whether a gradient of the backward that runs, on another stream, reaches a node made on the default one
+PyObject* py_reaches_default_stream(PyObject*, PyObject*) {
   HANDLE_TH_ERRORS
-  return PyBool_FromLong(crosses_streams());
+  return PyBool_FromLong(reaches_default_stream());
   END_HANDLE_TH_ERRORS
 }
 
@@ -1096,7 +1100,7 @@ PyMethodDef methods[] = {
     {"ffn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_ffn)), METH_FASTCALL, nullptr},
     {"grpo", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_grpo)), METH_FASTCALL, nullptr},
     {"scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_scores)), METH_FASTCALL, nullptr},
-    {"crosses_streams", py_crosses_streams, METH_NOARGS, nullptr},
+    {"reaches_default_stream", py_reaches_default_stream, METH_NOARGS, nullptr},
     {"linear_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_scores)), METH_FASTCALL, nullptr},
     {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm)), METH_FASTCALL, nullptr},
     {"mx8_swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx8_swiglu)), METH_FASTCALL, nullptr},

@@ -46,12 +46,12 @@ def native():
 
 def refuse_capture_into_another_graph() -> None:
     """For a backward in front of its first launch. A leaf keeps the node that gathers its gradient as long as any graph holds the leaf,
-    and the engine orders that node's stream behind the gradient. Under graph capture that stream is not part of the capture: the
-    engine's thread would end the process over it."""
+    and the engine orders that node's stream behind the gradient. Under graph capture a stream joins the capture by that, which the
+    default stream cannot: the process would end over it."""
     from rl_engine import _torch_host
 
-    if torch.cuda.is_current_stream_capturing() and _torch_host.crosses_streams():
+    if torch.cuda.is_current_stream_capturing() and _torch_host.reaches_default_stream():
         raise RuntimeError(
-            "a backward cannot be captured into a graph while an autograd graph that was made outside of the capture holds its inputs: "
+            "a backward cannot be captured into a graph while an autograd graph that was made on the default stream holds its inputs: "
             "drop the outputs of the earlier calls first"
         )

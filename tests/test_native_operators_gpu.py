@@ -245,8 +245,8 @@ def test_backward_on_the_stream_of_the_forward():
 
 @pytest.mark.parametrize("name", ["scores", "linear", "norm", "swiglu", "ffn", "behind a cast"])
 def test_a_backward_is_not_captured_into_another_graph(general, name):
-    """The leaf's gatherer belongs to the stream that an earlier graph was made on, which no capture may wait for: refused in front of
-    any launch. The capture goes on, and so does the earlier graph; without it the same capture is taken."""
+    """The leaf's gatherer belongs to the stream that an earlier graph was made on; the default stream cannot join a capture: refused in
+    front of any launch. The capture goes on, and so does the earlier graph; without it the same capture is taken."""
     from rl_engine.ops.ffn import qwen3_ffn
 
     w = _normal(64, 64, seed=3)
@@ -313,7 +313,7 @@ def test_what_wants_no_gradient_is_no_obstacle(general):
     general(captured)
 
 
-def test_a_leaf_of_another_stream_is_seen(general):
+def test_a_leaf_of_the_default_stream_is_seen(general):
     """Outside of a capture such a backward runs, on the stream of its forward."""
     from rl_engine import _host
 
@@ -327,7 +327,7 @@ def test_a_leaf_of_another_stream_is_seen(general):
 
         @staticmethod
         def backward(ctx, g):
-            seen.append(_host.native().crosses_streams())
+            seen.append(_host.native().reaches_default_stream())
             return g * 2
 
     held = Look.apply(x)  # noqa: F841
@@ -336,7 +336,7 @@ def test_a_leaf_of_another_stream_is_seen(general):
     for stream in (torch.cuda.current_stream(), side):
         with torch.cuda.stream(stream):
             torch.autograd.grad(Look.apply(x).sum(), [x])
-    assert seen == [False, True] and not _host.native().crosses_streams()
+    assert seen == [False, True] and not _host.native().reaches_default_stream()
     call = _calls()["norm"]
     held = call(x)  # noqa: F841
     want = torch.autograd.grad(call(x).sum(), [x])[0]

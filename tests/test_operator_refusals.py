@@ -148,7 +148,7 @@ def test_cpu_tensors_are_not_everyday(rlk_lib):
     assert native.norm(x, x, None, None, x[0], 1e-6, 1.0) is None and native.norm(None, x, None, None, x[0], 1e-6, 1.0) is None
     assert native.norm(x, x, None, None, x[0], "1e-6", 1.0) is None and native.norm(x) is None
     assert native.mx8_swiglu(x, x) is None and native.mx8_swiglu(x) is None and native.mx8_encode(x) is None and native.mx8_encode(3) is None
-    assert native.crosses_streams() is False
+    assert native.reaches_default_stream() is False
 
 
 def test_the_entry_points_word_their_errors():

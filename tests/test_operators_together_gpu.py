@@ -227,3 +227,47 @@ def test_a_rollout_scores_its_tokens():
             one = score(batch["stream"][r, rows], batch["ids"][r, rows])
             for a, b in zip(one, whole):
                 assert torch.equal(a[-1], b[r, t])
+
+
+def test_graphed_callables():
+    """A module whose forward and backward are captured one by one, after warm-up on a stream of its own, and replayed by autograd."""
+    from rl_engine.ops.ffn import qwen3_ffn_block
+    from rl_engine.ops.logprob import deterministic_linear_scores
+    from rl_engine.ops.norm import rms_norm
+
+    batch = _batch(BF16)
+    ids = batch["ids"].reshape(-1)
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            for name, t in _parameters().items():
+                if not name.endswith("_2"):
+                    self.register_parameter(name, torch.nn.Parameter(t.detach()))
+
+        def forward(self, stream):
+            p = dict(self.named_parameters())
+            x = rms_norm(stream, p["first_norm"], eps=EPS)
+            _, x = qwen3_ffn_block(
+                stream, x, p["gate_weight_1"], p["up_weight_1"], p["down_weight_1"], p["next_norm_weight_1"],
+                post_norm_weight=p["post_norm_weight_1"], gate=p["gate_1"], residual_scale=SCALE, eps=EPS, checkpoint_bits=8,
+            )  # fmt: skip
+            scores = deterministic_linear_scores(x, p["head"], ids, real_vocab_size=REAL)
+            return scores.logp, scores.entropy
+
+    eager, net = Net(), Net()
+    first = batch["stream"].reshape(-1, HIDDEN).clone().requires_grad_(True)
+    graphed = torch.cuda.make_graphed_callables(net, (first,))
+    g = _normal(ids.numel(), seed=7, dtype=FP32), _normal(ids.numel(), seed=8, dtype=FP32)
+    for seed in range(3):
+        stream = _normal(ids.numel(), HIDDEN, seed=70 + seed).requires_grad_(True)
+        results = []
+        for module in (graphed, eager):
+            module.zero_grad()
+            out = module(stream)
+            torch.autograd.backward(out, [t.clone() for t in g])
+            results.append([*(t.detach().clone() for t in out), stream.grad.clone(), *(q.grad.clone() for q in module.parameters())])
+            stream.grad = None
+            torch.cuda.synchronize()
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
