@@ -164,9 +164,9 @@ def hip_deterministic_scores_from_logits(
 
 
 def _token_chunks(tokens: int, vocab: int):
-    """Row ranges whose fp32 logits fit the buffer."""
-    per_row = 4 * _C.linear_logp_logits_row_stride(vocab)
-    step = max(_LOGITS_BUFFER_BYTES // per_row // _CHUNK_TOKENS, 1) * _CHUNK_TOKENS
+    """Row ranges whose fp32 logits fit the buffer, whole token tiles where it takes one (a single row always)."""
+    rows = max(_LOGITS_BUFFER_BYTES // (4 * _C.linear_logp_logits_row_stride(vocab)), 1)
+    step = rows // _CHUNK_TOKENS * _CHUNK_TOKENS or rows
     return [(first, min(first + step, tokens)) for first in range(0, tokens, step)]
 
 

@@ -202,3 +202,16 @@ def test_division_of_a_piece_by_the_pieces_of_a_row():
                 continue
             total = ((n * factor) >> 32) + n
             assert total < 2**32 and total >> shift == n // d, (n, d)
+
+
+def test_parts_of_the_tokens_fit_their_buffer(rlk_lib):
+    from rl_engine import _C
+    from rl_engine.backends.rocm.logprob import token_scores
+
+    for tokens, vocab in ((1, 151936), (3328, 151936), (3329, 151936), (70000, 1000), (5, 1 << 28), (300, 1 << 23), (0, 100), (1000, 9_000_000)):
+        parts = token_scores._token_chunks(tokens, vocab)
+        per_row = 4 * _C.linear_logp_logits_row_stride(vocab)
+        assert [r for first, end in parts for r in range(first, end)] == list(range(tokens))
+        assert all((end - first) * per_row <= token_scores._LOGITS_BUFFER_BYTES or end - first == 1 for first, end in parts)
+        assert all(first % 256 == 0 for first, _ in parts) or token_scores._LOGITS_BUFFER_BYTES // per_row < 256
+    assert len(token_scores._token_chunks(3328, 151936)) == 1 and len(token_scores._token_chunks(3329, 151936)) == 2

@@ -386,7 +386,9 @@ def test_linear_gradients(ops, tokens, vocab, hidden, k, tempered):
     assert only.shape == w.shape
 
 
-def test_a_buffer_of_some_tokens_gives_the_same_bits(ops, monkeypatch):
+@pytest.mark.parametrize("rows,parts_of_it", [(256, 3), (100, 7)])
+def test_a_buffer_of_some_tokens_gives_the_same_bits(ops, monkeypatch, rows, parts_of_it):
+    from rl_engine import _C
     from rl_engine.backends.rocm.logprob import token_scores
 
     h, w, target = _head(700, 1030, 256, 55)
@@ -395,8 +397,8 @@ def test_a_buffer_of_some_tokens_gives_the_same_bits(ops, monkeypatch):
     h.requires_grad_(True), w.requires_grad_(True)
     with ops.recompute_logits():
         first = torch.autograd.grad([ops.deterministic_linear_scores(h, w, target, top_k=5, temperature=temp).entropy.sum()], [h, w])
-        monkeypatch.setattr(token_scores, "_LOGITS_BUFFER_BYTES", 1)
-        assert len(token_scores._token_chunks(700, 1030)) == 3
+        monkeypatch.setattr(token_scores, "_LOGITS_BUFFER_BYTES", rows * 4 * _C.linear_logp_logits_row_stride(1030))
+        assert len(token_scores._token_chunks(700, 1030)) == parts_of_it
         parts = ops.deterministic_linear_scores(h, w, target, top_k=5, temperature=temp)
         second = torch.autograd.grad([parts.entropy.sum()], [h, w])
     for a, b in zip([*whole, *first], [*parts, *second]):
