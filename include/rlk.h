@@ -485,7 +485,8 @@ int rlk_logits_logp_backward(const void* logits, int dtype, int64_t row_stride, 
  * temperature [T] may be NULL. A target outside [0, real_vocab) gives logp = NaN; a temperature that is not positive, a NaN or
  * +inf logit and a row without a logit above -inf give NaN throughout (lse is -inf for the latter). The bits of logp and lse are
  * those of rlk_logp_from_logits with 64 tiles where 64 divides V.
- * top_k: 0 (top_logp and top_ids may be NULL) to RLK_SCORES_MAX_TOP_K. A row's results never depend on the other rows.
+ * top_k: 0 (top_logp and top_ids may be NULL) to RLK_SCORES_MAX_TOP_K; at most RLK_SCORES_MAX_ROWS rows and RLK_SCORES_MAX_VOCAB columns. A
+ * row's results never depend on the other rows.
  */
 #define RLK_SCORES_MAX_TOP_K 64
 #define RLK_SCORES_MAX_VOCAB (1 << 28)
@@ -537,7 +538,7 @@ int rlk_linear_dlogits_bwd(const void* dlogits, const void* hidden, int64_t h_ro
  *   normed = total * r2 * pre_weight, r2 = 1 / sqrt(mean(total^2) + eps)      (none where pre_weight is NULL; of the unrounded total)
  * block and normed have `dtype`, residual and total residual_dtype (dtype or fp32), gate and the weights theirs (dtype or fp32).
  * gate: RLK_GATE_CHANNEL [width], RLK_GATE_TOKEN [tokens] (gate_row_stride apart), RLK_GATE_FULL [tokens, width], or none. Outputs
- * and gradients are contiguous. Arithmetic and sums in fp32, each result rounded once.
+ * and gradients are contiguous. eps is at least 0. Arithmetic and sums in fp32, each result rounded once.
  */
 typedef enum rlk_gate { RLK_GATE_NONE = 0, RLK_GATE_CHANNEL = 1, RLK_GATE_TOKEN = 2, RLK_GATE_FULL = 3 } rlk_gate;
 #define RLK_NORM_MAX_WIDTH 16384

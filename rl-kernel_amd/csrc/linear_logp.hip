@@ -1074,6 +1074,7 @@ hipError_t linear_logp_launch(const MatView& H, const MatView& W, const int64_t*
       return hipErrorInvalidValue;
   }
   if (err != hipSuccess) return err;
+  if (logp == nullptr && lse == nullptr && target_logit == nullptr) return hipSuccess;  // (the caller merges the partials itself)
   // The whole-vocabulary entries (those that write logp) mark rows whose target lies outside the real vocabulary;
   // a shard's target logit is legitimately 0 for a target another shard owns.
   return linear_logp_merge_launch(workspace, logp, lse, target_logit, T, a.n_split, true, stream,

@@ -711,12 +711,12 @@ int rlk_linear_scores_fwd(const void* hidden, int64_t h_row_stride, const void* 
     }
   }
   // (the weighted sums lie right behind the three planes that the merge reads; above the stream groups' token counts nothing else does)
-  int rc = linear_logp_fwd_checked(who, hidden, h_row_stride, weight, w_row_stride, target, bias, temperature, logp, lse, nullptr, workspace,
-                                   workspace_bytes, T, D, V, 0, real_vocab_end, RLK_LOGP_CFG_AUTO, stream, logits, logits_row_stride,
+  int rc = linear_logp_fwd_checked(who, hidden, h_row_stride, weight, w_row_stride, target, bias, temperature, nullptr, nullptr, nullptr,
+                                   workspace, workspace_bytes, T, D, V, 0, real_vocab_end, RLK_LOGP_CFG_AUTO, stream, logits, logits_row_stride,
                                    entropy_in_fold);
   if (rc != RLK_OK || T == 0) return rc;
-  hipError_t err = linear_scores_launch(logits, logits_row_stride, temperature, lse, reinterpret_cast<const float*>(workspace), entropy_in_fold,
-                                        T, V, real_vocab_end, linear_logp_split_count(V), top_k, entropy, top_logp, top_ids,
+  hipError_t err = linear_scores_launch(logits, logits_row_stride, target, temperature, reinterpret_cast<const float*>(workspace), entropy_in_fold,
+                                        T, V, real_vocab_end, linear_logp_split_count(V), top_k, logp, lse, entropy, top_logp, top_ids,
                                         reinterpret_cast<char*>(workspace) + base, reinterpret_cast<hipStream_t>(stream));
   return err == hipSuccess ? RLK_OK : device_error(who, err);
 }

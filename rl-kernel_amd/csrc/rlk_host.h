@@ -160,7 +160,7 @@ size_t linear_logp_workspace_bytes(int T, int V);
 // linear_logp_workspace_bytes(T, V) bytes of fp32 partials. logp, lse and target_logit
 // (the unclamped scaled logit of a target this weight owns, else 0) may each be null, and so may
 // logits ([T, logits_ld] fp32: the accumulators with the bias added and padded lanes -inf, before
-// the temperature, stored by the same pass).
+// the temperature, stored by the same pass). With all three null the partials stay for the caller to merge.
 hipError_t linear_logp_launch(const MatView& H, const MatView& W, const int64_t* target, const float* bias,
                               const float* temperature, float* logp, float* lse, float* target_logit,
                               float* logits, int64_t logits_ld, float* workspace, int T, int D, int V,
@@ -223,9 +223,9 @@ hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride
 // The scores of the fused linear-LogP from its partials [n_split][T] of maxima, sums and weighted sums; the latter from the fp32 logits
 // that it stored unless the launch left them (`have_weighted`, at the start of `extra`), as do the alternatives.
 size_t linear_scores_extra_bytes(int T, int V, int top_k);  // right behind the three planes of the linear-LogP
-hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const float* temperature, const float* lse, const float* part,
-                                bool have_weighted, int T, int V, int real, int n_split, int top_k, float* entropy, float* top_logp,
-                                int64_t* top_ids, void* extra, hipStream_t stream);
+hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const int64_t* target, const float* temperature, const float* part,
+                                bool have_weighted, int T, int V, int real, int n_split, int top_k, float* logp, float* lse, float* entropy,
+                                float* top_logp, int64_t* top_ids, void* extra, hipStream_t stream);
 // Their gradient, in the type of the logits or (fp32 logits) in bf16; columns [V, grad_cols) are written as zeros.
 hipError_t token_scores_backward_launch(const void* logits, int dtype, int64_t row_stride, const int64_t* target,
                                         const float* temperature, const float* lse, const float* entropy, const float* g_logp,

@@ -235,7 +235,6 @@ struct ScoreFinishArgs {
   int64_t row_stride;
   const int64_t* target;
   const float* temperature;
-  const float* row_lse;  // LINEAR: [T], the log-sum-exps
   const float* stats;
   const uint32_t* best;
   const uint32_t* where;
@@ -245,7 +244,7 @@ struct ScoreFinishArgs {
   float* top_logp;   // [T][top_k]
   int64_t* top_ids;  // [T][top_k]
   int T, V, real, tile_size, top_k;
-  const float* part;      // LINEAR: [n_split][T] maxima, then sums
+  const float* part;      // LINEAR: [n_split][T] maxima, sums, target logits
   const float* weighted;  // LINEAR: [n_split][T]
   int n_split;
 };
@@ -593,22 +592,34 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
   const bool bad_temperature = !(temperature > 0.f);
   const float nan = __builtin_nanf("");
   float lse;
-  if constexpr (LINEAR) {  // a lane takes every 64th split, ascending
+  if constexpr (LINEAR) {  // a lane takes every 64th split; the sums of all are added ascending, as linear_logp_merge_kernel does
     const int64_t plane = (int64_t)a.n_split * a.T;
-    float m = kNegInf, s = 0.f, w = 0.f;
+    const int64_t target = a.target[row];
+    const bool bad_target = target < 0 || target >= a.real;
+    const float zt = bad_target ? nan : a.part[2 * plane + target / kLogpSplitCols * a.T + row];
+    float m = kNegInf, w = 0.f, sum = 0.f;
     for (int p = lane; p < a.n_split; p += kWave) m = fmaxf(m, a.part[(int64_t)p * a.T + row]);
     const float big = wave_max_f32(m);
-    for (int p = lane; p < a.n_split; p += kWave) {
-      const int64_t at = (int64_t)p * a.T + row;
-      const float pm = a.part[at], ps = a.part[plane + at];
-      if (pm > kNegInf) {
-        s = __builtin_fmaf(ps, pinned_exp(pm - big), s);
+    for (int base = 0; base < a.n_split; base += kWave) {
+      float term = 0.f;
+      if (base + lane < a.n_split) {
+        const int64_t at = (int64_t)(base + lane) * a.T + row;
+        const float pm = a.part[at], ps = a.part[plane + at];
+        const float scaled = ps * pinned_exp(pm - big);
+        term = pm > kNegInf ? scaled : 0.f;
         w = w + logp_weighted_term(pm, ps, a.weighted[at], big);
       }
+#pragma unroll 8
+      for (int t = 0; t < kWave; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
     }
-    const float sum = wave_sum_f32(s), weighted = wave_sum_f32(w);
-    lse = a.row_lse[row];
-    if (lane == 0) a.entropy[row] = bad_temperature ? nan : logf(sum) - weighted / sum;
+    const float weighted = wave_sum_f32(w);
+    const float log_sum = logf(sum);
+    lse = bad_temperature ? nan : big + log_sum;
+    if (lane == 0) {
+      a.entropy[row] = bad_temperature ? nan : log_sum - weighted / sum;
+      a.lse[row] = lse;
+      a.logp[row] = bad_temperature || bad_target ? nan : fminf(zt - lse, 0.f);
+    }
   } else {
     const float* stats = a.stats + (int64_t)row * kScorePlanes * kScoreTiles + lane;
     const float m = stats[0], s = stats[kScoreTiles], w = stats[3 * kScoreTiles];
@@ -878,7 +889,7 @@ hipError_t token_scores_launch(const void* logits, int dtype, int64_t row_stride
   a.tile_size = (int)(((int64_t)V + kScoreTiles - 1) / kScoreTiles);
   const int64_t bytes = (int64_t)T * V * (dtype == RLK_DTYPE_FP32 ? 4 : 2);
   a.streamed = bytes > kCachedLogitsBytes ? (int64_t)((double)T * (kScoreTiles / kGroupTiles) * (1.0 - (double)kCachedLogitsBytes / bytes)) : 0;
-  const ScoreFinishArgs f{logits, row_stride, target, temperature, nullptr, a.stats, a.best, a.where, logp, lse, entropy,
+  const ScoreFinishArgs f{logits, row_stride, target, temperature, a.stats, a.best, a.where, logp, lse, entropy,
                           top_logp, top_ids, T, V, real, a.tile_size, top_k, nullptr, nullptr, 0};
   switch (dtype) {
     case RLK_DTYPE_BF16: return token_scores_typed<RLK_DTYPE_BF16>(a, f, stream);
@@ -893,9 +904,9 @@ size_t linear_scores_extra_bytes(int T, int V, int top_k) {
   return weighted + 16 + (top_k > 0 ? (size_t)T * 2 * kScoreSlices * sizeof(uint32_t) : 0);
 }
 
-hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const float* temperature, const float* lse, const float* part,
-                                bool have_weighted, int T, int V, int real, int n_split, int top_k, float* entropy, float* top_logp,
-                                int64_t* top_ids, void* extra, hipStream_t stream) {
+hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const int64_t* target, const float* temperature, const float* part,
+                                bool have_weighted, int T, int V, int real, int n_split, int top_k, float* logp, float* lse, float* entropy,
+                                float* top_logp, int64_t* top_ids, void* extra, hipStream_t stream) {
   float* weighted = reinterpret_cast<float*>(extra);
   uint32_t* best = reinterpret_cast<uint32_t*>((reinterpret_cast<uintptr_t>(weighted + (size_t)n_split * T) + 15) / 16 * 16);
   uint32_t* where = best + (size_t)T * kScoreSlices;
@@ -909,7 +920,7 @@ hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const fl
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  const ScoreFinishArgs f{logits, logits_ld, nullptr, temperature, lse, nullptr, best, where, nullptr, nullptr, entropy,
+  const ScoreFinishArgs f{logits, logits_ld, target, temperature, nullptr, best, where, logp, lse, entropy,
                           top_logp, top_ids, T, V, real, 0, top_k, part, weighted, n_split};
   hipLaunchKernelGGL((score_finish_kernel<RLK_DTYPE_FP32, true>), dim3((unsigned)T), dim3(kWave), 0,
                      stream, f);

@@ -345,6 +345,28 @@ def test_linear_scores_match_the_definitions(ops, tokens, vocab, hidden, real, k
     assert torch.equal(scores.lse.view(torch.int32), lse.view(torch.int32))
 
 
+@pytest.mark.parametrize("tokens", [40, 1100])
+@pytest.mark.parametrize("k", [0, 3])
+def test_linear_scores_of_ids_and_temperatures_that_name_nothing(ops, tokens, k):
+    h, w, target = _head(tokens, 3000, 64, 5)
+    temp = 0.5 + torch.rand(tokens, generator=_gen(6), device=DEV)
+    clean = ops.deterministic_linear_scores(h, w, target.clamp(max=2899), top_k=k, temperature=temp, real_vocab_size=2900)
+    target = target.clamp(max=2899)
+    for row, value in ((1, -1), (4, 2900), (7, 2999), (9, 3000), (30, 1 << 40)):
+        target[row] = value
+    for row, value in ((4, 0.0), (12, -1.0), (13, float("nan"))):
+        temp[row] = value
+    s = ops.deterministic_linear_scores(h, w, target, top_k=k, temperature=temp, real_vocab_size=2900)
+    logp, lse = ops.deterministic_linear_logp(h, w, target, temperature=temp, real_vocab_size=2900)
+    assert torch.equal(s.logp.view(torch.int32), logp.view(torch.int32)) and torch.equal(s.lse.view(torch.int32), lse.view(torch.int32))
+    no_id, no_temperature = torch.tensor([1, 4, 7, 9, 30], device=DEV), torch.tensor([4, 12, 13], device=DEV)
+    assert bool(torch.isnan(s.logp[no_id]).all()) and all(bool(torch.isnan(t[no_temperature]).all()) for t in s[:3])
+    rest = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    rest[no_id], rest[no_temperature] = False, False
+    for a, b in zip(s, clean):
+        assert a is None or torch.equal(a[rest], b[rest])
+
+
 def test_linear_scores_with_a_bias(ops):
     h, w, target = _head(9, 640, 64, 31)
     bias = torch.randn(640, generator=_gen(33), device=DEV).mul(64).round().div(64)
