@@ -670,11 +670,12 @@ __global__ __launch_bounds__(256) void linear_score_rows_kernel(LinearRowArgs a)
   const int l16 = lane & (kTileLanes - 1);
   const float* row_ptr = a.logits + (int64_t)row * a.logits_ld;
   const float inv_t = HAS_TEMP ? 1.0f / a.temperature[row] : 1.0f;
-  const int c0 = blockIdx.y * kGroupTiles + wave * kTilesPerWave;
-  const int mine = c0 + lane / kTileLanes;  // this lane's split, TOP: its class of them
+  // A wave has four splits at a time. TOP: those of the same classes are the other three waves' and its next ones.
+  const int c0 = blockIdx.y * (TOP ? kTilesPerWave : kGroupTiles) + (TOP ? 0 : wave * kTilesPerWave);
+  const int mine = c0 + lane / kTileLanes;
   float best = kNegInf, other = kNegInf;
   int at = 0;
-  for (int base = 0; base + c0 < a.n_split; base += kScoreTiles) {  // uniform
+  for (int base = TOP ? wave * kScoreTiles : 0; base + c0 < a.n_split; base += 4 * kScoreTiles) {  // uniform
     const int split = base + mine;
     const int col0 = split * kLogpSplitCols + l16 * 16;
     f32x4_t raw[kLogpSplitTiles][4];
@@ -725,7 +726,23 @@ __global__ __launch_bounds__(256) void linear_score_rows_kernel(LinearRowArgs a)
     if (l16 == 0 && split < a.n_split) a.weighted[(int64_t)split * a.T + row] = sum;
     if constexpr (!TOP) break;
   }
-  if constexpr (TOP) {
+  if constexpr (TOP) {  // the waves' notes of a slice: the larger best one, of equal ones the first vector, and what is left as the other
+    __shared__ float bests[4][kWave], others[4][kWave];
+    __shared__ int ats[4][kWave];
+    bests[wave][lane] = best;
+    others[wave][lane] = other;
+    ats[wave][lane] = at;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int v = 1; v < 4; ++v) {
+      const float theirs = bests[v][lane];
+      const int their_at = ats[v][lane];
+      const bool win = theirs > best || (theirs == best && their_at < at);
+      other = fmaxf(fmaxf(other, others[v][lane]), win ? best : theirs);
+      best = win ? theirs : best;
+      at = win ? their_at : at;
+    }
     const int64_t slice = (int64_t)row * kScoreSlices + mine * kTileLanes + l16;
     a.best[slice] = mine * kLogpSplitCols + l16 * 16 < a.real ? ordered_bits(best) : 0u;
     a.where[slice] = (ordered_bits(other) & 0xffff0000u) | (uint32_t)at;
@@ -913,8 +930,9 @@ hipError_t linear_scores_launch(const float* logits, int64_t logits_ld, const in
   uint32_t* where = best + (size_t)T * kScoreSlices;
   if (!have_weighted || top_k > 0) {
     LinearRowArgs a{logits, logits_ld, temperature, weighted, best, where, T, V, real, n_split};
-    // (a wave's splits one after the other only where they share slices: 1 to 16 tokens of V = 151936 4.6 us less)
-    const dim3 grid((unsigned)T, top_k > 0 ? kScoreTiles / kGroupTiles : (n_split + kGroupTiles - 1) / kGroupTiles), block(256);
+    // (four splits to a wave, and a wave for all of them: with 64 classes of splits, each the work of one lane, 1 to 16 tokens of V = 151936
+    // took 4.6 us more)
+    const dim3 grid((unsigned)T, top_k > 0 ? kScoreTiles / kTilesPerWave : (n_split + kGroupTiles - 1) / kGroupTiles), block(256);
     if (temperature && top_k > 0) hipLaunchKernelGGL((linear_score_rows_kernel<true, true>), grid, block, 0, stream, a);
     else if (temperature) hipLaunchKernelGGL((linear_score_rows_kernel<true, false>), grid, block, 0, stream, a);
     else if (top_k > 0) hipLaunchKernelGGL((linear_score_rows_kernel<false, true>), grid, block, 0, stream, a);

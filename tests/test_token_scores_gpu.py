@@ -367,6 +367,34 @@ def test_linear_scores_of_ids_and_temperatures_that_name_nothing(ops, tokens, k)
         assert a is None or torch.equal(a[rest], b[rest])
 
 
+@pytest.mark.parametrize("kind", ["five rows", "one row", "rising", "falling", "a block at the end", "all but some masked"])
+@pytest.mark.parametrize("vocab,real", [(1030, 1001), (70000, 70000), (151936, 151669)])
+def test_alternatives_of_hidden_states_wherever_they_lie(ops, kind, vocab, real):
+    """Columns of one logit in many splits of the vocabulary, and the largest ones side by side."""
+    h = torch.ones((3, 64), dtype=torch.bfloat16, device=DEV)
+    h[1] *= -1
+    column = torch.arange(vocab, device=DEV)
+    bias = None
+    if kind == "five rows":
+        value = torch.randn(5, generator=_gen(1), device=DEV)[torch.randint(0, 5, (vocab,), generator=_gen(2), device=DEV)]
+    elif kind == "one row":
+        value = torch.ones(vocab, device=DEV)
+    elif kind == "a block at the end":
+        value = torch.where(column >= real - 70, 2.0, 1.0) + torch.randn(vocab, generator=_gen(3), device=DEV) * 0.01
+    else:
+        value = column / vocab * (-1 if kind == "falling" else 1)
+    if kind == "all but some masked":
+        bias = torch.full((vocab,), NEG, device=DEV)
+        bias[[3, 1000, real - 1]] = 0.0
+    w = value.to(torch.bfloat16)[:, None].expand(vocab, 64).contiguous()
+    z = h.double() @ w.double().t()
+    z = (z if bias is None else z + bias.double())[:, :real]
+    for k in (1, 20, 64):
+        s = ops.deterministic_linear_scores(h, w, torch.zeros(3, dtype=torch.long, device=DEV), bias, top_k=k, real_vocab_size=real)
+        want = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :k]
+        assert torch.equal(s.top_ids, want), (k, s.top_ids, want)
+
+
 def test_linear_scores_with_a_bias(ops):
     h, w, target = _head(9, 640, 64, 31)
     bias = torch.randn(640, generator=_gen(33), device=DEV).mul(64).round().div(64)
