@@ -569,7 +569,7 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
 // 5 with 20 alternatives, a chain of dependent reads and searches whose code is fetched as it is run: short loops throughout.
 template <int ELEM, bool LINEAR>
 __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) {
-  __shared__ uint64_t keys[kFinishKeys];
+  __shared__ __align__(16) uint64_t keys[kFinishKeys];
   __shared__ uint32_t picked[kFinishPicked];
   __shared__ uint32_t slices[kScoreSlices];
   const int lane = threadIdx.x;
@@ -592,25 +592,43 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
   const bool bad_temperature = !(temperature > 0.f);
   const float nan = __builtin_nanf("");
   float lse;
-  if constexpr (LINEAR) {  // a lane takes every 64th split; the sums of all are added ascending, as linear_logp_merge_kernel does
+  if constexpr (LINEAR) {  // a lane takes every 64th split; the sums of all are added ascending, as in linear_logp_merge_kernel
     const int64_t plane = (int64_t)a.n_split * a.T;
     const int64_t target = a.target[row];
     const bool bad_target = target < 0 || target >= a.real;
     const float zt = bad_target ? nan : a.part[2 * plane + target / kLogpSplitCols * a.T + row];
-    float m = kNegInf, w = 0.f, sum = 0.f;
-    for (int p = lane; p < a.n_split; p += kWave) m = fmaxf(m, a.part[(int64_t)p * a.T + row]);
-    const float big = wave_max_f32(m);
-    for (int base = 0; base < a.n_split; base += kWave) {
-      float term = 0.f;
-      if (base + lane < a.n_split) {
-        const int64_t at = (int64_t)(base + lane) * a.T + row;
-        const float pm = a.part[at], ps = a.part[plane + at];
-        const float scaled = ps * pinned_exp(pm - big);
-        term = pm > kNegInf ? scaled : 0.f;
-        w = w + logp_weighted_term(pm, ps, a.weighted[at], big);
+    constexpr int kHeld = 4;  // splits of a lane at a time, as loaded: up to a vocabulary of 262144 all of them
+    float pm[kHeld], ps[kHeld], pw[kHeld];
+    auto fetch = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+      for (int r = 0; r < kHeld; ++r) {
+        const int p = base + r * kWave + lane;
+        const int64_t at = (int64_t)p * a.T + row;
+        pm[r] = p < a.n_split ? a.part[at] : kNegInf;
+        ps[r] = p < a.n_split ? a.part[plane + at] : 0.f;
+        pw[r] = p < a.n_split ? a.weighted[at] : 0.f;
       }
-#pragma unroll 8
-      for (int t = 0; t < kWave; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
+    };
+    fetch(0);
+    float m = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), w = 0.f, sum = 0.f;
+    for (int p = kHeld * kWave + lane; p < a.n_split; p += kWave) m = fmaxf(m, a.part[(int64_t)p * a.T + row]);
+    const float big = wave_max_f32(m);
+    float* const terms = reinterpret_cast<float*>(keys);  // (not in use yet)
+    for (int base = 0; base < a.n_split; base += kHeld * kWave) {
+      if (base > 0) fetch(base);
+#pragma unroll
+      for (int r = 0; r < kHeld; ++r) {
+        const float scaled = ps[r] * pinned_exp(pm[r] - big);
+        terms[r * kWave + lane] = pm[r] > kNegInf ? scaled : 0.f;
+        w = w + logp_weighted_term(pm[r], ps[r], pw[r], big);
+      }
+      wave_lds_sync();
+      const int count = min(kHeld * kWave, a.n_split - base);
+      for (int j = 0; j < count; j += 4) {  // (terms behind the last split are 0)
+        const f32x4_t four = *reinterpret_cast<const f32x4_t*>(terms + j);
+        sum = (((sum + four[0]) + four[1]) + four[2]) + four[3];
+      }
+      wave_lds_sync();
     }
     const float weighted = wave_sum_f32(w);
     const float log_sum = logf(sum);

@@ -345,6 +345,17 @@ def test_linear_scores_match_the_definitions(ops, tokens, vocab, hidden, real, k
     assert torch.equal(scores.lse.view(torch.int32), lse.view(torch.int32))
 
 
+@pytest.mark.parametrize("tokens,k", [(5, 64), (5, 0), (1030, 0)])
+def test_linear_scores_of_more_splits_than_a_wave_holds(ops, tokens, k):
+    h, w, target = _head(tokens, 600011, 64, 77)
+    s = ops.deterministic_linear_scores(h, w, target, top_k=k)
+    logp, lse = ops.deterministic_linear_logp(h, w, target)
+    assert torch.equal(s.logp.view(torch.int32), logp.view(torch.int32)) and torch.equal(s.lse.view(torch.int32), lse.view(torch.int32))
+    rows = slice(tokens - 5, tokens)
+    some = type(s)(*(None if t is None else t[rows] for t in s))
+    _check(some, h[rows].double() @ w.double().t(), target[rows], k, None, 16 * 600011)
+
+
 @pytest.mark.parametrize("tokens", [40, 1100])
 @pytest.mark.parametrize("k", [0, 3])
 def test_linear_scores_of_ids_and_temperatures_that_name_nothing(ops, tokens, k):
