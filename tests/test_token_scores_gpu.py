@@ -218,7 +218,8 @@ def _gradient(z, target, temp, ids, g_logp, g_lse, g_entropy, g_top):
     """The definition's gradient in 64 bits and, per element, by how much it may be off before the last rounding: the sizes of
     its factors times p's relative error. With y the scaled logit and d = y - lse, in units of 2^-24: 2 |y| for the reciprocal
     temperature and the product with it, |lse| for the rounding of lse beside the V / 1024 + 90 of its sum, |d| for the
-    difference, |d| for its product with log2 e, and 8 for the exponential and the products behind it."""
+    difference, |d| for its product with log2 e, and 8 for the exponential and the products behind it. The gradients that are summed
+    to p's factor may cancel: the sum of g_top takes 6 steps over a wave and 2 more with the others, 8 of the sizes of what is summed."""
     z = z.double()
     rows = torch.arange(z.size(0), device=DEV)
     inv = torch.ones(z.size(0), dtype=torch.float64, device=DEV) if temp is None else 1 / temp.double()
@@ -237,7 +238,8 @@ def _gradient(z, target, temp, ids, g_logp, g_lse, g_entropy, g_top):
     d = torch.where(p > 0, y - torch.logsumexp(y, 1)[:, None], 0.0).abs()
     y = torch.where(p > 0, y, 0.0).abs()
     steps = 2 * y + torch.logsumexp(y, 1)[:, None].abs() + 2 * d + 8 + z.size(1) / 1024 + 90
-    return dz * inv[:, None], 2.0**-24 * steps * size * inv[:, None]
+    summed = g_lse.double().abs() + g_logp.double().abs() + (g_top.double().abs().sum(1) if g_top is not None else 0.0)
+    return dz * inv[:, None], 2.0**-24 * (steps * size + 8 * p * summed[:, None]) * inv[:, None]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
