@@ -268,10 +268,12 @@ __device__ __forceinline__ uint32_t wave_reduce(uint32_t v, uint32_t neutral, Op
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ float wave_sum_f32(float v) {
-  return __uint_as_float(wave_reduce(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+  auto add = [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); };
+  return __uint_as_float(wave_reduce(__float_as_uint(v), 0u, add));
 }
 __device__ __forceinline__ float wave_max_f32(float v) {
-  return __uint_as_float(wave_reduce(__float_as_uint(v), __float_as_uint(kNegInf), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+  auto larger = [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); };
+  return __uint_as_float(wave_reduce(__float_as_uint(v), __float_as_uint(kNegInf), larger));
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) { return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) { return wave_reduce(v, ~0u, [](uint32_t a, uint32_t b) { return a < b ? a : b; }); }
