@@ -121,8 +121,9 @@ __device__ __forceinline__ void logp_fold_run(const float (&y)[16], int tl, floa
 }
 
 // The same step with the weighted sum w = sum e(y - m) (y - m) beside (m, s), for the entropy of the distribution: seen from a larger
-// maximum n it is e(m - n) (w + s (m - n)). (m, s) have the bits of logp_fold_run(). A masked logit is -inf below the maximum:
-// kFarBelow, from where e() is zero, stands for it, as zero times infinity is no number.
+// maximum n it is e(m - n) (w + s (m - n)). (m, s) have the bits of logp_fold_run(). A masked logit is -inf below the maximum, or, under a mask
+// of a finite lowest value, so far that its product with a sum is: kFarBelow, from where e() is zero, stands for such distances, as zero
+// times infinity is no number.
 constexpr float kFarBelow = -256.f;
 __device__ __forceinline__ void logp_fold_run_weighted(const float (&y)[16], int tl, float& run_m, float& run_s, float& run_w,
                                                        float& run_zt) {
@@ -158,7 +159,7 @@ __device__ __forceinline__ void logp_fold_run_weighted(const float (&y)[16], int
 }
 // A stream's share of its split's weighted sum, seen from the split's maximum.
 __device__ __forceinline__ float logp_weighted_term(float m, float s, float w, float big) {
-  const float back = m - big;
+  const float back = fmaxf(m - big, kFarBelow);
   const float term = pinned_exp(back) * __builtin_fmaf(s, back, w);
   return m > kNegInf ? term : 0.f;
 }

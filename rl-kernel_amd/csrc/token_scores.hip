@@ -101,8 +101,8 @@ __device__ __forceinline__ void merge_score_lanes(int lane, ScoreState& st) {
   const float my_shrink = pinned_exp(st.m - n), other_shrink = pinned_exp(om - n);
   const float mine = st.m > kNegInf ? st.s * my_shrink : 0.f;
   const float theirs = om > kNegInf ? os * other_shrink : 0.f;
-  const float my_w = st.m > kNegInf ? my_shrink * __builtin_fmaf(st.s, st.m - n, st.w) : 0.f;
-  const float their_w = om > kNegInf ? other_shrink * __builtin_fmaf(os, om - n, ow) : 0.f;
+  const float my_w = st.m > kNegInf ? my_shrink * __builtin_fmaf(st.s, fmaxf(st.m - n, kFarBelow), st.w) : 0.f;
+  const float their_w = om > kNegInf ? other_shrink * __builtin_fmaf(os, fmaxf(om - n, kFarBelow), ow) : 0.f;
   // the lower lane's term first on both sides, so that both lanes add in the same order
   st.s = (lane & OFFSET) ? theirs + mine : mine + theirs;
   st.w = (lane & OFFSET) ? their_w + my_w : my_w + their_w;
@@ -649,7 +649,7 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
     float sum = 0.f;  // (ascending)
 #pragma unroll 8
     for (int t = 0; t < kScoreTiles; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
-    const float weighted = wave_sum_f32(m > kNegInf ? shrink * __builtin_fmaf(s, m - big, w) : 0.f);
+    const float weighted = wave_sum_f32(m > kNegInf ? shrink * __builtin_fmaf(s, fmaxf(m - big, kFarBelow), w) : 0.f);
     const float log_sum = logf(sum);
     lse = bad_temperature ? nan : big + log_sum;
     const float zt = wave_sum_f32(stats[2 * kScoreTiles]);

@@ -1,0 +1,134 @@
+"""Token scores of rows that hold what a mask or a diverged model leaves in them, on a real MI355X against the definitions in 64 bits
+(tolerances: test_token_scores_gpu.py)."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import test_operators_random_gpu as draws
+import test_token_scores_gpu as plain
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+NEG = plain.NEG
+BF16_LOWEST, FP32_LOWEST = torch.finfo(torch.bfloat16).min, torch.finfo(torch.float32).min
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from rl_engine.ops import logprob
+
+    return logprob
+
+
+# ---------------------------------------------------------------------------
+# Masks of a finite lowest value: their probability is 0 in 64 bits too, so the definitions are those of a mask of -inf
+# ---------------------------------------------------------------------------
+
+MASKS = ["all but one", "all but some", "half", "whole vectors", "whole tiles", "the end"]
+
+
+def _left(kind, vocab):
+    """Which columns a mask leaves."""
+    column = torch.arange(vocab, device=DEV)
+    return {
+        "all but one": column == vocab // 3,
+        "all but some": column % 401 == 17,
+        "half": torch.rand(vocab, generator=plain._gen(4), device=DEV) < 0.5,
+        "whole vectors": (column // 8) % 16 < 5,
+        "whole tiles": (column // -(-vocab // 64)) % 3 == 1,
+        "the end": column < vocab - vocab // 4,
+    }[kind]
+
+
+@pytest.mark.parametrize("kind", MASKS)
+@pytest.mark.parametrize("dtype,value", [(torch.bfloat16, BF16_LOWEST), (torch.bfloat16, -1e38), (torch.float32, FP32_LOWEST), (torch.float32, -1e38), (torch.float16, -65504.0)])
+@pytest.mark.parametrize("rows,vocab,tempered", [(3, 1000, False), (2, 50257, True), (40, 4096, True)])
+def test_masks_of_a_finite_lowest_value(ops, kind, dtype, value, rows, vocab, tempered):
+    left = _left(kind, vocab)
+    z = plain._logits(rows, vocab, vocab, dtype).masked_fill(~left, NEG)
+    masked = z.masked_fill(~left, value).requires_grad_(True)
+    columns = left.nonzero()[:, 0]
+    target = columns[torch.randint(0, columns.numel(), (rows,), generator=plain._gen(5), device=DEV)]
+    temp = 0.5 + torch.rand(rows, generator=plain._gen(6), device=DEV) if tempered else None
+    g = [torch.randn(rows, generator=plain._gen(20 + i), device=DEV) for i in range(3)]
+    for k in (0, min(8, columns.numel())):
+        scores = ops.deterministic_scores_from_logits(masked, target, top_k=k, temperature=temp)
+        plain._check(scores, z, target, k, temp, vocab)
+        g_top = torch.randn((rows, k), generator=plain._gen(30), device=DEV) if k else None
+        (grad,) = torch.autograd.grad([scores.logp, scores.lse, scores.entropy] + ([scores.top_logp] if k else []), [masked], g + ([g_top] if k else []))
+        want, size = plain._gradient(z, target, temp, scores.top_ids, *g, g_top)
+        tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-115
+        assert bool(((grad.double() - want).abs() <= plain.HALF_STEP[dtype] * want.abs() + size + tiny).all())
+
+
+def _linear_case(kind, tokens, vocab, value, by):
+    """Hidden states and a head whose masked logits are `value`, by a bias or by a column of the weight, and the logits with -inf in
+    their place. A sum of products of some hundreds at most changes nothing in a `value` of 10^38."""
+    hidden = 64
+    h, w, _ = plain._head(tokens, vocab, hidden, tokens + vocab)
+    left = _left(kind, vocab)
+    bias = None
+    if by == "bias":
+        bias = torch.where(left, 0.0, value)
+    else:
+        h[:, hidden - 1] = 1.0
+        w[:, hidden - 1] = torch.where(left, 0.0, value).bfloat16()
+    with torch.no_grad():
+        z = (h[:, : hidden - 1].double() @ w[:, : hidden - 1].double().t()) if by == "weight" else h.double() @ w.double().t()
+    columns = left.nonzero()[:, 0]
+    target = columns[torch.randint(0, columns.numel(), (tokens,), generator=plain._gen(5), device=DEV)]
+    return h, w, bias, z.masked_fill(~left, NEG), target, columns.numel()
+
+
+@pytest.mark.parametrize("kind", MASKS)
+@pytest.mark.parametrize("by,value", [("bias", FP32_LOWEST), ("bias", -1e38), ("weight", BF16_LOWEST)])
+@pytest.mark.parametrize("tokens,tempered", [(5, False), (300, True), (1100, True), (1281, False)])
+def test_masked_scores_of_hidden_states(ops, kind, by, value, tokens, tempered):
+    """One token tile, the stream groups, and the entropy in the product's fold."""
+    vocab = 5000
+    h, w, bias, z, target, left = _linear_case(kind, tokens, vocab, value, by)
+    temp = 0.5 + torch.rand(tokens, generator=plain._gen(6), device=DEV) if tempered else None
+    h.requires_grad_(True), w.requires_grad_(True)
+    g = [torch.randn(tokens, generator=plain._gen(20 + i), device=DEV) for i in range(3)]
+    for k in (0, min(3, left)):
+        scores = ops.deterministic_linear_scores(h, w, target, bias, top_k=k, temperature=temp)
+        plain._check(scores, z, target, k, temp, 16 * vocab)
+        dh, dw = torch.autograd.grad([scores.logp, scores.lse, scores.entropy], [h, w], g)
+        with torch.no_grad():
+            dz, size = plain._gradient(z, target, temp, None, *g, None)
+            slack = 2.0**-8 * dz.abs() + 1.01 * size
+            for got, want, room in ((dh, dz @ w.double(), slack @ w.double().abs()), (dw, dz.t() @ h.double(), slack.t() @ h.double().abs())):
+                assert bool(((got.double() - want).abs() <= 2.0**-8 * want.abs() + 1.01 * room + 2.0**-115).all())
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_draws_with_masks_of_any_value(ops, seed):
+    rng = random.Random(500 + seed)
+    rows, vocab, dtype = draws._log_int(rng, 1, 300), draws._log_int(rng, 1, 60000), rng.choice(draws.DTYPES)
+    real, gen = rng.randint(max(1, vocab - 100), vocab), plain._gen(seed)
+    value = rng.choice([torch.finfo(dtype).min, torch.finfo(dtype).min / 2, -30000.0])
+    mask = torch.rand((rows, vocab), generator=gen, device=DEV) < rng.choice([0.1, 0.9, 0.999])
+    mask[:, rng.randrange(real)] = False
+    if rng.random() < 0.5:
+        mask[:, : vocab // 2] = mask[:, :1]
+        mask[:, real - 1] = False
+    z = plain._logits(rows, vocab, seed, dtype, scale=rng.choice([0.01, 1.0, 4.0])).masked_fill(mask, NEG)
+    k = min(int((~mask[:, :real]).sum(1).min()), rng.choice([0, 1, 8, 64]))
+    target = (torch.rand((rows, real), generator=gen, device=DEV) * ~mask[:, :real]).argmax(1)
+    temp = 0.3 + 2 * torch.rand(rows, generator=gen, device=DEV) if rng.random() < 0.5 else None
+    given = z.masked_fill(mask, value)
+    given[:, real:] = rng.choice([float("nan"), float("inf"), value])
+    given = draws._inside(rng, given).requires_grad_(True)
+    s = ops.deterministic_scores_from_logits(given, target, top_k=k, temperature=temp, real_vocab_size=real)
+    plain._check(s, z[:, :real], target, k, temp, vocab)
+    g = [torch.randn(rows, generator=gen, device=DEV) for _ in range(3)]
+    (grad,) = torch.autograd.grad([s.logp, s.lse, s.entropy], [given], g)
+    with torch.no_grad():
+        want, size = plain._gradient(z[:, :real], target, temp, None, *g, None)
+        off = (grad[:, :real].double() - want).abs()
+        tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-115
+        assert bool((off <= plain.HALF_STEP[dtype] * want.abs() + size + tiny).all()) and not bool(grad[:, real:].any())
