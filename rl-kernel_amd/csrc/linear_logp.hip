@@ -686,8 +686,9 @@ __global__ __launch_bounds__(kMergeThreads) void linear_logp_merge_kernel(const 
     if (bad_temperature) l = __builtin_nanf("");
     if (lse) lse[m] = l;
     if (logp) {
-      float value = clamp ? fminf(zt - l, 0.f) : zt - l;
-      if (bad_temperature || bad_target) value = __builtin_nanf("");  // fminf would drop a NaN operand
+      float value = zt - l;
+      if (clamp && value > 0.f) value = 0.f;  // (fminf would drop a NaN: a row without a distribution must not look certain)
+      if (bad_temperature || bad_target) value = __builtin_nanf("");
       logp[m] = value;
     }
     if (target_logit) target_logit[m] = zt;

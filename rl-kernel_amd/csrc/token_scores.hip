@@ -638,7 +638,8 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
     if (lane == 0) {
       a.entropy[row] = bad_temperature ? nan : log_sum - weighted / sum;
       a.lse[row] = lse;
-      a.logp[row] = bad_temperature || bad_target ? nan : fminf(zt - lse, 0.f);
+      const float value = zt - lse;
+      a.logp[row] = bad_temperature || bad_target ? nan : value > 0.f ? 0.f : value;  // (fminf would drop a NaN)
     }
   } else {
     const float* stats = a.stats + (int64_t)row * kScorePlanes * kScoreTiles + lane;

@@ -132,3 +132,46 @@ def test_draws_with_masks_of_any_value(ops, seed):
         off = (grad[:, :real].double() - want).abs()
         tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-115
         assert bool((off <= plain.HALF_STEP[dtype] * want.abs() + size + tiny).all()) and not bool(grad[:, real:].any())
+
+
+# ---------------------------------------------------------------------------
+# Rows that have no distribution
+# ---------------------------------------------------------------------------
+
+
+def _nan(t):
+    return torch.isnan(t).reshape(t.size(0), -1).all(1)
+
+
+@pytest.mark.parametrize("tokens", [6, 300, 1100])
+@pytest.mark.parametrize("k", [0, 4])
+def test_diverged_hidden_states(ops, tokens, k):
+    vocab, hidden = 3000, 64
+    h, w, target = plain._head(tokens, vocab, hidden, 9)
+    w[:, hidden - 1] = 0.0
+    w[9, hidden - 1] = 4.0
+    h[:, hidden - 1] = 0.0
+    clean = ops.deterministic_linear_scores(h, w, target, top_k=k)
+    h[1] = float("nan")
+    h[2, 5] = float("nan")
+    h[3, hidden - 1] = 3e38  # its logit 9 is +inf
+    s = ops.deterministic_linear_scores(h, w, target, top_k=k)
+    logp, _ = ops.deterministic_linear_logp(h, w, target)
+    for t in [s.logp, s.entropy, logp] + ([s.top_logp] if k else []):
+        assert _nan(t)[:6].tolist() == [False, True, True, True, False, False]
+    assert k == 0 or (s.top_ids[3, 0] == 9 and bool(((s.top_ids >= 0) & (s.top_ids < vocab)).all()))
+    for a, b in zip(s, clean):
+        assert a is None or (torch.equal(a[0], b[0]) and torch.equal(a[4:], b[4:]))
+
+
+@pytest.mark.parametrize("tokens", [6, 300, 1100])
+@pytest.mark.parametrize("k", [0, 4])
+def test_a_bias_that_masks_everything(ops, tokens, k):
+    h, w, target = plain._head(tokens, 3000, 64, 9)
+    bias = torch.full((3000,), NEG, device=DEV)
+    s = ops.deterministic_linear_scores(h, w, target, bias, top_k=k)
+    logp, lse = ops.deterministic_linear_logp(h, w, target, bias)
+    assert bool((s.lse == NEG).all()) and torch.equal(lse, s.lse)
+    for t in (s.logp, s.entropy, s.top_logp, logp):
+        assert t is None or bool(torch.isnan(t).all())
+    assert k == 0 or s.top_ids[0].tolist() == [0, 1, 2, 3]
