@@ -483,8 +483,8 @@ int rlk_logits_logp_backward(const void* logits, int dtype, int64_t row_stride, 
  *   entropy = -sum p log p with p = exp(y - lse); top_ids / top_logp [T, top_k]: the columns with the largest logits, equal
  *   ones from the lowest column on (a NaN ranks with -inf), and their log-probabilities.
  * temperature [T] may be NULL. A target outside [0, real_vocab) gives logp = NaN; a temperature that is not positive, a NaN or
- * +inf logit and a row without a logit above -inf give NaN throughout (lse is -inf for the latter). The bits of logp and lse are
- * those of rlk_logp_from_logits with 64 tiles where 64 divides V.
+ * +inf logit and a row without a logit above -inf give NaN throughout (lse is -inf for the latter, unless one is NaN). The bits of logp
+ * and lse are those of rlk_logp_from_logits with 64 tiles where 64 divides V and the row's logits are numbers.
  * top_k: 0 (top_logp and top_ids may be NULL) to RLK_SCORES_MAX_TOP_K; at most RLK_SCORES_MAX_ROWS rows and RLK_SCORES_MAX_VOCAB columns. A
  * row's results never depend on the other rows.
  */
@@ -511,7 +511,8 @@ int rlk_logits_scores_backward(const void* logits, int dtype, int64_t row_stride
  * The same scores from hidden states [T, D] and the lm_head weight [V, D] (bf16): logp and lse are those of rlk_linear_logp_fwd, entropy and
  * alternatives those of its fp32 logits. The logits go through `logits` (fp32 [T, logits_row_stride], as rlk_linear_logp_fwd_logits
  * stores them; 16-byte aligned rows of whole 64 columns), which holds them afterwards; where rlk_linear_scores_needs_logits() is 0
- * it may be NULL, and no logits are written. A token's results never depend on its batch, on top_k or on whether it has logits.
+ * it may be NULL, and no logits are written. A token's results never depend on its batch, on top_k or on whether it has logits. A NaN or
+ * +inf logit gives NaN throughout, as above (rlk_linear_logp_fwd passes over a NaN among nothing but NaN and masked logits).
  */
 size_t rlk_linear_scores_workspace_bytes(int T, int V, int top_k);
 int rlk_linear_scores_needs_logits(const void* hidden, int64_t h_row_stride, const void* weight, int64_t w_row_stride, int has_bias, int T,

@@ -125,6 +125,9 @@ __device__ __forceinline__ void logp_fold_run(const float (&y)[16], int tl, floa
 // of a finite lowest value, so far that its product with a sum is: kFarBelow, from where e() is zero, stands for such distances, as zero
 // times infinity is no number.
 constexpr float kFarBelow = -256.f;
+// Distances are taken from the lowest finite number where nothing is above -inf: exponentials of masked logits are 0 there too, and a NaN
+// among them stays in the sums (which hold 0 until then) until the row's answers are made.
+constexpr float kLowest = -__FLT_MAX__;
 __device__ __forceinline__ void logp_fold_run_weighted(const float (&y)[16], int tl, float& run_m, float& run_s, float& run_w,
                                                        float& run_zt) {
   float tmax = kNegInf;
@@ -137,31 +140,27 @@ __device__ __forceinline__ void logp_fold_run_weighted(const float (&y)[16], int
     run_zt = sel;
   }
   const float old_m = run_m;
-  const float new_m = fmaxf(old_m, tmax);
-  float d = y[0] - new_m;
+  const float new_m = fmaxf(old_m, tmax), from = fmaxf(new_m, kLowest);
+  float d = y[0] - from;
   float e = pinned_exp(d);
   float sum = e, weighted = e * fmaxf(d, kFarBelow);
 #pragma unroll
   for (int c = 1; c < 16; ++c) {
-    d = y[c] - new_m;
+    d = y[c] - from;
     e = pinned_exp(d);
     sum = sum + e;
     weighted = __builtin_fmaf(e, fmaxf(d, kFarBelow), weighted);
   }
-  const float back = old_m - new_m;
+  const float back = old_m - from;
   const float shrink = pinned_exp(back);
-  const float scaled = run_s * shrink;
-  const float moved = __builtin_fmaf(shrink, __builtin_fmaf(run_s, fmaxf(back, kFarBelow), run_w), weighted);
-  const bool any = new_m > kNegInf;
-  run_s = any ? (scaled + sum) : run_s;
-  run_w = any ? moved : run_w;
+  run_w = __builtin_fmaf(shrink, __builtin_fmaf(run_s, fmaxf(back, kFarBelow), run_w), weighted);
+  run_s = run_s * shrink + sum;
   run_m = new_m;
 }
-// A stream's share of its split's weighted sum, seen from the split's maximum.
+// A stream's share of its split's weighted sum, seen from the split's maximum; NaN where it has met one.
 __device__ __forceinline__ float logp_weighted_term(float m, float s, float w, float big) {
-  const float back = fmaxf(m - big, kFarBelow);
-  const float term = pinned_exp(back) * __builtin_fmaf(s, back, w);
-  return m > kNegInf ? term : 0.f;
+  const float back = fmaxf(m - fmaxf(big, kLowest), kFarBelow);
+  return pinned_exp(back) * __builtin_fmaf(s, back, w);
 }
 
 // The 16 stream states of a (split, token), merged in ascending stream order. pm / ps / pz

@@ -6,8 +6,8 @@
 //   alternatives: the top_k columns by (z descending, column ascending), their log-probabilities y - lse
 //
 // One pass over the logits. The running (M, S) follow the reduction contract of logits_logp.hip with 64 tiles to a row
-// (tile = ceil(V / 64) columns), so that logp and lse are that entry's bits wherever 64 divides V; W is carried beside
-// S: a state (m, s, w) seen from a larger maximum n is (s e(m - n), e(m - n) (w + s (m - n))).
+// (tile = ceil(V / 64) columns), so that logp and lse are that entry's bits wherever 64 divides V and the logits are numbers; W is
+// carried beside S: a state (m, s, w) seen from a larger maximum n is (s e(m - n), e(m - n) (w + s (m - n))).
 //
 // The alternatives cost the pass two instructions for each vector of eight logits. A lane of a tile sees a fixed slice of
 // the row (every sixteenth vector of its tile), 1024 slices in all, and notes the largest logit of each, the vector
@@ -57,7 +57,8 @@ struct ScoreState {
 };
 
 // The eight logits of vector g folded into a lane's state. The maximum is taken before the temperature (times a positive
-// number it is the maximum of the products, to the bit), so that alternatives are told apart that scaling makes equal.
+// number it is the maximum of the products, to the bit), so that alternatives are told apart that scaling makes equal. A NaN stays in
+// the sums, wherever it stands (kLowest).
 template <bool HAS_TEMP, bool TOP>
 __device__ __forceinline__ void fold_score_vector(float (&y)[8], float inv_t, int g, ScoreState& st) {
   const float most = max3_f32(max3_f32(max3_f32(y[0], y[1], y[2]), y[3], y[4]), y[5], y[6]);
@@ -73,23 +74,21 @@ __device__ __forceinline__ void fold_score_vector(float (&y)[8], float inv_t, in
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = y[i] * inv_t;
   }
-  float d = y[0] - n;
+  const float from = fmaxf(n, kLowest);
+  float d = y[0] - from;
   float e = pinned_exp(d);
   float sum = e, weighted = e * fmaxf(d, kFarBelow);  // (a masked logit is -inf below: 0 times that is no number)
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
-    d = y[i] - n;
+    d = y[i] - from;
     e = pinned_exp(d);
     sum = sum + e;
     weighted = __builtin_fmaf(e, fmaxf(d, kFarBelow), weighted);
   }
-  const float back = st.m - n;
+  const float back = st.m - from;
   const float shrink = pinned_exp(back);
-  const float scaled = st.s * shrink;
-  const float moved = __builtin_fmaf(shrink, __builtin_fmaf(st.s, fmaxf(back, kFarBelow), st.w), weighted);
-  const bool any = n > kNegInf;
-  st.s = any ? scaled + sum : st.s;
-  st.w = any ? moved : st.w;
+  st.w = __builtin_fmaf(shrink, __builtin_fmaf(st.s, fmaxf(back, kFarBelow), st.w), weighted);
+  st.s = st.s * shrink + sum;
   st.m = n;
 }
 
@@ -97,12 +96,11 @@ __device__ __forceinline__ void fold_score_vector(float (&y)[8], float inv_t, in
 template <int OFFSET>
 __device__ __forceinline__ void merge_score_lanes(int lane, ScoreState& st) {
   const float om = xor_lane<OFFSET>(st.m), os = xor_lane<OFFSET>(st.s), ow = xor_lane<OFFSET>(st.w);
-  const float n = fmaxf(st.m, om);
-  const float my_shrink = pinned_exp(st.m - n), other_shrink = pinned_exp(om - n);
-  const float mine = st.m > kNegInf ? st.s * my_shrink : 0.f;
-  const float theirs = om > kNegInf ? os * other_shrink : 0.f;
-  const float my_w = st.m > kNegInf ? my_shrink * __builtin_fmaf(st.s, fmaxf(st.m - n, kFarBelow), st.w) : 0.f;
-  const float their_w = om > kNegInf ? other_shrink * __builtin_fmaf(os, fmaxf(om - n, kFarBelow), ow) : 0.f;
+  const float n = fmaxf(st.m, om), from = fmaxf(n, kLowest);
+  const float my_shrink = pinned_exp(st.m - from), other_shrink = pinned_exp(om - from);
+  const float mine = st.s * my_shrink, theirs = os * other_shrink;
+  const float my_w = my_shrink * __builtin_fmaf(st.s, fmaxf(st.m - from, kFarBelow), st.w);
+  const float their_w = other_shrink * __builtin_fmaf(os, fmaxf(om - from, kFarBelow), ow);
   // the lower lane's term first on both sides, so that both lanes add in the same order
   st.s = (lane & OFFSET) ? theirs + mine : mine + theirs;
   st.w = (lane & OFFSET) ? their_w + my_w : my_w + their_w;
@@ -204,14 +202,13 @@ __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
   merge_score_lanes<2>(lane, st);
   merge_score_lanes<1>(lane, st);
   if (l16 == 0) {
-    const bool finite = st.m > kNegInf && st.m < -kNegInf;
     float zt = holds_target ? LogitElem<ELEM>::to_float(target_logit) : 0.f;
     if (HAS_TEMP) zt = holds_target ? zt * inv_t : zt;
     float* out = a.stats + (int64_t)row * kScorePlanes * kScoreTiles + tile;
     out[0] = st.m;
-    out[kScoreTiles] = finite ? st.s : 0.f;
+    out[kScoreTiles] = st.s;
     out[2 * kScoreTiles] = zt;
-    out[3 * kScoreTiles] = finite ? st.w : 0.f;
+    out[3 * kScoreTiles] = st.w;
   }
 }
 
@@ -634,7 +631,8 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
     }
     const float weighted = wave_sum_f32(w);
     const float log_sum = logf(sum);
-    lse = bad_temperature ? nan : big + log_sum;
+    const bool diverged = weighted != weighted;  // (the linear-LogP's maxima and sums pass over a NaN that stands among masked logits)
+    lse = bad_temperature || diverged ? nan : big + log_sum;
     if (lane == 0) {
       a.entropy[row] = bad_temperature ? nan : log_sum - weighted / sum;
       a.lse[row] = lse;
@@ -644,13 +642,13 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
   } else {
     const float* stats = a.stats + (int64_t)row * kScorePlanes * kScoreTiles + lane;
     const float m = stats[0], s = stats[kScoreTiles], w = stats[3 * kScoreTiles];
-    const float big = wave_max_f32(m);
-    const float shrink = pinned_exp(m - big);
-    const float term = m > kNegInf ? s * shrink : 0.f;
+    const float big = wave_max_f32(m), from = fmaxf(big, kLowest);
+    const float shrink = pinned_exp(m - from);
+    const float term = s * shrink;
     float sum = 0.f;  // (ascending)
 #pragma unroll 8
     for (int t = 0; t < kScoreTiles; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
-    const float weighted = wave_sum_f32(m > kNegInf ? shrink * __builtin_fmaf(s, fmaxf(m - big, kFarBelow), w) : 0.f);
+    const float weighted = wave_sum_f32(shrink * __builtin_fmaf(s, fmaxf(m - from, kFarBelow), w));
     const float log_sum = logf(sum);
     lse = bad_temperature ? nan : big + log_sum;
     const float zt = wave_sum_f32(stats[2 * kScoreTiles]);

@@ -175,3 +175,69 @@ def test_a_bias_that_masks_everything(ops, tokens, k):
     for t in (s.logp, s.entropy, s.top_logp, logp):
         assert t is None or bool(torch.isnan(t).all())
     assert k == 0 or s.top_ids[0].tolist() == [0, 1, 2, 3]
+
+
+def _answers(s):
+    return [t for t in (s.logp, s.lse, s.entropy, s.top_logp) if t is not None]
+
+
+def _rows_with_nan(vocab, dtype, mask):
+    """Rows in which a NaN has nothing but NaN and masked logits around it, or before it, and two that have none."""
+    nan = float("nan")
+    z = plain._logits(9, vocab, 3, dtype)
+    z[0, :8] = nan  # a whole vector
+    z[1, :8], z[1, 3] = mask, nan
+    z[2] = nan
+    z[3, : -(-vocab // 64)] = nan  # a whole tile
+    z[4], z[4, vocab // 2] = mask, nan
+    z[5, vocab - 1] = nan
+    z[6, 8:16], z[6, 16:24] = mask, nan
+    z[7, : vocab // 2] = mask
+    return z
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("vocab", [100, 5000, 151936])
+@pytest.mark.parametrize("k,tempered", [(0, False), (5, True)])
+def test_nan_in_any_place_of_a_row(ops, dtype, vocab, k, tempered):
+    target = torch.full((9,), vocab - 2, device=DEV)
+    temp = torch.full((9,), 0.75, device=DEV) if tempered else None
+    for mask in (NEG, torch.finfo(dtype).min):
+        z = _rows_with_nan(vocab, dtype, mask)
+        s = ops.deterministic_scores_from_logits(z, target, top_k=k, temperature=temp)
+        for t in _answers(s):
+            assert _nan(t).tolist() == [True] * 7 + [False] * 2
+        alone = ops.deterministic_scores_from_logits(z[7:], target[7:], top_k=k, temperature=None if temp is None else temp[7:])
+        for a, b in zip(s, alone):
+            assert a is None or torch.equal(a[7:], b)
+        if k:
+            want = torch.sort(z.masked_fill(torch.isnan(z), NEG), dim=1, descending=True, stable=True).indices[:, :k]
+            assert torch.equal(s.top_ids, want)
+
+
+@pytest.mark.parametrize("tokens", [3, 300, 1100])
+@pytest.mark.parametrize("by", ["weight", "bias"])
+@pytest.mark.parametrize("k", [0, 4])
+def test_nan_in_any_place_of_a_head(ops, tokens, by, k):
+    """Sixteen columns are what a lane folds at a time, 1024 a split."""
+    vocab = 3000
+    for first, end, masked in ((0, 16, None), (16, 32, (0, 16)), (1024, 2048, None), (5, 6, (0, 16)), (0, vocab, None)):
+        h, w, target = plain._head(tokens, vocab, 64, 9)
+        bias = torch.zeros(vocab, device=DEV) if by == "bias" or masked else None
+        if masked:
+            bias[slice(*masked)] = NEG
+        if by == "bias":
+            bias[first:end] = float("nan")
+        else:
+            w[first:end] = float("nan")
+        s = ops.deterministic_linear_scores(h, w, target.clamp(min=2500), bias, top_k=k)
+        for t in _answers(s):
+            assert bool(torch.isnan(t).all()), (first, end, masked)
+
+
+@pytest.mark.parametrize("tokens", [6, 300, 1100])
+def test_lse_of_diverged_hidden_states(ops, tokens):
+    h, w, target = plain._head(tokens, 3000, 64, 9)
+    h[1], h[2, 5] = float("nan"), float("nan")
+    for k in (0, 4):
+        assert _nan(ops.deterministic_linear_scores(h, w, target, top_k=k).lse)[:6].tolist() == [False, True, True, False, False, False]
