@@ -803,6 +803,7 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
   __shared__ int hit_col[kScoreMostTop + 1];
   __shared__ float hit_grad[kScoreMostTop + 1];
   __shared__ int hit_count;
+  __shared__ bool any_top;  // a gradient of an alternative that is not 0
   __shared__ float top_sum;
   // from the last row and columns to the first: the forward has left the last ones in the memory-side cache
   const int row = gridDim.x - 1 - blockIdx.x;
@@ -823,6 +824,7 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
     const int64_t wanted = lane < a.top_k && a.g_top ? a.top_ids[(int64_t)row * a.top_k + lane] : -1;
     const float g = wanted >= 0 ? a.g_top[(int64_t)row * a.top_k + lane] : 0.f;
     const float all = wave_sum_f32(g);
+    const uint64_t not_zero = __ballot(g != 0.f);
     const int64_t at = wanted - first;
     const bool take = wanted >= 0 && wanted < a.real && at >= 0 && at < kScoreBackCols;
     const uint64_t mask = __ballot(take);
@@ -838,17 +840,22 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
         hit_grad[count++] = g_logp;
       }
       hit_count = count;
+      any_top = not_zero != 0;
       top_sum = all;
     }
   }
   __syncthreads();
-  const int hits = hit_count;
   const float lse = a.lse[row];
   const bool finite = lse > kNegInf && lse < -kNegInf;
   const float inv_t = a.temperature ? 1.0f / a.temperature[row] : 1.0f;
   const float g_entropy = a.g_entropy ? a.g_entropy[row] : 0.f;
   const float entropy = a.g_entropy ? a.entropy[row] : 0.f;
-  const float slope = (a.g_lse ? a.g_lse[row] : 0.f) - g_logp - top_sum;
+  const float g_lse = a.g_lse ? a.g_lse[row] : 0.f;
+  const float slope = g_lse - g_logp - top_sum;
+  // A row that no gradient reaches has none, whatever it holds: a token that a loss leaves out must not make a weight's gradient NaN.
+  const bool reached = g_logp != 0.f || g_lse != 0.f || g_entropy != 0.f || any_top;
+  const int hits = reached ? hit_count : 0;
+  const float scale = reached ? inv_t : 0.f;
   // lse and the gradients of the row in registers: from here on a logit costs an exponential and a few products
 #pragma unroll
   for (int u = 0; u < kScoreBackVectors; ++u) {
@@ -863,7 +870,6 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
         const float d = __builtin_fmaf(z[i], inv_t, -lse);  // log p
         const float p = pinned_exp(d);
         out[i] = p * __builtin_fmaf(-g_entropy, fmaxf(d, kFarBelow) + entropy, slope);
-        out[i] = col + i < a.real ? out[i] : 0.f;
       }
     } else {
 #pragma unroll
@@ -875,7 +881,7 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
       for (int i = 0; i < 8; ++i) out[i] = at == i ? out[i] + hit_grad[h] : out[i];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = out[i] * inv_t;
+    for (int i = 0; i < 8; ++i) out[i] = col + i < a.real ? out[i] * scale : 0.f;
     RowVector<OUT> packed;
     packed.pack(out);
     packed.template store_edge<STREAM>(row_out, col, a.grad_cols);

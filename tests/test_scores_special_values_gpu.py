@@ -4,6 +4,7 @@
 from __future__ import annotations
 
 import random
+from contextlib import nullcontext
 
 import pytest
 import test_operators_random_gpu as draws
@@ -241,3 +242,51 @@ def test_lse_of_diverged_hidden_states(ops, tokens):
     h[1], h[2, 5] = float("nan"), float("nan")
     for k in (0, 4):
         assert _nan(ops.deterministic_linear_scores(h, w, target, top_k=k).lse)[:6].tolist() == [False, True, True, False, False, False]
+
+
+# ---------------------------------------------------------------------------
+# Their gradients
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("k", [0, 3])
+def test_rows_that_no_gradient_reaches(ops, dtype, k):
+    """Zeros, and zeros behind the real columns of every row, temperatures of nothing among them."""
+    rows, vocab, real = 6, 9000, 8990
+    z = plain._logits(rows, vocab, 3, dtype)
+    z[:, real:] = float("nan")
+    z[3, 5] = float("nan")
+    temp = torch.tensor([1.0, 0.0, -1.0, 1.0, 0.0, 0.7], device=DEV)
+    z.requires_grad_(True)
+    s = ops.deterministic_scores_from_logits(z, torch.arange(rows, device=DEV), top_k=k, temperature=temp, real_vocab_size=real)
+    outputs = [s.logp, s.lse, s.entropy] + ([s.top_logp] if k else [])
+    g = [torch.ones_like(o) for o in outputs]
+    for t in g:
+        t[1:4] = 0.0
+    (grad,) = torch.autograd.grad(outputs, [z], g)
+    assert not bool(grad[1:4].any()) and not bool(grad[:, real:].any()) and bool(grad[[0, 5]].any(1).all())
+
+
+@pytest.mark.parametrize("tokens", [7, 300, 1100])
+@pytest.mark.parametrize("k", [0, 3])
+@pytest.mark.parametrize("kept", [True, False])
+def test_tokens_that_a_loss_leaves_out(ops, tokens, k, kept):
+    h, w, target = plain._head(tokens, 3001, 64, 9)
+    temp = torch.ones(tokens, device=DEV)
+    quiet = [2, 5]
+    h.requires_grad_(True), w.requires_grad_(True)
+
+    def grads():
+        with nullcontext() if kept else ops.recompute_logits():
+            s = ops.deterministic_linear_scores(h, w, target, top_k=k, temperature=temp)
+            outputs = [s.logp, s.entropy] + ([s.top_logp] if k else [])
+            g = [torch.randn(o.shape, generator=plain._gen(20 + i), device=DEV) for i, o in enumerate(outputs)]
+            for t in g:
+                t[quiet] = 0.0
+            return torch.autograd.grad(outputs, [h, w], g)
+
+    clean = grads()
+    temp[quiet] = 0.0
+    for a, b in zip(grads(), clean):
+        assert torch.equal(a, b)
