@@ -854,8 +854,10 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
   const float slope = g_lse - g_logp - top_sum;
   // A row that no gradient reaches has none, whatever it holds: a token that a loss leaves out must not make a weight's gradient NaN.
   const bool reached = g_logp != 0.f || g_lse != 0.f || g_entropy != 0.f || any_top;
-  const int hits = reached ? hit_count : 0;
-  const float scale = reached ? inv_t : 0.f;
+  // Of a row without a distribution: zeros where everything is masked (lse = -inf), as no answer moves with a logit; NaN where the row is NaN.
+  const int hits = reached && finite ? hit_count : 0;
+  const float scale = !reached ? 0.f : finite ? inv_t : 1.f;
+  const float without = reached && lse != kNegInf ? __builtin_nanf("") : 0.f;
   // lse and the gradients of the row in registers: from here on a logit costs an exponential and a few products
 #pragma unroll
   for (int u = 0; u < kScoreBackVectors; ++u) {
@@ -873,7 +875,7 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = 0.f;
+      for (int i = 0; i < 8; ++i) out[i] = without;  // (columns behind the real ones: 0 below)
     }
     for (int h = 0; h < hits; ++h) {
       const int at = hit_col[h] - (int)col;

@@ -123,7 +123,8 @@ def hip_deterministic_scores_from_logits(
 
     ``temperature`` (a number, or one per row; not differentiated) divides the logits; ``real_vocab_size`` leaves out the columns behind it, whatever
     they hold. Logits of ``-inf`` are tokens that cannot be drawn: they add nothing to ``lse`` and ``entropy`` and have no
-    gradient of their own. A row without any other has no distribution: its ``lse`` is ``-inf``, its other answers are NaN.
+    gradient of their own. A row without any other has no distribution: its ``lse`` is ``-inf``, its other answers are NaN, its
+    gradient is zero. A row that is NaN has a NaN gradient where one of its answers is differentiated with a factor other than 0.
 
     Without ``validate`` no value is read back: an id outside of the real vocabulary gives ``logp = NaN``, a temperature that is
     not positive NaN throughout. With it such a call raises ``ValueError`` (and cannot be captured into a graph).

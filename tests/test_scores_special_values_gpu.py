@@ -290,3 +290,67 @@ def test_tokens_that_a_loss_leaves_out(ops, tokens, k, kept):
     temp[quiet] = 0.0
     for a, b in zip(grads(), clean):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("asked", ["logp", "lse", "entropy", "top_logp", "all"])
+def test_gradients_of_rows_without_a_distribution(ops, dtype, asked):
+    """NaN on the real columns where a row is NaN and a gradient reaches it, zeros where a mask has left nothing or where none does."""
+    rows, vocab, real, k = 9, 9000, 8999, 3
+    z = plain._logits(rows, vocab, 3, dtype)
+    z[1, 77] = float("nan")
+    z[2, 8500] = float("inf")
+    z[3] = NEG
+    z[6, 77] = float("nan")
+    z[8] = float("nan")
+    z[:, real:] = float("nan")
+    temp = torch.ones(rows, device=DEV)
+    temp[4], temp[7] = 0.0, -1.0
+    target = torch.arange(rows, device=DEV) * 900
+    g = [torch.randn(rows, generator=plain._gen(20 + i), device=DEV) for i in range(3)] + [torch.randn((rows, k), generator=plain._gen(30), device=DEV)]
+    for t in g:
+        t[5:8] = 0.0
+    z.requires_grad_(True)
+    s = ops.deterministic_scores_from_logits(z, target, top_k=k, temperature=temp, real_vocab_size=real)
+    outputs = dict(zip(("logp", "lse", "entropy", "top_logp"), zip((s.logp, s.lse, s.entropy, s.top_logp), g)))
+    picked = list(outputs.values()) if asked == "all" else [outputs[asked]]
+    (grad,) = torch.autograd.grad([o for o, _ in picked], [z], [g for _, g in picked])
+    assert _nan(grad[:, :real]).tolist() == [False, True, True, False, True, False, False, False, True]
+    assert not bool(grad[:, real:].any()) and not bool(grad[[3, 5, 6, 7]].any())
+    with torch.no_grad():
+        zero = [t if asked == "all" or name == asked else torch.zeros_like(t) for name, t in zip(outputs, g)]
+        want, size = plain._gradient(z[:1, :real], target[:1], None, s.top_ids[:1], *(t[:1] for t in zero))
+        tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-115
+        assert bool(((grad[:1, :real].double() - want).abs() <= plain.HALF_STEP[dtype] * want.abs() + size + tiny).all())
+
+
+@pytest.mark.parametrize("tokens", [7, 300, 1100])
+@pytest.mark.parametrize("k", [0, 3])
+@pytest.mark.parametrize("kept", [True, False])
+def test_gradients_of_diverged_hidden_states(ops, tokens, k, kept):
+    h, w, target = plain._head(tokens, 3001, 64, 9)
+    h.requires_grad_(True), w.requires_grad_(True)
+
+    def grads():
+        with nullcontext() if kept else ops.recompute_logits():
+            s = ops.deterministic_linear_scores(h, w, target, top_k=k)
+            outputs = [s.logp, s.entropy] + ([s.top_logp] if k else [])
+            return torch.autograd.grad(outputs, [h, w], [torch.randn(o.shape, generator=plain._gen(20 + i), device=DEV) for i, o in enumerate(outputs)])
+
+    clean, _ = grads()
+    with torch.no_grad():
+        h[4, 3] = float("nan")
+    dh, dw = grads()
+    assert _nan(dh)[:7].tolist() == [False] * 4 + [True] + [False] * 2 and bool(torch.isnan(dw).all())
+    rest = torch.arange(tokens, device=DEV) != 4
+    assert torch.equal(dh[rest], clean[rest])
+
+
+@pytest.mark.parametrize("tokens", [5, 1100])
+def test_gradients_under_a_bias_that_masks_everything(ops, tokens):
+    h, w, target = plain._head(tokens, 1000, 64, 9)
+    h.requires_grad_(True), w.requires_grad_(True)
+    s = ops.deterministic_linear_scores(h, w, target, torch.full((1000,), NEG, device=DEV), top_k=2)
+    one = torch.ones(tokens, device=DEV)
+    dh, dw = torch.autograd.grad([s.logp, s.entropy, s.top_logp], [h, w], [one, one, torch.ones((tokens, 2), device=DEV)])
+    assert not bool(dh.any()) and not bool(dw.any())
