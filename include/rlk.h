@@ -500,7 +500,8 @@ int rlk_logits_scores(const void* logits, int dtype, int64_t row_stride, const i
  * d(logits) of sum(g_logp logp + g_lse lse + g_entropy entropy) + sum(g_top top_logp), each gradient [T] (g_top [T, top_k]) or
  * NULL; lse, entropy and top_ids are the forward's. Written once in grad_dtype: that of the logits, or bf16 for fp32 logits; zero on
  * the columns [real_vocab, grad_cols), grad_cols >= V, and on rows whose gradients are all 0 or whose lse is -inf
- * (masked throughout). A row whose lse is NaN gives NaN on its real columns.
+ * (masked throughout). A row whose lse is NaN gives NaN on its real columns. A column of -inf has p = 0, and the gradient of its logp or
+ * top_logp where it is named.
  */
 int rlk_logits_scores_backward(const void* logits, int dtype, int64_t row_stride, const int64_t* target, const float* temperature,
                                const float* lse, const float* entropy, const float* g_logp, const float* g_lse,

@@ -122,8 +122,9 @@ def hip_deterministic_scores_from_logits(
     """:class:`TokenScores` of ``logits [..., V]`` (bf16 / fp16 / fp32) for ``target_ids [...]``; differentiable in ``logits``.
 
     ``temperature`` (a number, or one per row; not differentiated) divides the logits; ``real_vocab_size`` leaves out the columns behind it, whatever
-    they hold. Logits of ``-inf`` are tokens that cannot be drawn: they add nothing to ``lse`` and ``entropy`` and have no
-    gradient of their own. A row without any other has no distribution: its ``lse`` is ``-inf``, its other answers are NaN, its
+    they hold. Logits of ``-inf`` are tokens that cannot be drawn: they add nothing to ``lse`` and ``entropy`` and have ``p = 0``. One that
+    is named nevertheless, by its id or among the alternatives, has a log-probability of ``-inf``, whose gradient is that of any
+    other: 1 for its own logit, ``-p`` for all. A row without any other has no distribution: its ``lse`` is ``-inf``, its other answers are NaN, its
     gradient is zero. A row that is NaN has a NaN gradient where one of its answers is differentiated with a factor other than 0.
 
     Without ``validate`` no value is read back: an id outside of the real vocabulary gives ``logp = NaN``, a temperature that is

@@ -354,3 +354,53 @@ def test_gradients_under_a_bias_that_masks_everything(ops, tokens):
     one = torch.ones(tokens, device=DEV)
     dh, dw = torch.autograd.grad([s.logp, s.entropy, s.top_logp], [h, w], [one, one, torch.ones((tokens, 2), device=DEV)])
     assert not bool(dh.any()) and not bool(dw.any())
+
+
+# ---------------------------------------------------------------------------
+# Masked columns that are asked for
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("vocab,left", [(50, 3), (9000, 20), (9000, 1)])
+def test_masked_targets_and_alternatives(ops, dtype, vocab, left):
+    """logp and top_logp of a masked column are -inf; its gradient is that of any other column, with p = 0."""
+    rows, k = 6, 8 if left < 8 else 40
+    z = plain._logits(rows, vocab, 3, dtype)
+    keep = torch.rand((rows, vocab), generator=plain._gen(4), device=DEV).topk(left, dim=1).indices
+    mask = torch.ones_like(z, dtype=torch.bool).scatter_(1, keep, False)
+    z = z.masked_fill(mask, NEG).requires_grad_(True)
+    target = keep[:, 0].clone()
+    target[:3] = mask[:3].int().argmax(1)
+    s = ops.deterministic_scores_from_logits(z, target, top_k=k)
+    plain._check(s, z.detach(), target, k, None, vocab)
+    assert bool((s.logp[:3] == NEG).all()) and bool((s.top_logp[:, left:] == NEG).all())
+    g = [torch.randn(rows, generator=plain._gen(20 + i), device=DEV) for i in range(3)]
+    g_top = torch.randn((rows, k), generator=plain._gen(30), device=DEV)
+    (grad,) = torch.autograd.grad([s.logp, s.lse, s.entropy, s.top_logp], [z], [*g, g_top])
+    with torch.no_grad():
+        want, size = plain._gradient(z, target, None, s.top_ids, *g, g_top)
+        tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-115
+        assert bool(((grad.double() - want).abs() <= plain.HALF_STEP[dtype] * want.abs() + size + tiny).all())
+
+
+@pytest.mark.parametrize("tokens", [6, 1100])
+def test_masked_targets_and_alternatives_of_hidden_states(ops, tokens):
+    h, w, target = plain._head(tokens, 3000, 64, 9)
+    left = torch.zeros(3000, dtype=torch.bool, device=DEV)
+    left[[7, 1500, 2999]] = True
+    target[:5] = torch.tensor([7, 8, 1500, 0, 2999], device=DEV)
+    bias = torch.where(left, 0.0, NEG)
+    h.requires_grad_(True), w.requires_grad_(True)
+    s = ops.deterministic_linear_scores(h, w, target, bias, top_k=5)
+    with torch.no_grad():
+        z = h.double() @ w.double().t() + bias.double()
+    plain._check(s, z, target, 5, None, 16 * 3000)
+    g, g_top = torch.randn(tokens, generator=plain._gen(20), device=DEV), torch.randn((tokens, 5), generator=plain._gen(30), device=DEV)
+    dh, dw = torch.autograd.grad([s.logp, s.top_logp], [h, w], [g, g_top])
+    with torch.no_grad():
+        zero = torch.zeros_like(g)
+        dz, size = plain._gradient(z, target, None, s.top_ids, g, zero, zero, g_top)
+        slack = 2.0**-8 * dz.abs() + 1.01 * size
+        for got, want, room in ((dh, dz @ w.double(), slack @ w.double().abs()), (dw, dz.t() @ h.double(), slack.t() @ h.double().abs())):
+            assert bool(((got.double() - want).abs() <= 2.0**-8 * want.abs() + 1.01 * room + 2.0**-115).all())
