@@ -479,12 +479,13 @@ int rlk_logits_logp_backward(const void* logits, int dtype, int64_t row_stride, 
 
 /*
  * Scores of given tokens from materialised logits [T, V] (rlk_dtype, rows row_stride elements apart, any alignment):
- *   y = z / temperature over the columns [0, real_vocab); lse = log sum exp(y); logp = y_target - lse;
+ *   y = z / temperature over the columns [0, real_vocab); lse = log sum exp(y); logp = y_target - lse (from |lse| = 65536 on, which
+ *   rounding leaves without the logarithm of the sum, y_target - max y - log sum exp(y - max y), in the gradient too);
  *   entropy = -sum p log p with p = exp(y - lse); top_ids / top_logp [T, top_k]: the columns with the largest logits, equal
  *   ones from the lowest column on (a NaN ranks with -inf), and their log-probabilities.
  * temperature [T] may be NULL. A target outside [0, real_vocab) gives logp = NaN; a temperature that is not positive, a NaN or
  * +inf logit and a row without a logit above -inf give NaN throughout (lse is -inf for the latter, unless one is NaN). The bits of logp
- * and lse are those of rlk_logp_from_logits with 64 tiles where 64 divides V and the row's logits are numbers.
+ * and lse are those of rlk_logp_from_logits with 64 tiles where 64 divides V, the row's logits are numbers and |lse| is below 65536.
  * top_k: 0 (top_logp and top_ids may be NULL) to RLK_SCORES_MAX_TOP_K; at most RLK_SCORES_MAX_ROWS rows and RLK_SCORES_MAX_VOCAB columns. A
  * row's results never depend on the other rows.
  */
@@ -514,7 +515,7 @@ int rlk_logits_scores_backward(const void* logits, int dtype, int64_t row_stride
  * alternatives those of its fp32 logits. The logits go through `logits` (fp32 [T, logits_row_stride], as rlk_linear_logp_fwd_logits
  * stores them; 16-byte aligned rows of whole 64 columns), which holds them afterwards; where rlk_linear_scores_needs_logits() is 0
  * it may be NULL, and no logits are written. A token's results never depend on its batch, on top_k or on whether it has logits. A NaN or
- * +inf logit gives NaN throughout, as above (rlk_linear_logp_fwd passes over a NaN among nothing but NaN and masked logits).
+ * +inf logit gives NaN throughout and |lse| from 65536 on is taken apart, as above; rlk_linear_logp_fwd does neither.
  */
 size_t rlk_linear_scores_workspace_bytes(int T, int V, int top_k);
 int rlk_linear_scores_needs_logits(const void* hidden, int64_t h_row_stride, const void* weight, int64_t w_row_stride, int has_bias, int T,

@@ -275,6 +275,10 @@ __device__ __forceinline__ float wave_max_f32(float v) {
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) { return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) { return wave_reduce(v, ~0u, [](uint32_t a, uint32_t b) { return a < b ? a : b; }); }
 
+// From this size on lse = M + log S loses log S to rounding, all of it where a row is masked throughout with a finite lowest value (its
+// tokens would all look certain): log-probabilities are y - M - log S then, as they are in the row's entropy.
+constexpr float kFarOut = 65536.f;
+
 // What one lane of a wave wrote to LDS is seen by the others behind it.
 __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -384,7 +388,7 @@ __device__ __forceinline__ void tile_columns(const ScoreFinishArgs& a, int tile,
 
 template <int ELEM, bool LINEAR>
 __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, int row, int lane, const uint32_t (&most)[kTileLanes],
-                                                    const uint32_t (&at)[kTileLanes], float lse, float inv_t, uint64_t* keys,
+                                                    const uint32_t (&at)[kTileLanes], float base, float rest, float inv_t, uint64_t* keys,
                                                     uint32_t* picked, uint32_t* where) {
   using E = typename LogitElem<ELEM>::type;
   const int k = a.top_k;
@@ -556,7 +560,7 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     if (i * kWave + lane >= n || rank[i] >= k) continue;
-    float v = from_ordered_bits((uint32_t)(mine[i] >> 32)) * inv_t - lse;
+    float v = (from_ordered_bits((uint32_t)(mine[i] >> 32)) * inv_t - base) - rest;
     if (LINEAR && v > 0.f) v = 0.f;  // the fused linear-LogP clamps its log-probabilities
     const int64_t out = (int64_t)row * k + rank[i];
     a.top_ids[out] = (int64_t)(0xffffffffu - (uint32_t)mine[i]);
@@ -590,7 +594,7 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
   const float temperature = a.temperature ? a.temperature[row] : 1.0f;
   const bool bad_temperature = !(temperature > 0.f);
   const float nan = __builtin_nanf("");
-  float lse;
+  float base, rest;  // log p = y - base - rest
   if constexpr (LINEAR) {  // a lane takes every 64th split; the sums of all are added ascending, as in linear_logp_merge_kernel
     const int64_t plane = (int64_t)a.n_split * a.T;
     const int64_t target = a.target[row];
@@ -632,11 +636,14 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
     const float weighted = wave_sum_f32(w);
     const float log_sum = logf(sum);
     const bool diverged = weighted != weighted;  // (the linear-LogP's maxima and sums pass over a NaN that stands among masked logits)
-    lse = bad_temperature || diverged ? nan : big + log_sum;
+    const float lse = bad_temperature || diverged ? nan : big + log_sum;
+    const bool far = fabsf(lse) >= kFarOut && lse > kNegInf;
+    base = far ? big : lse;
+    rest = far ? log_sum : 0.f;
     if (lane == 0) {
       a.entropy[row] = bad_temperature ? nan : log_sum - weighted / sum;
       a.lse[row] = lse;
-      const float value = zt - lse;
+      const float value = (zt - base) - rest;
       a.logp[row] = bad_temperature || bad_target ? nan : value > 0.f ? 0.f : value;  // (fminf would drop a NaN)
     }
   } else {
@@ -650,16 +657,19 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
     for (int t = 0; t < kScoreTiles; ++t) sum = sum + __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(term), t));
     const float weighted = wave_sum_f32(shrink * __builtin_fmaf(s, fmaxf(m - from, kFarBelow), w));
     const float log_sum = logf(sum);
-    lse = bad_temperature ? nan : big + log_sum;
+    const float lse = bad_temperature ? nan : big + log_sum;
+    const bool far = fabsf(lse) >= kFarOut && lse > kNegInf;
+    base = far ? big : lse;
+    rest = far ? log_sum : 0.f;
     const float zt = wave_sum_f32(stats[2 * kScoreTiles]);
     if (lane == 0) {
       const bool bad_target = a.target[row] < 0 || a.target[row] >= a.real;
       a.entropy[row] = bad_temperature ? nan : log_sum - weighted / sum;
       a.lse[row] = lse;
-      a.logp[row] = bad_target ? nan : zt - lse;
+      a.logp[row] = bad_target ? nan : (zt - base) - rest;
     }
   }
-  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, most, at, lse, a.temperature ? 1.0f / temperature : 1.0f, keys, picked, slices);
+  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, most, at, base, rest, a.temperature ? 1.0f / temperature : 1.0f, keys, picked, slices);
 }
 
 // ---------------------------------------------------------------------------
@@ -796,6 +806,45 @@ constexpr int kScoreBackThreads = 256;
 constexpr int kScoreBackVectors = 4;
 constexpr int kScoreBackCols = kScoreBackThreads * kScoreBackVectors * 8;
 
+// A workgroup's sum or maximum of a value per thread, in all of them.
+template <class Op>
+__device__ __forceinline__ float score_block_reduce(float v, float (*waves)[kScoreBackThreads / kWave], Op op) {
+  if ((threadIdx.x & 63) == 0) (*waves)[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = (*waves)[0];
+#pragma unroll
+  for (int w = 1; w < kScoreBackThreads / kWave; ++w) v = op(v, (*waves)[w]);
+  return v;
+}
+
+// The columns [first, end) of a far-out row (kFarOut): its maximum and the logarithm of its sum, which lse does not hold, from the whole row
+// again.
+template <int ELEM, int OUT>
+__device__ __forceinline__ void far_out_columns(const typename LogitElem<ELEM>::type* row, typename LogitElem<OUT>::type* grad, int first, int end,
+                                                int real, float inv_t, float slope, float g_entropy, float entropy, float scale, int hits,
+                                                const int* hit_col, const float* hit_grad) {
+  __shared__ float waves[2][kScoreBackThreads / kWave];
+  auto scaled = [&](int c) __attribute__((always_inline)) { return LogitElem<ELEM>::to_float(row[c]) * inv_t; };
+  float big = kNegInf, sum = 0.f;
+#pragma unroll 1
+  for (int c = threadIdx.x; c < real; c += kScoreBackThreads) big = fmaxf(big, scaled(c));
+  big = score_block_reduce(wave_max_f32(big), &waves[0], [](float a, float b) { return fmaxf(a, b); });
+#pragma unroll 1
+  for (int c = threadIdx.x; c < real; c += kScoreBackThreads) sum = sum + pinned_exp(scaled(c) - big);
+  const float log_sum = logf(score_block_reduce(wave_sum_f32(sum), &waves[1], [](float a, float b) { return a + b; }));
+#pragma unroll 1
+  for (int c = first + threadIdx.x; c < end; c += kScoreBackThreads) {
+    float out = 0.f;
+    if (c < real) {
+      const float d = (scaled(c) - big) - log_sum;
+      out = pinned_exp(d) * __builtin_fmaf(-g_entropy, fmaxf(d, kFarBelow) + entropy, slope);
+      for (int h = 0; h < hits; ++h) out = hit_col[h] == c ? out + hit_grad[h] : out;
+      out = out * scale;
+    }
+    grad[c] = LogitElem<OUT>::from_float(out);
+  }
+}
+
 template <int ELEM, int OUT, bool STREAM>
 __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(ScoreBackwardArgs a) {
   using E = typename LogitElem<ELEM>::type;
@@ -858,6 +907,11 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
   const int hits = reached && finite ? hit_count : 0;
   const float scale = !reached ? 0.f : finite ? inv_t : 1.f;
   const float without = reached && lse != kNegInf ? __builtin_nanf("") : 0.f;
+  if (finite && fabsf(lse) >= kFarOut) {
+    far_out_columns<ELEM, OUT>(row_in, row_out, first, min(first + kScoreBackCols, a.grad_cols), a.real, inv_t, slope, g_entropy, entropy, scale,
+                               hits, hit_col, hit_grad);
+    return;
+  }
   // lse and the gradients of the row in registers: from here on a logit costs an exponential and a few products
 #pragma unroll
   for (int u = 0; u < kScoreBackVectors; ++u) {

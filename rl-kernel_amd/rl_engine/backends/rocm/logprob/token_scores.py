@@ -3,8 +3,9 @@
 What :mod:`.vocab_parallel_logp` and :mod:`.linear_logp` answer with ``(logp, lse)``, with the statistics that a policy update
 and a sampler ask for next to them, from the same pass over the logits, and differentiable in all of them: an entropy bonus is
 ``scores.entropy``, a loss on alternatives ``scores.top_logp``. ``logp`` and ``lse`` carry the bits of those entries (of
-:func:`~.vocab_parallel_logp.hip_deterministic_logp_from_logits` with its 64 tiles, wherever they divide the vocabulary) for rows
-without a NaN; one with a NaN logit, or one of ``+inf``, is NaN throughout.
+:func:`~.vocab_parallel_logp.hip_deterministic_logp_from_logits` with its 64 tiles, wherever they divide the vocabulary) but for two
+kinds of rows: one with a NaN logit, or one of ``+inf``, is NaN throughout; and where ``|lse|`` is 65536 or more, a row masked
+throughout with a finite value, log-probabilities are taken from the row's maximum, as ``lse`` has lost the logarithm of the sum.
 
 Results of a row never depend on the rest of the batch. Nothing is read back from the device unless ``validate`` asks for it,
 so a call can be captured in a HIP graph.

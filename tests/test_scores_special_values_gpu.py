@@ -3,6 +3,7 @@
 
 from __future__ import annotations
 
+import math
 import random
 from contextlib import nullcontext
 
@@ -404,3 +405,79 @@ def test_masked_targets_and_alternatives_of_hidden_states(ops, tokens):
         slack = 2.0**-8 * dz.abs() + 1.01 * size
         for got, want, room in ((dh, dz @ w.double(), slack @ w.double().abs()), (dw, dz.t() @ h.double(), slack.t() @ h.double().abs())):
             assert bool(((got.double() - want).abs() <= 2.0**-8 * want.abs() + 1.01 * room + 2.0**-115).all())
+
+
+# ---------------------------------------------------------------------------
+# Logits so far out that lse does not hold the logarithm of the sum: a row that is masked throughout with a finite value, or an offset
+# ---------------------------------------------------------------------------
+
+
+def _far_out(rows, vocab, dtype):
+    z = plain._logits(rows, vocab, 3)
+    z[0], z[1], z[2] = torch.finfo(dtype).min if dtype != torch.float32 else FP32_LOWEST, -30000.0 if dtype == torch.float16 else -1e9, 60000.0
+    if dtype != torch.float16:
+        z[3] += 1e6
+        z[4] -= 3e6
+        z[5, : vocab // 2], z[5, vocab // 2 :] = -1e30, FP32_LOWEST if dtype == torch.float32 else BF16_LOWEST
+    return z.to(dtype)
+
+
+def _shifted(z):
+    """The logits from the row's largest on, those without a probability in 64 bits masked."""
+    d = z.double() - z.double().amax(1, keepdim=True)
+    return d.masked_fill(d < -1500.0, NEG)
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("vocab", [70, 5000, 20000])
+@pytest.mark.parametrize("tempered", [False, True])
+def test_logits_far_out(ops, dtype, vocab, tempered):
+    """The steps of the tolerances are those of rows around 0: a temperature of 2 scales without rounding, and the distances from the
+    largest logit are what is rounded."""
+    rows, k = 8, 5
+    z = _far_out(rows, vocab, dtype).requires_grad_(True)
+    target = z.argmax(1)
+    temp = torch.full((rows,), 2.0, device=DEV) if tempered else None
+    s = ops.deterministic_scores_from_logits(z, target, top_k=k, temperature=temp)
+    g = [torch.randn(rows, generator=plain._gen(20 + i), device=DEV) for i in range(3)]
+    g_top = torch.randn((rows, k), generator=plain._gen(30), device=DEV)
+    (grad,) = torch.autograd.grad([s.logp, s.lse, s.entropy, s.top_logp], [z], [*g, g_top])
+    with torch.no_grad():
+        d = _shifted(z)
+        want, bound = plain._reference(d, target, k, temp), plain._bound(d, vocab, temp)
+        top = z.double().amax(1) / (2.0 if tempered else 1.0)
+        plain._close(s.lse, want["lse"] + top, bound + 2.0**-23 * top.abs())
+        # (below 65536, in fp16 and of ordinary rows, log p is a difference with the rounded lse)
+        rounded = torch.where(s.lse.abs() < 65536, 2.0**-23 * s.lse.double().abs(), 0.0)
+        plain._close(s.logp, want["logp"], bound + rounded)
+        plain._close(s.entropy, want["entropy"], 2 * (math.log(vocab) + 1) * bound)
+        assert torch.equal(s.top_ids, want["top_ids"])
+        plain._close(s.top_logp, want["top_logp"], (bound + rounded)[:, None])
+        dz, size = plain._gradient(d, target, temp, s.top_ids, *g, g_top)
+        tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-115
+        room = size * (1 + rounded[:, None] * 2.0**24 / (vocab / 1024 + 90))
+        assert bool(((grad.double() - dz).abs() <= plain.HALF_STEP[dtype] * dz.abs() + room + tiny).all())
+
+
+@pytest.mark.parametrize("tokens", [5, 300, 1100])
+@pytest.mark.parametrize("kept", [True, False])
+def test_logits_of_hidden_states_far_out(ops, tokens, kept):
+    """A bias of -10^9 on every column leaves nothing of logits around 0: all tokens are the same, and none is certain."""
+    vocab, k = 3000, 4
+    h, w, target = plain._head(tokens, vocab, 64, 9)
+    h.requires_grad_(True), w.requires_grad_(True)
+    g, g_entropy, g_top = (torch.randn(shape, generator=plain._gen(20 + i), device=DEV) for i, shape in enumerate([(tokens,), (tokens,), (tokens, k)]))
+    with nullcontext() if kept else ops.recompute_logits():
+        s = ops.deterministic_linear_scores(h, w, target, torch.full((vocab,), -1e9, device=DEV), top_k=k)
+        dh, dw = torch.autograd.grad([s.logp, s.entropy, s.top_logp], [h, w], [g, g_entropy, g_top])
+    with torch.no_grad():
+        z = torch.zeros((tokens, vocab), dtype=torch.float64, device=DEV)
+        want, bound = plain._reference(z, target, k), plain._bound(z, 16 * vocab)
+        plain._close(s.logp, want["logp"], bound)
+        plain._close(s.entropy, want["entropy"], 2 * (math.log(vocab) + 1) * bound)
+        plain._close(s.top_logp, want["top_logp"], bound[:, None])
+        assert torch.equal(s.top_ids, want["top_ids"])
+        dz, size = plain._gradient(z, target, None, s.top_ids, g, torch.zeros_like(g), g_entropy, g_top)
+        slack = 2.0**-8 * dz.abs() + 1.01 * size
+        for got, exact, room in ((dh, dz @ w.double(), slack @ w.double().abs()), (dw, dz.t() @ h.double(), slack.t() @ h.double().abs())):
+            assert bool(((got.double() - exact).abs() <= 2.0**-8 * exact.abs() + 1.01 * room + 2.0**-115).all())
