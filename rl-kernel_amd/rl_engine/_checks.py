@@ -16,6 +16,7 @@ from collections.abc import Callable, Iterable
 from typing import Union
 
 import torch
+from torch.autograd import forward_ad
 
 Lazy = Union[bool, Callable[[], bool]]
 Text = Union[str, Callable[[], str]]
@@ -38,6 +39,12 @@ def assert_async_or_raise(condition: torch.Tensor, exception: type, message: str
         torch._assert_async(condition, message)
     elif not bool(condition):
         raise exception(host_message or message)
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """For a kernel's host side, in front of its first look at the values: a forward-mode tangent would be lost there."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
 
 
 class _NoSecondDerivative(torch.autograd.Function):

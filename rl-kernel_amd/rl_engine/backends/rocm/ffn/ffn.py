@@ -22,7 +22,7 @@ import torch
 from torch import Tensor
 
 from rl_engine import _C, _host, _lib
-from rl_engine._checks import enforce, without_second_derivative
+from rl_engine._checks import enforce, refuse_tangents, without_second_derivative
 from rl_engine.backends.rocm.gemm import swiglu_gemm
 from rl_engine.backends.rocm.gemm.det_gemm import (
     det_gemm_backend,
@@ -222,6 +222,7 @@ class _CheckpointedFFNFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
+        refuse_tangents("the gradient of a checkpointed FFN", grad_output)
         _host.refuse_capture_into_another_graph()
         with torch.no_grad():
             grads = _CheckpointedFFNFunction.gradients(ctx, grad_output)
@@ -247,6 +248,7 @@ class _CheckpointedFFNFunction(torch.autograd.Function):
 
 def kept_swiglu_gradients(dy, gate_codes, gate_scales, up_codes, up_scales) -> tuple:
     """``(d_gate, d_up)`` in the shape of ``dy``, from the copies of gate and up."""
+    refuse_tangents("the gradient of checkpointed_swiglu", dy)
     _host.refuse_capture_into_another_graph()
     with torch.no_grad():
         d_gate, d_up, _ = _C.swiglu_mx8_backward(dy.reshape(gate_codes.shape), gate_codes, gate_scales, up_codes, up_scales)
@@ -277,6 +279,7 @@ def checkpointed_swiglu(gate: Tensor, up: Tensor) -> Tensor:
         y = _host.native().mx8_swiglu(gate, up)  # everyday operands, natively
         if y is not None:
             return y
+    refuse_tangents("checkpointed_swiglu", gate, up)
     enforce([
         (isinstance(gate, Tensor) and isinstance(up, Tensor), TypeError, "gate and up must be torch.Tensors."),
         (lambda: gate.dim() >= 1 and gate.shape == up.shape, ValueError, lambda: f"gate and up must share shape, got {tuple(gate.shape)} and {tuple(up.shape)}."),

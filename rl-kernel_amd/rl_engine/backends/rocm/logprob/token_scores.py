@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from rl_engine import _C, _host, _lib
-from rl_engine._checks import enforce, without_second_derivative
+from rl_engine._checks import enforce, refuse_tangents, without_second_derivative
 from rl_engine.backends.rocm.logprob.linear_logp import _logits_to_save, _prepare, _requires_grad
 
 # Logits that nobody keeps go through a buffer of at most this size, whole rows of tiles of 256 tokens at a time: 3328 tokens of
@@ -86,6 +86,7 @@ def _shaped(scores, shape: torch.Size) -> TokenScores:
 def scores_gradient(logits, target_1d, temp, lse, entropy, top_ids, real, g_logp, g_lse, g_entropy, g_top) -> torch.Tensor:
     """d(logits) of the scores of ``logits [rows, V]``, from the forward's answers and the gradients of its outputs (or ``None``)."""
     grads = (g_logp, g_lse, g_entropy, g_top)
+    refuse_tangents("the gradient of token scores", *grads)
     _host.refuse_capture_into_another_graph()
     with torch.no_grad():
         grad = _C.logits_scores_backward(logits, target_1d, real, lse, entropy, top_ids, grads, temperature=temp)
@@ -136,6 +137,7 @@ def hip_deterministic_scores_from_logits(
         scores = _host.native().scores(logits, target_ids, temperature, real, top_k)  # everyday arguments, natively
         if scores is not None:
             return TokenScores(*scores)
+    refuse_tangents("token scores", logits)
     enforce([
         (isinstance(logits, torch.Tensor) and logits.dim() >= 2, ValueError, "logits must be a tensor [..., vocabulary] of at least two dimensions"),
         (lambda: logits.dtype in (torch.bfloat16, torch.float16, torch.float32), TypeError, lambda: f"logits must be bf16, fp16 or fp32, got {logits.dtype}"),
@@ -204,6 +206,7 @@ def linear_scores_gradients(
     """The gradients of ``hidden`` and ``weight`` that are wanted, ``None`` for the other; ``kept``: the forward's logits, or ``None``
     where they are computed again, a part of the tokens at a time."""
     grads = (g_logp, g_lse, g_entropy, g_top)
+    refuse_tangents("the gradient of token scores", *grads)
     _host.refuse_capture_into_another_graph()
     with torch.no_grad():
         tokens, vocab = hidden.size(0), weight.size(0)
@@ -265,6 +268,7 @@ def hip_deterministic_linear_scores(
     tokens without ``top_k``, and else they go through a buffer of at most 2 GiB, a part of the tokens at a time. d(logits) is
     rounded to bf16 once, as there. A ``bias`` is added but not differentiated.
     """
+    refuse_tangents("token scores", hidden, lm_head_weight, bias)
     if bias is not None and torch.is_grad_enabled() and bias.requires_grad:
         raise RuntimeError("token scores do not differentiate the lm_head bias: pass bias.detach()")
     if target_ids.shape != hidden.shape[:-1]:

@@ -16,7 +16,7 @@ from torch import Tensor
 
 from rl_engine import _host, _lib
 from rl_engine._C import _on, _row_stride, _stream_handle
-from rl_engine._checks import enforce, without_second_derivative
+from rl_engine._checks import enforce, refuse_tangents, without_second_derivative
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
 
@@ -64,6 +64,7 @@ def norm_gradients(
 ) -> tuple:  # fmt: skip
     """The gradients of ``block``, ``residual``, ``gate`` and the weights that are wanted, ``None`` for the others. ``block`` and
     ``residual`` are rows or batches of rows; ``dtype``: the type of the normed result (that of ``block``, or of ``residual``)."""
+    refuse_tangents("the gradient of a norm", g_total, g_normed)
     _host.refuse_capture_into_another_graph()
     dtype = dtype or (residual if block is None else block).dtype
     device, width = residual.device, residual.size(-1)
@@ -180,6 +181,7 @@ def gated_residual_norm(
         both = _host.native().norm(block, residual, gate, post_weight, weight, eps, residual_scale)  # everyday arguments, natively
         if both is not None:
             return both
+    refuse_tangents("gated_residual_norm", block, residual, weight, post_weight, gate)
     _check_rows(block, "block")
     _check_beside(residual, "residual", block, block.dtype)
     if residual.shape != block.shape:
@@ -206,6 +208,7 @@ def rms_norm(x: Tensor, weight: Tensor, *, eps: float = 1e-6, dtype: Optional[to
         both = _host.native().norm(None, x, None, None, weight, eps, 1.0)
         if both is not None:
             return both[1]
+    refuse_tangents("rms_norm", x, weight)
     _check_rows(x, "x")
     dtype = x.dtype if dtype is None else dtype
     if dtype not in _DTYPES or x.dtype not in (dtype, torch.float32):
