@@ -297,6 +297,11 @@ def checkpointed_swiglu(gate: Tensor, up: Tensor) -> Tensor:
     return y.reshape(shape)
 
 
+def _check_checkpoint_bits(checkpoint_bits) -> None:
+    if checkpoint_bits not in (None, 8) or isinstance(checkpoint_bits, bool):
+        raise ValueError(f"checkpoint_bits must be None or 8, got {checkpoint_bits!r}.")
+
+
 def qwen3_ffn(
     rmsnorm_output: Tensor, gate_weight: Tensor, up_weight: Tensor, down_weight: Tensor, *,
     fused_gate_up_weight: Tensor | None = None, tp_group: Any = None, cp_group: Any = None,
@@ -310,8 +315,7 @@ def qwen3_ffn(
     gradients are still returned for the separate gate / up weights. ``checkpoint_bits=8``: what waits for the backward waits in
     eight bits (:func:`checkpointed_swiglu`); the output's bits are the same, the gradients those of the copies.
     """
-    if checkpoint_bits not in (None, 8) or isinstance(checkpoint_bits, bool):
-        raise ValueError(f"checkpoint_bits must be None or 8, got {checkpoint_bits!r}.")
+    _check_checkpoint_bits(checkpoint_bits)
     if not isinstance(sequence_parallel, bool):
         raise TypeError("sequence_parallel must be a bool.")
     for name, value in (("deterministic", deterministic), ("disable_split_k", disable_split_k)):
@@ -344,6 +348,7 @@ def qwen3_ffn_block(
     """One FFN block of a transformer: ``normed``, the norm of the ``residual`` stream (``ops.norm.rms_norm`` for the first block),
     through :func:`qwen3_ffn`, and what stands behind it (``ops.norm.gated_residual_norm``). Returns the new residual stream and
     its norm with ``next_norm_weight``, which the next block takes."""
+    _check_checkpoint_bits(checkpoint_bits)
     if fused_gate_up_weight is not None and not torch.is_grad_enabled():
         y = qwen3_ffn_packed_inference(normed, fused_gate_up_weight, down_weight)
     else:

@@ -215,3 +215,15 @@ def test_parts_of_the_tokens_fit_their_buffer(rlk_lib):
         assert all((end - first) * per_row <= token_scores._LOGITS_BUFFER_BYTES or end - first == 1 for first, end in parts)
         assert all(first % 256 == 0 for first, _ in parts) or token_scores._LOGITS_BUFFER_BYTES // per_row < 256
     assert len(token_scores._token_chunks(3328, 151936)) == 1 and len(token_scores._token_chunks(3329, 151936)) == 2
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("differentiated", [False, True])
+def test_bits_of_a_block(fused, differentiated):
+    """The packed way of an inference call looks at them as well."""
+    from rl_engine.ops.ffn import qwen3_ffn_block
+
+    x = torch.zeros(64, 64, dtype=BF16)
+    for bits in (4, 16, True, "8"):
+        with torch.set_grad_enabled(differentiated), pytest.raises(ValueError, match="checkpoint_bits"):
+            qwen3_ffn_block(x, x, x, x, x, fused_gate_up_weight=torch.zeros(128, 64, dtype=BF16) if fused else None, checkpoint_bits=bits)
