@@ -257,7 +257,7 @@ size_t rlk_linear_logp_workspace_bytes(int T, int V);
  *   weight  [V, D] bf16, row stride w_row_stride, unit stride along D (native lm_head layout)
  *   target  [T] int64 GLOBAL vocabulary ids; the local column is target - vocab_start
  *   bias    [V] fp32 or NULL;  temperature [T] fp32 (> 0) or NULL
- *   logp    [T] fp32 out (may be NULL): min(y_target - lse, 0)
+ *   logp    [T] fp32 out (may be NULL): min(y_target - lse, 0), NaN where the difference is
  *   lse     [T] fp32 out (may be NULL)
  *   real_vocab_end: local column bound of the real vocabulary (columns >= it are
  *                   padding and contribute -inf / 0); pass V for "no padding".

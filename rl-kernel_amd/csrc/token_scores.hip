@@ -107,9 +107,9 @@ __device__ __forceinline__ void merge_score_lanes(int lane, ScoreState& st) {
   st.m = n;
 }
 
-// HBM-bound: 2048 x 131072 bf16 93 us = 5.8 TB/s, with alternatives 105; one row of 151936 7 us, launch and latency. (A form for few rows,
-// one wave to a workgroup and eight vectors of a lane on their way, took 0.3 us less up to 64 rows of 151936 bf16 logits, 0.3 to 2
-// more at the other sizes.)
+// HBM-bound: 2048 x 131072 bf16 104 us = 5.2 TB/s, with alternatives 115 (logits that rotate through 1.6 GB); one row of 151936 7 us, launch
+// and latency. (A form for few rows, one wave to a workgroup and eight vectors of a lane on their way, took 0.3 us less up to 64 rows of
+// 151936 bf16 logits, 0.3 to 2 more at the other sizes.)
 template <int ELEM, bool HAS_TEMP, bool TOP, bool NT>
 __device__ __forceinline__ void score_tiles(const ScoreArgs& a) {
   using E = typename LogitElem<ELEM>::type;
@@ -568,7 +568,7 @@ __device__ __forceinline__ void finish_alternatives(const ScoreFinishArgs& a, in
   }
 }
 
-// 2048 rows: 3 us, 17 with 64 alternatives (17 MB of slices, then two lines of logits for each of some 80 vectors of a row); one row: 2 us,
+// 2048 rows: 5 us, 17 with 64 alternatives (17 MB of slices, then two lines of logits for each of some 80 vectors of a row); one row: 2 us,
 // 5 with 20 alternatives, a chain of dependent reads and searches whose code is fetched as it is run: short loops throughout.
 template <int ELEM, bool LINEAR>
 __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) {
@@ -780,8 +780,8 @@ __global__ __launch_bounds__(256) void linear_score_rows_kernel(LinearRowArgs a)
 
 // ---------------------------------------------------------------------------
 // Gradient: dz = 1/T [ p (g_lse - g_logp - sum g_top - g_entropy (y - lse + entropy)) + g_logp [target] + g_top [ids] ],
-// p = e(y - lse). Elementwise; rounded once to the element type of the output. HBM-bound: 2047 x 151936 bf16 218 us = 5.7 TB/s, fp32 logits to
-// bf16 of 2060 x 151936 365 us = 5.1.
+// p = e(y - lse). Elementwise; rounded once to the element type of the output. HBM-bound: 2047 x 151936 bf16 225 us = 5.5 TB/s, fp32 logits to
+// bf16 of 2060 x 151936 364 us = 5.2.
 // ---------------------------------------------------------------------------
 
 struct ScoreBackwardArgs {
