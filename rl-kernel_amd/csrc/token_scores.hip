@@ -895,7 +895,6 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
   }
   __syncthreads();
   const float lse = a.lse[row];
-  const bool finite = lse > kNegInf && lse < -kNegInf;
   const float inv_t = a.temperature ? 1.0f / a.temperature[row] : 1.0f;
   const float g_entropy = a.g_entropy ? a.g_entropy[row] : 0.f;
   const float entropy = a.g_entropy ? a.entropy[row] : 0.f;
@@ -903,11 +902,12 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
   const float slope = g_lse - g_logp - top_sum;
   // A row that no gradient reaches has none, whatever it holds: a token that a loss leaves out must not make a weight's gradient NaN.
   const bool reached = g_logp != 0.f || g_lse != 0.f || g_entropy != 0.f || any_top;
+  const bool any = reached && lse > kNegInf && lse < -kNegInf;
   // Of a row without a distribution: zeros where everything is masked (lse = -inf), as no answer moves with a logit; NaN where the row is NaN.
-  const int hits = reached && finite ? hit_count : 0;
-  const float scale = !reached ? 0.f : finite ? inv_t : 1.f;
+  const int hits = any ? hit_count : 0;
+  const float scale = any ? inv_t : 1.f;
   const float without = reached && lse != kNegInf ? __builtin_nanf("") : 0.f;
-  if (finite && fabsf(lse) >= kFarOut) {
+  if (any && fabsf(lse) >= kFarOut) {
     far_out_columns<ELEM, OUT>(row_in, row_out, first, min(first + kScoreBackCols, a.grad_cols), a.real, inv_t, slope, g_entropy, entropy, scale,
                                hits, hit_col, hit_grad);
     return;
@@ -918,7 +918,7 @@ __global__ __launch_bounds__(kScoreBackThreads) void score_backward_kernel(Score
     const int64_t col = first + (int64_t)(u * kScoreBackThreads + threadIdx.x) * 8;
     if (col >= a.grad_cols) break;
     float out[8];
-    if (col < a.real && finite) {
+    if (col < a.real && any) {
       float z[8];
       raw[u].unpack(z);
 #pragma unroll

@@ -481,3 +481,15 @@ def test_logits_of_hidden_states_far_out(ops, tokens, kept):
         slack = 2.0**-8 * dz.abs() + 1.01 * size
         for got, exact, room in ((dh, dz @ w.double(), slack @ w.double().abs()), (dw, dz.t() @ h.double(), slack.t() @ h.double().abs())):
             assert bool(((got.double() - exact).abs() <= 2.0**-8 * exact.abs() + 1.01 * room + 2.0**-115).all())
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+def test_logits_far_out_that_no_gradient_reaches(ops, dtype):
+    z = _far_out(8, 9000, dtype).requires_grad_(True)
+    s = ops.deterministic_scores_from_logits(z, z.argmax(1), top_k=2)
+    outputs = [s.logp, s.lse, s.entropy, s.top_logp]
+    g = [torch.zeros_like(o) for o in outputs]
+    for t in g:
+        t[6] = 1.0
+    (grad,) = torch.autograd.grad(outputs, [z], g)
+    assert not bool(grad[:6].any()) and not bool(grad[7].any()) and bool(grad[6].any())
