@@ -483,9 +483,10 @@ int rlk_logits_logp_backward(const void* logits, int dtype, int64_t row_stride, 
  *   rounding leaves without the logarithm of the sum, y_target - max y - log sum exp(y - max y), in the gradient too);
  *   entropy = -sum p log p with p = exp(y - lse); top_ids / top_logp [T, top_k]: the columns with the largest logits, equal
  *   ones from the lowest column on (a NaN ranks with -inf), and their log-probabilities.
- * temperature [T] may be NULL. A target outside [0, real_vocab) gives logp = NaN; a temperature that is not positive, a NaN or
- * +inf logit and a row without a logit above -inf give NaN throughout (lse is -inf for the latter, unless one is NaN). The bits of logp
- * and lse are those of rlk_logp_from_logits with 64 tiles where 64 divides V, the row's logits are numbers and |lse| is below 65536.
+ * temperature [T] may be NULL. A target outside [0, real_vocab) gives logp = NaN; a temperature whose reciprocal is not a positive finite
+ * number, a NaN or +inf logit and a row without a logit above -inf give NaN throughout (lse is -inf for the latter, unless one is NaN). The
+ * bits of logp and lse are those of rlk_logp_from_logits with 64 tiles where 64 divides V, the row's logits are numbers and |lse| is below
+ * 65536.
  * top_k: 0 (top_logp and top_ids may be NULL) to RLK_SCORES_MAX_TOP_K; at most RLK_SCORES_MAX_ROWS rows and RLK_SCORES_MAX_VOCAB columns. A
  * row's results never depend on the other rows.
  */

@@ -591,8 +591,8 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
       }
     }
   }
-  const float temperature = a.temperature ? a.temperature[row] : 1.0f;
-  const bool bad_temperature = !(temperature > 0.f);
+  const float inv_t = a.temperature ? 1.0f / a.temperature[row] : 1.0f;
+  const bool bad_temperature = !(inv_t > 0.f && inv_t < -kNegInf);  // (0 or infinity times a masked logit, or one of 0, is no number)
   const float nan = __builtin_nanf("");
   float base, rest;  // log p = y - base - rest
   if constexpr (LINEAR) {  // a lane takes every 64th split; the sums of all are added ascending, as in linear_logp_merge_kernel
@@ -669,7 +669,7 @@ __global__ __launch_bounds__(kWave) void score_finish_kernel(ScoreFinishArgs a) 
       a.logp[row] = bad_target ? nan : (zt - base) - rest;
     }
   }
-  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, most, at, base, rest, a.temperature ? 1.0f / temperature : 1.0f, keys, picked, slices);
+  if (a.top_k > 0) finish_alternatives<ELEM, LINEAR>(a, row, lane, most, at, base, rest, inv_t, keys, picked, slices);
 }
 
 // ---------------------------------------------------------------------------

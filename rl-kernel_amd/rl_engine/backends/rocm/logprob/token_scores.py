@@ -130,7 +130,8 @@ def hip_deterministic_scores_from_logits(
     gradient is zero. A row that is NaN has a NaN gradient where one of its answers is differentiated with a factor other than 0.
 
     Without ``validate`` no value is read back: an id outside of the real vocabulary gives ``logp = NaN``, a temperature that is
-    not positive NaN throughout. With it such a call raises ``ValueError`` (and cannot be captured into a graph).
+    not positive NaN throughout. With it such a call raises ``ValueError`` (and cannot be captured into a graph). An infinite
+    temperature, or one so small that its reciprocal is, gives NaN throughout as well.
     """
     if not validate and isinstance(logits, torch.Tensor) and logits.dim() == 2 and not torch.compiler.is_compiling():
         real = logits.size(1) if real_vocab_size is None else real_vocab_size

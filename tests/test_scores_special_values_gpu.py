@@ -493,3 +493,24 @@ def test_logits_far_out_that_no_gradient_reaches(ops, dtype):
         t[6] = 1.0
     (grad,) = torch.autograd.grad(outputs, [z], g)
     assert not bool(grad[:6].any()) and not bool(grad[7].any()) and bool(grad[6].any())
+
+
+@pytest.mark.parametrize("vocab", [4096, 5000])
+@pytest.mark.parametrize("k", [0, 3])
+def test_temperatures_without_a_reciprocal(ops, vocab, k):
+    """NaN throughout, whatever masked lanes a row's geometry leaves, and zeros or NaN for the gradient by whether one reaches the row."""
+    temp = torch.tensor([1.0, math.inf, 1e-40, 2.0**126, 2.0**-126], device=DEV)
+    z = plain._logits(5, vocab, 3)
+    z[4] *= 2.0**-126
+    z.requires_grad_(True)
+    s = ops.deterministic_scores_from_logits(z, torch.arange(5, device=DEV), top_k=k, temperature=temp)
+    for t in (s.logp, s.lse, s.entropy, s.top_logp):
+        assert t is None or _nan(t).tolist() == [False, True, True, False, False]
+    (grad,) = torch.autograd.grad(s.logp.sum(), [z])
+    assert _nan(grad)[1:4].tolist() == [True, True, False]
+    for tokens in (5, 300, 1100):
+        h, w, target = plain._head(tokens, vocab, 64, 9)
+        temps = torch.ones(tokens, device=DEV)
+        temps[1], temps[2] = math.inf, 1e-40
+        for t in ops.deterministic_linear_scores(h, w, target, top_k=k, temperature=temps)[:4]:
+            assert t is None or _nan(t)[:5].tolist() == [False, True, True, False, False]
