@@ -588,6 +588,85 @@ int rlk_mx8_swiglu_backward(const void* dy, int64_t ld_dy, int dtype, const int8
                             void* stream);
 
 /*
+ * Rotary positions. Pair i < pairs of a head's elements, (2 i, 2 i + 1) where interleaved and (i, pairs + i) otherwise, is turned by
+ * position * frequencies[i] radians and scaled by magnitude:
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)
+ * and elements from 2 * pairs on are copied. Angles are reduced in 64 bits, the rest is fp32, rounded once. `inverse` turns the
+ * other way (the gradient). tokens = any number of rows of inner_tokens: token t of a tensor starts at
+ * (t / inner_tokens) * outer_stride + (t % inner_tokens) * token_stride; strides in elements, a head's elements are contiguous.
+ */
+#define RLK_ROTARY_MAX_WIDTH 1024
+typedef struct rlk_rotary {
+  const double* frequencies; /* [pairs] */
+  const void* positions;     /* [tokens], int64_t or int32_t */
+  int positions_are_64, pairs, interleaved;
+  float magnitude;
+} rlk_rotary;
+typedef struct rlk_head_rows {
+  const void* x;
+  void* y;
+  int64_t x_outer_stride, x_token_stride, x_head_stride;
+  int64_t y_outer_stride, y_token_stride, y_head_stride;
+  int heads;
+} rlk_head_rows;
+/* host_k may be NULL. y may not alias another token's or head's x. */
+int rlk_rotary_embedding(const rlk_rotary* host_rotary, const rlk_head_rows* host_q, const rlk_head_rows* host_k, int64_t tokens,
+                         int64_t inner_tokens, int width, int dtype, int inverse, void* stream);
+
+/*
+ * A paged cache of keys and values, and the new tokens of a call: sequence s has the tokens [starts[s], starts[s + 1]), the last
+ * ones of its lengths[s] (which counts them). Position p of a sequence lies in row p % page_size of page table[s][p / page_size].
+ * Positions outside of the table's columns and entries outside of [0, pages) are missing: nothing is written there, and a row that
+ * sees one becomes NaN. Nothing is read back: all of it is checked on the device.
+ */
+typedef struct rlk_paged_cache {
+  void* keys;   /* [pages, page_size, key_heads, width], any strides but the last, which is 1 */
+  void* values;
+  const int32_t* table;   /* [sequences, table_columns] */
+  const int32_t* lengths; /* [sequences] */
+  const int32_t* starts;  /* [sequences + 1], ascending */
+  int64_t key_page_stride, key_row_stride, key_head_stride;
+  int64_t value_page_stride, value_row_stride, value_head_stride;
+  int64_t table_row_stride, pages;
+  int page_size, key_heads, width, dtype, sequences, table_columns;
+} rlk_paged_cache;
+
+/*
+ * Writes k and v [tokens, key_heads, width] of the new tokens into their places, k turned by its position on the way, and q
+ * (optional) likewise into host_q->y. host_rotary NULL: nothing turns. Its positions may be NULL: those in the sequence. Tokens
+ * behind the last sequence are not written, their rows of host_q->y become zeros. host_k->y and host_v->y are not read.
+ */
+int rlk_paged_append(const rlk_paged_cache* host_cache, const rlk_rotary* host_rotary, const rlk_head_rows* host_q,
+                     const rlk_head_rows* host_k, const rlk_head_rows* host_v, int64_t tokens, void* stream);
+
+/*
+ * Attention of new tokens over a paged cache that holds their keys and values already:
+ *   out = sum_j softmax_j(scale q k_j) v_j
+ * over the keys j that a row sees: of a token at position p those up to p (causal), of them the last `window` ones (0: all), or the
+ * whole context (not causal; window 0). q head h reads key head h / (heads / key_heads). A row that sees no key is 0, its lse -inf. What a row does not
+ * see does not reach it, whatever it holds. lse (optional, [tokens, heads]) is the natural logarithm of the sum of exponentials.
+ * bf16 or fp16; width a multiple of 8 up to 256; rows of q, keys and values start on 16 bytes. Rows of out behind the last sequence
+ * are left as they were, or become zeros with zero_rest.
+ *
+ * The order of a row's sums is a function of the positions it sees (contract rlk_attention_contract_id()), so its bits do not
+ * depend on the batch, the chunk it came in, the page size or the configuration: keys in tiles of 64 positions, one chain of running
+ * maximum, sum and output over the tiles of a run, and the runs (of 256 positions up to 4096, of 512 up to 16384, of 1024 up to
+ * 65536, of 2048 behind) combined in ascending order.
+ */
+typedef enum rlk_attention_config {
+  RLK_ATTENTION_CFG_AUTO = 0,
+  RLK_ATTENTION_CFG_ROWS16 = 1,  /* a wave for 16 rows of a key head and a run; the runs are combined by a second launch */
+  RLK_ATTENTION_CFG_ROWS64 = 2,  /* four waves of 16 rows, all runs one after the other */
+  RLK_ATTENTION_CFG_ROWS256 = 3, /* eight waves of 32 rows (16 for heads wider than 128) */
+  RLK_ATTENTION_CFG_SPLIT = 0x100 /* OR-ed into the last two: runs side by side, combined by a second launch */
+} rlk_attention_config;
+const char* rlk_attention_contract_id(void);
+size_t rlk_paged_attention_workspace_bytes(const rlk_paged_cache* host_cache, int64_t tokens, int heads, int config);
+int rlk_paged_attention(const rlk_paged_cache* host_cache, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                        int64_t out_token_stride, int64_t out_head_stride, float* lse, int64_t tokens, int heads, float scale,
+                        int causal, int window, int zero_rest, int config, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Value checks without a copy back: flags[0] is set to 1 when one of the n ids lies outside [lo, hi), flags[1] when a
  * temperature (may be NULL) is <= 0. `flags` points to two words the device can write, normally pinned host memory that
  * the caller has zeroed and reads after an event behind this call.

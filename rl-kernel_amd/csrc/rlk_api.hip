@@ -921,6 +921,115 @@ int rlk_block_norm_backward(const rlk_block_norm* n, const void* g_total, const 
   return err == hipSuccess ? RLK_OK : device_error("rlk_block_norm_backward", err);
 }
 
+static int refuse_argument(const char* who, const char* what) {
+  set_last_error("%s: %s", who, what);
+  return RLK_ERR_INVALID_ARGUMENT;
+}
+
+static int check_rotary(const char* who, const rlk_rotary* r, int width, bool own_positions) {
+  if (r == nullptr) return RLK_OK;
+  if (r->pairs < 0 || 2 * (int64_t)r->pairs > width) return refuse_argument(who, "more pairs than a head has room for");
+  if (r->pairs > 0 && r->frequencies == nullptr) return refuse_argument(who, "null frequencies");
+  if (r->positions == nullptr && !own_positions) return refuse_argument(who, "null positions");
+  return RLK_OK;
+}
+
+// One launch's rows: what its index arithmetic holds in 32 bits.
+static bool head_rows_fit(int64_t tokens, int64_t heads, int width) {
+  return tokens >= 0 && tokens < 0x7fffffff && heads >= 0 && heads <= 0x10000 && width >= 1 && width <= RLK_ROTARY_MAX_WIDTH;
+}
+
+int rlk_rotary_embedding(const rlk_rotary* rotary, const rlk_head_rows* q, const rlk_head_rows* k, int64_t tokens, int64_t inner_tokens,
+                         int width, int dtype, int inverse, void* stream) {
+  const char* who = "rlk_rotary_embedding";
+  if (rotary == nullptr || q == nullptr || q->heads < 0 || (k && k->heads < 0) || !head_rows_fit(tokens, (int64_t)q->heads + (k ? k->heads : 0), width))
+    return refuse_argument(who, "null description, or tokens, heads or width out of range");
+  if (!activation_dtype_ok(dtype)) return refuse_argument(who, "unknown dtype");
+  const int rc = check_rotary(who, rotary, width, tokens == 0);
+  if (rc != RLK_OK) return rc;
+  if (tokens == 0 || q->heads + (k ? k->heads : 0) == 0) return RLK_OK;
+  if (inner_tokens < 1 || inner_tokens > tokens || tokens % inner_tokens != 0) return refuse_argument(who, "tokens are no whole number of inner_tokens");
+  if ((q->heads > 0 && (!q->x || !q->y)) || (k && k->heads > 0 && (!k->x || !k->y))) return refuse_argument(who, "null operand");
+  const hipError_t err = rotary_launch(*rotary, *q, k, tokens, inner_tokens, width, dtype, inverse != 0, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error(who, err);
+}
+
+static int check_paged_cache(const char* who, const rlk_paged_cache* c, int64_t tokens, int64_t heads) {
+  if (c == nullptr || c->sequences < 0 || c->sequences > (1 << 24) || c->page_size < 1 || c->page_size > (1 << 24) || c->table_columns < 0 ||
+      c->pages < 0 || c->pages > 0x7fffffff || c->key_heads < 1 || !head_rows_fit(tokens, heads, c->width) || tokens * heads >= 0x7fffffff ||
+      tokens + c->sequences >= 0x7fffffff)
+    return refuse_argument(who, "null description, or sizes out of range");
+  if (tokens == 0) return RLK_OK;
+  if (c->starts == nullptr || (c->sequences > 0 && (c->lengths == nullptr || (c->table_columns > 0 && c->table == nullptr))) ||
+      (c->pages > 0 && (c->keys == nullptr || c->values == nullptr)))
+    return refuse_argument(who, "null cache, table, lengths or starts");
+  if (c->key_page_stride < 0 || c->key_row_stride < 0 || c->key_head_stride < 0 || c->value_page_stride < 0 || c->value_row_stride < 0 ||
+      c->value_head_stride < 0 || c->table_row_stride < 0)
+    return refuse_argument(who, "negative stride");
+  return RLK_OK;
+}
+
+int rlk_paged_append(const rlk_paged_cache* cache, const rlk_rotary* rotary, const rlk_head_rows* q, const rlk_head_rows* k,
+                     const rlk_head_rows* v, int64_t tokens, void* stream) {
+  const char* who = "rlk_paged_append";
+  if (k == nullptr || v == nullptr || cache == nullptr || (q && q->heads < 1)) return refuse_argument(who, "null description, or queries without heads");
+  int rc = check_paged_cache(who, cache, tokens, (q ? (int64_t)q->heads : 0) + 2 * (int64_t)cache->key_heads);
+  if (rc != RLK_OK) return rc;
+  if (!activation_dtype_ok(cache->dtype)) return refuse_argument(who, "unknown dtype");
+  if (k->heads != cache->key_heads || v->heads != cache->key_heads) return refuse_argument(who, "keys and values have the cache's heads");
+  rc = check_rotary(who, rotary, cache->width, true);
+  if (rc != RLK_OK || tokens == 0) return rc;
+  if (!k->x || !v->x || (q && (!q->x || !q->y))) return refuse_argument(who, "null operand");
+  const hipError_t err = paged_append_launch(*cache, rotary, q, *k, *v, tokens, reinterpret_cast<hipStream_t>(stream));
+  return err == hipSuccess ? RLK_OK : device_error(who, err);
+}
+
+const char* rlk_attention_contract_id(void) { return "rlkernel.paged_attention.hip_tiles64_runs256to2048_gfx950.v1"; }
+
+static int check_attention(const char* who, const rlk_paged_cache* c, int64_t tokens, int heads, int config) {
+  int rc = check_paged_cache(who, c, tokens, heads);
+  if (rc != RLK_OK) return rc;
+  if (c->dtype != RLK_DTYPE_BF16 && c->dtype != RLK_DTYPE_FP16) return refuse_argument(who, "dtype is neither bf16 nor fp16");
+  if (heads < 1 || heads % c->key_heads != 0) return refuse_argument(who, "heads are no whole number of key heads");
+  if (c->width % 8 != 0 || c->width > 256) return refuse_argument(who, "width is no multiple of 8 up to 256");
+  const int choice = config & 0xff;
+  if ((config & ~(0xff | RLK_ATTENTION_CFG_SPLIT)) != 0 || choice > RLK_ATTENTION_CFG_ROWS256 ||
+      ((config & RLK_ATTENTION_CFG_SPLIT) != 0 && choice < RLK_ATTENTION_CFG_ROWS64))
+    return refuse_argument(who, "unknown configuration");
+  return RLK_OK;
+}
+
+size_t rlk_paged_attention_workspace_bytes(const rlk_paged_cache* cache, int64_t tokens, int heads, int config) {
+  if (check_attention("rlk_paged_attention_workspace_bytes", cache, tokens, heads, config) != RLK_OK) return 0;
+  return paged_attention_workspace_bytes(*cache, tokens, heads, config);
+}
+
+int rlk_paged_attention(const rlk_paged_cache* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                        int64_t out_token_stride, int64_t out_head_stride, float* lse, int64_t tokens, int heads, float scale,
+                        int causal, int window, int zero_rest, int config, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "rlk_paged_attention";
+  const int rc = check_attention(who, cache, tokens, heads, config);
+  if (rc != RLK_OK || tokens == 0) return rc;
+  if (!(scale > 0.f) || scale > 3.0e38f) return refuse_argument(who, "scale is not a positive finite number");
+  if (window < 0 || (window > 0 && !causal)) return refuse_argument(who, "a window is positive, or 0 for none, and goes with causal");
+  if (!q || !out || q_token_stride < 0 || q_head_stride < 0 || out_token_stride < 0 || out_head_stride < 0) return refuse_argument(who, "null operand or negative stride");
+  auto on16 = [](const void* base, int64_t a, int64_t b, int64_t c) { return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && a % 8 == 0 && b % 8 == 0 && c % 8 == 0; };
+  if (!on16(q, q_token_stride, q_head_stride, 0) || !on16(out, out_token_stride, out_head_stride, 0) ||
+      !on16(cache->keys, cache->key_page_stride, cache->key_row_stride, cache->key_head_stride) ||
+      !on16(cache->values, cache->value_page_stride, cache->value_row_stride, cache->value_head_stride))
+    return refuse_argument(who, "rows of q, out, keys and values start on 16 bytes");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (cache->sequences == 0) return refuse_argument(who, "tokens without a sequence");
+  const size_t need = paged_attention_workspace_bytes(*cache, tokens, heads, config);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) {
+    set_last_error("%s: a 16-byte aligned workspace of %zu bytes is needed, %zu given", who, need, workspace_bytes);
+    return RLK_ERR_INVALID_ARGUMENT;
+  }
+  const hipError_t err = paged_attention_launch(*cache, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, lse, tokens, heads,
+                                                scale, causal != 0, window, zero_rest != 0, config, workspace, s);
+  return err == hipSuccess ? RLK_OK : device_error(who, err);
+}
+
 static int check_mx8(const char* who, int64_t rows, int cols, int dtype, bool complete, bool strides) {
   if (rows < 0 || cols < 0 || cols > (1 << 28)) {
     set_last_error("%s: bad sizes rows=%lld cols=%d", who, (long long)rows, cols);

@@ -249,6 +249,16 @@ hipError_t mx8_swiglu_backward_launch(const void* dy, int64_t ld_dy, int dtype, 
                                       const int8_t* up_codes, const uint8_t* up_scales, void* d_gate, void* d_up, void* y, int64_t rows,
                                       int cols, hipStream_t stream);
 
+// Rotary positions, on their own and on the way into a paged cache (rotary.hip); attention over such a cache (paged_attention.hip).
+hipError_t rotary_launch(const rlk_rotary& rotary, const rlk_head_rows& q, const rlk_head_rows* k, int64_t tokens, int64_t inner, int width,
+                         int dtype, bool inverse, hipStream_t stream);
+hipError_t paged_append_launch(const rlk_paged_cache& cache, const rlk_rotary* rotary, const rlk_head_rows* q, const rlk_head_rows& k,
+                               const rlk_head_rows& v, int64_t tokens, hipStream_t stream);
+size_t paged_attention_workspace_bytes(const rlk_paged_cache& cache, int64_t tokens, int heads, int config);
+hipError_t paged_attention_launch(const rlk_paged_cache& cache, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                                  int64_t out_token_stride, int64_t out_head_stride, float* lse, int64_t tokens, int heads, float scale,
+                                  bool causal, int window, bool zero_rest, int config, void* workspace, hipStream_t stream);
+
 // SwiGLU on rows of `dtype` (rlk_dtype; strides in elements): forward writes y = out; backward
 // writes d_gate = out, d_up = out2.
 hipError_t swiglu_launch(const void* gate, int64_t ld_g, const void* up, int64_t ld_u, const void* dy, int64_t ld_dy,

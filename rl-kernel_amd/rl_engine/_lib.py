@@ -117,6 +117,11 @@ EXPORTED_SYMBOLS = (
     "rlk_mx8_decode",
     "rlk_mx8_swiglu_forward",
     "rlk_mx8_swiglu_backward",
+    "rlk_rotary_embedding",
+    "rlk_paged_append",
+    "rlk_attention_contract_id",
+    "rlk_paged_attention_workspace_bytes",
+    "rlk_paged_attention",
     "rlk_check_rows",
     "rlk_swiglu_fwd",
     "rlk_swiglu_bwd",
@@ -129,6 +134,12 @@ EXPORTED_SYMBOLS = (
 )
 
 
+# rlk_attention_config
+ATTENTION_CONFIGS = {"auto": 0, "rows16": 1, "rows64": 2, "rows256": 3, "rows64_split": 0x102, "rows256_split": 0x103}
+ROTARY_MAX_WIDTH = 1024
+ATTENTION_MAX_WIDTH = 256
+
+
 class BlockNorm(ctypes.Structure):
     """rlk_block_norm."""
 
@@ -139,6 +150,35 @@ class BlockNorm(ctypes.Structure):
         ("eps", ctypes.c_float),
         ("residual_scale", ctypes.c_float),
     ]
+
+
+class Rotary(ctypes.Structure):
+    """rlk_rotary."""
+
+    _fields_ = [
+        ("frequencies", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        *((name, ctypes.c_int) for name in ("positions_are_64", "pairs", "interleaved")), ("magnitude", ctypes.c_float),
+    ]  # fmt: skip
+
+
+class HeadRows(ctypes.Structure):
+    """rlk_head_rows."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        *((f"{t}_{name}_stride", ctypes.c_int64) for t in "xy" for name in ("outer", "token", "head")), ("heads", ctypes.c_int),
+    ]  # fmt: skip
+
+
+class PagedCache(ctypes.Structure):
+    """rlk_paged_cache."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("keys", "values", "table", "lengths", "starts")),
+        *((f"{t}_{name}_stride", ctypes.c_int64) for t in ("key", "value") for name in ("page", "row", "head")),
+        ("table_row_stride", ctypes.c_int64), ("pages", ctypes.c_int64),
+        *((name, ctypes.c_int) for name in ("page_size", "key_heads", "width", "dtype", "sequences", "table_columns")),
+    ]  # fmt: skip
 
 
 class RlkLibraryMissing(RuntimeError):
@@ -273,6 +313,18 @@ def load() -> ctypes.CDLL:
     lib.rlk_mx8_swiglu_forward.argtypes = [vp, i64, vp, i64, i32, vp, vp, vp, vp, vp, i64, i32, vp]
     lib.rlk_mx8_swiglu_backward.restype = i32
     lib.rlk_mx8_swiglu_backward.argtypes = [vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp]
+
+    rotary, rows, cache = c.POINTER(Rotary), c.POINTER(HeadRows), c.POINTER(PagedCache)
+    lib.rlk_rotary_embedding.restype = i32
+    lib.rlk_rotary_embedding.argtypes = [rotary, rows, rows, i64, i64, i32, i32, i32, vp]
+    lib.rlk_paged_append.restype = i32
+    lib.rlk_paged_append.argtypes = [cache, rotary, rows, rows, rows, i64, vp]
+    lib.rlk_attention_contract_id.restype = c.c_char_p
+    lib.rlk_attention_contract_id.argtypes = []
+    lib.rlk_paged_attention_workspace_bytes.restype = sz
+    lib.rlk_paged_attention_workspace_bytes.argtypes = [cache, i64, i32, i32]
+    lib.rlk_paged_attention.restype = i32
+    lib.rlk_paged_attention.argtypes = [cache, vp, i64, i64, vp, i64, i64, vp, i64, i32, f32, i32, i32, i32, i32, vp, sz, vp]
 
     lib.rlk_check_rows.restype = i32
     lib.rlk_check_rows.argtypes = [vp, vp, i32, i64, i64, vp, vp]
