@@ -6,15 +6,14 @@
 // Sums. Scores come transposed, S^T = K Q^T: the matrix instruction's result then has a row's scores in four lanes (and its
 // statistics need two lane swaps), and two 16-key blocks of it, rounded to 16 bits, are the operand of O^T = V^T P^T as they
 // stand: slot 8 g + e of lane group g holds key 16 (e / 4) + 4 g + e % 4 of 32, and the transposing LDS read brings the values in
-// that order. The sum of a row is one more product, with ones, of the same rounded weights.
-//   tile of 64 keys:  m' = max(m, max s),  a = 2^(m - m'),  p = 2^(s - m') rounded to 16 bits,  o = a o + p V,  l = a l + sum p
+// that order. Each of a row's four lanes sums the weights of its own keys; they meet at the end of a run.
+//   tile of 64 keys:  m' = max(m, max s),  a = 2^(m - m'),  p = 2^(s - m'),  o = a o + round(p) V,  l = a l + sum p
 // with s in units of log2(e) * scale. A run of tiles starts from nothing; runs are combined in ascending order:
 //   M' = max(M, m),  O = 2^(m - M') o + 2^(M - M') O  (one fused step), L likewise;  out = O / L,  lse = ln 2 (M + log2 L)
 // Which keys form a tile and which tiles a run is a function of their positions, and keys that a row does not see leave its chain as it is (a
 // factor of 1, a sum with 0). So a row's bits are the same in every kernel below, however its runs are spread over the chip.
-// Statistics and outputs are fp32 throughout; weights are rounded to the inputs' 16 bits (half a step, 2^-9 of a weight in bf16, and the
-// sum under an output is that of the rounded ones, so that a row's weights still add up to one). The logarithm of the sum, where it is
-// wanted, is that of the unrounded ones, summed in 32 bits beside them: a rounding of 2^-9 would be its largest error by far.
+// Statistics and outputs are fp32 throughout; weights are rounded to the inputs' 16 bits for the matrix units (half a step, 2^-9 of a
+// weight in bf16, which averages out over the keys), not for their sum: its logarithm is an answer in 32 bits.
 //
 // What a row does not see may hold anything. Scores are replaced, not added to. Keys and values that no row of a tile sees are
 // read as zeros. Where some rows see a value and others do not, a zero weight would not save them from infinities and NaN in
@@ -53,7 +52,6 @@ struct AttentionArgs {
   float* part_out;  // [run][token][head][width]
   float* part_max;  // [run][token][head]
   float* part_sum;
-  float* part_whole;  // sums of unrounded weights, with lse
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
   int64_t part_rows;  // tokens * heads
   PageDivider by_page, by_group, by_key_heads;
@@ -170,26 +168,30 @@ __device__ __forceinline__ int64_t first_row_tile(const AttentionArgs& a, int s)
 }
 
 // The running state of RB blocks of 16 rows of a wave. Lane l holds row l & 15 of each; of the output elements 16 d + 4 (l >> 4) + i.
-template <int DTYPE, int SLABS, int RB>
+template <int DTYPE, int SLABS, int RB, bool KEEP_Q = true>
 struct Rows {
   typedef Half<DTYPE> H;
   static constexpr int kBlocks = 4 * SLABS;  // of 16 elements
   static constexpr int kSteps = 2 * SLABS;   // of 32 elements
-  u32x4_t q[kSteps][RB];
-  f32x4_t o[kBlocks][RB], l[RB];
+  u32x4_t q[KEEP_Q ? kSteps : 1][RB];  // (or they stay in LDS)
+  f32x4_t o[kBlocks][RB];
   float m[RB];
-  float whole[RB];  // of this lane's keys: the sum of unrounded weights (with lse)
+  float l[RB];  // the sum of the weights of this lane's keys
   Sight sight[RB];
 
   __device__ __forceinline__ void load_q(const AttentionArgs& a, int key_head, const int (&token)[RB], const int (&head)[RB], const bool (&live)[RB],
-                                         int grp) {
+                                         int l16, int grp, char* shelf) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const char* row = a.q + (int64_t)token[rb] * a.q_token_stride + (int64_t)(key_head * a.group + head[rb]) * a.q_head_stride;
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) {
         const int element = 32 * ks + 8 * grp;
-        q[ks][rb] = live[rb] && element < a.cache.width ? *reinterpret_cast<const u32x4_t*>(row + 2 * element) : u32x4_t{0, 0, 0, 0};
+        const u32x4_t v = live[rb] && element < a.cache.width ? *reinterpret_cast<const u32x4_t*>(row + 2 * element) : u32x4_t{0, 0, 0, 0};
+        if (KEEP_Q)
+          q[KEEP_Q ? ks : 0][rb] = v;
+        else
+          *reinterpret_cast<u32x4_t*>(shelf + (rb * SLABS + (ks >> 1)) * 2048 + l16 * 128 + (((4 * (ks & 1) + grp) ^ key_swizzle(l16)) << 4)) = v;
       }
     }
   }
@@ -197,29 +199,31 @@ struct Rows {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       m[rb] = -INFINITY;
-      whole[rb] = 0.f;
-      l[rb] = f32x4_t{0, 0, 0, 0};
+      l[rb] = 0.f;
 #pragma unroll
       for (int d = 0; d < kBlocks; ++d) o[d][rb] = f32x4_t{0, 0, 0, 0};
     }
   }
 
-  // Scores of a tile to weights: s[b][rb] holds keys key0 + 16 b + 4 grp + i. The state is taken to the new maximum.
-  template <bool MASKED, bool WHOLE>
-  __device__ __forceinline__ void weigh_as(const AttentionArgs& a, f32x4_t (&s)[4][RB], int key0, int grp, u32x4_t (&p)[2][RB]) {
+  // Scores of a tile, s[b][rb] of keys key0 + 16 b + 4 grp + i: those of keys that a row does not see go.
+  __device__ __forceinline__ void mask(f32x4_t (&s)[4][RB], int key0, int grp) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const uint32_t range = sight[rb].high > sight[rb].low ? sight[rb].high - sight[rb].low : 0;
+      const uint32_t from = (uint32_t)(key0 + 4 * grp - sight[rb].low);
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b][rb][i] = from + 16 * b + i < range ? s[b][rb][i] : -INFINITY;
+    }
+  }
+
+  // Scores to weights; the state is taken to the new maximum.
+  __device__ __forceinline__ void weigh(const AttentionArgs& a, const f32x4_t (&s)[4][RB], u32x4_t (&p)[2][RB]) {
     float before[RB];
     bool moved = false;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      if (MASKED) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 16 * b + 4 * grp + i;
-            s[b][rb][i] = key >= sight[rb].low && key < sight[rb].high ? s[b][rb][i] : -INFINITY;
-          }
-      }
       float top = s[0][rb][0];
 #pragma unroll
       for (int b = 0; b < 4; ++b)
@@ -234,7 +238,6 @@ struct Rows {
       for (int rb = 0; rb < RB; ++rb) {
         const float f = m[rb] != before[rb] ? exp2_fast(before[rb] - m[rb]) : 1.f;
         l[rb] *= f;
-        if (WHOLE) whole[rb] *= f;
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) o[d][rb] *= f;
       }
@@ -242,24 +245,17 @@ struct Rows {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const float from = m[rb] == -INFINITY ? 0.f : m[rb];
+      float sum[2][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const f32x4_t& v = s[2 * h + (e >> 1)][rb];
           const float x = exp2_fast(__builtin_fmaf(v[2 * (e & 1)], a.scale, -from)), y = exp2_fast(__builtin_fmaf(v[2 * (e & 1) + 1], a.scale, -from));
-          if (WHOLE) whole[rb] += x + y;
+          sum[h][e] = x + y;
           p[h][rb][e] = H::pack(x, y);
         }
-    }
-  }
-  __device__ __forceinline__ void weigh(const AttentionArgs& a, bool masked, f32x4_t (&s)[4][RB], int key0, int grp, u32x4_t (&p)[2][RB]) {
-    if (a.lse != nullptr) {
-      weigh_as<true, true>(a, s, key0, grp, p);  // (masking a whole tile changes nothing)
-    } else if (masked) {
-      weigh_as<true, false>(a, s, key0, grp, p);
-    } else {
-      weigh_as<false, false>(a, s, key0, grp, p);
+      l[rb] += ((sum[0][0] + sum[0][1]) + (sum[0][2] + sum[0][3])) + ((sum[1][0] + sum[1][1]) + (sum[1][2] + sum[1][3]));
     }
   }
 
@@ -272,83 +268,88 @@ struct Rows {
       for (int d = 0; d < 4; ++d) at[d] = row * 128 + (((2 * d + ((l16 >> 1) & 1)) ^ value_swizzle(row)) << 4) + (l16 & 1) * 8;
     }
   };
-  static __device__ __forceinline__ u32x4_t value_fragment(value_bytes_t tile, const ValuePlace& place, int d, int h) {
-    const value_bytes_t at = tile + place.at[d & 3] + (d >> 2) * kSlabBytes + h * 4096;
+  static __device__ __forceinline__ u32x4_t value_fragment(value_bytes_t tile, int place, int d, int h) {
+    const value_bytes_t at = tile + place + (d >> 2) * kSlabBytes + h * 4096;
     const u32x2_t x = read_values_transposed(at), y = read_values_transposed(at + 2048);
     return u32x4_t{x.x, x.y, y.x, y.y};
   }
 
+  // Fragments are read a few products ahead of their use.
+  static constexpr int kAhead = 4;
   __device__ __forceinline__ void add_values(value_bytes_t tile, const ValuePlace& place, const u32x4_t (&p)[2][RB]) {
-    const u32x4_t ones = {H::kOnes, H::kOnes, H::kOnes, H::kOnes};
+    u32x4_t v[kAhead];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int n = 0; n < kAhead; ++n) v[n] = value_fragment(tile, place.at[n & 3], n, 0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) l[rb] = H::mfma(ones, p[h][rb], l[rb]);
+    for (int n = 0; n < 2 * kBlocks; ++n) {
+      const int d = n % kBlocks, h = n / kBlocks, next = n + kAhead;
 #pragma unroll
-      for (int d = 0; d < kBlocks; ++d) {
-        const u32x4_t v = value_fragment(tile, place, d, h);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) o[d][rb] = H::mfma(v, p[h][rb], o[d][rb]);
-      }
+      for (int rb = 0; rb < RB; ++rb) o[d][rb] = H::mfma(v[n % kAhead], p[h][rb], o[d][rb]);
+      if (next < 2 * kBlocks) v[n % kAhead] = value_fragment(tile, place.at[next & 3], next % kBlocks, next / kBlocks);
+      __builtin_amdgcn_sched_barrier(0);  // (or the reads move back to their use)
     }
   }
 
-  // The same for a tile with infinities or NaN among the values that some rows see and others do not: they leave the product, and
-  // what they make of an element (an infinity, or NaN where both come together, from NaN, or from an infinity with a weight of
-  // 0) is added to it. They are counted in one more product: 1 for inf, 128 for -inf, 16384 for NaN, 64 at most of each.
-  __device__ __forceinline__ void add_special_values(value_bytes_t tile, const ValuePlace& place, const u32x4_t (&p)[2][RB], int key0, int grp) {
-    const u32x4_t ones = {H::kOnes, H::kOnes, H::kOnes, H::kOnes};
-    u32x4_t seen[2][RB], lost[2][RB];  // 1 where a row sees a key with a weight, and without one
+  // A tile with infinities or NaN among the values that some rows see and others do not. They leave the product (take_out), and what they
+  // make of an element is added to it behind (an infinity, or NaN where both come together, from NaN, or from an infinity
+  // with a weight of 0). One more product counts them: 1 for inf, 128 for -inf, 16384 for NaN, 64 at most of each. The results wait
+  // in memory, and nothing here is unrolled: this is rare, and in registers it would cost the ordinary tiles theirs.
+  __device__ __forceinline__ void find_special(value_bytes_t tile, const ValuePlace& place, const u32x4_t (&p)[2][RB], int key0, int grp, volatile float* effect) {
+    const uint32_t one = H::kOnes & 0xffffu;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const uint32_t range = sight[rb].high > sight[rb].low ? sight[rb].high - sight[rb].low : 0;
+#pragma unroll 1
+      for (int d = 0; d < kBlocks; ++d) {
+        f32x4_t count = {0, 0, 0, 0};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[rb] = H::mfma(ones, p[h][rb], l[rb]);
+        for (int h = 0; h < 2; ++h) {
+          const u32x4_t v = value_fragment(tile, place.at[0] ^ ((d & 3) << 5), d, h);
+          u32x4_t kinds, any, seen, lost;  // of the values; 1 where a row sees a key with a weight, and without one
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t from = (uint32_t)(key0 + 32 * h + 16 * (e >> 1) + 4 * grp + 2 * (e & 1) - sight[rb].low);
-          const uint32_t sees = (from < range ? 0x8000u : 0u) | (from + 1 < range ? 0x80000000u : 0u);
-          const uint32_t weighs = ((p[h][rb][e] & 0x7fff7fffu) + 0x7fff7fffu) & sees;
-          seen[h][rb][e] = (weighs >> 15) * (H::kOnes & 0xffffu);
-          lost[h][rb][e] = ((sees ^ weighs) >> 15) * (H::kOnes & 0xffffu);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t from = (uint32_t)(key0 + 32 * h + 16 * (e >> 1) + 4 * grp + 2 * (e & 1) - sight[rb].low);
+            const uint32_t sees = (from < range ? 0x8000u : 0u) | (from + 1 < range ? 0x80000000u : 0u);
+            const uint32_t weighs = ((p[h][rb][e] & 0x7fff7fffu) + 0x7fff7fffu) & sees;
+            seen[e] = (weighs >> 15) * one;
+            lost[e] = ((sees ^ weighs) >> 15) * one;
+            const uint32_t w = v[e], special = special_halves<DTYPE>(w);
+            const uint32_t none = special & ((w & H::kFraction) + 0x7fff7fffu);
+            kinds[e] = ((special & ~none & ~w) >> 15) * one | ((special & ~none & w) >> 15) * H::k128 | (none >> 15) * H::k16384;
+            any[e] = (special >> 15) * H::k16384;
+          }
+          count = H::mfma(kinds, seen, count);
+          count = H::mfma(any, lost, count);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t n = (uint32_t)count[i];
+          const float up = (n & 127) != 0 ? INFINITY : 0.f, down = (n & (127 << 7)) != 0 ? -INFINITY : 0.f;
+          effect[4 * (d * RB + rb) + i] = n >= 16384 ? NAN : up + down;
         }
       }
     }
+  }
+  __device__ __forceinline__ void add_special(const volatile float* effect) {
 #pragma unroll
-    for (int d = 0; d < kBlocks; ++d) {
-      f32x4_t count[RB];
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) count[rb] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4_t v = value_fragment(tile, place, d, h), kinds, any;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t w = v[e], special = special_halves<DTYPE>(w);
-          const uint32_t none = special & ((w & H::kFraction) + 0x7fff7fffu);
-          kinds[e] = ((special & ~none & ~w) >> 15) * (H::kOnes & 0xffffu) | ((special & ~none & w) >> 15) * H::k128 | (none >> 15) * H::k16384;
-          any[e] = (special >> 15) * H::k16384;
-          v[e] = w & ~((special >> 15) * 0xffffu);
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          o[d][rb] = H::mfma(v, p[h][rb], o[d][rb]);
-          count[rb] = H::mfma(kinds, seen[h][rb], count[rb]);
-          count[rb] = H::mfma(any, lost[h][rb], count[rb]);
-        }
-      }
+    for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t n = (uint32_t)count[rb][i];
-          const float up = (n & 127) != 0 ? INFINITY : 0.f, down = (n & (127 << 7)) != 0 ? -INFINITY : 0.f;
-          o[d][rb][i] += n >= 16384 ? NAN : up + down;
-        }
-    }
+        for (int i = 0; i < 4; ++i) o[d][rb][i] += effect[4 * (d * RB + rb) + i];
   }
 };
+
+// Zeros in the place of a chunk's infinities and NaN.
+template <int DTYPE>
+__device__ __forceinline__ void take_out_special(char* at) {
+  typedef __attribute__((address_space(3))) u32x4_t* chunk_ptr_t;
+  u32x4_t w = *(chunk_ptr_t)at;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] &= ~((special_halves<DTYPE>(w[e]) >> 15) * 0xffffu);
+  *(chunk_ptr_t)at = w;
+}
 
 // A run joins those before it: factors for both, and the new maximum.
 struct Join {
@@ -385,16 +386,25 @@ struct TileLoader {
   }
 };
 
-// The page of a key's position (what page_at says) where a tile needs the key, -2 where it does not.
-__device__ __forceinline__ int page_of_key(const AttentionArgs& a, int sequence, int key, int low, int high) {
-  if (key < low || key >= high) return -2;
-  return page_at(a.cache, sequence, (int)divide_by((uint32_t)key, a.by_page));
-}
-// The start of a key's row.
-__device__ __forceinline__ const char* key_row_address(const AttentionArgs& a, const char* base, int64_t page_bytes, int64_t row_bytes, int page,
-                                                       int key) {
-  const int row = key - (int)divide_by((uint32_t)key, a.by_page) * a.cache.page_size;
-  return page >= 0 ? base + page * page_bytes + row * row_bytes : reinterpret_cast<const char*>(kSpecialRows[page == -1]);
+// Where a key's row lies. Its table entry is asked for a tile ahead and looked at when the tile is loaded: looked at sooner, it would
+// be waited for together with every load in flight.
+struct KeyPlace {
+  int entry;
+  __device__ __forceinline__ void ask(const AttentionArgs& a, int sequence, int key) {
+    const int column = (int)divide_by((uint32_t)key, a.by_page), last = a.cache.table_columns - 1;
+    const int32_t* from = last >= 0 ? a.cache.table + (int64_t)sequence * a.cache.table_row_stride + min(column, last) : a.cache.starts;
+    entry = *from;
+  }
+};
+// The start of a key's row in a cache: zeros where the tile does not need the key, NaN where its page is missing.
+__device__ __forceinline__ const char* key_row_address(const AttentionArgs& a, const char* base, int64_t page_bytes, int64_t row_bytes, int entry, int key,
+                                                       int low, int high) {
+  const int column = (int)divide_by((uint32_t)key, a.by_page);
+  const int row = key - column * a.cache.page_size;
+  const bool there = (uint32_t)entry < (uint32_t)a.cache.pages && column < a.cache.table_columns;
+  const bool wanted = key >= low && key < high;
+  const char* const special = reinterpret_cast<const char*>(kSpecialRows[wanted]);
+  return wanted && there ? base + entry * page_bytes + row * row_bytes : special;
 }
 
 // ---------------------------------------------------------------------------
@@ -402,13 +412,16 @@ __device__ __forceinline__ const char* key_row_address(const AttentionArgs& a, c
 // tile. SPLIT: a workgroup takes every chunks-th run and leaves the parts in memory.
 // ---------------------------------------------------------------------------
 template <int DTYPE, int SLABS, int RB, int WAVES, bool SPLIT>
-__global__ __launch_bounds__(WAVES * 64) void attention_tile_kernel(const AttentionArgs a) {
-  typedef Rows<DTYPE, SLABS, RB> State;
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_tile_kernel(const AttentionArgs a) {
+  constexpr bool kKeepQ = RB == 1;
+  typedef Rows<DTYPE, SLABS, RB, kKeepQ> State;
   constexpr int kRows = 16 * RB * WAVES;
   constexpr int kGroups = 8 / WAVES;  // groups of 8 keys that a wave loads
   constexpr int kTileBytes = SLABS * kSlabBytes;
-  extern __shared__ char lds[];  // [2][keys, values]
-  __shared__ int special_tile[2];
+  // [2][keys, values], then the queries, block of 16 rows by block, unless they are in registers, then special_tile. Nothing lies in
+  // front of it: 16-byte reads that start on 8 bytes took 62 cycles each instead of 8, and the kernel twice as long.
+  extern __shared__ __align__(16) char lds[];
+  int* const special_tile = reinterpret_cast<int*>(lds + 4 * kTileBytes + (kKeepQ ? 0 : WAVES * RB * SLABS * 2048));  // [2]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, grp = lane >> 4;
 
   // Heads change fastest, so that an XCD's workgroups read few of them; the tiles with the most keys come first.
@@ -462,7 +475,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_tile_kernel(const Attent
     token[rb] = c.first_token + t;
     st.sight[rb] = live[rb] ? sight_of(a, c, t) : Sight{0, 0};
   }
-  st.load_q(a, key_head, token, head, live, grp);
+  char* const shelf = lds + 4 * kTileBytes + wave * RB * SLABS * 2048;
+  st.load_q(a, key_head, token, head, live, l16, grp, shelf);
   st.clear();
   if (tid < 2) special_tile[tid] = 0;
 
@@ -482,10 +496,10 @@ __global__ __launch_bounds__(WAVES * 64) void attention_tile_kernel(const Attent
     const int r = run_of_tile(tile);
     return tile + 1 < run_first_tile(r + 1) ? tile + 1 : run_first_tile(r + a.chunks);
   };
-  int pages[kGroups];
+  KeyPlace where[kGroups];  // of the tile that is loaded next
   auto find_pages = [&](int tile) {
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) pages[j] = page_of_key(a, s, tile * kTileKeys + (wave + j * WAVES) * 8 + (lane >> 3), low, high);
+    for (int j = 0; j < kGroups; ++j) where[j].ask(a, s, tile * kTileKeys + (wave + j * WAVES) * 8 + (lane >> 3));
   };
   auto load_tile = [&](int tile, int stage) {
     char* const to = lds + stage * 2 * kTileBytes;
@@ -493,8 +507,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_tile_kernel(const Attent
     for (int j = 0; j < kGroups; ++j) {
       const int group_of_keys = wave + j * WAVES;
       const int key = tile * kTileKeys + group_of_keys * 8 + (lane >> 3);
-      const char* k = key_row_address(a, loader.keys, loader.key_page, loader.key_row, pages[j], key);
-      const char* v = key_row_address(a, loader.values, loader.value_page, loader.value_row, pages[j], key);
+      const char* k = key_row_address(a, loader.keys, loader.key_page, loader.key_row, where[j].entry, key, low, high);
+      const char* v = key_row_address(a, loader.values, loader.value_page, loader.value_row, where[j].entry, key, low, high);
       const char* const none = reinterpret_cast<const char*>(kSpecialRows[0]);
 #pragma unroll
       for (int slab = 0; slab < SLABS; ++slab) {
@@ -509,10 +523,10 @@ __global__ __launch_bounds__(WAVES * 64) void attention_tile_kernel(const Attent
 
   // Runs combined so far.
   f32x4_t all_o[SPLIT ? 1 : State::kBlocks][RB];
-  float all_m[RB], all_l[RB], all_whole[RB];
+  float all_m[RB], all_l[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    all_m[rb] = -INFINITY, all_l[rb] = all_whole[rb] = 0.f;
+    all_m[rb] = -INFINITY, all_l[rb] = 0.f;
 #pragma unroll
     for (int d = 0; d < (SPLIT ? 1 : State::kBlocks); ++d) all_o[d][rb] = f32x4_t{0, 0, 0, 0};
   }
@@ -551,47 +565,72 @@ __global__ __launch_bounds__(WAVES * 64) void attention_tile_kernel(const Attent
       const int after = next_tile(next);
       if (after < end_tile) find_pages(after);
     }
-    if (wave_live && key0 < wave_last.high && key0 + kTileKeys > wave_first.low) {
-      const value_bytes_t keys = (value_bytes_t)(lds + stage * 2 * kTileBytes), values = keys + kTileBytes;
+    const bool special = mixed && special_tile[stage] == t + 1;
+    const bool busy = wave_live && key0 < wave_last.high && key0 + kTileKeys > wave_first.low;
+    const value_bytes_t keys = (value_bytes_t)(lds + stage * 2 * kTileBytes), values = keys + kTileBytes;
+    u32x4_t p[2][RB];
+    volatile float effect[4 * State::kBlocks * RB];  // (in memory, see find_special)
+    if (busy) {
       f32x4_t scores[4][RB];
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) scores[b][rb] = f32x4_t{0, 0, 0, 0};
+      constexpr int kAhead = 4;
+      u32x4_t k[kAhead], q[2][RB];
+      auto key_fragment = [&](int n) { return read_chunk(keys + key_at[(n >> 2) & 1] + (n >> 3) * kSlabBytes + (n & 3) * 2048); };
+      auto query_fragment = [&](int ks, int rb) {
+        return kKeepQ ? st.q[kKeepQ ? ks : 0][rb] : read_chunk((value_bytes_t)shelf + key_at[ks & 1] + (rb * SLABS + (ks >> 1)) * 2048);
+      };
 #pragma unroll
-      for (int ks = 0; ks < State::kSteps; ++ks)
+      for (int rb = 0; rb < RB; ++rb) q[0][rb] = query_fragment(0, rb);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const u32x4_t k = read_chunk(keys + key_at[ks & 1] + (ks >> 1) * kSlabBytes + b * 2048);
+      for (int n = 0; n < kAhead; ++n) k[n] = key_fragment(n);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) scores[b][rb] = Half<DTYPE>::mfma(k, st.q[ks][rb], scores[b][rb]);
-        }
-      u32x4_t p[2][RB];
-      const bool masked = key0 + kTileKeys > wave_first.high || key0 < wave_last.low;
-      st.weigh(a, masked, scores, key0, grp, p);
-      if (masked && mixed && special_tile[stage] == t + 1)
-        st.add_special_values(values, place, p, key0, grp);
-      else
-        st.add_values(values, place, p);
+      for (int n = 0; n < 4 * State::kSteps; ++n) {
+        const int ks = n >> 2, b = n & 3;
+        if (b == 0 && ks + 1 < State::kSteps)
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) q[(ks + 1) & 1][rb] = query_fragment(ks + 1, rb);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) scores[b][rb] = Half<DTYPE>::mfma(k[n % kAhead], q[ks & 1][rb], scores[b][rb]);
+        if (n + kAhead < 4 * State::kSteps) k[n % kAhead] = key_fragment(n + kAhead);
+        __builtin_amdgcn_sched_barrier(0);  // (or the reads move back to their use)
+      }
+      if (key0 + kTileKeys > wave_first.high || key0 < wave_last.low) st.mask(scores, key0, grp);
+      st.weigh(a, scores, p);
     }
+    if (special) {
+      if (busy) st.find_special(values, place, p, key0, grp, effect);
+      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+      wg_barrier();
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+        for (int slab = 0; slab < SLABS; ++slab)
+          take_out_special<DTYPE>(lds + stage * 2 * kTileBytes + kTileBytes + slab * kSlabBytes + (wave + j * WAVES) * 1024 + lane * 16);
+      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+      wg_barrier();
+    }
+    if (busy) st.add_values(values, place, p);
+    if (special && busy) st.add_special(effect);
     const int this_run = run_of_tile(t);
     if (next >= end_tile || run_of_tile(next) != this_run) {  // the run ends
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        const float whole = sum_over_groups(st.whole[rb]);
+        const float sum = sum_over_groups(st.l[rb]);
         if (SPLIT) {
           if (live[rb]) {
             const int64_t at = (int64_t)this_run * a.part_rows + (int64_t)token[rb] * a.heads + key_head * a.group + head[rb];
-            if (grp == 0) a.part_max[at] = st.m[rb], a.part_sum[at] = st.l[rb][0];
-            if (grp == 0 && a.lse) a.part_whole[at] = whole;
+            if (grp == 0) a.part_max[at] = st.m[rb], a.part_sum[at] = sum;
 #pragma unroll
             for (int d = 0; d < State::kBlocks; ++d)
               if (16 * d + 4 * grp < a.cache.width) *reinterpret_cast<f32x4_t*>(a.part_out + at * a.cache.width + 16 * d + 4 * grp) = st.o[d][rb];
           }
-        } else if (st.l[rb][0] != 0.f) {  // (NaN is a sum too)
+        } else if (sum != 0.f) {  // (NaN is a sum too)
           const Join j = join_maxima(all_m[rb], st.m[rb]);
-          all_l[rb] = join_sums(all_l[rb], st.l[rb][0], j);
-          all_whole[rb] = join_sums(all_whole[rb], whole, j);
+          all_l[rb] = join_sums(all_l[rb], sum, j);
 #pragma unroll
           for (int d = 0; d < State::kBlocks; ++d)
 #pragma unroll
@@ -619,7 +658,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_tile_kernel(const Attent
       if (16 * d + 4 * grp < a.cache.width)
         *reinterpret_cast<u32x2_t*>(to + 2 * (16 * d + 4 * grp)) = u32x2_t{Half<DTYPE>::pack(y[0], y[1]), Half<DTYPE>::pack(y[2], y[3])};
     }
-    if (a.lse && grp == 0) a.lse[(int64_t)token[rb] * a.heads + key_head * a.group + head[rb]] = sees ? lse_of(all_m[rb], all_whole[rb]) : -INFINITY;
+    if (a.lse && grp == 0) a.lse[(int64_t)token[rb] * a.heads + key_head * a.group + head[rb]] = sees ? lse_of(all_m[rb], all_l[rb]) : -INFINITY;
   }
 }
 
@@ -634,7 +673,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void attention_rows_kernel(const At
   typedef Rows<DTYPE, SLABS, 1> State;
   constexpr int kRows = 16;
   constexpr int kTileBytes = SLABS * kSlabBytes;
-  extern __shared__ char lds[];  // [wave][2][values]
+  extern __shared__ __align__(16) char lds[];  // [wave][2][values]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, grp = lane >> 4;
   char* const mine = lds + wave * 2 * kTileBytes;
 
@@ -670,7 +709,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void attention_rows_kernel(const At
     token[0] = c.first_token + i;
     st.sight[0] = live[0] ? sight_of(a, c, i) : Sight{0, 0};
   }
-  st.load_q(a, key_head, token, head, live, grp);
+  st.load_q(a, key_head, token, head, live, l16, grp, nullptr);
   st.clear();
   TileLoader<SLABS> loader;
   loader.init(a, key_head, lane);
@@ -682,17 +721,17 @@ __global__ __launch_bounds__(kRowWaves * 64) void attention_rows_kernel(const At
     const int r = run_of_tile(tile);
     return tile + 1 < run_first_tile(r + 1) ? tile + 1 : run_first_tile(r + a.chunks);
   };
-  int key_pages[4], value_pages[8];
+  KeyPlace key_where[4], value_where[8];  // of the tile that is loaded next
   auto find_pages = [&](int tile) {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) key_pages[b] = page_of_key(a, s, tile * kTileKeys + 16 * b + l16, low, high);
+    for (int b = 0; b < 4; ++b) key_where[b].ask(a, s, tile * kTileKeys + 16 * b + l16);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) value_pages[j] = page_of_key(a, s, tile * kTileKeys + 8 * j + (lane >> 3), low, high);
+    for (int j = 0; j < 8; ++j) value_where[j].ask(a, s, tile * kTileKeys + 8 * j + (lane >> 3));
   };
   auto load_values = [&](int tile, int stage) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const char* v = key_row_address(a, loader.values, loader.value_page, loader.value_row, value_pages[j], tile * kTileKeys + 8 * j + (lane >> 3));
+      const char* v = key_row_address(a, loader.values, loader.value_page, loader.value_row, value_where[j].entry, tile * kTileKeys + 8 * j + (lane >> 3), low, high);
 #pragma unroll
       for (int slab = 0; slab < SLABS; ++slab) {
         const int vc = slab * 8 + loader.value_chunk;
@@ -705,7 +744,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void attention_rows_kernel(const At
   auto load_keys = [&](int tile) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const char* from = key_row_address(a, loader.keys, loader.key_page, loader.key_row, key_pages[b], tile * kTileKeys + 16 * b + l16);
+      const char* from = key_row_address(a, loader.keys, loader.key_page, loader.key_row, key_where[b].entry, tile * kTileKeys + 16 * b + l16, low, high);
 #pragma unroll
       for (int ks = 0; ks < State::kSteps; ++ks) {
         const int element = 32 * ks + 8 * grp;
@@ -752,19 +791,23 @@ __global__ __launch_bounds__(kRowWaves * 64) void attention_rows_kernel(const At
       if (next_tile(next) < end_tile) find_pages(next_tile(next));
     }
     u32x4_t p[2][1];
-    const bool masked = key0 + kTileKeys > first_sight.high || key0 < last_sight.low;
-    st.weigh(a, masked, scores, key0, grp, p);
-    if (special)
-      st.add_special_values(values, place, p, key0, grp);
-    else
-      st.add_values(values, place, p);
+    volatile float effect[4 * State::kBlocks];
+    if (key0 + kTileKeys > first_sight.high || key0 < last_sight.low) st.mask(scores, key0, grp);
+    st.weigh(a, scores, p);
+    if (special) {
+      st.find_special(values, place, p, key0, grp, effect);
+#pragma unroll 1
+      for (int j = 0; j < 8 * SLABS; ++j) take_out_special<DTYPE>(mine + stage * kTileBytes + j * 1024 + lane * 16);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    st.add_values(values, place, p);
+    if (special) st.add_special(effect);
     const int this_run = run_of_tile(t);
     if (next >= end_tile || run_of_tile(next) != this_run) {
-      const float whole = sum_over_groups(st.whole[0]);
+      const float sum = sum_over_groups(st.l[0]);
       if (live[0]) {
         const int64_t at = (int64_t)this_run * a.part_rows + (int64_t)token[0] * a.heads + key_head * a.group + head[0];
-        if (grp == 0) a.part_max[at] = st.m[0], a.part_sum[at] = st.l[0][0];
-        if (grp == 0 && a.lse) a.part_whole[at] = whole;
+        if (grp == 0) a.part_max[at] = st.m[0], a.part_sum[at] = sum;
 #pragma unroll
         for (int d = 0; d < State::kBlocks; ++d)
           if (16 * d + 4 * grp < a.cache.width) *reinterpret_cast<f32x4_t*>(a.part_out + at * a.cache.width + 16 * d + 4 * grp) = st.o[d][0];
@@ -783,7 +826,7 @@ constexpr int kJoinRuns = 64;
 
 template <int DTYPE>
 __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const AttentionArgs a) {
-  __shared__ float run_max[kJoinRuns], run_sum[kJoinRuns], run_whole[kJoinRuns];
+  __shared__ float run_max[kJoinRuns], run_sum[kJoinRuns];
   const int tid = threadIdx.x, lane = tid & 63, width = a.cache.width;
   const int token = blockIdx.x / a.heads, head = blockIdx.x - token * a.heads;
   const int64_t row = (int64_t)token * a.heads + head;
@@ -797,7 +840,7 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
     if (known) sight = sight_of(a, c, token - c.first_token);
   }
   if (!known && !a.zero_rest) return;
-  float top = -INFINITY, sum = 0.f, whole = 0.f, o = 0.f;
+  float top = -INFINITY, sum = 0.f, o = 0.f;
   const int capacity = capacity_of(a);
   const int high = min(sight.high, capacity + 1);
   if (sight.low < high) {
@@ -806,7 +849,6 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
       const int count = min(kJoinRuns, last + 1 - r0);
       __syncthreads();
       if (tid < count) run_max[tid] = a.part_max[(r0 + tid) * a.part_rows + row], run_sum[tid] = a.part_sum[(r0 + tid) * a.part_rows + row];
-      if (tid < count) run_whole[tid] = a.lse ? a.part_whole[(r0 + tid) * a.part_rows + row] : 0.f;
       __syncthreads();
       const float* from = a.part_out + ((int64_t)r0 * a.part_rows + row) * width + (tid < width ? tid : 0);
       const int64_t step = a.part_rows * width;
@@ -820,7 +862,6 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
           if (r + i < count && run_sum[r + i] != 0.f) {
             const Join j = join_maxima(top, run_max[r + i]);
             sum = join_sums(sum, run_sum[r + i], j);
-            whole = join_sums(whole, run_whole[r + i], j);
             o = join_sums(o, v[i], j);
           }
       }
@@ -829,7 +870,7 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
   const bool sees = sight.high > sight.low;
   const float y = sees ? output_of(o, 1.f / sum) : 0.f;
   if (tid < width) *reinterpret_cast<uint16_t*>(out) = (uint16_t)Half<DTYPE>::pack(y, 0.f);
-  if (a.lse && tid == 0) a.lse[row] = sees ? lse_of(top, whole) : -INFINITY;
+  if (a.lse && tid == 0) a.lse[row] = sees ? lse_of(top, sum) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -870,12 +911,12 @@ static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, in
 size_t paged_attention_workspace_bytes(const rlk_paged_cache& c, int64_t tokens, int heads, int config) {
   if (tokens == 0 || c.sequences == 0 || heads == 0) return 0;
   if (!attention_plan(c, tokens, heads, config).split) return 0;
-  return (size_t)run_limit(c) * tokens * heads * (c.width + 3) * sizeof(float);
+  return (size_t)run_limit(c) * tokens * heads * (c.width + 2) * sizeof(float);
 }
 
 template <int DTYPE, int SLABS, int RB, int WAVES, bool SPLIT>
 static hipError_t attention_tiles_launch(const AttentionArgs& a, hipStream_t stream) {
-  constexpr int kLds = 4 * SLABS * kSlabBytes;
+  constexpr int kLds = 4 * SLABS * kSlabBytes + (RB == 1 ? 0 : WAVES * RB * SLABS * 2048) + 16;
   static PerDeviceOnce once;
   const auto kernel = attention_tile_kernel<DTYPE, SLABS, RB, WAVES, SPLIT>;
   const hipError_t err = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, once);
@@ -930,7 +971,6 @@ hipError_t paged_attention_launch(const rlk_paged_cache& cache, const void* q, i
     a.part_out = static_cast<float*>(workspace);
     a.part_max = a.part_out + parts * cache.width;
     a.part_sum = a.part_max + parts;
-    a.part_whole = a.part_sum + parts;
   }
   a.group = heads / cache.key_heads;
   a.by_page = page_divider((uint32_t)cache.page_size);
