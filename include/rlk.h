@@ -645,19 +645,20 @@ int rlk_paged_append(const rlk_paged_cache* host_cache, const rlk_rotary* host_r
  * over the keys j that a row sees: of a token at position p those up to p (causal), of them the last `window` ones (0: all), or the
  * whole context (not causal; window 0). q head h reads key head h / (heads / key_heads). A row that sees no key is 0, its lse -inf. What a row does not
  * see does not reach it, whatever it holds. lse (optional, [tokens, heads]) is the natural logarithm of the sum of exponentials.
- * bf16 or fp16; width a multiple of 8 up to 256; rows of q, keys and values start on 16 bytes. Rows of out behind the last sequence
+ * bf16 or fp16; width a multiple of 8 up to 256; rows of q, keys and values start on 16 bytes; pages and rows of the cache lie less than
+ * 2^31 elements apart. Rows of out behind the last sequence
  * are left as they were, or become zeros with zero_rest.
  *
  * The order of a row's sums is a function of the positions it sees (contract rlk_attention_contract_id()), so its bits do not
  * depend on the batch, the chunk it came in, the page size or the configuration: keys in tiles of 64 positions, one chain of running
- * maximum, sum and output over the tiles of a run, and the runs (of 256 positions up to 4096, of 512 up to 16384, of 1024 up to
+ * maximum (changed by more than 8 binary orders at a time), sum and output over the tiles of a run, and the runs (of 256 positions up to 4096, of 512 up to 16384, of 1024 up to
  * 65536, of 2048 behind) combined in ascending order.
  */
 typedef enum rlk_attention_config {
   RLK_ATTENTION_CFG_AUTO = 0,
-  RLK_ATTENTION_CFG_ROWS16 = 1,  /* a wave for 16 rows of a key head and a run; the runs are combined by a second launch */
-  RLK_ATTENTION_CFG_ROWS64 = 2,  /* four waves of 16 rows, all runs one after the other */
-  RLK_ATTENTION_CFG_ROWS256 = 3, /* eight waves of 32 rows (16 for heads wider than 128) */
+  RLK_ATTENTION_CFG_ROWS32 = 1,  /* a wave for 32 rows of a key head, runs side by side, combined by a second launch */
+  RLK_ATTENTION_CFG_ROWS128 = 2, /* four waves of 32 rows, all runs one after the other */
+  RLK_ATTENTION_CFG_ROWS256 = 3, /* eight waves of 32 rows (four for heads wider than 128) */
   RLK_ATTENTION_CFG_SPLIT = 0x100 /* OR-ed into the last two: runs side by side, combined by a second launch */
 } rlk_attention_config;
 const char* rlk_attention_contract_id(void);

@@ -3,13 +3,15 @@
 // Rows. A sequence's new tokens and the heads that share a key head are rows of one matrix, token by token, so that every key and
 // value that is read serves all of them. A tile is a run of such rows of one sequence and one key head.
 //
-// Sums. Scores come transposed, S^T = K Q^T: the matrix instruction's result then has a row's scores in four lanes (and its
-// statistics need two lane swaps), and two 16-key blocks of it, rounded to 16 bits, are the operand of O^T = V^T P^T as they
-// stand: slot 8 g + e of lane group g holds key 16 (e / 4) + 4 g + e % 4 of 32, and the transposing LDS read brings the values in
-// that order. Each of a row's four lanes sums the weights of its own keys; they meet at the end of a run.
-//   tile of 64 keys:  m' = max(m, max s),  a = 2^(m - m'),  p = 2^(s - m'),  o = a o + round(p) V,  l = a l + sum p
+// Sums. Scores come transposed, S^T = K Q^T, 32 keys by 32 rows: the matrix instruction's result then has a row's scores in two
+// lanes (and its statistics need one lane swap), and its registers, rounded to 16 bits, are the operands of O^T = V^T P^T as they
+// stand: of 16 keys, slot 8 g + e of half-wave g holds key 8 (e / 4) + 4 g + e % 4, and the transposing LDS read brings the values in
+// that order. Each of a row's two lanes sums the weights of its own keys; they meet at the end of a run.
+//   tile of 64 keys:  m' = next(m, max s),  a = 2^(m - m'),  p = 2^(s - m'),  o = a o + round(p) V,  l = a l + sum p
 // with s in units of log2(e) * scale. A run of tiles starts from nothing; runs are combined in ascending order:
-//   M' = max(M, m),  O = 2^(m - M') o + 2^(M - M') O  (one fused step), L likewise;  out = O / L,  lse = ln 2 (M + log2 L)
+//   M' = next(M, m),  O = 2^(m - M') o + 2^(M - M') O  (one fused step), L likewise;  out = O / L,  lse = ln 2 (M + log2 L)
+// next(m, x) is x where x is more than 8 above m, else m: weights of up to 2^8 do no harm, and rows then hardly ever change their scale, which
+// takes a product for every element (with the plain maximum nearly every tile of 32 rows did).
 // Which keys form a tile and which tiles a run is a function of their positions, and keys that a row does not see leave its chain as it is (a
 // factor of 1, a sum with 0). So a row's bits are the same in every kernel below, however its runs are spread over the chip.
 // Statistics and outputs are fp32 throughout; weights are rounded to the inputs' 16 bits for the matrix units (half a step, 2^-9 of a
@@ -19,6 +21,7 @@
 // read as zeros. Where some rows see a value and others do not, a zero weight would not save them from infinities and NaN in
 // it: such a tile is looked through before it is used, and if it holds any they are taken out of the product and added to the
 // rows that see them.
+#include "det_gemm_solo.h"
 #include "paged.h"
 
 namespace rlk {
@@ -59,22 +62,27 @@ struct AttentionArgs {
   float scale;  // times log2(e)
 };
 
+// Operands: lane l holds row l % 32 of the first and column l % 32 of the second, slots 8 (l / 32) ... + 7 of 16. Result: register
+// i of lane l is row 8 (i / 4) + 4 (l / 32) + i % 4, column l % 32.
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 template <int DTYPE>
 struct Half;
 template <>
 struct Half<RLK_DTYPE_BF16> {
   static constexpr uint32_t kOnes = 0x3f803f80u, kExponent = 0x7f807f80u, kLowest = 0x00800080u, kFraction = 0x007f007fu;
   static constexpr uint32_t k128 = 0x4300u, k16384 = 0x4680u;
-  static __device__ __forceinline__ f32x4_t mfma(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) { return mfma_16x16x32(a, b, c); }
+  static __device__ __forceinline__ f32x16_t mfma(const u32x4_t& a, const u32x4_t& b, const f32x16_t& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
 };
 template <>
 struct Half<RLK_DTYPE_FP16> {
   static constexpr uint32_t kOnes = 0x3c003c00u, kExponent = 0x7c007c00u, kLowest = 0x04000400u, kFraction = 0x03ff03ffu;
   static constexpr uint32_t k128 = 0x5800u, k16384 = 0x7400u;
-  static __device__ __forceinline__ f32x4_t mfma(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
+  static __device__ __forceinline__ f32x16_t mfma(const u32x4_t& a, const u32x4_t& b, const f32x16_t& c) {
     typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16;
@@ -89,22 +97,20 @@ __device__ __forceinline__ uint32_t special_halves(uint32_t w) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The largest value of a row over the four lanes that hold it (lanes l, l + 16, l + 32, l + 48). NaN loses, as in fmaxf.
-__device__ __forceinline__ float max_over_groups(float v) {
-  const uint32_t w = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-  const uint32_t u = __float_as_uint(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-  const auto t = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
+// The maximum that weights are taken from, once a value x has come up.
+constexpr float kSlack = 8.f;
+__device__ __forceinline__ float next_top(float top, float x) { return x > top + kSlack ? x : top; }
 
-// The sum of what the four lanes of a row hold, in one order.
-__device__ __forceinline__ float sum_over_groups(float v) {
+// The largest value of a row over the two lanes that hold it (l and l + 32), and the sum. NaN loses, as in fmaxf.
+__device__ __forceinline__ float max_over_halves(float v) {
   const uint32_t w = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-  const uint32_t u = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-  const auto t = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+  const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_over_halves(float v) {
+  const uint32_t w = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // Four values of one element, of four consecutive keys (see read_kmajor_fragment in det_gemm_tile.h, also for the qualifier).
@@ -119,18 +125,18 @@ __device__ __forceinline__ u32x4_t read_chunk(value_bytes_t __restrict__ at) {
 }
 
 // LDS image of a tile: slabs of 64 elements, each 64 rows (keys) of 128 bytes, as the direct loads lay blocks of 8 rows down.
-// Chunks of 16 bytes change places within a row so that the reads are free of bank conflicts: by the row's last three bits for
-// keys (16 lanes read one chunk of 16 rows), by twice its bits 1 and 2 for values (32 lanes read 32 bytes of 8 rows, two rows
-// to 256 bytes of banks).
-__device__ __forceinline__ int key_swizzle(int row) { return row & 7; }
-__device__ __forceinline__ int value_swizzle(int row) { return 2 * ((row >> 1) & 3); }
+// Chunks of 16 bytes change places within a row so that the reads are free of bank conflicts: by three bits of the row for
+// keys (lanes read one chunk of 32 rows, 16 of them at a time, two rows to 256 bytes of banks: bits 1 to 3 tell them apart whichever
+// 16), by bits 1 and 2 for values (32 lanes read 64 bytes of four rows or 32 bytes of eight).
+__device__ __forceinline__ int key_swizzle(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int value_swizzle(int row) { return 4 * ((row >> 1) & 1) + 2 * ((row >> 2) & 1); }
 
 // One sequence's part of a launch.
 struct Chunk {
   int sequence, first_token, tokens, length;
 };
 
-// What a row (of the 16 of a block, lane & 15) sees: keys [low, high).
+// What a row sees: keys [low, high).
 struct Sight {
   int low, high;
 };
@@ -167,196 +173,88 @@ __device__ __forceinline__ int64_t first_row_tile(const AttentionArgs& a, int s)
   return (int64_t)clamp_to(a.cache.starts[s], 0, a.tokens) * a.group / ROWS + s;
 }
 
-// The running state of RB blocks of 16 rows of a wave. Lane l holds row l & 15 of each; of the output elements 16 d + 4 (l >> 4) + i.
-template <int DTYPE, int SLABS, int RB, bool KEEP_Q = true>
+// The running state of 32 rows of a wave. Lane l holds row l & 31; of the output, register i of block d is element
+// 32 d + 8 (i / 4) + 4 (l / 32) + i % 4.
+template <int DTYPE, int SLABS>
 struct Rows {
   typedef Half<DTYPE> H;
-  static constexpr int kBlocks = 4 * SLABS;  // of 16 elements
-  static constexpr int kSteps = 2 * SLABS;   // of 32 elements
-  u32x4_t q[KEEP_Q ? kSteps : 1][RB];  // (or they stay in LDS)
-  f32x4_t o[kBlocks][RB];
-  float m[RB];
-  float l[RB];  // the sum of the weights of this lane's keys
-  Sight sight[RB];
+  static constexpr int kBlocks = 2 * SLABS;  // of 32 elements
+  static constexpr int kSteps = 4 * SLABS;   // of 16 elements
+  f32x16_t o[kBlocks];
+  float m;
+  float l;  // the sum of the weights of this lane's keys
+  Sight sight;
 
-  __device__ __forceinline__ void load_q(const AttentionArgs& a, int key_head, const int (&token)[RB], const int (&head)[RB], const bool (&live)[RB],
-                                         int l16, int grp, char* shelf) {
+  __device__ __forceinline__ void clear_output() {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const char* row = a.q + (int64_t)token[rb] * a.q_token_stride + (int64_t)(key_head * a.group + head[rb]) * a.q_head_stride;
+    for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) {
-        const int element = 32 * ks + 8 * grp;
-        const u32x4_t v = live[rb] && element < a.cache.width ? *reinterpret_cast<const u32x4_t*>(row + 2 * element) : u32x4_t{0, 0, 0, 0};
-        if (KEEP_Q)
-          q[KEEP_Q ? ks : 0][rb] = v;
-        else
-          *reinterpret_cast<u32x4_t*>(shelf + (rb * SLABS + (ks >> 1)) * 2048 + l16 * 128 + (((4 * (ks & 1) + grp) ^ key_swizzle(l16)) << 4)) = v;
-      }
-    }
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   }
-  __device__ __forceinline__ void clear() {
+  // Scores of a tile, s[b][i] of keys key0 + 32 b + 8 (i / 4) + 4 half + i % 4: those of keys that a row does not see go.
+  __device__ __forceinline__ void mask(f32x16_t (&s)[2], int key0) {
+    const int half = solo_lane() >> 5;
+    const uint32_t range = sight.high > sight.low ? sight.high - sight.low : 0;
+    const uint32_t from = (uint32_t)(key0 + 4 * half - sight.low);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      m[rb] = -INFINITY;
-      l[rb] = 0.f;
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int d = 0; d < kBlocks; ++d) o[d][rb] = f32x4_t{0, 0, 0, 0};
-    }
+      for (int i = 0; i < 16; ++i) s[b][i] = from + 32 * b + 8 * (i >> 2) + (i & 3) < range ? s[b][i] : -INFINITY;
   }
-
-  // Scores of a tile, s[b][rb] of keys key0 + 16 b + 4 grp + i: those of keys that a row does not see go.
-  __device__ __forceinline__ void mask(f32x4_t (&s)[4][RB], int key0, int grp) {
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const uint32_t range = sight[rb].high > sight[rb].low ? sight[rb].high - sight[rb].low : 0;
-      const uint32_t from = (uint32_t)(key0 + 4 * grp - sight[rb].low);
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[b][rb][i] = from + 16 * b + i < range ? s[b][rb][i] : -INFINITY;
-    }
-  }
-
-  // Scores to weights; the state is taken to the new maximum.
-  __device__ __forceinline__ void weigh(const AttentionArgs& a, const f32x4_t (&s)[4][RB], u32x4_t (&p)[2][RB]) {
-    float before[RB];
-    bool moved = false;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      float top = s[0][rb][0];
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][rb][i]);
-      before[rb] = m[rb];
-      m[rb] = fmaxf(m[rb], max_over_groups(top) * a.scale);
-      moved |= m[rb] != before[rb];
-    }
-    if (__any(moved)) {
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const float f = m[rb] != before[rb] ? exp2_fast(before[rb] - m[rb]) : 1.f;
-        l[rb] *= f;
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d) o[d][rb] *= f;
-      }
-    }
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const float from = m[rb] == -INFINITY ? 0.f : m[rb];
-      float sum[2][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x4_t& v = s[2 * h + (e >> 1)][rb];
-          const float x = exp2_fast(__builtin_fmaf(v[2 * (e & 1)], a.scale, -from)), y = exp2_fast(__builtin_fmaf(v[2 * (e & 1) + 1], a.scale, -from));
-          sum[h][e] = x + y;
-          p[h][rb][e] = H::pack(x, y);
-        }
-      l[rb] += ((sum[0][0] + sum[0][1]) + (sum[0][2] + sum[0][3])) + ((sum[1][0] + sum[1][1]) + (sum[1][2] + sum[1][3]));
-    }
-  }
-
-  // A lane's place in the values' image: for element blocks 0 ... 3 of a slab.
-  struct ValuePlace {
-    int at[4];
-    __device__ __forceinline__ void init(int l16, int grp) {
-      const int row = 4 * grp + (l16 >> 2);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) at[d] = row * 128 + (((2 * d + ((l16 >> 1) & 1)) ^ value_swizzle(row)) << 4) + (l16 & 1) * 8;
-    }
-  };
-  static __device__ __forceinline__ u32x4_t value_fragment(value_bytes_t tile, int place, int d, int h) {
-    const value_bytes_t at = tile + place + (d >> 2) * kSlabBytes + h * 4096;
-    const u32x2_t x = read_values_transposed(at), y = read_values_transposed(at + 2048);
-    return u32x4_t{x.x, x.y, y.x, y.y};
-  }
-
-  // Fragments are read a few products ahead of their use.
-  static constexpr int kAhead = 4;
-  __device__ __forceinline__ void add_values(value_bytes_t tile, const ValuePlace& place, const u32x4_t (&p)[2][RB]) {
-    u32x4_t v[kAhead];
-#pragma unroll
-    for (int n = 0; n < kAhead; ++n) v[n] = value_fragment(tile, place.at[n & 3], n, 0);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int n = 0; n < 2 * kBlocks; ++n) {
-      const int d = n % kBlocks, h = n / kBlocks, next = n + kAhead;
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) o[d][rb] = H::mfma(v[n % kAhead], p[h][rb], o[d][rb]);
-      if (next < 2 * kBlocks) v[n % kAhead] = value_fragment(tile, place.at[next & 3], next % kBlocks, next / kBlocks);
-      __builtin_amdgcn_sched_barrier(0);  // (or the reads move back to their use)
-    }
-  }
-
-  // A tile with infinities or NaN among the values that some rows see and others do not. They leave the product (take_out), and what they
-  // make of an element is added to it behind (an infinity, or NaN where both come together, from NaN, or from an infinity
-  // with a weight of 0). One more product counts them: 1 for inf, 128 for -inf, 16384 for NaN, 64 at most of each. The results wait
-  // in memory, and nothing here is unrolled: this is rare, and in registers it would cost the ordinary tiles theirs.
-  __device__ __forceinline__ void find_special(value_bytes_t tile, const ValuePlace& place, const u32x4_t (&p)[2][RB], int key0, int grp, volatile float* effect) {
-    const uint32_t one = H::kOnes & 0xffffu;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const uint32_t range = sight[rb].high > sight[rb].low ? sight[rb].high - sight[rb].low : 0;
-#pragma unroll 1
-      for (int d = 0; d < kBlocks; ++d) {
-        f32x4_t count = {0, 0, 0, 0};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const u32x4_t v = value_fragment(tile, place.at[0] ^ ((d & 3) << 5), d, h);
-          u32x4_t kinds, any, seen, lost;  // of the values; 1 where a row sees a key with a weight, and without one
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t from = (uint32_t)(key0 + 32 * h + 16 * (e >> 1) + 4 * grp + 2 * (e & 1) - sight[rb].low);
-            const uint32_t sees = (from < range ? 0x8000u : 0u) | (from + 1 < range ? 0x80000000u : 0u);
-            const uint32_t weighs = ((p[h][rb][e] & 0x7fff7fffu) + 0x7fff7fffu) & sees;
-            seen[e] = (weighs >> 15) * one;
-            lost[e] = ((sees ^ weighs) >> 15) * one;
-            const uint32_t w = v[e], special = special_halves<DTYPE>(w);
-            const uint32_t none = special & ((w & H::kFraction) + 0x7fff7fffu);
-            kinds[e] = ((special & ~none & ~w) >> 15) * one | ((special & ~none & w) >> 15) * H::k128 | (none >> 15) * H::k16384;
-            any[e] = (special >> 15) * H::k16384;
-          }
-          count = H::mfma(kinds, seen, count);
-          count = H::mfma(any, lost, count);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t n = (uint32_t)count[i];
-          const float up = (n & 127) != 0 ? INFINITY : 0.f, down = (n & (127 << 7)) != 0 ? -INFINITY : 0.f;
-          effect[4 * (d * RB + rb) + i] = n >= 16384 ? NAN : up + down;
-        }
-      }
-    }
-  }
+  // (see find_special)
   __device__ __forceinline__ void add_special(const volatile float* effect) {
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[d][rb][i] += effect[4 * (d * RB + rb) + i];
+      for (int i = 0; i < 16; ++i) o[d][i] += effect[16 * d + i];
   }
 };
 
-// Zeros in the place of a chunk's infinities and NaN.
+// Scores to weights, in pieces that stand between matrix instructions: the maximum of eight scores each, the new maximum and what the
+// state is scaled by, the weights of four scores each.
 template <int DTYPE>
-__device__ __forceinline__ void take_out_special(char* at) {
-  typedef __attribute__((address_space(3))) u32x4_t* chunk_ptr_t;
-  u32x4_t w = *(chunk_ptr_t)at;
+struct Weighing {
+  static constexpr int kPieces = 13;
+  float top[4], from, factor, sum[4];
+  bool moved;
+  template <int SLABS>
+  __device__ __forceinline__ void piece(int n, const AttentionArgs& a, Rows<DTYPE, SLABS>& st, const f32x16_t (&s)[2], u32x4_t (&p)[4]) {
+    if (n < 4) {
+      const int b = n >> 1, first = 8 * (n & 1);
+      float x = s[b][first];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] &= ~((special_halves<DTYPE>(w[e]) >> 15) * 0xffffu);
-  *(chunk_ptr_t)at = w;
-}
+      for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b][first + i]);
+      asm volatile("" : "+v"(x));  // (here and below: computed in its piece, not where it is used)
+      top[n] = x;
+    } else if (n == 4) {
+      const float before = st.m;
+      st.m = next_top(before, max_over_halves(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))) * a.scale);
+      moved = st.m != before;
+      factor = moved ? exp2_fast(before - st.m) : 1.f;
+      from = st.m == -INFINITY ? 0.f : st.m;
+    } else {
+      const int j = n - 5, b = j >> 2, first = 4 * (j & 3);
+      float x[4] = {s[b][first], s[b][first + 1], s[b][first + 2], s[b][first + 3]};
+      asm volatile("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));  // (nor before its piece)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], a.scale, -from));
+      uint32_t pair = Half<DTYPE>::pack(x[0], x[1]), other = Half<DTYPE>::pack(x[2], x[3]);
+      float four = (x[0] + x[1]) + (x[2] + x[3]);
+      asm volatile("" : "+v"(pair), "+v"(other), "+v"(four));
+      p[j >> 1][2 * (j & 1)] = pair;
+      p[j >> 1][2 * (j & 1) + 1] = other;
+      sum[j >> 1] = (j & 1) ? sum[j >> 1] + four : four;
+      if (n == kPieces - 1) st.l = __builtin_fmaf(st.l, factor, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    }
+  }
+};
 
 // A run joins those before it: factors for both, and the new maximum.
 struct Join {
   float kept, added;
 };
 __device__ __forceinline__ Join join_maxima(float& all, float run) {
-  const float top = fmaxf(all, run);
+  const float top = next_top(all, run);
   Join j;
   j.kept = top == all ? 1.f : exp2_fast(all - top);
   j.added = top == run ? 1.f : exp2_fast(run - top);
@@ -369,20 +267,13 @@ __device__ __forceinline__ float join_sums(float all, float run, const Join& j) 
 __device__ __forceinline__ float output_of(float sum, float reciprocal) { return sum * reciprocal + 0.f; }
 __device__ __forceinline__ float lse_of(float top, float sum) { return 0.6931471805599453f * (top + __builtin_amdgcn_logf(sum)); }
 
-// Loads a wave's share of a tile, GROUPS groups of 8 keys (the WAVES-th ones), straight into LDS.
-template <int SLABS>
-struct TileLoader {
-  const char *keys, *values;  // of the key head
-  int64_t key_page, key_row, value_page, value_row;  // bytes
-  int key_chunk, value_chunk;  // of this lane's 16 bytes in a slab's row
-
-  __device__ __forceinline__ void init(const AttentionArgs& a, int key_head, int lane) {
-    keys = static_cast<const char*>(a.cache.keys) + 2 * key_head * a.cache.key_head_stride;
-    values = static_cast<const char*>(a.cache.values) + 2 * key_head * a.cache.value_head_stride;
-    key_page = 2 * a.cache.key_page_stride, key_row = 2 * a.cache.key_row_stride;
-    value_page = 2 * a.cache.value_page_stride, value_row = 2 * a.cache.value_row_stride;
-    key_chunk = (lane & 7) ^ key_swizzle(lane >> 3);
-    value_chunk = (lane & 7) ^ value_swizzle(lane >> 3);
+// One of the two caches, of a key head; distances in bytes.
+struct CacheSide {
+  const char* base;
+  uint32_t page, row;
+  __device__ __forceinline__ void init(const void* cache, int64_t head, int64_t page_stride, int64_t row_stride) {
+    base = static_cast<const char*>(cache) + 2 * head;
+    page = (uint32_t)(2 * page_stride), row = (uint32_t)(2 * row_stride);
   }
 };
 
@@ -396,33 +287,162 @@ struct KeyPlace {
     entry = *from;
   }
 };
-// The start of a key's row in a cache: zeros where the tile does not need the key, NaN where its page is missing.
-__device__ __forceinline__ const char* key_row_address(const AttentionArgs& a, const char* base, int64_t page_bytes, int64_t row_bytes, int entry, int key,
-                                                       int low, int high) {
-  const int column = (int)divide_by((uint32_t)key, a.by_page);
-  const int row = key - column * a.cache.page_size;
-  const bool there = (uint32_t)entry < (uint32_t)a.cache.pages && column < a.cache.table_columns;
-  const bool wanted = key >= low && key < high;
-  const char* const special = reinterpret_cast<const char*>(kSpecialRows[wanted]);
-  return wanted && there ? base + entry * page_bytes + row * row_bytes : special;
+struct KeyRow {
+  uint32_t page, row;
+  const char* special;  // instead: zeros where the tile does not need the key, NaN where its page is missing
+  __device__ __forceinline__ void find(const AttentionArgs& a, int entry, int key, int low, int high) {
+    const int column = (int)divide_by((uint32_t)key, a.by_page);
+    const bool there = (uint32_t)entry < (uint32_t)a.cache.pages && column < a.cache.table_columns;
+    const bool wanted = key >= low && key < high;
+    special = wanted && there ? nullptr : reinterpret_cast<const char*>(kSpecialRows[wanted]);
+    page = wanted && there ? entry : 0;
+    row = key - column * a.cache.page_size;
+  }
+  __device__ __forceinline__ const char* in(const CacheSide& c) const {
+    const char* at = c.base + (uint64_t)page * c.page + (uint64_t)row * c.row;
+    return special != nullptr ? special : at;
+  }
+};
+
+// 16 bytes of each lane straight into LDS, at a distance from a wave's base; zeros for kSoloOutside.
+__device__ __forceinline__ void load_block(char* base, uint32_t offset, char* to) {
+  const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(base, 0, kSoloRange, 0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_ptr_t)to, 16, offset, 0, 0, 0);
+}
+// Eight keys of one page straight into LDS, at the address of the first (odd where the page is missing), each lane 16 bytes of every slab
+// of its key's row: `offset` from there where all of them are needed, else what a lane has to work out (from its number as if it had just
+// been read, so that nothing is kept for that through the turns that do not need it). SWIZZLE: of the image.
+template <int SLABS, class Swizzle>
+__device__ __forceinline__ void load_group(uint32_t low_word, uint32_t high_word, const uint32_t (&offset)[SLABS], bool whole, int first_key, int low,
+                                           int high, uint32_t row_bytes, int width, Swizzle swizzle, char* to) {
+  uint32_t at[SLABS];
+#pragma unroll
+  for (int slab = 0; slab < SLABS; ++slab) at[slab] = offset[slab];
+  if ((low_word & 1) != 0 || !whole) {
+    const int lane = solo_lane(), key = first_key + (lane >> 3), chunk = (lane & 7) ^ swizzle(first_key + (lane >> 3));
+#pragma unroll
+    for (int slab = 0; slab < SLABS; ++slab) {
+      at[slab] = ((low_word & 1) == 0 ? (lane >> 3) * row_bytes : 0) + chunk * 16 + slab * 128;
+      if (key < low || key >= high || (slab * 8 + chunk) * 8 >= width) at[slab] = kSoloOutside;
+    }
+  }
+#pragma unroll
+  for (int slab = 0; slab < SLABS; ++slab) load_block(reinterpret_cast<char*>((uint64_t)high_word << 32 | (low_word & ~1u)), at[slab], to + slab * kSlabBytes);
+}
+// The same for keys of any pages.
+template <int SLABS>
+__device__ __forceinline__ void load_rows(const AttentionArgs& a, const CacheSide& side, const KeyPlace& where, int chunk, int key, int low, int high,
+                                          char* to) {
+  const char* const none = reinterpret_cast<const char*>(kSpecialRows[0]);
+  KeyRow row;
+  row.find(a, where.entry, key, low, high);
+  const char* const from = row.in(side) + chunk * 16;
+#pragma unroll
+  for (int slab = 0; slab < SLABS; ++slab) {
+    const char* const at = (slab * 8 + chunk) * 8 < a.cache.width ? from + slab * 128 : none;
+    __builtin_amdgcn_global_load_lds((global_ptr_t)at, (lds_ptr_t)(to + slab * kSlabBytes), 16, 0, 0);
+  }
+}
+
+// A tile with infinities or NaN among the values that some rows see and others do not. They have left the tile in LDS (take_out_special), and
+// what they make of an element is added to it behind the product: an infinity, or NaN where both come together, from NaN, or from
+// an infinity with a weight of 0. One more product counts them: 1 for inf, 128 for -inf, 16384 for NaN, 64 at most of each. The values are
+// read from the cache again, the results wait in memory, and nothing here is unrolled: this is rare, and in registers it would cost the
+// ordinary tiles theirs.
+template <int DTYPE, class State>
+__device__ __forceinline__ void find_special(const AttentionArgs& a, const State& st, const CacheSide& values, int sequence, const u32x4_t (&p)[4],
+                                             int key0, int low, int high, int lane, volatile float* effect) {
+  typedef Half<DTYPE> H;
+  const uint32_t one = H::kOnes & 0xffffu;
+  const uint32_t range = st.sight.high > st.sight.low ? st.sight.high - st.sight.low : 0;
+#pragma unroll 1
+  for (int d = 0; d < State::kBlocks; ++d) {
+    f32x16_t count;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) count[i] = 0.f;
+#pragma unroll 1
+    for (int f = 0; f < 4; ++f) {
+      u32x4_t kinds, any, seen, lost;  // of the values; 1 where a row sees a key with a weight, and without one
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int first = key0 + 16 * f + 8 * (e >> 1) + 4 * (lane >> 5) + 2 * (e & 1);
+        uint32_t w = 0;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          KeyPlace where;
+          where.ask(a, sequence, first + i);
+          KeyRow row;
+          row.find(a, where.entry, first + i, low, high);
+          const int element = 32 * d + (lane & 31);
+          if (element < a.cache.width) w |= (uint32_t)reinterpret_cast<const uint16_t*>(row.in(values))[element] << (16 * i);
+        }
+        const uint32_t from = (uint32_t)(first - st.sight.low);
+        const uint32_t sees = (from < range ? 0x8000u : 0u) | (from + 1 < range ? 0x80000000u : 0u);
+        const uint32_t bits = f == 0 ? p[0][e] : f == 1 ? p[1][e] : f == 2 ? p[2][e] : p[3][e];
+        const uint32_t weighs = ((bits & 0x7fff7fffu) + 0x7fff7fffu) & sees;
+        seen[e] = (weighs >> 15) * one;
+        lost[e] = ((sees ^ weighs) >> 15) * one;
+        const uint32_t special = special_halves<DTYPE>(w);
+        const uint32_t none = special & ((w & H::kFraction) + 0x7fff7fffu);
+        kinds[e] = ((special & ~none & ~w) >> 15) * one | ((special & ~none & w) >> 15) * H::k128 | (none >> 15) * H::k16384;
+        any[e] = (special >> 15) * H::k16384;
+      }
+      count = H::mfma(kinds, seen, count);
+      count = H::mfma(any, lost, count);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t n = (uint32_t)count[i];
+      const float up = (n & 127) != 0 ? INFINITY : 0.f, down = (n & (127 << 7)) != 0 ? -INFINITY : 0.f;
+      effect[16 * d + i] = n >= 16384 ? NAN : up + down;
+    }
+  }
+}
+// Zeros in the place of a chunk's infinities and NaN; whether there were any.
+template <int DTYPE>
+__device__ __forceinline__ bool take_out_special(char* at) {
+  typedef __attribute__((address_space(3))) u32x4_t* chunk_ptr_t;
+  u32x4_t w = *(chunk_ptr_t)at;
+  uint32_t any = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t special = special_halves<DTYPE>(w[e]);
+    w[e] &= ~((special >> 15) * 0xffffu);
+    any |= special;
+  }
+  if (any != 0) *(chunk_ptr_t)at = w;
+  return any != 0;
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: WAVES waves of 16 RB rows each share the keys and values of their tile through LDS, two tiles deep, one barrier a
-// tile. SPLIT: a workgroup takes every chunks-th run and leaves the parts in memory.
+// WAVES waves of 32 rows each share the keys and values of their tile through LDS, two tiles of each deep, one barrier a tile. SPLIT:
+// a workgroup takes some of the runs and leaves the parts in memory. GROUPED: eight keys that a load instruction brings lie in one page
+// (page sizes that 8 divides), so that a wave-uniform base and constant lane offsets address them, a buffer load's range makes
+// zeros of the keys that a tile does not need, and the compiler counts LDS reads one by one (beside a direct load with lane
+// addresses, which it takes for one that might have gone to LDS, it waits for all of them at every step).
+//
+// In turn i a wave multiplies its queries with tile i's keys, and then tile i - 1's weights with its values; between these
+// products stands, piece by piece, what turns tile i's scores into weights, because a wave's vector instructions run beside its own
+// matrix instructions (and exponentials, 16 cycles each, are a third of the time of both products) but two waves a SIMD are too
+// few to fill one with the other's. Tile i + 1's keys and tile i's values are asked for at the start of turn i and have landed at
+// its end; the places they go to were last read in turn i - 1.
 // ---------------------------------------------------------------------------
-template <int DTYPE, int SLABS, int RB, int WAVES, bool SPLIT>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_tile_kernel(const AttentionArgs a) {
-  constexpr bool kKeepQ = RB == 1;
-  typedef Rows<DTYPE, SLABS, RB, kKeepQ> State;
-  constexpr int kRows = 16 * RB * WAVES;
+template <int DTYPE, int SLABS, int WAVES, bool SPLIT, bool GROUPED>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES == 8 ? 2 : 1, WAVES == 8 ? 2 : 1))) void attention_tile_kernel(
+    const AttentionArgs a) {
+  typedef Rows<DTYPE, SLABS> State;
+  typedef Half<DTYPE> H;
+  constexpr int kRows = 32 * WAVES;
+  constexpr bool kKeepQ = SLABS > 2;  // queries stay in registers; else in LDS
   constexpr int kGroups = 8 / WAVES;  // groups of 8 keys that a wave loads
+  constexpr int kSpan = 64 / kGroups;  // tiles whose addresses the lanes of a wave have
   constexpr int kTileBytes = SLABS * kSlabBytes;
-  // [2][keys, values], then the queries, block of 16 rows by block, unless they are in registers, then special_tile. Nothing lies in
-  // front of it: 16-byte reads that start on 8 bytes took 62 cycles each instead of 8, and the kernel twice as long.
+  constexpr int kShelfBytes = kKeepQ ? 0 : SLABS * 4096;  // of a wave
+  // [2][keys, values], then the queries, wave by wave, then special_tile. Nothing lies in front of it: 16-byte reads that
+  // start on 8 bytes took 62 cycles each instead of 8.
   extern __shared__ __align__(16) char lds[];
-  int* const special_tile = reinterpret_cast<int*>(lds + 4 * kTileBytes + (kKeepQ ? 0 : WAVES * RB * SLABS * 2048));  // [2]
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, grp = lane >> 4;
+  int* const special_tile = reinterpret_cast<int*>(lds + 4 * kTileBytes + WAVES * kShelfBytes);  // [2]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
   // Heads change fastest, so that an XCD's workgroups read few of them; the tiles with the most keys come first.
   const uint32_t id = blockIdx.x;
@@ -458,365 +478,356 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
   const Sight first_sight = sight_of(a, c, (int)divide_by(row0, a.by_group)), last_sight = sight_of(a, c, (int)divide_by(last_row, a.by_group));
   const int capacity = capacity_of(a);
   const int low = first_sight.low, high = min(last_sight.high, capacity + 1);
-  const int wave_row0 = row0 + wave * 16 * RB, wave_row1 = min(wave_row0 + 16 * RB, rows) - 1;
+  const int wave_row0 = row0 + wave * 32, wave_row1 = min(wave_row0 + 32, rows) - 1;
   const bool wave_live = wave_row0 < rows;
   const Sight wave_first = sight_of(a, c, (int)divide_by(wave_live ? wave_row0 : row0, a.by_group));
   const Sight wave_last = sight_of(a, c, (int)divide_by(wave_live ? wave_row1 : row0, a.by_group));
 
+  struct RowPlace {
+    int token, head;
+    bool live;
+  };
+  auto row_place = [&]() __attribute__((always_inline)) {
+    const int row = wave_row0 + (lane & 31);
+    RowPlace r;
+    r.live = row < rows;
+    const int t = (int)divide_by(r.live ? row : row0, a.by_group);
+    r.head = key_head * a.group + (r.live ? row : row0) - t * a.group;
+    r.token = c.first_token + t;
+    return r;
+  };
   State st;
-  int token[RB], head[RB];
-  bool live[RB];
+  char* const shelf = lds + 4 * kTileBytes + wave * kShelfBytes;
+  u32x4_t kept_q[kKeepQ ? State::kSteps : 1];
+  {
+    const RowPlace r = row_place();
+    st.sight = r.live ? sight_of(a, c, r.token - c.first_token) : Sight{0, 0};
+    const char* const row = a.q + (int64_t)r.token * a.q_token_stride + (int64_t)r.head * a.q_head_stride;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int row = wave_row0 + 16 * rb + l16;
-    live[rb] = row < rows;
-    const int t = (int)divide_by(live[rb] ? row : row0, a.by_group);
-    head[rb] = (live[rb] ? row : row0) - t * a.group;
-    token[rb] = c.first_token + t;
-    st.sight[rb] = live[rb] ? sight_of(a, c, t) : Sight{0, 0};
+    for (int ks = 0; ks < State::kSteps; ++ks) {
+      const int element = 16 * ks + 8 * half;
+      const u32x4_t v = r.live && element < a.cache.width ? *reinterpret_cast<const u32x4_t*>(row + 2 * element) : u32x4_t{0, 0, 0, 0};
+      if (kKeepQ)
+        kept_q[kKeepQ ? ks : 0] = v;
+      else
+        *reinterpret_cast<u32x4_t*>(shelf + (ks >> 2) * 4096 + (lane & 31) * 128 + (((2 * (ks & 3) + half) ^ key_swizzle(lane)) << 4)) = v;
+    }
   }
-  char* const shelf = lds + 4 * kTileBytes + wave * RB * SLABS * 2048;
-  st.load_q(a, key_head, token, head, live, l16, grp, shelf);
-  st.clear();
   if (tid < 2) special_tile[tid] = 0;
 
-  TileLoader<SLABS> loader;
-  loader.init(a, key_head, lane);
-  typename State::ValuePlace place;
-  place.init(l16, grp);
-  int key_at[2];  // this lane's chunks of a key block for even and odd steps
+  CacheSide key_side, value_side;
+  key_side.init(a.cache.keys, key_head * a.cache.key_head_stride, a.cache.key_page_stride, a.cache.key_row_stride);
+  value_side.init(a.cache.values, key_head * a.cache.value_head_stride, a.cache.value_page_stride, a.cache.value_row_stride);
+  // Of a loading lane; of keys for even and odd groups of eight.
+  const int odd_wave = WAVES == 1 ? 0 : 8 * (wave & 1);
+  const int key_chunk[2] = {(lane & 7) ^ key_swizzle(odd_wave + (lane >> 3)), (lane & 7) ^ key_swizzle(odd_wave + 8 + (lane >> 3))};
+  const int value_chunk = (lane & 7) ^ value_swizzle(lane >> 3);
+  // This lane's places in the images: of 16 elements of its key (or query) for every step of a slab, of its elements' values for even
+  // and odd blocks of 32.
+  int key_at[4], value_at[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) key_at[h] = l16 * 128 + (((4 * h + grp) ^ key_swizzle(l16)) << 4);
+  for (int i = 0; i < 4; ++i) key_at[i] = (lane & 31) * 128 + (((2 * i + half) ^ key_swizzle(lane)) << 4);
+  {
+    const int row = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) value_at[i] = row * 128 + (((4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ value_swizzle(row)) << 4) + (lane & 1) * 8;
+  }
 
-  const int end_tile = (high + kTileKeys - 1) / kTileKeys;
-  int run = run_of_tile(low / kTileKeys) + chunk_id;
-  int t = SPLIT ? max(run_first_tile(run), low / kTileKeys) : low / kTileKeys;
-  auto next_tile = [&](int tile) {
-    if (!SPLIT) return tile + 1;
-    const int r = run_of_tile(tile);
-    return tile + 1 < run_first_tile(r + 1) ? tile + 1 : run_first_tile(r + a.chunks);
+  // This workgroup's tiles: those of runs that start in its part.
+  int t = low / kTileKeys, end_tile = (high + kTileKeys - 1) / kTileKeys;
+  if (SPLIT) {
+    const int first = t, count = end_tile - t;
+    auto border = [&](int chunk) __attribute__((always_inline)) {  // the first run that starts there or later
+      const int tile = first + (int)((int64_t)count * chunk / a.chunks);
+      const int run = run_of_tile(tile);
+      return tile <= first ? first : run_first_tile(run) >= tile ? tile : run_first_tile(run + 1);
+    };
+    t = border(chunk_id);
+    end_tile = min(end_tile, border(chunk_id + 1));
+  }
+  if (t >= end_tile && SPLIT) return;
+  auto keys_of = [&](int stage) __attribute__((always_inline)) { return lds + stage * 2 * kTileBytes; };
+  auto values_of = [&](int stage) __attribute__((always_inline)) { return lds + stage * 2 * kTileBytes + kTileBytes; };
+
+  // GROUPED: lane kGroups i + j has the addresses of group j of tile from + i, odd ones where the page is missing, of keys and of values; the
+  // next ones' table entries are on their way. They change hands at the start of a turn, when nothing is in flight.
+  uint32_t key_low = 0, key_high = 0, value_low = 0, value_high = 0, later_low = 0, later_high = 0;
+  int key_from = t, value_from = t;
+  KeyPlace lane_where;
+  auto key_of_lane = [&](int tile) __attribute__((always_inline)) { return (tile + lane / kGroups) * kTileKeys + (wave + (lane % kGroups) * WAVES) * 8; };
+  auto find_addresses = [&](int tile) __attribute__((always_inline)) {
+    const int key = key_of_lane(tile), column = (int)divide_by((uint32_t)key, a.by_page);
+    const bool there = (uint32_t)lane_where.entry < (uint32_t)a.cache.pages && column < a.cache.table_columns;
+    const uint64_t page = (uint32_t)lane_where.entry, row = (uint32_t)(key - column * a.cache.page_size);
+    const uint64_t missing = reinterpret_cast<uint64_t>(kSpecialRows[1]) + 1;
+    const uint64_t k = there ? reinterpret_cast<uint64_t>(key_side.base) + page * key_side.page + row * key_side.row : missing;
+    const uint64_t v = there ? reinterpret_cast<uint64_t>(value_side.base) + page * value_side.page + row * value_side.row : missing;
+    key_low = (uint32_t)k, key_high = (uint32_t)(k >> 32);
+    later_low = (uint32_t)v, later_high = (uint32_t)(v >> 32);
+    key_from = tile;
+    lane_where.ask(a, s, key_of_lane(tile + kSpan));
   };
-  KeyPlace where[kGroups];  // of the tile that is loaded next
-  auto find_pages = [&](int tile) {
-#pragma unroll
-    for (int j = 0; j < kGroups; ++j) where[j].ask(a, s, tile * kTileKeys + (wave + j * WAVES) * 8 + (lane >> 3));
-  };
-  auto load_tile = [&](int tile, int stage) {
-    char* const to = lds + stage * 2 * kTileBytes;
+  // Else: the table's entries of the tile whose keys have been asked for, and of the one behind.
+  KeyPlace here[kGroups], ahead[kGroups];
+  auto find_entries = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < kGroups; ++j) {
-      const int group_of_keys = wave + j * WAVES;
-      const int key = tile * kTileKeys + group_of_keys * 8 + (lane >> 3);
-      const char* k = key_row_address(a, loader.keys, loader.key_page, loader.key_row, where[j].entry, key, low, high);
-      const char* v = key_row_address(a, loader.values, loader.value_page, loader.value_row, where[j].entry, key, low, high);
-      const char* const none = reinterpret_cast<const char*>(kSpecialRows[0]);
-#pragma unroll
-      for (int slab = 0; slab < SLABS; ++slab) {
-        const int kc = slab * 8 + loader.key_chunk, vc = slab * 8 + loader.value_chunk;
-        const char* ks = kc * 8 < a.cache.width ? k + kc * 16 : none;
-        const char* vs = vc * 8 < a.cache.width ? v + vc * 16 : none;
-        __builtin_amdgcn_global_load_lds((global_ptr_t)ks, (lds_ptr_t)(to + slab * kSlabBytes + group_of_keys * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((global_ptr_t)vs, (lds_ptr_t)(to + kTileBytes + slab * kSlabBytes + group_of_keys * 1024), 16, 0, 0);
-      }
+      here[j] = ahead[j];
+      ahead[j].ask(a, s, tile * kTileKeys + (wave + j * WAVES) * 8 + (lane >> 3));
     }
+  };
+  uint32_t key_offset[2][SLABS], value_offset[SLABS];
+#pragma unroll
+  for (int slab = 0; slab < SLABS; ++slab) {
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd)
+      key_offset[odd][slab] = (slab * 8 + key_chunk[odd]) * 8 < a.cache.width ? (lane >> 3) * key_side.row + key_chunk[odd] * 16 + slab * 128 : kSoloOutside;
+    value_offset[slab] = (slab * 8 + value_chunk) * 8 < a.cache.width ? (lane >> 3) * value_side.row + value_chunk * 16 + slab * 128 : kSoloOutside;
+  }
+  const int whole_from = (low + kTileKeys - 1) / kTileKeys, whole_to = high / kTileKeys;  // tiles all of whose keys are needed
+  auto load_keys = [&](const KeyPlace (&where)[kGroups], int tile, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      const int i = (tile - key_from) * kGroups + j, first_key = tile * kTileKeys + (wave + j * WAVES) * 8;
+      char* const to = keys_of(stage) + (wave + j * WAVES) * 1024;
+      const int odd = WAVES == 1 ? j & 1 : 0;  // (more waves: a wave's groups are all even or all odd)
+      if (GROUPED)
+        load_group<SLABS>(__builtin_amdgcn_readlane(key_low, i), __builtin_amdgcn_readlane(key_high, i), key_offset[odd],
+                          tile >= whole_from && tile < whole_to, first_key, low, high, key_side.row, a.cache.width, key_swizzle, to);
+      else
+        load_rows<SLABS>(a, key_side, where[j], (lane & 7) ^ key_swizzle(first_key + (lane >> 3)), first_key + (lane >> 3), low, high, to);
+    }
+  };
+  auto load_values = [&](int tile, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      const int i = (tile - value_from) * kGroups + j, first_key = tile * kTileKeys + (wave + j * WAVES) * 8;
+      char* const to = values_of(stage) + (wave + j * WAVES) * 1024;
+      if (GROUPED)
+        load_group<SLABS>(__builtin_amdgcn_readlane(value_low, i), __builtin_amdgcn_readlane(value_high, i), value_offset,
+                          tile >= whole_from && tile < whole_to, first_key, low, high, value_side.row, a.cache.width, value_swizzle, to);
+      else
+        load_rows<SLABS>(a, value_side, here[j], (lane & 7) ^ value_swizzle(lane >> 3), first_key + (lane >> 3), low, high, to);
+    }
+  };
+  // What turn `tile` asks for: its values, the next one's keys.
+  auto ask_for = [&](int tile, int stage) __attribute__((always_inline)) {
+    if (GROUPED) {
+      if (tile - value_from >= kSpan) {
+        value_low = later_low, value_high = later_high;
+        value_from = tile;
+      }
+      if (tile + 1 - key_from >= kSpan) find_addresses(tile + 1);
+    }
+    load_values(tile, stage);
+    if (tile + 1 < end_tile) load_keys(ahead, tile + 1, stage ^ 1);
+    if (!GROUPED) find_entries(tile + 2 < end_tile ? tile + 2 : tile);
+  };
+  // Some rows of the workgroup see a key of the tile that others do not.
+  const int mixed_from = first_sight.high < high ? first_sight.high / kTileKeys : 0x7fffffff;
+  const int mixed_to = low < last_sight.low ? (last_sight.low + kTileKeys - 1) / kTileKeys : 0;
+  auto mixed = [&](int tile) __attribute__((always_inline)) { return tile >= mixed_from || tile < mixed_to; };
+  // The end of a turn: what I asked for has landed. Values that not everybody sees are looked through.
+  auto landed = [&](int tile, int stage, bool plain) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(kWaitAll0);
+    asm volatile("" ::: "memory");
+    if (!plain && mixed(tile)) {
+      bool special = false;
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+        for (int slab = 0; slab < SLABS; ++slab) special |= take_out_special<DTYPE>(values_of(stage) + slab * kSlabBytes + (wave + j * WAVES) * 1024 + lane * 16);
+      if (special) special_tile[stage] = tile + 1;
+      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    }
+    wg_barrier();
   };
 
   // Runs combined so far.
-  f32x4_t all_o[SPLIT ? 1 : State::kBlocks][RB];
-  float all_m[RB], all_l[RB];
+  f32x16_t all_o[SPLIT ? 1 : State::kBlocks];
+  float all_m = -INFINITY, all_l = 0.f;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    all_m[rb] = -INFINITY, all_l[rb] = 0.f;
+  for (int d = 0; d < (SPLIT ? 1 : State::kBlocks); ++d)
 #pragma unroll
-    for (int d = 0; d < (SPLIT ? 1 : State::kBlocks); ++d) all_o[d][rb] = f32x4_t{0, 0, 0, 0};
-  }
-
-  int stage = 0;
-  if (t < end_tile) {
-    find_pages(t);
-    load_tile(t, 0);
-    const int next = next_tile(t);
-    if (next < end_tile) find_pages(next);
-  }
-  wg_barrier();  // special_tile is there
-  while (t < end_tile) {
-    const int key0 = t * kTileKeys;
-    const int next = next_tile(t);
-    // some rows of the workgroup see a key that others do not
-    const bool mixed = min(key0 + kTileKeys, high) > first_sight.high || max(key0, low) < last_sight.low;
-    __builtin_amdgcn_s_waitcnt(kWaitAll0);  // my part of the tile has landed, and I have read what I wanted of the one before
-    asm volatile("" ::: "memory");
-    if (mixed) {
-      uint32_t special = 0;
-#pragma unroll
-      for (int j = 0; j < kGroups; ++j)
-#pragma unroll
-        for (int slab = 0; slab < SLABS; ++slab) {
-          const u32x4_t w = read_chunk((value_bytes_t)(lds + stage * 2 * kTileBytes + kTileBytes + slab * kSlabBytes + (wave + j * WAVES) * 1024 + lane * 16));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) special |= special_halves<DTYPE>(w[e]);
-        }
-      if (special != 0) special_tile[stage] = t + 1;
-      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-    }
-    wg_barrier();  // everybody's has, and the other stage is no longer read
-    if (next < end_tile) {
-      load_tile(next, stage ^ 1);
-      const int after = next_tile(next);
-      if (after < end_tile) find_pages(after);
-    }
-    const bool special = mixed && special_tile[stage] == t + 1;
-    const bool busy = wave_live && key0 < wave_last.high && key0 + kTileKeys > wave_first.low;
-    const value_bytes_t keys = (value_bytes_t)(lds + stage * 2 * kTileBytes), values = keys + kTileBytes;
-    u32x4_t p[2][RB];
-    volatile float effect[4 * State::kBlocks * RB];  // (in memory, see find_special)
-    if (busy) {
-      f32x4_t scores[4][RB];
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) scores[b][rb] = f32x4_t{0, 0, 0, 0};
-      constexpr int kAhead = 4;
-      u32x4_t k[kAhead], q[2][RB];
-      auto key_fragment = [&](int n) { return read_chunk(keys + key_at[(n >> 2) & 1] + (n >> 3) * kSlabBytes + (n & 3) * 2048); };
-      auto query_fragment = [&](int ks, int rb) {
-        return kKeepQ ? st.q[kKeepQ ? ks : 0][rb] : read_chunk((value_bytes_t)shelf + key_at[ks & 1] + (rb * SLABS + (ks >> 1)) * 2048);
-      };
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) q[0][rb] = query_fragment(0, rb);
-#pragma unroll
-      for (int n = 0; n < kAhead; ++n) k[n] = key_fragment(n);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int n = 0; n < 4 * State::kSteps; ++n) {
-        const int ks = n >> 2, b = n & 3;
-        if (b == 0 && ks + 1 < State::kSteps)
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb) q[(ks + 1) & 1][rb] = query_fragment(ks + 1, rb);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) scores[b][rb] = Half<DTYPE>::mfma(k[n % kAhead], q[ks & 1][rb], scores[b][rb]);
-        if (n + kAhead < 4 * State::kSteps) k[n % kAhead] = key_fragment(n + kAhead);
-        __builtin_amdgcn_sched_barrier(0);  // (or the reads move back to their use)
-      }
-      if (key0 + kTileKeys > wave_first.high || key0 < wave_last.low) st.mask(scores, key0, grp);
-      st.weigh(a, scores, p);
-    }
-    if (special) {
-      if (busy) st.find_special(values, place, p, key0, grp, effect);
-      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-      wg_barrier();
-#pragma unroll
-      for (int j = 0; j < kGroups; ++j)
-#pragma unroll
-        for (int slab = 0; slab < SLABS; ++slab)
-          take_out_special<DTYPE>(lds + stage * 2 * kTileBytes + kTileBytes + slab * kSlabBytes + (wave + j * WAVES) * 1024 + lane * 16);
-      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-      wg_barrier();
-    }
-    if (busy) st.add_values(values, place, p);
-    if (special && busy) st.add_special(effect);
-    const int this_run = run_of_tile(t);
-    if (next >= end_tile || run_of_tile(next) != this_run) {  // the run ends
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const float sum = sum_over_groups(st.l[rb]);
-        if (SPLIT) {
-          if (live[rb]) {
-            const int64_t at = (int64_t)this_run * a.part_rows + (int64_t)token[rb] * a.heads + key_head * a.group + head[rb];
-            if (grp == 0) a.part_max[at] = st.m[rb], a.part_sum[at] = sum;
-#pragma unroll
-            for (int d = 0; d < State::kBlocks; ++d)
-              if (16 * d + 4 * grp < a.cache.width) *reinterpret_cast<f32x4_t*>(a.part_out + at * a.cache.width + 16 * d + 4 * grp) = st.o[d][rb];
-          }
-        } else if (sum != 0.f) {  // (NaN is a sum too)
-          const Join j = join_maxima(all_m[rb], st.m[rb]);
-          all_l[rb] = join_sums(all_l[rb], sum, j);
-#pragma unroll
-          for (int d = 0; d < State::kBlocks; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) all_o[SPLIT ? 0 : d][rb][i] = join_sums(all_o[SPLIT ? 0 : d][rb][i], st.o[d][rb][i], j);
-        }
-      }
-      st.clear();
-    }
-    t = next;
-    stage ^= 1;
-  }
-  if (SPLIT) return;
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    if (!live[rb]) continue;
-    const bool sees = st.sight[rb].high > st.sight[rb].low;
-    const float reciprocal = sees ? 1.f / all_l[rb] : 0.f;
-    char* to = a.out + (int64_t)token[rb] * a.out_token_stride + (int64_t)(key_head * a.group + head[rb]) * a.out_head_stride;
-#pragma unroll
-    for (int d = 0; d < State::kBlocks; ++d) {
-      const f32x4_t& o = all_o[SPLIT ? 0 : d][rb];
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = sees ? output_of(o[i], reciprocal) : 0.f;
-      if (16 * d + 4 * grp < a.cache.width)
-        *reinterpret_cast<u32x2_t*>(to + 2 * (16 * d + 4 * grp)) = u32x2_t{Half<DTYPE>::pack(y[0], y[1]), Half<DTYPE>::pack(y[2], y[3])};
-    }
-    if (a.lse && grp == 0) a.lse[(int64_t)token[rb] * a.heads + key_head * a.group + head[rb]] = sees ? lse_of(all_m[rb], all_l[rb]) : -INFINITY;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Few rows: a wave takes 16 rows and every chunks-th run, on its own. Keys go straight into registers (a lane reads the pieces
-// of its key that the matrix instruction wants), values through the wave's own two tiles of LDS.
-// ---------------------------------------------------------------------------
-constexpr int kRowWaves = 2;
-
-template <int DTYPE, int SLABS>
-__global__ __launch_bounds__(kRowWaves * 64) void attention_rows_kernel(const AttentionArgs a) {
-  typedef Rows<DTYPE, SLABS, 1> State;
-  constexpr int kRows = 16;
-  constexpr int kTileBytes = SLABS * kSlabBytes;
-  extern __shared__ __align__(16) char lds[];  // [wave][2][values]
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, grp = lane >> 4;
-  char* const mine = lds + wave * 2 * kTileBytes;
-
-  const uint32_t id = blockIdx.x;
-  const uint32_t outer = divide_by(id, a.by_key_heads);
-  const int key_head = (int)(id - outer * a.cache.key_heads);
-  const int workgroups = a.chunks / kRowWaves;
-  const int chunk_id = (int)(outer % (uint32_t)workgroups) * kRowWaves + wave;
-  const int tile_id = (int)(outer / (uint32_t)workgroups);
-  const int s = wave_search(a.cache.sequences + 1, tile_id, lane, [&](int i) { return first_row_tile<kRows>(a, i); });
-  if (s < 0 || s >= a.cache.sequences) return;
-  const Chunk c = chunk_of(a, s);
-  const int rows = c.tokens * a.group;
-  const int row0 = (int)(tile_id - first_row_tile<kRows>(a, s)) * kRows;
-  if (row0 >= rows) return;
-  const int last_row = min(row0 + kRows, rows) - 1;
-  const Sight first_sight = sight_of(a, c, (int)divide_by(row0, a.by_group)), last_sight = sight_of(a, c, (int)divide_by(last_row, a.by_group));
-  const int capacity = capacity_of(a);
-  const int low = first_sight.low, high = min(last_sight.high, capacity + 1);
-  const int end_tile = (high + kTileKeys - 1) / kTileKeys;
-  int run = run_of_tile(low / kTileKeys) + chunk_id;
-  int t = max(run_first_tile(run), low / kTileKeys);
-  if (t >= end_tile) return;
-
-  State st;
-  int token[1], head[1];
-  bool live[1];
-  {
-    const int row = row0 + l16;
-    live[0] = row < rows;
-    const int i = (int)divide_by(live[0] ? row : row0, a.by_group);
-    head[0] = (live[0] ? row : row0) - i * a.group;
-    token[0] = c.first_token + i;
-    st.sight[0] = live[0] ? sight_of(a, c, i) : Sight{0, 0};
-  }
-  st.load_q(a, key_head, token, head, live, l16, grp, nullptr);
-  st.clear();
-  TileLoader<SLABS> loader;
-  loader.init(a, key_head, lane);
-  typename State::ValuePlace place;
-  place.init(l16, grp);
-  const char* const none = reinterpret_cast<const char*>(kSpecialRows[0]);
-
-  auto next_tile = [&](int tile) {
-    const int r = run_of_tile(tile);
-    return tile + 1 < run_first_tile(r + 1) ? tile + 1 : run_first_tile(r + a.chunks);
-  };
-  KeyPlace key_where[4], value_where[8];  // of the tile that is loaded next
-  auto find_pages = [&](int tile) {
-#pragma unroll
-    for (int b = 0; b < 4; ++b) key_where[b].ask(a, s, tile * kTileKeys + 16 * b + l16);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) value_where[j].ask(a, s, tile * kTileKeys + 8 * j + (lane >> 3));
-  };
-  auto load_values = [&](int tile, int stage) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const char* v = key_row_address(a, loader.values, loader.value_page, loader.value_row, value_where[j].entry, tile * kTileKeys + 8 * j + (lane >> 3), low, high);
-#pragma unroll
-      for (int slab = 0; slab < SLABS; ++slab) {
-        const int vc = slab * 8 + loader.value_chunk;
-        const char* from = vc * 8 < a.cache.width ? v + vc * 16 : none;
-        __builtin_amdgcn_global_load_lds((global_ptr_t)from, (lds_ptr_t)(mine + stage * kTileBytes + slab * kSlabBytes + j * 1024), 16, 0, 0);
-      }
-    }
-  };
-  u32x4_t k[State::kSteps][4];
-  auto load_keys = [&](int tile) {
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const char* from = key_row_address(a, loader.keys, loader.key_page, loader.key_row, key_where[b].entry, tile * kTileKeys + 16 * b + l16, low, high);
-#pragma unroll
-      for (int ks = 0; ks < State::kSteps; ++ks) {
-        const int element = 32 * ks + 8 * grp;
-        k[ks][b] = *reinterpret_cast<const u32x4_t*>(element < a.cache.width ? from + 2 * element : none);
-      }
-    }
-  };
-
-  int stage = 0;
-  find_pages(t);
-  load_values(t, 0);
-  asm volatile("" ::: "memory");
-  load_keys(t);
-  if (next_tile(t) < end_tile) find_pages(next_tile(t));
-  while (t < end_tile) {
-    const int key0 = t * kTileKeys;
-    const int next = next_tile(t);
-    f32x4_t scores[4][1];
-#pragma unroll
-    for (int b = 0; b < 4; ++b) scores[b][0] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int ks = 0; ks < State::kSteps; ++ks)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) scores[b][0] = Half<DTYPE>::mfma(k[ks][b], st.q[ks][0], scores[b][0]);
-    __builtin_amdgcn_s_waitcnt(kWaitAll0);  // its values are here too, and those of the tile before have been read
-    asm volatile("" ::: "memory");
-    const bool mixed = min(key0 + kTileKeys, high) > first_sight.high || max(key0, low) < last_sight.low;
-    const value_bytes_t values = (value_bytes_t)(mine + stage * kTileBytes);
-    bool special = false;
-    if (mixed) {
-      uint32_t any = 0;
-#pragma unroll
-      for (int j = 0; j < 8 * SLABS; ++j) {
-        const u32x4_t w = read_chunk(values + j * 1024 + lane * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) any |= special_halves<DTYPE>(w[e]);
-      }
-      special = __any(any != 0);
-    }
-    if (next < end_tile) {
-      load_values(next, stage ^ 1);
-      asm volatile("" ::: "memory");
-      load_keys(next);
-      if (next_tile(next) < end_tile) find_pages(next_tile(next));
-    }
-    u32x4_t p[2][1];
-    volatile float effect[4 * State::kBlocks];
-    if (key0 + kTileKeys > first_sight.high || key0 < last_sight.low) st.mask(scores, key0, grp);
-    st.weigh(a, scores, p);
-    if (special) {
-      st.find_special(values, place, p, key0, grp, effect);
-#pragma unroll 1
-      for (int j = 0; j < 8 * SLABS; ++j) take_out_special<DTYPE>(mine + stage * kTileBytes + j * 1024 + lane * 16);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    st.add_values(values, place, p);
-    if (special) st.add_special(effect);
-    const int this_run = run_of_tile(t);
-    if (next >= end_tile || run_of_tile(next) != this_run) {
-      const float sum = sum_over_groups(st.l[0]);
-      if (live[0]) {
-        const int64_t at = (int64_t)this_run * a.part_rows + (int64_t)token[0] * a.heads + key_head * a.group + head[0];
-        if (grp == 0) a.part_max[at] = st.m[0], a.part_sum[at] = sum;
+    for (int i = 0; i < 16; ++i) all_o[d][i] = 0.f;
+  // A run ends, with the maximum and this lane's sum.
+  auto end_run = [&](int run, float its_m, float its_l) __attribute__((always_inline)) {
+    const float sum = sum_over_halves(its_l);
+    if (SPLIT) {
+      const RowPlace r = row_place();
+      if (r.live) {
+        const int64_t at = (int64_t)run * a.part_rows + (int64_t)r.token * a.heads + r.head;
+        if (half == 0) a.part_max[at] = its_m, a.part_sum[at] = sum;
 #pragma unroll
         for (int d = 0; d < State::kBlocks; ++d)
-          if (16 * d + 4 * grp < a.cache.width) *reinterpret_cast<f32x4_t*>(a.part_out + at * a.cache.width + 16 * d + 4 * grp) = st.o[d][0];
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const int element = 32 * d + 2 * i + 4 * half;
+            if (element < a.cache.width)
+              *reinterpret_cast<f32x4_t*>(a.part_out + at * a.cache.width + element) = f32x4_t{st.o[d][i], st.o[d][i + 1], st.o[d][i + 2], st.o[d][i + 3]};
+          }
       }
-      st.clear();
+    } else if (sum != 0.f) {  // (NaN is a sum too)
+      const Join j = join_maxima(all_m, its_m);
+      all_l = join_sums(all_l, sum, j);
+      if (__any(j.kept != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < State::kBlocks; ++d) all_o[SPLIT ? 0 : d] *= j.kept;
+      }
+#pragma unroll
+      for (int d = 0; d < State::kBlocks; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) all_o[SPLIT ? 0 : d][i] = __builtin_fmaf(st.o[d][i], j.added, all_o[SPLIT ? 0 : d][i]);
     }
-    t = next;
-    stage ^= 1;
+    st.clear_output();
+  };
+
+  if (t < end_tile) {
+    if (GROUPED) {
+      lane_where.ask(a, s, key_of_lane(t));
+      find_addresses(t);
+      value_low = later_low, value_high = later_high;
+    } else {
+      find_entries(t);
+      find_entries(t + 1 < end_tile ? t + 1 : t);
+    }
+    load_keys(here, t, 0);
+    // The first turn multiplies weights of 0 with what lies where its values would: it must be numbers.
+    for (int i = tid * 16; i < kTileBytes; i += WAVES * 64 * 16) *reinterpret_cast<u32x4_t*>(values_of(1) + i) = u32x4_t{0, 0, 0, 0};
+    __builtin_amdgcn_s_waitcnt(kWaitAll0);
+    wg_barrier();
   }
+  int stage = 0, before = -1;  // the tile whose weights wait for its values
+  if (!wave_live) {  // loads its share, no more
+    for (; t < end_tile; ++t, stage ^= 1) {
+      ask_for(t, stage);
+      landed(t, stage, false);
+    }
+    return;
+  }
+  const int masked_from = wave_first.high / kTileKeys, masked_to = (wave_last.low + kTileKeys - 1) / kTileKeys;
+  int run_end = t < end_tile ? run_first_tile(run_of_tile(t) + 1) : 0;
+  st.clear_output();
+  st.m = -INFINITY;
+  st.l = 0.f;
+  u32x4_t p[4];
+#pragma unroll
+  for (int f = 0; f < 4; ++f) p[f] = u32x4_t{0, 0, 0, 0};
+  // The products read their fragments a few ahead of their use.
+  constexpr int kAhead = 4, kValueFragments = 4 * State::kBlocks, kKeyFragments = 2 * State::kSteps;
+  auto value_fragment = [&](int n, int its_stage) __attribute__((always_inline)) {  // 16 keys n / kBlocks, block n % kBlocks
+    const int d = n % State::kBlocks, f = n / State::kBlocks;
+    const value_bytes_t at = (value_bytes_t)values_of(its_stage) + value_at[d & 1] + (d >> 1) * kSlabBytes + f * 2048;
+    const u32x2_t x = read_values_transposed(at), y = read_values_transposed(at + 1024);
+    return u32x4_t{x.x, x.y, y.x, y.y};
+  };
+  auto key_fragment = [&](int n) __attribute__((always_inline)) {  // step n / 2, 32 keys n % 2
+    return read_chunk((value_bytes_t)keys_of(stage) + key_at[(n >> 1) & 3] + (n >> 3) * kSlabBytes + (n & 1) * 4096);
+  };
+  auto query_fragment = [&](int ks) __attribute__((always_inline)) { return kKeepQ ? kept_q[kKeepQ ? ks : 0] : read_chunk((value_bytes_t)shelf + key_at[ks & 3] + (ks >> 2) * 4096); };
+
+  // One turn. PLAIN: every row sees every key of the tile, and the last tile's values hold nothing special and do not end a run.
+  auto turn = [&](auto plain, float& its_m, float& its_l) __attribute__((always_inline)) {
+    constexpr bool PLAIN = decltype(plain)::value != 0;
+    ask_for(t, stage);
+    f32x16_t scores[2];
+    u32x4_t ring[kAhead], q[2];
+    q[0] = query_fragment(0);
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) ring[n] = key_fragment(n);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) scores[b][i] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < kKeyFragments; ++n) {
+      const int ks = n >> 1, b = n & 1, next = n + kAhead;
+      if (b == 0 && ks + 1 < State::kSteps) q[(ks + 1) & 1] = query_fragment(ks + 1);
+      scores[b] = H::mfma(ring[n % kAhead], q[ks & 1], scores[b]);
+      if (next < kKeyFragments)
+        ring[n % kAhead] = key_fragment(next);
+      else
+        ring[n % kAhead] = value_fragment(next - kKeyFragments, stage ^ 1);
+      __builtin_amdgcn_sched_barrier(0);  // (or the reads move back to their use)
+    }
+    if (!PLAIN) {
+      if (t >= masked_from || t < masked_to) st.mask(scores, t * kTileKeys);
+      // A run that has ended waits with its statistics for its last values.
+      its_m = st.m, its_l = st.l;
+      if (t == run_end) st.m = -INFINITY, st.l = 0.f;
+    }
+    Weighing<DTYPE> weighing;
+    u32x4_t next_p[4];
+#pragma unroll
+    for (int n = 0; n < kValueFragments; ++n) {
+      const int d = n % State::kBlocks, f = n / State::kBlocks, next = n + kAhead;
+      st.o[d] = H::mfma(ring[n % kAhead], p[f], st.o[d]);
+      if (next < kValueFragments) ring[n % kAhead] = value_fragment(next, stage ^ 1);
+#pragma unroll
+      for (int j = 0; j < Weighing<DTYPE>::kPieces; ++j)
+        if (j * kValueFragments / Weighing<DTYPE>::kPieces == n) weighing.template piece<SLABS>(j, a, st, scores, next_p);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int f = 0; f < 4; ++f) p[f] = next_p[f];
+    landed(t, stage, PLAIN);
+    before = t, ++t, stage ^= 1;
+    return weighing.factor;
+  };
+  while (t < end_tile) {
+    // A turn with everything that may come up, then plain ones as long as nothing does: what changes the outputs besides the
+    // products stands outside of their loop, where it would have them copied from register to register in every turn.
+    const bool run_starts = t == run_end;
+    float its_m, its_l;
+    volatile float effect[16 * State::kBlocks];  // (in memory, see find_special)
+    const bool special = before >= 0 && mixed(before) && special_tile[stage ^ 1] == before + 1;
+    if (special) find_special<DTYPE, State>(a, st, value_side, s, p, before * kTileKeys, low, high, lane, effect);
+    float factor = turn(IntTag<0>{}, its_m, its_l);
+    if (special) st.add_special(effect);
+    if (run_starts) {
+      const int run = run_of_tile(before);
+      end_run(run - 1, its_m, its_l);
+      run_end = run_first_tile(run + 1);
+      factor = 1.f;
+    }
+    const int plain_to = min(min(run_end, end_tile), min(masked_from, mixed_from)), plain_from = max(masked_to, mixed_to + 1);
+    while (t >= plain_from && t < plain_to && !__any(factor != 1.f)) factor = turn(IntTag<1>{}, its_m, its_l);
+    if (__any(factor != 1.f)) {
+#pragma unroll
+      for (int d = 0; d < State::kBlocks; ++d) st.o[d] *= factor;
+    }
+  }
+  if (before >= 0) {  // the last tile's values
+    volatile float effect[16 * State::kBlocks];
+    const bool special = mixed(before) && special_tile[stage ^ 1] == before + 1;
+    if (special) find_special<DTYPE, State>(a, st, value_side, s, p, before * kTileKeys, low, high, lane, effect);
+#pragma unroll
+    for (int n = 0; n < kValueFragments; ++n) {
+      const int d = n % State::kBlocks, f = n / State::kBlocks;
+      st.o[d] = H::mfma(value_fragment(n, stage ^ 1), p[f], st.o[d]);
+    }
+    if (special) st.add_special(effect);
+    end_run(run_of_tile(before), st.m, st.l);
+  }
+  if (SPLIT) return;
+  const RowPlace r = row_place();
+  if (!r.live) return;
+  const bool any = st.sight.high > st.sight.low;
+  const float reciprocal = any ? 1.f / all_l : 0.f;
+  char* const to = a.out + (int64_t)r.token * a.out_token_stride + (int64_t)r.head * a.out_head_stride;
+#pragma unroll
+  for (int d = 0; d < State::kBlocks; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const f32x16_t& o = all_o[SPLIT ? 0 : d];
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = any ? output_of(o[i + e], reciprocal) : 0.f;
+      const int element = 32 * d + 2 * i + 4 * half;
+      if (element < a.cache.width) *reinterpret_cast<u32x2_t*>(to + 2 * element) = u32x2_t{H::pack(y[0], y[1]), H::pack(y[2], y[3])};
+    }
+  if (a.lse && half == 0) a.lse[(int64_t)r.token * a.heads + r.head] = any ? lse_of(all_m, all_l) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -893,17 +904,16 @@ static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, in
   const int most = c.width > 128 ? 128 : 256;  // rows of the largest tile
   const int choice = config & 0xff;
   const int64_t each = (tokens + c.sequences - 1) / c.sequences * group;  // rows of a sequence and key head
-  p.rows = choice == RLK_ATTENTION_CFG_ROWS16 ? 16 : choice == RLK_ATTENTION_CFG_ROWS64 ? 64 : choice == RLK_ATTENTION_CFG_ROWS256 ? most : each <= 16 ? 16 : each <= 64 ? 64 : most;
+  p.rows = choice == RLK_ATTENTION_CFG_ROWS32 ? 32 : choice == RLK_ATTENTION_CFG_ROWS128 ? 128 : choice == RLK_ATTENTION_CFG_ROWS256 ? most : each <= 32 ? 32 : each <= 128 ? 128 : most;
   p.tiles = (int)(tokens * group / p.rows) + c.sequences + 1;
   const int runs = run_limit(c);
   const int64_t side_by_side = (int64_t)(p.tiles - 1) * c.key_heads;
   const int cus = device_cu_count();
-  p.split = p.rows == 16 || (choice != RLK_ATTENTION_CFG_AUTO ? (config & RLK_ATTENTION_CFG_SPLIT) != 0 : side_by_side < cus && runs > 1);
+  p.split = p.rows == 32 || (choice != RLK_ATTENTION_CFG_AUTO ? (config & RLK_ATTENTION_CFG_SPLIT) != 0 : side_by_side < cus && runs > 1);
   p.chunks = 1;
   if (p.split) {
-    const int64_t wanted = p.rows == 16 ? (16 * cus + side_by_side - 1) / side_by_side : (2 * cus + side_by_side - 1) / side_by_side;
+    const int64_t wanted = p.rows == 32 ? (8 * cus + side_by_side - 1) / side_by_side : (2 * cus + side_by_side - 1) / side_by_side;
     p.chunks = (int)(wanted < 1 ? 1 : wanted < runs ? wanted : runs);
-    if (p.rows == 16) p.chunks = (p.chunks + kRowWaves - 1) / kRowWaves * kRowWaves;
   }
   return p;
 }
@@ -914,35 +924,29 @@ size_t paged_attention_workspace_bytes(const rlk_paged_cache& c, int64_t tokens,
   return (size_t)run_limit(c) * tokens * heads * (c.width + 2) * sizeof(float);
 }
 
-template <int DTYPE, int SLABS, int RB, int WAVES, bool SPLIT>
+template <int DTYPE, int SLABS, int WAVES, bool SPLIT, bool GROUPED>
 static hipError_t attention_tiles_launch(const AttentionArgs& a, hipStream_t stream) {
-  constexpr int kLds = 4 * SLABS * kSlabBytes + (RB == 1 ? 0 : WAVES * RB * SLABS * 2048) + 16;
+  constexpr int kLds = 4 * SLABS * kSlabBytes + (SLABS > 2 ? 0 : WAVES * SLABS * 4096) + 16;
   static PerDeviceOnce once;
-  const auto kernel = attention_tile_kernel<DTYPE, SLABS, RB, WAVES, SPLIT>;
+  const auto kernel = attention_tile_kernel<DTYPE, SLABS, WAVES, SPLIT, GROUPED>;
   const hipError_t err = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, once);
   if (err != hipSuccess) return err;
   kernel<<<dim3((unsigned)(a.tiles * a.chunks * a.cache.key_heads)), WAVES * 64, kLds, stream>>>(a);
   return hipGetLastError();
 }
-template <int DTYPE, int SLABS, bool SPLIT>
-static hipError_t attention_tiles_of(const AttentionArgs& a, int rows, hipStream_t stream) {
-  if (rows == 64) return attention_tiles_launch<DTYPE, SLABS, 1, 4, SPLIT>(a, stream);
-  return attention_tiles_launch<DTYPE, SLABS, SLABS <= 2 ? 2 : 1, 8, SPLIT>(a, stream);
+template <int DTYPE, int SLABS, bool GROUPED>
+static hipError_t attention_tiles_of(const AttentionArgs& a, const AttentionPlan& p, hipStream_t stream) {
+  if (p.rows == 32) return attention_tiles_launch<DTYPE, SLABS, 1, true, GROUPED>(a, stream);
+  if constexpr (SLABS <= 2)
+    if (p.rows == 256)
+      return p.split ? attention_tiles_launch<DTYPE, SLABS, 8, true, GROUPED>(a, stream) : attention_tiles_launch<DTYPE, SLABS, 8, false, GROUPED>(a, stream);
+  return p.split ? attention_tiles_launch<DTYPE, SLABS, 4, true, GROUPED>(a, stream) : attention_tiles_launch<DTYPE, SLABS, 4, false, GROUPED>(a, stream);
 }
 template <int DTYPE, int SLABS>
 static hipError_t attention_launch_of(const AttentionArgs& a, const AttentionPlan& p, hipStream_t stream) {
-  hipError_t err;
-  if (p.rows == 16) {
-    constexpr int kLds = kRowWaves * 2 * SLABS * kSlabBytes;
-    static PerDeviceOnce once;
-    const auto kernel = attention_rows_kernel<DTYPE, SLABS>;
-    err = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, once);
-    if (err != hipSuccess) return err;
-    kernel<<<dim3((unsigned)(a.tiles * (a.chunks / kRowWaves) * a.cache.key_heads)), kRowWaves * 64, kLds, stream>>>(a);
-    err = hipGetLastError();
-  } else {
-    err = p.split ? attention_tiles_of<DTYPE, SLABS, true>(a, p.rows, stream) : attention_tiles_of<DTYPE, SLABS, false>(a, p.rows, stream);
-  }
+  const int64_t most = kSoloRange / 16;  // elements between rows: eight of them stay within a buffer's range
+  const bool grouped = a.cache.page_size % 8 == 0 && a.cache.key_row_stride < most && a.cache.value_row_stride < most;
+  const hipError_t err = grouped ? attention_tiles_of<DTYPE, SLABS, true>(a, p, stream) : attention_tiles_of<DTYPE, SLABS, false>(a, p, stream);
   if (err != hipSuccess || !p.split) return err;
   attention_join_kernel<DTYPE><<<dim3((unsigned)a.part_rows), (a.cache.width + 63) / 64 * 64, 0, stream>>>(a);
   return hipGetLastError();

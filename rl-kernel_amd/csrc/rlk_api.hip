@@ -994,7 +994,7 @@ static int check_attention(const char* who, const rlk_paged_cache* c, int64_t to
   if (c->width % 8 != 0 || c->width > 256) return refuse_argument(who, "width is no multiple of 8 up to 256");
   const int choice = config & 0xff;
   if ((config & ~(0xff | RLK_ATTENTION_CFG_SPLIT)) != 0 || choice > RLK_ATTENTION_CFG_ROWS256 ||
-      ((config & RLK_ATTENTION_CFG_SPLIT) != 0 && choice < RLK_ATTENTION_CFG_ROWS64))
+      ((config & RLK_ATTENTION_CFG_SPLIT) != 0 && choice < RLK_ATTENTION_CFG_ROWS128))
     return refuse_argument(who, "unknown configuration");
   return RLK_OK;
 }
@@ -1018,6 +1018,9 @@ int rlk_paged_attention(const rlk_paged_cache* cache, const void* q, int64_t q_t
       !on16(cache->keys, cache->key_page_stride, cache->key_row_stride, cache->key_head_stride) ||
       !on16(cache->values, cache->value_page_stride, cache->value_row_stride, cache->value_head_stride))
     return refuse_argument(who, "rows of q, out, keys and values start on 16 bytes");
+  auto within = [](int64_t stride) { return stride < (int64_t)1 << 31; };  // (4 GiB: the kernels multiply 32 bits by 32)
+  if (!within(cache->key_page_stride) || !within(cache->key_row_stride) || !within(cache->value_page_stride) || !within(cache->value_row_stride))
+    return refuse_argument(who, "pages and rows of the cache lie less than 2^31 elements apart");
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (cache->sequences == 0) return refuse_argument(who, "tokens without a sequence");
   const size_t need = paged_attention_workspace_bytes(*cache, tokens, heads, config);

@@ -135,7 +135,7 @@ EXPORTED_SYMBOLS = (
 
 
 # rlk_attention_config
-ATTENTION_CONFIGS = {"auto": 0, "rows16": 1, "rows64": 2, "rows256": 3, "rows64_split": 0x102, "rows256_split": 0x103}
+ATTENTION_CONFIGS = {"auto": 0, "rows32": 1, "rows128": 2, "rows256": 3, "rows128_split": 0x102, "rows256_split": 0x103}
 ROTARY_MAX_WIDTH = 1024
 ATTENTION_MAX_WIDTH = 256
 

@@ -10,7 +10,7 @@ from attention_cases import DEV, Batch, same_bits
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
-CONFIGS = ("rows16", "rows64", "rows256", "rows64_split", "rows256_split")
+CONFIGS = ("rows32", "rows128", "rows256", "rows128_split", "rows256_split")
 
 
 @pytest.fixture(scope="module")
