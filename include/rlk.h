@@ -656,13 +656,14 @@ int rlk_paged_append(const rlk_paged_cache* host_cache, const rlk_rotary* host_r
  */
 typedef enum rlk_attention_config {
   RLK_ATTENTION_CFG_AUTO = 0,
-  RLK_ATTENTION_CFG_ROWS32 = 1,  /* a wave for 32 rows of a key head, runs side by side, combined by a second launch */
-  RLK_ATTENTION_CFG_ROWS128 = 2, /* four waves of 32 rows, all runs one after the other */
-  RLK_ATTENTION_CFG_ROWS256 = 3, /* eight waves of 32 rows (four for heads wider than 128) */
-  RLK_ATTENTION_CFG_SPLIT = 0x100 /* OR-ed into the last two: runs side by side, combined by a second launch */
+  /* rows of a key head that share what is read, all runs one after the other; pages of a number of rows that 8 does not divide: always 128 */
+  RLK_ATTENTION_CFG_ROWS64 = 1,
+  RLK_ATTENTION_CFG_ROWS128 = 2,
+  RLK_ATTENTION_CFG_ROWS256 = 3, /* (128 for heads wider than 128) */
+  RLK_ATTENTION_CFG_SPLIT = 0x100 /* OR-ed into these: runs side by side, combined by a second launch */
 } rlk_attention_config;
 const char* rlk_attention_contract_id(void);
-size_t rlk_paged_attention_workspace_bytes(const rlk_paged_cache* host_cache, int64_t tokens, int heads, int config);
+size_t rlk_paged_attention_workspace_bytes(const rlk_paged_cache* host_cache, int64_t tokens, int heads, int window, int config);
 int rlk_paged_attention(const rlk_paged_cache* host_cache, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
                         int64_t out_token_stride, int64_t out_head_stride, float* lse, int64_t tokens, int heads, float scale,
                         int causal, int window, int zero_rest, int config, void* workspace, size_t workspace_bytes, void* stream);

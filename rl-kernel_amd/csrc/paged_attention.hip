@@ -433,7 +433,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   typedef Rows<DTYPE, SLABS> State;
   typedef Half<DTYPE> H;
   constexpr int kRows = 32 * WAVES;
-  constexpr bool kKeepQ = SLABS > 2;  // queries stay in registers; else in LDS
+  constexpr bool kKeepQ = SLABS > 2 || WAVES <= 2;  // queries stay in registers; else in LDS
   constexpr int kGroups = 8 / WAVES;  // groups of 8 keys that a wave loads
   constexpr int kSpan = 64 / kGroups;  // tiles whose addresses the lanes of a wave have
   constexpr int kTileBytes = SLABS * kSlabBytes;
@@ -518,9 +518,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   CacheSide key_side, value_side;
   key_side.init(a.cache.keys, key_head * a.cache.key_head_stride, a.cache.key_page_stride, a.cache.key_row_stride);
   value_side.init(a.cache.values, key_head * a.cache.value_head_stride, a.cache.value_page_stride, a.cache.value_row_stride);
-  // Of a loading lane; of keys for even and odd groups of eight.
-  const int odd_wave = WAVES == 1 ? 0 : 8 * (wave & 1);
-  const int key_chunk[2] = {(lane & 7) ^ key_swizzle(odd_wave + (lane >> 3)), (lane & 7) ^ key_swizzle(odd_wave + 8 + (lane >> 3))};
+  // Of a loading lane.
+  const int key_chunk = (lane & 7) ^ key_swizzle(8 * (wave & 1) + (lane >> 3));  // (a wave's groups of eight keys are all even or all odd)
   const int value_chunk = (lane & 7) ^ value_swizzle(lane >> 3);
   // This lane's places in the images: of 16 elements of its key (or query) for every step of a slab, of its elements' values for even
   // and odd blocks of 32.
@@ -576,12 +575,10 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
       ahead[j].ask(a, s, tile * kTileKeys + (wave + j * WAVES) * 8 + (lane >> 3));
     }
   };
-  uint32_t key_offset[2][SLABS], value_offset[SLABS];
+  uint32_t key_offset[SLABS], value_offset[SLABS];
 #pragma unroll
   for (int slab = 0; slab < SLABS; ++slab) {
-#pragma unroll
-    for (int odd = 0; odd < 2; ++odd)
-      key_offset[odd][slab] = (slab * 8 + key_chunk[odd]) * 8 < a.cache.width ? (lane >> 3) * key_side.row + key_chunk[odd] * 16 + slab * 128 : kSoloOutside;
+    key_offset[slab] = (slab * 8 + key_chunk) * 8 < a.cache.width ? (lane >> 3) * key_side.row + key_chunk * 16 + slab * 128 : kSoloOutside;
     value_offset[slab] = (slab * 8 + value_chunk) * 8 < a.cache.width ? (lane >> 3) * value_side.row + value_chunk * 16 + slab * 128 : kSoloOutside;
   }
   const int whole_from = (low + kTileKeys - 1) / kTileKeys, whole_to = high / kTileKeys;  // tiles all of whose keys are needed
@@ -590,9 +587,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
     for (int j = 0; j < kGroups; ++j) {
       const int i = (tile - key_from) * kGroups + j, first_key = tile * kTileKeys + (wave + j * WAVES) * 8;
       char* const to = keys_of(stage) + (wave + j * WAVES) * 1024;
-      const int odd = WAVES == 1 ? j & 1 : 0;  // (more waves: a wave's groups are all even or all odd)
       if (GROUPED)
-        load_group<SLABS>(__builtin_amdgcn_readlane(key_low, i), __builtin_amdgcn_readlane(key_high, i), key_offset[odd],
+        load_group<SLABS>(__builtin_amdgcn_readlane(key_low, i), __builtin_amdgcn_readlane(key_high, i), key_offset,
                           tile >= whole_from && tile < whole_to, first_key, low, high, key_side.row, a.cache.width, key_swizzle, to);
       else
         load_rows<SLABS>(a, key_side, where[j], (lane & 7) ^ key_swizzle(first_key + (lane >> 3)), first_key + (lane >> 3), low, high, to);
@@ -898,35 +894,51 @@ static int run_limit(const rlk_paged_cache& c) {
   return run_of_tile(capacity_of(c) / kTileKeys) + 1;  // (with the position behind the table)
 }
 
-static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, int heads, int config) {
+static bool pages_of_groups(const rlk_paged_cache& c) {
+  const int64_t most = kSoloRange / 16;  // elements between rows: eight of them stay within a buffer's range
+  return c.page_size % 8 == 0 && c.key_row_stride < most && c.value_row_stride < most;
+}
+
+// Tiles. A call is sized by what it may need: its tokens, spread evenly over the sequences, and the table's positions (or the window's).
+static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, int heads, int window, int config) {
   AttentionPlan p;
   const int group = heads / c.key_heads;
   const int most = c.width > 128 ? 128 : 256;  // rows of the largest tile
   const int choice = config & 0xff;
   const int64_t each = (tokens + c.sequences - 1) / c.sequences * group;  // rows of a sequence and key head
-  p.rows = choice == RLK_ATTENTION_CFG_ROWS32 ? 32 : choice == RLK_ATTENTION_CFG_ROWS128 ? 128 : choice == RLK_ATTENTION_CFG_ROWS256 ? most : each <= 32 ? 32 : each <= 128 ? 128 : most;
-  p.tiles = (int)(tokens * group / p.rows) + c.sequences + 1;
+  const int64_t cus = device_cu_count();
   const int runs = run_limit(c);
-  const int64_t side_by_side = (int64_t)(p.tiles - 1) * c.key_heads;
-  const int cus = device_cu_count();
-  p.split = p.rows == 32 || (choice != RLK_ATTENTION_CFG_AUTO ? (config & RLK_ATTENTION_CFG_SPLIT) != 0 : side_by_side < cus && runs > 1);
+  auto side_by_side = [&](int rows) { return (int64_t)c.sequences * ((each + rows - 1) / rows) * c.key_heads; };
+  const int64_t seen = window > 0 ? window + tokens / c.sequences : kMostKeys;
+  const int64_t depth = (seen < capacity_of(c) ? seen : capacity_of(c)) / kTileKeys + 1;  // tiles that a row tile goes through
+  if (choice != RLK_ATTENTION_CFG_AUTO) {
+    p.rows = 64 << (choice - RLK_ATTENTION_CFG_ROWS64);
+    p.split = (config & RLK_ATTENTION_CFG_SPLIT) != 0;
+  } else {
+    p.rows = each <= 64 ? 64 : each <= 128 ? 128 : most;
+    if (p.rows == 256 && side_by_side(256) < cus && (4 * side_by_side(128) >= 3 * cus || depth < 32)) p.rows = 128;
+    const int64_t units = side_by_side(p.rows);
+    p.split = p.rows == 64 ? (units < cus && depth > 8) || (units < 4 * cus && depth >= 64) : 4 * units < 3 * cus && depth >= 32;
+  }
+  if (p.rows > most || !pages_of_groups(c)) p.rows = 128;
+  p.tiles = (int)(tokens * group / p.rows) + c.sequences + 1;
   p.chunks = 1;
   if (p.split) {
-    const int64_t wanted = p.rows == 32 ? (8 * cus + side_by_side - 1) / side_by_side : (2 * cus + side_by_side - 1) / side_by_side;
-    p.chunks = (int)(wanted < 1 ? 1 : wanted < runs ? wanted : runs);
+    const int64_t units = side_by_side(p.rows), wanted = ((p.rows == 64 ? 8 : 2) * cus + units - 1) / units, of_runs = depth / 4 + 1 < runs ? depth / 4 + 1 : runs;
+    p.chunks = (int)(wanted < of_runs ? wanted : of_runs);
   }
   return p;
 }
 
-size_t paged_attention_workspace_bytes(const rlk_paged_cache& c, int64_t tokens, int heads, int config) {
+size_t paged_attention_workspace_bytes(const rlk_paged_cache& c, int64_t tokens, int heads, int window, int config) {
   if (tokens == 0 || c.sequences == 0 || heads == 0) return 0;
-  if (!attention_plan(c, tokens, heads, config).split) return 0;
+  if (!attention_plan(c, tokens, heads, window, config).split) return 0;
   return (size_t)run_limit(c) * tokens * heads * (c.width + 2) * sizeof(float);
 }
 
 template <int DTYPE, int SLABS, int WAVES, bool SPLIT, bool GROUPED>
 static hipError_t attention_tiles_launch(const AttentionArgs& a, hipStream_t stream) {
-  constexpr int kLds = 4 * SLABS * kSlabBytes + (SLABS > 2 ? 0 : WAVES * SLABS * 4096) + 16;
+  constexpr int kLds = 4 * SLABS * kSlabBytes + (SLABS > 2 || WAVES <= 2 ? 0 : WAVES * SLABS * 4096) + 16;
   static PerDeviceOnce once;
   const auto kernel = attention_tile_kernel<DTYPE, SLABS, WAVES, SPLIT, GROUPED>;
   const hipError_t err = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, once);
@@ -934,19 +946,19 @@ static hipError_t attention_tiles_launch(const AttentionArgs& a, hipStream_t str
   kernel<<<dim3((unsigned)(a.tiles * a.chunks * a.cache.key_heads)), WAVES * 64, kLds, stream>>>(a);
   return hipGetLastError();
 }
-template <int DTYPE, int SLABS, bool GROUPED>
+template <int DTYPE, int SLABS, bool SPLIT, bool GROUPED>
 static hipError_t attention_tiles_of(const AttentionArgs& a, const AttentionPlan& p, hipStream_t stream) {
-  if (p.rows == 32) return attention_tiles_launch<DTYPE, SLABS, 1, true, GROUPED>(a, stream);
-  if constexpr (SLABS <= 2)
-    if (p.rows == 256)
-      return p.split ? attention_tiles_launch<DTYPE, SLABS, 8, true, GROUPED>(a, stream) : attention_tiles_launch<DTYPE, SLABS, 8, false, GROUPED>(a, stream);
-  return p.split ? attention_tiles_launch<DTYPE, SLABS, 4, true, GROUPED>(a, stream) : attention_tiles_launch<DTYPE, SLABS, 4, false, GROUPED>(a, stream);
+  if constexpr (GROUPED)
+    if (p.rows == 64) return attention_tiles_launch<DTYPE, SLABS, 2, SPLIT, GROUPED>(a, stream);
+  if constexpr (GROUPED && SLABS <= 2)
+    if (p.rows == 256) return attention_tiles_launch<DTYPE, SLABS, 8, SPLIT, GROUPED>(a, stream);
+  return attention_tiles_launch<DTYPE, SLABS, 4, SPLIT, GROUPED>(a, stream);
 }
 template <int DTYPE, int SLABS>
 static hipError_t attention_launch_of(const AttentionArgs& a, const AttentionPlan& p, hipStream_t stream) {
-  const int64_t most = kSoloRange / 16;  // elements between rows: eight of them stay within a buffer's range
-  const bool grouped = a.cache.page_size % 8 == 0 && a.cache.key_row_stride < most && a.cache.value_row_stride < most;
-  const hipError_t err = grouped ? attention_tiles_of<DTYPE, SLABS, true>(a, p, stream) : attention_tiles_of<DTYPE, SLABS, false>(a, p, stream);
+  const bool grouped = pages_of_groups(a.cache);
+  const hipError_t err = p.split ? (grouped ? attention_tiles_of<DTYPE, SLABS, true, true>(a, p, stream) : attention_tiles_of<DTYPE, SLABS, true, false>(a, p, stream))
+                                 : (grouped ? attention_tiles_of<DTYPE, SLABS, false, true>(a, p, stream) : attention_tiles_of<DTYPE, SLABS, false, false>(a, p, stream));
   if (err != hipSuccess || !p.split) return err;
   attention_join_kernel<DTYPE><<<dim3((unsigned)a.part_rows), (a.cache.width + 63) / 64 * 64, 0, stream>>>(a);
   return hipGetLastError();
@@ -961,7 +973,7 @@ static hipError_t attention_launch_as(const AttentionArgs& a, const AttentionPla
 hipError_t paged_attention_launch(const rlk_paged_cache& cache, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
                                   int64_t out_token_stride, int64_t out_head_stride, float* lse, int64_t tokens, int heads, float scale,
                                   bool causal, int window, bool zero_rest, int config, void* workspace, hipStream_t stream) {
-  const AttentionPlan p = attention_plan(cache, tokens, heads, config);
+  const AttentionPlan p = attention_plan(cache, tokens, heads, window, config);
   AttentionArgs a{};
   a.cache = cache;
   a.q = static_cast<const char*>(q);

@@ -994,14 +994,18 @@ static int check_attention(const char* who, const rlk_paged_cache* c, int64_t to
   if (c->width % 8 != 0 || c->width > 256) return refuse_argument(who, "width is no multiple of 8 up to 256");
   const int choice = config & 0xff;
   if ((config & ~(0xff | RLK_ATTENTION_CFG_SPLIT)) != 0 || choice > RLK_ATTENTION_CFG_ROWS256 ||
-      ((config & RLK_ATTENTION_CFG_SPLIT) != 0 && choice < RLK_ATTENTION_CFG_ROWS128))
+      ((config & RLK_ATTENTION_CFG_SPLIT) != 0 && choice == RLK_ATTENTION_CFG_AUTO))
     return refuse_argument(who, "unknown configuration");
   return RLK_OK;
 }
 
-size_t rlk_paged_attention_workspace_bytes(const rlk_paged_cache* cache, int64_t tokens, int heads, int config) {
+size_t rlk_paged_attention_workspace_bytes(const rlk_paged_cache* cache, int64_t tokens, int heads, int window, int config) {
   if (check_attention("rlk_paged_attention_workspace_bytes", cache, tokens, heads, config) != RLK_OK) return 0;
-  return paged_attention_workspace_bytes(*cache, tokens, heads, config);
+  if (window < 0) {
+    refuse_argument("rlk_paged_attention_workspace_bytes", "window is negative");
+    return 0;
+  }
+  return paged_attention_workspace_bytes(*cache, tokens, heads, window, config);
 }
 
 int rlk_paged_attention(const rlk_paged_cache* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
@@ -1023,7 +1027,7 @@ int rlk_paged_attention(const rlk_paged_cache* cache, const void* q, int64_t q_t
     return refuse_argument(who, "pages and rows of the cache lie less than 2^31 elements apart");
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (cache->sequences == 0) return refuse_argument(who, "tokens without a sequence");
-  const size_t need = paged_attention_workspace_bytes(*cache, tokens, heads, config);
+  const size_t need = paged_attention_workspace_bytes(*cache, tokens, heads, window, config);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) {
     set_last_error("%s: a 16-byte aligned workspace of %zu bytes is needed, %zu given", who, need, workspace_bytes);
     return RLK_ERR_INVALID_ARGUMENT;

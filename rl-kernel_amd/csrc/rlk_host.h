@@ -254,7 +254,7 @@ hipError_t rotary_launch(const rlk_rotary& rotary, const rlk_head_rows& q, const
                          int dtype, bool inverse, hipStream_t stream);
 hipError_t paged_append_launch(const rlk_paged_cache& cache, const rlk_rotary* rotary, const rlk_head_rows* q, const rlk_head_rows& k,
                                const rlk_head_rows& v, int64_t tokens, hipStream_t stream);
-size_t paged_attention_workspace_bytes(const rlk_paged_cache& cache, int64_t tokens, int heads, int config);
+size_t paged_attention_workspace_bytes(const rlk_paged_cache& cache, int64_t tokens, int heads, int window, int config);
 hipError_t paged_attention_launch(const rlk_paged_cache& cache, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
                                   int64_t out_token_stride, int64_t out_head_stride, float* lse, int64_t tokens, int heads, float scale,
                                   bool causal, int window, bool zero_rest, int config, void* workspace, hipStream_t stream);

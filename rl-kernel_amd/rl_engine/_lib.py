@@ -135,7 +135,7 @@ EXPORTED_SYMBOLS = (
 
 
 # rlk_attention_config
-ATTENTION_CONFIGS = {"auto": 0, "rows32": 1, "rows128": 2, "rows256": 3, "rows128_split": 0x102, "rows256_split": 0x103}
+ATTENTION_CONFIGS = {"auto": 0, **{f"rows{64 << i}{split}": (i + 1) | bit for i in range(3) for split, bit in (("", 0), ("_split", 0x100))}}
 ROTARY_MAX_WIDTH = 1024
 ATTENTION_MAX_WIDTH = 256
 
@@ -322,7 +322,7 @@ def load() -> ctypes.CDLL:
     lib.rlk_attention_contract_id.restype = c.c_char_p
     lib.rlk_attention_contract_id.argtypes = []
     lib.rlk_paged_attention_workspace_bytes.restype = sz
-    lib.rlk_paged_attention_workspace_bytes.argtypes = [cache, i64, i32, i32]
+    lib.rlk_paged_attention_workspace_bytes.argtypes = [cache, i64, i32, i32, i32]
     lib.rlk_paged_attention.restype = i32
     lib.rlk_paged_attention.argtypes = [cache, vp, i64, i64, vp, i64, i64, vp, i64, i32, f32, i32, i32, i32, i32, vp, sz, vp]
 

@@ -227,7 +227,7 @@ def paged_attention(
     elif tokens > 0:
         q = q if _on_16_bytes(q) else q.clone(memory_format=torch.contiguous_format)
         lib, how = _lib.load(), _lib.ATTENTION_CONFIGS[config]
-        size = int(lib.rlk_paged_attention_workspace_bytes(ctypes.byref(cache.c), tokens, heads, how))
+        size = int(lib.rlk_paged_attention_workspace_bytes(ctypes.byref(cache.c), tokens, heads, window or 0, how))
         workspace = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
         with _on(device):
             status = lib.rlk_paged_attention(

@@ -83,18 +83,19 @@ def test_attention_entry(rlk_lib):
             cache or _cache(), q, *strides, out, *out_strides, None, tokens, heads, scale, causal, window, 1, config, workspace, size, None
         )
 
-    need = int(rlk_lib.rlk_paged_attention_workspace_bytes(_cache(), 6, 4, 0))
-    assert need > 0 and rlk_lib.rlk_paged_attention_workspace_bytes(_cache(), 6, 4, 3) == 0
-    assert rlk_lib.rlk_paged_attention_workspace_bytes(_cache(), 6, 4, 0x103) > 0
+    need = int(rlk_lib.rlk_paged_attention_workspace_bytes(_cache(), 6, 4, 0, 0x101))
+    assert need > 0 and rlk_lib.rlk_paged_attention_workspace_bytes(_cache(), 6, 4, 0, 3) == 0
+    assert rlk_lib.rlk_paged_attention_workspace_bytes(_cache(), 6, 4, 0, 0x103) > 0
+    assert rlk_lib.rlk_paged_attention_workspace_bytes(_cache(), 6, 4, -1, 0) == 0
     for kwargs, words in (
         ({"cache": _cache(dtype=2)}, "bf16 nor fp16"), ({"cache": _cache(width=60)}, "multiple of 8"), ({"cache": _cache(width=264)}, "multiple of 8"),
         ({"cache": _cache(sequences=0)}, "without a sequence"), ({"cache": _cache(keys=AT + 8)}, "16 bytes"), ({"cache": _cache(value_head_stride=4)}, "16 bytes"),
         ({"cache": _cache(key_page_stride=68)}, "16 bytes"), ({"q": AT + 2}, "16 bytes"), ({"strides": (255, 64)}, "16 bytes"), ({"out": AT + 8}, "16 bytes"),
         ({"out_strides": (256, 4)}, "16 bytes"), ({"q": None}, "null"), ({"out": None}, "null"), ({"strides": (-256, 64)}, "negative"), ({"heads": 3}, "heads"),
         ({"heads": 0}, "heads"), ({"scale": 0.0}, "scale"), ({"scale": -1.0}, "scale"), ({"scale": math.nan}, "scale"), ({"scale": math.inf}, "scale"),
-        ({"window": -1}, "window"), ({"window": 5, "causal": 0}, "window"), ({"config": 4}, "configuration"), ({"config": 0x101}, "configuration"),
-        ({"config": 0x203}, "configuration"), ({"config": 0x100}, "configuration"), ({"workspace": None}, "workspace"), ({"workspace": AT + 8}, "workspace"),
-        ({"size": need - 1}, "workspace"), ({"tokens": 2**30}, "range"), ({"tokens": -1}, "range"), ({"cache": _cache(lengths=None)}, "null"),
+        ({"window": -1}, "window"), ({"window": 5, "causal": 0}, "window"), ({"config": 4}, "configuration"), ({"config": 0x104}, "configuration"),
+        ({"config": 0x203}, "configuration"), ({"config": 0x100}, "configuration"), ({"config": 0x101, "workspace": None}, "workspace"), ({"config": 0x101, "workspace": AT + 8}, "workspace"),
+        ({"config": 0x101, "size": need - 1}, "workspace"), ({"tokens": 2**30}, "range"), ({"tokens": -1}, "range"), ({"cache": _cache(lengths=None)}, "null"),
     ):  # fmt: skip
         _refused(rlk_lib, call(**kwargs), words)
     assert call(tokens=0, q=None, out=None, workspace=None) == 0

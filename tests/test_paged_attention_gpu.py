@@ -7,10 +7,11 @@ import pytest
 import torch
 
 from attention_cases import DEV, Batch, same_bits
+from rl_engine import _lib
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
-CONFIGS = ("rows32", "rows128", "rows256", "rows128_split", "rows256_split")
+CONFIGS = tuple(name for name in _lib.ATTENTION_CONFIGS if name != "auto")
 
 
 @pytest.fixture(scope="module")
