@@ -1,11 +1,13 @@
 // The host side of the smallest calls in C++: checks, allocations and launches of an everyday inference projection, the packed
-// FFN, the differentiable linear layer and the GRPO loss, on top of the C entry points of librlk_gfx950.so.
+// FFN, the differentiable linear layer, the GRPO loss, rotary positions and the paged cache, on top of the C entry points of
+// librlk_gfx950.so.
 //
 // Small calls are bound by their host time. In Python / here, us a call: a projection 13.9 / 5.2 (5 were the dispatch of the
 // torch.library operator around it), the packed FFN 28.7 / 11.0, a linear layer with both gradients 40.6 / 27.0, the FFN with all
 // its gradients 116 / 58, the GRPO loss with its gradient 59.7 / 33.5, beside kernels of 2 to 12 each; 87 / 50, 197 / 99 and 114 / 59
 // in the stretches in which autograd's device thread has to be woken for every backward; in those, the SwiGLU of eight-bit copies with
 // its gradients 132 / 59 and scores of hidden states with theirs 189 / 97.
+// A new token's rotation 23.2 / 6.2, appending to a paged cache 27.1 / 6.0, attention over 1025 positions 26.4 / 16.5 (there its kernels).
 //
 // Every function takes everyday arguments only and answers None to anything else - other types, layouts and devices, subclasses,
 // batched and functorch tensors, tangents, dispatch and function modes (torch.set_default_device() is one), tracing, profilers -, for
@@ -66,6 +68,10 @@ decltype(&rlk_block_norm_backward) norm_bwd_entry = nullptr;
 decltype(&rlk_mx8_encode) mx8_encode_entry = nullptr;
 decltype(&rlk_mx8_swiglu_forward) mx8_swiglu_entry = nullptr;
 decltype(&rlk_mx8_swiglu_backward) mx8_swiglu_bwd_entry = nullptr;
+decltype(&rlk_rotary_embedding) rotary_entry = nullptr;
+decltype(&rlk_paged_append) append_entry = nullptr;
+decltype(&rlk_paged_attention_workspace_bytes) attention_workspace_entry = nullptr;
+decltype(&rlk_paged_attention) attention_entry = nullptr;
 decltype(&rlk_last_error) last_error_entry = nullptr;
 PyObject* general_linear_gradients = nullptr;  // (a, weight, grad, need_a, need_weight) -> (da, dw)
 PyObject* general_ffn_gradients = nullptr;     // (x, gate, up, activated, three weights, grad, need of x and the weights) -> four
@@ -73,6 +79,7 @@ PyObject* general_scores_gradient = nullptr;   // (logits, target, temperature, 
 PyObject* general_linear_scores = nullptr;     // (hidden, weight, target, temperature, lse, entropy, top ids, logits, real, four gradients, two needs) -> two
 PyObject* general_norm_gradients = nullptr;    // (block, residual, gate, two weights, rstd, kind, eps, scale, two gradients, five needs) -> five
 PyObject* general_swiglu_gradients = nullptr;  // (dy, codes and scales of gate and up) -> (d_gate, d_up)
+PyObject* general_rotary_gradients = nullptr;  // (two gradients, positions, frequencies, interleaved, magnitude, inverse) -> two
 PyObject* general_grpo_gradient = nullptr;     // (cur, old, ref, adv, mask, g_loss, g_policy, g_kl, clip_eps, beta) -> grad
 
 // What _lib.check() raises.
@@ -788,6 +795,140 @@ struct Mx8SwigluFn : torch::autograd::Function<Mx8SwigluFn> {
 };
 
 // ---------------------------------------------------------------------------
+// Rotary positions and the paged cache: the everyday calls of backends/rocm/attention
+// ---------------------------------------------------------------------------
+
+// [tokens, heads, width] or [outer, tokens, heads, width] with whole heads.
+bool everyday_heads(const Tensor& t) {
+  return t.dim() >= 3 && t.dim() <= 4 && t.numel() > 0 && (t.stride(-1) == 1 || t.size(-1) == 1) && t.size(-1) <= RLK_ROTARY_MAX_WIDTH && t.size(-2) <= INT_MAX;
+}
+rlk_head_rows head_rows(const Tensor& x, const Tensor& y) {
+  rlk_head_rows r{};
+  r.x = x.data_ptr();
+  r.x_outer_stride = x.dim() == 4 ? x.stride(0) : 0, r.x_token_stride = x.stride(-3), r.x_head_stride = x.stride(-2);
+  if (y.defined()) {
+    r.y = y.data_ptr();
+    r.y_outer_stride = y.dim() == 4 ? y.stride(0) : 0, r.y_token_stride = y.stride(-3), r.y_head_stride = y.stride(-2);
+  }
+  r.heads = (int)x.size(-2);
+  return r;
+}
+bool everyday_frequencies(const Tensor& f, const Tensor& beside) {
+  return everyday(f, at::kDouble, beside) && f.dim() == 1 && f.is_contiguous() && 2 * f.size(0) <= beside.size(-1);
+}
+bool everyday_positions(const Tensor& p, const Tensor& beside, at::IntArrayRef shape) {
+  return p.defined() && (p.scalar_type() == at::kInt || p.scalar_type() == at::kLong) && everyday(p, p.scalar_type(), beside) && p.sizes() == shape &&
+         p.is_contiguous();
+}
+rlk_rotary rotary_of(const Tensor& frequencies, const Tensor& positions, bool interleaved, double magnitude) {
+  rlk_rotary r{};
+  r.frequencies = static_cast<const double*>(frequencies.data_ptr());
+  r.positions = address(positions);
+  r.positions_are_64 = positions.defined() && positions.scalar_type() == at::kLong;
+  r.pairs = (int)frequencies.size(0);
+  r.interleaved = interleaved;
+  r.magnitude = (float)magnitude;
+  return r;
+}
+
+struct RotaryInputs {
+  Tensor q, k, positions, frequencies;  // (k may be missing)
+  bool interleaved;
+  double magnitude;
+
+  bool usual() const {
+    if (!everyday_floats(q) || !everyday_heads(q)) return false;
+    const at::IntArrayRef tokens = q.sizes().slice(0, q.dim() - 2);
+    if (k.defined() && !(everyday(k, q.scalar_type(), q) && everyday_heads(k) && k.dim() == q.dim() && k.sizes().slice(0, k.dim() - 2) == tokens && k.size(-1) == q.size(-1)))
+      return false;
+    return everyday_positions(positions, q, tokens) && everyday_frequencies(frequencies, q);
+  }
+};
+
+variable_list rotate(const RotaryInputs& in, bool inverse) {
+  const Tensor q = empty(in.q.sizes(), in.q.scalar_type(), in.q), k = in.k.defined() ? empty(in.k.sizes(), in.k.scalar_type(), in.q) : Tensor();
+  const rlk_rotary rotary = rotary_of(in.frequencies, in.positions, in.interleaved, in.magnitude);
+  const rlk_head_rows rows_q = head_rows(in.q, q), rows_k = in.k.defined() ? head_rows(in.k, k) : rlk_head_rows{};
+  const int64_t tokens = in.positions.numel();
+  check_status(rotary_entry(&rotary, &rows_q, in.k.defined() ? &rows_k : nullptr, tokens, in.q.dim() == 4 ? in.q.size(1) : tokens, (int)in.q.size(-1),
+                            dtype_code(in.q), inverse, stream_of(in.q)),
+               "rlk_rotary_embedding failed");
+  return {q, k};
+}
+
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k, const RotaryInputs* in) {
+    variable_list out = rotate(*in, false);
+    ctx->save_for_backward({in->positions, in->frequencies});
+    ctx->saved_data["interleaved"] = in->interleaved;
+    ctx->saved_data["magnitude"] = in->magnitude;
+    ctx->set_materialize_grads(false);
+    if (!k.has_value()) out.pop_back();
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    grads.resize(2);
+    if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
+    const variable_list s = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), swap = !grads[0].defined();
+    const double magnitude = ctx->saved_data["magnitude"].toDouble();
+    const RotaryInputs in{grads[swap], swap ? Tensor() : grads[1], s[0], s[1], interleaved, magnitude};
+    if (!at::GradMode::is_enabled() && everyday_thread() && !leaves_capture() && in.usual()) {
+      const c10::OptionalDeviceGuard guard(in.q.device());
+      variable_list out = rotate(in, true);
+      if (swap) std::swap(out[0], out[1]);
+      return {out[0], out[1], Tensor()};
+    }
+    const pybind11::gil_scoped_acquire gil;
+    const PyRef g_q(wrap(grads[0])), g_k(wrap(grads[1])), positions(wrap(s[0])), frequencies(wrap(s[1])), by(PyFloat_FromDouble(magnitude));
+    const PyRef two(PyObject_CallFunctionObjArgs(general_rotary_gradients, g_q.get(), g_k.get(), positions.get(), frequencies.get(),
+                                                 interleaved ? Py_True : Py_False, by.get(), nullptr));
+    const variable_list out = tensors_of(two, 2);
+    return {out[0], out[1], Tensor()};
+  }
+};
+
+struct CacheInputs {
+  Tensor keys, values, table, lengths, starts;
+
+  bool usual(const Tensor& beside) const {
+    if (!everyday_floats(keys, beside) || keys.dim() != 4 || keys.scalar_type() != beside.scalar_type() || !everyday(values, keys.scalar_type(), keys) ||
+        values.sizes() != keys.sizes() || keys.numel() == 0)
+      return false;
+    for (const Tensor* t : {&keys, &values})
+      if (t->stride(3) != 1) return false;
+    for (int i = 1; i < 4; ++i)
+      if (keys.size(i) > INT_MAX) return false;
+    for (const Tensor* t : {&table, &lengths, &starts})
+      if (!everyday(*t, at::kInt, keys)) return false;
+    return table.dim() == 2 && table.stride(1) == 1 && table.size(0) > 0 && table.size(0) < INT_MAX && table.size(1) > 0 && table.size(1) <= INT_MAX &&
+           lengths.dim() == 1 && lengths.is_contiguous() && lengths.size(0) == table.size(0) && starts.dim() == 1 && starts.is_contiguous() &&
+           starts.size(0) == table.size(0) + 1;
+  }
+  bool wants_gradient() const { return keys.requires_grad() || values.requires_grad(); }
+  rlk_paged_cache describe() const {
+    rlk_paged_cache c{};
+    c.keys = keys.data_ptr();
+    c.values = values.data_ptr();
+    c.table = static_cast<const int32_t*>(table.data_ptr());
+    c.lengths = static_cast<const int32_t*>(lengths.data_ptr());
+    c.starts = static_cast<const int32_t*>(starts.data_ptr());
+    c.key_page_stride = keys.stride(0), c.key_row_stride = keys.stride(1), c.key_head_stride = keys.stride(2);
+    c.value_page_stride = values.stride(0), c.value_row_stride = values.stride(1), c.value_head_stride = values.stride(2);
+    c.table_row_stride = table.stride(0);
+    c.pages = keys.size(0);
+    c.page_size = (int)keys.size(1), c.key_heads = (int)keys.size(2), c.width = (int)keys.size(3);
+    c.dtype = dtype_code(keys);
+    c.sequences = (int)table.size(0), c.table_columns = (int)table.size(1);
+    return c;
+  }
+};
+bool everyday_tokens(const Tensor& t, const CacheInputs& cache) {
+  return everyday(t, cache.keys.scalar_type(), cache.keys) && t.dim() == 3 && t.numel() > 0 && t.stride(2) == 1 && t.size(2) == cache.keys.size(3) && t.size(1) <= INT_MAX;
+}
+
+// ---------------------------------------------------------------------------
 // The Python module
 // ---------------------------------------------------------------------------
 
@@ -1042,12 +1183,132 @@ PyObject* py_mx8_encode(PyObject*, PyObject* const* args, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
+bool number_of(PyObject* o, double* value) {
+  if (!PyFloat_CheckExact(o)) return false;
+  *value = PyFloat_AS_DOUBLE(o);
+  return true;
+}
+bool flag_of(PyObject* o, bool* value) {
+  *value = o == Py_True;
+  return o == Py_True || o == Py_False;
+}
+bool cache_of(PyObject* const* args, CacheInputs* cache) {
+  return tensor_or_nothing(args[0], &cache->keys) && tensor_or_nothing(args[1], &cache->values) && tensor_or_nothing(args[2], &cache->table) &&
+         tensor_or_nothing(args[3], &cache->lengths) && tensor_or_nothing(args[4], &cache->starts);
+}
+
+// rotary(q, k or None, positions, frequencies, interleaved, magnitude) -> (q, k or None) turned, or None
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  RotaryInputs in;
+  if (count != 6 || rotary_entry == nullptr || !tensor_or_nothing(args[0], &in.q) || !tensor_or_nothing(args[1], &in.k) ||
+      !tensor_or_nothing(args[2], &in.positions) || !tensor_or_nothing(args[3], &in.frequencies) || !flag_of(args[4], &in.interleaved) ||
+      !number_of(args[5], &in.magnitude) || !everyday_caller() || !in.usual())
+    return none();
+  variable_list out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const c10::OptionalDeviceGuard guard(in.q.device());
+    if (at::GradMode::is_enabled() && (in.q.requires_grad() || (in.k.defined() && in.k.requires_grad())))
+      out = RotaryFn::apply(in.q, in.k.defined() ? std::optional<Tensor>(in.k) : std::nullopt, &in);
+    else
+      out = rotate(in, false);
+  }
+  out.resize(2);
+  const PyRef q(wrap(out[0])), k(wrap(out[1]));
+  return PyTuple_Pack(2, q.get(), k.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_append(k, v, keys, values, table, lengths, starts, frequencies or None, q or None, positions or None, interleaved, magnitude)
+// -> (q turned or None), or None
+PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  Tensor k, v, frequencies, q, positions;
+  CacheInputs cache;
+  bool interleaved;
+  double magnitude;
+  if (count != 12 || append_entry == nullptr || !tensor_or_nothing(args[0], &k) || !tensor_or_nothing(args[1], &v) || !cache_of(args + 2, &cache) ||
+      !tensor_or_nothing(args[7], &frequencies) || !tensor_or_nothing(args[8], &q) || !tensor_or_nothing(args[9], &positions) ||
+      !flag_of(args[10], &interleaved) || !number_of(args[11], &magnitude) || !everyday_caller() || !everyday_floats(k) || !cache.usual(k))
+    return none();
+  if (!everyday_tokens(k, cache) || !everyday_tokens(v, cache) || k.size(1) != cache.keys.size(2) || v.sizes() != k.sizes() || k.size(2) > RLK_ROTARY_MAX_WIDTH)
+    return none();
+  if (q.defined() && !(everyday_tokens(q, cache) && q.size(0) == k.size(0))) return none();
+  if (frequencies.defined() ? !everyday_frequencies(frequencies, k) || (positions.defined() && !everyday_positions(positions, k, k.sizes().slice(0, 1)))
+                            : positions.defined())
+    return none();
+  if (at::GradMode::is_enabled() && (k.requires_grad() || v.requires_grad() || (q.defined() && q.requires_grad()) || cache.wants_gradient())) return none();
+  Tensor turned;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const c10::OptionalDeviceGuard guard(k.device());
+    if (q.defined()) turned = empty(q.sizes(), q.scalar_type(), q);
+    const rlk_paged_cache described = cache.describe();
+    const rlk_rotary rotary = frequencies.defined() ? rotary_of(frequencies, positions, interleaved, magnitude) : rlk_rotary{};
+    const rlk_head_rows rows_q = q.defined() ? head_rows(q, turned) : rlk_head_rows{}, rows_k = head_rows(k, Tensor()), rows_v = head_rows(v, Tensor());
+    check_status(append_entry(&described, frequencies.defined() ? &rotary : nullptr, q.defined() ? &rows_q : nullptr, &rows_k, &rows_v, k.size(0), stream_of(k)),
+                 "rlk_paged_append failed");
+  }
+  const PyRef result(wrap(turned));
+  return PyTuple_Pack(1, result.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, keys, values, table, lengths, starts, scale or None, causal, window or None, whether the logarithms are wanted)
+// -> (out, logarithms or None), or None
+PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  Tensor q;
+  CacheInputs cache;
+  double scale = 0.0;
+  bool causal, with_lse;
+  if (count != 10 || attention_entry == nullptr || !tensor_or_nothing(args[0], &q) || !cache_of(args + 1, &cache) ||
+      (args[6] != Py_None && !number_of(args[6], &scale)) || !flag_of(args[7], &causal) || !flag_of(args[9], &with_lse) || !everyday_caller() ||
+      !everyday_floats(q) || q.scalar_type() == at::kFloat || !cache.usual(q) || !everyday_tokens(q, cache))
+    return none();
+  int window = 0;
+  if (args[8] != Py_None) {
+    if (!PyLong_CheckExact(args[8]) || !causal) return none();
+    int overflow;
+    const long n = PyLong_AsLongAndOverflow(args[8], &overflow);
+    if (overflow != 0 || n < 1 || n > INT_MAX) return none();
+    window = (int)n;
+  }
+  const int64_t width = q.size(2), heads = q.size(1), key_heads = cache.keys.size(2);
+  if (args[6] == Py_None) scale = std::pow((double)width, -0.5);
+  if (!(scale > 0.0 && scale < 3e38) || width % 8 != 0 || heads % key_heads != 0) return none();
+  auto on_16_bytes = [](const Tensor& t) {
+    bool on = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) on = on && t.stride(i) % 8 == 0;
+    return on;
+  };
+  if (!on_16_bytes(q) || !on_16_bytes(cache.keys) || !on_16_bytes(cache.values)) return none();
+  if (at::GradMode::is_enabled() && (q.requires_grad() || cache.wants_gradient())) return none();
+  Tensor out, lse;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const c10::OptionalDeviceGuard guard(q.device());
+    out = empty(q.sizes(), q.scalar_type(), q);
+    if (with_lse) lse = empty({q.size(0), heads}, at::kFloat, q);
+    const rlk_paged_cache described = cache.describe();
+    const size_t bytes = attention_workspace_entry(&described, q.size(0), (int)heads, window, RLK_ATTENTION_CFG_AUTO);
+    const Tensor workspace = bytes > 0 ? empty({(int64_t)bytes}, at::kByte, q) : Tensor();
+    check_status(attention_entry(&described, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), writable(lse), q.size(0),
+                                 (int)heads, (float)scale, causal, window, 1, RLK_ATTENTION_CFG_AUTO, address(workspace), bytes, stream_of(q)),
+                 "rlk_paged_attention failed");
+  }
+  const PyRef result(wrap(out)), logarithms(wrap(lse));
+  return PyTuple_Pack(2, result.get(), logarithms.get());
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(addresses of the entry points by name, the general gradients of the linear layer, the FFN, the GRPO loss, the token scores, the
-// norm between blocks, the SwiGLU of eight-bit copies and the token scores of hidden states)
+// norm between blocks, the SwiGLU of eight-bit copies, the token scores of hidden states and rotary positions)
 PyObject* py_bind(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
-  PyObject *addresses, *linear, *ffn, *loss, *of_scores = Py_None, *of_norm = Py_None, *of_swiglu = Py_None, *of_linear_scores = Py_None;
-  if (!PyArg_ParseTuple(args, "O!OOO|OOOO", &PyDict_Type, &addresses, &linear, &ffn, &loss, &of_scores, &of_norm, &of_swiglu, &of_linear_scores)) return nullptr;
+  PyObject *addresses, *linear, *ffn, *loss, *of_scores = Py_None, *of_norm = Py_None, *of_swiglu = Py_None, *of_linear_scores = Py_None, *of_rotary = Py_None;
+  if (!PyArg_ParseTuple(args, "O!OOO|OOOOO", &PyDict_Type, &addresses, &linear, &ffn, &loss, &of_scores, &of_norm, &of_swiglu, &of_linear_scores, &of_rotary)) return nullptr;
   auto entry = [&](const char* name, auto& to) {
     PyObject* const at = PyDict_GetItemString(addresses, name);
     void* const address = at != nullptr ? PyLong_AsVoidPtr(at) : nullptr;
@@ -1073,7 +1334,8 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   for (const auto& [from, to] : {std::pair<PyObject*, PyObject**>{of_scores, &general_scores_gradient},
                                  {of_norm, &general_norm_gradients},
                                  {of_swiglu, &general_swiglu_gradients},
-                                 {of_linear_scores, &general_linear_scores}}) {
+                                 {of_linear_scores, &general_linear_scores},
+                                 {of_rotary, &general_rotary_gradients}}) {
     Py_INCREF(from);
     Py_XSETREF(*to, from);
   }
@@ -1081,6 +1343,10 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   entry("rlk_linear_dlogits_row_stride", dlogits_stride_entry);
   entry("rlk_linear_dlogits_bwd", dlogits_bwd_entry);
   entry("rlk_logits_scores", scores_entry);
+  entry("rlk_rotary_embedding", rotary_entry);
+  entry("rlk_paged_append", append_entry);
+  entry("rlk_paged_attention_workspace_bytes", attention_workspace_entry);
+  entry("rlk_paged_attention", attention_entry);
   entry("rlk_linear_scores_fwd", linear_scores_entry);
   entry("rlk_block_norm_forward", norm_entry);
   entry("rlk_mx8_swiglu_forward", mx8_swiglu_entry);
@@ -1104,6 +1370,9 @@ PyMethodDef methods[] = {
     {"reaches_default_stream", py_reaches_default_stream, METH_NOARGS, nullptr},
     {"linear_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_scores)), METH_FASTCALL, nullptr},
     {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rotary)), METH_FASTCALL, nullptr},
+    {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_attention)), METH_FASTCALL, nullptr},
     {"mx8_swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx8_swiglu)), METH_FASTCALL, nullptr},
     {"mx8_encode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx8_encode)), METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_VARARGS, nullptr},

@@ -14,6 +14,7 @@ _ENTRIES = (
     "rlk_logits_scores_workspace_bytes", "rlk_logits_scores", "rlk_logits_scores_backward", "rlk_block_norm_forward",
     "rlk_block_norm_workspace_bytes", "rlk_block_norm_backward", "rlk_linear_scores_workspace_bytes", "rlk_linear_scores_fwd",
     "rlk_linear_dlogits_row_stride", "rlk_linear_dlogits_bwd", "rlk_mx8_encode", "rlk_mx8_swiglu_forward", "rlk_mx8_swiglu_backward",
+    "rlk_rotary_embedding", "rlk_paged_append", "rlk_paged_attention_workspace_bytes", "rlk_paged_attention",
 )  # fmt: skip
 _native = None
 
@@ -29,6 +30,7 @@ def native():
             raise _lib.RlkLibraryMissing(
                 f"rl_engine/_torch_host.so could not be loaded ({missing}): build it with `python rl-kernel_amd/build.py`"
             ) from missing
+        from rl_engine.backends.rocm.attention.rotary import rotary_gradients
         from rl_engine.backends.rocm.ffn.ffn import ffn_gradients, kept_swiglu_gradients
         from rl_engine.backends.rocm.gemm.det_gemm import linear_gradients
         from rl_engine.backends.rocm.logprob.token_scores import linear_scores_gradients, scores_gradient
@@ -38,7 +40,7 @@ def native():
         addresses = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ENTRIES}
         _torch_host.bind(
             addresses, linear_gradients, ffn_gradients, _elementwise_gradient, scores_gradient, norm_gradients, kept_swiglu_gradients,
-            linear_scores_gradients,
+            linear_scores_gradients, rotary_gradients,
         )  # fmt: skip
         _native = _torch_host
     return _native

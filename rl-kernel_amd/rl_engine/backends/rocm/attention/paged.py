@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from rl_engine import _lib
+from rl_engine import _host, _lib
 from rl_engine._C import _on, _stream_handle
 from rl_engine._checks import enforce, refuse_tangents
 from rl_engine.backends.rocm.attention.rotary import _DTYPES, check_frequencies, check_positions, rotary_of
@@ -126,6 +126,12 @@ def paged_append(
     written belong to one sequence (others may share the pages in front of them). The cache is not differentiable: arguments that require
     a gradient are refused.
     """
+    if isinstance(k, Tensor) and k.is_cuda and not torch.compiler.is_compiling():
+        done = _host.native().paged_append(  # everyday arguments, natively
+            k, v, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, q, positions, interleaved, magnitude
+        )
+        if done is not None:
+            return done[0]
     _inference_only("paged_append", k, v, q, key_cache, value_cache)
     cache = _Cache(key_cache, value_cache, page_table, context_lengths, query_starts)
     heads, width, device = key_cache.size(2), key_cache.size(3), key_cache.device
@@ -191,6 +197,12 @@ def paged_attention(
     kernel that runs and never changes them. A call is sized by the width of ``page_table``: pass ``page_table[:, :n]`` where the longest
     context is known. No gradient: tensors that require one are refused.
     """
+    if out is None and config == "auto" and isinstance(q, Tensor) and q.is_cuda and not torch.compiler.is_compiling():
+        both = _host.native().paged_attention(  # everyday arguments, natively
+            q, key_cache, value_cache, page_table, context_lengths, query_starts, scale, causal, window, return_lse
+        )
+        if both is not None:
+            return both if return_lse else both[0]
     _inference_only("paged_attention", q, key_cache, value_cache, out)
     cache = _Cache(key_cache, value_cache, page_table, context_lengths, query_starts)
     key_heads, width, device = key_cache.size(2), key_cache.size(3), key_cache.device

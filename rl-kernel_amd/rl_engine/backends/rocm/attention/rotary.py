@@ -129,13 +129,20 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_q, g_k):
-        refuse_tangents("the gradient of a rotation", g_q, g_k)
-        _host.refuse_capture_into_another_graph()
-        given = [g for g in (g_q, g_k) if g is not None]
-        if not given:
-            return (None,) * 7
-        turned = iter(_Rotary.apply(given[0], given[1] if len(given) > 1 else None, *ctx.saved_tensors, *ctx.how, not ctx.inverse))
-        return *(None if g is None else next(turned) for g in (g_q, g_k)), None, None, None, None, None
+        return *rotary_gradients(g_q, g_k, *ctx.saved_tensors, *ctx.how, not ctx.inverse), None, None, None, None, None
+
+
+def rotary_gradients(
+    g_q: Optional[Tensor], g_k: Optional[Tensor], positions: Tensor, frequencies: Tensor, interleaved: bool, magnitude: float, inverse: bool = True
+) -> tuple[Optional[Tensor], Optional[Tensor]]:
+    """The gradients of ``q`` and ``k`` from those of their turned forms, differentiable; ``None`` where there is none."""
+    refuse_tangents("the gradient of a rotation", g_q, g_k)
+    _host.refuse_capture_into_another_graph()
+    given = [g for g in (g_q, g_k) if g is not None]
+    if not given:
+        return None, None
+    turned = iter(_Rotary.apply(given[0], given[1] if len(given) > 1 else None, positions, frequencies, interleaved, magnitude, inverse))
+    return tuple(None if g is None else next(turned) for g in (g_q, g_k))
 
 
 def check_frequencies(frequencies: Tensor, device: torch.device, width: int) -> Tensor:
@@ -181,6 +188,10 @@ def rotary_embedding(
 
     Angles are reduced to a turn in 64 bits, so that far positions lose nothing; the rest is fp32, rounded once.
     """
+    if isinstance(q, Tensor) and q.is_cuda and not torch.compiler.is_compiling():
+        both = _host.native().rotary(q, k, positions, frequencies, interleaved, magnitude)  # everyday arguments, natively
+        if both is not None:
+            return both
     refuse_tangents("rotary_embedding", q, k)
     _check_heads(q, "q")
     if k is not None:

@@ -127,7 +127,7 @@ def test_gradients_against_differences_and_of_gradients(attention):
         d[at] = step
         with torch.no_grad():
             slope = (loss(q + d) - loss(q - d)) / (2 * step)
-        assert abs(float(slope - grad[at])) <= 100 * 8 * 2.0**-23 / step
+        assert abs(float(slope.detach() - grad[at])) <= 100 * 8 * 2.0**-23 / step
     (second,) = torch.autograd.grad(grad.sum(), q)  # 2 R^T diag(w) R 1
     ones = torch.ones_like(q)
     turned = attention.rotary_embedding(ones, None, positions, f, magnitude=1.5)[0].double()
