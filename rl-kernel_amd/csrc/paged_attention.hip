@@ -167,10 +167,11 @@ __host__ __device__ __forceinline__ int capacity_of(const rlk_paged_cache& c) {
 }
 __device__ __forceinline__ int capacity_of(const AttentionArgs& a) { return capacity_of(a.cache); }
 
-// Where row tiles lie: sequence s has those from floor(starts[s] * group / rows) + s on, at least as many as it needs.
+// Row tiles: the first one of every sequence (a workgroup knows it without a search, and of sequences of single tokens there are no others), then
+// the others, of sequence s at floor(starts[s] * group / rows) and behind, at least as many as it needs.
 template <int ROWS>
-__device__ __forceinline__ int64_t first_row_tile(const AttentionArgs& a, int s) {
-  return (int64_t)clamp_to(a.cache.starts[s], 0, a.tokens) * a.group / ROWS + s;
+__device__ __forceinline__ int64_t other_row_tiles(const AttentionArgs& a, int s) {
+  return (int64_t)clamp_to(a.cache.starts[s], 0, a.tokens) * a.group / ROWS;
 }
 
 // The running state of 32 rows of a wave. Lane l holds row l & 31; of the output, register i of block d is element
@@ -444,33 +445,39 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   int* const special_tile = reinterpret_cast<int*>(lds + 4 * kTileBytes + WAVES * kShelfBytes);  // [2]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
-  // Heads change fastest, so that an XCD's workgroups read few of them; the tiles with the most keys come first.
+  // Heads change fastest, so that an XCD's workgroups read few of them; of a sequence's other tiles those with the most keys come first.
   const uint32_t id = blockIdx.x;
   const uint32_t outer = divide_by(id, a.by_key_heads);
   const int key_head = (int)(id - outer * a.cache.key_heads);
   const int chunk_id = SPLIT ? (int)(outer % (uint32_t)a.chunks) : 0;
-  const int tile_id = a.tiles - 1 - (int)(SPLIT ? outer / (uint32_t)a.chunks : outer);
-  const int s = wave_search(a.cache.sequences + 1, tile_id, lane, [&](int i) { return first_row_tile<kRows>(a, i); });
-  if (s >= a.cache.sequences) {  // behind the last sequence
-    if (!SPLIT && a.zero_rest) {
-      const int before = clamp_to(a.cache.starts[0], 0, a.tokens), behind = clamp_to(a.cache.starts[s], before, a.tokens);
-      const int tail = tile_id - (int)first_row_tile<kRows>(a, s), tails = a.tiles - (int)first_row_tile<kRows>(a, s);
-      const int each = a.cache.width / 8;
-      for (int n = tail; n < before + a.tokens - behind; n += tails) {
-        const int t = n < before ? n : behind + n - before;
-        for (int i = tid; i < a.group * each; i += WAVES * 64) {
-          const int head = key_head * a.group + i / each;
-          *reinterpret_cast<u32x4_t*>(a.out + t * a.out_token_stride + head * a.out_head_stride + (i % each) * 16) = u32x4_t{0, 0, 0, 0};
-          if (a.lse && i % each == 0) a.lse[(int64_t)t * a.heads + head] = -INFINITY;
+  const int tile_id = (int)(SPLIT ? outer / (uint32_t)a.chunks : outer);
+  int s = tile_id, row0 = 0;
+  if (tile_id >= a.cache.sequences) {
+    const int others = a.tiles - a.cache.sequences, i = tile_id - a.cache.sequences;
+    const int other = i + 1 < others ? others - 2 - i : others - 1;  // (that one is hardly ever needed)
+    s = wave_search(a.cache.sequences + 1, other, lane, [&](int i) { return other_row_tiles<kRows>(a, i); });
+    if (s < 0) return;
+    const int first = (int)other_row_tiles<kRows>(a, s);
+    if (s >= a.cache.sequences) {  // behind the last sequence
+      if (!SPLIT && a.zero_rest) {
+        const int before = clamp_to(a.cache.starts[0], 0, a.tokens), behind = clamp_to(a.cache.starts[s], before, a.tokens);
+        const int tails = others - first;
+        const int each = a.cache.width / 8;
+        for (int n = other - first; n < before + a.tokens - behind; n += tails) {
+          const int t = n < before ? n : behind + n - before;
+          for (int i = tid; i < a.group * each; i += WAVES * 64) {
+            const int head = key_head * a.group + i / each;
+            *reinterpret_cast<u32x4_t*>(a.out + t * a.out_token_stride + head * a.out_head_stride + (i % each) * 16) = u32x4_t{0, 0, 0, 0};
+            if (a.lse && i % each == 0) a.lse[(int64_t)t * a.heads + head] = -INFINITY;
+          }
         }
       }
+      return;
     }
-    return;
+    row0 = (1 + other - first) * kRows;
   }
-  if (s < 0) return;
   const Chunk c = chunk_of(a, s);
   const int rows = c.tokens * a.group;
-  const int row0 = (int)(tile_id - first_row_tile<kRows>(a, s)) * kRows;
   if (row0 >= rows) return;
 
   // What this workgroup's and this wave's rows see.
