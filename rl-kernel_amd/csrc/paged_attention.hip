@@ -58,7 +58,7 @@ struct AttentionArgs {
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
   int64_t part_rows;  // tokens * heads
   PageDivider by_page, by_group, by_key_heads;
-  int tokens, heads, group, causal, window, zero_rest, tiles, chunks;
+  int tokens, heads, group, causal, window, zero_rest, longest_first, tiles, chunks;
   float scale;  // times log2(e)
 };
 
@@ -452,6 +452,16 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   const int chunk_id = SPLIT ? (int)(outer % (uint32_t)a.chunks) : 0;
   const int tile_id = (int)(SPLIT ? outer / (uint32_t)a.chunks : outer);
   int s = tile_id, row0 = 0;
+  if (tile_id < a.cache.sequences && a.longest_first) {  // of 64 sequences: this one's place is its length's
+    const int first = tile_id & ~63, count = min(64, a.cache.sequences - first);
+    const int mine = lane < count ? a.cache.lengths[first + lane] : 0;
+    int rank = 0;
+    for (int i = 0; i < count; ++i) {
+      const int other = __builtin_amdgcn_readlane(mine, i);
+      rank += other > mine || (other == mine && i < lane);
+    }
+    s = first + __ffsll(__ballot(lane < count && rank == (tile_id & 63))) - 1;
+  }
   if (tile_id >= a.cache.sequences) {
     const int others = a.tiles - a.cache.sequences, i = tile_id - a.cache.sequences;
     const int other = i + 1 < others ? others - 2 - i : others - 1;  // (that one is hardly ever needed)
@@ -894,6 +904,7 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
 struct AttentionPlan {
   int rows;    // of a tile
   bool split;  // runs side by side
+  bool longest_first;  // of the sequences
   int chunks, tiles;
 };
 
@@ -931,9 +942,10 @@ static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, in
   p.tiles = (int)(tokens * group / p.rows) + c.sequences + 1;
   p.chunks = 1;
   if (p.split) {
-    const int64_t units = side_by_side(p.rows), wanted = ((p.rows == 64 ? 8 : 2) * cus + units - 1) / units, of_runs = depth / 4 + 1 < runs ? depth / 4 + 1 : runs;
+    const int64_t units = side_by_side(p.rows), wanted = ((p.rows == 64 ? 4 : 2) * cus + units - 1) / units, of_runs = depth / 4 + 1 < runs ? depth / 4 + 1 : runs;
     p.chunks = (int)(wanted < of_runs ? wanted : of_runs);
   }
+  p.longest_first = c.sequences > 1 && side_by_side(p.rows) * p.chunks > (p.rows == 64 ? 2 : 1) * cus;
   return p;
 }
 
@@ -1002,7 +1014,7 @@ hipError_t paged_attention_launch(const rlk_paged_cache& cache, const void* q, i
   a.tokens = (int)tokens;
   a.heads = heads;
   a.causal = causal, a.window = window, a.zero_rest = zero_rest;
-  a.tiles = p.tiles, a.chunks = p.chunks;
+  a.tiles = p.tiles, a.chunks = p.chunks, a.longest_first = p.longest_first;
   a.scale = (float)((double)scale * 1.4426950408889634074);
   return cache.dtype == RLK_DTYPE_BF16 ? attention_launch_as<RLK_DTYPE_BF16>(a, p, stream) : attention_launch_as<RLK_DTYPE_FP16>(a, p, stream);
 }
