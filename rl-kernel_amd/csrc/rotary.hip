@@ -6,15 +6,16 @@
 // rounded to fp32 for the sine and cosine.
 //
 // HBM-bound: every element is read once and written once. A token's sines and cosines are the same for all its heads: a
-// workgroup computes those of its tokens once into LDS (one 64-bit product and one sincospi for a thread at 4 tokens of 64 pairs)
-// and then goes through their heads a 16-byte piece of a thread at a time (both halves of eight pairs where they lie apart). Four tokens a workgroup,
-// one where that leaves CUs without work.
+// workgroup has one token, computes them once into LDS (one 64-bit product and one sincospi for each pair) and then goes through the
+// heads, a 16-byte piece of a thread at a time (both halves of eight pairs where they lie apart). Four tokens a workgroup computed the
+// same in fewer, longer workgroups: 8192 tokens of 40 heads of 128 with their gradient 70 us, with one each 66 (5.1 TB/s, above a
+// large copy's 4.9); 4095 tokens into a paged cache 36 and 28.5 (3.5 TB/s: its sequence, page and place are three loads one after the other
+// before the first store).
 #include "paged.h"
 
 namespace rlk {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryTokens = 4;
 
 template <int ELEM>
 struct RotaryElem;
@@ -64,7 +65,7 @@ struct RotaryArgs {
   float sign;
 };
 
-// What a workgroup knows of a token.
+// What a workgroup knows of its token.
 struct TokenPlace {
   int64_t key_base, value_base;  // of its cache row, -1 where it has none
   int64_t position;
@@ -72,49 +73,40 @@ struct TokenPlace {
 };
 
 template <int ELEM, bool WHOLE, bool APPEND>
-__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a, const int tokens_each) {
+__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
   typedef RotaryElem<ELEM> E;
   typedef typename E::type T;
-  extern __shared__ float2 turn[];  // [tokens_each][pairs] cosine and sine, scaled
-  __shared__ TokenPlace place[kRotaryTokens];
+  extern __shared__ float2 turn[];  // [pairs] cosine and sine, scaled
   const int tid = threadIdx.x, pairs = a.rotary.pairs;
-  const int64_t t0 = (int64_t)blockIdx.x * tokens_each;
-  const int tokens = a.tokens - t0 < tokens_each ? (int)(a.tokens - t0) : tokens_each;
+  const int64_t t = blockIdx.x;
 
-  if (APPEND) {
-    const int lane = tid & 63, wave = tid >> 6;
-    if (wave < tokens) {
-      const int64_t t = t0 + wave;
-      const int s = wave_search(a.cache.sequences + 1, t, lane, [&](int i) { return (int64_t)a.cache.starts[i]; });
-      TokenPlace p = {-1, -1, 0, 0};
-      if (s >= 0 && s < a.cache.sequences && t < a.cache.starts[s + 1]) {
-        p.known = 1;
-        p.position = (int64_t)a.cache.lengths[s] - a.cache.starts[s + 1] + t;
-        if (p.position >= 0 && p.position < 0x7fffffff) {
-          const uint32_t column = divide_by((uint32_t)p.position, a.by_page);
-          const int page = page_at(a.cache, s, (int)column);
-          if (page >= 0) {
-            const int64_t row = p.position - (int64_t)column * a.cache.page_size;
-            p.key_base = page * a.cache.key_page_stride + row * a.cache.key_row_stride;
-            p.value_base = page * a.cache.value_page_stride + row * a.cache.value_row_stride;
-          }
+  TokenPlace place = {-1, -1, 0, 0};
+  if (APPEND) {  // every wave for itself
+    const int s = wave_search(a.cache.sequences + 1, t, tid & 63, [&](int i) { return (int64_t)a.cache.starts[i]; });
+    if (s >= 0 && s < a.cache.sequences && t < a.cache.starts[s + 1]) {
+      place.known = 1;
+      place.position = (int64_t)a.cache.lengths[s] - a.cache.starts[s + 1] + t;
+      if (place.position >= 0 && place.position < 0x7fffffff) {
+        const uint32_t column = divide_by((uint32_t)place.position, a.by_page);
+        const int page = page_at(a.cache, s, (int)column);
+        if (page >= 0) {
+          const int64_t row = place.position - (int64_t)column * a.cache.page_size;
+          place.key_base = page * a.cache.key_page_stride + row * a.cache.key_row_stride;
+          place.value_base = page * a.cache.value_page_stride + row * a.cache.value_row_stride;
         }
       }
-      if (lane == 0) place[wave] = p;
     }
-    __syncthreads();
   }
-  for (int i = tid; i < tokens * pairs; i += kRotaryThreads) {
-    const int token = i / pairs, pair = i - token * pairs;
+  for (int i = tid; i < pairs; i += kRotaryThreads) {
     int64_t position;
     if (a.rotary.positions == nullptr)
-      position = APPEND ? place[token].position : 0;
+      position = place.position;
     else if (a.rotary.positions_are_64)
-      position = static_cast<const int64_t*>(a.rotary.positions)[t0 + token];
+      position = static_cast<const int64_t*>(a.rotary.positions)[t];
     else
-      position = static_cast<const int32_t*>(a.rotary.positions)[t0 + token];
+      position = static_cast<const int32_t*>(a.rotary.positions)[t];
     constexpr double kTurnsPerRadian = 0.15915494309189533577;
-    double turns = (double)position * (a.rotary.frequencies[pair] * kTurnsPerRadian);
+    double turns = (double)position * (a.rotary.frequencies[i] * kTurnsPerRadian);
     turns -= rint(turns);
     float s, c;
     sincospif(2.0f * (float)turns, &s, &c);
@@ -122,33 +114,30 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
   }
   __syncthreads();
 
-  const int per_token = a.heads * a.items;
-  for (int i = tid; i < tokens * per_token; i += kRotaryThreads) {
-    const int row = (int)divide_by((uint32_t)i, a.by_items);  // token of the workgroup and head
-    const int item = i - row * a.items;
-    const int token = row / a.heads, any_head = row - token * a.heads;
+  const int64_t outer = (int64_t)(a.inner == a.tokens ? 0 : divide_by((uint32_t)t, a.by_inner)), inner = t - outer * a.inner;
+  for (int i = tid; i < a.heads * a.items; i += kRotaryThreads) {
+    const int any_head = (int)divide_by((uint32_t)i, a.by_items);
+    const int item = i - any_head * a.items;
     int which = 0;
     if (a.parts > 1 && any_head >= a.part[1].first_head) which = 1;
     if (APPEND && a.parts > 2 && any_head >= a.part[2].first_head) which = 2;
     const RotaryPart& part = a.part[which];
     const int head = any_head - part.first_head;
-    const int64_t t = t0 + token;
-    const int64_t outer = (int64_t)(a.inner == a.tokens ? 0 : divide_by((uint32_t)t, a.by_inner)), inner = t - outer * a.inner;
     const T* x = static_cast<const T*>(part.rows.x) + outer * part.rows.x_outer_stride + inner * part.rows.x_token_stride + head * part.rows.x_head_stride;
     T* y;
     bool turns = pairs > 0, zero = false;
     if (!APPEND || part.target == kToRows) {
       y = static_cast<T*>(part.rows.y) + outer * part.rows.y_outer_stride + inner * part.rows.y_token_stride + head * part.rows.y_head_stride;
-      zero = APPEND && !place[token].known;
+      zero = APPEND && !place.known;
     } else if (part.target == kToKeys) {
-      if (place[token].key_base < 0) continue;
-      y = static_cast<T*>(a.cache.keys) + place[token].key_base + head * a.cache.key_head_stride;
+      if (place.key_base < 0) continue;
+      y = static_cast<T*>(a.cache.keys) + place.key_base + head * a.cache.key_head_stride;
     } else {
-      if (place[token].key_base < 0) continue;
-      y = static_cast<T*>(a.cache.values) + place[token].value_base + head * a.cache.value_head_stride;
+      if (place.key_base < 0) continue;
+      y = static_cast<T*>(a.cache.values) + place.value_base + head * a.cache.value_head_stride;
       turns = false;
     }
-    const float2* by = turn + token * pairs;
+    const float2* const by = turn;
     if (WHOLE) {
       typedef RowPiece<T> Piece;
       constexpr int kCount = Piece::kCount;
@@ -223,19 +212,18 @@ static hipError_t rotary_launch_as(RotaryArgs& a, bool append, hipStream_t strea
             whole_pieces(a.cache.values, a.cache.value_page_stride, a.cache.value_row_stride, a.cache.value_head_stride, kCount);
   a.items = whole ? (a.rotary.interleaved ? a.width : a.width - pairs) / kCount : a.width - pairs;
   a.by_items = page_divider(a.items);
-  const int each = a.tokens >= (int64_t)kRotaryTokens * device_cu_count() ? kRotaryTokens : 1;
-  const dim3 grid((unsigned)((a.tokens + each - 1) / each));
-  const size_t lds = sizeof(float2) * each * (pairs > 0 ? pairs : 1);
+  const dim3 grid((unsigned)a.tokens);
+  const size_t lds = sizeof(float2) * (pairs > 0 ? pairs : 1);
   if (append) {
     if (whole)
-      rotary_kernel<ELEM, true, true><<<grid, kRotaryThreads, lds, stream>>>(a, each);
+      rotary_kernel<ELEM, true, true><<<grid, kRotaryThreads, lds, stream>>>(a);
     else
-      rotary_kernel<ELEM, false, true><<<grid, kRotaryThreads, lds, stream>>>(a, each);
+      rotary_kernel<ELEM, false, true><<<grid, kRotaryThreads, lds, stream>>>(a);
   } else {
     if (whole)
-      rotary_kernel<ELEM, true, false><<<grid, kRotaryThreads, lds, stream>>>(a, each);
+      rotary_kernel<ELEM, true, false><<<grid, kRotaryThreads, lds, stream>>>(a);
     else
-      rotary_kernel<ELEM, false, false><<<grid, kRotaryThreads, lds, stream>>>(a, each);
+      rotary_kernel<ELEM, false, false><<<grid, kRotaryThreads, lds, stream>>>(a);
   }
   return hipGetLastError();
 }
