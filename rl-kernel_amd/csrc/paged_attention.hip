@@ -21,6 +21,12 @@
 // read as zeros. Where some rows see a value and others do not, a zero weight would not save them from infinities and NaN in
 // it: such a tile is looked through before it is used, and if it holds any they are taken out of the product and added to the
 // rows that see them.
+//
+// What bounds it. With few rows a tile's keys and values, HBM: 4 sequences of 131071 positions 411 us, 5.2 TB/s (a large copy reaches 4.9);
+// 64 of up to 8192 223 us, 4.6 TB/s. With many the two products beside the vector work of the weights (32 matrix instructions of 32
+// cycles against some 200 vector instructions, 33 of them exponentials, for 32 rows and a tile): prompts of up to 12000 tokens 2.3 ms, 0.95
+// PFLOP/s (2.1 ms on zeros, where the clock does not drop). A short call is a chain of latencies: 1025 positions of one token take 16 us, of
+// which 4 go by until the first keys are there and 2 for each of the four tiles of a run.
 #include "det_gemm_solo.h"
 #include "paged.h"
 
@@ -32,7 +38,7 @@ constexpr int kMaxWidth = 256;
 constexpr int kMostKeys = 0x7fffff00;  // of a sequence
 
 // Runs: their lengths grow with the position, so that a short context still has enough of them for the chip and a long
-// one's partial results stay few. Tiles 0 ... 63 in fours, ... 255 in eights, ... 1023 in sixteens, then 32 at a time.
+// one's partial results stay few (of 8 rows a part is 1/32 of the keys and values that a run of 256 reads, 1/256 of 2048). Tiles 0 ... 63 in fours, ... 255 in eights, ... 1023 in sixteens, then 32 at a time.
 __host__ __device__ __forceinline__ int run_of_tile(int t) {
   return t < 64 ? t >> 2 : t < 256 ? 16 + ((t - 64) >> 3) : t < 1024 ? 40 + ((t - 256) >> 4) : 88 + ((t - 1024) >> 5);
 }
@@ -416,16 +422,19 @@ __device__ __forceinline__ bool take_out_special(char* at) {
 }
 
 // ---------------------------------------------------------------------------
-// WAVES waves of 32 rows each share the keys and values of their tile through LDS, two tiles of each deep, one barrier a tile. SPLIT:
+// WAVES waves of 32 rows each (2, 4 or 8) share the keys and values of their tile through LDS, two tiles of each deep, one barrier a tile. SPLIT:
 // a workgroup takes some of the runs and leaves the parts in memory. GROUPED: eight keys that a load instruction brings lie in one page
 // (page sizes that 8 divides), so that a wave-uniform base and constant lane offsets address them, a buffer load's range makes
 // zeros of the keys that a tile does not need, and the compiler counts LDS reads one by one (beside a direct load with lane
-// addresses, which it takes for one that might have gone to LDS, it waits for all of them at every step).
+// addresses, which it takes for one that might have gone to LDS, it waits for all of them at every step: prompts of 12000 tokens
+// 2.9 ms). Other page sizes get tiles of 128 rows whatever their number, so that there are fewer kernels to build.
 //
 // In turn i a wave multiplies its queries with tile i's keys, and then tile i - 1's weights with its values; between these
 // products stands, piece by piece, what turns tile i's scores into weights, because a wave's vector instructions run beside its own
 // matrix instructions (and exponentials, 16 cycles each, are a third of the time of both products) but two waves a SIMD are too
-// few to fill one with the other's. Tile i + 1's keys and tile i's values are asked for at the start of turn i and have landed at
+// few to fill one with the other's (half a turn apart they took as long as side by side). Half of a tile's weights beside the next
+// tile's first product took longer (2.38 ms for 2.35, with one wave a SIMD 1.66 for 1.57), as did more loads ahead: four stages and waits
+// for one tile of three gave the same times with 64 rows and 1.60 ms for 1.55 with 128. Tile i + 1's keys and tile i's values are asked for at the start of turn i and have landed at
 // its end; the places they go to were last read in turn i - 1.
 // ---------------------------------------------------------------------------
 template <int DTYPE, int SLABS, int WAVES, bool SPLIT, bool GROUPED>
@@ -434,7 +443,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   typedef Rows<DTYPE, SLABS> State;
   typedef Half<DTYPE> H;
   constexpr int kRows = 32 * WAVES;
-  constexpr bool kKeepQ = SLABS > 2 || WAVES <= 2;  // queries stay in registers; else in LDS
+  constexpr bool kKeepQ = SLABS > 2 || WAVES <= 2;  // queries stay in registers; else in LDS (with four waves both took as long)
   constexpr int kGroups = 8 / WAVES;  // groups of 8 keys that a wave loads
   constexpr int kSpan = 64 / kGroups;  // tiles whose addresses the lanes of a wave have
   constexpr int kTileBytes = SLABS * kSlabBytes;
@@ -918,6 +927,14 @@ static bool pages_of_groups(const rlk_paged_cache& c) {
 }
 
 // Tiles. A call is sized by what it may need: its tokens, spread evenly over the sequences, and the table's positions (or the window's).
+// Measured, us, heads of 128, 8 key heads:
+//   64 rows, runs one after the other / side by side: one token over 700 positions 25.6 / 16.1, 16 sequences over up to 1000 34 / 20, 64 of up to
+//     8192 259 / 223, but 256 of up to 4000 384 / 452 (parts cost traffic), 32 with a window of 1024 47 / 49. Two workgroups share a CU.
+//     A kernel of a single wave was slower everywhere (42 / 34 / 142 where two take 34 / 26 / 112): two share the loads.
+//   rows 256 or 128, one after the other / side by side at 256: a chunk of 1000 over 4096 125, 107 / 169, over 65500 1724, 1570 / 1717,
+//     of 256 over 1000 40, 34 / 40, over 16000 433, 351 / 161, 4 of 100 over up to 8192 230, 188 / 115, of 2000 over 4096 138, 166 / 302.
+//   longest sequences first / as they come, where workgroups outnumber the chip: 64 of up to 8192 223 / 246, 128 368 / 462, with fewer
+//     the ranks cost half a microsecond (16 of up to 1000 20.0 / 19.1). Twice as many parts for 64 rows: 236 / 244 for the first.
 static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, int heads, int window, int config) {
   AttentionPlan p;
   const int group = heads / c.key_heads;
@@ -962,7 +979,9 @@ static hipError_t attention_tiles_launch(const AttentionArgs& a, hipStream_t str
   const auto kernel = attention_tile_kernel<DTYPE, SLABS, WAVES, SPLIT, GROUPED>;
   const hipError_t err = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, once);
   if (err != hipSuccess) return err;
-  kernel<<<dim3((unsigned)(a.tiles * a.chunks * a.cache.key_heads)), WAVES * 64, kLds, stream>>>(a);
+  const int64_t groups = (int64_t)a.tiles * a.chunks * a.cache.key_heads;
+  if (groups * WAVES * 64 >= (int64_t)1 << 32) return hipErrorInvalidConfiguration;
+  kernel<<<dim3((unsigned)groups), WAVES * 64, kLds, stream>>>(a);
   return hipGetLastError();
 }
 template <int DTYPE, int SLABS, bool SPLIT, bool GROUPED>

@@ -229,6 +229,7 @@ def paged_attention(
             (lambda: out.dtype == q.dtype, TypeError, lambda: f"out must be {q.dtype}, got {out.dtype}."),
             (lambda: out.device == device, RuntimeError, lambda: f"out must be on {device}, got {out.device}."),
             (lambda: out.stride(2) == 1 and _on_16_bytes(out), ValueError, "the heads of out must be contiguous and start on 16 bytes."),
+            (lambda: all(n <= 1 or stride > 0 for n, stride in zip(out.shape, out.stride())), ValueError, lambda: f"out must have memory of its own for every element, got strides {out.stride()}."),
         ])  # fmt: skip
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
     if cache.c.sequences == 0:

@@ -80,13 +80,15 @@ class Batch:
     def bounds(self, size, want, most, causal=True):
         """How far out and lse may be off. A score is a chain of `width` products in 32 bits, scaled, subtracted from a maximum and raised: under
         width + 8 roundings of 2^-24 of the sum of its magnitudes, and the hardware's exponential an ulp of 2^-23 more; as many of its logarithm
-        move a weight by that factor. Weights are rounded to the type, in the sum above and in the sum below (2 half steps), both
-        sums are chains of as many 32-bit additions as there are keys, with a factor for every 64 of them and two for a run. The result is rounded once."""
+        move a weight by that factor. Weights are rounded to the type in the sum above (half a step), both
+        sums are chains of as many 32-bit additions as there are keys, with a factor for every 64 of them and two for a run. The result is rounded once.
+        Weights below 2^-14 are off by up to 2^-25 each in fp16 (2^-134 in bf16), next to a sum of 1 at least: the largest belongs to a key at the maximum."""
         longest = max([1, *(c for _, c in self.lengths)])
         score = (self.width + 8) * 2.0**-24 * most + 2.0**-22
         chain = (longest + longest / 32 + 64) * 2.0**-24
         half = HALF_STEP[self.dtype]
-        return half * want.abs() + (2 * half + 2 * score + 2 * chain) * size * (1 + 2.0**-6) + 2.0**-24, score + chain
+        small = longest * 2.0**-25 * max([0.0, *(float(v.abs().max()) for v in self.v if v.numel())]) if self.dtype == torch.float16 else 0.0
+        return half * want.abs() + (half + 2 * score + 2 * chain) * size * (1 + 2.0**-6) + 2.0**-24 + small, score + chain
 
     def check(self, got, lse=None, **how):
         want, size, want_lse, most = self.definition(**how)

@@ -99,17 +99,17 @@ def test_a_rows_bits_do_not_depend_on_its_chunk_or_batch(attention, heads, key_h
 
 
 @pytest.mark.parametrize("config", ("auto", *CONFIGS))
-@pytest.mark.parametrize("dtype, width", [(BF16, 128), (FP16, 64), (BF16, 256)])
-def test_what_a_row_does_not_see_does_not_reach_it(attention, config, dtype, width):
+@pytest.mark.parametrize("dtype, width, page_size", [(BF16, 128, 16), (FP16, 64, 16), (BF16, 256, 16), (FP16, 128, 7), (BF16, 96, 1)])
+def test_what_a_row_does_not_see_does_not_reach_it(attention, config, dtype, width, page_size):
     lengths = [(40, 100), (1, 50), (130, 300)]
     inf, nan = float("inf"), float("nan")
     for window in (None, 20):
-        clean = Batch(lengths, 4, 2, width, 16, dtype, seed=6)
+        clean = Batch(lengths, 4, 2, width, page_size, dtype, seed=6)
         want, want_lse = attention.paged_attention(clean.q, *clean.where, window=window, return_lse=True, config=config)
-        b = Batch(lengths, 4, 2, width, 16, dtype, seed=6)
+        b = Batch(lengths, 4, 2, width, page_size, dtype, seed=6)
         # keys and values at the places of some of the new tokens, and of the context
         for i, p, key, value in ((0, 80, nan, nan), (0, 85, 1.0, inf), (0, 95, inf, -inf), (2, 170, nan, 1.0), (2, 201, 1.0, -inf), (2, 260, 1.0, nan), (2, 262, 1.0, inf)):
-            page, row = int(b.table[i, p // 16]), p % 16
+            page, row = int(b.table[i, p // page_size]), p % page_size
             if key != 1.0:
                 b.keys[page, row, :, 3] = key
             if value != 1.0:

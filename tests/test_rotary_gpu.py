@@ -127,7 +127,7 @@ def test_gradients_against_differences_and_of_gradients(attention):
         d[at] = step
         with torch.no_grad():
             slope = (loss(q + d) - loss(q - d)) / (2 * step)
-        assert abs(float(slope.detach() - grad[at])) <= 100 * 8 * 2.0**-23 / step
+        assert abs(float(slope.detach() - grad.detach()[at])) <= 100 * 8 * 2.0**-23 / step
     (second,) = torch.autograd.grad(grad.sum(), q)  # 2 R^T diag(w) R 1
     ones = torch.ones_like(q)
     turned = attention.rotary_embedding(ones, None, positions, f, magnitude=1.5)[0].double()
@@ -254,3 +254,13 @@ def test_a_backward_in_a_graph(attention):
         want, size = _definition(g, positions, f, False, inverse=True)
         _near(grad, want, size)
     assert warm.shape == grad.shape
+
+
+def test_more_tokens_than_a_launch_has_workgroups(attention):
+    tokens, f = 2**24 + 5, attention.rotary_frequencies(8, device=DEV)
+    q = torch.randn((1024, 1, 8), device=DEV).to(BF16).repeat(tokens // 1024 + 1, 1, 1)[:tokens]
+    positions = torch.arange(tokens, device=DEV)
+    turned = attention.rotary_embedding(q, None, positions, f)[0]
+    for first in (0, 2**20 - 3, 2**23, tokens - 7):
+        rows = slice(first, first + 7)
+        assert same_bits(turned[rows], attention.rotary_embedding(q[rows].clone(), None, positions[rows].clone(), f)[0])
