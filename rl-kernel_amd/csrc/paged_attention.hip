@@ -107,11 +107,14 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 constexpr float kSlack = 8.f;
 __device__ __forceinline__ float next_top(float top, float x) { return x > top + kSlack ? x : top; }
 
-// The largest value of a row over the two lanes that hold it (l and l + 32), and the sum. NaN loses, as in fmaxf.
+// NaN wins, and next_top() leaves the maximum as it is: such a row is NaN by its weights. (fmaxf, where it loses, takes an instruction more for
+// each first operand: 31 a tile, not 19; a chunk of 1000 tokens over 65500 0.5 to 1.4 % longer.)
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+// The largest value of a row over the two lanes that hold it (l and l + 32), and the sum.
 __device__ __forceinline__ float max_over_halves(float v) {
   const uint32_t w = __float_as_uint(v);
   const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  return larger(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float sum_over_halves(float v) {
   const uint32_t w = __float_as_uint(v);
@@ -230,12 +233,12 @@ struct Weighing {
       const int b = n >> 1, first = 8 * (n & 1);
       float x = s[b][first];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b][first + i]);
+      for (int i = 1; i < 8; ++i) x = larger(x, s[b][first + i]);
       asm volatile("" : "+v"(x));  // (here and below: computed in its piece, not where it is used)
       top[n] = x;
     } else if (n == 4) {
       const float before = st.m;
-      st.m = next_top(before, max_over_halves(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))) * a.scale);
+      st.m = next_top(before, max_over_halves(larger(larger(top[0], top[1]), larger(top[2], top[3]))) * a.scale);
       moved = st.m != before;
       factor = moved ? exp2_fast(before - st.m) : 1.f;
       from = st.m == -INFINITY ? 0.f : st.m;

@@ -3,6 +3,8 @@ may not depend on."""
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -272,3 +274,54 @@ def test_many_sequences(attention):
         want = out if want is None else want
         assert same_bits(out, want)
     b.check(want)
+
+
+def test_from_several_threads(attention):
+    batches = [Batch([(1, 3000 + 100 * s), (5, 2000), (300, 900)], 8, 2, 128, 16, BF16, seed=s) for s in range(4)]
+    want = [attention.paged_attention(b.q, *b.where) for b in batches]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            wrong.extend(i for _ in range(20) if not same_bits(attention.paged_attention(batches[i].q, *batches[i].where), want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_two_graphs_of_one_pool(attention):
+    batches = [Batch([(1, 3000), (5, 2000 + 300 * s)], 8, 2, 128, 16, BF16, seed=s) for s in range(2)]
+    want = [attention.paged_attention(b.q, *b.where) for b in batches]
+    graphs, outs, pool = [torch.cuda.CUDAGraph() for _ in range(2)], [], torch.cuda.graph_pool_handle()
+    for b, graph in zip(batches, graphs):
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(attention.paged_attention(b.q, *b.where))
+    for _ in range(3):
+        for i, graph in enumerate(graphs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert same_bits(outs[i], want[i])
+            assert same_bits(attention.paged_attention(batches[i].q, *batches[i].where), want[i])
+
+
+def test_views_and_repeated_memory(attention):
+    b = Batch([(1, 3000), (5, 2000)], 8, 2, 128, 16, BF16, seed=3)
+    want = attention.paged_attention(b.q, *b.where)
+    repeated = b.q[:1].expand(6, 8, 128)
+    assert same_bits(attention.paged_attention(repeated, *b.where), attention.paged_attention(repeated.contiguous(), *b.where))
+    wide = torch.zeros((6, 8, 160), device=DEV, dtype=BF16)
+    wide[..., 16:144] = b.q
+    assert same_bits(attention.paged_attention(wide[..., 16:144], *b.where), want)
+    wide[..., 1:129] = b.q  # rows that do not start on 16 bytes
+    assert same_bits(attention.paged_attention(wide[..., 1:129], *b.where), want)
+    with torch.inference_mode():
+        assert same_bits(attention.paged_attention(b.q * 1, *b.where), want)
+    with pytest.raises(ValueError, match="memory of its own"):
+        attention.paged_attention(b.q, *b.where, out=torch.empty((1, 8, 128), device=DEV, dtype=BF16).expand(6, 8, 128))
+    b.table[0, 1] = b.table[0, 0]  # a page twice
+    assert same_bits(attention.paged_attention(b.q, *b.where), attention.paged_attention(b.q, *b.where, config="rows128"))
