@@ -219,6 +219,7 @@ def paged_attention(
         (window is None or causal, ValueError, "a window goes with causal=True."),
         (config in _lib.ATTENTION_CONFIGS, ValueError, lambda: f"config must be one of {tuple(_lib.ATTENTION_CONFIGS)}, got {config!r}."),
     ])  # fmt: skip
+    window = 0 if window is None else min(window, 2**31 - 1)  # (no position is further out)
     given = out
     if out is None:
         out = torch.empty((tokens, heads, width), dtype=q.dtype, device=device)
@@ -240,12 +241,12 @@ def paged_attention(
     elif tokens > 0:
         q = q if _on_16_bytes(q) else q.clone(memory_format=torch.contiguous_format)
         lib, how = _lib.load(), _lib.ATTENTION_CONFIGS[config]
-        size = int(lib.rlk_paged_attention_workspace_bytes(ctypes.byref(cache.c), tokens, heads, window or 0, how))
+        size = int(lib.rlk_paged_attention_workspace_bytes(ctypes.byref(cache.c), tokens, heads, window, how))
         workspace = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
         with _on(device):
             status = lib.rlk_paged_attention(
                 ctypes.byref(cache.c), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                None if lse is None else lse.data_ptr(), tokens, heads, scale, int(causal), window or 0, int(given is None), how,
+                None if lse is None else lse.data_ptr(), tokens, heads, scale, int(causal), window, int(given is None), how,
                 None if workspace is None else workspace.data_ptr(), size, _stream_handle(device),
             )  # fmt: skip
         _lib.check(status, "rlk_paged_attention failed")

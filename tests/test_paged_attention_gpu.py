@@ -325,3 +325,10 @@ def test_views_and_repeated_memory(attention):
         attention.paged_attention(b.q, *b.where, out=torch.empty((1, 8, 128), device=DEV, dtype=BF16).expand(6, 8, 128))
     b.table[0, 1] = b.table[0, 0]  # a page twice
     assert same_bits(attention.paged_attention(b.q, *b.where), attention.paged_attention(b.q, *b.where, config="rows128"))
+
+
+def test_windows_beyond_32_bits(attention):
+    b = Batch([(3, 300), (40, 129)], 4, 2, 64, 16, BF16, seed=5)
+    want = attention.paged_attention(b.q, *b.where)
+    for window in (2**31 - 1, 2**31, 2**32 + 5):
+        assert same_bits(attention.paged_attention(b.q, *b.where, window=window), want)
