@@ -63,7 +63,7 @@ struct AttentionArgs {
   float* part_sum;
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
   int64_t part_rows;  // tokens * heads
-  PageDivider by_page, by_group, by_key_heads;
+  PageDivider by_page, by_group, by_key_heads, by_chunks;
   int tokens, heads, group, causal, window, zero_rest, longest_first, tiles, chunks;
   float scale;  // times log2(e)
 };
@@ -461,8 +461,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   const uint32_t id = blockIdx.x;
   const uint32_t outer = divide_by(id, a.by_key_heads);
   const int key_head = (int)(id - outer * a.cache.key_heads);
-  const int chunk_id = SPLIT ? (int)(outer % (uint32_t)a.chunks) : 0;
-  const int tile_id = (int)(SPLIT ? outer / (uint32_t)a.chunks : outer);
+  const int tile_id = (int)(SPLIT ? divide_by(outer, a.by_chunks) : outer);
+  const int chunk_id = SPLIT ? (int)outer - tile_id * a.chunks : 0;
   int s = tile_id, row0 = 0;
   if (tile_id < a.cache.sequences && a.longest_first) {  // of 64 sequences: this one's place is its length's
     const int first = tile_id & ~63, count = min(64, a.cache.sequences - first);
@@ -535,7 +535,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
 #pragma unroll
     for (int ks = 0; ks < State::kSteps; ++ks) {
       const int element = 16 * ks + 8 * half;
-      const u32x4_t v = r.live && element < a.cache.width ? *reinterpret_cast<const u32x4_t*>(row + 2 * element) : u32x4_t{0, 0, 0, 0};
+      const bool wanted = r.live && element < a.cache.width;
+      u32x4_t v = *reinterpret_cast<const u32x4_t*>(row + (wanted ? 2 * element : 0));
+      if (!wanted) v = u32x4_t{0, 0, 0, 0};
       if (kKeepQ)
         kept_q[kKeepQ ? ks : 0] = v;
       else
@@ -564,14 +566,13 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   // This workgroup's tiles: those of runs that start in its part.
   int t = low / kTileKeys, end_tile = (high + kTileKeys - 1) / kTileKeys;
   if (SPLIT) {
-    const int first = t, count = end_tile - t;
-    auto border = [&](int chunk) __attribute__((always_inline)) {  // the first run that starts there or later
-      const int tile = first + (int)((int64_t)count * chunk / a.chunks);
-      const int run = run_of_tile(tile);
-      return tile <= first ? first : run_first_tile(run) >= tile ? tile : run_first_tile(run + 1);
-    };
-    t = border(chunk_id);
-    end_tile = min(end_tile, border(chunk_id + 1));
+    // The first run that starts at a part's border or later: even lanes for this part, odd ones for the next (in one go, without branches).
+    const int first = t, count = end_tile - first, each = (int)divide_by((uint32_t)max(count, 0), a.by_chunks);
+    const int part = chunk_id + (lane & 1), tile = first + each * part + min(part, max(count, 0) - each * a.chunks);
+    const int run = run_of_tile(tile), run_start = run_first_tile(run), next_start = run_first_tile(run + 1);
+    const int border = tile <= first ? first : run_start >= tile ? tile : next_start;
+    t = __builtin_amdgcn_readlane(border, 0);
+    end_tile = min(end_tile, __builtin_amdgcn_readlane(border, 1));
   }
   if (t >= end_tile && SPLIT) return;
   auto keys_of = [&](int stage) __attribute__((always_inline)) { return lds + stage * 2 * kTileBytes; };
@@ -1036,7 +1037,8 @@ hipError_t paged_attention_launch(const rlk_paged_cache& cache, const void* q, i
   a.tokens = (int)tokens;
   a.heads = heads;
   a.causal = causal, a.window = window, a.zero_rest = zero_rest;
-  a.tiles = p.tiles, a.chunks = p.chunks, a.longest_first = p.longest_first;
+  a.tiles = p.tiles, a.by_chunks = page_divider((uint32_t)p.chunks);
+  a.chunks = p.chunks, a.longest_first = p.longest_first;
   a.scale = (float)((double)scale * 1.4426950408889634074);
   return cache.dtype == RLK_DTYPE_BF16 ? attention_launch_as<RLK_DTYPE_BF16>(a, p, stream) : attention_launch_as<RLK_DTYPE_FP16>(a, p, stream);
 }
