@@ -804,7 +804,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   while (t < end_tile) {
     // A turn with everything that may come up, then plain ones as long as nothing does: what changes the outputs besides the
     // products stands outside of their loop, where it would have them copied from register to register in every turn.
-    const bool run_starts = t == run_end;
+    const bool run_starts = t == run_end, first_turn = before < 0;
     float its_m, its_l;
     volatile float effect[16 * State::kBlocks];  // (in memory, see find_special)
     const bool special = before >= 0 && mixed(before) && special_tile[stage ^ 1] == before + 1;
@@ -815,8 +815,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
       const int run = run_of_tile(before);
       end_run(run - 1, its_m, its_l);
       run_end = run_first_tile(run + 1);
-      factor = 1.f;
     }
+    if (run_starts || first_turn) factor = 1.f;  // (nothing is there to be scaled)
     const int plain_to = min(min(run_end, end_tile), min(masked_from, mixed_from)), plain_from = max(masked_to, mixed_to + 1);
     while (t >= plain_from && t < plain_to && !__any(factor != 1.f)) factor = turn(IntTag<1>{}, its_m, its_l);
     if (__any(factor != 1.f)) {
