@@ -16,7 +16,7 @@
 namespace rlk {
 
 constexpr int kRotaryThreads = 256;
-constexpr int64_t kRotaryGroups = 1 << 20;  // workgroups at most (a grid has fewer than 2^32 threads)
+constexpr int64_t kRotaryGroups = 1 << 23;  // workgroups of a launch at most (a grid has fewer than 2^32 threads)
 
 template <int ELEM>
 struct RotaryElem;
@@ -61,7 +61,7 @@ struct RotaryArgs {
   rlk_rotary rotary;
   rlk_paged_cache cache;  // of an append
   PageDivider by_page, by_items, by_inner;
-  int64_t tokens, inner;
+  int64_t tokens, inner, first;  // (of this launch)
   int width, items;  // pieces (or single pairs and elements) of a head
   float sign;
 };
@@ -74,10 +74,13 @@ struct TokenPlace {
 };
 
 template <int ELEM, bool WHOLE, bool APPEND>
-__device__ __forceinline__ void rotary_token(const RotaryArgs& a, int64_t t, float2* turn) {
+__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
   typedef RotaryElem<ELEM> E;
   typedef typename E::type T;
+  extern __shared__ float2 turn[];  // [pairs] cosine and sine, scaled
   const int tid = threadIdx.x, pairs = a.rotary.pairs;
+  const int64_t t = a.first + blockIdx.x;
+
   TokenPlace place = {-1, -1, 0, 0};
   if (APPEND) {  // every wave for itself
     const int s = wave_search(a.cache.sequences + 1, t, tid & 63, [&](int i) { return (int64_t)a.cache.starts[i]; });
@@ -189,15 +192,6 @@ __device__ __forceinline__ void rotary_token(const RotaryArgs& a, int64_t t, flo
   }
 }
 
-template <int ELEM, bool WHOLE, bool APPEND>
-__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
-  extern __shared__ float2 turn[];  // [pairs] cosine and sine, scaled
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    if (t != blockIdx.x) __syncthreads();  // (the last token's angles have been used)
-    rotary_token<ELEM, WHOLE, APPEND>(a, t, turn);
-  }
-}
-
 // Whether every head of the tensor starts on 16 bytes.
 static bool whole_pieces(const void* base, int64_t outer, int64_t token, int64_t head, int count) {
   return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && outer % count == 0 && token % count == 0 && head % count == 0;
@@ -219,15 +213,14 @@ static hipError_t rotary_launch_as(RotaryArgs& a, bool append, hipStream_t strea
             whole_pieces(a.cache.values, a.cache.value_page_stride, a.cache.value_row_stride, a.cache.value_head_stride, kCount);
   a.items = whole ? (a.rotary.interleaved ? a.width : a.width - pairs) / kCount : a.width - pairs;
   a.by_items = page_divider(a.items);
-  const dim3 grid((unsigned)(a.tokens < kRotaryGroups ? a.tokens : kRotaryGroups));
   const size_t lds = sizeof(float2) * (pairs > 0 ? pairs : 1);
-  if (append) {
-    if (whole)
+  for (a.first = 0; a.first < a.tokens; a.first += kRotaryGroups) {
+    const dim3 grid((unsigned)(a.tokens - a.first < kRotaryGroups ? a.tokens - a.first : kRotaryGroups));
+    if (append && whole)
       rotary_kernel<ELEM, true, true><<<grid, kRotaryThreads, lds, stream>>>(a);
-    else
+    else if (append)
       rotary_kernel<ELEM, false, true><<<grid, kRotaryThreads, lds, stream>>>(a);
-  } else {
-    if (whole)
+    else if (whole)
       rotary_kernel<ELEM, true, false><<<grid, kRotaryThreads, lds, stream>>>(a);
     else
       rotary_kernel<ELEM, false, false><<<grid, kRotaryThreads, lds, stream>>>(a);
