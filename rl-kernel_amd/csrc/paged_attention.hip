@@ -22,11 +22,11 @@
 // it: such a tile is looked through before it is used, and if it holds any they are taken out of the product and added to the
 // rows that see them.
 //
-// What bounds it. With few rows a tile's keys and values, HBM: 4 sequences of 131071 positions 411 us, 5.2 TB/s (a large copy reaches 4.9);
-// 64 of up to 8192 223 us, 4.6 TB/s. With many the two products beside the vector work of the weights (32 matrix instructions of 32
+// What bounds it. With few rows a tile's keys and values, HBM: 4 sequences of 131071 positions 415 us, 5.2 TB/s (a large copy reaches 4.9);
+// 64 of up to 8192 222 us, 4.5 TB/s. With many the two products beside the vector work of the weights (32 matrix instructions of 32
 // cycles against some 200 vector instructions, 33 of them exponentials, for 32 rows and a tile): prompts of up to 12000 tokens 2.3 ms, 0.95
-// PFLOP/s (2.1 ms on zeros, where the clock does not drop). A short call is a chain of latencies: 1025 positions of one token take 16 us, of
-// which 4 go by until the first keys are there and 2 for each of the four tiles of a run.
+// PFLOP/s (2.1 ms on zeros, where the clock does not drop). A short call is a chain of latencies: 1025 positions of one token take 15 us, of
+// which 3 to 4 go by until the first keys are there, 2 for each of the four tiles of a run and 4 for joining the runs.
 #include "det_gemm_solo.h"
 #include "paged.h"
 
