@@ -480,6 +480,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
     s = wave_search(a.cache.sequences + 1, other, lane, [&](int i) { return other_row_tiles<kRows>(a, i); });
     if (s < 0) return;
     const int first = (int)other_row_tiles<kRows>(a, s);
+    if (other < first) return;  // (starts that do not ascend: what the search finds need not lie in front; row0 and tails below would be negative)
     if (s >= a.cache.sequences) {  // behind the last sequence
       if (!SPLIT && a.zero_rest) {
         const int before = clamp_to(a.cache.starts[0], 0, a.tokens), behind = clamp_to(a.cache.starts[s], before, a.tokens);
@@ -873,7 +874,7 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
   bool known = false;
   if (s >= 0 && s < a.cache.sequences) {
     const Chunk c = chunk_of(a, s);
-    known = token - c.first_token < c.tokens;
+    known = token >= c.first_token && token - c.first_token < c.tokens;
     if (known) sight = sight_of(a, c, token - c.first_token);
   }
   if (!known && !a.zero_rest) return;

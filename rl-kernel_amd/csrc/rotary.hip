@@ -84,7 +84,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
   TokenPlace place = {-1, -1, 0, 0};
   if (APPEND) {  // every wave for itself
     const int s = wave_search(a.cache.sequences + 1, t, tid & 63, [&](int i) { return (int64_t)a.cache.starts[i]; });
-    if (s >= 0 && s < a.cache.sequences && t < a.cache.starts[s + 1]) {
+    if (s >= 0 && s < a.cache.sequences && t >= a.cache.starts[s] && t < a.cache.starts[s + 1]) {  // (starts need not ascend)
       place.known = 1;
       place.position = (int64_t)a.cache.lengths[s] - a.cache.starts[s + 1] + t;
       if (place.position >= 0 && place.position < 0x7fffffff) {

@@ -3,8 +3,9 @@
 The cache is two tensors of the caller's, ``[pages, page_size, key heads, width]`` in any order in memory whose last dimension is
 contiguous. ``page_table[s, i]`` is the page of positions ``i * page_size ...`` of sequence s, ``context_lengths[s]`` counts its
 positions with the new tokens of the call, and those are rows ``query_starts[s] ... query_starts[s + 1]`` of the tensors of tokens: the last
-ones of the context. All three are int32 tensors on the device; nothing of them is read back, so a call can be captured into a
-HIP graph and replayed with other lengths.
+ones of the context. ``query_starts`` ascend; where they do not, it is not specified which rows are computed, but nothing outside of the
+tensors is touched and no cache row but a new token's written. All three are int32 tensors on the device; nothing of them is read
+back, so a call can be captured into a HIP graph and replayed with other lengths.
 """
 
 from __future__ import annotations

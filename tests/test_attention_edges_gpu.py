@@ -1,0 +1,73 @@
+"""Paged attention and appending at the edges of what they are given: starts out of order, rows behind the page table, the largest
+positions, memory that autograd watches."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from attention_cases import DEV, Batch, same_bits
+from rl_engine import _lib
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+CONFIGS = tuple(name for name in _lib.ATTENTION_CONFIGS if name != "auto")
+
+
+@pytest.fixture(scope="module")
+def attention():
+    from rl_engine.ops import attention
+
+    return attention
+
+
+def _ints(*values):
+    return torch.tensor(values, device=DEV, dtype=torch.int32)
+
+
+def _normal(*shape, seed=0, dtype=BF16):
+    return torch.randn(shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(dtype)
+
+
+OUT_OF_ORDER = [(0, 1000, 10, 1010), (1010, 500, 0, 3), (700, 0, 1010, 20), (-5, 2000, -7, 900), (3, 3, 1, 1), (1010, 0, 0, 0), (0, 5, 900, 1)]
+
+
+@pytest.mark.parametrize("starts", OUT_OF_ORDER)
+def test_starts_that_do_not_ascend_stay_within_the_tensors(attention, starts):
+    b = Batch([(1, 700), (1, 900), (1, 1010)], 8, 2, 64, 16, BF16, seed=1)
+    tokens, guard = 1010, 64
+    room = torch.full((tokens + 2 * guard, 8, 64), 7.0, device=DEV, dtype=BF16)
+    q = torch.zeros_like(room)[guard:-guard]
+    for config in ("auto", *CONFIGS):
+        for out in (None, room[guard:-guard]):
+            attention.paged_attention(q, b.keys, b.values, b.table, b.contexts, _ints(*starts), out=out, return_lse=True, config=config)
+        assert bool((room[:guard] == 7).all()) and bool((room[-guard:] == 7).all())
+
+
+@pytest.mark.parametrize("starts", OUT_OF_ORDER)
+def test_appending_with_starts_that_do_not_ascend_writes_new_places_alone(attention, starts):
+    contexts = (700, 900, 1010)
+    b = Batch([(1, c) for c in contexts], 8, 2, 64, 16, BF16, seed=1)
+    k = _normal(1010, 2, 64, seed=2)
+    keys = b.keys.clone()
+    attention.paged_append(k, k, b.keys, b.values, b.table, b.contexts, _ints(*starts), q=k)
+    for s, c in enumerate(contexts):
+        new = min(max(0, starts[s + 1] - starts[s]), c)
+        place = torch.arange(c - new, device=DEV)
+        page, row = b.table[s].long()[place // 16], place % 16
+        assert same_bits(b.keys[page, row], keys[page, row]), s
+    used = torch.cat([b.table[s, : -(-c // 16)] for s, c in enumerate(contexts)]).long()
+    rest = torch.ones(b.keys.size(0), dtype=torch.bool, device=DEV)
+    rest[used] = False
+    assert same_bits(b.keys[rest], keys[rest])
+
+
+def test_a_token_that_no_ascending_search_finds_is_not_written(attention):
+    """Token 3 of starts 0, 5, 6, 1: two of them are at most 3, and the second sequence starts behind it."""
+    b = Batch([(1, 40), (1, 40), (1, 40)], 2, 1, 64, 16, BF16, seed=3)
+    keys = b.keys.clone()
+    k = _normal(6, 1, 64, seed=4)
+    attention.paged_append(k, k, b.keys, b.values, b.table, b.contexts, _ints(0, 5, 6, 1))
+    place = torch.arange(39, device=DEV)
+    page, row = b.table[1].long()[place // 16], place % 16
+    assert same_bits(b.keys[page, row], keys[page, row])
