@@ -617,8 +617,9 @@ int rlk_rotary_embedding(const rlk_rotary* host_rotary, const rlk_head_rows* hos
  * A paged cache of keys and values, and the new tokens of a call: sequence s has the tokens [starts[s], starts[s + 1]), the last
  * ones of its lengths[s] (which counts them). Position p of a sequence lies in row p % page_size of page table[s][p / page_size].
  * Positions outside of the table's columns and entries outside of [0, pages) are missing: nothing is written there, and a row that
- * sees one becomes NaN. Nothing is read back: all of it is checked on the device. Where starts do not ascend, which rows and places a
- * call computes is not specified, but it stays within the tensors and writes no cache row that is not a new token's.
+ * sees one becomes NaN (attention: so do rows that see positions from 2^31 - 256 on). Nothing is read back: all of it is checked on
+ * the device. Where starts do not ascend, which rows and places a call computes is not specified, but it stays within the tensors and
+ * writes no cache row that is not a new token's.
  */
 typedef struct rlk_paged_cache {
   void* keys;   /* [pages, page_size, key_heads, width], any strides but the last, which is 1 */

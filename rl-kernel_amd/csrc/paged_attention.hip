@@ -35,7 +35,7 @@ namespace rlk {
 constexpr int kTileKeys = 64;
 constexpr int kSlabBytes = kTileKeys * 128;  // 64 keys x 64 elements
 constexpr int kMaxWidth = 256;
-constexpr int kMostKeys = 0x7fffff00;  // of a sequence
+constexpr int kMostKeys = 0x7fffff00;  // of a sequence: positions behind have no place (32-bit numbers of keys and tiles ahead must not overflow)
 
 // Runs: their lengths grow with the position, so that a short context still has enough of them for the chip and a long
 // one's partial results stay few (of 8 rows a part is 1/32 of the keys and values that a run of 256 reads, 1/256 of 2048). Tiles 0 ... 63 in fours, ... 255 in eights, ... 1023 in sixteens, then 32 at a time.
@@ -169,7 +169,8 @@ __device__ __forceinline__ Chunk chunk_of(const AttentionArgs& a, int sequence) 
   return c;
 }
 
-// Positions that the page table has room for. A row that sees more of them sees the one behind, which is missing.
+// Positions that the page table has room for. A row that sees any behind them is NaN: without a window it sees the first of those, which is
+// loaded as NaN, but a window may begin behind it, where nothing is loaded, so the end of a row asks for its last position.
 __host__ __device__ __forceinline__ int capacity_of(const rlk_paged_cache& c) {
   const int64_t keys = (int64_t)c.table_columns * c.page_size;
   return keys < kMostKeys ? (int)keys : kMostKeys;
@@ -840,8 +841,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
   if (SPLIT) return;
   const RowPlace r = row_place();
   if (!r.live) return;
-  const bool any = st.sight.high > st.sight.low;
-  const float reciprocal = any ? 1.f / all_l : 0.f;
+  const bool any = st.sight.high > st.sight.low, behind = st.sight.high > capacity;
+  const float reciprocal = behind ? NAN : any ? 1.f / all_l : 0.f;
   char* const to = a.out + (int64_t)r.token * a.out_token_stride + (int64_t)r.head * a.out_head_stride;
 #pragma unroll
   for (int d = 0; d < State::kBlocks; ++d)
@@ -854,7 +855,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
       const int element = 32 * d + 2 * i + 4 * half;
       if (element < a.cache.width) *reinterpret_cast<u32x2_t*>(to + 2 * element) = u32x2_t{H::pack(y[0], y[1]), H::pack(y[2], y[3])};
     }
-  if (a.lse && half == 0) a.lse[(int64_t)r.token * a.heads + r.head] = any ? lse_of(all_m, all_l) : -INFINITY;
+  if (a.lse && half == 0) a.lse[(int64_t)r.token * a.heads + r.head] = behind ? NAN : any ? lse_of(all_m, all_l) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -905,10 +906,10 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
       }
     }
   }
-  const bool sees = sight.high > sight.low;
-  const float y = sees ? output_of(o, 1.f / sum) : 0.f;
+  const bool sees = sight.high > sight.low, behind = sight.high > capacity;
+  const float y = behind ? NAN : sees ? output_of(o, 1.f / sum) : 0.f;
   if (tid < width) *reinterpret_cast<uint16_t*>(out) = (uint16_t)Half<DTYPE>::pack(y, 0.f);
-  if (a.lse && tid == 0) a.lse[row] = sees ? lse_of(top, sum) : -INFINITY;
+  if (a.lse && tid == 0) a.lse[row] = behind ? NAN : sees ? lse_of(top, sum) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------

@@ -71,3 +71,34 @@ def test_a_token_that_no_ascending_search_finds_is_not_written(attention):
     place = torch.arange(39, device=DEV)
     page, row = b.table[1].long()[place // 16], place % 16
     assert same_bits(b.keys[page, row], keys[page, row])
+
+
+@pytest.mark.parametrize("config", ("auto", *CONFIGS))
+@pytest.mark.parametrize("columns, window, new, context", [(4, 8, 1, 100), (4, 8, 1, 400), (4, 8, 40, 100), (4, 8, 1, 67), (4, 70, 30, 100), (8, 40, 300, 700), (20, 300, 5, 4000), (0, 8, 3, 100)])
+@pytest.mark.parametrize("width, page", [(64, 16), (128, 16), (96, 17)])
+def test_windowed_rows_behind_the_table(attention, config, columns, window, new, context, width, page):
+    """Missing, whether the window reaches back into the table or not: NaN and a NaN logarithm. The rows in front keep their bits."""
+    b = Batch([(new, context)], 4, 2, width, page, BF16, seed=7)
+    want, want_lse = attention.paged_attention(b.q, *b.where, window=window, return_lse=True)
+    table = b.table[:, :columns].contiguous()
+    out, lse = attention.paged_attention(b.q, b.keys, b.values, table, b.contexts, b.starts, window=window, return_lse=True, config=config)
+    inside = max(0, min(new, columns * page - (context - new)))  # rows at positions that the table has room for
+    assert same_bits(out[:inside], want[:inside]) and same_bits(lse[:inside], want_lse[:inside])
+    assert bool(out[inside:].isnan().all()) and bool(lse[inside:].isnan().all())
+
+
+@pytest.mark.parametrize("config", ("auto", *CONFIGS))
+def test_the_last_positions(attention, config):
+    """Positions from 2^31 - 256 on have no place, whatever the table holds; the one in front of them is as any other."""
+    page = 2**24
+    keys, values = (torch.zeros((1, page, 1, 8), device=DEV, dtype=BF16) for _ in range(2))
+    keys[0, -320:, 0], values[0, -320:, 0] = _normal(320, 8, seed=1), _normal(320, 8, seed=2)
+    table, q = torch.zeros((1, 128), device=DEV, dtype=torch.int32), _normal(2, 2, 8, seed=3)
+    run = lambda q, k, v, t, c: attention.paged_attention(q, k, v, t, _ints(c), _ints(0, q.size(0)), window=8, return_lse=True, config=config)  # noqa: E731
+    near = keys[:, -320:-256].contiguous(), values[:, -320:-256].contiguous()
+    want, want_lse = run(q[:1], *near, table[:, :1], 64)  # position 63 there, 2^31 - 257 here
+    out, lse = run(q, keys, values, table, 2**31 - 255)
+    assert same_bits(out[:1], want) and same_bits(lse[:1], want_lse)
+    assert bool(out[1].isnan().all()) and bool(lse[1].isnan().all())
+    out, lse = run(q, keys, values, table, 2**31 - 1)
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())
