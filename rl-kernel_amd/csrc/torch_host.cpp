@@ -924,6 +924,10 @@ struct CacheInputs {
     return c;
   }
 };
+// What a kernel has written counts as written for autograd (a tensor of inference mode has no versions).
+void count_write(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 bool everyday_tokens(const Tensor& t, const CacheInputs& cache) {
   return everyday(t, cache.keys.scalar_type(), cache.keys) && t.dim() == 3 && t.numel() > 0 && t.stride(2) == 1 && t.size(2) == cache.keys.size(3) && t.size(1) <= INT_MAX;
 }
@@ -1249,6 +1253,8 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t count) {
     const rlk_head_rows rows_q = q.defined() ? head_rows(q, turned) : rlk_head_rows{}, rows_k = head_rows(k, Tensor()), rows_v = head_rows(v, Tensor());
     check_status(append_entry(&described, frequencies.defined() ? &rotary : nullptr, q.defined() ? &rows_q : nullptr, &rows_k, &rows_v, k.size(0), stream_of(k)),
                  "rlk_paged_append failed");
+    count_write(cache.keys);
+    count_write(cache.values);
   }
   const PyRef result(wrap(turned));
   return PyTuple_Pack(1, result.get());

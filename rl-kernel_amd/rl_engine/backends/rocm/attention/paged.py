@@ -16,6 +16,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from rl_engine import _host, _lib
 from rl_engine._C import _on, _stream_handle
@@ -160,6 +161,7 @@ def paged_append(
             ctypes.byref(cache.c), by(rotary), by(described), by(_rows(k)), by(_rows(v)), tokens, _stream_handle(device)
         )
     _lib.check(status, "rlk_paged_append failed")
+    increment_version((key_cache, value_cache))  # (what a kernel has written counts as written for autograd)
     return turned
 
 
@@ -251,6 +253,8 @@ def paged_attention(
                 None if workspace is None else workspace.data_ptr(), size, _stream_handle(device),
             )  # fmt: skip
         _lib.check(status, "rlk_paged_attention failed")
+        if given is not None:
+            increment_version(out)
     return (out, lse) if return_lse else out
 
 

@@ -102,3 +102,53 @@ def test_the_last_positions(attention, config):
     assert bool(out[1].isnan().all()) and bool(lse[1].isnan().all())
     out, lse = run(q, keys, values, table, 2**31 - 1)
     assert bool(out.isnan().all()) and bool(lse.isnan().all())
+
+
+class _Nothing:
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.fixture(params=("native", "general"))
+def way(request, monkeypatch):
+    if request.param == "general":
+        from rl_engine import _host
+
+        monkeypatch.setattr(_host, "_native", _Nothing())
+    return request.param
+
+
+def test_autograd_sees_what_is_written(attention, way):
+    b = Batch([(2, 40), (1, 33)], 4, 2, 64, 16, BF16, seed=5)
+    k, f = _normal(3, 2, 64, seed=6), attention.rotary_frequencies(64, device=DEV)
+    for which in ("keys", "values"):
+        w = torch.ones((), device=DEV, dtype=BF16, requires_grad=True)
+        kept = getattr(b, which) * w  # its backward reads the cache
+        attention.paged_append(k, k, *b.where, f, q=b.q)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.sum().backward()
+    whole = torch.zeros((3, 6, 64), device=DEV, dtype=BF16)
+    w = torch.ones((), device=DEV, dtype=BF16, requires_grad=True)
+    kept = whole * w
+    before = [t._version for t in (*b.where, b.q)]
+    attention.paged_attention(b.q, *b.where, out=whole[:, 1:5])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.sum().backward()
+    assert before == [t._version for t in (*b.where, b.q)]  # it reads the others
+    with pytest.raises(ValueError):
+        attention.paged_append(k, k[:2], *b.where, f)
+    assert before == [t._version for t in (*b.where, b.q)]
+
+
+def test_caches_of_inference_mode(attention, way):
+    b = Batch([(2, 40), (1, 33)], 4, 2, 64, 16, BF16, seed=5)
+    k = _normal(3, 2, 64, seed=6)
+    with torch.inference_mode():
+        keys, values, out = b.keys.clone(), b.values.clone(), torch.zeros_like(b.q)
+    attention.paged_append(k, k, *b.where)
+    attention.paged_append(k, k, keys, values, *b.where[2:])  # (outside of the mode, they have no versions)
+    assert same_bits(keys, b.keys) and same_bits(values, b.values)
+    attention.paged_attention(b.q, keys, values, *b.where[2:], out=out)
+    assert same_bits(out, attention.paged_attention(b.q, *b.where))
+    with torch.inference_mode():
+        attention.paged_append(k, k, *b.where)
