@@ -1201,6 +1201,19 @@ bool cache_of(PyObject* const* args, CacheInputs* cache) {
          tensor_or_nothing(args[3], &cache->lengths) && tensor_or_nothing(args[4], &cache->starts);
 }
 
+// plain(tensors or None...) -> whether they are values in GPU memory and nothing records the operations on them, so that a kernel may be
+// launched on their addresses
+PyObject* py_plain(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  bool plain = everyday_caller();
+  for (Py_ssize_t i = 0; plain && i < count; ++i) {
+    const Tensor* const t = exact_tensor(args[i]);
+    plain = args[i] == Py_None || (t != nullptr && everyday(*t, t->scalar_type()));
+  }
+  return PyBool_FromLong(plain);
+  END_HANDLE_TH_ERRORS
+}
+
 // rotary(q, k or None, positions, frequencies, interleaved, magnitude) -> (q, k or None) turned, or None
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
@@ -1376,6 +1389,7 @@ PyMethodDef methods[] = {
     {"reaches_default_stream", py_reaches_default_stream, METH_NOARGS, nullptr},
     {"linear_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_scores)), METH_FASTCALL, nullptr},
     {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm)), METH_FASTCALL, nullptr},
+    {"plain", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_plain)), METH_FASTCALL, nullptr},
     {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rotary)), METH_FASTCALL, nullptr},
     {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL, nullptr},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_attention)), METH_FASTCALL, nullptr},

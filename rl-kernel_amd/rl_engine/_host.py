@@ -46,6 +46,12 @@ def native():
     return _native
 
 
+def recorded(*tensors) -> bool:
+    """Whether something records or takes over the operations on ``tensors`` (``None`` among them is passed over): a compiler, a tracer, a
+    mode, a profiler, a subclass. A launch on their addresses would escape it: the caller goes through a registered operator."""
+    return torch.compiler.is_compiling() or not native().plain(*tensors)
+
+
 def refuse_capture_into_another_graph() -> None:
     """For a backward in front of its first launch. A leaf keeps the node that gathers its gradient as long as any graph holds the leaf,
     and the engine orders that node's stream behind the gradient. Under graph capture a stream joins the capture by that, which the

@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -87,7 +87,6 @@ class _Cache:
     __slots__ = ("c", "held")
 
     def __init__(self, key_cache, value_cache, page_table, context_lengths, query_starts):
-        _check_cache(key_cache, value_cache, page_table, context_lengths, query_starts)
         table = page_table if page_table.stride(1) == 1 or page_table.size(1) <= 1 else page_table.contiguous()
         lengths, starts = context_lengths.contiguous(), query_starts.contiguous()
         self.held = (table, lengths, starts)
@@ -135,34 +134,61 @@ def paged_append(
         if done is not None:
             return done[0]
     _inference_only("paged_append", k, v, q, key_cache, value_cache)
-    cache = _Cache(key_cache, value_cache, page_table, context_lengths, query_starts)
+    where = (key_cache, value_cache, page_table, context_lengths, query_starts)
+    _check_cache(*where)
     heads, width, device = key_cache.size(2), key_cache.size(3), key_cache.device
     k = _check_tokens(k, "k", key_cache, heads=heads)
     tokens = k.size(0)
     v = _check_tokens(v, "v", key_cache, tokens, heads)
     if width > _lib.ROTARY_MAX_WIDTH:
         raise ValueError(f"heads of up to {_lib.ROTARY_MAX_WIDTH} elements are served, got {width}.")
-    turned = None
     if q is not None:
         q = _check_tokens(q, "q", key_cache, tokens)
-        turned = torch.empty(q.shape, dtype=q.dtype, device=device)
-    rotary = None
     if frequencies is not None:
         frequencies = check_frequencies(frequencies, device, width)
         if positions is not None:
             positions = check_positions(positions, (tokens,), device)
-        rotary = rotary_of(frequencies, positions, interleaved, float(magnitude))
     elif positions is not None:
         raise ValueError("positions without frequencies: nothing turns.")
-    described = _rows(q, turned) if q is not None and q.size(1) > 0 else None
+    args = (k, v, *where, frequencies, q, positions)
+    if _host.recorded(*args):
+        turned = [_append_operator(*args, bool(interleaved), float(magnitude))]
+    else:
+        turned = _append(*args, interleaved, float(magnitude))
+        increment_version((key_cache, value_cache))  # (what a kernel has written counts as written for autograd)
+    return None if q is None else turned[0]
+
+
+def _append(k, v, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, q, positions, interleaved, magnitude) -> list:
+    """The launch, on arguments that have been checked: ``q`` turned, if there is one."""
+    cache = _Cache(key_cache, value_cache, page_table, context_lengths, query_starts)
+    device = key_cache.device
+    turned = [] if q is None else [torch.empty(q.shape, dtype=q.dtype, device=device)]
+    rotary = None if frequencies is None else rotary_of(frequencies, positions, interleaved, magnitude)
+    described = _rows(q, turned[0]) if q is not None and q.size(1) > 0 else None
     by = lambda x: None if x is None else ctypes.byref(x)  # noqa: E731
     with _on(device):
         status = _lib.load().rlk_paged_append(
-            ctypes.byref(cache.c), by(rotary), by(described), by(_rows(k)), by(_rows(v)), tokens, _stream_handle(device)
+            ctypes.byref(cache.c), by(rotary), by(described), by(_rows(k)), by(_rows(v)), k.size(0), _stream_handle(device)
         )
     _lib.check(status, "rlk_paged_append failed")
-    increment_version((key_cache, value_cache))  # (what a kernel has written counts as written for autograd)
     return turned
+
+
+@torch.library.custom_op("rl_kernel::paged_append", mutates_args={"key_cache", "value_cache"})
+def _append_operator(
+    k: Tensor, v: Tensor, key_cache: Tensor, value_cache: Tensor, page_table: Tensor, context_lengths: Tensor, query_starts: Tensor,
+    frequencies: Optional[Tensor], q: Optional[Tensor], positions: Optional[Tensor], interleaved: bool, magnitude: float,
+) -> Tensor:  # fmt: skip
+    turned = _append(k, v, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, q, positions, interleaved, magnitude)
+    return turned[0] if turned else k.new_empty((0,))  # (a compiler wants tensors of an operator that writes)
+
+
+@_append_operator.register_fake
+def _append_operator_fake(
+    k, v, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, q, positions, interleaved, magnitude
+):
+    return k.new_empty((0,)) if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 
 def _on_16_bytes(t: Tensor) -> bool:
@@ -207,16 +233,18 @@ def paged_attention(
         if both is not None:
             return both if return_lse else both[0]
     _inference_only("paged_attention", q, key_cache, value_cache, out)
-    cache = _Cache(key_cache, value_cache, page_table, context_lengths, query_starts)
+    where = (key_cache, value_cache, page_table, context_lengths, query_starts)
+    _check_cache(*where)
     key_heads, width, device = key_cache.size(2), key_cache.size(3), key_cache.device
     q = _check_tokens(q, "q", key_cache)
     tokens, heads = q.shape[:2]
     scale = width**-0.5 if scale is None else float(scale)
+    recorded = _host.recorded(q, *where, out)  # (then there need not be addresses yet)
     enforce([
         (key_cache.dtype in (torch.bfloat16, torch.float16), TypeError, lambda: f"attention is served in bf16 and fp16, got {key_cache.dtype}."),
         (width % 8 == 0 and width <= _lib.ATTENTION_MAX_WIDTH, ValueError, lambda: f"heads must have a multiple of 8 elements, up to {_lib.ATTENTION_MAX_WIDTH}, got {width}."),
         (heads >= 1 and heads % key_heads == 0, ValueError, lambda: f"q must have a whole number of heads for each of the {key_heads} key heads, got {heads}."),
-        (_on_16_bytes(key_cache) and _on_16_bytes(value_cache), ValueError, "the rows of key_cache and value_cache must start on 16 bytes."),
+        (lambda: recorded or (_on_16_bytes(key_cache) and _on_16_bytes(value_cache)), ValueError, "the rows of key_cache and value_cache must start on 16 bytes."),
         (0.0 < scale < 3e38, ValueError, lambda: f"scale must be positive and finite, got {scale}."),
         (window is None or (isinstance(window, int) and not isinstance(window, bool) and window >= 1), ValueError, lambda: f"window must be a number of positions or None, got {window!r}."),
         (window is None or causal, ValueError, "a window goes with causal=True."),
@@ -232,30 +260,61 @@ def paged_attention(
             (lambda: tuple(out.shape) == tuple(q.shape), ValueError, lambda: f"out must have shape {tuple(q.shape)}, got {tuple(out.shape)}."),
             (lambda: out.dtype == q.dtype, TypeError, lambda: f"out must be {q.dtype}, got {out.dtype}."),
             (lambda: out.device == device, RuntimeError, lambda: f"out must be on {device}, got {out.device}."),
-            (lambda: out.stride(2) == 1 and _on_16_bytes(out), ValueError, "the heads of out must be contiguous and start on 16 bytes."),
+            (lambda: out.stride(2) == 1 and (recorded or _on_16_bytes(out)), ValueError, "the heads of out must be contiguous and start on 16 bytes."),
             (lambda: all(n <= 1 or stride > 0 for n, stride in zip(out.shape, out.stride())), ValueError, lambda: f"out must have memory of its own for every element, got strides {out.stride()}."),
         ])  # fmt: skip
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
-    if cache.c.sequences == 0:
+    if page_table.size(0) == 0:
         if given is None:
             out.zero_()
-        if lse is not None:
-            lse.fill_(-math.inf)
-    elif tokens > 0:
-        q = q if _on_16_bytes(q) else q.clone(memory_format=torch.contiguous_format)
-        lib, how = _lib.load(), _lib.ATTENTION_CONFIGS[config]
-        size = int(lib.rlk_paged_attention_workspace_bytes(ctypes.byref(cache.c), tokens, heads, window, how))
-        workspace = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
-        with _on(device):
-            status = lib.rlk_paged_attention(
-                ctypes.byref(cache.c), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                None if lse is None else lse.data_ptr(), tokens, heads, scale, int(causal), window, int(given is None), how,
-                None if workspace is None else workspace.data_ptr(), size, _stream_handle(device),
-            )  # fmt: skip
-        _lib.check(status, "rlk_paged_attention failed")
-        if given is not None:
-            increment_version(out)
+        lse = torch.full((tokens, heads), -math.inf, dtype=torch.float32, device=device)
+    elif tokens == 0:
+        lse = torch.empty((0, heads), dtype=torch.float32, device=device)
+    else:
+        args = (q, *where, out, scale, bool(causal), window, given is None, bool(return_lse), config)
+        if recorded:
+            lse = [_attention_operator(*args)]
+        else:
+            lse = _attend(*args)
+            if given is not None:
+                increment_version(out)
+        lse = lse[0] if return_lse else None
     return (out, lse) if return_lse else out
+
+
+def _attend(q, key_cache, value_cache, page_table, context_lengths, query_starts, out, scale, causal, window, zero_rest, with_lse, config) -> list:
+    """The launches, on arguments that have been checked: the logarithms, if they are wanted."""
+    cache = _Cache(key_cache, value_cache, page_table, context_lengths, query_starts)
+    tokens, heads = q.shape[:2]
+    device = key_cache.device
+    lse = [torch.empty((tokens, heads), dtype=torch.float32, device=device)] if with_lse else []
+    q = q if _on_16_bytes(q) else q.clone(memory_format=torch.contiguous_format)
+    lib, how = _lib.load(), _lib.ATTENTION_CONFIGS[config]
+    size = int(lib.rlk_paged_attention_workspace_bytes(ctypes.byref(cache.c), tokens, heads, window, how))
+    workspace = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+    with _on(device):
+        status = lib.rlk_paged_attention(
+            ctypes.byref(cache.c), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+            lse[0].data_ptr() if with_lse else None, tokens, heads, scale, int(causal), window, int(zero_rest), how,
+            None if workspace is None else workspace.data_ptr(), size, _stream_handle(device),
+        )  # fmt: skip
+    _lib.check(status, "rlk_paged_attention failed")
+    return lse
+
+
+@torch.library.custom_op("rl_kernel::paged_attention", mutates_args={"out"})
+def _attention_operator(
+    q: Tensor, key_cache: Tensor, value_cache: Tensor, page_table: Tensor, context_lengths: Tensor, query_starts: Tensor, out: Tensor,
+    scale: float, causal: bool, window: int, zero_rest: bool, with_lse: bool, config: str,
+) -> Tensor:  # fmt: skip
+    lse = _attend(q, key_cache, value_cache, page_table, context_lengths, query_starts, out, scale, causal, window, zero_rest, with_lse, config)
+    return lse[0] if with_lse else torch.empty((0,), dtype=torch.float32, device=q.device)
+
+
+@_attention_operator.register_fake
+def _attention_operator_fake(
+    q, key_cache, value_cache, page_table, context_lengths, query_starts, out, scale, causal, window, zero_rest, with_lse, config
+):
+    return torch.empty(q.shape[:2] if with_lse else (0,), dtype=torch.float32, device=q.device)
 
 
 def qwen3_attention_block(
@@ -295,6 +354,24 @@ def qwen3_attention_block(
         (lambda: qkv_weight.size(0) % width == 0 and qkv_weight.size(0) // width > 2 * key_heads, ValueError, lambda: f"qkv_weight must have (heads + {2 * key_heads}) * {width} rows, got {qkv_weight.size(0)}."),
         (isinstance(normed, Tensor) and normed.dim() == 2, ValueError, "normed must be [tokens, hidden]."),
     ])  # fmt: skip
+    tensors = (
+        residual, normed, qkv_weight, o_weight, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, next_norm_weight,
+        q_norm_weight, k_norm_weight, post_norm_weight, gate,
+    )  # fmt: skip
+    how = (bool(interleaved), float(magnitude), None if scale is None else float(scale), window, float(residual_scale), float(eps))
+    if _host.recorded(*tensors):
+        total, after = _block_operator(*tensors, *how)
+    else:
+        total, after = _block(*tensors, *how)
+    return total, None if next_norm_weight is None else after
+
+
+def _block(
+    residual, normed, qkv_weight, o_weight, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, next_norm_weight,
+    q_norm_weight, k_norm_weight, post_norm_weight, gate, interleaved, magnitude, scale, window, residual_scale, eps,
+) -> tuple[Tensor, Optional[Tensor]]:  # fmt: skip
+    """The block, operator by operator."""
+    key_heads, width = key_cache.shape[2:]
     heads = qkv_weight.size(0) // width - 2 * key_heads
     with torch.no_grad():
         qkv = det_gemm_linear(normed, qkv_weight)
@@ -309,6 +386,29 @@ def qwen3_attention_block(
         return gated_residual_norm(
             y, residual, next_norm_weight, post_weight=post_norm_weight, gate=gate, residual_scale=residual_scale, eps=eps
         )
+
+
+@torch.library.custom_op("rl_kernel::qwen3_attention_block", mutates_args={"key_cache", "value_cache"})
+def _block_operator(
+    residual: Tensor, normed: Tensor, qkv_weight: Tensor, o_weight: Tensor, key_cache: Tensor, value_cache: Tensor, page_table: Tensor,
+    context_lengths: Tensor, query_starts: Tensor, frequencies: Optional[Tensor], next_norm_weight: Optional[Tensor], q_norm_weight: Optional[Tensor],
+    k_norm_weight: Optional[Tensor], post_norm_weight: Optional[Tensor], gate: Optional[Tensor], interleaved: bool, magnitude: float,
+    scale: Optional[float], window: Optional[int], residual_scale: float, eps: float,
+) -> Tuple[Tensor, Tensor]:  # fmt: skip
+    total, after = _block(
+        residual, normed, qkv_weight, o_weight, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, next_norm_weight,
+        q_norm_weight, k_norm_weight, post_norm_weight, gate, interleaved, magnitude, scale, window, residual_scale, eps,
+    )  # fmt: skip
+    return total, normed.new_empty((0,)) if after is None else after
+
+
+@_block_operator.register_fake
+def _block_operator_fake(
+    residual, normed, qkv_weight, o_weight, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, next_norm_weight,
+    q_norm_weight, k_norm_weight, post_norm_weight, gate, interleaved, magnitude, scale, window, residual_scale, eps,
+):  # fmt: skip
+    after = normed.new_empty((0,)) if next_norm_weight is None else torch.empty(residual.shape, dtype=normed.dtype, device=normed.device)
+    return torch.empty(residual.shape, dtype=residual.dtype, device=residual.device), after
 
 
 __all__ = ["attention_contract_id", "paged_append", "paged_attention", "qwen3_attention_block"]

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional
+from typing import List, Optional
 
 import torch
 from torch import Tensor
@@ -94,6 +94,25 @@ def _head_rows(x: Tensor, y: Tensor) -> _lib.HeadRows:
 
 def _rotate(tensors: list, positions: Tensor, frequencies: Tensor, interleaved: bool, magnitude: float, inverse: bool) -> list:
     """``tensors`` (one or two) rotated, into new ones."""
+    if _host.recorded(*tensors, positions, frequencies):
+        return _rotate_operator(tensors[0], tensors[1] if len(tensors) > 1 else None, positions, frequencies, interleaved, magnitude, inverse)
+    return _launch(tensors, positions, frequencies, interleaved, magnitude, inverse)
+
+
+@torch.library.custom_op("rl_kernel::rotary_embedding", mutates_args=())
+def _rotate_operator(
+    q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Tensor, interleaved: bool, magnitude: float, inverse: bool
+) -> List[Tensor]:
+    _host.refuse_capture_into_another_graph()  # (in a compiler's backward)
+    return _launch([t for t in (q, k) if t is not None], positions, frequencies, interleaved, magnitude, inverse)
+
+
+@_rotate_operator.register_fake
+def _rotate_operator_fake(q, k, positions, frequencies, interleaved, magnitude, inverse):
+    return [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k) if t is not None]
+
+
+def _launch(tensors: list, positions: Tensor, frequencies: Tensor, interleaved: bool, magnitude: float, inverse: bool) -> list:
     device = tensors[0].device
     made, described, held = [], [], []
     for x in tensors:
@@ -137,7 +156,8 @@ def rotary_gradients(
 ) -> tuple[Optional[Tensor], Optional[Tensor]]:
     """The gradients of ``q`` and ``k`` from those of their turned forms, differentiable; ``None`` where there is none."""
     refuse_tangents("the gradient of a rotation", g_q, g_k)
-    _host.refuse_capture_into_another_graph()
+    if not torch.compiler.is_compiling():  # (the operator does it when it runs)
+        _host.refuse_capture_into_another_graph()
     given = [g for g in (g_q, g_k) if g is not None]
     if not given:
         return None, None

@@ -152,3 +152,135 @@ def test_caches_of_inference_mode(attention, way):
     assert same_bits(out, attention.paged_attention(b.q, *b.where))
     with torch.inference_mode():
         attention.paged_append(k, k, *b.where)
+
+
+# ---------------------------------------------------------------------------
+# Tracers and compilers: what they record computes on other inputs what the call does
+# ---------------------------------------------------------------------------
+
+
+def _fx(f, *args):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    return make_fx(f)(*args)
+
+
+def _fx_of_shapes(f, *args):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    return make_fx(f, tracing_mode="fake")(*args)
+
+
+def _jit(f, *args):
+    return torch.jit.trace(f, args, check_trace=False)
+
+
+def _compiled(f, *args):
+    return torch.compile(f, backend="aot_eager", fullgraph=True)
+
+
+RECORDERS = pytest.mark.parametrize("record", (_fx, _fx_of_shapes, _jit, _compiled))
+
+
+@RECORDERS
+def test_a_recorded_rotation(attention, record):
+    f, positions = attention.rotary_frequencies(32, device=DEV), torch.arange(9, device=DEV)
+    run = lambda q, k, p, f: attention.rotary_embedding(q, k, p, f)  # noqa: E731
+    recorded = record(run, _normal(9, 4, 48, seed=1), _normal(9, 2, 48, seed=2), positions, f)
+    q, k = _normal(9, 4, 48, seed=3), _normal(9, 2, 48, seed=4)
+    for got, want in zip(recorded(q, k, positions + 5, f), run(q, k, positions + 5, f)):
+        assert same_bits(got, want)
+
+
+@pytest.mark.parametrize("record", (_fx, _fx_of_shapes, _compiled))
+def test_a_recorded_gradient_of_a_rotation(attention, record):
+    f, positions = attention.rotary_frequencies(32, device=DEV), torch.arange(9, device=DEV)
+
+    def run(q, g, positions, f):
+        q = q.detach().requires_grad_()
+        return torch.autograd.grad(attention.rotary_embedding(q, None, positions, f, interleaved=True)[0], q, g)[0]
+
+    if record is _compiled:  # (a compiler takes the forward, its backward comes with it)
+        rotate = torch.compile(lambda q: attention.rotary_embedding(q, None, positions, f, interleaved=True)[0], backend="aot_eager", fullgraph=True)
+        q, g = _normal(9, 4, 48, seed=3).requires_grad_(), _normal(9, 4, 48, seed=4)
+        assert same_bits(torch.autograd.grad(rotate(q), q, g)[0], run(q, g, positions, f))
+        return
+    recorded = record(run, _normal(9, 4, 48, seed=1), _normal(9, 4, 48, seed=2), positions, f)
+    q, g = _normal(9, 4, 48, seed=3), _normal(9, 4, 48, seed=4)
+    assert same_bits(recorded(q, g, positions, f), run(q, g, positions, f))
+
+
+@RECORDERS
+def test_a_recorded_append_and_attention(attention, record):
+    f = attention.rotary_frequencies(64, device=DEV)
+
+    def run(f, q, k, v, keys, values, table, contexts, starts):
+        where = (keys, values, table, contexts, starts)
+        q = attention.paged_append(k, v, *where, f, q=q)
+        attention.paged_append(v, k, *where)  # (returns nothing: what it writes must not be dropped)
+        out = torch.zeros_like(q)
+        attention.paged_attention(q, *where, out=out)
+        return out, *attention.paged_attention(q, *where, return_lse=True, window=20)
+
+    def inputs(seed):
+        b = Batch([(3, 20), (1, 33)], 4, 2, 64, 16, BF16, seed=seed)
+        return b, (f, b.q, _normal(4, 2, 64, seed=seed + 1), _normal(4, 2, 64, seed=seed + 2), *b.where)
+
+    recorded = record(run, *inputs(1)[1])
+    b, args = inputs(10)
+    got = recorded(*args)
+    eager, args = inputs(10)
+    for g, w in zip(got, run(*args)):
+        assert same_bits(g, w)
+    assert same_bits(b.keys, eager.keys) and same_bits(b.values, eager.values)
+
+
+@RECORDERS
+def test_a_recorded_block(attention, record):
+    hidden = 128
+    weights = _normal(8 * 64, hidden, seed=1), _normal(hidden, 4 * 64, seed=2)
+    f, one, norm = attention.rotary_frequencies(64, device=DEV), torch.ones(64, device=DEV, dtype=BF16), torch.ones(hidden, device=DEV, dtype=BF16)
+
+    def run(residual, normed, qkv, o, f, one, norm, *where):
+        total, after = attention.qwen3_attention_block(residual, normed, qkv, o, *where, f, norm, q_norm_weight=one, window=16)
+        total, none = attention.qwen3_attention_block(total, after, qkv, o, *where, None)
+        assert none is None
+        return total, after
+
+    def inputs(seed):
+        b = Batch([(3, 20), (1, 33)], 4, 2, 64, 16, BF16, seed=seed)
+        return b, (_normal(4, hidden, seed=seed + 1), _normal(4, hidden, seed=seed + 2), *weights, f, one, norm, *b.where)
+
+    recorded = record(run, *inputs(1)[1])
+    b, args = inputs(10)
+    got = recorded(*args)
+    eager, args = inputs(10)
+    for g, w in zip(got, run(*args)):
+        assert same_bits(g, w)
+    assert same_bits(b.keys, eager.keys) and same_bits(b.values, eager.values)
+
+
+def test_a_profiler_and_a_mode_see_the_operators(attention):
+    b, f, k = Batch([(3, 20), (1, 33)], 4, 2, 64, 16, BF16), attention.rotary_frequencies(64, device=DEV), _normal(4, 2, 64, seed=1)
+
+    def run():
+        attention.rotary_embedding(b.q, None, torch.arange(4, device=DEV), f)
+        attention.paged_append(k, k, *b.where, f)
+        return attention.paged_attention(b.q, *b.where)
+
+    seen = []
+
+    class Mode(torch.utils._python_dispatch.TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    want = run()
+    with Mode():
+        assert same_bits(run(), want)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as profile:
+        run()
+    names = " ".join(seen), " ".join(e.key for e in profile.key_averages())
+    assert all(f"rl_kernel.{name}" in names[0] and f"rl_kernel::{name}" in names[1] for name in ("rotary_embedding", "paged_append", "paged_attention"))
+    for tensors in ((b.q.as_subclass(type("Sub", (torch.Tensor,), {})), *b.where), (torch.nn.Parameter(b.q, requires_grad=False), *b.where)):
+        assert same_bits(attention.paged_attention(*tensors).as_subclass(torch.Tensor), want)
