@@ -653,8 +653,11 @@ int rlk_paged_append(const rlk_paged_cache* host_cache, const rlk_rotary* host_r
  *
  * The order of a row's sums is a function of the positions it sees (contract rlk_attention_contract_id()), so its bits do not
  * depend on the batch, the chunk it came in, the page size or the configuration: keys in tiles of 64 positions, one chain of running
- * maximum (changed by more than 8 binary orders at a time), sum and output over the tiles of a run, and the runs (of 256 positions up to 4096, of 512 up to 16384, of 1024 up to
- * 65536, of 2048 behind) combined in ascending order.
+ * maximum (changed by more than 8 binary orders at a time), sum and output over the tiles of a run, and the runs (of 256 positions up
+ * to 4096, of 512 up to 16384, of 1024 up to 65536, of 2048 behind) combined in ascending order.
+ *
+ * The workspace is sized by the table's width, or the window where that has fewer runs: 1 GiB at most, but for a configuration that
+ * asks for SPLIT where a single key head has more.
  */
 typedef enum rlk_attention_config {
   RLK_ATTENTION_CFG_AUTO = 0,

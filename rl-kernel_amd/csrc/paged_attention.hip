@@ -39,6 +39,7 @@ constexpr int kMostKeys = 0x7fffff00;  // of a sequence: positions behind have n
 
 // Runs: their lengths grow with the position, so that a short context still has enough of them for the chip and a long
 // one's partial results stay few (of 8 rows a part is 1/32 of the keys and values that a run of 256 reads, 1/256 of 2048). Tiles 0 ... 63 in fours, ... 255 in eights, ... 1023 in sixteens, then 32 at a time.
+constexpr int kFirstRunTiles = 4;
 __host__ __device__ __forceinline__ int run_of_tile(int t) {
   return t < 64 ? t >> 2 : t < 256 ? 16 + ((t - 64) >> 3) : t < 1024 ? 40 + ((t - 256) >> 4) : 88 + ((t - 1024) >> 5);
 }
@@ -58,13 +59,13 @@ struct AttentionArgs {
   const char* q;
   char* out;
   float* lse;
-  float* part_out;  // [run][token][head][width]
+  float* part_out;  // [run of those that a row sees][token][head][width]
   float* part_max;  // [run][token][head]
   float* part_sum;
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
   int64_t part_rows;  // tokens * heads
   PageDivider by_page, by_group, by_key_heads, by_chunks;
-  int tokens, heads, group, causal, window, zero_rest, longest_first, tiles, chunks;
+  int tokens, heads, lse_heads, group, causal, window, zero_rest, longest_first, tiles, chunks;  // (lse_heads: of a row of lse)
   float scale;  // times log2(e)
 };
 
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
           for (int i = tid; i < a.group * each; i += WAVES * 64) {
             const int head = key_head * a.group + i / each;
             *reinterpret_cast<u32x4_t*>(a.out + t * a.out_token_stride + head * a.out_head_stride + (i % each) * 16) = u32x4_t{0, 0, 0, 0};
-            if (a.lse && i % each == 0) a.lse[(int64_t)t * a.heads + head] = -INFINITY;
+            if (a.lse && i % each == 0) a.lse[(int64_t)t * a.lse_heads + head] = -INFINITY;
           }
         }
       }
@@ -683,8 +684,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
     const float sum = sum_over_halves(its_l);
     if (SPLIT) {
       const RowPlace r = row_place();
-      if (r.live) {
-        const int64_t at = (int64_t)run * a.part_rows + (int64_t)r.token * a.heads + r.head;
+      const int its_first = run_of_tile(st.sight.low / kTileKeys), its_last = run_of_tile((min(st.sight.high, capacity + 1) - 1) / kTileKeys);
+      if (r.live && run >= its_first && run <= its_last) {
+        const int64_t at = (int64_t)(run - its_first) * a.part_rows + (int64_t)r.token * a.heads + r.head;
         if (half == 0) a.part_max[at] = its_m, a.part_sum[at] = sum;
 #pragma unroll
         for (int d = 0; d < State::kBlocks; ++d)
@@ -855,7 +857,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
       const int element = 32 * d + 2 * i + 4 * half;
       if (element < a.cache.width) *reinterpret_cast<u32x2_t*>(to + 2 * element) = u32x2_t{H::pack(y[0], y[1]), H::pack(y[2], y[3])};
     }
-  if (a.lse && half == 0) a.lse[(int64_t)r.token * a.heads + r.head] = behind ? NAN : any ? lse_of(all_m, all_l) : -INFINITY;
+  if (a.lse && half == 0) a.lse[(int64_t)r.token * a.lse_heads + r.head] = behind ? NAN : any ? lse_of(all_m, all_l) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -884,8 +886,8 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
   const int high = min(sight.high, capacity + 1);
   if (sight.low < high) {
     const int first = run_of_tile(sight.low / kTileKeys), last = run_of_tile((high - 1) / kTileKeys);
-    for (int r0 = first; r0 <= last; r0 += kJoinRuns) {
-      const int count = min(kJoinRuns, last + 1 - r0);
+    for (int r0 = 0; r0 <= last - first; r0 += kJoinRuns) {
+      const int count = min(kJoinRuns, last - first + 1 - r0);
       __syncthreads();
       if (tid < count) run_max[tid] = a.part_max[(r0 + tid) * a.part_rows + row], run_sum[tid] = a.part_sum[(r0 + tid) * a.part_rows + row];
       __syncthreads();
@@ -909,7 +911,7 @@ __global__ __launch_bounds__(kMaxWidth) void attention_join_kernel(const Attenti
   const bool sees = sight.high > sight.low, behind = sight.high > capacity;
   const float y = behind ? NAN : sees ? output_of(o, 1.f / sum) : 0.f;
   if (tid < width) *reinterpret_cast<uint16_t*>(out) = (uint16_t)Half<DTYPE>::pack(y, 0.f);
-  if (a.lse && tid == 0) a.lse[row] = behind ? NAN : sees ? lse_of(top, sum) : -INFINITY;
+  if (a.lse && tid == 0) a.lse[(int64_t)token * a.lse_heads + head] = behind ? NAN : sees ? lse_of(top, sum) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -921,11 +923,25 @@ struct AttentionPlan {
   bool split;  // runs side by side
   bool longest_first;  // of the sequences
   int chunks, tiles;
+  int key_heads;  // of a launch
 };
 
-static int run_limit(const rlk_paged_cache& c) {
-  return run_of_tile(capacity_of(c) / kTileKeys) + 1;  // (with the position behind the table)
+// The most runs that a row sees: those of the table (with the position behind it), or of a window's tiles, which touch most runs where
+// these are shortest and the first tile is the last one of a run.
+static int run_limit(const rlk_paged_cache& c, int window) {
+  const int all = run_of_tile(capacity_of(c) / kTileKeys) + 1;
+  if (window == 0) return all;
+  const int tiles = (int)(((int64_t)window + kTileKeys - 2) / kTileKeys) + 1, of_window = run_of_tile(kFirstRunTiles - 1 + tiles - 1) + 1;
+  return of_window < all ? of_window : all;
 }
+static size_t parts_bytes(const rlk_paged_cache& c, int64_t tokens, int heads, int window) {
+  return (size_t)run_limit(c, window) * tokens * heads * (c.width + 2) * sizeof(float);
+}
+// Parts take no more memory than this: a call that has more goes through its key heads in several launches, each of which fills the chip, and
+// where a single key head has more, all runs go one after the other. In one launch / several / one after the other, us (32 heads, 8 key heads of
+// 128, a table of 2^20 positions): 512 tokens over 2^20 10600 with 5.1 GB / 12000 with 1 / 20700, over 131072 1550 / 1810 / 2650; with a table
+// of 131072, 100 sequences of 8 tokens 11640 with 1.6 GB / 10370 / 8830, 127 of 16 over 30000 3890 with 4.1 GB / 3180 / 2400.
+constexpr size_t kMostParts = (size_t)1 << 30;
 
 static bool pages_of_groups(const rlk_paged_cache& c) {
   const int64_t most = kSoloRange / 16;  // elements between rows: eight of them stay within a buffer's range
@@ -948,8 +964,9 @@ static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, in
   const int choice = config & 0xff;
   const int64_t each = (tokens + c.sequences - 1) / c.sequences * group;  // rows of a sequence and key head
   const int64_t cus = device_cu_count();
-  const int runs = run_limit(c);
-  auto side_by_side = [&](int rows) { return (int64_t)c.sequences * ((each + rows - 1) / rows) * c.key_heads; };
+  const int runs = run_limit(c, 0);
+  p.key_heads = c.key_heads;
+  auto side_by_side = [&](int rows) { return (int64_t)c.sequences * ((each + rows - 1) / rows) * p.key_heads; };
   const int64_t seen = window > 0 ? window + tokens / c.sequences : kMostKeys;
   const int64_t depth = (seen < capacity_of(c) ? seen : capacity_of(c)) / kTileKeys + 1;  // tiles that a row tile goes through
   if (choice != RLK_ATTENTION_CFG_AUTO) {
@@ -962,6 +979,15 @@ static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, in
     p.split = p.rows == 64 ? (units < cus && depth > 8) || (units < 4 * cus && depth >= 64) : 4 * units < 3 * cus && depth >= 32;
   }
   if (p.rows > most || !pages_of_groups(c)) p.rows = 128;
+  const size_t of_key_head = parts_bytes(c, tokens, group, window);
+  if (p.split && of_key_head * c.key_heads > kMostParts) {
+    if (of_key_head > kMostParts && choice == RLK_ATTENTION_CFG_AUTO) {
+      p.split = false;
+    } else {
+      const int at_once = of_key_head > kMostParts ? 1 : (int)(kMostParts / of_key_head), launches = (c.key_heads + at_once - 1) / at_once;
+      p.key_heads = (c.key_heads + launches - 1) / launches;
+    }
+  }
   p.tiles = (int)(tokens * group / p.rows) + c.sequences + 1;
   p.chunks = 1;
   if (p.split) {
@@ -974,8 +1000,8 @@ static AttentionPlan attention_plan(const rlk_paged_cache& c, int64_t tokens, in
 
 size_t paged_attention_workspace_bytes(const rlk_paged_cache& c, int64_t tokens, int heads, int window, int config) {
   if (tokens == 0 || c.sequences == 0 || heads == 0) return 0;
-  if (!attention_plan(c, tokens, heads, window, config).split) return 0;
-  return (size_t)run_limit(c) * tokens * heads * (c.width + 2) * sizeof(float);
+  const AttentionPlan p = attention_plan(c, tokens, heads, window, config);
+  return p.split ? parts_bytes(c, tokens, heads / c.key_heads * p.key_heads, window) : 0;
 }
 
 template <int DTYPE, int SLABS, int WAVES, bool SPLIT, bool GROUPED>
@@ -1020,29 +1046,38 @@ hipError_t paged_attention_launch(const rlk_paged_cache& cache, const void* q, i
   const AttentionPlan p = attention_plan(cache, tokens, heads, window, config);
   AttentionArgs a{};
   a.cache = cache;
-  a.q = static_cast<const char*>(q);
-  a.out = static_cast<char*>(out);
-  a.lse = lse;
   a.q_token_stride = 2 * q_token_stride, a.q_head_stride = 2 * q_head_stride;
   a.out_token_stride = 2 * out_token_stride, a.out_head_stride = 2 * out_head_stride;
-  a.part_rows = tokens * heads;
-  if (p.split) {
-    const int64_t parts = run_limit(cache) * a.part_rows;
-    a.part_out = static_cast<float*>(workspace);
-    a.part_max = a.part_out + parts * cache.width;
-    a.part_sum = a.part_max + parts;
-  }
   a.group = heads / cache.key_heads;
   a.by_page = page_divider((uint32_t)cache.page_size);
   a.by_group = page_divider((uint32_t)a.group);
-  a.by_key_heads = page_divider((uint32_t)cache.key_heads);
   a.tokens = (int)tokens;
-  a.heads = heads;
+  a.lse_heads = heads;
   a.causal = causal, a.window = window, a.zero_rest = zero_rest;
   a.tiles = p.tiles, a.by_chunks = page_divider((uint32_t)p.chunks);
   a.chunks = p.chunks, a.longest_first = p.longest_first;
   a.scale = (float)((double)scale * 1.4426950408889634074);
-  return cache.dtype == RLK_DTYPE_BF16 ? attention_launch_as<RLK_DTYPE_BF16>(a, p, stream) : attention_launch_as<RLK_DTYPE_FP16>(a, p, stream);
+  for (int first = 0; first < cache.key_heads; first += p.key_heads) {
+    const int count = cache.key_heads - first < p.key_heads ? cache.key_heads - first : p.key_heads;
+    a.cache.keys = static_cast<char*>(cache.keys) + 2 * first * cache.key_head_stride;
+    a.cache.values = static_cast<char*>(cache.values) + 2 * first * cache.value_head_stride;
+    a.cache.key_heads = count;
+    a.q = static_cast<const char*>(q) + first * a.group * a.q_head_stride;
+    a.out = static_cast<char*>(out) + first * a.group * a.out_head_stride;
+    a.lse = lse != nullptr ? lse + first * a.group : nullptr;
+    a.heads = count * a.group;
+    a.by_key_heads = page_divider((uint32_t)count);
+    a.part_rows = tokens * a.heads;
+    if (p.split) {
+      const int64_t parts = run_limit(cache, window) * a.part_rows;
+      a.part_out = static_cast<float*>(workspace);
+      a.part_max = a.part_out + parts * cache.width;
+      a.part_sum = a.part_max + parts;
+    }
+    const hipError_t err = cache.dtype == RLK_DTYPE_BF16 ? attention_launch_as<RLK_DTYPE_BF16>(a, p, stream) : attention_launch_as<RLK_DTYPE_FP16>(a, p, stream);
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
 }
 
 }  // namespace rlk

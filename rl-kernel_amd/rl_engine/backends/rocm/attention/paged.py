@@ -223,8 +223,8 @@ def paged_attention(
 
     A row's bits depend on its query and on the keys, values and positions that it sees: a prompt that comes in chunks, next to
     other sequences or token by token has the same results (:func:`attention_contract_id` names the order of the sums). ``config`` names the
-    kernel that runs and never changes them. A call is sized by the width of ``page_table``: pass ``page_table[:, :n]`` where the longest
-    context is known. No gradient: tensors that require one are refused.
+    kernel that runs and never changes them. A call is sized by the width of ``page_table`` (and the window), its temporary memory too, which is
+    1 GiB at most: pass ``page_table[:, :n]`` where the longest context is known. No gradient: tensors that require one are refused.
     """
     if out is None and config == "auto" and isinstance(q, Tensor) and q.is_cuda and not torch.compiler.is_compiling():
         both = _host.native().paged_attention(  # everyday arguments, natively

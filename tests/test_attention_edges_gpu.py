@@ -104,6 +104,25 @@ def test_the_last_positions(attention, config):
     assert bool(out.isnan().all()) and bool(lse.isnan().all())
 
 
+@pytest.mark.parametrize("heads, key_heads, width", [(32, 8, 64), (24, 3, 72), (32, 1, 64)])
+@pytest.mark.parametrize("window", (None, 900))
+def test_a_table_so_wide_that_the_parts_do_not_fit_at_once(attention, heads, key_heads, width, window):
+    """Without a window the key heads take several launches, or, where one of them has too many parts, all runs go one after the other."""
+    b = Batch([(700, 5000)], heads, key_heads, width, 16, BF16, seed=8)
+    table = torch.full((1, 2**16), -1, device=DEV, dtype=torch.int32)
+    table[:, : b.table.size(1)] = b.table
+    want, want_lse = attention.paged_attention(b.q, *b.where, window=window, return_lse=True, config="rows128")
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    out, lse = attention.paged_attention(b.q, b.keys, b.values, table, b.contexts, b.starts, window=window, return_lse=True)
+    assert same_bits(out, want) and same_bits(lse, want_lse)
+    assert torch.cuda.max_memory_allocated() - held <= 2**30 + 2**26
+    given = torch.zeros((700, heads + 2, width), device=DEV, dtype=BF16)
+    attention.paged_attention(b.q, b.keys, b.values, table, b.contexts, b.starts, window=window, out=given[:, 1:-1])
+    assert same_bits(given[:, 1:-1], want) and not bool(given[:, 0].any()) and not bool(given[:, -1].any())
+
+
 class _Nothing:
     def __getattr__(self, name):
         return lambda *args: None
