@@ -647,9 +647,9 @@ int rlk_paged_append(const rlk_paged_cache* host_cache, const rlk_rotary* host_r
  * over the keys j that a row sees: of a token at position p those up to p (causal), of them the last `window` ones (0: all), or the
  * whole context (not causal; window 0). q head h reads key head h / (heads / key_heads). A row that sees no key is 0, its lse -inf. What a row does not
  * see does not reach it, whatever it holds. lse (optional, [tokens, heads]) is the natural logarithm of the sum of exponentials.
- * bf16 or fp16; width a multiple of 8 up to 256; rows of q, keys and values start on 16 bytes; pages and rows of the cache lie less than
- * 2^31 elements apart. Rows of out behind the last sequence
- * are left as they were, or become zeros with zero_rest.
+ * bf16 or fp16; scale above 0, up to 2.3e38; width a multiple of 8 up to 256; rows of q, keys and values start on 16 bytes; pages and
+ * rows of the cache lie less than 2^31 elements apart. Rows of out behind the last sequence are left as they were, or become zeros with
+ * zero_rest.
  *
  * The order of a row's sums is a function of the positions it sees (contract rlk_attention_contract_id()), so its bits do not
  * depend on the batch, the chunk it came in, the page size or the configuration: keys in tiles of 64 positions, one chain of running

@@ -939,7 +939,7 @@ static size_t parts_bytes(const rlk_paged_cache& c, int64_t tokens, int heads, i
 }
 // Parts take no more memory than this: a call that has more goes through its key heads in several launches, each of which fills the chip, and
 // where a single key head has more, all runs go one after the other. In one launch / several / one after the other, us (32 heads, 8 key heads of
-// 128, a table of 2^20 positions): 512 tokens over 2^20 10600 with 5.1 GB / 12000 with 1 / 20700, over 131072 1550 / 1810 / 2650; with a table
+// 128, a table of 2^20 positions): 512 tokens over 2^20 10600 with 4.8 GB / 12000 with 0.6 / 20700, over 131072 1550 / 1810 / 2650; with a table
 // of 131072, 100 sequences of 8 tokens 11640 with 1.6 GB / 10370 / 8830, 127 of 16 over 30000 3890 with 4.1 GB / 3180 / 2400.
 constexpr size_t kMostParts = (size_t)1 << 30;
 

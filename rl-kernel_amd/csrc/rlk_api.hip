@@ -1014,7 +1014,7 @@ int rlk_paged_attention(const rlk_paged_cache* cache, const void* q, int64_t q_t
   const char* who = "rlk_paged_attention";
   const int rc = check_attention(who, cache, tokens, heads, config);
   if (rc != RLK_OK || tokens == 0) return rc;
-  if (!(scale > 0.f) || scale > 3.0e38f) return refuse_argument(who, "scale is not a positive finite number");
+  if (!(scale > 0.f) || scale > 2.3e38f) return refuse_argument(who, "scale is not a positive number up to 2.3e38 (finite in units of log2)");
   if (window < 0 || (window > 0 && !causal)) return refuse_argument(who, "a window is positive, or 0 for none, and goes with causal");
   if (!q || !out || q_token_stride < 0 || q_head_stride < 0 || out_token_stride < 0 || out_head_stride < 0) return refuse_argument(who, "null operand or negative stride");
   auto on16 = [](const void* base, int64_t a, int64_t b, int64_t c) { return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && a % 8 == 0 && b % 8 == 0 && c % 8 == 0; };

@@ -1296,7 +1296,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t count)
   }
   const int64_t width = q.size(2), heads = q.size(1), key_heads = cache.keys.size(2);
   if (args[6] == Py_None) scale = std::pow((double)width, -0.5);
-  if (!(scale > 0.0 && scale < 3e38) || width % 8 != 0 || heads % key_heads != 0) return none();
+  if (!(scale > 0.0 && scale <= 2.3e38) || width % 8 != 0 || heads % key_heads != 0) return none();
   auto on_16_bytes = [](const Tensor& t) {
     bool on = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
     for (int64_t i = 0; i + 1 < t.dim(); ++i) on = on && t.stride(i) % 8 == 0;

@@ -245,7 +245,7 @@ def paged_attention(
         (width % 8 == 0 and width <= _lib.ATTENTION_MAX_WIDTH, ValueError, lambda: f"heads must have a multiple of 8 elements, up to {_lib.ATTENTION_MAX_WIDTH}, got {width}."),
         (heads >= 1 and heads % key_heads == 0, ValueError, lambda: f"q must have a whole number of heads for each of the {key_heads} key heads, got {heads}."),
         (lambda: recorded or (_on_16_bytes(key_cache) and _on_16_bytes(value_cache)), ValueError, "the rows of key_cache and value_cache must start on 16 bytes."),
-        (0.0 < scale < 3e38, ValueError, lambda: f"scale must be positive and finite, got {scale}."),
+        (0.0 < scale <= 2.3e38, ValueError, lambda: f"scale must be positive and at most 2.3e38 (finite in units of log2), got {scale}."),
         (window is None or (isinstance(window, int) and not isinstance(window, bool) and window >= 1), ValueError, lambda: f"window must be a number of positions or None, got {window!r}."),
         (window is None or causal, ValueError, "a window goes with causal=True."),
         (config in _lib.ATTENTION_CONFIGS, ValueError, lambda: f"config must be one of {tuple(_lib.ATTENTION_CONFIGS)}, got {config!r}."),
