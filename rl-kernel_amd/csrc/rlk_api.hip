@@ -989,6 +989,7 @@ const char* rlk_attention_contract_id(void) { return "rlkernel.paged_attention.h
 static int check_attention(const char* who, const rlk_paged_cache* c, int64_t tokens, int heads, int config) {
   int rc = check_paged_cache(who, c, tokens, heads);
   if (rc != RLK_OK) return rc;
+  if (tokens * heads > 0x7ffffc00) return refuse_argument(who, "sizes out of range");  // (the tiles behind the last row have 32-bit numbers too)
   if (c->dtype != RLK_DTYPE_BF16 && c->dtype != RLK_DTYPE_FP16) return refuse_argument(who, "dtype is neither bf16 nor fp16");
   if (heads < 1 || heads % c->key_heads != 0) return refuse_argument(who, "heads are no whole number of key heads");
   if (c->width % 8 != 0 || c->width > 256) return refuse_argument(who, "width is no multiple of 8 up to 256");

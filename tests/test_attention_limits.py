@@ -30,3 +30,11 @@ def test_the_largest_scale():
     for config in ("auto", "rows64"):
         with pytest.raises(ValueError, match="scale"):
             attention.paged_attention(new(3, 2, 64), *where, scale=2.4e38, config=config)
+
+
+def test_rows_whose_numbers_do_not_fit(rlk_lib):
+    """A row tile's first number and the next tile's are 32-bit numbers: two tiles of 256 rows above the last row must still fit."""
+    one = lambda: _cache(key_heads=1, width=8, key_row_stride=8)  # noqa: E731
+    for tokens, heads in ((2**31 - 1000, 1), (2**30 - 500, 2), (2**31 - 2, 1)):
+        _refused(rlk_lib, _attention(rlk_lib, cache=one(), strides=(8, 8), tokens=tokens, heads=heads), "range")
+        assert rlk_lib.rlk_paged_attention_workspace_bytes(one(), tokens, heads, 0, 0x101) == 0
