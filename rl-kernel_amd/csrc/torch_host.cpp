@@ -814,6 +814,7 @@ rlk_head_rows head_rows(const Tensor& x, const Tensor& y) {
   return r;
 }
 bool everyday_frequencies(const Tensor& f, const Tensor& beside) {
+  if (f.defined() && f.requires_grad() && at::GradMode::is_enabled()) return false;  // (refused)
   return everyday(f, at::kDouble, beside) && f.dim() == 1 && f.is_contiguous() && 2 * f.size(0) <= beside.size(-1);
 }
 bool everyday_positions(const Tensor& p, const Tensor& beside, at::IntArrayRef shape) {

@@ -33,7 +33,7 @@ def attention_contract_id() -> str:
 
 def _inference_only(who: str, *tensors: Optional[Tensor]) -> None:
     refuse_tangents(who, *tensors)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in tensors):
         raise RuntimeError(f"{who} has no gradient: call it under torch.no_grad(), or with tensors that require none.")
 
 
@@ -133,7 +133,7 @@ def paged_append(
         )
         if done is not None:
             return done[0]
-    _inference_only("paged_append", k, v, q, key_cache, value_cache)
+    _inference_only("paged_append", k, v, q, key_cache, value_cache, frequencies)
     where = (key_cache, value_cache, page_table, context_lengths, query_starts)
     _check_cache(*where)
     heads, width, device = key_cache.size(2), key_cache.size(3), key_cache.device
@@ -346,7 +346,10 @@ def qwen3_attention_block(
     :func:`paged_append`, :func:`paged_attention` and ``o_weight [hidden, heads * width]``, and what stands behind it
     (``ops.norm.gated_residual_norm``). Returns the new residual stream and its norm with ``next_norm_weight``, which the FFN block
     (``ops.ffn.qwen3_ffn_block``) takes. A token's bits do not depend on what else is in the batch or on the chunk that it came in."""
-    _inference_only("qwen3_attention_block", residual, normed, qkv_weight, o_weight, q_norm_weight, k_norm_weight, next_norm_weight, post_norm_weight, gate)
+    _inference_only(
+        "qwen3_attention_block", residual, normed, qkv_weight, o_weight, key_cache, value_cache, frequencies, q_norm_weight, k_norm_weight, next_norm_weight,
+        post_norm_weight, gate,
+    )  # fmt: skip
     _check_cache(key_cache, value_cache, page_table, context_lengths, query_starts)
     key_heads, width = key_cache.shape[2:]
     enforce([

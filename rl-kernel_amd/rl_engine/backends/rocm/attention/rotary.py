@@ -169,6 +169,7 @@ def check_frequencies(frequencies: Tensor, device: torch.device, width: int) -> 
     enforce([
         (isinstance(frequencies, Tensor), TypeError, lambda: f"frequencies must be a torch.Tensor, got {type(frequencies)!r}."),
         (lambda: frequencies.dtype == torch.float64, TypeError, lambda: f"frequencies must be fp64 (rotary_frequencies makes them), got {frequencies.dtype}."),
+        (lambda: not (torch.is_grad_enabled() and frequencies.requires_grad), RuntimeError, "frequencies have no gradient: pass frequencies.detach()."),
         (lambda: frequencies.device == device, RuntimeError, lambda: f"frequencies must be on {device}, got {frequencies.device}."),
         (lambda: frequencies.dim() == 1 and 2 * frequencies.numel() <= width, ValueError, lambda: f"frequencies must be [pairs] with at most {width // 2} of them, got shape {tuple(frequencies.shape)}."),
     ])  # fmt: skip
@@ -198,7 +199,8 @@ def _check_heads(t: Tensor, name: str) -> None:
 def rotary_embedding(
     q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Tensor, *, interleaved: bool = False, magnitude: float = 1.0
 ) -> tuple[Tensor, Optional[Tensor]]:
-    """``q`` and ``k`` (or ``None``) turned by their positions, as new contiguous tensors; differentiable in both, to any order.
+    """``q`` and ``k`` (or ``None``) turned by their positions, as new contiguous tensors; differentiable in both, to any order (not in the
+    frequencies: some that require a gradient are refused).
 
     ``q [..., heads, width]`` and ``k [..., key heads, width]`` are bf16, fp16 or fp32, of any strides, ``positions [...]`` int32 or int64,
     ``frequencies [pairs]`` fp64 (:func:`rotary_frequencies`). The first ``2 * pairs`` elements of a head are turned, the others copied. Pair i is
@@ -212,7 +214,7 @@ def rotary_embedding(
         both = _host.native().rotary(q, k, positions, frequencies, interleaved, magnitude)  # everyday arguments, natively
         if both is not None:
             return both
-    refuse_tangents("rotary_embedding", q, k)
+    refuse_tangents("rotary_embedding", q, k, frequencies)
     _check_heads(q, "q")
     if k is not None:
         _check_heads(k, "k")

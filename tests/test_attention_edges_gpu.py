@@ -303,3 +303,30 @@ def test_a_profiler_and_a_mode_see_the_operators(attention):
     assert all(f"rl_kernel.{name}" in names[0] and f"rl_kernel::{name}" in names[1] for name in ("rotary_embedding", "paged_append", "paged_attention"))
     for tensors in ((b.q.as_subclass(type("Sub", (torch.Tensor,), {})), *b.where), (torch.nn.Parameter(b.q, requires_grad=False), *b.where)):
         assert same_bits(attention.paged_attention(*tensors).as_subclass(torch.Tensor), want)
+
+
+def test_frequencies_that_want_a_gradient_are_refused(attention, way):
+    b = Batch([(2, 40), (1, 33)], 4, 2, 64, 16, BF16, seed=5)
+    k, positions = _normal(3, 2, 64, seed=6), torch.arange(3, device=DEV)
+    f = attention.rotary_frequencies(64, device=DEV)
+    asks = f.clone().requires_grad_()
+    weights = _normal(8 * 64, 128, seed=1), _normal(128, 4 * 64, seed=2)
+    x = _normal(3, 128, seed=7)
+    keys = b.keys.clone()
+    calls = (
+        lambda f: attention.rotary_embedding(b.q, k, positions, f)[0], lambda f: attention.paged_append(k, k, *b.where, f, q=b.q),
+        lambda f: attention.rotary_embedding(b.q.clone().requires_grad_(), None, positions, f)[0].detach(),
+        lambda f: attention.qwen3_attention_block(x, x, *weights, *b.where, f)[0],
+    )  # fmt: skip
+    for call in calls:
+        with pytest.raises(RuntimeError, match="gradient"):
+            call(asks)
+        assert same_bits(b.keys, keys)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(f, torch.ones_like(f))
+        for call in calls[:2]:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+    with torch.no_grad():
+        for call in calls:
+            assert same_bits(call(asks), call(f))
