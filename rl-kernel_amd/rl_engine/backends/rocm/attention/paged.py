@@ -23,7 +23,7 @@ from rl_engine._C import _on, _stream_handle
 from rl_engine._checks import enforce, refuse_tangents
 from rl_engine.backends.rocm.attention.rotary import _DTYPES, check_frequencies, check_positions, rotary_of
 from rl_engine.backends.rocm.gemm.det_gemm import det_gemm_linear
-from rl_engine.backends.rocm.norm.block_norm import gated_residual_norm, rms_norm
+from rl_engine.backends.rocm.norm.block_norm import check_block_norm, gated_residual_norm, rms_norm
 
 
 def attention_contract_id() -> str:
@@ -195,6 +195,20 @@ def _on_16_bytes(t: Tensor) -> bool:
     return t.data_ptr() % 16 == 0 and all(stride % 8 == 0 for stride in t.stride()[:-1])
 
 
+def _check_attention(key_cache: Tensor, value_cache: Tensor, heads: int, scale: float, causal: bool, window: Optional[int], config: str, recorded: bool) -> None:
+    key_heads, width = key_cache.shape[2:]
+    enforce([
+        (key_cache.dtype in (torch.bfloat16, torch.float16), TypeError, lambda: f"attention is served in bf16 and fp16, got {key_cache.dtype}."),
+        (width % 8 == 0 and width <= _lib.ATTENTION_MAX_WIDTH, ValueError, lambda: f"heads must have a multiple of 8 elements, up to {_lib.ATTENTION_MAX_WIDTH}, got {width}."),
+        (heads >= 1 and heads % key_heads == 0, ValueError, lambda: f"q must have a whole number of heads for each of the {key_heads} key heads, got {heads}."),
+        (lambda: recorded or (_on_16_bytes(key_cache) and _on_16_bytes(value_cache)), ValueError, "the rows of key_cache and value_cache must start on 16 bytes."),
+        (0.0 < scale <= 2.3e38, ValueError, lambda: f"scale must be positive and at most 2.3e38 (finite in units of log2), got {scale}."),
+        (window is None or (isinstance(window, int) and not isinstance(window, bool) and window >= 1), ValueError, lambda: f"window must be a number of positions or None, got {window!r}."),
+        (window is None or causal, ValueError, "a window goes with causal=True."),
+        (config in _lib.ATTENTION_CONFIGS, ValueError, lambda: f"config must be one of {tuple(_lib.ATTENTION_CONFIGS)}, got {config!r}."),
+    ])  # fmt: skip
+
+
 def paged_attention(
     q: Tensor,
     key_cache: Tensor,
@@ -235,21 +249,12 @@ def paged_attention(
     _inference_only("paged_attention", q, key_cache, value_cache, out)
     where = (key_cache, value_cache, page_table, context_lengths, query_starts)
     _check_cache(*where)
-    key_heads, width, device = key_cache.size(2), key_cache.size(3), key_cache.device
+    width, device = key_cache.size(3), key_cache.device
     q = _check_tokens(q, "q", key_cache)
     tokens, heads = q.shape[:2]
     scale = width**-0.5 if scale is None else float(scale)
     recorded = _host.recorded(q, *where, out)  # (then there need not be addresses yet)
-    enforce([
-        (key_cache.dtype in (torch.bfloat16, torch.float16), TypeError, lambda: f"attention is served in bf16 and fp16, got {key_cache.dtype}."),
-        (width % 8 == 0 and width <= _lib.ATTENTION_MAX_WIDTH, ValueError, lambda: f"heads must have a multiple of 8 elements, up to {_lib.ATTENTION_MAX_WIDTH}, got {width}."),
-        (heads >= 1 and heads % key_heads == 0, ValueError, lambda: f"q must have a whole number of heads for each of the {key_heads} key heads, got {heads}."),
-        (lambda: recorded or (_on_16_bytes(key_cache) and _on_16_bytes(value_cache)), ValueError, "the rows of key_cache and value_cache must start on 16 bytes."),
-        (0.0 < scale <= 2.3e38, ValueError, lambda: f"scale must be positive and at most 2.3e38 (finite in units of log2), got {scale}."),
-        (window is None or (isinstance(window, int) and not isinstance(window, bool) and window >= 1), ValueError, lambda: f"window must be a number of positions or None, got {window!r}."),
-        (window is None or causal, ValueError, "a window goes with causal=True."),
-        (config in _lib.ATTENTION_CONFIGS, ValueError, lambda: f"config must be one of {tuple(_lib.ATTENTION_CONFIGS)}, got {config!r}."),
-    ])  # fmt: skip
+    _check_attention(key_cache, value_cache, heads, scale, causal, window, config, recorded)
     window = 0 if window is None else min(window, 2**31 - 1)  # (no position is further out)
     given = out
     if out is None:
@@ -357,12 +362,25 @@ def qwen3_attention_block(
         (lambda: qkv_weight.size(0) % width == 0 and qkv_weight.size(0) // width > 2 * key_heads, ValueError, lambda: f"qkv_weight must have (heads + {2 * key_heads}) * {width} rows, got {qkv_weight.size(0)}."),
         (isinstance(normed, Tensor) and normed.dim() == 2, ValueError, "normed must be [tokens, hidden]."),
     ])  # fmt: skip
+    # What the operators behind the append would refuse is refused here, in front of it: a call that fails leaves the caches as they were.
+    heads = qkv_weight.size(0) // width - 2 * key_heads
+    scale = None if scale is None else float(scale)
+    enforce([
+        (isinstance(o_weight, Tensor) and o_weight.dim() == 2 and o_weight.size(1) == heads * width, ValueError, lambda: f"o_weight must be [hidden, {heads * width}]."),
+        (isinstance(residual, Tensor) and tuple(residual.shape) == (normed.size(0), o_weight.size(0)), ValueError, lambda: f"residual must have shape {(normed.size(0), o_weight.size(0))}."),
+        (o_weight.dtype == normed.dtype == key_cache.dtype, TypeError, lambda: f"normed, o_weight and the caches must have one type, got {normed.dtype}, {o_weight.dtype} and {key_cache.dtype}."),
+        (normed.device == o_weight.device == key_cache.device, RuntimeError, lambda: f"normed and o_weight must be on {key_cache.device}, got {normed.device} and {o_weight.device}."),
+    ])  # fmt: skip
+    like = normed if normed.shape == residual.shape else normed.new_empty((1, 1)).expand(residual.shape)
+    check_block_norm(like, residual, next_norm_weight, post_norm_weight, gate, eps)
     tensors = (
         residual, normed, qkv_weight, o_weight, key_cache, value_cache, page_table, context_lengths, query_starts, frequencies, next_norm_weight,
         q_norm_weight, k_norm_weight, post_norm_weight, gate,
     )  # fmt: skip
-    how = (bool(interleaved), float(magnitude), None if scale is None else float(scale), window, float(residual_scale), float(eps))
-    if _host.recorded(*tensors):
+    how = (bool(interleaved), float(magnitude), scale, window, float(residual_scale), float(eps))
+    recorded = _host.recorded(*tensors)
+    _check_attention(key_cache, value_cache, heads, width**-0.5 if scale is None else scale, True, window, "auto", recorded)
+    if recorded:
         total, after = _block_operator(*tensors, *how)
     else:
         total, after = _block(*tensors, *how)

@@ -154,6 +154,18 @@ def _gate_rows(gate: Optional[Tensor], block: Tensor) -> tuple:
     raise ValueError(f"gate must have shape ({width},), {(*block.shape[:-1], 1)} or {tuple(block.shape)}, got {tuple(gate.shape)}.")
 
 
+def check_block_norm(
+    block: Tensor, residual: Tensor, weight: Optional[Tensor], post_weight: Optional[Tensor], gate: Optional[Tensor], eps: float
+) -> None:
+    """What :func:`gated_residual_norm` refuses beside a block with the shape, type and device of ``block``."""
+    _check_rows(block, "block")
+    _check_beside(residual, "residual", block, block.dtype)
+    _vector(post_weight, "post_weight", block, block.dtype)
+    _vector(weight, "weight", block, block.dtype)
+    _gate_rows(gate, block)
+    _check_eps(eps)
+
+
 def _differentiable(*tensors: Optional[Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 

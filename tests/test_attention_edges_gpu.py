@@ -330,3 +330,28 @@ def test_frequencies_that_want_a_gradient_are_refused(attention, way):
     with torch.no_grad():
         for call in calls:
             assert same_bits(call(asks), call(f))
+
+
+def test_a_block_that_is_refused_leaves_the_caches_as_they_were(attention):
+    b = Batch([(2, 40), (1, 33)], 4, 2, 64, 16, BF16, seed=5)
+    keys, values = b.keys.clone(), b.values.clone()
+    given = {"residual": _normal(3, 128, seed=6), "normed": _normal(3, 128, seed=7), "qkv_weight": _normal(8 * 64, 128, seed=1), "o_weight": _normal(128, 4 * 64, seed=2)}
+    names = ("key_cache", "value_cache", "page_table", "context_lengths", "query_starts")
+    given |= {**dict(zip(names, b.where)), "frequencies": attention.rotary_frequencies(64, device=DEV), "next_norm_weight": _normal(128, seed=3)}
+    odd = torch.zeros(b.keys.numel() + 4, device=DEV, dtype=BF16)[4:].view(b.keys.shape)
+    for wrong, kind in (
+        ({"o_weight": given["o_weight"][:, :-64]}, ValueError), ({"o_weight": given["o_weight"].half()}, TypeError), ({"o_weight": given["o_weight"].cpu()}, RuntimeError),
+        ({"residual": given["residual"][:2]}, ValueError), ({"residual": given["residual"].half()}, TypeError), ({"next_norm_weight": _normal(64, seed=3)}, ValueError),
+        ({"post_norm_weight": _normal(64, seed=3)}, ValueError), ({"gate": _normal(3, 64, seed=3)}, ValueError), ({"eps": -1.0}, ValueError), ({"scale": -1.0}, ValueError),
+        ({"window": 0}, ValueError), ({"window": 1.5}, ValueError), ({"qkv_weight": _normal(7 * 64, 128, seed=1), "o_weight": _normal(128, 3 * 64, seed=2)}, ValueError),
+        ({"value_cache": odd}, ValueError), ({"normed": given["normed"][:, :64]}, (RuntimeError, ValueError, AssertionError)),
+    ):  # fmt: skip
+        with pytest.raises(kind):
+            attention.qwen3_attention_block(**{**given, **wrong})
+        torch.cuda.synchronize()
+        assert same_bits(b.keys, keys) and same_bits(b.values, values), wrong.keys()
+    before = given["residual"].clone()
+    attention.qwen3_attention_block(**given, gate=_normal(3, 1, seed=3), post_norm_weight=_normal(128, seed=4), window=5)
+    assert same_bits(given["residual"], before) and not same_bits(b.keys, keys)
+    fp32 = {**given, "residual": given["residual"].float()}
+    assert attention.qwen3_attention_block(**fp32)[0].dtype == torch.float32
