@@ -636,7 +636,8 @@ typedef struct rlk_paged_cache {
 /*
  * Writes k and v [tokens, key_heads, width] of the new tokens into their places, k turned by its position on the way, and q
  * (optional) likewise into host_q->y. host_rotary NULL: nothing turns. Its positions may be NULL: those in the sequence. Tokens
- * behind the last sequence are not written, their rows of host_q->y become zeros. host_k->y and host_v->y are not read.
+ * behind the last sequence are not written, their rows of host_q->y become zeros. host_k->y and host_v->y are not read. Every element of
+ * the cache has memory of its own (strides of 0 and keys that are the values are refused).
  */
 int rlk_paged_append(const rlk_paged_cache* host_cache, const rlk_rotary* host_rotary, const rlk_head_rows* host_q,
                      const rlk_head_rows* host_k, const rlk_head_rows* host_v, int64_t tokens, void* stream);

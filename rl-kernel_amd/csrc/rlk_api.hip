@@ -980,6 +980,12 @@ int rlk_paged_append(const rlk_paged_cache* cache, const rlk_rotary* rotary, con
   rc = check_rotary(who, rotary, cache->width, true);
   if (rc != RLK_OK || tokens == 0) return rc;
   if (!k->x || !v->x || (q && (!q->x || !q->y))) return refuse_argument(who, "null operand");
+  auto shared = [&](int64_t page, int64_t row, int64_t head) {
+    return (page == 0 && cache->pages > 1) || (row == 0 && cache->page_size > 1) || (head == 0 && cache->key_heads > 1);
+  };
+  if (cache->pages > 0 && (cache->keys == cache->values || shared(cache->key_page_stride, cache->key_row_stride, cache->key_head_stride) ||
+                           shared(cache->value_page_stride, cache->value_row_stride, cache->value_head_stride)))
+    return refuse_argument(who, "every element of a cache that is written has memory of its own");
   const hipError_t err = paged_append_launch(*cache, rotary, q, *k, *v, tokens, reinterpret_cast<hipStream_t>(stream));
   return err == hipSuccess ? RLK_OK : device_error(who, err);
 }

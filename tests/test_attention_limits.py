@@ -38,3 +38,24 @@ def test_rows_whose_numbers_do_not_fit(rlk_lib):
     for tokens, heads in ((2**31 - 1000, 1), (2**30 - 500, 2), (2**31 - 2, 1)):
         _refused(rlk_lib, _attention(rlk_lib, cache=one(), strides=(8, 8), tokens=tokens, heads=heads), "range")
         assert rlk_lib.rlk_paged_attention_workspace_bytes(one(), tokens, heads, 0, 0x101) == 0
+
+
+def test_appending_to_memory_that_elements_share(rlk_lib):
+    call = lambda **kwargs: rlk_lib.rlk_paged_append(_cache(values=AT << 1, **kwargs), None, None, _rows(), _rows(), 6, None)  # noqa: E731
+    for kwargs in ({"key_page_stride": 0}, {"key_row_stride": 0}, {"key_head_stride": 0}, {"value_page_stride": 0}, {"value_row_stride": 0}, {"value_head_stride": 0}):
+        _refused(rlk_lib, call(**kwargs), "memory of its own")
+    _refused(rlk_lib, rlk_lib.rlk_paged_append(_cache(), None, None, _rows(), _rows(), 6, None), "memory of its own")
+
+
+@pytest.mark.gpu
+def test_appending_to_an_expanded_cache():
+    from rl_engine.ops import attention
+
+    new = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    k, behind = new(3, 2, 64), (ints(0, 1).view(1, 2), ints(20), ints(0, 3))
+    for keys, values in ((new(1, 16, 2, 64).expand(5, 16, 2, 64), new(5, 16, 2, 64)), (new(5, 16, 2, 64), new(5, 16, 1, 64).expand(5, 16, 2, 64)), (new(5, 16, 2, 64),) * 2):
+        with pytest.raises(ValueError, match="memory of its own"):
+            attention.paged_append(k, k, keys, values, *behind)
+    one = new(1, 16, 1, 64)  # a single page and head may have any strides
+    attention.paged_append(k[:, :1], k[:, :1], one.as_strided((1, 16, 1, 64), (0, 64, 0, 1)), torch.zeros_like(one), ints(0).view(1, 1), ints(3), ints(0, 3))
