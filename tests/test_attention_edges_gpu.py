@@ -355,3 +355,30 @@ def test_a_block_that_is_refused_leaves_the_caches_as_they_were(attention):
     assert same_bits(given["residual"], before) and not same_bits(b.keys, keys)
     fp32 = {**given, "residual": given["residual"].float()}
     assert attention.qwen3_attention_block(**fp32)[0].dtype == torch.float32
+
+
+def test_every_call_of_several_threads(attention):
+    """What a thread raises is raised here, and all of their calls are counted."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    f = attention.rotary_frequencies(128, device=DEV)
+    batches = [Batch([(1, 3000 + 100 * s), (5, 2000), (300, 900)], 8, 2, 128, 16, BF16, seed=s) for s in range(4)]
+    new = [_normal(306, 2, 128, seed=10 + s) for s in range(4)]
+
+    def call(i):
+        q = attention.paged_append(new[i], new[i], *batches[i].where, f, q=batches[i].q)
+        return q, attention.paged_attention(q, *batches[i].where)
+
+    want = [call(i) for i in range(4)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        right = 0
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = call(i)
+                right += all(same_bits(g, w) for g, w in zip(got, want[i]))
+        return right
+
+    with ThreadPoolExecutor(4) as pool:
+        assert [future.result() for future in [pool.submit(work, i) for i in range(4)]] == [20] * 4
