@@ -7,7 +7,7 @@
 // its gradients 116 / 58, the GRPO loss with its gradient 59.7 / 33.5, beside kernels of 2 to 12 each; 87 / 50, 197 / 99 and 114 / 59
 // in the stretches in which autograd's device thread has to be woken for every backward; in those, the SwiGLU of eight-bit copies with
 // its gradients 132 / 59 and scores of hidden states with theirs 189 / 97.
-// A new token's rotation 23.2 / 6.2, appending to a paged cache 27.1 / 6.0, attention over 1025 positions 26.4 / 15.1 (there its kernels).
+// A new token's rotation 23.2 / 6.2, appending to a paged cache 27.1 / 6.0, attention over 1025 positions 26.4 / 15.3 (there its kernels).
 //
 // Every function takes everyday arguments only and answers None to anything else - other types, layouts and devices, subclasses,
 // batched and functorch tensors, tangents, dispatch and function modes (torch.set_default_device() is one), tracing, profilers -, for

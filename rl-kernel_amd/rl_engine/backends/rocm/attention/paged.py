@@ -124,8 +124,8 @@ def paged_append(
     ``context_lengths[s] - (query_starts[s + 1] - query_starts[s]) + i``; where they go is always that place. Rows of the cache that no new
     token goes to are left as they are. A token whose place lies before the start, outside of the table or in a page that does not exist is not
     written; neither are tokens behind the last sequence, whose rows of the returned ``q`` are zeros. Pages that are
-    written belong to one sequence (others may share the pages in front of them). The cache is not differentiable: arguments that require
-    a gradient are refused.
+    written belong to one sequence (others may share the pages in front of them), and the caches share no memory with each other or within
+    themselves. The caches count as written in place for autograd; they are not differentiable: arguments that require a gradient are refused.
     """
     if isinstance(k, Tensor) and k.is_cuda and not torch.compiler.is_compiling():
         done = _host.native().paged_append(  # everyday arguments, natively
@@ -228,12 +228,13 @@ def paged_attention(
 
     ``q [tokens, heads, width]`` and the caches are bf16 or fp16, ``width`` a multiple of 8 up to 256; head h reads key head
     ``h // (heads / key heads)``. A token at position p sees the positions up to p, with a ``window`` the last ``window`` of them; with
-    ``causal=False`` the whole context. Weights are ``softmax(scale * q k)``, ``scale`` ``width**-0.5`` by default. A row that sees nothing is
-    0 and its logarithm -inf; what a row does not see does not reach it, be it NaN. A row that sees a missing page (outside of
-    the table, or an entry that is no page) is NaN.
+    ``causal=False`` the whole context. Weights are ``softmax(scale * q k)``, ``scale`` ``width**-0.5`` by default; they are rounded to the
+    type of ``q`` for the product with the values (half a step each: in bf16 the result is off by 0.0022 of its 2-norm, by 0.0017 with weights of 32
+    bits), everything else is held in 32 bits. A row that sees nothing is 0 and its logarithm -inf; what a row does not see does
+    not reach it, be it NaN. A row that sees a missing page (outside of the table, or an entry that is no page) is NaN, its logarithm too.
 
-    Returns ``[tokens, heads, width]`` (``out`` where given, which overlaps no other argument), with ``return_lse`` also the fp32 natural logarithm of the sum
-    of exponentials ``[tokens, heads]``. Rows behind the last sequence are zeros (and -inf), in a given ``out`` left as they were.
+    Returns ``[tokens, heads, width]`` (``out`` where given, which overlaps no other argument and counts as written in place for autograd), with
+    ``return_lse`` also the fp32 natural logarithm of the sum of exponentials ``[tokens, heads]``. Rows behind the last sequence are zeros (and -inf), in a given ``out`` left as they were.
 
     A row's bits depend on its query and on the keys, values and positions that it sees: a prompt that comes in chunks, next to
     other sequences or token by token has the same results (:func:`attention_contract_id` names the order of the sums). ``config`` names the
